@@ -186,6 +186,96 @@ int qms_cuda_ep_combine(const float *ret, const int *slot, const float *wts, int
 int qms_cuda_sample(const float *logits, int vocab, float temp, float top_p, int top_k, uint64_t *rng,
                     int *token, void *stream);
 
+/* ---- serving behind a shared prompt: a paged KV cache, drafted tokens ----------------------------
+ * The reference keeps one contiguous fp32 cache per model (src/model.c:459-460), attends one
+ * sequence (src/model.c:465-492) and draws one token per row (src/chat.c:36-69). These entries serve
+ * a batch of sequences whose caches are made of pages from one pool, each with any number of new
+ * tokens per call (one when decoding, 1 + drafted tokens when verifying, a chunk of a prompt), and
+ * read a prompt that all of them share once instead of once per sequence. All buffers are device
+ * memory; nothing is read back to the host, and every call can be captured in a CUDA graph and
+ * replayed while q_start, kv_len, the table and the inputs change in place.
+ *
+ * Device-side errors are OR-ed into *err (device int; NULL: not reported); the work concerned is left
+ * out as said below, and nothing outside the buffers is read or written. */
+enum {
+    QMS_PAGED_ELEN = 1,        /* q_start, kv_len, a position or a draft length outside its bounds */
+    QMS_PAGED_EPAGE = 2,       /* a page id outside [0, n_pages) */
+    QMS_PAGED_ETOKEN = 4,      /* a drafted token id outside [0, vocab) */
+    QMS_PAGED_EMASS = 8,       /* a row of probabilities without any positive value */
+    QMS_PAGED_ETIMEOUT = 16    /* a bounded wait inside a kernel gave up; the call's output is invalid */
+};
+
+/* A pool of n_pages pages of page_size positions (a power of two). K of (page, position in it, kv
+ * head) starts at k + page * page_stride + position * pos_stride + head * head_stride elements of
+ * `type` (QMS_T_F32 or QMS_T_F16), its head_dim values contiguous; V alike. Any order of the three
+ * strides; the pointers and strides are multiples of 16 bytes. head_dim 64 or 128. */
+typedef struct {
+    int type, n_pages, page_size, n_head_kv, head_dim;
+    int64_t page_stride, pos_stride, head_stride;
+    void *k, *v;
+} QmsCudaPages;
+
+/* The new tokens of a batch. Sequence b owns rows q_start[b] .. q_start[b+1] - 1 of the call's token
+ * rows (none: it is idle) and, these included, kv_len[b] positions of cache: its i-th row is position
+ * kv_len[b] - (number of its rows) + i. Position j is at page table[b * table_stride + j / page_size].
+ * Rows past q_start[n_seq] are padding. The first prefix_len positions are the same in every
+ * sequence and are read through table row 0 (0: nothing is shared); they may end inside a page, of
+ * which each sequence then has its own copy. max_q and max_kv bound the rows and positions of a
+ * sequence (they size grids and workspaces; a sequence beyond them sets QMS_PAGED_ELEN and is
+ * treated as idle); max_kv <= table_stride * page_size. Pointers: device int. */
+typedef struct {
+    int n_seq, n_tok;              /* n_tok: token rows of the call, padding included */
+    const int *q_start;            /* [n_seq + 1], ascending */
+    const int *kv_len;             /* [n_seq] */
+    const int *table;              /* [n_seq][table_stride] */
+    int table_stride, max_q, max_kv, prefix_len;
+} QmsCudaPagedBatch;
+
+/* QK-norm, NEOX rotation and the cache append of new tokens in one pass (src/model.c:436-462, the
+ * arithmetic of the whole model's own cache, value for value). qkv: fp32 [n_tok] rows of ldqkv: n_head
+ * q heads, n_head_kv k heads, n_head_kv v heads of head_dim, as the projections leave them; q_norm,
+ * k_norm: fp32 [head_dim]; rope_cos / rope_sin: fp32 [n_rope][head_dim / 2]. q receives the normalised and
+ * rotated q heads (rows of ldq; may be qkv itself), K and V go to the pages. Padding rows are left
+ * alone; a row whose position is negative, at or past n_rope, or on a bad page sets *err and
+ * writes nothing. */
+int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *qkv, int64_t ldqkv,
+                          int n_head, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+                          const float *rope_sin, int n_rope, float *q, int64_t ldq, int *err, void *stream);
+
+/* Causal grouped-query attention of the batch's rows over the paged cache: out[t][h] = sum over
+ * positions j <= position of t of softmax_j(scale * q[t][h] . K[j]) V[j], fp32 in and out (rows of
+ * ldq / ldo), q head h reading kv head h / (n_head / n_head_kv). What lies at positions that a row
+ * does not see has no effect on it, whatever its bits. A row that sees nothing (padding, a negative
+ * position, an idle sequence) is zero; positions on a bad page set *err and count as not seen.
+ * ws: device workspace, 256-byte aligned, of at least qms_cuda_paged_attention_ws() bytes (a function
+ * of the sizes in the two descriptors; negative: a status), contents irrelevant before and after. */
+int64_t qms_cuda_paged_attention_ws(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, int n_head);
+int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *q, int64_t ldq,
+                             int n_head, float scale, float *out, int64_t ldo, void *ws, int64_t ws_bytes, int *err,
+                             void *stream);
+
+/* Probabilities of rows of logits at a temperature: p = exp((l - max) / temp) / sum, fp32 rows of ldl /
+ * ldp (p may be the logits themselves); temp <= 0: 1 at the first maximum, 0 elsewhere, the greedy
+ * choice of qms_cuda_sample. -inf logits have probability 0; a row of nothing else is all 0; a row with
+ * NaN or +inf is NaN (greedy: NaN is never chosen). */
+int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float temp, float *p, int64_t ldp, void *stream);
+
+/* Speculative verification: which drafted tokens stand, and the token after them, such that the
+ * result is distributed as draws from the target's p. Sequence b has rows row_start[b] + i (NULL:
+ * b * (max_draft + 1) + i), i = 0 .. n_draft[b], of p (p_rows rows of ldp), drafted tokens draft[b][i] with i <
+ * n_draft[b] (NULL: max_draft each), and the draft's probabilities q [n_seq * max_draft] rows of ldq
+ * (NULL: the drafts were certain, probability 1). u [n_seq][max_draft + 1]: uniform numbers in [0, 1).
+ * Draft i stands when those before it do and u[b][i] * q(x_i) < p(x_i). n_accept[b] of them stand; the
+ * next token comes from max(0, p - q) at the first that does not (from p where that is 0
+ * everywhere), or from the row after the last: the lowest index whose cumulative weight exceeds
+ * u[b][max_draft] * total, weights rounded to multiples of 2^-40 (and limited to 1) and added as
+ * integers, so the token does not depend on the order of the additions. tokens [n_seq][max_draft +
+ * 1]: the standing drafts, the next token, then -1. A draft id outside the vocabulary never stands;
+ * no positive weight gives token -1; bad row or draft counts give n_accept 0 and token -1. */
+int qms_cuda_verify(const float *p, int64_t ldp, int p_rows, const int *row_start, const float *q, int64_t ldq,
+                    const int *draft, const int *n_draft, int n_seq, int max_draft, int vocab, const float *u,
+                    int *n_accept, int *tokens, int *err, void *stream);
+
 /* Waits for the device and reports whether any bounded wait inside the layer's kernels gave up
  * since the last call (QMS_CUDA_ETIMEOUT; the outputs of the affected call are invalid), then
  * clears the flag. The batch-1 kernels never spin without a limit, so a stuck pipeline turns into

@@ -9,6 +9,14 @@ with ctypes and mirrors the reference's operator interface for tests and benchma
     MoeLayer(...).forward(xn)    moe()             (src/model.c:1032)
     Model(...).forward(ids, pos) qms_forward       (src/model.c:1252), the whole token step
 
+and adds the operators of batched serving behind a shared prompt, with drafted tokens:
+
+    KvPages, PagedBatch          a paged KV cache, and a batch of new tokens over it
+    paged_append(...)            QK-norm, rotation and the cache append in one pass
+    paged_attention(...)         causal attention over the pages, a shared prompt read once
+    probs(logits, temp)          probabilities of logits rows
+    verify(p, draft, u)          which drafted tokens stand, and the token after them
+
 Device buffers are torch CUDA tensors (plumbing only); every computation runs in
 libqms_cuda's kernels. There is no CPU fallback: if the library is missing or no sm_100 GPU is
 present, the calls raise.
@@ -49,6 +57,18 @@ class ModelDesc(C.Structure):
                 ("vocab", C.c_int), ("eps", C.c_float), ("rope_base", C.c_double), ("ctx", C.c_int),
                 ("embd_type", C.c_int), ("embd", C.c_void_p), ("out_norm", C.c_void_p),
                 ("output_type", C.c_int), ("output", C.c_void_p), ("src_on_device", C.c_int)]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_head_kv", C.c_int),
+                ("head_dim", C.c_int), ("page_stride", C.c_int64), ("pos_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_tok", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("table", C.c_void_p), ("table_stride", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int),
+                ("prefix_len", C.c_int)]
 
 
 class LayerDesc(C.Structure):
@@ -113,6 +133,13 @@ def lib() -> C.CDLL:
     L.qms_cuda_model_status.argtypes = [vp]
     L.qms_cuda_model_profile.argtypes = [vp, i32, vp]
     L.qms_cuda_moe_route_noalloc.argtypes = [vp, i32, i32, i32, vp, i32, vp, vp, vp, vp]
+    pg, pb, f32 = C.POINTER(PagesDesc), C.POINTER(PagedBatchDesc), C.c_float
+    L.qms_cuda_paged_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, vp, i64, vp, vp]
+    L.qms_cuda_paged_attention_ws.argtypes = [pg, pb, i32]
+    L.qms_cuda_paged_attention_ws.restype = i64
+    L.qms_cuda_paged_attention.argtypes = [pg, pb, vp, i64, i32, f32, vp, i64, vp, i64, vp, vp]
+    L.qms_cuda_probs.argtypes = [vp, i64, i32, i32, f32, vp, i64, vp]
+    L.qms_cuda_verify.argtypes = [vp, i64, i32, vp, vp, i64, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp]
     _lib = L
     return L
 
@@ -370,6 +397,189 @@ def ep_combine(ret, slot, wts, resid=None, out=None, stream=None):
     check(lib().qms_cuda_ep_combine(_ptr(ret), _ptr(slot), _ptr(wts), T, K, E, _ptr(resid), _ptr(out),
                                     _stream(stream)))
     return out
+
+
+# ---- serving behind a shared prompt: a paged KV cache, drafted tokens --------------------------------
+
+def _rows(t, cols: int, what: str):
+    """A CUDA float32 tensor of rows whose last dimensions are contiguous: (address, rows, stride)."""
+    torch = _torch()
+    if t.dtype != torch.float32 or not t.is_cuda:
+        raise ValueError(f"{what}: a CUDA float32 tensor is needed, got {t.dtype} on {t.device}")
+    if t.dim() != 2:
+        t = t.view(-1, cols)                # raises where the rows are not contiguous
+    if t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: rows of {cols} contiguous values are needed, got {tuple(t.shape)}, "
+                         f"strides {tuple(t.stride())}")
+    return t.data_ptr(), t.shape[0], max(t.stride(0), cols) if t.shape[0] < 2 else t.stride(0)
+
+
+def _ints(t, shape: tuple, what: str):
+    """The address of a contiguous CUDA int32 tensor of that shape."""
+    torch = _torch()
+    if t.dtype != torch.int32 or not t.is_cuda or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous CUDA int32 tensor {shape} is needed, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _raw_stream(stream, device) -> int:
+    return (stream if stream is not None else _torch().cuda.current_stream(device)).cuda_stream
+
+
+class KvPages:
+    """A pool of KV cache pages (QmsCudaPages): k, v CUDA tensors [n_pages][page_size][n_head_kv][head_dim] of
+    one shape, type (float32 or float16) and strides, the last dimension contiguous. Another order in
+    memory, such as heads before positions, is a transposed view."""
+
+    def __init__(self, k, v):
+        torch = _torch()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("KvPages: k and v need one shape [n_pages][page_size][n_head_kv][head_dim], one type and "
+                             "one set of strides, the last of them 1")
+        if not (k.is_cuda and k.device == v.device):
+            raise ValueError("KvPages: k and v must be on one CUDA device")
+        typ = {torch.float32: T_F32, torch.float16: T_F16}.get(k.dtype)
+        if typ is None:
+            raise ValueError(f"KvPages: float32 or float16, got {k.dtype}")
+        self.k, self.v = k, v
+        self.n_head_kv, self.head_dim = k.shape[2], k.shape[3]
+        st = k.stride()
+        self.desc = PagesDesc(typ, k.shape[0], k.shape[1], k.shape[2], k.shape[3], st[0], st[1], st[2], k.data_ptr(),
+                              v.data_ptr())
+        self._ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, kv_type: int = T_F32) -> "KvPages":
+        torch = _torch()
+        dt = {T_F32: torch.float32, T_F16: torch.float16}[kv_type]
+        k, v = (torch.zeros((n_pages, page_size, n_head_kv, head_dim), dtype=dt, device="cuda") for _ in range(2))
+        return cls(k, v)
+
+
+class PagedBatch:
+    """New tokens of a batch of sequences over a paged cache (QmsCudaPagedBatch): q_start CUDA int32 [n_seq + 1],
+    kv_len int32 [n_seq], table int32 [n_seq][pages]; n_tok token rows; max_q / max_kv bound a sequence's
+    rows and positions. The tensors may be rewritten in place between calls (and between replays of a
+    captured graph); the bounds may not be exceeded. Device-side errors collect in `err`."""
+
+    def __init__(self, q_start, kv_len, table, n_tok: int, max_q: int, max_kv: int, prefix_len: int = 0):
+        torch = _torch()
+        n = kv_len.shape[0]
+        self.q_start, self.kv_len, self.table = q_start, kv_len, table
+        self.n_tok = int(n_tok)
+        self.err = torch.zeros((1,), dtype=torch.int32, device=kv_len.device)
+        self._err = self.err.data_ptr()
+        self.desc = PagedBatchDesc(n, self.n_tok, _ints(q_start, (n + 1,), "q_start"), _ints(kv_len, (n,), "kv_len"),
+                                   _ints(table, (n, table.shape[1]), "table"), table.shape[1], int(max_q), int(max_kv),
+                                   int(prefix_len))
+        self._ref = C.byref(self.desc)
+        self._ws = {}
+
+    def status(self):
+        """Raise if a device-side check refused work since the last call (waits for the device)."""
+        e = int(self.err.item())
+        if e:
+            self.err.zero_()
+            raise QmsCudaError(ETIMEOUT if e & 16 else EINVAL, f"paged batch: device-side errors 0x{e:x} (1 = lengths or "
+                               "positions, 2 = page id, 4 = drafted id, 8 = no probability, 16 = a wait gave up)")
+
+    def workspace(self, pages: KvPages, n_head: int):
+        """The attention's workspace for these sizes, allocated on first use and kept: (address, bytes).
+        Calls that overlap on the GPU (on several streams) need a batch object each."""
+        key = (pages.desc.type, pages.n_head_kv, pages.head_dim, n_head)
+        if key not in self._ws:
+            torch = _torch()
+            n = lib().qms_cuda_paged_attention_ws(pages._ref, self._ref, n_head)
+            if n < 0:
+                check(n)
+            w = torch.empty((n + 256,), dtype=torch.uint8, device=pages.k.device)
+            self._ws[key] = (w, (w.data_ptr() + 255) // 256 * 256, n)
+        return self._ws[key][1:]
+
+
+def rope_tables(n_pos: int, head_dim: int, base: float = 1e6, device="cuda"):
+    """cos and sin of position * base^(-2i / head_dim), computed in double and rounded once
+    (src/model.c:411-422, 446-447): CUDA float32 [n_pos][head_dim / 2] each."""
+    torch = _torch()
+    ang = np.arange(n_pos, dtype=np.float64)[:, None] * float(base) ** (-2.0 * np.arange(head_dim // 2) / head_dim)
+    return tuple(torch.from_numpy(f(ang).astype(np.float32)).to(device) for f in (np.cos, np.sin))
+
+
+def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_norm, eps: float, rope, q=None, stream=None):
+    """QK-norm, rotation and cache append of the batch's rows (qms_cuda_paged_append): qkv CUDA float32
+    [n_tok][(n_head + 2 n_head_kv) * head_dim], rope = rope_tables(...). Returns the q heads
+    [n_tok][n_head * head_dim]."""
+    torch = _torch()
+    D = pages.head_dim
+    if q is None:
+        q = torch.empty((batch.n_tok, n_head * D), dtype=torch.float32, device=qkv.device)
+    x, n, ldx = _rows(qkv, (n_head + 2 * pages.n_head_kv) * D, "qkv")
+    y, ny, ldy = _rows(q, n_head * D, "q")
+    (w1, _, _), (w2, _, _) = _rows(q_norm, D, "q_norm"), _rows(k_norm, D, "k_norm")
+    (c, nc, _), (sn, ns, _) = _rows(rope[0], D // 2, "rope cos"), _rows(rope[1], D // 2, "rope sin")
+    if n < batch.n_tok or ny < batch.n_tok or nc != ns:
+        raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens, rotation tables of {nc} / {ns}")
+    check(lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, w1, w2, eps, c, sn, nc, y, ldy, batch._err,
+                                      _raw_stream(stream, qkv.device)))
+    return q
+
+
+def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: float | None = None, out=None, stream=None):
+    """Causal attention of the batch's rows over its cache (qms_cuda_paged_attention): q CUDA float32
+    [n_tok][n_head * head_dim]; scale defaults to 1 / sqrt(head_dim). Returns [n_tok][n_head * head_dim]."""
+    torch = _torch()
+    D = pages.head_dim
+    if out is None:
+        out = torch.empty((batch.n_tok, n_head * D), dtype=torch.float32, device=q.device)
+    x, n, ldx = _rows(q, n_head * D, "q")
+    y, ny, ldy = _rows(out, n_head * D, "out")
+    if n < batch.n_tok or ny < batch.n_tok:
+        raise ValueError(f"paged_attention: {n} q and {ny} out rows for {batch.n_tok} tokens")
+    ws, nb = batch.workspace(pages, n_head)
+    check(lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y,
+                                         ldy, ws, nb, batch._err, _raw_stream(stream, q.device)))
+    return out
+
+
+def probs(logits, temp: float, out=None, stream=None):
+    """Probabilities of rows of logits (CUDA float32 [rows][vocab]) at a temperature (qms_cuda_probs); temp <= 0:
+    1 at the first maximum. out may be logits."""
+    torch = _torch()
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    V = logits.shape[-1]
+    x, n, ldx = _rows(logits, V, "logits")
+    y, ny, ldy = _rows(out, V, "out")
+    if n != ny:
+        raise ValueError(f"probs: {n} rows of logits, {ny} of out")
+    check(lib().qms_cuda_probs(x, ldx, n, V, temp, y, ldy, _raw_stream(stream, logits.device)))
+    return out
+
+
+def verify(p, draft, u, q=None, n_draft=None, row_start=None, n_accept=None, tokens=None, err=None, stream=None):
+    """Verification of drafted tokens (qms_cuda_verify): p CUDA float32 [rows][vocab], draft int32 [n_seq][max_draft],
+    u float32 [n_seq][max_draft + 1], q float32 [n_seq][max_draft][vocab] or None. Returns (n_accept int32
+    [n_seq], tokens int32 [n_seq][max_draft + 1]); err: CUDA int32 [1] or None."""
+    torch = _torch()
+    B, N = draft.shape
+    V = p.shape[-1]
+    if n_accept is None:
+        n_accept = torch.empty((B,), dtype=torch.int32, device=p.device)
+    if tokens is None:
+        tokens = torch.empty((B, N + 1), dtype=torch.int32, device=p.device)
+    x, n, ldx = _rows(p, V, "p")
+    y, ny, ldy = (None, B * N, V) if q is None else _rows(q, V, "q")
+    uu, _, ldu = _rows(u, N + 1, "u")
+    if ny != B * N or u.numel() != B * (N + 1) or ldu != N + 1:
+        raise ValueError(f"verify: {ny} draft rows and u {tuple(u.shape)} for {B} sequences of {N} drafts")
+    if row_start is None and n < B * (N + 1):
+        raise ValueError(f"verify: {n} rows of p for {B} sequences of {N} drafts")
+    check(lib().qms_cuda_verify(x, ldx, n, None if row_start is None else _ints(row_start, (B,), "row_start"), y, ldy,
+                                _ints(draft, (B, N), "draft"), None if n_draft is None else _ints(n_draft, (B,), "n_draft"),
+                                B, N, V, uu, _ints(n_accept, (B,), "n_accept"), _ints(tokens, (B, N + 1), "tokens"),
+                                None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, p.device)))
+    return n_accept, tokens
 
 
 # ---- the whole model (qms_model_load / qms_forward, src/model.h:135-141) ------------------------------
