@@ -161,9 +161,15 @@ def declared_functions() -> list[str]:
 
 # ---- torch plumbing ----------------------------------------------------------------------------
 
+_torch_mod = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _torch_mod
+    if _torch_mod is None:
+        import torch
+        _torch_mod = torch
+    return _torch_mod
 
 
 def _ptr(t) -> C.c_void_p | None:
@@ -402,29 +408,39 @@ def ep_combine(ret, slot, wts, resid=None, out=None, stream=None):
 # ---- serving behind a shared prompt: a paged KV cache, drafted tokens --------------------------------
 
 def _rows(t, cols: int, what: str):
-    """A CUDA float32 tensor of rows whose last dimensions are contiguous: (address, rows, stride)."""
-    torch = _torch()
-    if t.dtype != torch.float32 or not t.is_cuda:
-        raise ValueError(f"{what}: a CUDA float32 tensor is needed, got {t.dtype} on {t.device}")
+    """A CUDA float32 tensor of rows whose values are contiguous: (address, rows, stride)."""
     if t.dim() != 2:
         t = t.view(-1, cols)                # raises where the rows are not contiguous
-    if t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: rows of {cols} contiguous values are needed, got {tuple(t.shape)}, "
-                         f"strides {tuple(t.stride())}")
-    return t.data_ptr(), t.shape[0], max(t.stride(0), cols) if t.shape[0] < 2 else t.stride(0)
+    n, c = t.shape
+    ld, one = t.stride()
+    if c != cols or (one != 1 and cols > 1) or t.dtype is not _torch().float32 or not t.is_cuda:
+        raise ValueError(f"{what}: CUDA float32 rows of {cols} contiguous values are needed, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}, strides {tuple(t.stride())}")
+    return t.data_ptr(), n, ld if n > 1 else max(ld, cols)
 
 
-def _ints(t, shape: tuple, what: str):
+def _vec(t, n: int, what: str) -> int:
+    """The address of a contiguous CUDA float32 tensor of n values."""
+    if t.numel() != n or t.dtype is not _torch().float32 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous CUDA float32 values are needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _ints(t, shape: tuple, what: str) -> int:
     """The address of a contiguous CUDA int32 tensor of that shape."""
-    torch = _torch()
-    if t.dtype != torch.int32 or not t.is_cuda or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or t.dtype is not _torch().int32 or not t.is_cuda or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous CUDA int32 tensor {shape} is needed, got {t.dtype} {tuple(t.shape)} "
                          f"on {t.device}")
     return t.data_ptr()
 
 
-def _raw_stream(stream, device) -> int:
-    return (stream if stream is not None else _torch().cuda.current_stream(device)).cuda_stream
+def _raw_stream(stream, t) -> int:
+    """The given stream, or the current one of t's device."""
+    if stream is not None:
+        return stream.cuda_stream
+    torch = _torch()
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # a tenth of current_stream()'s time
+    return get(t.get_device()) if get else torch.cuda.current_stream(t.device).cuda_stream
 
 
 class KvPages:
@@ -448,6 +464,7 @@ class KvPages:
         self.desc = PagesDesc(typ, k.shape[0], k.shape[1], k.shape[2], k.shape[3], st[0], st[1], st[2], k.data_ptr(),
                               v.data_ptr())
         self._ref = C.byref(self.desc)
+        self._key = (typ,) + tuple(k.shape[1:])
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, kv_type: int = T_F32) -> "KvPages":
@@ -487,7 +504,7 @@ class PagedBatch:
     def workspace(self, pages: KvPages, n_head: int):
         """The attention's workspace for these sizes, allocated on first use and kept: (address, bytes).
         Calls that overlap on the GPU (on several streams) need a batch object each."""
-        key = (pages.desc.type, pages.n_head_kv, pages.head_dim, n_head)
+        key = (pages._key, n_head)
         if key not in self._ws:
             torch = _torch()
             n = lib().qms_cuda_paged_attention_ws(pages._ref, self._ref, n_head)
@@ -510,50 +527,54 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     """QK-norm, rotation and cache append of the batch's rows (qms_cuda_paged_append): qkv CUDA float32
     [n_tok][(n_head + 2 n_head_kv) * head_dim], rope = rope_tables(...). Returns the q heads
     [n_tok][n_head * head_dim]."""
-    torch = _torch()
     D = pages.head_dim
     if q is None:
-        q = torch.empty((batch.n_tok, n_head * D), dtype=torch.float32, device=qkv.device)
+        q = _torch().empty((batch.n_tok, n_head * D), dtype=_torch().float32, device=qkv.device)
     x, n, ldx = _rows(qkv, (n_head + 2 * pages.n_head_kv) * D, "qkv")
     y, ny, ldy = _rows(q, n_head * D, "q")
-    (w1, _, _), (w2, _, _) = _rows(q_norm, D, "q_norm"), _rows(k_norm, D, "k_norm")
-    (c, nc, _), (sn, ns, _) = _rows(rope[0], D // 2, "rope cos"), _rows(rope[1], D // 2, "rope sin")
-    if n < batch.n_tok or ny < batch.n_tok or nc != ns:
-        raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens, rotation tables of {nc} / {ns}")
-    check(lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, w1, w2, eps, c, sn, nc, y, ldy, batch._err,
-                                      _raw_stream(stream, qkv.device)))
+    cos, sin = rope
+    nc = cos.shape[0]
+    if n < batch.n_tok or ny < batch.n_tok:
+        raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens")
+    rc = lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
+                                     eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy,
+                                     batch._err, _raw_stream(stream, qkv))
+    if rc:
+        check(rc)
     return q
 
 
 def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: float | None = None, out=None, stream=None):
     """Causal attention of the batch's rows over its cache (qms_cuda_paged_attention): q CUDA float32
     [n_tok][n_head * head_dim]; scale defaults to 1 / sqrt(head_dim). Returns [n_tok][n_head * head_dim]."""
-    torch = _torch()
     D = pages.head_dim
     if out is None:
-        out = torch.empty((batch.n_tok, n_head * D), dtype=torch.float32, device=q.device)
+        out = _torch().empty((batch.n_tok, n_head * D), dtype=_torch().float32, device=q.device)
     x, n, ldx = _rows(q, n_head * D, "q")
     y, ny, ldy = _rows(out, n_head * D, "out")
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_attention: {n} q and {ny} out rows for {batch.n_tok} tokens")
     ws, nb = batch.workspace(pages, n_head)
-    check(lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y,
-                                         ldy, ws, nb, batch._err, _raw_stream(stream, q.device)))
+    rc = lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
+                                        ws, nb, batch._err, _raw_stream(stream, q))
+    if rc:
+        check(rc)
     return out
 
 
 def probs(logits, temp: float, out=None, stream=None):
     """Probabilities of rows of logits (CUDA float32 [rows][vocab]) at a temperature (qms_cuda_probs); temp <= 0:
     1 at the first maximum. out may be logits."""
-    torch = _torch()
     if out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+        out = _torch().empty(logits.shape, dtype=_torch().float32, device=logits.device)
     V = logits.shape[-1]
     x, n, ldx = _rows(logits, V, "logits")
     y, ny, ldy = _rows(out, V, "out")
     if n != ny:
         raise ValueError(f"probs: {n} rows of logits, {ny} of out")
-    check(lib().qms_cuda_probs(x, ldx, n, V, temp, y, ldy, _raw_stream(stream, logits.device)))
+    rc = lib().qms_cuda_probs(x, ldx, n, V, temp, y, ldy, _raw_stream(stream, logits))
+    if rc:
+        check(rc)
     return out
 
 
@@ -570,15 +591,16 @@ def verify(p, draft, u, q=None, n_draft=None, row_start=None, n_accept=None, tok
         tokens = torch.empty((B, N + 1), dtype=torch.int32, device=p.device)
     x, n, ldx = _rows(p, V, "p")
     y, ny, ldy = (None, B * N, V) if q is None else _rows(q, V, "q")
-    uu, _, ldu = _rows(u, N + 1, "u")
-    if ny != B * N or u.numel() != B * (N + 1) or ldu != N + 1:
-        raise ValueError(f"verify: {ny} draft rows and u {tuple(u.shape)} for {B} sequences of {N} drafts")
+    if ny != B * N:
+        raise ValueError(f"verify: {ny} draft rows for {B} sequences of {N} drafts")
     if row_start is None and n < B * (N + 1):
         raise ValueError(f"verify: {n} rows of p for {B} sequences of {N} drafts")
-    check(lib().qms_cuda_verify(x, ldx, n, None if row_start is None else _ints(row_start, (B,), "row_start"), y, ldy,
-                                _ints(draft, (B, N), "draft"), None if n_draft is None else _ints(n_draft, (B,), "n_draft"),
-                                B, N, V, uu, _ints(n_accept, (B,), "n_accept"), _ints(tokens, (B, N + 1), "tokens"),
-                                None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, p.device)))
+    rc = lib().qms_cuda_verify(x, ldx, n, None if row_start is None else _ints(row_start, (B,), "row_start"), y, ldy,
+                               _ints(draft, (B, N), "draft"), None if n_draft is None else _ints(n_draft, (B,), "n_draft"), B, N, V,
+                               _vec(u, B * (N + 1), "u"), _ints(n_accept, (B,), "n_accept"), _ints(tokens, (B, N + 1), "tokens"),
+                               None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, p))
+    if rc:
+        check(rc)
     return n_accept, tokens
 
 

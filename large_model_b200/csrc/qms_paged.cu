@@ -1,7 +1,5 @@
-// qms_paged.cu - a paged KV cache on B200 (sm_100a): the append of new tokens with QK-norm and rotation,
-// and causal grouped-query attention of a batch over the pages.
-//
-// Reference counterparts, on one contiguous cache: src/model.c:436-462 (append), 465-492 (attention).
+// qms_paged.cu - a paged KV cache on B200 (sm_100a): the append of new tokens with QK-norm and rotation
+// (src/model.c:436-462 on one contiguous cache), and the C entries of the paged operators.
 #include <math.h>
 #include <string.h>
 
@@ -63,49 +61,6 @@ __global__ void __launch_bounds__(256) k_paged_append(const Paged a, const float
     KT *dst = reinterpret_cast<KT *>((hh < a.H + a.Hk ? a.k : a.v) + at + kh * a.head_stride);
 #pragma unroll
     for (int j = 0; j < J; j++) kv_st(dst + lane + 32 * j, x[j]);
-}
-
-// ---- attention -----------------------------------------------------------------------------------
-// One warp per (token, q head), lanes over the head's dims, one pass over the positions with the running
-// maximum m and sum l of the softmax: o <- o e^(m - m') + e^(s - m') V.
-template <int D, typename KT>
-__global__ void __launch_bounds__(256) k_paged_attention(const Paged a, const float *q, int64_t ldq, float scale,
-                                                         float *out, int64_t ldo) {
-    constexpr int J = D / 32;
-    const int lane = threadIdx.x & 31, h = blockIdx.y * 8 + (threadIdx.x >> 5), t = blockIdx.x;
-    pdl_trigger();
-    pdl_wait();
-    if (h >= a.H) return;
-    int t0 = 0, n = 0, kv = 0;
-    const int b = paged_seq_of(a, t);
-    if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0 && h == 0) paged_err(a, QMS_PAGED_ELEN);
-    const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
-    float x[J], o[J], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < J; j++) {
-        x[j] = q[t * ldq + h * D + lane + 32 * j];
-        o[j] = 0.0f;
-    }
-    for (int p = 0; p <= pos; p++) {
-        const int64_t at = paged_at(a, a.table + (p < a.prefix ? 0 : (int64_t)b * a.table_stride), p);
-        if (at < 0) {
-            if (lane == 0 && h == 0) paged_err(a, QMS_PAGED_EPAGE);
-            continue;
-        }
-        const int64_t off = at + (h / a.G) * a.head_stride;
-        const KT *kr = reinterpret_cast<const KT *>(a.k + off), *vr = reinterpret_cast<const KT *>(a.v + off);
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < J; j++) s = fmaf(x[j], kv_ld(kr + lane + 32 * j), s);
-        s = warp_sum(s) * scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), e = expf(s - mn);
-        l = l * c + e;
-        m = mn;
-#pragma unroll
-        for (int j = 0; j < J; j++) o[j] = fmaf(e, kv_ld(vr + lane + 32 * j), o[j] * c);
-    }
-#pragma unroll
-    for (int j = 0; j < J; j++) out[t * ldo + h * D + lane + 32 * j] = l == 0.0f ? 0.0f : o[j] / l;
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -203,7 +158,10 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
 int64_t qms_cuda_paged_attention_ws(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, int n_head) {
     Paged a;
     const int rc = paged_args("paged_attention_ws", pages, batch, n_head, nullptr, a);
-    return rc ? rc : 0;
+    if (rc) return rc;
+    PagedPlan p;
+    paged_plan(a, pages->type, pages->head_dim, p);
+    return paged_ws_bytes(a, pages->head_dim, p);
 }
 
 int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *q, int64_t ldq,
@@ -217,19 +175,12 @@ int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch 
     const int D = pages->head_dim;
     if ((rc = paged_rows("paged_attention", "q", q, ldq, (int64_t)n_head * D))) return rc;
     if ((rc = paged_rows("paged_attention", "out", out, ldo, (int64_t)n_head * D))) return rc;
-    const int64_t need = qms_cuda_paged_attention_ws(pages, batch, n_head);
+    PagedPlan p;
+    paged_plan(a, pages->type, D, p);
+    const int64_t need = paged_ws_bytes(a, D, p);
     QMS_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= need), QMS_CUDA_EINVAL,
                 "paged_attention: needs a 256-byte aligned workspace of %lld bytes", (long long)need);
-    const dim3 grid(a.n_tok, (n_head + 7) / 8);
-#define QMS_ATT(D_, KT) \
-    QMS_CK(launch_pdl(k_paged_attention<D_, KT>, grid, dim3(256), 0, (cudaStream_t)stream, a, q, ldq, scale, out, ldo))
-    if (pages->type == QMS_T_F16) {
-        if (D == 128) QMS_ATT(128, __half); else QMS_ATT(64, __half);
-    } else {
-        if (D == 128) QMS_ATT(128, float); else QMS_ATT(64, float);
-    }
-#undef QMS_ATT
-    return QMS_CUDA_OK;
+    return launch_paged_attention(a, pages->type, D, p, q, ldq, scale, out, ldo, ws, (cudaStream_t)stream);
 }
 
 }  // extern "C"

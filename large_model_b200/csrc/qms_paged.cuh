@@ -47,4 +47,34 @@ __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int 
     return page * a.page_stride + (p & ((1 << a.page_log) - 1)) * a.pos_stride;
 }
 
+// ---- attention: the work and its split ----------------------------------------------------------
+// Two kinds of units, per kv head: the shared positions [0, prefix) against tiles of all token rows, and
+// a sequence's own positions [prefix, kv_len) against tiles of its rows. A row is a (token, q head of the
+// kv head's group) pair, row = token * G + head. Positions are cut into chunks; every (chunk, row) writes a
+// partial result to its slot of the workspace (prefix chunks first) and k_paged_merge joins a row's
+// slots: part_o [slots][n_tok * H][D] (not divided by l), part_ml [slots][n_tok * H] of (m, l),
+// m the base-2 exponent of the weights' common factor.
+struct PagedPlan {
+    int wr_p, wr_s;                  // row groups of 16 per tile: shared, own
+    int chunk_p, chunk_s;            // positions per chunk
+    int slots_p, slots_s;            // chunks of each kind
+    int tiles_p, tiles_s;            // row tiles of each kind
+};
+
+struct PagedAttn {
+    Paged a;
+    PagedPlan p;
+    const float *q;
+    float *out;
+    int64_t ldq, ldo;
+    float scale2;                    // scale * log2(e)
+    float *part_o;
+    float2 *part_ml;
+};
+
+void paged_plan(const Paged &a, int type, int D, PagedPlan &p);
+int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p);
+int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, const float *q, int64_t ldq, float scale,
+                           float *out, int64_t ldo, void *ws, cudaStream_t s);
+
 }  // namespace qms

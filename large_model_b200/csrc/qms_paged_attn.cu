@@ -1,0 +1,675 @@
+// qms_paged_attn.cu - causal grouped-query attention of a batch of new tokens over a paged KV cache on B200
+// (sm_100a); src/model.c:465-492 is the reference's, of one sequence over one contiguous cache.
+//
+// One pass over the positions with the running maximum and sum of the softmax, the two products on the
+// tensor cores with 22-bit operands: an fp32 operand x is split as x = hi + lo into two of the tensor
+// cores' types and the products with hi and lo are added in fp32. Over an fp16 cache K and V are
+// exact, so q and the weights split into two fp16 terms cost two mma.sync m16n8k16 per product (one
+// term alone would leave an error of 2^-12). Over an fp32 cache all four operands are split into two tf32 terms
+// and three m16n8k8 products are kept (lo * lo is below 2^-22).
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "qms_moe.cuh"
+#include "qms_paged.cuh"
+
+namespace qms {
+
+constexpr int kPaStage = 64;          // positions per stage
+constexpr float kPaShift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 bytes global -> shared, or 16 zero bytes.
+__device__ __forceinline__ void cp_async16_or0(uint32_t dst, const void *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+                   "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+__device__ __forceinline__ uint32_t pack_h2(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// (x, y) = hi + lo in fp16 pairs
+__device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    hi = pack_h2(x, y);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    lo = pack_h2(x - h.x, y - h.y);
+}
+// x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
+__device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
+// Zero what is not finite in a 16-byte piece of V; true if something was.
+__device__ __forceinline__ bool drop_nonfinite(const __half *, uint4 &v) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if ((w[i] & 0x7C00u) == 0x7C00u) {
+            w[i] &= 0xFFFF0000u;
+            any = true;
+        }
+        if ((w[i] & 0x7C000000u) == 0x7C000000u) {
+            w[i] &= 0x0000FFFFu;
+            any = true;
+        }
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+__device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if ((w[i] & 0x7F800000u) == 0x7F800000u) {
+            w[i] = 0;
+            any = true;
+        }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+
+// ---- the kernel over mma.sync ----------------------------------------------------------------------
+// A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows times WK = 4 / WR
+// groups of positions. K and V arrive in stages of 64 positions by cp.async (zeros where a position is
+// past the chunk or on a bad page); each warp scores its rows against its share of the stage, keeps its
+// own running (m, l, o), and the position groups are joined in shared memory at the end of the unit.
+template <int D, typename KT, int WR>
+struct PaCfg {
+    static constexpr bool F16 = sizeof(KT) == 2;
+    static constexpr int WK = 4 / WR, KW = kPaStage / WK, NT = KW / 8;       // positions and 8-position tiles per warp
+    static constexpr int CH = D * (int)sizeof(KT) / 16;                      // 16-byte pieces per row
+    // fp16 rows are dense with the pieces XOR-swizzled by the row (ldmatrix reads 8 rows at one piece);
+    // fp32 rows are padded so that the 8 lanes of a 16-byte read (K: 2 rows x 4 pieces, V: 4 rows two
+    // apart x 2 pieces) fall on different banks
+    static constexpr int KROW = D * (int)sizeof(KT) + (F16 ? 0 : 64), VROW = D * (int)sizeof(KT) + (F16 ? 0 : 16);
+    static constexpr int KB = KROW * kPaStage, STAGE = KB + VROW * kPaStage;
+    static constexpr int NS = F16 ? 3 : 2;
+    static constexpr int RED = WK > 1 ? 4 * 16 * (D + 2) * 4 : 0;            // the position groups' o, m, l
+    static constexpr int SMEM = NS * STAGE > RED ? NS * STAGE : RED;
+};
+
+// OWN: the sequences' own positions; else the shared ones. LAST: launched beside the kernel of the other kind,
+// whose end it waits for at its own end, so that what follows this kernel follows both.
+template <int D, typename KT, int WR>
+__global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const bool own, const bool last) {
+    using C = PaCfg<D, KT, WR>;
+    extern __shared__ __align__(1024) unsigned char sm[];
+    __shared__ int s_pos[64];                     // position of each row of the tile (-1: none)
+    __shared__ int s_tok[64];                     // token row * H + q head (-1: none)
+    __shared__ int s_bad[C::NS + 1][2];           // stage st's positions on bad pages, as a bit mask, at st % (NS + 1)
+    __shared__ int s_flag;                        // V had values that are not finite behind the mask
+    const Paged &a = A.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
+    const int wr = warp % WR, wk = warp / WR;
+    const uint32_t sm0 = smem_u32(sm);
+    // the trigger comes after the wait: a kernel that starts on it may read what this one waited for
+    if (!last) pdl_wait();
+    pdl_trigger();
+    const int n_unit = (own ? A.p.slots_s * a.n_seq * A.p.tiles_s : A.p.slots_p * A.p.tiles_p) * a.Hk;
+    for (int unit = blockIdx.x; unit < n_unit; unit += gridDim.x) {
+        // ---- which rows, which positions
+        int u = unit;
+        const int kh = u % a.Hk;
+        u /= a.Hk;
+        const int tile = u % (own ? A.p.tiles_s : A.p.tiles_p);
+        u /= own ? A.p.tiles_s : A.p.tiles_p;
+        int b = 0, slot, k0, k1, t0 = 0, n = 0, kv = 0;
+        if (own) {
+            b = u % a.n_seq;
+            slot = u / a.n_seq;
+            if (!paged_seq(a, b, t0, n, kv) && tid == 0 && slot == 0 && tile == 0 && kh == 0) paged_err(a, QMS_PAGED_ELEN);
+            k0 = a.prefix + slot * A.p.chunk_s;
+            k1 = min(kv, k0 + A.p.chunk_s);
+            if (k0 >= k1 || tile * 16 * WR >= n * a.G) continue;
+            slot += A.p.slots_p;
+        } else {
+            slot = u;
+            k0 = slot * A.p.chunk_p;
+            k1 = min(a.prefix, k0 + A.p.chunk_p);
+        }
+        const int *table = a.table + (own ? (int64_t)b * a.table_stride : 0);
+        __syncthreads();                          // the previous unit is done with shared memory
+        if (tid == 0) s_flag = 0;
+        if (tid < 2 * (C::NS + 1)) (&s_bad[0][0])[tid] = 0;
+        // rows of the tile: the sequence's own, or all tokens' (each token's sequence found by a warp)
+        const int r0 = tile * 16 * WR;
+        if (own) {
+            if (tid < 16 * WR) {
+                const int r = r0 + tid, i = r / a.G;
+                s_pos[tid] = i < n ? kv - n + i : -1;
+                s_tok[tid] = i < n ? (t0 + i) * a.H + kh * a.G + (r - i * a.G) : -1;
+            }
+        } else {
+            const int first = r0 / a.G, last = min(a.n_tok, (r0 + 16 * WR + a.G - 1) / a.G);
+            for (int t = first + warp; t < last; t += 4) {
+                int s0 = 0, sn = 0, skv = 0;
+                const int sb = paged_seq_of(a, t);
+                if (sb < a.n_seq && !paged_seq(a, sb, s0, sn, skv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
+                const int pos = t >= s0 && t < s0 + sn ? skv - sn + (t - s0) : -1;
+                for (int j = lane; j < a.G; j += 32) {
+                    const int r = t * a.G + j - r0;
+                    if (r >= 0 && r < 16 * WR) {
+                        s_pos[r] = pos;
+                        s_tok[r] = t * a.H + kh * a.G + j;
+                    }
+                }
+            }
+            if (tid < 16 * WR && r0 + tid >= a.n_tok * a.G) s_pos[tid] = s_tok[tid] = -1;
+        }
+        __syncthreads();
+        int lo_pos = 0x7fffffff, hi_pos = -1;     // least and largest position among the tile's rows
+        for (int r = 0; r < 16 * WR; r++) {
+            const int p = s_pos[r];
+            if (p >= 0) lo_pos = min(lo_pos, p);
+            hi_pos = max(hi_pos, p);
+        }
+        k1 = min(k1, hi_pos + 1);                 // nobody sees the rest
+        const int nst = k1 > k0 ? (k1 - k0 + kPaStage - 1) / kPaStage : 0;
+
+        auto load = [&](int st) {                 // stage st of the unit into its slot
+            const int slot_i = st % C::NS, base = k0 + st * kPaStage;
+            const uint32_t dk = sm0 + slot_i * C::STAGE, dv = dk + C::KB;
+#pragma unroll 4
+            for (int i = tid; i < kPaStage * C::CH; i += 128) {
+                const int r = i / C::CH, c = i % C::CH, p = base + r;
+                int64_t at = -1;
+                if (p < k1) {
+                    at = paged_at(a, table, p);
+                    if (at < 0 && c == 0) {
+                        atomicOr(&s_bad[st % (C::NS + 1)][r >> 5], 1 << (r & 31));
+                        paged_err(a, QMS_PAGED_EPAGE);
+                    }
+                }
+                const int64_t off = at < 0 ? 0 : at + kh * a.head_stride + c * 16;
+                const int cs = C::F16 ? c ^ (r & 7) : c;
+                cp_async16_or0(dk + r * C::KROW + cs * 16, a.k + off, at >= 0);
+                cp_async16_or0(dv + r * C::VROW + cs * 16, a.v + off, at >= 0);
+            }
+        };
+        for (int st = 0; st < C::NS - 1; st++) {
+            if (st < nst) load(st);
+            cp_commit();
+        }
+
+        // ---- q: this thread's elements of rows g and g + 8 of its row group, as mma A fragments
+        const int tok0 = s_tok[wr * 16 + g], tok1 = s_tok[wr * 16 + g + 8];
+        const int pos0 = s_pos[wr * 16 + g], pos1 = s_pos[wr * 16 + g + 8];
+        const int64_t qo0 = tok0 < 0 ? -1 : (tok0 / a.H) * A.ldq + (int64_t)(tok0 % a.H) * D;
+        const int64_t qo1 = tok1 < 0 ? -1 : (tok1 / a.H) * A.ldq + (int64_t)(tok1 % a.H) * D;
+        float f0 = A.scale2, f1 = A.scale2;       // score factors of the two rows
+        uint32_t qh[C::F16 ? D / 16 : 1][4], ql[C::F16 ? D / 16 : 1][4];
+        float qf[C::F16 ? 1 : D / 8][4];
+        if constexpr (C::F16) {
+            // each row scaled by a power of two into fp16's range (exact), undone in the score's factor
+            float x[2][D / 4], mx[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int64_t qo = r ? qo1 : qo0;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    const float2 v = qo < 0 ? make_float2(0.0f, 0.0f) : __ldcg(reinterpret_cast<const float2 *>(A.q + qo + i * 8 + tq * 2));
+                    x[r][2 * i] = v.x;
+                    x[r][2 * i + 1] = v.y;
+                    mx[r] = fmaxf(mx[r], fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(kFull, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(kFull, mx[r], 2));
+                const int e = mx[r] > 0.0f && mx[r] < INFINITY ? ilogbf(mx[r]) - 9 : 0;
+                (r ? f1 : f0) = ldexpf(A.scale2, e);
+                const float dn1 = ldexpf(1.0f, -e / 2), dn2 = ldexpf(1.0f, -e - -e / 2);   // 2^-e may not be a float
+#pragma unroll
+                for (int i = 0; i < D / 4; i++) x[r][i] = x[r][i] * dn1 * dn2;
+            }
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++) {
+                split_h2(x[0][4 * ks], x[0][4 * ks + 1], qh[ks][0], ql[ks][0]);
+                split_h2(x[1][4 * ks], x[1][4 * ks + 1], qh[ks][1], ql[ks][1]);
+                split_h2(x[0][4 * ks + 2], x[0][4 * ks + 3], qh[ks][2], ql[ks][2]);
+                split_h2(x[1][4 * ks + 2], x[1][4 * ks + 3], qh[ks][3], ql[ks][3]);
+            }
+        } else {
+            // the contraction's order is free: lane tq takes dims 16 i + 4 tq .. + 3, a 16-byte read of K
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 v0 = qo0 < 0 ? z : __ldcg(reinterpret_cast<const float4 *>(A.q + qo0 + i * 16 + tq * 4));
+                const float4 v1 = qo1 < 0 ? z : __ldcg(reinterpret_cast<const float4 *>(A.q + qo1 + i * 16 + tq * 4));
+                qf[2 * i][0] = v0.x, qf[2 * i][1] = v1.x, qf[2 * i][2] = v0.y, qf[2 * i][3] = v1.y;
+                qf[2 * i + 1][0] = v0.z, qf[2 * i + 1][1] = v1.z, qf[2 * i + 1][2] = v0.w, qf[2 * i + 1][3] = v1.w;
+            }
+        }
+
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+
+        for (int st = 0; st < nst; st++) {
+            cp_wait<C::NS - 2>();
+            __syncthreads();                      // the stage has landed; the slot before it is free
+            const int slot_i = st % C::NS, base = k0 + st * kPaStage;
+            const uint32_t kb = sm0 + slot_i * C::STAGE, vb = kb + C::KB;
+            const int bad0 = s_bad[st % (C::NS + 1)][0], bad1 = s_bad[st % (C::NS + 1)][1];
+            const bool masked = base + kPaStage - 1 > lo_pos || base + kPaStage > k1 || bad0 || bad1;
+            if (base + kPaStage - 1 > lo_pos) {
+                // behind the causal mask a weight is 0, but 0 * inf is not: such V are set aside
+                bool any = false;
+                for (int i = tid; i < kPaStage * C::CH; i += 128) {
+                    const int r = i / C::CH, c = i % C::CH;
+                    if (base + r <= lo_pos) continue;
+                    uint4 *pv = reinterpret_cast<uint4 *>(sm + slot_i * C::STAGE + C::KB + r * C::VROW + c * 16);
+                    uint4 v = *pv;
+                    if (drop_nonfinite((const KT *)nullptr, v)) {
+                        *pv = v;
+                        any = true;
+                    }
+                }
+                if (any) s_flag = 1;
+                __syncthreads();
+            }
+            if (tid < 2) s_bad[(st + C::NS) % (C::NS + 1)][tid] = 0;      // the mask that the next iteration fills
+            if (st + C::NS - 1 < nst) load(st + C::NS - 1);
+            cp_commit();
+
+            // ---- scores
+            float s[C::NT][4];
+            if constexpr (C::F16) {
+                float s2[C::NT][4];
+#pragma unroll
+                for (int i = 0; i < C::NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] = s2[i][j] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                    for (int i = 0; i < C::NT / 2; i++) {
+                        const int r = wk * C::KW + i * 16 + ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
+                        uint32_t kf[4];
+                        ldsm4(kf, kb + r * C::KROW + ((c ^ (r & 7)) << 4));
+                        mma_f16(s[2 * i], qh[ks], kf[0], kf[1]);
+                        mma_f16(s[2 * i + 1], qh[ks], kf[2], kf[3]);
+                        mma_f16(s2[2 * i], ql[ks], kf[0], kf[1]);
+                        mma_f16(s2[2 * i + 1], ql[ks], kf[2], kf[3]);
+                    }
+#pragma unroll
+                for (int i = 0; i < C::NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] += s2[i][j];
+            } else {
+                float s2[C::NT][4];
+#pragma unroll
+                for (int i = 0; i < C::NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] = s2[i][j] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++) {
+                    float ah[2][4], al[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            ah[h][j] = tf32_hi(qf[2 * ks + h][j]);
+                            al[h][j] = qf[2 * ks + h][j] - ah[h][j];
+                        }
+#pragma unroll
+                    for (int i = 0; i < C::NT; i++) {
+                        const float4 k = lds4(kb + (wk * C::KW + i * 8 + g) * C::KROW + ks * 64 + tq * 16);
+                        const float h0 = tf32_hi(k.x), h1 = tf32_hi(k.y), h2 = tf32_hi(k.z), h3 = tf32_hi(k.w);
+                        mma_tf32(s2[i], ah[0], k.x - h0, k.y - h1);
+                        mma_tf32(s2[i], al[0], h0, h1);
+                        mma_tf32(s[i], ah[0], h0, h1);
+                        mma_tf32(s2[i], ah[1], k.z - h2, k.w - h3);
+                        mma_tf32(s2[i], al[1], h2, h3);
+                        mma_tf32(s[i], ah[1], h2, h3);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < C::NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[i][j] += s2[i][j];
+            }
+            // ---- softmax of the stage: s becomes the weights
+            float n0 = m0, n1 = m1;
+#pragma unroll
+            for (int i = 0; i < C::NT; i++) {
+                const int r = wk * C::KW + i * 8 + tq * 2, p = base + r;
+                s[i][0] *= f0, s[i][1] *= f0, s[i][2] *= f1, s[i][3] *= f1;
+                if (masked) {
+                    const int bm = (r < 32 ? bad0 : bad1) >> (r & 31);
+                    const bool ok0 = p < k1 && !(bm & 1), ok1 = p + 1 < k1 && !(bm & 2);
+                    if (!ok0 || p > pos0) s[i][0] = -INFINITY;
+                    if (!ok1 || p + 1 > pos0) s[i][1] = -INFINITY;
+                    if (!ok0 || p > pos1) s[i][2] = -INFINITY;
+                    if (!ok1 || p + 1 > pos1) s[i][3] = -INFINITY;
+                }
+                n0 = fmaxf(n0, fmaxf(s[i][0], s[i][1]));
+                n1 = fmaxf(n1, fmaxf(s[i][2], s[i][3]));
+            }
+            n0 = fmaxf(n0, __shfl_xor_sync(kFull, n0, 1));
+            n1 = fmaxf(n1, __shfl_xor_sync(kFull, n1, 1));
+            n0 = fmaxf(n0, __shfl_xor_sync(kFull, n0, 2));
+            n1 = fmaxf(n1, __shfl_xor_sync(kFull, n1, 2));
+            const float b0 = n0 == -INFINITY ? 0.0f : n0 - kPaShift, b1 = n1 == -INFINITY ? 0.0f : n1 - kPaShift;
+            const float c0 = ex2(m0 - n0), c1 = ex2(m1 - n1);      // NaN only while nothing was seen: o and l are 0
+            if (n0 != m0 || n1 != m1) {
+                const float d0 = m0 == -INFINITY ? 0.0f : c0, d1 = m1 == -INFINITY ? 0.0f : c1;
+                l0 *= d0;
+                l1 *= d1;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
+            }
+            m0 = n0;
+            m1 = n1;
+#pragma unroll
+            for (int i = 0; i < C::NT; i++) {
+                s[i][0] = ex2(s[i][0] - b0), s[i][1] = ex2(s[i][1] - b0);
+                s[i][2] = ex2(s[i][2] - b1), s[i][3] = ex2(s[i][3] - b1);
+                l0 += s[i][0] + s[i][1];
+                l1 += s[i][2] + s[i][3];
+            }
+            // ---- o += weights * V
+            if constexpr (C::F16) {
+#pragma unroll
+                for (int kk = 0; kk < C::NT / 2; kk++) {
+                    uint32_t ph[4], pl[4];
+                    split_h2(s[2 * kk][0], s[2 * kk][1], ph[0], pl[0]);
+                    split_h2(s[2 * kk][2], s[2 * kk][3], ph[1], pl[1]);
+                    split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[2], pl[2]);
+                    split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[3], pl[3]);
+#pragma unroll
+                    for (int j = 0; j < D / 16; j++) {
+                        const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = 2 * j + (lane >> 4);
+                        uint32_t vf[4];
+                        ldsm4t(vf, vb + r * C::VROW + ((c ^ (r & 7)) << 4));
+                        mma_f16(o[2 * j], ph, vf[0], vf[1]);
+                        mma_f16(o[2 * j + 1], ph, vf[2], vf[3]);
+                        mma_f16(o[2 * j], pl, vf[0], vf[1]);
+                        mma_f16(o[2 * j + 1], pl, vf[2], vf[3]);
+                    }
+                }
+            } else {
+                // positions 2 tq, 2 tq + 1 of an 8-position tile are the fragment's k = tq, tq + 4; column g of
+                // output tile 4 j + c is dim 32 j + 4 g + c, so V too is read 16 bytes at a time
+#pragma unroll
+                for (int i = 0; i < C::NT; i++) {
+                    const float ah[4] = {tf32_hi(s[i][0]), tf32_hi(s[i][2]), tf32_hi(s[i][1]), tf32_hi(s[i][3])};
+                    const float al[4] = {s[i][0] - ah[0], s[i][2] - ah[1], s[i][1] - ah[2], s[i][3] - ah[3]};
+                    const uint32_t vr = vb + (wk * C::KW + i * 8 + tq * 2) * C::VROW + g * 16;
+#pragma unroll
+                    for (int j = 0; j < D / 32; j++) {
+                        const float4 x = lds4(vr + j * 128), y = lds4(vr + C::VROW + j * 128);
+                        const float xv[4] = {x.x, x.y, x.z, x.w}, yv[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const float xh = tf32_hi(xv[c]), yh = tf32_hi(yv[c]);
+                            mma_tf32(o[4 * j + c], ah, xv[c] - xh, yv[c] - yh);
+                            mma_tf32(o[4 * j + c], al, xh, yh);
+                            mma_tf32(o[4 * j + c], ah, xh, yh);
+                        }
+                    }
+                }
+            }
+        }
+        cp_wait<0>();
+        __syncthreads();                          // every warp is done with the stages
+        // dims of this thread's o[i][0..1] (row g) and o[i][2..3] (row g + 8)
+        auto dim = [&](int i, int j) {
+            if constexpr (C::F16) return i * 8 + tq * 2 + (j & 1);
+            else return (i >> 2) * 32 + (i & 3) + 4 * (tq * 2 + (j & 1));
+        };
+        if (s_flag && wk == 0) {
+            // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
+            for (int p = max(k0, lo_pos + 1); p < k1; p++) {
+                const int64_t at = paged_at(a, table, p);
+                if (at < 0) continue;
+                const KT *vr = reinterpret_cast<const KT *>(a.v + at + kh * a.head_stride);
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float v = kv_ld(vr + dim(i, j));
+                        if (!isfinite(v) && p <= (j < 2 ? pos0 : pos1)) o[i][j] += v;
+                    }
+            }
+        }
+        l0 += __shfl_xor_sync(kFull, l0, 1);
+        l1 += __shfl_xor_sync(kFull, l1, 1);
+        l0 += __shfl_xor_sync(kFull, l0, 2);
+        l1 += __shfl_xor_sync(kFull, l1, 2);
+        if (isnan(l0)) m0 = 0.0f;                 // scores that are all NaN leave no maximum, but are not nothing
+        if (isnan(l1)) m1 = 0.0f;
+        const int64_t po = (int64_t)slot * a.n_tok * a.H;
+        if constexpr (C::WK == 1) {
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int tok = r ? tok1 : tok0;
+                const float m = r ? m1 : m0, l = r ? l1 : l0;
+                if (tok < 0) continue;
+                float *dst = A.part_o + (po + tok) * D;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) dst[dim(i, j)] = m == -INFINITY ? 0.0f : o[i][2 * r + j];
+                if (tq == 0) A.part_ml[po + tok] = make_float2(m == -INFINITY ? m : m - kPaShift, l);
+            }
+        } else {
+            // join the position groups: group w's row r at red[(w * 16 WR + r)][D + 2]
+            float *red = reinterpret_cast<float *>(sm);
+            constexpr int LD = D + 2;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float *dst = red + ((wk * WR + wr) * 16 + g + 8 * r) * LD;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) dst[dim(i, j)] = o[i][2 * r + j];
+                if (tq == 0) {
+                    dst[D] = r ? m1 : m0;
+                    dst[D + 1] = r ? l1 : l0;
+                }
+            }
+            __syncthreads();
+            for (int r = warp; r < 16 * WR; r += 4) {
+                const int tok = s_tok[r];
+                if (tok < 0) continue;
+                float m = -INFINITY, l = 0.0f, x[D / 32], w[C::WK];
+#pragma unroll
+                for (int k = 0; k < C::WK; k++) m = fmaxf(m, red[(k * 16 * WR + r) * LD + D]);
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) x[d] = 0.0f;
+                if (m != -INFINITY) {
+#pragma unroll
+                    for (int k = 0; k < C::WK; k++) {
+                        const float *src = red + (k * 16 * WR + r) * LD;
+                        w[k] = ex2(src[D] - m);
+                        if (w[k] == 0.0f && src[D + 1] == 0.0f) continue;      // saw nothing: its o may be 0 * inf
+                        l = fmaf(w[k], src[D + 1], l);
+#pragma unroll
+                        for (int d = 0; d < D / 32; d++) x[d] = fmaf(w[k], src[lane + 32 * d], x[d]);
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) A.part_o[(po + tok) * D + lane + 32 * d] = x[d];
+                if (lane == 0) A.part_ml[po + tok] = make_float2(m == -INFINITY ? m : m - kPaShift, l);
+            }
+        }
+    }
+    if (last) pdl_wait();
+}
+
+// ---- joining the slots of a row --------------------------------------------------------------------
+// One warp per (token, q head): out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the row's slots in their
+// order; 0 where nothing was seen.
+template <int D>
+__global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
+    constexpr int J = D / 32;
+    const Paged &a = A.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)a.n_tok * a.H;
+    pdl_trigger();
+    pdl_wait();
+    if (row >= rows) return;
+    const int t = (int)(row / a.H);
+    int t0 = 0, n = 0, kv = 0;
+    const int b = paged_seq_of(a, t);
+    if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
+    float x[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) x[j] = 0.0f;
+    float l = 0.0f;
+    if (t >= t0 && t < t0 + n) {
+        const int ns = A.p.slots_p + (kv > a.prefix ? (kv - a.prefix + A.p.chunk_s - 1) / A.p.chunk_s : 0);
+        float M = -INFINITY;
+        for (int s = lane; s < ns; s += 32) M = fmaxf(M, __ldcg(&A.part_ml[s * rows + row]).x);
+        M = warp_max(M);
+        if (M != -INFINITY) {
+            for (int s0 = 0; s0 < ns; s0 += 32) {
+                const float2 ml = s0 + lane < ns ? __ldcg(&A.part_ml[(s0 + lane) * rows + row]) : make_float2(-INFINITY, 0.0f);
+                const float w = ex2(ml.x - M);
+                l += warp_sum(w * ml.y);
+                const int ne = min(32, ns - s0);
+#pragma unroll 8
+                for (int i = 0; i < ne; i++) {
+                    const float wi = __shfl_sync(kFull, w, i);
+                    const float *src = A.part_o + ((s0 + i) * rows + row) * D + lane * J;
+                    float v[J];
+                    if constexpr (J == 4) *reinterpret_cast<float4 *>(v) = __ldcg(reinterpret_cast<const float4 *>(src));
+                    else *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(src));
+#pragma unroll
+                    for (int j = 0; j < J; j++) x[j] = fmaf(wi, v[j], x[j]);
+                }
+            }
+        }
+    }
+    float *dst = A.out + t * A.ldo + (row - (int64_t)t * a.H) * D + lane * J;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < J; j++) dst[j] = l == 0.0f ? 0.0f : x[j] * inv;
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+// Row groups per tile: a tile as tall as the rows there are, up to 64 (more rows per K / V read).
+static int row_groups(int64_t rows) { return rows > 32 ? 4 : rows > 16 ? 2 : 1; }
+
+void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
+    const int resident = 148 * (type == QMS_T_F16 ? 2 : 1);
+    const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G;
+    const int own = std::max(0, a.max_kv - a.prefix);
+    p.wr_p = row_groups(rows_p);
+    p.wr_s = row_groups(rows_s);
+    p.tiles_p = (int)((rows_p + 16 * p.wr_p - 1) / (16 * p.wr_p));
+    p.tiles_s = (int)((rows_s + 16 * p.wr_s - 1) / (16 * p.wr_s));
+    // chunks: about two units per resident CTA
+    const int64_t st_p = (a.prefix + kPaStage - 1) / kPaStage, st_s = (own + kPaStage - 1) / kPaStage;
+    const int64_t work = (st_p * p.tiles_p + st_s * p.tiles_s * a.n_seq) * a.Hk;
+    const int64_t per = std::max<int64_t>(1, work / (2 * resident));
+    p.chunk_p = p.chunk_s = (int)(per * kPaStage);
+    p.slots_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
+    p.slots_s = (own + p.chunk_s - 1) / p.chunk_s;
+}
+
+static int64_t al256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
+    const int64_t n = (int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H;
+    return al256(n * D * 4) + al256(n * 8);
+}
+
+template <int D, typename KT, int WR>
+static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
+    using C = PaCfg<D, KT, WR>;
+    const int64_t units = own ? (int64_t)A.p.slots_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.slots_p * A.p.tiles_p * A.a.Hk;
+    QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
+    static unsigned long long set = 0;                          // per device
+    int dev = 0;
+    QMS_CK(cudaGetDevice(&dev));
+    if (!(set >> (dev & 63) & 1)) {
+        QMS_CK(cudaFuncSetAttribute(k_paged_attn<D, KT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        set |= 1ull << (dev & 63);
+    }
+    const int grid = (int)std::min<int64_t>(units, 148 * 8);
+    QMS_CK(launch_pdl(k_paged_attn<D, KT, WR>, dim3(grid), dim3(128), C::SMEM, s, A, own, last));
+    return QMS_CUDA_OK;
+}
+
+template <int D, typename KT>
+static int launch_attn(const PagedAttn &A, cudaStream_t s) {
+    bool before = false;
+    for (int kind = 0; kind < 2; kind++) {
+        const bool own = kind == 1;
+        if (own ? !(A.p.slots_s && A.p.tiles_s && A.a.n_seq) : !(A.p.slots_p && A.p.tiles_p)) continue;
+        const int wr = own ? A.p.wr_s : A.p.wr_p;
+        const int rc = wr == 4   ? launch_attn_wr<D, KT, 4>(A, own, before, s)
+                       : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
+                                 : launch_attn_wr<D, KT, 1>(A, own, before, s);
+        if (rc) return rc;
+        before = true;
+    }
+    return QMS_CUDA_OK;
+}
+
+int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, const float *q, int64_t ldq, float scale,
+                           float *out, int64_t ldo, void *ws, cudaStream_t s) {
+    PagedAttn A;
+    memset(&A, 0, sizeof A);
+    A.a = a;
+    A.p = p;
+    A.q = q;
+    A.out = out;
+    A.ldq = ldq;
+    A.ldo = ldo;
+    A.scale2 = scale * 1.4426950408889634f;
+    A.part_o = (float *)ws;
+    A.part_ml = (float2 *)((char *)ws + al256((int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H * D * 4));
+    int rc;
+    if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, s) : launch_attn<64, __half>(A, s);
+    else rc = D == 128 ? launch_attn<128, float>(A, s) : launch_attn<64, float>(A, s);
+    if (rc) return rc;
+    const int64_t rows = (int64_t)a.n_tok * a.H;
+    const dim3 grid((unsigned)((rows + 7) / 8));
+    if (D == 128) QMS_CK(launch_pdl(k_paged_merge<128>, grid, dim3(256), 0, s, A));
+    else QMS_CK(launch_pdl(k_paged_merge<64>, grid, dim3(256), 0, s, A));
+    return QMS_CUDA_OK;
+}
+
+}  // namespace qms
