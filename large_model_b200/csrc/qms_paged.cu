@@ -44,11 +44,11 @@ __global__ void __launch_bounds__(256) k_paged_append(const Paged a, const float
         const float *nw = hh < a.H ? q_norm : k_norm;
         float w[J], c[JH], s[JH];
 #pragma unroll
-        for (int j = 0; j < J; j++) w[j] = __ldg(nw + lane + 32 * j);
+        for (int j = 0; j < J; j++) w[j] = nw[lane + 32 * j];
 #pragma unroll
         for (int j = 0; j < JH; j++) {
-            c[j] = __ldg(rope_cos + (int64_t)p * (D / 2) + lane + 32 * j);
-            s[j] = __ldg(rope_sin + (int64_t)p * (D / 2) + lane + 32 * j);
+            c[j] = rope_cos[(int64_t)p * (D / 2) + lane + 32 * j];
+            s[j] = rope_sin[(int64_t)p * (D / 2) + lane + 32 * j];
         }
         norm_rope_pre<D>(x, w, c, s, eps);
     }

@@ -24,16 +24,16 @@ __device__ __forceinline__ void paged_err(const Paged &a, int bit) {
 // (independent loads: one round trip up to 32 sequences, not a chain of dependent ones).
 __device__ __forceinline__ int paged_seq_of(const Paged &a, int t) {
     int n = 0;
-    for (int b = threadIdx.x & 31; b < a.n_seq; b += 32) n += __ldg(a.q_start + b + 1) <= t;
+    for (int b = threadIdx.x & 31; b < a.n_seq; b += 32) n += a.q_start[b + 1] <= t;
     return __reduce_add_sync(kFull, n);
 }
 
 // Sequence b's rows [t0, t0 + n) and cache length. False (n = kv = 0) when the batch arrays do not make
 // sense for it; such a sequence counts as idle.
 __device__ __forceinline__ bool paged_seq(const Paged &a, int b, int &t0, int &n, int &kv) {
-    t0 = __ldg(a.q_start + b);
-    n = __ldg(a.q_start + b + 1) - t0;
-    kv = __ldg(a.kv_len + b);
+    t0 = a.q_start[b];
+    n = a.q_start[b + 1] - t0;
+    kv = a.kv_len[b];
     if (t0 >= 0 && n >= 0 && n <= a.max_q && n <= a.n_tok - t0 && kv >= 0 && kv <= a.max_kv) return true;
     n = kv = 0;
     return false;
@@ -42,7 +42,7 @@ __device__ __forceinline__ bool paged_seq(const Paged &a, int b, int &t0, int &n
 // Byte offset of position p of table row `row` in the K / V pool, or -1 on a bad page id.
 // 0 <= p < table_stride * page_size.
 __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int p) {
-    const int page = __ldg(row + (p >> a.page_log));
+    const int page = row[p >> a.page_log];
     if ((unsigned)page >= (unsigned)a.n_pages) return -1;
     return page * a.page_stride + (p & ((1 << a.page_log) - 1)) * a.pos_stride;
 }

@@ -1,73 +1,170 @@
 // qms_verify.cu - probabilities of logits rows and the verification of drafted tokens on B200 (sm_100a).
 //
 // The reference draws one token from one row on the host (sample(), src/chat.c:36-69); it has no drafts.
+#include <cooperative_groups.h>
 #include <math.h>
 #include <string.h>
 
-#include "qms_moe.cuh"
+#include "qms_kv.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace qms {
 
-constexpr int kRowThreads = 1024;
+// A row is cut over a cluster of up to 8 CTAs, which exchange their partial results through distributed
+// shared memory once.
+constexpr int kRowCtas = 8;
 
 // ---- probabilities -------------------------------------------------------------------------------
-// p = exp((l - max) / temp) / sum, one CTA per row.
-__global__ void __launch_bounds__(kRowThreads) k_probs(const float *l, int64_t ldl, int V, float temp, float *p, int64_t ldp) {
-    __shared__ float s_v[32];
-    __shared__ int s_i[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// (m, i): a maximum and its first index
+__device__ __forceinline__ void join_mi(float &m, int &i, float om, int oi) {
+    if (om > m || (om == m && oi < i)) {
+        m = om;
+        i = oi;
+    }
+}
+
+// Values of a row that a CTA keeps in shared memory (76 KB: three CTAs per SM, and a row of 155,648 values
+// in a cluster of 8); what a longer slice has beyond them is read from memory in each pass.
+constexpr int kProbsKeep = 19456, kProbsThreads = 512, kProbsWarps = kProbsThreads / 32;
+
+// p = 2^((l - max) c) / sum, c = log2(e) / temp; GREEDY: 1 at the first maximum. Grid: rows x
+// cluster. A slice comes into shared memory by cp.async (16 bytes at a time where the row is aligned); its
+// weights replace it there, relative to the slice's own maximum, and one exchange over the cluster gives every
+// CTA the common factor. The order of the additions does not depend on the row's address.
+// Bound by memory: 320 rows of 151,936 move 389 MB.
+template <bool GREEDY>
+__global__ void __launch_bounds__(kProbsThreads, 3) k_probs(const float *l, int64_t ldl, int V, float c, float *p, int64_t ldp) {
+    extern __shared__ __align__(16) float x[];
+    __shared__ float s_m[kProbsWarps], s_z[kProbsWarps], s_cm[kRowCtas], s_cz[kRowCtas];
+    __shared__ int s_i[kProbsWarps], s_ci[kRowCtas];
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
+    auto started = cl.barrier_arrive();                    // waited for before the first write to another CTA
     pdl_trigger();
     pdl_wait();
-    l += blockIdx.x * ldl;
-    p += blockIdx.x * ldp;
-    float m = -INFINITY;
-    int at = V;                                            // first index of the maximum (NaN never is)
-    for (int i = tid; i < V; i += kRowThreads) {
-        const float x = l[i];
-        if (x > m || (at == V && x == m)) {
-            m = x;
-            at = i;
-        }
+    const int64_t r = blockIdx.x / nc;
+    const int groups = (V + 3) >> 2;                       // slices start at multiples of 4 values
+    const int lo = (int)((int64_t)groups * rank / nc) * 4, n = min(V, (int)((int64_t)groups * (rank + 1) / nc) * 4) - lo;
+    l += r * ldl + lo;
+    p += r * ldp + lo;
+    const int kept = min(n, kProbsKeep), n4 = (kept + 3) >> 2;
+    float4 *x4 = reinterpret_cast<float4 *>(x);
+    const bool vec = ((uintptr_t)l & 15) == 0;
+    if (vec) {
+        for (int i = tid; i < kept >> 2; i += kProbsThreads) cp_async16(x + 4 * i, l + 4 * i);
+        if (tid < (kept & 3)) cp_async4(x + (kept & ~3) + tid, l + (kept & ~3) + tid);
+    } else {
+#pragma unroll 4
+        for (int i = tid; i < kept; i += kProbsThreads) cp_async4(x + i, l + i);
     }
+    if (tid >= kept && tid < 4 * n4) x[tid] = -INFINITY;   // (a slice below one group)
+    for (int i = max(kept, kProbsThreads) + tid; i < 4 * n4; i += kProbsThreads) x[i] = -INFINITY;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+
+    float m = -INFINITY;
+    int at = 0x7fffffff;
+    auto maximum = [&](float y, int i) {
+        if constexpr (GREEDY) {
+            if (y > m) at = lo + i;
+        }
+        m = fmaxf(m, y);
+    };
+#pragma unroll 4
+    for (int i = tid; i < n4; i += kProbsThreads) {
+        const float4 y = x4[i];
+        maximum(y.x, 4 * i);
+        maximum(y.y, 4 * i + 1);
+        maximum(y.z, 4 * i + 2);
+        maximum(y.w, 4 * i + 3);
+    }
+    for (int i = kept + tid; i < n; i += kProbsThreads) maximum(l[i], i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-        if (om > m || (om == m && oi < at)) {
-            m = om;
-            at = oi;
-        }
+        const float om = __shfl_xor_sync(kFull, m, o);
+        if constexpr (GREEDY) join_mi(m, at, om, __shfl_xor_sync(kFull, at, o));
+        else m = fmaxf(m, om);
     }
-    if (lane == 0) {
-        s_v[warp] = m;
-        s_i[warp] = at;
-    }
+    if (lane == 0) s_m[warp] = m, s_i[warp] = at;
     __syncthreads();
-    for (int w = 0; w < 32; w++)
-        if (s_v[w] > m || (s_v[w] == m && s_i[w] < at)) {
-            m = s_v[w];
-            at = s_i[w];
+    m = s_m[lane & (kProbsWarps - 1)], at = s_i[lane & (kProbsWarps - 1)];
+#pragma unroll
+    for (int o = kProbsWarps / 2; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(kFull, m, o);
+        if constexpr (GREEDY) join_mi(m, at, om, __shfl_xor_sync(kFull, at, o));
+        else m = fmaxf(m, om);
+    }
+    // the slice's weights under its own maximum
+    const float M = m == -INFINITY ? 0.0f : m;
+    float z = 0.0f;
+    if constexpr (!GREEDY) {
+        for (int i0 = tid; i0 < n4; i0 += 8 * kProbsThreads) {      // sums of 32: no long chain of roundings
+            float g = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = i0 + k * kProbsThreads;
+                if (i < n4) {
+                    float4 y = x4[i];
+                    y = make_float4(ex2f((y.x - M) * c), ex2f((y.y - M) * c), ex2f((y.z - M) * c), ex2f((y.w - M) * c));
+                    x4[i] = y;
+                    g += (y.x + y.y) + (y.z + y.w);
+                }
+            }
+            z += g;
         }
-    if (!(temp > 0.0f)) {
-        const bool none = m == -INFINITY;
+        for (int i0 = kept + tid; i0 < n; i0 += 32 * kProbsThreads) {
+            float g = 0.0f;
+            for (int i = i0; i < n && i < i0 + 32 * kProbsThreads; i += kProbsThreads) g += ex2f((l[i] - M) * c);
+            z += g;
+        }
+        z = warp_sum(z);
+        if (lane == 0) s_z[warp] = z;
         __syncthreads();
-        for (int i = tid; i < V; i += kRowThreads) p[i] = i == at && !none ? 1.0f : 0.0f;
-        return;
+        z = s_z[lane & (kProbsWarps - 1)];
+#pragma unroll
+        for (int o = kProbsWarps / 2; o > 0; o >>= 1) z += __shfl_xor_sync(kFull, z, o);
     }
-    const float base = m == -INFINITY ? 0.0f : m;
-    float z = 0.0f;                                        // in groups of 32: no long chain of roundings
-    for (int i = tid; i < V; i += 32 * kRowThreads) {
-        float g = 0.0f;
-        for (int j = i; j < V && j < i + 32 * kRowThreads; j += kRowThreads) g += expf(__fdiv_rn(l[j] - base, temp));
-        z += g;
+    cl.barrier_wait(std::move(started));
+    if (tid < nc) {                                        // to every CTA of the row
+        *cl.map_shared_rank(&s_cm[rank], tid) = m;
+        *cl.map_shared_rank(&s_cz[rank], tid) = z;
+        *cl.map_shared_rank(&s_ci[rank], tid) = at;
     }
-    z = warp_sum(z);
-    __syncthreads();
-    if (lane == 0) s_v[warp] = z;
-    __syncthreads();
-    z = 0.0f;
-    for (int w = 0; w < 32; w++) z += s_v[w];
-    for (int i = tid; i < V; i += kRowThreads) p[i] = z == 0.0f ? 0.0f : __fdiv_rn(expf(__fdiv_rn(l[i] - base, temp)), z);
+    cl.sync();
+    if constexpr (GREEDY) {
+        m = s_cm[0], at = s_ci[0];
+        for (int k = 1; k < nc; k++) join_mi(m, at, s_cm[k], s_ci[k]);
+        for (int i = tid; i < n; i += kProbsThreads) p[i] = lo + i == at ? 1.0f : 0.0f;
+    } else {
+        m = -INFINITY;
+        for (int k = 0; k < nc; k++) m = fmaxf(m, s_cm[k]);
+        const float top = m == -INFINITY ? 0.0f : m;
+        z = 0.0f;
+        for (int k = 0; k < nc; k++) {                     // a slice of -inf alone has no weight (0, or NaN)
+            const float zk = s_cz[k];
+            z += s_cm[k] == -INFINITY ? zk : zk * ex2f((s_cm[k] - top) * c);
+        }
+        const float inv = z == 0.0f ? 0.0f : __fdiv_rn(1.0f, z), f = s_cm[rank] == -INFINITY ? inv : ex2f((M - top) * c) * inv;
+        if (((uintptr_t)p & 15) == 0) {
+#pragma unroll 4
+            for (int i = tid; i < kept >> 2; i += kProbsThreads) {
+                const float4 y = x4[i];
+                *reinterpret_cast<float4 *>(p + 4 * i) = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+            }
+            if (tid < (kept & 3)) p[(kept & ~3) + tid] = x[(kept & ~3) + tid] * f;
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < kept; i += kProbsThreads) p[i] = x[i] * f;
+        }
+        for (int i = kept + tid; i < n; i += kProbsThreads) p[i] = ex2f((l[i] - top) * c) * inv;
+    }
 }
 
 // ---- verification --------------------------------------------------------------------------------
@@ -83,84 +180,248 @@ __device__ __forceinline__ void verify_err(const VerifyArgs &a, int bit) {
     if (a.err) atomicOr(a.err, bit);
 }
 
-// A probability as a whole number of 2^-40 (round half to even; NaN and negative: 0, above 1: 2^40).
-__device__ __forceinline__ unsigned long long verify_weight(float r) {
-    return r > 0.0f ? (unsigned long long)__float2ll_rn(fminf(r, 1.0f) * 1099511627776.0f) : 0ull;
+typedef unsigned long long u64;
+
+// A probability as a whole number of 2^-40 (round half to even; NaN and negative: 0, above 1: 2^40). Whole
+// numbers add up to the same sum in any order, so the drawn token does not depend on the split.
+__device__ __forceinline__ u64 verify_weight(float r) {
+    return r > 0.0f ? (u64)__float2ll_rn(fminf(r, 1.0f) * 1099511627776.0f) : 0ull;
 }
 
-// One CTA per sequence: the drafts in order, then the next token by inversion of the cumulative weights.
-__global__ void __launch_bounds__(kRowThreads) k_verify(const VerifyArgs a) {
-    __shared__ unsigned long long s_w[kRowThreads];
-    __shared__ int s_n, s_pick;
-    const int b = blockIdx.x, tid = threadIdx.x, N = a.max_draft;
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+// Which lane's interval of the cumulative sums holds `want` (31 bits set where none), and `before` up to it.
+__device__ __forceinline__ int warp_find_u64(u64 mine, u64 want, u64 &before) {
+    u64 inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(kFull, inc, o);
+        if ((threadIdx.x & 31) >= o) inc += t;
+    }
+    const unsigned hit = __ballot_sync(kFull, before + inc > want);
+    const int at = hit ? __ffs(hit) - 1 : -1;
+    const u64 e = __shfl_sync(kFull, inc - mine, at < 0 ? 0 : at), all = __shfl_sync(kFull, inc, 31);
+    before += at < 0 ? all : e;
+    return at;
+}
+
+constexpr int kVerBatch = 8;          // loads in flight per lane: a batch is 256 values of a warp's segment
+
+// What is left of p behind the rejected draft: p - q, p without token x, or p.
+struct Remains {
+    const float *p, *q;
+    int x;
+    __device__ __forceinline__ void load(int i0, int end, float (&r)[kVerBatch]) const {
+        float w[kVerBatch];
+#pragma unroll
+        for (int k = 0; k < kVerBatch; k++) r[k] = i0 + 32 * k < end ? __ldcg(p + i0 + 32 * k) : 0.0f;
+        if (q) {
+#pragma unroll
+            for (int k = 0; k < kVerBatch; k++) w[k] = i0 + 32 * k < end ? __ldcg(q + i0 + 32 * k) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < kVerBatch; k++) r[k] = __fsub_rn(r[k], w[k]);
+        } else if (x >= 0) {
+#pragma unroll
+            for (int k = 0; k < kVerBatch; k++)
+                if (i0 + 32 * k == x) r[k] = 0.0f;
+        }
+    }
+};
+
+// One cluster per sequence: the drafts first (every CTA finds the same count), then the next token by
+// inversion of the cumulative weights of the row. Every warp adds up its segment, 256 values at a time, and keeps
+// those sums; the one warp whose segment holds the wanted weight finds the 256, then the 32, then the value.
+// Bound by the latencies of that chain (drafts, their probabilities, the row, the exchange, the search) for
+// one sequence, by memory for many.
+template <int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) k_verify(const VerifyArgs a) {
+    constexpr int kWarps = NT / 32;
+    extern __shared__ u64 s_sum[];                         // [kWarps][batches] sums of 256 values
+    __shared__ u64 s_w[kWarps], s_c[2][kRowCtas];
+    __shared__ int s_n;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, N = a.max_draft, V = a.V;
+    const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks(), b = blockIdx.x / nc;
+    auto started = cl.barrier_arrive();
     pdl_trigger();
     pdl_wait();
     const int nd = a.n_draft ? a.n_draft[b] : N;
     const int r0 = a.row_start ? a.row_start[b] : b * (N + 1);
     int *tok = a.tokens + (int64_t)b * (N + 1);
-    if (nd < 0 || nd > N || r0 < 0 || r0 > a.p_rows - nd - 1) {
-        if (tid == 0) {
-            verify_err(a, QMS_PAGED_ELEN);
-            a.n_accept[b] = 0;
+    const int *draft = a.draft + (int64_t)b * N;
+    const float *u = a.u + (int64_t)b * (N + 1);
+    if (nd < 0 || nd > N || r0 < 0 || r0 > a.p_rows - nd - 1) {         // the same for the whole cluster
+        if (rank == 0) {
+            if (tid == 0) {
+                verify_err(a, QMS_PAGED_ELEN);
+                a.n_accept[b] = 0;
+            }
+            for (int i = tid; i <= N; i += NT) tok[i] = -1;
         }
-        for (int i = tid; i <= N; i += kRowThreads) tok[i] = -1;
+        cl.barrier_wait(std::move(started));
         return;
     }
-    if (tid == 0) {
+    if (warp == 0) {
         int n = 0;
-        for (; n < nd; n++) {
-            const int x = a.draft[(int64_t)b * N + n];
-            if (x < 0 || x >= a.V) {
-                verify_err(a, QMS_PAGED_ETOKEN);
-                break;
+        for (int i0 = 0; i0 < nd; i0 += 32) {              // 32 drafts at a time, up to the first that falls
+            const int i = i0 + lane;
+            bool fell = false;
+            if (i < nd) {
+                const int x = draft[i];
+                fell = x < 0 || x >= V;
+                if (!fell) {
+                    const float px = a.p[(int64_t)(r0 + i) * a.ldp + x];
+                    const float qx = a.q ? a.q[((int64_t)b * N + i) * a.ldq + x] : 1.0f;
+                    fell = !(__fmul_rn(u[i], qx) < px);
+                }
             }
-            const float qx = a.q ? a.q[((int64_t)b * N + n) * a.ldq + x] : 1.0f;
-            if (!(__fmul_rn(a.u[(int64_t)b * (N + 1) + n], qx) < a.p[(int64_t)(r0 + n) * a.ldp + x])) break;
+            const unsigned f = __ballot_sync(kFull, fell);
+            n = min(nd, f ? i0 + __ffs(f) - 1 : i0 + 32);
+            if (f) break;
         }
-        s_n = n;
-        s_pick = -1;
+        if (lane == 0) s_n = n;
     }
     __syncthreads();
-    const int n = s_n, x = n < nd ? a.draft[(int64_t)b * N + n] : -1;
-    const float *p = a.p + (int64_t)(r0 + n) * a.ldp;
-    const float *q = x >= 0 && x < a.V && a.q ? a.q + ((int64_t)b * N + n) * a.ldq : nullptr;
-    const int per = (a.V + kRowThreads - 1) / kRowThreads, i0 = min(a.V, tid * per), i1 = min(a.V, i0 + per);
-    const float u = a.u[(int64_t)b * (N + 1) + N];
-    for (int pass = 0; pass < 2; pass++) {                  // the remainder of p over q; then p itself
-        auto weight = [&](int i) {
-            float r = p[i];
-            if (pass == 0 && q) r = __fsub_rn(r, q[i]);
-            if (pass == 0 && !a.q && i == x) r = 0.0f;
-            return verify_weight(r);
-        };
-        unsigned long long w = 0, before = 0, total = 0;
-        for (int i = i0; i < i1; i++) w += weight(i);
-        s_w[tid] = w;
-        __syncthreads();
-        for (int i = 0; i < kRowThreads; i++) {
-            if (i < tid) before += s_w[i];
-            total += s_w[i];
+    const int n = s_n, x = n < nd ? draft[n] : -1;
+    const bool known = x >= 0 && x < V;
+    Remains rem;
+    rem.p = a.p + (int64_t)(r0 + n) * a.ldp;
+    rem.q = known && a.q ? a.q + ((int64_t)b * N + n) * a.ldq : nullptr;
+    rem.x = known ? x : -1;
+    const int seg = rank * kWarps + warp, segs = nc * kWarps, batches = (V / segs + 256) / 256;
+    const int lo = (int)((int64_t)V * seg / segs), hi = (int)((int64_t)V * (seg + 1) / segs);
+    const u64 m = (u64)floorf(fminf(fmaxf(u[N], 0.0f), 0.99999994f) * 16777216.0f);
+    bool found = false;
+    for (int pass = 0; pass < 2 && !found; pass++) {        // what p has over q; where that is nothing, p itself
+        u64 w = 0;
+        for (int k = 0; lo + 256 * k < hi; k++) {
+            float r[kVerBatch];
+            rem.load(lo + 256 * k + lane, hi, r);
+            u64 t = 0;
+#pragma unroll
+            for (int j = 0; j < kVerBatch; j++) t += verify_weight(r[j]);
+            t = warp_sum_u64(t);
+            if (lane == 0) s_sum[warp * batches + k] = t;
+            w += t;
         }
+        __syncthreads();                                   // the last pass is done with s_w
+        if (lane == 0) s_w[warp] = w;
         __syncthreads();
-        if (total == 0) continue;
-        const unsigned long long m = (unsigned long long)floorf(fminf(fmaxf(u, 0.0f), 0.99999994f) * 16777216.0f);
-        const unsigned long long want = (total >> 24) * m + (((total & 0xFFFFFFull) * m) >> 24);     // floor(total u)
-        if (before <= want && want < before + w) {
-            int i = i0;
-            for (; i < i1; i++) {
-                before += weight(i);
-                if (before > want) break;
+        u64 cta = 0, before = 0;
+        for (int k = 0; k < kWarps; k++) {
+            if (k < warp) before += s_w[k];
+            cta += s_w[k];
+        }
+        if (pass == 0) cl.barrier_wait(std::move(started));
+        if (tid < nc) *cl.map_shared_rank(&s_c[pass][rank], tid) = cta;
+        cl.sync();
+        u64 total = 0;
+        for (int k = 0; k < nc; k++) {
+            if (k < rank) before += s_c[pass][k];
+            total += s_c[pass][k];
+        }
+        if (total == 0) {
+            rem.q = nullptr;
+            rem.x = -1;
+            continue;
+        }
+        found = true;
+        const u64 want = (total >> 24) * m + (((total & 0xFFFFFFull) * m) >> 24);        // floor(total * u)
+        if (before > want || want >= before + w) continue;                             // in another warp's segment
+        int at = -1, k0 = 0;
+        for (; at < 0 && k0 < batches; k0 += 32)
+            at = warp_find_u64(k0 + lane < batches && lo + 256 * (k0 + lane) < hi ? s_sum[warp * batches + k0 + lane] : 0, want, before);
+        if (at < 0) continue;                              // not reached: the segment holds it
+        const int i0 = lo + 256 * (k0 - 32 + at);
+        float r[kVerBatch];
+        u64 t[kVerBatch];
+        rem.load(i0 + lane, hi, r);                        // the batch once more, from L2
+#pragma unroll
+        for (int j = 0; j < kVerBatch; j++) t[j] = warp_sum_u64(verify_weight(r[j]));
+        bool done = false;
+#pragma unroll
+        for (int j = 0; j < kVerBatch; j++) {
+            if (done) continue;
+            if (before + t[j] <= want) {
+                before += t[j];
+                continue;
             }
-            s_pick = i;
+            done = true;
+            const int e = warp_find_u64(verify_weight(r[j]), want, before);
+            if (lane == 0) tok[n] = i0 + 32 * j + e;
         }
-        break;
     }
-    __syncthreads();
-    if (tid == 0) {
-        a.n_accept[b] = n;
-        if (s_pick < 0) verify_err(a, QMS_PAGED_EMASS);
+    if (rank == 0) {
+        if (tid == 0) {
+            a.n_accept[b] = n;
+            if (!found) {
+                verify_err(a, QMS_PAGED_EMASS);
+                tok[n] = -1;
+            }
+            if (n < nd && !known) verify_err(a, QMS_PAGED_ETOKEN);
+        }
+        for (int i = tid; i <= N; i += NT)
+            if (i != n) tok[i] = i < n ? draft[i] : -1;
     }
-    for (int i = tid; i <= N; i += kRowThreads) tok[i] = i < n ? a.draft[(int64_t)b * N + i] : i == n ? s_pick : -1;
+}
+
+// Cluster and PDL launch of a row kernel.
+template <typename... P, typename... Q>
+static int launch_rows(void (*kern)(P...), int threads, int rows, int nc, size_t smem, cudaStream_t s, Q... args) {
+    QMS_REQUIRE((int64_t)rows * nc < (1ll << 31), QMS_CUDA_EINVAL, "too many rows (%d)", rows);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3((unsigned)(rows * nc));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = nc;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    QMS_CK(cudaLaunchKernelEx(&cfg, kern, ((P)args)...));
+    return QMS_CUDA_OK;
+}
+
+// CTAs per row: as many as hold it in shared memory (k_probs), then, while the rows leave SMs without a CTA, twice
+// as many (of 4096 values or more).
+static int row_ctas(int rows, int V) {
+    int nc = 1;
+    while (nc < kRowCtas && (V > nc * kProbsKeep || ((int64_t)rows * nc * 2 <= 148 && V > nc * 8192))) nc *= 2;
+    return nc;
+}
+
+static int launch_probs(const float *l, int64_t ldl, int rows, int V, float temp, float *p, int64_t ldp, cudaStream_t s) {
+    static unsigned long long set = 0;                     // per device
+    int dev = 0;
+    QMS_CK(cudaGetDevice(&dev));
+    if (!(set >> (dev & 63) & 1)) {
+        QMS_CK(cudaFuncSetAttribute(k_probs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsKeep * 4));
+        QMS_CK(cudaFuncSetAttribute(k_probs<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsKeep * 4));
+        set |= 1ull << (dev & 63);
+    }
+    const int nc = row_ctas(rows, V), slice = ((V + 3) / 4 / nc + 1) * 4;
+    const size_t smem = (size_t)(slice < kProbsKeep ? slice : kProbsKeep) * 4;
+    if (!(temp > 0.0f)) return launch_rows(k_probs<true>, kProbsThreads, rows, nc, smem, s, l, ldl, V, 0.0f, p, ldp);
+    // a scale of 0 or infinity would make NaN of the logits -inf and of the maximum
+    const float c = fminf(fmaxf(1.4426950408889634f / temp, 1e-37f), 1e37f);
+    return launch_rows(k_probs<false>, kProbsThreads, rows, nc, smem, s, l, ldl, V, c, p, ldp);
+}
+
+static int launch_verify(const VerifyArgs &a, cudaStream_t s) {
+    // few sequences: CTAs of 1024 threads, the shortest chain; more than the SMs hold of those: 256 threads, so
+    // that 64 sequences and more are resident at once
+    const int nc = row_ctas(a.n_seq, a.V), nt = a.n_seq * nc <= 148 ? 1024 : 256, segs = nc * (nt / 32);
+    const size_t smem = (size_t)(nt / 32) * ((a.V / segs + 256) / 256) * 8;
+    if (nt == 1024) return launch_rows(k_verify<1024>, nt, a.n_seq, nc, smem, s, a);
+    return launch_rows(k_verify<256>, nt, a.n_seq, nc, smem, s, a);
 }
 
 }  // namespace qms
@@ -176,8 +437,7 @@ int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float 
                 "probs: rows of %d need ldl and ldp of at least that (in place: equal ones)", vocab);
     QMS_REQUIRE(!isnan(temp), QMS_CUDA_EINVAL, "probs: temp is NaN");
     if (rows == 0) return QMS_CUDA_OK;
-    QMS_CK(launch_pdl(k_probs, dim3(rows), dim3(kRowThreads), 0, (cudaStream_t)stream, logits, ldl, vocab, temp, p, ldp));
-    return QMS_CUDA_OK;
+    return launch_probs(logits, ldl, rows, vocab, temp, p, ldp, (cudaStream_t)stream);
 }
 
 int qms_cuda_verify(const float *p, int64_t ldp, int p_rows, const int *row_start, const float *q, int64_t ldq,
@@ -209,8 +469,7 @@ int qms_cuda_verify(const float *p, int64_t ldp, int p_rows, const int *row_star
     a.n_accept = n_accept;
     a.tokens = tokens;
     a.err = err;
-    QMS_CK(launch_pdl(k_verify, dim3(n_seq), dim3(kRowThreads), 0, (cudaStream_t)stream, a));
-    return QMS_CUDA_OK;
+    return launch_verify(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

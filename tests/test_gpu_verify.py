@@ -246,6 +246,18 @@ def test_probs_rows_with_special_values(cuda):
     assert torch.equal(m.probs(l, -1.0), p)
 
 
+def test_probs_of_a_row_that_is_mostly_masked(cuda):
+    """All values far below 0, and so few of them that most threads see none."""
+    import torch
+    import large_model_b200 as m
+    l = torch.full((2, 151936), -float("inf"), device="cuda")
+    l[0, 77:80] = torch.tensor([-20000.0, -20001.0, -20000.0])
+    l[1, 151935] = 3e38
+    p = m.probs(l, 1.0)
+    want = torch.softmax(l.double(), -1)
+    assert ((p.double() - want).abs() <= 2.0 ** -19 * want).all() and torch.isfinite(p).all()
+
+
 def test_probs_small_and_large_temperatures(cuda):
     import torch
     import large_model_b200 as m
