@@ -47,6 +47,64 @@ __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int 
     return page * a.page_stride + (p & ((1 << a.page_log) - 1)) * a.pos_stride;
 }
 
+// ---- pieces of the attention kernels ----
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 bytes global -> shared, or 16 zero bytes.
+__device__ __forceinline__ void cp_async16_or0(uint32_t dst, const void *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// (x, y) = hi + lo in fp16 pairs
+__device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    hi = pack_h2(x, y);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    lo = pack_h2(x - h.x, y - h.y);
+}
+// Zero what is not finite in a 16-byte piece of V; true if something was.
+__device__ __forceinline__ bool drop_nonfinite(const __half *, uint4 &v) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if ((w[i] & 0x7C00u) == 0x7C00u) {
+            w[i] &= 0xFFFF0000u;
+            any = true;
+        }
+        if ((w[i] & 0x7C000000u) == 0x7C000000u) {
+            w[i] &= 0x0000FFFFu;
+            any = true;
+        }
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+__device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if ((w[i] & 0x7F800000u) == 0x7F800000u) {
+            w[i] = 0;
+            any = true;
+        }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+
 // ---- attention: the work and its split ----------------------------------------------------------
 // Two kinds of units, per kv head: the shared positions [0, prefix) against tiles of all token rows, and
 // a sequence's own positions [prefix, kv_len) against tiles of its rows. A row is a (token, q head of the
@@ -55,7 +113,7 @@ __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int 
 // slots: part_o [slots][n_tok * H][D] (not divided by l), part_ml [slots][n_tok * H] of (m, l),
 // m the base-2 exponent of the weights' common factor.
 struct PagedPlan {
-    int wr_p, wr_s;                  // row groups of 16 per tile: shared, own
+    int wr_p, wr_s;                  // row groups of 16 per tile: shared, own; 0: the wide kernel's 256 rows
     int chunk_p, chunk_s;            // positions per chunk
     int slots_p, slots_s;            // chunks of each kind
     int tiles_p, tiles_s;            // row tiles of each kind
@@ -74,6 +132,7 @@ struct PagedAttn {
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p);
 int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p);
+int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s);     // qms_paged_wide.cu
 int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, const float *q, int64_t ldq, float scale,
                            float *out, int64_t ldo, void *ws, cudaStream_t s);
 

@@ -20,22 +20,6 @@ namespace qms {
 constexpr int kPaStage = 64;          // positions per stage
 constexpr float kPaShift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// 16 bytes global -> shared, or 16 zero bytes.
-__device__ __forceinline__ void cp_async16_or0(uint32_t dst, const void *src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -64,49 +48,8 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], flo
                  : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
                    "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
-__device__ __forceinline__ uint32_t pack_h2(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// (x, y) = hi + lo in fp16 pairs
-__device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    hi = pack_h2(x, y);
-    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    lo = pack_h2(x - h.x, y - h.y);
-}
 // x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-
-// Zero what is not finite in a 16-byte piece of V; true if something was.
-__device__ __forceinline__ bool drop_nonfinite(const __half *, uint4 &v) {
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if ((w[i] & 0x7C00u) == 0x7C00u) {
-            w[i] &= 0xFFFF0000u;
-            any = true;
-        }
-        if ((w[i] & 0x7C000000u) == 0x7C000000u) {
-            w[i] &= 0x0000FFFFu;
-            any = true;
-        }
-    }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-    return any;
-}
-__device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if ((w[i] & 0x7F800000u) == 0x7F800000u) {
-            w[i] = 0;
-            any = true;
-        }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-    return any;
-}
 
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
 // A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows times WK = 4 / WR
@@ -204,7 +147,8 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             hi_pos = max(hi_pos, p);
         }
         k1 = min(k1, hi_pos + 1);                 // nobody sees the rest
-        const int nst = k1 > k0 ? (k1 - k0 + kPaStage - 1) / kPaStage : 0;
+        if (k0 >= k1) continue;
+        const int nst = (k1 - k0 + kPaStage - 1) / kPaStage;
 
         auto load = [&](int st) {                 // stage st of the unit into its slot
             const int slot_i = st % C::NS, base = k0 + st * kPaStage;
@@ -557,8 +501,9 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
 #pragma unroll
     for (int j = 0; j < J; j++) x[j] = 0.0f;
     float l = 0.0f;
-    if (t >= t0 && t < t0 + n) {
-        const int ns = A.p.slots_p + (kv > a.prefix ? (kv - a.prefix + A.p.chunk_s - 1) / A.p.chunk_s : 0);
+    const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
+    if (pos >= 0) {                               // the slots of chunks that begin past the row's position are not written
+        const int ns = pos < a.prefix ? pos / A.p.chunk_p + 1 : A.p.slots_p + (pos - a.prefix) / A.p.chunk_s + 1;
         float M = -INFINITY;
         for (int s = lane; s < ns; s += 32) M = fmaxf(M, __ldcg(&A.part_ml[s * rows + row]).x);
         M = warp_max(M);
@@ -588,22 +533,44 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Row groups per tile: a tile as tall as the rows there are, up to 64 (more rows per K / V read).
-static int row_groups(int64_t rows) { return rows > 32 ? 4 : rows > 16 ? 2 : 1; }
+// Row groups of 16 per tile of the mma.sync kernel: as tall as the rows there are, up to 64 (more rows per K / V
+// read); 0 = the tcgen05 kernel, for an fp16 cache and more rows than that.
+static int row_groups(int type, int64_t rows) {
+    if (type == QMS_T_F16 && rows > 64) return 0;
+    return rows > 32 ? 4 : rows > 16 ? 2 : 1;
+}
+
+// Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
+// of resident CTAs, stages of `stage` positions (us each, us_unit once per unit) and 1 KB of partial results
+// written and read back per row and chunk.
+static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int resident, double us_stage, double us_unit) {
+    const int st = (len + stage - 1) / stage;
+    int best = st;
+    double least = 1e30;
+    for (int per = st; per >= 1; per = per > 64 ? per - per / 16 : per - 1) {
+        const int n = (st + per - 1) / per;
+        const int64_t waves = (tiles * n + resident - 1) / resident;
+        const double us = (double)waves * (per * us_stage + us_unit) + (double)rows * n * 2.0e-4;
+        if (us < least) least = us, best = per;
+    }
+    return (best > 0 ? best : 1) * stage;
+}
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
-    const int resident = 148 * (type == QMS_T_F16 ? 2 : 1);
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G;
     const int own = std::max(0, a.max_kv - a.prefix);
-    p.wr_p = row_groups(rows_p);
-    p.wr_s = row_groups(rows_s);
-    p.tiles_p = (int)((rows_p + 16 * p.wr_p - 1) / (16 * p.wr_p));
-    p.tiles_s = (int)((rows_s + 16 * p.wr_s - 1) / (16 * p.wr_s));
-    // chunks: about two units per resident CTA
-    const int64_t st_p = (a.prefix + kPaStage - 1) / kPaStage, st_s = (own + kPaStage - 1) / kPaStage;
-    const int64_t work = (st_p * p.tiles_p + st_s * p.tiles_s * a.n_seq) * a.Hk;
-    const int64_t per = std::max<int64_t>(1, work / (2 * resident));
-    p.chunk_p = p.chunk_s = (int)(per * kPaStage);
+    p.wr_p = row_groups(type, rows_p);
+    p.wr_s = row_groups(type, rows_s);
+    const int mp = p.wr_p ? 16 * p.wr_p : 256, ms = p.wr_s ? 16 * p.wr_s : 256;
+    p.tiles_p = (int)((rows_p + mp - 1) / mp);
+    p.tiles_s = (int)((rows_s + ms - 1) / ms);
+    const int64_t all = (int64_t)a.n_tok * a.H;
+    const double slow = type == QMS_T_F16 ? 1.0 : 2.0;
+    const int res = 148 * (type == QMS_T_F16 ? 2 : 1);
+    p.chunk_p = p.wr_p ? chunk_of(a.prefix, (int64_t)p.tiles_p * a.Hk, all, kPaStage, res, slow * 0.4, 2.0)
+                       : chunk_of(a.prefix, (int64_t)p.tiles_p * a.Hk, all, 128, 148, 2.4, 5.0);
+    p.chunk_s = p.wr_s ? chunk_of(own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all, kPaStage, res, slow * 0.4, 2.0)
+                       : chunk_of(own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all, 128, 148, 2.4, 5.0);
     p.slots_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
     p.slots_s = (own + p.chunk_s - 1) / p.chunk_s;
 }
@@ -639,7 +606,8 @@ static int launch_attn(const PagedAttn &A, cudaStream_t s) {
         const bool own = kind == 1;
         if (own ? !(A.p.slots_s && A.p.tiles_s && A.a.n_seq) : !(A.p.slots_p && A.p.tiles_p)) continue;
         const int wr = own ? A.p.wr_s : A.p.wr_p;
-        const int rc = wr == 4   ? launch_attn_wr<D, KT, 4>(A, own, before, s)
+        const int rc = wr == 0   ? launch_paged_wide(A, D, own, before, s)
+                       : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
                        : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
                                  : launch_attn_wr<D, KT, 1>(A, own, before, s);
         if (rc) return rc;
