@@ -74,6 +74,9 @@ __device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_
     const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     lo = pack_h2(x - h.x, y - h.y);
 }
+// x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
+__device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
 // Zero what is not finite in a 16-byte piece of V; true if something was.
 __device__ __forceinline__ bool drop_nonfinite(const __half *, uint4 &v) {
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -113,11 +116,19 @@ __device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
 // slots: part_o [slots][n_tok * H][D] (not divided by l), part_ml [slots][n_tok * H] of (m, l),
 // m the base-2 exponent of the weights' common factor.
 struct PagedPlan {
-    int wr_p, wr_s;                  // row groups of 16 per tile: shared, own; 0: the wide kernel's 256 rows
+    int wr_p, wr_s;                  // shared, own: row groups of 16 per tile (k_paged_attn), or kPaWide...
     int chunk_p, chunk_s;            // positions per chunk
-    int slots_p, slots_s;            // chunks of each kind
+    int base_s;                      // where the own positions' chunks start: prefix, or the tile boundary before it
+    int chunks_p, chunks_s;          // chunks of each kind
+    int slots_p, slots_s;            // slots of each kind
     int tiles_p, tiles_s;            // row tiles of each kind
+    int64_t line;                    // k_paged_wide's runs over the shared positions: their total length, or 0
+    int line_ctas;                   // CTAs that share it
 };
+constexpr int kPaWidePair = 0, kPaWideSplit = -1;    // k_paged_wide: two tiles of 128 rows; one, in two streams
+
+// Which of n CTAs holds place x of a line cut into n runs [line i / n, line (i + 1) / n).
+__host__ __device__ inline int line_cta(int64_t x, int64_t line, int n) { return (int)(((x + 1) * n - 1) / line); }
 
 struct PagedAttn {
     Paged a;

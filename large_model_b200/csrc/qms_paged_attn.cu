@@ -48,9 +48,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], flo
                  : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
                    "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
-// x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
-__device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
 // A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows times WK = 4 / WR
 // groups of positions. K and V arrive in stages of 64 positions by cp.async (zeros where a position is
@@ -88,7 +85,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
     // the trigger comes after the wait: a kernel that starts on it may read what this one waited for
     if (!last) pdl_wait();
     pdl_trigger();
-    const int n_unit = (own ? A.p.slots_s * a.n_seq * A.p.tiles_s : A.p.slots_p * A.p.tiles_p) * a.Hk;
+    const int n_unit = (own ? A.p.chunks_s * a.n_seq * A.p.tiles_s : A.p.chunks_p * A.p.tiles_p) * a.Hk;
     for (int unit = blockIdx.x; unit < n_unit; unit += gridDim.x) {
         // ---- which rows, which positions
         int u = unit;
@@ -503,20 +500,37 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
     float l = 0.0f;
     const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
     if (pos >= 0) {                               // the slots of chunks that begin past the row's position are not written
-        const int ns = pos < a.prefix ? pos / A.p.chunk_p + 1 : A.p.slots_p + (pos - a.prefix) / A.p.chunk_s + 1;
+        // slots of a kind up to place d of it: one per chunk, or two where k_paged_wide has two streams
+        auto upto = [](int d, int chunk, int wr) {
+            const int c = d / chunk;
+            return wr == kPaWideSplit ? 2 * c + (d - c * chunk >= 128 ? 2 : 1) : c + 1;
+        };
+        int np = 0;
+        if (a.prefix > 0) {
+            const int d = min(pos, a.prefix - 1);
+            if (A.p.line > 0) {
+                const int h = (int)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
+                const int64_t u = (int64_t)((t * a.G + h - kh * a.G) / 256) * a.Hk + kh;
+                np = line_cta(u * nt + d / 128, A.p.line, A.p.line_ctas) - line_cta(u * nt, A.p.line, A.p.line_ctas) + 1;
+            } else {
+                np = upto(d, A.p.chunk_p, A.p.wr_p);
+            }
+        }
+        const int ns = np + (pos < a.prefix ? 0 : upto(pos - A.p.base_s, A.p.chunk_s, A.p.wr_s));
+        auto at = [&](int s) { return (s < np ? s : s - np + A.p.slots_p) * rows + row; };
         float M = -INFINITY;
-        for (int s = lane; s < ns; s += 32) M = fmaxf(M, __ldcg(&A.part_ml[s * rows + row]).x);
+        for (int s = lane; s < ns; s += 32) M = fmaxf(M, __ldcg(&A.part_ml[at(s)]).x);
         M = warp_max(M);
         if (M != -INFINITY) {
             for (int s0 = 0; s0 < ns; s0 += 32) {
-                const float2 ml = s0 + lane < ns ? __ldcg(&A.part_ml[(s0 + lane) * rows + row]) : make_float2(-INFINITY, 0.0f);
+                const float2 ml = s0 + lane < ns ? __ldcg(&A.part_ml[at(s0 + lane)]) : make_float2(-INFINITY, 0.0f);
                 const float w = ex2(ml.x - M);
                 l += warp_sum(w * ml.y);
                 const int ne = min(32, ns - s0);
 #pragma unroll 8
                 for (int i = 0; i < ne; i++) {
                     const float wi = __shfl_sync(kFull, w, i);
-                    const float *src = A.part_o + ((s0 + i) * rows + row) * D + lane * J;
+                    const float *src = A.part_o + at(s0 + i) * D + lane * J;
                     float v[J];
                     if constexpr (J == 4) *reinterpret_cast<float4 *>(v) = __ldcg(reinterpret_cast<const float4 *>(src));
                     else *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(src));
@@ -533,10 +547,10 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Row groups of 16 per tile of the mma.sync kernel: as tall as the rows there are, up to 64 (more rows per K / V
-// read); 0 = the tcgen05 kernel, for an fp16 cache and more rows than that.
-static int row_groups(int type, int64_t rows) {
-    if (type == QMS_T_F16 && rows > 64) return 0;
+// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); an fp16 cache
+// in pages of 8 positions or more (a swizzle unit of k_paged_wide's tiles) and more rows than that: k_paged_wide.
+static int row_groups(int type, int page_log, int64_t rows) {
+    if (type == QMS_T_F16 && rows > 64 && page_log >= 3) return rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
 }
 
@@ -556,23 +570,37 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
     return (best > 0 ? best : 1) * stage;
 }
 
-void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
-    const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G;
-    const int own = std::max(0, a.max_kv - a.prefix);
-    p.wr_p = row_groups(type, rows_p);
-    p.wr_s = row_groups(type, rows_s);
-    const int mp = p.wr_p ? 16 * p.wr_p : 256, ms = p.wr_s ? 16 * p.wr_s : 256;
-    p.tiles_p = (int)((rows_p + mp - 1) / mp);
-    p.tiles_s = (int)((rows_s + ms - 1) / ms);
-    const int64_t all = (int64_t)a.n_tok * a.H;
+static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
+    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, 128, 148, 3.0, 6.0);
+    if (wr == kPaWideSplit) return chunk_of(len, tiles, 2 * rows, 256, 148, 3.0, 6.0);
     const double slow = type == QMS_T_F16 ? 1.0 : 2.0;
-    const int res = 148 * (type == QMS_T_F16 ? 2 : 1);
-    p.chunk_p = p.wr_p ? chunk_of(a.prefix, (int64_t)p.tiles_p * a.Hk, all, kPaStage, res, slow * 0.4, 2.0)
-                       : chunk_of(a.prefix, (int64_t)p.tiles_p * a.Hk, all, 128, 148, 2.4, 5.0);
-    p.chunk_s = p.wr_s ? chunk_of(own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all, kPaStage, res, slow * 0.4, 2.0)
-                       : chunk_of(own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all, 128, 148, 2.4, 5.0);
-    p.slots_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
-    p.slots_s = (own + p.chunk_s - 1) / p.chunk_s;
+    return chunk_of(len, tiles, rows, kPaStage, 148 * (type == QMS_T_F16 ? 2 : 1), slow * 0.7, 4.0);
+}
+
+void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
+    const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
+    p.wr_p = row_groups(type, a.page_log, rows_p);
+    p.wr_s = row_groups(type, a.page_log, rows_s);
+    p.base_s = p.wr_s <= 0 ? a.prefix & ~(std::min(1 << a.page_log, 128) - 1) : a.prefix;
+    const int own = std::max(0, a.max_kv - p.base_s);
+    auto height = [](int wr) { return wr == kPaWidePair ? 256 : wr == kPaWideSplit ? 128 : 16 * wr; };
+    p.tiles_p = (int)((rows_p + height(p.wr_p) - 1) / height(p.wr_p));
+    p.tiles_s = (int)((rows_s + height(p.wr_s) - 1) / height(p.wr_s));
+    p.chunk_p = chunk_for(type, p.wr_p, a.prefix, (int64_t)p.tiles_p * a.Hk, all);
+    p.chunk_s = chunk_for(type, p.wr_s, own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all);
+    p.chunks_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
+    p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
+    p.slots_p = p.chunks_p * (p.wr_p == kPaWideSplit ? 2 : 1);
+    p.slots_s = p.chunks_s * (p.wr_s == kPaWideSplit ? 2 : 1);
+    p.line = 0;
+    p.line_ctas = 0;
+    if (p.wr_p == kPaWidePair && a.prefix > 0 && rows_p > 0) {
+        const int64_t nt = (a.prefix + 127) / 128;
+        p.line = nt * p.tiles_p * a.Hk;
+        p.line_ctas = (int)std::min<int64_t>(148, p.line);
+        // a row tile's positions meet at most this many runs
+        p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / (p.line / p.line_ctas) + 2);
+    }
 }
 
 static int64_t al256(int64_t x) { return (x + 255) & ~(int64_t)255; }
@@ -585,7 +613,7 @@ int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
 template <int D, typename KT, int WR>
 static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
     using C = PaCfg<D, KT, WR>;
-    const int64_t units = own ? (int64_t)A.p.slots_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.slots_p * A.p.tiles_p * A.a.Hk;
+    const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.chunks_p * A.p.tiles_p * A.a.Hk;
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     static unsigned long long set = 0;                          // per device
     int dev = 0;
@@ -604,9 +632,9 @@ static int launch_attn(const PagedAttn &A, cudaStream_t s) {
     bool before = false;
     for (int kind = 0; kind < 2; kind++) {
         const bool own = kind == 1;
-        if (own ? !(A.p.slots_s && A.p.tiles_s && A.a.n_seq) : !(A.p.slots_p && A.p.tiles_p)) continue;
+        if (own ? !(A.p.chunks_s && A.p.tiles_s && A.a.n_seq) : !(A.p.chunks_p && A.p.tiles_p)) continue;
         const int wr = own ? A.p.wr_s : A.p.wr_p;
-        const int rc = wr == 0   ? launch_paged_wide(A, D, own, before, s)
+        const int rc = wr <= 0   ? launch_paged_wide(A, D, own, before, s)
                        : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
                        : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
                                  : launch_attn_wr<D, KT, 1>(A, own, before, s);

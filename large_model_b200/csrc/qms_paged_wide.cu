@@ -1,7 +1,10 @@
 // qms_paged_wide.cu - paged attention where one K / V tile meets many rows (a shared prompt against a batch, drafted
 // tokens, a chunk of a prompt): tcgen05 tensor cores, fp16 cache, on B200 (sm_100a).
 //
-// A unit is 256 rows (two tiles of 128) of one kv head against a chunk of positions, 128 at a time:
+// A unit is a run of positions, 128 at a time, of one kv head against 256 rows (two tiles of 128: PAIR) or, where there
+// are no more than 128 rows, against one tile whose even and odd position tiles are two streams with an O and
+// a softmax of their own (SPLIT): either way the tensor cores have one stream to work on while the other's
+// softmax runs.
 //   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128 x N 128, K = head_dim, twice: Q = hi + lo
 //               in fp16 (22 bits, each row scaled by a power of two into fp16's range), K exact
 //   softmax     one thread per row reads its S from TMEM, keeps the running base B and sum l, writes the
@@ -11,11 +14,14 @@
 // since its base was set, which a base 2^8 below the first maximum and fp16's range of 2^16 allow; the
 // result does not depend on it beyond rounding.
 //
-// Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 bring K and V in by cp.async (any page size,
-// layout and length; positions past the chunk or on bad pages are zeros), one thread of warp 12 issues the
-// MMAs: while it works on one row tile, the other's softmax runs. Shared memory: Q 128 KB, a ring of 3
-// tiles of 32 KB; TMEM: S 2 x 128, O 2 x 128 columns (head_dim 128).
+// Warps 0-3 and 4-7 are the softmax of the two streams, warp 8 brings K and V in by TMA (a box of 64 values x up to 128
+// positions per page, swizzled), warps 9 and 10 clear values that are not finite out of V rows that some row
+// does not see (a weight of 0 does not cancel them), one thread of warp 11 issues the MMAs. Tiles start on a
+// page boundary (or, in larger pages, a multiple of 128), so a tile may begin before the first position of its
+// unit; such rows are masked. Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB, or (SPLIT) Q 64 KB and 5
+// tiles; TMEM: S 2 x 128, O 2 x 128 columns.
 // Bound by the tensor cores: 4 * 128 * 128 * head_dim flop per tile and product pair, twice for the split.
+#include <cuda.h>
 #include <math.h>
 #include <string.h>
 
@@ -25,19 +31,19 @@
 
 namespace qms {
 
-constexpr int kWTile = 128, kWThreads = 416;
+constexpr int kWTile = 128, kWThreads = 384;         // 12 warps: 168 registers each
 constexpr uint32_t kWSpin = 1u << 22;
 constexpr float kWLow = 8.0f, kWHigh = 15.0f;       // a new base is 2^8 below the maximum; weights stay below 2^15
 
-template <int D>
+template <int D, bool SPLIT>
 struct WideCfg {
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t HALF = kWTile * 128;              // bytes of 128 rows x 64 values
     static constexpr uint32_t TILE = HALVES * HALF;             // a K or V tile; one term of a Q tile
-    static constexpr int SLOTS = 3, CH = D / 8;                 // CH: 16-byte pieces per row
-    static constexpr uint32_t RING = 4 * TILE, META = RING + SLOTS * TILE;
-    // meta: page offsets [2][128] int64, bad-page masks [4][4], barriers, flags
-    static constexpr uint32_t BAD = META + 2 * kWTile * 8, BARS = BAD + 64, SMEM = BARS + 16 * 8 + 64;
+    static constexpr int SLOTS = SPLIT ? 5 : 3, CH = D / 8;     // CH: 16-byte pieces per row
+    static constexpr uint32_t RING = (SPLIT ? 2 : 4) * TILE, META = RING + SLOTS * TILE;
+    // meta: bad-page masks [8][4], barriers, flags
+    static constexpr uint32_t BAD = META, BARS = BAD + 128, SMEM = BARS + (3 * SLOTS + 8) * 8 + 16;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
 };
 
@@ -80,6 +86,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A box of a paged pool: 64 values from x of one head, the positions of the map's box from y of a page.
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int head, int y, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(head), "r"(y), "r"(page), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_tie(uint32_t (&r)[32]) {      // the same for a second array of that wait
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Bounded wait for a phase of a barrier; a wait that gives up ends the CTA's work (flag) and is reported.
 struct WideSync {
     volatile int *abort;
@@ -98,55 +122,89 @@ struct WideSync {
     }
 };
 
-// One unit of work; every role derives it from the unit's number.
+// One unit of work, as every role derives it.
 struct WideUnit {
-    bool any;                        // there is something to do
-    int kh, b, t0, n, kv, slot, k0, k1, r0, rows, nt, tiles, lo;
+    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, tiles, lo;
     // kv head; sequence, its first row, rows and length (own); slot of the partial result; positions [k0, k1) in
-    // nt tiles; first row and number of rows of the segment; row tiles (1 or 2); every row of the unit sees
-    // the positions up to lo
-    __device__ WideUnit(const PagedAttn &A, bool own, int lo_p, int u) {
-        const Paged &a = A.a;
-        kh = u % a.Hk;
-        u /= a.Hk;
-        const int nt_rows = own ? A.p.tiles_s : A.p.tiles_p, tile = u % nt_rows;
-        u /= nt_rows;
-        r0 = tile * 2 * kWTile;
-        b = t0 = n = kv = 0;
-        if (own) {
-            b = u % a.n_seq;
-            slot = u / a.n_seq;
-            paged_seq(a, b, t0, n, kv);
-            rows = n * a.G;
-            k0 = a.prefix + slot * A.p.chunk_s;
-            k1 = min(kv, k0 + A.p.chunk_s);
-            lo = kv - n + r0 / a.G;
-            k1 = min(k1, kv - n + min(n - 1, (r0 + 2 * kWTile - 1) / a.G) + 1);     // nobody sees the rest
-            slot += A.p.slots_p;
+    // nt tiles, of which those below kmin belong to another unit; first row and number of rows of the
+    // segment; row tiles (1 or 2); every row of the unit sees the positions up to lo
+};
+
+// The units of this CTA in order. Own positions: units blockIdx.x, + gridDim.x, ... of (chunk, sequence, row tile, kv
+// head). Shared positions against pairs of row tiles: all (row tile, kv head, position tile) triples in one line, cut
+// into equal runs, one per CTA; a run is one unit per row tile and kv head that it crosses.
+struct WideWork {
+    const PagedAttn &A;
+    const bool own, line;
+    const int lo_p;
+    int64_t x, end;
+    __device__ WideWork(const PagedAttn &A_, bool own_, int lo_p_) : A(A_), own(own_), line(!own_ && A_.p.line > 0), lo_p(lo_p_) {
+        if (line) {
+            x = A.p.line * blockIdx.x / gridDim.x;
+            end = A.p.line * (blockIdx.x + 1) / gridDim.x;
         } else {
-            slot = u;
-            rows = a.n_tok * a.G;
-            k0 = slot * A.p.chunk_p;
-            k1 = min(a.prefix, k0 + A.p.chunk_p);
-            lo = lo_p;
+            x = blockIdx.x;
+            end = (int64_t)(own ? A.p.chunks_s * A.a.n_seq * A.p.tiles_s : A.p.chunks_p * A.p.tiles_p) * A.a.Hk;
         }
-        any = r0 < rows && k0 < k1;
-        nt = (k1 - k0 + kWTile - 1) / kWTile;
-        tiles = rows - r0 > kWTile ? 2 : 1;
+    }
+    __device__ bool next(WideUnit &w) {
+        const Paged &a = A.a;
+        const int rows_tile = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit ? kWTile : 2 * kWTile;
+        for (; x < end;) {
+            w.b = w.t0 = w.n = w.kv = 0;
+            if (line) {
+                const int nt = (a.prefix + kWTile - 1) / kWTile;
+                const int64_t u = x / nt;
+                const int j = (int)(x - u * nt), c = (int)min((int64_t)(nt - j), end - x);
+                w.kh = (int)(u % a.Hk);
+                w.r0 = (int)(u / a.Hk) * rows_tile;
+                w.slot = blockIdx.x - line_cta(u * nt, A.p.line, gridDim.x);
+                w.k0 = w.kmin = j * kWTile;
+                w.k1 = min(a.prefix, (j + c) * kWTile);
+                x += c;
+            } else {
+                int u = (int)x;
+                x += gridDim.x;
+                w.kh = u % a.Hk;
+                u /= a.Hk;
+                const int nr = own ? A.p.tiles_s : A.p.tiles_p;
+                w.r0 = u % nr * rows_tile;
+                u /= nr;
+                if (own) {
+                    w.b = u % a.n_seq;
+                    u /= a.n_seq;
+                    paged_seq(a, w.b, w.t0, w.n, w.kv);
+                    w.k0 = A.p.base_s + u * A.p.chunk_s;
+                    w.kmin = max(w.k0, a.prefix);
+                    w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
+                    w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (w.r0 + rows_tile - 1) / a.G) + 1);     // nobody sees the rest
+                } else {
+                    w.k0 = w.kmin = u * A.p.chunk_p;
+                    w.k1 = min(a.prefix, w.k0 + A.p.chunk_p);
+                }
+                w.slot = (own ? A.p.slots_p : 0) + u * (rows_tile == kWTile ? 2 : 1);
+            }
+            w.rows = own ? w.n * a.G : a.n_tok * a.G;
+            w.lo = own ? w.kv - w.n + w.r0 / a.G : lo_p;
+            w.nt = (w.k1 - w.k0 + kWTile - 1) / kWTile;
+            w.tiles = w.rows - w.r0 > kWTile ? 2 : 1;
+            if (w.r0 < w.rows && w.kmin < w.k1) return true;
+        }
+        return false;
     }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, const bool own, const bool last) {
-    using C = WideCfg<D>;
+template <int D, bool SPLIT>
+__global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                                             const bool own, const bool last) {
+    using C = WideCfg<D, SPLIT>;
     extern __shared__ __align__(1024) unsigned char sm[];
     const Paged &a = A.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sm0 = smem_u32(sm);
-    int64_t *s_off = reinterpret_cast<int64_t *>(sm + C::META);
     uint32_t *s_bad = reinterpret_cast<uint32_t *>(sm + C::BAD);
-    uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + C::SLOTS;
-    uint64_t *q_full = empty + C::SLOTS, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + C::SLOTS, *landed = empty + C::SLOTS;
+    uint64_t *staged = landed + C::SLOTS, *q_full = staged + 1, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
     int *s_int = reinterpret_cast<int *>(drain + 1);              // abort, V set aside, TMEM base, least position
     volatile int *s_abort = s_int, *s_flag = s_int + 1;
     int *s_lo = s_int + 3;
@@ -158,8 +216,9 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
     }
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
-            mbar_init(&full[i], 128);
+            mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
+            mbar_init(&landed[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 128);
@@ -167,11 +226,12 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
             mbar_init(&p_full[i], 4);
         }
         mbar_init(drain, 1);
+        mbar_init(staged, 4);
         s_int[0] = s_int[1] = 0;
         *s_lo = 0x7fffffff;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -192,119 +252,127 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
         __syncthreads();
     }
     const int lo_p = *s_lo;
-    const int n_unit = (own ? A.p.slots_s * a.n_seq * A.p.tiles_s : A.p.slots_p * A.p.tiles_p) * a.Hk;
     const WideSync sy{s_abort, &a};
+    WideWork work(A, own, lo_p);
+    WideUnit w;
 
     if (warp < 8) {
-        // ---- softmax of row tile i: thread = row = TMEM lane
+        // ---- softmax of stream i: thread = row = TMEM lane
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_col = lanes + i * kWTile, o_col = lanes + C::O_COL + i * D;
-        uint32_t ns = 0, tiles_done = 0;          // phases of s_full; tiles seen by the CTA (for s_bad)
+        uint32_t ns = 0, before = 0, units = 0;   // phases of s_full; position tiles of the CTA's earlier units (for s_bad)
         bool ok = true;
-        for (int u = blockIdx.x; u < n_unit && ok; u += gridDim.x) {
-            const WideUnit w(A, own, lo_p, u);
-            if (!w.any) continue;
-            if (i >= w.tiles) {
-                tiles_done += w.nt;
-                continue;
+        for (; ok && work.next(w); before += w.nt) {
+            if (!SPLIT && i >= w.tiles) continue;
+            const int r = w.r0 + (SPLIT ? 0 : i * kWTile) + row, t = r / a.G;    // this row: its token, position below
+            int tok = -1;                                                        // token row * H + head (-1: none)
+            if (r < w.rows) tok = (w.t0 + t) * a.H + w.kh * a.G + (r - t * a.G);
+            // q: 8 lanes per row, 4 rows at a time: row maximum, power-of-two scale, two fp16 terms, swizzled
+            // rows (SPLIT: one stream writes them for both, the other one only wants the scales)
+            float f = 0.0f;
+            const float sign = A.scale2 < 0.0f ? -1.0f : 1.0f;     // f >= 0: the largest s f has the largest s
+            const uint32_t qb = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
+            if (SPLIT && i == 0 && units++ > 0 && !(ok = __all_sync(kFull, sy.wait(staged, units & 1)))) break;
+#pragma unroll 1
+            for (int g0 = 0; g0 < 8; g0 += 4) {
+                float4 x[4][D / 32];              // 16 rows of the warp in flight
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int tk = __shfl_sync(kFull, tok, 4 * (g0 + g) + (lane >> 3));
+                    const float *src = A.q + (tk < 0 ? 0 : (tk / a.H) * A.ldq + (int64_t)(tk % a.H) * D) + (lane & 7) * 4;
+#pragma unroll
+                    for (int k = 0; k < D / 32; k++)
+                        x[g][k] = tk < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(reinterpret_cast<const float4 *>(src + k * 32));
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float mx = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < D / 32; k++)
+                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[g][k].x), fabsf(x[g][k].y)), fmaxf(fabsf(x[g][k].z), fabsf(x[g][k].w))));
+                    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
+                    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+                    const int e = mx > 0.0f && mx < INFINITY ? ilogbf(mx) - 9 : 0;
+                    const float got = __shfl_sync(kFull, ldexpf(fabsf(A.scale2), e), (lane & 3) * 8);
+                    if (lane >> 2 == g0 + g) f = got;
+                    if (SPLIT && i == 1) continue;
+                    const float d1 = ldexpf(sign, -e / 2), d2 = ldexpf(1.0f, -e - -e / 2);
+                    const int rr = (warp & 3) * 32 + 4 * (g0 + g) + (lane >> 3);
+#pragma unroll
+                    for (int k = 0; k < D / 32; k++) {
+                        uint32_t h[2], l[2];
+                        split_h2(x[g][k].x * d1 * d2, x[g][k].y * d1 * d2, h[0], l[0]);
+                        split_h2(x[g][k].z * d1 * d2, x[g][k].w * d1 * d2, h[1], l[1]);
+                        const int d = (lane & 7) * 4 + k * 32;
+                        const uint32_t at = qb + (d >> 6) * C::HALF + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(h[0]), "r"(h[1]) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + C::TILE), "r"(l[0]), "r"(l[1]) : "memory");
+                    }
+                }
             }
-            // this row: position, token row * H + head (-1: none)
-            const int r = w.r0 + i * kWTile + row;
-            int pos = -1, tok = -1;
+            fence_async_smem();
+            if (!SPLIT || i == 0) mbar_arrive(&q_full[i]);
+            int pos = -1;
             if (own) {
-                const int t = r / a.G;
-                if (r < w.rows) pos = w.kv - w.n + t, tok = (w.t0 + t) * a.H + w.kh * a.G + (r - t * a.G);
+                if (r < w.rows) pos = w.kv - w.n + t;
             } else {
-                const int t = r / a.G, t_end = min(a.n_tok - 1, __shfl_sync(kFull, t, 31));
+                const int t_end = min(a.n_tok - 1, __shfl_sync(kFull, t, 31));
                 for (int x = __shfl_sync(kFull, t, 0); x <= t_end; x++) {
                     int s0 = 0, sn = 0, skv = 0;
                     const int sb = paged_seq_of(a, x);
                     if (sb < a.n_seq) paged_seq(a, sb, s0, sn, skv);
-                    if (t == x && r < w.rows) {
-                        pos = x >= s0 && x < s0 + sn ? skv - sn + (x - s0) : -1;
-                        tok = x * a.H + w.kh * a.G + (r - x * a.G);
-                    }
+                    if (t == x && r < w.rows && x >= s0 && x < s0 + sn) pos = skv - sn + (x - s0);
                 }
             }
-            // q: 8 lanes per row, 4 rows at a time: row maximum, power-of-two scale, two fp16 terms, swizzled rows
-            float f = 0.0f;
-            const float sign = A.scale2 < 0.0f ? -1.0f : 1.0f;     // f >= 0: the largest s f has the largest s
-            const uint32_t qb = sm0 + i * 2 * C::TILE;
-#pragma unroll 2
-            for (int g = 0; g < 8; g++) {
-                const int src = 4 * g + (lane >> 3), part = lane & 7;
-                const int tk = __shfl_sync(kFull, tok, src);
-                float4 x[D / 32];
-                float mx = 0.0f;
-#pragma unroll
-                for (int k = 0; k < D / 32; k++) {
-                    x[k] = tk < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                  : __ldcg(reinterpret_cast<const float4 *>(A.q + (tk / a.H) * A.ldq + (int64_t)(tk % a.H) * D + part * 4 + k * 32));
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
-                }
-                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-                mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-                const int e = mx > 0.0f && mx < INFINITY ? ilogbf(mx) - 9 : 0;
-                const float fr = ldexpf(fabsf(A.scale2), e), got = __shfl_sync(kFull, fr, (lane & 3) * 8);
-                if (lane >> 2 == g) f = got;
-                const float d1 = ldexpf(sign, -e / 2), d2 = ldexpf(1.0f, -e - -e / 2);
-                const int rr = (warp & 3) * 32 + src;
-#pragma unroll
-                for (int k = 0; k < D / 32; k++) {
-                    const float y[4] = {x[k].x * d1 * d2, x[k].y * d1 * d2, x[k].z * d1 * d2, x[k].w * d1 * d2};
-                    uint32_t h[2], l[2];
-                    split_h2(y[0], y[1], h[0], l[0]);
-                    split_h2(y[2], y[3], h[1], l[1]);
-                    const int d = part * 4 + k * 32;
-                    const uint32_t at = qb + (d >> 6) * C::HALF + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(h[0]), "r"(h[1]) : "memory");
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + C::TILE), "r"(l[0]), "r"(l[1]) : "memory");
-                }
-            }
-            fence_async_smem();
-            mbar_arrive(&q_full[i]);
 
             const int lim = min(pos, w.k1 - 1);   // last position that this row sees
-            float B = -INFINITY, l = 0.0f;
-            for (int j = 0; j < w.nt; j++, tiles_done++) {
+            float B = -INFINITY;
+            float2 l2 = make_float2(0.0f, 0.0f);
+            for (int j = SPLIT ? i : 0; j < w.nt; j += SPLIT ? 2 : 1) {
                 if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;    // the whole warp or none of it
                 ns++;
                 tc_fence_after();
                 const int base = w.k0 + j * kWTile;
-                const uint32_t *bad = s_bad + (tiles_done & 3) * 4;
-                const uint32_t bads[4] = {bad[0], bad[1], bad[2], bad[3]};
-                // rows that see nothing of this chunk are not read from its slot: no mask for them
-                const bool mask = __any_sync(kFull, lim >= w.k0 && lim < base + kWTile - 1) || (bads[0] | bads[1] | bads[2] | bads[3]);
-                uint32_t vis[4];
+                const uint32_t *bad = s_bad + ((before + j) & 7) * 4;
+                // rows that see nothing of this unit are not read from its slot: no mask for them
+                if (__any_sync(kFull, lim >= w.kmin && lim < base + kWTile - 1) || base < w.kmin || (bad[0] | bad[1] | bad[2] | bad[3])) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        const int d = lim - base - 32 * c;
+                        const int below = w.kmin - base - 32 * c;
+                        const uint32_t vis = (d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u) & ~bad[c] &
+                                             (below <= 0 ? 0xffffffffu : below >= 32 ? 0u : 0xffffffffu << below);
+                        uint32_t x[32];
+                        tmem_ld<32>(s_col + 32 * c, x);
+                        tmem_wait_ld(x);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int d = lim - base - 32 * c;
-                    vis[c] = (d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u) & ~bads[c];
+                        for (int e = 0; e < 32; e++) x[e] = vis >> e & 1 ? x[e] : 0xff800000u;
+                        tmem_st32(s_col + 32 * c, x);
+                    }
+                    tmem_wait_st();
                 }
+                uint32_t x[32], y[32];
                 float mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t s[32];
-                    tmem_ld<32>(s_col + 32 * c, s);
-                    tmem_wait_ld(s);
-                    if (mask) {
+                for (int c = 0; c < 4; c += 2) {
+                    tmem_ld<32>(s_col + 32 * c, x);
+                    tmem_ld<32>(s_col + 32 * c + 32, y);
+                    tmem_wait_ld(x);
+                    tmem_tie(y);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) mx = fmaxf(mx, vis[c] >> e & 1 ? __uint_as_float(s[e]) : -INFINITY);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(s[e]));
-                    }
+                    for (int e = 0; e < 32; e++) mx = max3(mx, __uint_as_float(x[e]), __uint_as_float(y[e]));
                 }
                 mx = mx == -INFINITY ? mx : mx * f;
                 const bool rise = mx > B + kWHigh;
                 if (__any_sync(kFull, rise)) {
                     const float nb = rise ? mx - kWLow : B, fac = B == -INFINITY ? 0.0f : ex2(B - nb);
                     B = nb;
-                    l *= fac;
-                    if (j > 0) {                  // the MMAs up to tile j - 1 ended before S of tile j was announced
-#pragma unroll
+                    l2.x *= fac;
+                    l2.y *= fac;
+                    if (j > 1 || (!SPLIT && j > 0)) {     // the MMAs on O ended before this tile's S was announced
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
                             tmem_ld<32>(o_col + 32 * c, o);
@@ -315,45 +383,58 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
                         }
                     }
                 }
-                const float nB = B == -INFINITY ? 0.0f : -B;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t s[32], o[32];
-                    tmem_ld<32>(s_col + 32 * c, s);
-                    tmem_wait_ld(s);
-                    float g = 0.0f;
+                const float2 f2 = make_float2(f, f), nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
+                // scores of 32 positions in z become weights: hi terms in the first 16 columns, lo in the next 16
+                auto weights = [&](uint32_t (&z)[32], uint32_t col) {
+                    uint32_t o[32];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float p0 = ex2(fmaf(__uint_as_float(s[e]), f, nB)), p1 = ex2(fmaf(__uint_as_float(s[e + 1]), f, nB));
-                        if (mask) {
-                            p0 = vis[c] >> e & 1 ? p0 : 0.0f;
-                            p1 = vis[c] >> e & 2 ? p1 : 0.0f;
-                        }
-                        g += p0 + p1;
-                        split_h2(p0, p1, o[e / 2], o[16 + e / 2]);
+                        const float2 q = f2_fma(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), f2, nB);
+                        const float2 w2 = make_float2(ex2(q.x), ex2(q.y));
+                        const float2 h = make_float2(tf32_hi(w2.x), tf32_hi(w2.y));        // 11 bits: an fp16 value
+                        const float2 lo = f2_fma(h, make_float2(-1.0f, -1.0f), w2);
+                        l2 = f2_add(l2, w2);
+                        o[e / 2] = pack_h2(h.x, h.y);
+                        o[16 + e / 2] = pack_h2(lo.x, lo.y);
                     }
-                    l += g;
-                    tmem_st32(s_col + 32 * c, o); // hi of 32 positions in 16 columns, lo in the next 16
-                }
+                    tmem_st32(col, o);
+                };
+                weights(x, s_col + 64);           // chunks 2 and 3 are still here; 0 and 1 come again meanwhile
+                tmem_ld<32>(s_col, x);
+                weights(y, s_col + 96);
+                tmem_wait_ld(x);
+                tmem_ld<32>(s_col + 32, y);
+                weights(x, s_col);
+                tmem_wait_ld(y);
+                weights(y, s_col + 32);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[i]);
             }
+            if (SPLIT && i >= w.nt) {             // no position tile for this stream
+                if (lane == 0) mbar_arrive(staged);
+                continue;
+            }
             if (!ok || !(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;     // O is complete
             ns++;
             tc_fence_after();
+            const float l = l2.x + l2.y;
             if (isnan(l) && B == -INFINITY) B = 0.0f;
-            const bool put = tok >= 0 && lim >= w.k0, none = l == 0.0f, fix = *s_flag != 0;
-            float *dst = A.part_o + ((int64_t)w.slot * a.n_tok * a.H + (put ? tok : 0)) * D;
-#pragma unroll
+            const bool put = tok >= 0 && lim >= (SPLIT && i ? w.k0 + kWTile : w.kmin), none = l == 0.0f, fix = *s_flag != 0;
+            const int64_t out = (int64_t)(w.slot + (SPLIT ? i : 0)) * a.n_tok * a.H + (put ? tok : 0);
+            // the rows leave by way of shared memory (where this warp's rows of Q are; SPLIT's second stream: of
+            // their low terms), 128 bytes of a row per 8 lanes
+            unsigned char *stage = sm + i * (SPLIT ? 1 : 2) * C::TILE + (warp & 3) * 4096;
+#pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
                 tmem_ld<32>(o_col + 32 * c, o);
                 tmem_wait_ld(o);
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
-                    for (int p = max(w.k0, w.lo + 1); p <= lim; p++) {
+                    for (int p = w.kmin; p <= lim; p++) {
+                        if (SPLIT && ((p - w.k0) / kWTile & 1) != i) continue;
                         const int64_t at = paged_at(a, a.table + (own ? (int64_t)w.b * a.table_stride : 0), p);
                         if (at < 0) continue;
                         const __half *vr = reinterpret_cast<const __half *>(a.v + at + w.kh * a.head_stride) + 32 * c;
@@ -364,98 +445,95 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
                         }
                     }
                 }
-                if (put) {
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(dst + 32 * c + e) =
-                            none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                 : make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                for (int e = 0; e < 32; e += 4)   // 16-byte piece e / 4 of row `lane`, XOR-placed against bank conflicts
+                    *reinterpret_cast<uint4 *>(stage + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)) =
+                        none ? make_uint4(0, 0, 0, 0) : make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 8; k++) {     // 4 rows of 128 bytes at a time
+                    const int rr = 4 * k + (lane >> 3), pc = lane & 7;
+                    const int64_t to = __shfl_sync(kFull, put ? out : (int64_t)-1, rr);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + ((pc ^ (rr & 7)) << 4));
+                    if (to >= 0) *reinterpret_cast<uint4 *>(A.part_o + to * D + 32 * c + pc * 4) = v;
                 }
             }
-            if (put) A.part_ml[(int64_t)w.slot * a.n_tok * a.H + tok] = make_float2(none ? -INFINITY : B, l);
+            if (SPLIT && i == 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(staged);
+            }
+            if (put) A.part_ml[out] = make_float2(none ? -INFINITY : B, l);
             tc_fence_before();
         }
-    } else if (warp < 12) {
-        // ---- K and V: load c = 2 t (K), 2 t + 1 (V) of the CTA's tile t into ring slot c % SLOTS
-        const int pt = tid - 256, pw = warp - 8, piece = pt % C::CH, row0 = pt / C::CH;
-        constexpr int RS = 128 / C::CH;           // rows between a thread's pieces
-        uint32_t c = 0, t = 0;
-        int pend = -1;                            // the load that is issued but not announced
-        bool pend_scan = false, ok = true;
-        int pend_base = 0, pend_lo = 0;
-        auto announce = [&]() {
-            const uint32_t dst = sm0 + C::RING + (pend % C::SLOTS) * C::TILE;
-            if (pend_scan) {                      // V behind the causal mask: a weight of 0 does not cancel inf
-#pragma unroll 4
-                for (int k = 0; k < kWTile / RS; k++) {
-                    const int r = row0 + k * RS;
-                    if (pend_base + r <= pend_lo) continue;
-                    const uint32_t at = dst + (piece >> 3) * C::HALF + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-                    uint4 *pv = reinterpret_cast<uint4 *>(sm + (at - sm0));
-                    uint4 v = *pv;
-                    if (drop_nonfinite((const __half *)nullptr, v)) {
-                        *pv = v;
-                        *s_flag = 1;
-                    }
-                }
-            }
-            fence_async_smem();
-            mbar_arrive(&full[pend % C::SLOTS]);
-            pend = -1;
-        };
-        auto issue = [&](const int64_t *off, const char *pool, int kh, bool scan, int base, int lo) {
-            const uint32_t slot = c % C::SLOTS;
-            if (c >= C::SLOTS) {
-                const uint32_t ph = (c / C::SLOTS - 1) & 1;
-                if (!mbar_test_wait(&empty[slot], ph)) {
-                    if (pend >= 0) {              // do not hold back what has landed
-                        cp_wait<0>();
-                        announce();
-                    }
-                    if (!sy.wait(&empty[slot], ph)) return false;
-                }
-            }
-            const uint32_t dst = sm0 + C::RING + slot * C::TILE;
-#pragma unroll 4
-            for (int k = 0; k < kWTile / RS; k++) {
-                const int r = row0 + k * RS;
-                const int64_t at = off[r];
-                cp_async16_or0(dst + (piece >> 3) * C::HALF + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
-                               pool + (at < 0 ? 0 : at + kh * a.head_stride + piece * 16), at >= 0);
-            }
-            cp_commit();
-            if (pend >= 0) {
-                cp_wait<1>();
-                announce();
-            }
-            pend = (int)c++;
-            pend_scan = scan;
-            pend_base = base;
-            pend_lo = lo;
-            return true;
-        };
-        for (int u = blockIdx.x; u < n_unit; u += gridDim.x) {     // after a failed wait: the barriers, no copies
-            const WideUnit w(A, own, lo_p, u);
-            if (!w.any) continue;
+    } else if (warp < 11) {
+        // ---- K and V, in the order of their use, load c into ring slot c % SLOTS: K, V of each position tile, or
+        // (SPLIT) K, K, V, V of two. Warp 8 issues them; V tiles with rows that not every row sees (or that were
+        // not loaded) land on a barrier of their own and are passed on by warps 9 and 10.
+        uint32_t c = 0, t = 0, phases = 0;
+        bool ok = true;
+        const int R = min(1 << a.page_log, kWTile), boxes = kWTile / R;        // positions per box, boxes per 64 values
+        while (work.next(w)) {                    // (after a failed wait: the barriers, no copies)
             const int *table = a.table + (own ? (int64_t)w.b * a.table_stride : 0);
-            for (int j = 0; j < w.nt; j++, t++) {
-                const int base = w.k0 + j * kWTile, p = base + pt;
-                int64_t *off = s_off + (t & 1) * kWTile;
-                int64_t at = -1;
-                if (p < w.k1) {
-                    at = paged_at(a, table, p);
-                    if (at < 0) paged_err(a, QMS_PAGED_EPAGE);
+            constexpr int STEP = SPLIT ? 2 : 1;
+            for (int j0 = 0; j0 < w.nt; j0 += STEP) {
+                const int m = min(STEP, w.nt - j0);
+                for (int k = 0; k < 2 * m; k++, c++) {
+                    const bool is_v = k >= m;
+                    const int jj = is_v ? k - m : k, base = w.k0 + (j0 + jj) * kWTile;
+                    const uint32_t slot = c % C::SLOTS;
+                    // lane x: page of box x (positions base + x R ..); boxes past the unit are not loaded
+                    const int p = base + lane * R;
+                    int page = -1;
+                    if (lane < boxes && p < w.k1) {
+                        page = table[p >> a.page_log];
+                        if ((unsigned)page >= (unsigned)a.n_pages) {
+                            page = -1;
+                            if (warp == 8) paged_err(a, QMS_PAGED_EPAGE);
+                        }
+                    }
+                    const uint32_t have = __ballot_sync(kFull, page >= 0), want = __ballot_sync(kFull, lane < boxes && p < w.k1);
+                    const int seen = min(w.lo, w.k1 - 1);
+                    const bool scan = is_v && (base + kWTile - 1 > seen || base < w.kmin || want != have);
+                    if (warp == 8) {
+                        if (!is_v && lane < 4) {  // bits of the tile's positions on bad pages
+                            uint32_t bits = 0;
+                            if (want != have)
+                                for (int e = 0; e < 32; e++) bits |= ((want & ~have) >> ((lane * 32 + e) / R) & 1u) << e;
+                            s_bad[((t + jj) & 7) * 4 + lane] = bits;
+                        }
+                        __syncwarp();
+                        if (c >= C::SLOTS) ok = __all_sync(kFull, ok && sy.wait(&empty[slot], (c / C::SLOTS - 1) & 1));
+                        if (!ok) continue;
+                        uint64_t *bar = scan ? &landed[slot] : &full[slot];
+                        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * (uint32_t)(R * 128 * C::HALVES));
+                        __syncwarp();
+                        const uint32_t dst = sm0 + C::RING + slot * C::TILE + lane * R * 128;
+                        if (page >= 0)
+#pragma unroll
+                            for (int h = 0; h < C::HALVES; h++) tma_load4(dst + h * C::HALF, is_v ? &mv : &mk, h * 64, w.kh, p & ((1 << a.page_log) - 1), page, bar);
+                    } else if (scan) {
+                        ok = ok && sy.wait(&landed[slot], phases >> slot & 1);
+                        phases ^= 1u << slot;
+                        for (int x = tid - 288; ok && x < kWTile * C::CH; x += 64) {
+                            const int r = x / C::CH, piece = x % C::CH;
+                            if (base + r >= w.kmin && base + r <= seen && want == have) continue;
+                            uint4 *pv = reinterpret_cast<uint4 *>(sm + C::RING + slot * C::TILE + (piece >> 3) * C::HALF + r * 128 +
+                                                                  (((piece & 7) ^ (r & 7)) << 4));
+                            uint4 v = *pv;
+                            if (drop_nonfinite((const __half *)nullptr, v)) {
+                                *pv = v;
+                                *s_flag = 1;
+                            }
+                        }
+                        fence_async_smem();
+                        asm volatile("bar.sync 1, 64;" ::: "memory");
+                        if (tid == 288) mbar_arrive(&full[slot]);
+                    }
                 }
-                off[pt] = at;
-                const uint32_t bad = __ballot_sync(kFull, p < w.k1 && at < 0);
-                if (lane == 0) s_bad[(t & 3) * 4 + pw] = bad;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                ok = ok && issue(off, a.k, w.kh, false, 0, 0) && issue(off, a.v, w.kh, base + kWTile - 1 > w.lo, base, w.lo);
-                ok = __all_sync(kFull, ok) && !*s_abort;
+                t += m;
             }
         }
-        cp_wait<0>();
-        if (pend >= 0) announce();
     } else {
         // ---- the MMAs, by one thread
         if (lane == 0) {
@@ -463,7 +541,7 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
             uint32_t c = 0, nq[2] = {0, 0}, np[2] = {0, 0};
             bool ok = true;
             auto score = [&](int i, uint32_t kc) {             // S_i = (hi + lo of Q_i) K^T
-                const uint32_t k = sm0 + C::RING + (kc % C::SLOTS) * C::TILE, q = sm0 + i * 2 * C::TILE;
+                const uint32_t k = sm0 + C::RING + (kc % C::SLOTS) * C::TILE, q = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
 #pragma unroll
                 for (int term = 0; term < 2; term++)
 #pragma unroll
@@ -482,33 +560,39 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
                                     desc_sw128(v + ks * 2048, C::HALF, 1024), id_o, !first || term || ks);
             };
             auto full_at = [&](uint32_t x) { return sy.wait(&full[x % C::SLOTS], (x / C::SLOTS) & 1); };
-            for (int u = blockIdx.x; u < n_unit && ok; u += gridDim.x) {
-                const WideUnit w(A, own, lo_p, u);
-                if (!w.any) continue;
-                if (!(ok = full_at(c))) break;
-                for (int i = 0; i < w.tiles && ok; i++) {
-                    if (!(ok = sy.wait(&q_full[i], nq[i]++ & 1))) break;
+            while (ok && work.next(w)) {
+                // step = one position tile for both streams, or (SPLIT) one for each; m: tiles of the step; loads c ..
+                auto tiles_of = [&](int j) { return SPLIT ? min(2, w.nt - j) : 1; };
+                auto streams_of = [&](int j) { return SPLIT ? min(2, w.nt - j) : w.tiles; };
+                for (int i = 0; i < streams_of(0) && ok; i++) {
+                    const uint32_t k = c + (SPLIT ? i : 0);
+                    if ((SPLIT || i == 0) && !(ok = full_at(k))) break;
+                    if ((!SPLIT || i == 0) && !(ok = sy.wait(&q_full[i], nq[i] & 1))) break;
                     tc_fence_after();
-                    score(i, c);
+                    score(i, k);
                     umma_commit(&s_full[i]);
+                    if (SPLIT || i == w.tiles - 1) umma_commit(&empty[k % C::SLOTS]);
                 }
-                if (!ok) break;
-                umma_commit(&empty[c % C::SLOTS]);
-                for (int j = 0; j < w.nt && ok; j++, c += 2) {
-                    if (!(ok = full_at(c + 1))) break;
-                    const bool more = j + 1 < w.nt;
-                    for (int i = 0; i < w.tiles && ok; i++) {
+                nq[0]++;
+                if (w.tiles > 1) nq[1]++;
+                for (int j = 0; j < w.nt && ok; j += SPLIT ? 2 : 1) {
+                    const int m = tiles_of(j), jn = j + (SPLIT ? 2 : 1), more = jn < w.nt ? streams_of(jn) : 0;
+                    const uint32_t cn = c + 2 * m;
+                    for (int i = 0; i < streams_of(j) && ok; i++) {
+                        const uint32_t v = c + m + (SPLIT ? i : 0), k = cn + (SPLIT ? i : 0);
+                        if ((SPLIT || i == 0) && !(ok = full_at(v))) break;
                         if (!(ok = sy.wait(&p_full[i], np[i]++ & 1))) break;
                         tc_fence_after();
-                        weigh(i, c + 1, j == 0);
-                        if (i == w.tiles - 1) umma_commit(&empty[(c + 1) % C::SLOTS]);
-                        if (more) {
-                            if (i == 0 && !(ok = full_at(c + 2))) break;
-                            score(i, c + 2);
+                        weigh(i, v, j == 0);
+                        if (SPLIT || i == w.tiles - 1) umma_commit(&empty[v % C::SLOTS]);
+                        if (i < more) {
+                            if ((SPLIT || i == 0) && !(ok = full_at(k))) break;
+                            score(i, k);
                         }
                         umma_commit(&s_full[i]);
+                        if (i < more && (SPLIT || i == w.tiles - 1)) umma_commit(&empty[k % C::SLOTS]);
                     }
-                    if (ok && more) umma_commit(&empty[(c + 2) % C::SLOTS]);
+                    c = cn;
                 }
             }
             if (!ok) {                                          // nothing of this CTA's is in flight when TMEM goes
@@ -520,33 +604,64 @@ __global__ void __launch_bounds__(kWThreads, 1) k_paged_wide(const PagedAttn A, 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 11) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
     if (last) pdl_wait();
 }
 
-template <int D>
+// The pool as a tensor [page][position][head][value] for boxes of 64 values x min(page size, 128) positions.
+static int pool_map(const Paged &a, int D, const char *pool, CUtensorMap *map) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    if (!encode) {
+        cudaDriverEntryPointQueryResult found;
+        void *f = nullptr;
+        QMS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
+        QMS_REQUIRE(f, QMS_CUDA_ECUDA, "paged_attention: the driver has no cuTensorMapEncodeTiled");
+        encode = (Encode)f;
+    }
+    const cuuint64_t ps = 1ull << a.page_log;
+    const cuuint64_t dim[4] = {(cuuint64_t)D, (cuuint64_t)a.Hk, ps, (cuuint64_t)a.n_pages};
+    // (the stride of a dimension of one has no meaning, and 0 none that the encoder takes)
+    const cuuint64_t stride[3] = {(cuuint64_t)(a.Hk > 1 ? a.head_stride : 2 * D), (cuuint64_t)(ps > 1 ? a.pos_stride : 2 * D),
+                                  (cuuint64_t)(a.n_pages > 1 ? a.page_stride : 2 * D)};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)(ps < kWTile ? ps : kWTile), 1}, one[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void *)pool, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    QMS_REQUIRE(rc == CUDA_SUCCESS, QMS_CUDA_EINVAL, "paged_attention: the pool's strides do not make a tensor map (%d)", (int)rc);
+    return QMS_CUDA_OK;
+}
+
+template <int D, bool SPLIT>
 static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
-    using C = WideCfg<D>;
+    using C = WideCfg<D, SPLIT>;
     static_assert(C::SMEM <= 232448, "shared memory per CTA");
-    const int64_t units = own ? (int64_t)A.p.slots_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.slots_p * A.p.tiles_p * A.a.Hk;
+    const int64_t units = !own && A.p.line > 0 ? A.p.line
+                          : own                ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk
+                                               : (int64_t)A.p.chunks_p * A.p.tiles_p * A.a.Hk;
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     static unsigned long long set = 0;                          // per device
     int dev = 0;
     QMS_CK(cudaGetDevice(&dev));
     if (!(set >> (dev & 63) & 1)) {
-        QMS_CK(cudaFuncSetAttribute(k_paged_wide<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        QMS_CK(cudaFuncSetAttribute(k_paged_wide<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         set |= 1ull << (dev & 63);
     }
+    CUtensorMap mk, mv;
+    int rc = pool_map(A.a, D, A.a.k, &mk);
+    if (rc || (rc = pool_map(A.a, D, A.a.v, &mv))) return rc;
     const int grid = (int)(units < 148 ? units : 148);
-    QMS_CK(launch_pdl(k_paged_wide<D>, dim3(grid), dim3(kWThreads), C::SMEM, s, A, own, last));
+    QMS_CK(launch_pdl(k_paged_wide<D, SPLIT>, dim3(grid), dim3(kWThreads), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
 }
 
 int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s) {
-    return D == 128 ? launch_wide<128>(A, own, last, s) : launch_wide<64>(A, own, last, s);
+    const bool split = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit;
+    if (D == 128) return split ? launch_wide<128, true>(A, own, last, s) : launch_wide<128, false>(A, own, last, s);
+    return split ? launch_wide<64, true>(A, own, last, s) : launch_wide<64, false>(A, own, last, s);
 }
 
 }  // namespace qms
