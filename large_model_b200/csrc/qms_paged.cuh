@@ -122,13 +122,20 @@ struct PagedPlan {
     int chunks_p, chunks_s;          // chunks of each kind
     int slots_p, slots_s;            // slots of each kind
     int tiles_p, tiles_s;            // row tiles of each kind
-    int64_t line;                    // k_paged_wide's runs over the shared positions: their total length, or 0
-    int line_ctas;                   // CTAs that share it
+    unsigned line, line_ctas;        // k_paged_wide's runs over the shared positions: total length (0: none), and CTAs
 };
 constexpr int kPaWidePair = 0, kPaWideSplit = -1;    // k_paged_wide: two tiles of 128 rows; one, in two streams
 
-// Which of n CTAs holds place x of a line cut into n runs [line i / n, line (i + 1) / n).
-__host__ __device__ inline int line_cta(int64_t x, int64_t line, int n) { return (int)(((x + 1) * n - 1) / line); }
+// A line of `line` places in n runs, the first line % n of them one place longer: where run i starts, and which run
+// holds place x. (32 bits: a 64-bit division costs the kernels some 500 cycles.)
+__host__ __device__ inline unsigned line_start(unsigned i, unsigned line, unsigned n) {
+    const unsigned q = line / n, r = line - q * n;
+    return i * q + (i < r ? i : r);
+}
+__host__ __device__ inline unsigned line_run(unsigned x, unsigned line, unsigned n) {
+    const unsigned q = line / n, r = line - q * n;
+    return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
+}
 
 struct PagedAttn {
     Paged a;

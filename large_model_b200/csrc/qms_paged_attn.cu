@@ -509,9 +509,9 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
         if (a.prefix > 0) {
             const int d = min(pos, a.prefix - 1);
             if (A.p.line > 0) {
-                const int h = (int)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
-                const int64_t u = (int64_t)((t * a.G + h - kh * a.G) / 256) * a.Hk + kh;
-                np = line_cta(u * nt + d / 128, A.p.line, A.p.line_ctas) - line_cta(u * nt, A.p.line, A.p.line_ctas) + 1;
+                const unsigned h = (unsigned)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
+                const unsigned x = ((t * a.G + h - kh * a.G) / 256 * a.Hk + kh) * nt;
+                np = line_run(x + d / 128, A.p.line, A.p.line_ctas) - line_run(x, A.p.line, A.p.line_ctas) + 1;
             } else {
                 np = upto(d, A.p.chunk_p, A.p.wr_p);
             }
@@ -594,10 +594,10 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     p.slots_s = p.chunks_s * (p.wr_s == kPaWideSplit ? 2 : 1);
     p.line = 0;
     p.line_ctas = 0;
-    if (p.wr_p == kPaWidePair && a.prefix > 0 && rows_p > 0) {
-        const int64_t nt = (a.prefix + 127) / 128;
-        p.line = nt * p.tiles_p * a.Hk;
-        p.line_ctas = (int)std::min<int64_t>(148, p.line);
+    const int64_t nt = (a.prefix + 127) / 128, line = nt * p.tiles_p * a.Hk;
+    if (p.wr_p == kPaWidePair && line > 0 && line < (1ll << 31)) {
+        p.line = (unsigned)line;
+        p.line_ctas = (unsigned)std::min<int64_t>(148, line);
         // a row tile's positions meet at most this many runs
         p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / (p.line / p.line_ctas) + 2);
     }

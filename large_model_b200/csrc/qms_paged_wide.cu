@@ -10,16 +10,18 @@
 //   softmax     one thread per row reads its S from TMEM, keeps the running base B and sum l, writes the
 //               weights 2^(s f - B) back over S as two fp16 terms
 //   O += P V    tcgen05.mma with P from TMEM (hi, then lo) and V as it lies in shared memory (MN-major)
-// O stays in TMEM over the whole chunk. It is rescaled only when a row's maximum rises by more than 2^7
-// since its base was set, which a base 2^8 below the first maximum and fp16's range of 2^16 allow; the
-// result does not depend on it beyond rounding.
+// O stays in TMEM over the whole unit. A base is set 2^8 below a maximum and stays until a score lies 2^15 above it
+// (fp16 holds weights to 2^16), so that the maximum needs no pass of its own; the result does not depend on
+// it beyond rounding.
 //
 // Warps 0-3 and 4-7 are the softmax of the two streams, warp 8 brings K and V in by TMA (a box of 64 values x up to 128
-// positions per page, swizzled), warps 9 and 10 clear values that are not finite out of V rows that some row
-// does not see (a weight of 0 does not cancel them), one thread of warp 11 issues the MMAs. Tiles start on a
+// positions per page, swizzled), warp 9 clears values that are not finite out of V rows that some row does
+// not see (a weight of 0 does not cancel them), one thread each of warps 10 and 11 issues the MMAs of a stream, 16 or
+// 32 at a time under a lock: one thread for both leaves the tensor cores idle while it waits and commits (some
+// 1200 of 6150 cycles per pair of tiles: hardly one MMA is queued), two that interleave slow every MMA down. Tiles start on a
 // page boundary (or, in larger pages, a multiple of 128), so a tile may begin before the first position of its
-// unit; such rows are masked. Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB, or (SPLIT) Q 64 KB and 5
-// tiles; TMEM: S 2 x 128, O 2 x 128 columns.
+// unit; such rows are masked. Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB, or (SPLIT) Q 64 KB and a
+// ring of 2 for each stream; TMEM: S 2 x 128, O 2 x 128 columns.
 // Bound by the tensor cores: 4 * 128 * 128 * head_dim flop per tile and product pair, twice for the split.
 #include <cuda.h>
 #include <math.h>
@@ -40,11 +42,16 @@ struct WideCfg {
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t HALF = kWTile * 128;              // bytes of 128 rows x 64 values
     static constexpr uint32_t TILE = HALVES * HALF;             // a K or V tile; one term of a Q tile
-    static constexpr int SLOTS = SPLIT ? 5 : 3, CH = D / 8;     // CH: 16-byte pieces per row
+    static constexpr int SLOTS = SPLIT ? 4 : 3, CH = D / 8;     // CH: 16-byte pieces per row
     static constexpr uint32_t RING = (SPLIT ? 2 : 4) * TILE, META = RING + SLOTS * TILE;
     // meta: bad-page masks [8][4], barriers, flags
-    static constexpr uint32_t BAD = META, BARS = BAD + 128, SMEM = BARS + (3 * SLOTS + 8) * 8 + 16;
+    static constexpr uint32_t BAD = META, BARS = BAD + 128, SMEM = BARS + (3 * SLOTS + 9) * 8 + 32;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
+    // load n of a ring: its slot and the parity of that slot's phase. (A ring per stream in SPLIT: whoever waits
+    // for a slot waits for each of its phases.)
+    static constexpr uint32_t RINGLEN = SPLIT ? 2 : 3;
+    static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return SPLIT ? 2 * stream + (n & 1) : n % 3; }
+    static __device__ __forceinline__ uint32_t phase(uint32_t n) { return n / RINGLEN & 1; }
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) { return umma_desc(saddr, lbo, sbo) | (2ull << 61); }
@@ -137,47 +144,49 @@ struct WideWork {
     const PagedAttn &A;
     const bool own, line;
     const int lo_p;
-    int64_t x, end;
+    unsigned x, end;
     __device__ WideWork(const PagedAttn &A_, bool own_, int lo_p_) : A(A_), own(own_), line(!own_ && A_.p.line > 0), lo_p(lo_p_) {
         if (line) {
-            x = A.p.line * blockIdx.x / gridDim.x;
-            end = A.p.line * (blockIdx.x + 1) / gridDim.x;
+            x = line_start(blockIdx.x, A.p.line, gridDim.x);
+            end = line_start(blockIdx.x + 1, A.p.line, gridDim.x);
         } else {
             x = blockIdx.x;
-            end = (int64_t)(own ? A.p.chunks_s * A.a.n_seq * A.p.tiles_s : A.p.chunks_p * A.p.tiles_p) * A.a.Hk;
+            end = (unsigned)(own ? A.p.chunks_s * A.a.n_seq * A.p.tiles_s : A.p.chunks_p * A.p.tiles_p) * A.a.Hk;
         }
     }
     __device__ bool next(WideUnit &w) {
         const Paged &a = A.a;
-        const int rows_tile = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit ? kWTile : 2 * kWTile;
+        const unsigned rows_tile = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit ? kWTile : 2 * kWTile;
         for (; x < end;) {
             w.b = w.t0 = w.n = w.kv = 0;
             if (line) {
-                const int nt = (a.prefix + kWTile - 1) / kWTile;
-                const int64_t u = x / nt;
-                const int j = (int)(x - u * nt), c = (int)min((int64_t)(nt - j), end - x);
-                w.kh = (int)(u % a.Hk);
-                w.r0 = (int)(u / a.Hk) * rows_tile;
-                w.slot = blockIdx.x - line_cta(u * nt, A.p.line, gridDim.x);
+                const unsigned nt = (a.prefix + kWTile - 1) / kWTile, u = x / nt, j = x - u * nt, c = min(nt - j, end - x);
+                const unsigned tile = u / a.Hk;
+                w.kh = u - tile * a.Hk;
+                w.r0 = tile * rows_tile;
+                w.slot = blockIdx.x - line_run(u * nt, A.p.line, gridDim.x);
                 w.k0 = w.kmin = j * kWTile;
-                w.k1 = min(a.prefix, (j + c) * kWTile);
+                w.k1 = min(a.prefix, (int)(j + c) * kWTile);
                 x += c;
             } else {
-                int u = (int)x;
+                unsigned u = x;
                 x += gridDim.x;
-                w.kh = u % a.Hk;
-                u /= a.Hk;
-                const int nr = own ? A.p.tiles_s : A.p.tiles_p;
-                w.r0 = u % nr * rows_tile;
-                u /= nr;
+                unsigned d = u / a.Hk;
+                w.kh = u - d * a.Hk;
+                u = d;
+                const unsigned nr = own ? A.p.tiles_s : A.p.tiles_p;
+                d = u / nr;
+                w.r0 = (u - d * nr) * rows_tile;
+                u = d;
                 if (own) {
-                    w.b = u % a.n_seq;
-                    u /= a.n_seq;
+                    d = u / a.n_seq;
+                    w.b = u - d * a.n_seq;
+                    u = d;
                     paged_seq(a, w.b, w.t0, w.n, w.kv);
                     w.k0 = A.p.base_s + u * A.p.chunk_s;
                     w.kmin = max(w.k0, a.prefix);
                     w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
-                    w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (w.r0 + rows_tile - 1) / a.G) + 1);     // nobody sees the rest
+                    w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (int)(w.r0 + rows_tile - 1) / a.G) + 1);     // nobody sees the rest
                 } else {
                     w.k0 = w.kmin = u * A.p.chunk_p;
                     w.k1 = min(a.prefix, w.k0 + A.p.chunk_p);
@@ -204,10 +213,10 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     const uint32_t sm0 = smem_u32(sm);
     uint32_t *s_bad = reinterpret_cast<uint32_t *>(sm + C::BAD);
     uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + C::SLOTS, *landed = empty + C::SLOTS;
-    uint64_t *staged = landed + C::SLOTS, *q_full = staged + 1, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
+    uint64_t *staged = landed + C::SLOTS, *q_free = staged + 1, *q_full = q_free + 1, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
     int *s_int = reinterpret_cast<int *>(drain + 1);              // abort, V set aside, TMEM base, least position
     volatile int *s_abort = s_int, *s_flag = s_int + 1;
-    int *s_lo = s_int + 3;
+    int *s_lo = s_int + 3, *s_lock = s_int + 4;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(s_int + 2);
     if (sm0 & 1023) {                             // the swizzled tiles need it; never seen
         if (tid == 0) paged_err(a, QMS_PAGED_ETIMEOUT);
@@ -217,7 +226,7 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], SPLIT ? 1 : 2);
             mbar_init(&landed[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -225,9 +234,10 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
         }
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);
         mbar_init(staged, 4);
-        s_int[0] = s_int[1] = 0;
+        mbar_init(q_free, 2);
+        s_int[0] = s_int[1] = *s_lock = 0;
         *s_lo = 0x7fffffff;
         fence_mbar_init();
     }
@@ -261,57 +271,66 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_col = lanes + i * kWTile, o_col = lanes + C::O_COL + i * D;
-        uint32_t ns = 0, before = 0, units = 0;   // phases of s_full; position tiles of the CTA's earlier units (for s_bad)
+        uint32_t ns = 0, before = 0, unit_no = 0; // phases of s_full; position tiles of the CTA's earlier units (for s_bad)
         bool ok = true;
-        for (; ok && work.next(w); before += w.nt) {
+        for (; ok && work.next(w); before += w.nt, unit_no++) {
             if (!SPLIT && i >= w.tiles) continue;
             const int r = w.r0 + (SPLIT ? 0 : i * kWTile) + row, t = r / a.G;    // this row: its token, position below
             int tok = -1;                                                        // token row * H + head (-1: none)
-            if (r < w.rows) tok = (w.t0 + t) * a.H + w.kh * a.G + (r - t * a.G);
+            int64_t qo = -1;                                                     // where its q is
+            if (r < w.rows) {
+                const int h = w.kh * a.G + (r - t * a.G);
+                tok = (w.t0 + t) * a.H + h;
+                qo = (w.t0 + t) * A.ldq + (int64_t)h * D;
+            }
             // q: 8 lanes per row, 4 rows at a time: row maximum, power-of-two scale, two fp16 terms, swizzled
             // rows (SPLIT: one stream writes them for both, the other one only wants the scales)
             float f = 0.0f;
-            const float sign = A.scale2 < 0.0f ? -1.0f : 1.0f;     // f >= 0: the largest s f has the largest s
-            const uint32_t qb = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
-            if (SPLIT && i == 0 && units++ > 0 && !(ok = __all_sync(kFull, sy.wait(staged, units & 1)))) break;
-#pragma unroll 1
-            for (int g0 = 0; g0 < 8; g0 += 4) {
-                float4 x[4][D / 32];              // 16 rows of the warp in flight
+            const uint32_t sign = A.scale2 < 0.0f ? 0x80000000u : 0u;  // f >= 0: the largest s f has the largest s
+            float4 x[2][4][D / 32];
+            auto fetch = [&](float4 (&z)[4][D / 32], int g0) {         // 16 rows of the warp
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const int tk = __shfl_sync(kFull, tok, 4 * (g0 + g) + (lane >> 3));
-                    const float *src = A.q + (tk < 0 ? 0 : (tk / a.H) * A.ldq + (int64_t)(tk % a.H) * D) + (lane & 7) * 4;
+                    const int64_t from = __shfl_sync(kFull, qo, 4 * (g0 + g) + (lane >> 3));
+                    const float4 *src = reinterpret_cast<const float4 *>(A.q + from) + (lane & 7);
 #pragma unroll
-                    for (int k = 0; k < D / 32; k++)
-                        x[g][k] = tk < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(reinterpret_cast<const float4 *>(src + k * 32));
+                    for (int k = 0; k < D / 32; k++) z[g][k] = from < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(src + 8 * k);
                 }
+            };
+            auto place = [&](float4 (&z)[4][D / 32], int g0) {
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     float mx = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < D / 32; k++)
-                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[g][k].x), fabsf(x[g][k].y)), fmaxf(fabsf(x[g][k].z), fabsf(x[g][k].w))));
+                    for (int k = 0; k < D / 32; k++) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(z[g][k].x), fabsf(z[g][k].y)), fmaxf(fabsf(z[g][k].z), fabsf(z[g][k].w))));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-                    const int e = mx > 0.0f && mx < INFINITY ? ilogbf(mx) - 9 : 0;
-                    const float got = __shfl_sync(kFull, ldexpf(fabsf(A.scale2), e), (lane & 3) * 8);
+                    // the maximum goes to 2^9 .. 2^10: times 2^(up - 127), undone by 2^(127 - up) in the score
+                    const uint32_t up = mx == 0.0f ? 127u : min(263u - (__float_as_uint(mx) >> 23), 253u);
+                    const float got = __shfl_sync(kFull, fabsf(A.scale2) * __uint_as_float((254u - up) << 23), (lane & 3) * 8);
                     if (lane >> 2 == g0 + g) f = got;
                     if (SPLIT && i == 1) continue;
-                    const float d1 = ldexpf(sign, -e / 2), d2 = ldexpf(1.0f, -e - -e / 2);
+                    const float m = __uint_as_float(up << 23 | sign);
                     const int rr = (warp & 3) * 32 + 4 * (g0 + g) + (lane >> 3);
+                    const uint32_t at = sm0 + (SPLIT ? 0 : i * 2 * C::TILE) + rr * 128 + (lane & 1) * 8;
 #pragma unroll
                     for (int k = 0; k < D / 32; k++) {
-                        uint32_t h[2], l[2];
-                        split_h2(x[g][k].x * d1 * d2, x[g][k].y * d1 * d2, h[0], l[0]);
-                        split_h2(x[g][k].z * d1 * d2, x[g][k].w * d1 * d2, h[1], l[1]);
-                        const int d = (lane & 7) * 4 + k * 32;
-                        const uint32_t at = qb + (d >> 6) * C::HALF + rr * 128 + ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(h[0]), "r"(h[1]) : "memory");
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + C::TILE), "r"(l[0]), "r"(l[1]) : "memory");
+                        const float2 y0 = f2_mul(make_float2(z[g][k].x, z[g][k].y), make_float2(m, m)), y1 = f2_mul(make_float2(z[g][k].z, z[g][k].w), make_float2(m, m));
+                        const float2 h0 = make_float2(tf32_hi(y0.x), tf32_hi(y0.y)), h1 = make_float2(tf32_hi(y1.x), tf32_hi(y1.y));
+                        const float2 l0 = f2_fma(h0, make_float2(-1.0f, -1.0f), y0), l1 = f2_fma(h1, make_float2(-1.0f, -1.0f), y1);
+                        // values 4 (lane & 7) + 32 k .. + 3: 16-byte piece (lane & 7) / 2 + 4 (k & 1) of half k / 2
+                        const uint32_t to = at + (k >> 1) * C::HALF + (((((lane & 7) >> 1) + 4 * (k & 1)) ^ (rr & 7)) << 4);
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(pack_h2(h0.x, h0.y)), "r"(pack_h2(h1.x, h1.y)) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + C::TILE), "r"(pack_h2(l0.x, l0.y)), "r"(pack_h2(l1.x, l1.y)) : "memory");
                     }
                 }
-            }
+            };
+            fetch(x[0], 0);
+            fetch(x[1], 4);
+            if (SPLIT && i == 0 && unit_no > 0 && !(ok = __all_sync(kFull, sy.wait(staged, (unit_no - 1) & 1)))) break;
+            place(x[0], 0);
+            place(x[1], 4);
             fence_async_smem();
             if (!SPLIT || i == 0) mbar_arrive(&q_full[i]);
             int pos = -1;
@@ -353,39 +372,49 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                     }
                     tmem_wait_st();
                 }
-                uint32_t x[32], y[32];
-                float mx = -INFINITY;
+                // scores of 32 positions in z become weights, hi terms in the first 16 columns, lo in the next 16. The
+                // base of the weights is a whole number and stays, unless a score lies 2^kWHigh above it: then
+                // what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
+                const float2 f2 = make_float2(f, f);
+                auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {
+                    float mx = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    tmem_ld<32>(s_col + 32 * c, x);
-                    tmem_ld<32>(s_col + 32 * c + 32, y);
-                    tmem_wait_ld(x);
-                    tmem_tie(y);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) mx = max3(mx, __uint_as_float(x[e]), __uint_as_float(y[e]));
-                }
-                mx = mx == -INFINITY ? mx : mx * f;
-                const bool rise = mx > B + kWHigh;
-                if (__any_sync(kFull, rise)) {
-                    const float nb = rise ? mx - kWLow : B, fac = B == -INFINITY ? 0.0f : ex2(B - nb);
-                    B = nb;
-                    l2.x *= fac;
-                    l2.y *= fac;
-                    if (j > 1 || (!SPLIT && j > 0)) {     // the MMAs on O ended before this tile's S was announced
+                    for (int e = 3; e < 31; e += 2) mx = max3(mx, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                    mx = fmaxf(mx, __uint_as_float(z[31]));
+                    mx = mx == -INFINITY ? mx : mx * f;
+                    if (__any_sync(kFull, mx > B + kWHigh)) {
+                        const float nb = mx > B + kWHigh ? ceilf(mx) - kWLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
+                        B = nb;
+                        l2.x *= fac;
+                        l2.y *= fac;
+                        if (j > 1 || (!SPLIT && j > 0)) {      // (the MMAs on O ended before this tile's S was announced)
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; c++) {
+                            for (int k = 0; k < D / 32; k++) {
+                                uint32_t o[32];
+                                tmem_ld<32>(o_col + 32 * k, o);
+                                tmem_wait_ld(o);
+#pragma unroll
+                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+                                tmem_st32(o_col + 32 * k, o);
+                            }
+                        }
+                        const __half2 fh = __float2half2_rn(fac);
+#pragma unroll 1
+                        for (int k = 0; k < 4; k++) {
+                            if (!(done >> k & 1)) continue;
                             uint32_t o[32];
-                            tmem_ld<32>(o_col + 32 * c, o);
+                            tmem_wait_st();
+                            tmem_ld<32>(s_col + 32 * k, o);
                             tmem_wait_ld(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
-                            tmem_st32(o_col + 32 * c, o);
+                            for (int e = 0; e < 32; e++) {
+                                const __half2 p2 = __hmul2(*reinterpret_cast<const __half2 *>(&o[e]), fh);
+                                o[e] = *reinterpret_cast<const uint32_t *>(&p2);
+                            }
+                            tmem_st32(s_col + 32 * k, o);
                         }
                     }
-                }
-                const float2 f2 = make_float2(f, f), nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
-                // scores of 32 positions in z become weights: hi terms in the first 16 columns, lo in the next 16
-                auto weights = [&](uint32_t (&z)[32], uint32_t col) {
+                    const float2 nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
                     uint32_t o[32];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
@@ -397,16 +426,21 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                         o[e / 2] = pack_h2(h.x, h.y);
                         o[16 + e / 2] = pack_h2(lo.x, lo.y);
                     }
-                    tmem_st32(col, o);
+                    tmem_st32(s_col + 32 * c, o);
                 };
-                weights(x, s_col + 64);           // chunks 2 and 3 are still here; 0 and 1 come again meanwhile
+                uint32_t x[32], y[32];
                 tmem_ld<32>(s_col, x);
-                weights(y, s_col + 96);
                 tmem_wait_ld(x);
-                tmem_ld<32>(s_col + 32, y);
-                weights(x, s_col);
+                tmem_ld<32>(s_col + 32, y);       // the next 32 come while these are worked on
+                weights(x, 0, 0);
                 tmem_wait_ld(y);
-                weights(y, s_col + 32);
+                tmem_ld<32>(s_col + 64, x);
+                weights(y, 1, 1);
+                tmem_wait_ld(x);
+                tmem_ld<32>(s_col + 96, y);
+                weights(x, 2, 3);
+                tmem_wait_ld(y);
+                weights(y, 3, 7);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -419,10 +453,14 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
             if (!ok || !(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;     // O is complete
             ns++;
             tc_fence_after();
+            // SPLIT: Q, where the rows are staged, is both streams'
+            if (SPLIT && !(ok = __all_sync(kFull, sy.wait(q_free, unit_no & 1)))) break;
             const float l = l2.x + l2.y;
             if (isnan(l) && B == -INFINITY) B = 0.0f;
             const bool put = tok >= 0 && lim >= (SPLIT && i ? w.k0 + kWTile : w.kmin), none = l == 0.0f, fix = *s_flag != 0;
-            const int64_t out = (int64_t)(w.slot + (SPLIT ? i : 0)) * a.n_tok * a.H + (put ? tok : 0);
+            const int64_t first = (int64_t)(w.slot + (SPLIT ? i : 0)) * a.n_tok * a.H;
+            const int row_out = put ? tok : -1;
+            float *part = A.part_o + first * D + (lane & 7) * 4;
             // the rows leave by way of shared memory (where this warp's rows of Q are; SPLIT's second stream: of
             // their low terms), 128 bytes of a row per 8 lanes
             unsigned char *stage = sm + i * (SPLIT ? 1 : 2) * C::TILE + (warp & 3) * 4096;
@@ -453,35 +491,33 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 __syncwarp();
 #pragma unroll
                 for (int k = 0; k < 8; k++) {     // 4 rows of 128 bytes at a time
-                    const int rr = 4 * k + (lane >> 3), pc = lane & 7;
-                    const int64_t to = __shfl_sync(kFull, put ? out : (int64_t)-1, rr);
-                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + ((pc ^ (rr & 7)) << 4));
-                    if (to >= 0) *reinterpret_cast<uint4 *>(A.part_o + to * D + 32 * c + pc * 4) = v;
+                    const int rr = 4 * k + (lane >> 3), to = __shfl_sync(kFull, row_out, rr);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                    if (to >= 0) *reinterpret_cast<uint4 *>(part + (int64_t)to * D + 32 * c) = v;
                 }
             }
             if (SPLIT && i == 1) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(staged);
             }
-            if (put) A.part_ml[out] = make_float2(none ? -INFINITY : B, l);
+            if (put) A.part_ml[first + tok] = make_float2(none ? -INFINITY : B, l);
             tc_fence_before();
         }
-    } else if (warp < 11) {
-        // ---- K and V, in the order of their use, load c into ring slot c % SLOTS: K, V of each position tile, or
-        // (SPLIT) K, K, V, V of two. Warp 8 issues them; V tiles with rows that not every row sees (or that were
-        // not loaded) land on a barrier of their own and are passed on by warps 9 and 10.
-        uint32_t c = 0, t = 0, phases = 0;
+    } else if (warp < 10) {
+        // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. Warp 8 issues them; V tiles with rows that not every row sees (or that were
+        // not loaded) land on a barrier of their own and are passed on by warp 9.
+        uint32_t c[2] = {0, 0}, t = 0, phases = 0;       // loads so far (SPLIT: of each stream); tiles; of `landed`
         bool ok = true;
         const int R = min(1 << a.page_log, kWTile), boxes = kWTile / R;        // positions per box, boxes per 64 values
-        while (work.next(w)) {                    // (after a failed wait: the barriers, no copies)
+        while (ok && work.next(w)) {
             const int *table = a.table + (own ? (int64_t)w.b * a.table_stride : 0);
             constexpr int STEP = SPLIT ? 2 : 1;
-            for (int j0 = 0; j0 < w.nt; j0 += STEP) {
+            for (int j0 = 0; ok && j0 < w.nt; j0 += STEP) {
                 const int m = min(STEP, w.nt - j0);
-                for (int k = 0; k < 2 * m; k++, c++) {
+                for (int k = 0; ok && k < 2 * m; k++) {
                     const bool is_v = k >= m;
                     const int jj = is_v ? k - m : k, base = w.k0 + (j0 + jj) * kWTile;
-                    const uint32_t slot = c % C::SLOTS;
+                    const uint32_t n = SPLIT && jj ? c[1]++ : c[0]++, slot = C::slot(jj, n);
                     // lane x: page of box x (positions base + x R ..); boxes past the unit are not loaded
                     const int p = base + lane * R;
                     int page = -1;
@@ -503,8 +539,8 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                             s_bad[((t + jj) & 7) * 4 + lane] = bits;
                         }
                         __syncwarp();
-                        if (c >= C::SLOTS) ok = __all_sync(kFull, ok && sy.wait(&empty[slot], (c / C::SLOTS - 1) & 1));
-                        if (!ok) continue;
+                        if (n >= C::RINGLEN) ok = __all_sync(kFull, sy.wait(&empty[slot], C::phase(n) ^ 1));
+                        if (!ok) break;
                         uint64_t *bar = scan ? &landed[slot] : &full[slot];
                         if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * (uint32_t)(R * 128 * C::HALVES));
                         __syncwarp();
@@ -513,9 +549,9 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
 #pragma unroll
                             for (int h = 0; h < C::HALVES; h++) tma_load4(dst + h * C::HALF, is_v ? &mv : &mk, h * 64, w.kh, p & ((1 << a.page_log) - 1), page, bar);
                     } else if (scan) {
-                        ok = ok && sy.wait(&landed[slot], phases >> slot & 1);
+                        ok = __all_sync(kFull, ok && sy.wait(&landed[slot], phases >> slot & 1));
                         phases ^= 1u << slot;
-                        for (int x = tid - 288; ok && x < kWTile * C::CH; x += 64) {
+                        for (int x = lane; ok && x < kWTile * C::CH; x += 32) {
                             const int r = x / C::CH, piece = x % C::CH;
                             if (base + r >= w.kmin && base + r <= seen && want == have) continue;
                             uint4 *pv = reinterpret_cast<uint4 *>(sm + C::RING + slot * C::TILE + (piece >> 3) * C::HALF + r * 128 +
@@ -527,21 +563,22 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                             }
                         }
                         fence_async_smem();
-                        asm volatile("bar.sync 1, 64;" ::: "memory");
-                        if (tid == 288) mbar_arrive(&full[slot]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[slot]);
                     }
                 }
                 t += m;
             }
         }
     } else {
-        // ---- the MMAs, by one thread
+        // ---- the MMAs of stream i, by one thread
+        const int i = warp - 10;
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_f16(kWTile, false), id_o = idesc_f16(D, true);
-            uint32_t c = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+            uint32_t c = 0, nq = 0, np = 0;                     // loads of the ring so far; phases of q_full, p_full
             bool ok = true;
-            auto score = [&](int i, uint32_t kc) {             // S_i = (hi + lo of Q_i) K^T
-                const uint32_t k = sm0 + C::RING + (kc % C::SLOTS) * C::TILE, q = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
+            auto score = [&](uint32_t n) {                     // S_i = (hi + lo of Q_i) K^T
+                const uint32_t k = sm0 + C::RING + C::slot(i, n) * C::TILE, q = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
 #pragma unroll
                 for (int term = 0; term < 2; term++)
 #pragma unroll
@@ -550,8 +587,8 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                         umma_f16_ss(tmem + i * kWTile, desc_sw128(q + term * C::TILE + o, 16, 1024), desc_sw128(k + o, 16, 1024), id_s, term || ks);
                     }
             };
-            auto weigh = [&](int i, uint32_t vc, bool first) { // O_i (+)= (hi + lo of P_i) V
-                const uint32_t v = sm0 + C::RING + (vc % C::SLOTS) * C::TILE;
+            auto weigh = [&](uint32_t n, bool first) {         // O_i (+)= (hi + lo of P_i) V
+                const uint32_t v = sm0 + C::RING + C::slot(i, n) * C::TILE;
 #pragma unroll
                 for (int term = 0; term < 2; term++)
 #pragma unroll
@@ -559,44 +596,57 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                         umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * kWTile + (ks >> 1) * 32 + term * 16 + (ks & 1) * 8,
                                     desc_sw128(v + ks * 2048, C::HALF, 1024), id_o, !first || term || ks);
             };
-            auto full_at = [&](uint32_t x) { return sy.wait(&full[x % C::SLOTS], (x / C::SLOTS) & 1); };
+            auto lock = [&]() {
+                uint32_t x = 0;
+                do {                                            // (reading costs less than trying)
+                    while (*(volatile int *)s_lock != 0 && ++x < kWSpin) {}
+                } while (atomicCAS(s_lock, 0, 1) != 0 && x < kWSpin);
+            };
+            auto unlock = [&]() { *(volatile int *)s_lock = 0; };
+            auto full_at = [&](uint32_t n) { return sy.wait(&full[C::slot(i, n)], C::phase(n)); };
             while (ok && work.next(w)) {
-                // step = one position tile for both streams, or (SPLIT) one for each; m: tiles of the step; loads c ..
-                auto tiles_of = [&](int j) { return SPLIT ? min(2, w.nt - j) : 1; };
-                auto streams_of = [&](int j) { return SPLIT ? min(2, w.nt - j) : w.tiles; };
-                for (int i = 0; i < streams_of(0) && ok; i++) {
-                    const uint32_t k = c + (SPLIT ? i : 0);
-                    if ((SPLIT || i == 0) && !(ok = full_at(k))) break;
-                    if ((!SPLIT || i == 0) && !(ok = sy.wait(&q_full[i], nq[i] & 1))) break;
-                    tc_fence_after();
-                    score(i, k);
-                    umma_commit(&s_full[i]);
-                    if (SPLIT || i == w.tiles - 1) umma_commit(&empty[k % C::SLOTS]);
-                }
-                nq[0]++;
-                if (w.tiles > 1) nq[1]++;
-                for (int j = 0; j < w.nt && ok; j += SPLIT ? 2 : 1) {
-                    const int m = tiles_of(j), jn = j + (SPLIT ? 2 : 1), more = jn < w.nt ? streams_of(jn) : 0;
-                    const uint32_t cn = c + 2 * m;
-                    for (int i = 0; i < streams_of(j) && ok; i++) {
-                        const uint32_t v = c + m + (SPLIT ? i : 0), k = cn + (SPLIT ? i : 0);
-                        if ((SPLIT || i == 0) && !(ok = full_at(v))) break;
-                        if (!(ok = sy.wait(&p_full[i], np[i]++ & 1))) break;
+                // this stream's position tiles; loads c + 2 j (K) and c + 2 j + 1 (V) of its ring are tile j of them
+                const int nt = SPLIT ? (w.nt + 1 - i) / 2 : w.nt;
+                if (SPLIT || i < w.tiles) {
+                    ok = sy.wait(&q_full[SPLIT ? 0 : i], nq++ & 1);
+                    if (ok && nt > 0 && (ok = full_at(c))) {
                         tc_fence_after();
-                        weigh(i, v, j == 0);
-                        if (SPLIT || i == w.tiles - 1) umma_commit(&empty[v % C::SLOTS]);
-                        if (i < more) {
-                            if ((SPLIT || i == 0) && !(ok = full_at(k))) break;
-                            score(i, k);
-                        }
+                        lock();
+                        score(c);
+                        unlock();
                         umma_commit(&s_full[i]);
-                        if (i < more && (SPLIT || i == w.tiles - 1)) umma_commit(&empty[k % C::SLOTS]);
+                        umma_commit(&empty[C::slot(i, c)]);
                     }
-                    c = cn;
+                    if (SPLIT && ok && nt == 0) mbar_arrive(q_free);
+                    if (SPLIT && ok && nt == 1) umma_commit(q_free);
+                    for (int j = 0; ok && j < nt; j++, c += 2) {
+                        const bool more = j + 1 < nt;
+                        if (!(ok = full_at(c + 1) && sy.wait(&p_full[i], np++ & 1))) break;
+                        tc_fence_after();
+                        lock();
+                        weigh(c + 1, j == 0);
+                        if (more) {
+                            if (!mbar_test_wait(&full[C::slot(i, c + 2)], C::phase(c + 2))) {      // K is late: not at the other's cost
+                                unlock();
+                                if (!(ok = full_at(c + 2))) break;
+                                lock();
+                            }
+                            score(c + 2);
+                        }
+                        unlock();
+                        umma_commit(&s_full[i]);
+                        umma_commit(&empty[C::slot(i, c + 1)]);
+                        if (more) umma_commit(&empty[C::slot(i, c + 2)]);
+                        if (SPLIT && j + 2 == nt) umma_commit(q_free);          // the last of the unit's reads of Q
+                    }
+                } else {                                        // one row tile: the other stream's loads are read once
+                    for (int x = 0; ok && x < 2 * nt; x++, c++)
+                        if ((ok = full_at(c))) mbar_arrive(&empty[C::slot(i, c)]);
                 }
             }
             if (!ok) {                                          // nothing of this CTA's is in flight when TMEM goes
                 umma_commit(drain);
+                *s_abort = 1;
                 for (uint32_t n = 0; n < kWSpin && !mbar_try_wait(drain, 0); n++) __nanosleep(32);
             }
         }
