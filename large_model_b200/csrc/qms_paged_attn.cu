@@ -1,12 +1,12 @@
 // qms_paged_attn.cu - causal grouped-query attention of a batch of new tokens over a paged KV cache on B200
 // (sm_100a); src/model.c:465-492 is the reference's, of one sequence over one contiguous cache.
 //
-// One pass over the positions with the running maximum and sum of the softmax, the two products on the
-// tensor cores with 22-bit operands: an fp32 operand x is split as x = hi + lo into two of the tensor
-// cores' types and the products with hi and lo are added in fp32. Over an fp16 cache K and V are
-// exact, so q and the weights split into two fp16 terms cost two mma.sync m16n8k16 per product (one
-// term alone would leave an error of 2^-12). Over an fp32 cache all four operands are split into two tf32 terms
-// and three m16n8k8 products are kept (lo * lo is below 2^-22).
+// One pass over the positions with the running maximum and sum of the softmax, the two products on the tensor
+// cores with 22-bit operands: an fp32 operand x, scaled by a power of two into fp16's range, is split as x = hi + lo
+// into two fp16 terms (one alone would leave an error of 2^-12), and their products are added in fp32.
+// Over an fp16 cache K and V are exact: two mma.sync m16n8k16 per product. Over an fp32 cache K and V are split too,
+// once per stage in shared memory, and three products kept (lo * lo is below 2^-22); the tf32 form of the same
+// (m16n8k8, three products, split in every warp) took about twice as long.
 #include <math.h>
 #include <string.h>
 
@@ -17,8 +17,8 @@
 
 namespace qms {
 
-constexpr int kPaStage = 64;          // positions per stage
 constexpr float kPaShift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
+constexpr int pa_stage(int type) { return type == QMS_T_F16 ? 64 : 32; }       // positions per stage: 32 KB of K and V
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -32,55 +32,59 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ float4 lds4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
-                   "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+// Biased exponent of the largest finite |value|, as an ordered integer: of one value (0 if it is not finite).
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
 }
+// Values whose largest has the biased exponent e go to 2^9 .. 2^10 when multiplied by 2^(up - 127), which
+// 2^(127 - up) undoes; both are normal numbers.
+__device__ __forceinline__ uint32_t scale_up(uint32_t e) { return e == 0 ? 127u : min(263u - e, 253u); }
+__device__ __forceinline__ float pow2_bits(uint32_t biased) { return __uint_as_float(biased << 23); }
+
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
-// A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows times WK = 4 / WR
-// groups of positions. K and V arrive in stages of 64 positions by cp.async (zeros where a position is
-// past the chunk or on a bad page); each warp scores its rows against its share of the stage, keeps its
-// own running (m, l, o), and the position groups are joined in shared memory at the end of the unit.
+// A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows x WK groups of
+// positions x WD parts of head_dim (in the second product; the first is done by each). K and V arrive in stages
+// by cp.async (zeros where a position is past the chunk or on a bad page; page ids are fetched a stage ahead of
+// the copies), each warp scores its rows against its share of the stage, keeps its own running (m, l, o), and the
+// position groups are joined in shared memory at the end of the unit.
 template <int D, typename KT, int WR>
 struct PaCfg {
     static constexpr bool F16 = sizeof(KT) == 2;
-    static constexpr int WK = 4 / WR, KW = kPaStage / WK, NT = KW / 8;       // positions and 8-position tiles per warp
-    static constexpr int CH = D * (int)sizeof(KT) / 16;                      // 16-byte pieces per row
-    // fp16 rows are dense with the pieces XOR-swizzled by the row (ldmatrix reads 8 rows at one piece);
-    // fp32 rows are padded so that the 8 lanes of a 16-byte read (K: 2 rows x 4 pieces, V: 4 rows two
-    // apart x 2 pieces) fall on different banks
-    static constexpr int KROW = D * (int)sizeof(KT) + (F16 ? 0 : 64), VROW = D * (int)sizeof(KT) + (F16 ? 0 : 16);
-    static constexpr int KB = KROW * kPaStage, STAGE = KB + VROW * kPaStage;
-    static constexpr int NS = F16 ? 3 : 2;
-    static constexpr int RED = WK > 1 ? 4 * 16 * (D + 2) * 4 : 0;            // the position groups' o, m, l
-    static constexpr int SMEM = NS * STAGE > RED ? NS * STAGE : RED;
+    static constexpr int PS = F16 ? 64 : 32;
+    static constexpr int WD = !F16 && WR == 1 ? 2 : 1, WK = 4 / WR / WD;
+    static constexpr int KW = PS / WK, NT = KW / 8, DW = D / WD;             // positions, 8-position tiles, output dims per warp
+    static constexpr int CH = D * (int)sizeof(KT) / 16, ROW = D * (int)sizeof(KT);      // a row as it comes: 16-byte pieces, bytes
+    static constexpr int STAGE = 2 * ROW * PS;                               // K, then V
+    // The tiles that the MMAs read: fp16 rows with their 16-byte pieces XOR-swizzled by the row (ldmatrix reads 8
+    // rows at one piece): the stages themselves, or (fp32) hi and lo of K, hi and lo of V after the ring.
+    static constexpr int HROW = 2 * D, HTILE = HROW * PS;
+    static constexpr int NS = WR == 1 || !F16 ? 2 : 3, MINB = WR == 1 && F16 ? 3 : 2;    // stages; CTAs per SM
+    static constexpr int CONV = NS * STAGE;
+    static constexpr int RED = WK > 1 ? WK * WR * 16 * (D + 2) * 4 : 0;      // the position groups' o, m, l
+    static constexpr int USED = CONV + (F16 ? 0 : 4 * HTILE), SMEM = USED > RED ? USED : RED;
 };
 
 // OWN: the sequences' own positions; else the shared ones. LAST: launched beside the kernel of the other kind,
 // whose end it waits for at its own end, so that what follows this kernel follows both.
 template <int D, typename KT, int WR>
-__global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const bool own, const bool last) {
+__global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(const PagedAttn A, const bool own, const bool last) {
     using C = PaCfg<D, KT, WR>;
     extern __shared__ __align__(1024) unsigned char sm[];
     __shared__ int s_pos[64];                     // position of each row of the tile (-1: none)
     __shared__ int s_tok[64];                     // token row * H + q head (-1: none)
-    __shared__ int s_bad[C::NS + 1][2];           // stage st's positions on bad pages, as a bit mask, at st % (NS + 1)
+    __shared__ int s_page[4][C::PS];              // stage st's page ids at st % 4 (-1: past the unit, or bad)
+    __shared__ int s_bad[4][2];                   // its positions on bad pages, as a bit mask
+    __shared__ uint32_t s_max[4][2];              // largest |K| and |V| of a stage (fp32), by warp
     __shared__ int s_flag;                        // V had values that are not finite behind the mask
     const Paged &a = A.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
-    const int wr = warp % WR, wk = warp / WR;
+    const int wr = warp % WR, wk = warp / WR % C::WK, wd = warp / WR / C::WK;
     const uint32_t sm0 = smem_u32(sm);
     // the trigger comes after the wait: a kernel that starts on it may read what this one waited for
     if (!last) pdl_wait();
@@ -108,11 +112,23 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             k1 = min(a.prefix, k0 + A.p.chunk_p);
         }
         const int *table = a.table + (own ? (int64_t)b * a.table_stride : 0);
-        __syncthreads();                          // the previous unit is done with shared memory
-        if (tid == 0) s_flag = 0;
-        if (tid < 2 * (C::NS + 1)) (&s_bad[0][0])[tid] = 0;
-        // rows of the tile: the sequence's own, or all tokens' (each token's sequence found by a warp)
+        // page id and bad-page bit of position `i` of stage st, by one thread per position
+        auto page_of = [&](int st, int i) {
+            const int p = k0 + st * C::PS + i;
+            return p < k1 ? table[p >> a.page_log] : -2;
+        };
+        auto put_page = [&](int st, int i, int page) {
+            const bool bad = page != -2 && (unsigned)page >= (unsigned)a.n_pages;
+            s_page[st & 3][i] = bad || page == -2 ? -1 : page;
+            const unsigned bits = __ballot_sync(kFull, bad);
+            if (lane == 0) s_bad[st & 3][i >> 5] = (int)bits;
+            if (bad) paged_err(a, QMS_PAGED_EPAGE);
+        };
         const int r0 = tile * 16 * WR;
+        __syncthreads();                          // the previous unit is done with shared memory
+        for (int i = tid; i < C::NS * C::PS; i += 128) put_page(i / C::PS, i % C::PS, page_of(i / C::PS, i % C::PS));
+        if (tid == 0) s_flag = 0;
+        // rows of the tile: the sequence's own, or all tokens' (each token's sequence found by a warp)
         if (own) {
             if (tid < 16 * WR) {
                 const int r = r0 + tid, i = r / a.G;
@@ -120,8 +136,8 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
                 s_tok[tid] = i < n ? (t0 + i) * a.H + kh * a.G + (r - i * a.G) : -1;
             }
         } else {
-            const int first = r0 / a.G, last = min(a.n_tok, (r0 + 16 * WR + a.G - 1) / a.G);
-            for (int t = first + warp; t < last; t += 4) {
+            const int first = r0 / a.G, end = min(a.n_tok, (r0 + 16 * WR + a.G - 1) / a.G);
+            for (int t = first + warp; t < end; t += 4) {
                 int s0 = 0, sn = 0, skv = 0;
                 const int sb = paged_seq_of(a, t);
                 if (sb < a.n_seq && !paged_seq(a, sb, s0, sn, skv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
@@ -137,69 +153,61 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             if (tid < 16 * WR && r0 + tid >= a.n_tok * a.G) s_pos[tid] = s_tok[tid] = -1;
         }
         __syncthreads();
+        auto load = [&](int st) {                 // stage st of the unit into its slot
+            const int base = k0 + st * C::PS;
+            const uint32_t dk = sm0 + st % C::NS * C::STAGE, dv = dk + C::STAGE / 2;
+#pragma unroll
+            for (int i = tid; i < C::PS * C::CH; i += 128) {
+                const int r = i / C::CH, c = i % C::CH, page = s_page[st & 3][r];
+                const int64_t off = page < 0 ? 0 : page * a.page_stride + ((base + r) & ((1 << a.page_log) - 1)) * a.pos_stride + kh * a.head_stride + c * 16;
+                const int cs = C::F16 ? c ^ (r & 7) : c;
+                cp_async16_or0(dk + r * C::ROW + cs * 16, a.k + off, page >= 0);
+                cp_async16_or0(dv + r * C::ROW + cs * 16, a.v + off, page >= 0);
+            }
+        };
         int lo_pos = 0x7fffffff, hi_pos = -1;     // least and largest position among the tile's rows
-        for (int r = 0; r < 16 * WR; r++) {
+        for (int r = lane; r < 16 * WR; r += 32) {
             const int p = s_pos[r];
             if (p >= 0) lo_pos = min(lo_pos, p);
             hi_pos = max(hi_pos, p);
         }
-        k1 = min(k1, hi_pos + 1);                 // nobody sees the rest
-        if (k0 >= k1) continue;
-        const int nst = (k1 - k0 + kPaStage - 1) / kPaStage;
-
-        auto load = [&](int st) {                 // stage st of the unit into its slot
-            const int slot_i = st % C::NS, base = k0 + st * kPaStage;
-            const uint32_t dk = sm0 + slot_i * C::STAGE, dv = dk + C::KB;
-#pragma unroll 4
-            for (int i = tid; i < kPaStage * C::CH; i += 128) {
-                const int r = i / C::CH, c = i % C::CH, p = base + r;
-                int64_t at = -1;
-                if (p < k1) {
-                    at = paged_at(a, table, p);
-                    if (at < 0 && c == 0) {
-                        atomicOr(&s_bad[st % (C::NS + 1)][r >> 5], 1 << (r & 31));
-                        paged_err(a, QMS_PAGED_EPAGE);
-                    }
-                }
-                const int64_t off = at < 0 ? 0 : at + kh * a.head_stride + c * 16;
-                const int cs = C::F16 ? c ^ (r & 7) : c;
-                cp_async16_or0(dk + r * C::KROW + cs * 16, a.k + off, at >= 0);
-                cp_async16_or0(dv + r * C::VROW + cs * 16, a.v + off, at >= 0);
-            }
-        };
+        lo_pos = __reduce_min_sync(kFull, lo_pos);
+        hi_pos = __reduce_max_sync(kFull, hi_pos);
+        if (k0 > hi_pos) continue;                // nobody sees any of it
+        const int k_end = min(k1, hi_pos + 1), nst = (k_end - k0 + C::PS - 1) / C::PS;
+#pragma unroll
         for (int st = 0; st < C::NS - 1; st++) {
             if (st < nst) load(st);
             cp_commit();
         }
 
-        // ---- q: this thread's elements of rows g and g + 8 of its row group, as mma A fragments
+        // ---- q: this thread's elements of rows g and g + 8 of its row group, as mma A fragments, each row scaled by a
+        // power of two into fp16's range (exact), undone in the score's factor
         const int tok0 = s_tok[wr * 16 + g], tok1 = s_tok[wr * 16 + g + 8];
         const int pos0 = s_pos[wr * 16 + g], pos1 = s_pos[wr * 16 + g + 8];
-        const int64_t qo0 = tok0 < 0 ? -1 : (tok0 / a.H) * A.ldq + (int64_t)(tok0 % a.H) * D;
-        const int64_t qo1 = tok1 < 0 ? -1 : (tok1 / a.H) * A.ldq + (int64_t)(tok1 % a.H) * D;
-        float f0 = A.scale2, f1 = A.scale2;       // score factors of the two rows
-        uint32_t qh[C::F16 ? D / 16 : 1][4], ql[C::F16 ? D / 16 : 1][4];
-        float qf[C::F16 ? 1 : D / 8][4];
-        if constexpr (C::F16) {
-            // each row scaled by a power of two into fp16's range (exact), undone in the score's factor
-            float x[2][D / 4], mx[2] = {0.0f, 0.0f};
+        float f0, f1;
+        uint32_t qh[D / 16][4], ql[D / 16][4];
+        {
+            float x[2][D / 4];
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const int64_t qo = r ? qo1 : qo0;
+                const int tok = r ? tok1 : tok0;
+                const float *src = A.q + (tok < 0 ? 0 : (tok / a.H) * A.ldq + (int64_t)(tok % a.H) * D) + tq * 2;
+                uint32_t mx = 0;
 #pragma unroll
                 for (int i = 0; i < D / 8; i++) {
-                    const float2 v = qo < 0 ? make_float2(0.0f, 0.0f) : __ldcg(reinterpret_cast<const float2 *>(A.q + qo + i * 8 + tq * 2));
+                    const float2 v = tok < 0 ? make_float2(0.0f, 0.0f) : __ldcg(reinterpret_cast<const float2 *>(src + i * 8));
                     x[r][2 * i] = v.x;
                     x[r][2 * i + 1] = v.y;
-                    mx[r] = fmaxf(mx[r], fmaxf(fabsf(v.x), fabsf(v.y)));
+                    mx = max(mx, max(finite_bits(v.x), finite_bits(v.y)));
                 }
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(kFull, mx[r], 1));
-                mx[r] = fmaxf(mx[r], __shfl_xor_sync(kFull, mx[r], 2));
-                const int e = mx[r] > 0.0f && mx[r] < INFINITY ? ilogbf(mx[r]) - 9 : 0;
-                (r ? f1 : f0) = ldexpf(A.scale2, e);
-                const float dn1 = ldexpf(1.0f, -e / 2), dn2 = ldexpf(1.0f, -e - -e / 2);   // 2^-e may not be a float
+                mx = max(mx, __shfl_xor_sync(kFull, mx, 1));
+                mx = max(mx, __shfl_xor_sync(kFull, mx, 2));
+                const uint32_t up = scale_up(mx >> 23);
+                (r ? f1 : f0) = A.scale2 * pow2_bits(254u - up);
+                const float m = pow2_bits(up);
 #pragma unroll
-                for (int i = 0; i < D / 4; i++) x[r][i] = x[r][i] * dn1 * dn2;
+                for (int i = 0; i < D / 4; i++) x[r][i] *= m;
             }
 #pragma unroll
             for (int ks = 0; ks < D / 16; ks++) {
@@ -208,113 +216,127 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
                 split_h2(x[0][4 * ks + 2], x[0][4 * ks + 3], qh[ks][2], ql[ks][2]);
                 split_h2(x[1][4 * ks + 2], x[1][4 * ks + 3], qh[ks][3], ql[ks][3]);
             }
-        } else {
-            // the contraction's order is free: lane tq takes dims 16 i + 4 tq .. + 3, a 16-byte read of K
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float4 v0 = qo0 < 0 ? z : __ldcg(reinterpret_cast<const float4 *>(A.q + qo0 + i * 16 + tq * 4));
-                const float4 v1 = qo1 < 0 ? z : __ldcg(reinterpret_cast<const float4 *>(A.q + qo1 + i * 16 + tq * 4));
-                qf[2 * i][0] = v0.x, qf[2 * i][1] = v1.x, qf[2 * i][2] = v0.y, qf[2 * i][3] = v1.y;
-                qf[2 * i + 1][0] = v0.z, qf[2 * i + 1][1] = v1.z, qf[2 * i + 1][2] = v0.w, qf[2 * i + 1][3] = v1.w;
-            }
         }
 
-        float o[D / 8][4];
+        float o[C::DW / 8][4];
 #pragma unroll
-        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < C::DW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        uint32_t v_exp = 0;                       // fp32: largest exponent of V so far; o is in units of its scale
 
         for (int st = 0; st < nst; st++) {
             cp_wait<C::NS - 2>();
             __syncthreads();                      // the stage has landed; the slot before it is free
-            const int slot_i = st % C::NS, base = k0 + st * kPaStage;
-            const uint32_t kb = sm0 + slot_i * C::STAGE, vb = kb + C::KB;
-            const int bad0 = s_bad[st % (C::NS + 1)][0], bad1 = s_bad[st % (C::NS + 1)][1];
-            const bool masked = base + kPaStage - 1 > lo_pos || base + kPaStage > k1 || bad0 || bad1;
-            if (base + kPaStage - 1 > lo_pos) {
-                // behind the causal mask a weight is 0, but 0 * inf is not: such V are set aside
-                bool any = false;
-                for (int i = tid; i < kPaStage * C::CH; i += 128) {
-                    const int r = i / C::CH, c = i % C::CH;
-                    if (base + r <= lo_pos) continue;
-                    uint4 *pv = reinterpret_cast<uint4 *>(sm + slot_i * C::STAGE + C::KB + r * C::VROW + c * 16);
-                    uint4 v = *pv;
-                    if (drop_nonfinite((const KT *)nullptr, v)) {
-                        *pv = v;
-                        any = true;
-                    }
-                }
-                if (any) s_flag = 1;
-                __syncthreads();
-            }
-            if (tid < 2) s_bad[(st + C::NS) % (C::NS + 1)][tid] = 0;      // the mask that the next iteration fills
+            const int base = k0 + st * C::PS, next = st + C::NS;
             if (st + C::NS - 1 < nst) load(st + C::NS - 1);
             cp_commit();
+            const int page_next = next < nst && tid < C::PS ? page_of(next, tid) : -2;
+            const int bad0 = s_bad[st & 3][0], bad1 = C::PS > 32 ? s_bad[st & 3][1] : 0;
+            const bool behind = base + C::PS - 1 > lo_pos;         // some row does not see all of it
+            const bool masked = behind || base + C::PS > k1 || bad0 || bad1;
+            unsigned char *raw = sm + st % C::NS * C::STAGE;
+            uint32_t kb = sm0 + st % C::NS * C::STAGE, vb = kb + C::STAGE / 2;
+            float fk = 1.0f;                      // undoes the scale of this stage's K
+            if constexpr (C::F16) {
+                if (behind) {                     // behind the causal mask a weight is 0, but 0 * inf is not
+                    bool any = false;
+                    for (int i = tid; i < C::PS * C::CH; i += 128) {
+                        if (base + i / C::CH <= lo_pos) continue;
+                        uint4 *pv = reinterpret_cast<uint4 *>(raw + C::STAGE / 2) + i;
+                        uint4 v = *pv;
+                        if (drop_nonfinite((const KT *)nullptr, v)) {
+                            *pv = v;
+                            any = true;
+                        }
+                    }
+                    if (any) s_flag = 1;
+                    __syncthreads();
+                }
+            } else {
+                // hi and lo of K and V: the stage's largest values, then scaled and split
+                constexpr int N = C::PS * C::CH / 128;             // 16-byte pieces of K (and of V) per thread
+                float4 x[2][N];
+                uint32_t mx[2] = {0, 0};
+#pragma unroll
+                for (int w = 0; w < 2; w++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int at = tid + 128 * i;
+                        x[w][i] = *reinterpret_cast<const float4 *>(raw + w * (C::STAGE / 2) + at * 16);
+                        if (w == 1 && behind && base + at / C::CH > lo_pos) {
+                            uint4 v = *reinterpret_cast<const uint4 *>(&x[w][i]);
+                            if (drop_nonfinite((const KT *)nullptr, v)) {
+                                x[w][i] = *reinterpret_cast<const float4 *>(&v);
+                                s_flag = 1;
+                            }
+                        }
+                        mx[w] = max(mx[w], max(max(finite_bits(x[w][i].x), finite_bits(x[w][i].y)), max(finite_bits(x[w][i].z), finite_bits(x[w][i].w))));
+                    }
+                mx[0] = __reduce_max_sync(kFull, mx[0]);
+                mx[1] = __reduce_max_sync(kFull, mx[1]);
+                if (lane == 0) s_max[warp][0] = mx[0], s_max[warp][1] = mx[1];
+                __syncthreads();                  // (and the tiles of the last stage are no longer read)
+                const uint32_t ke = max(max(s_max[0][0], s_max[1][0]), max(s_max[2][0], s_max[3][0])) >> 23;
+                const uint32_t ve = max(max(max(s_max[0][1], s_max[1][1]), max(s_max[2][1], s_max[3][1])) >> 23, v_exp);
+                if (ve != v_exp) {
+                    const uint32_t down = scale_up(v_exp) - scale_up(ve);
+                    const float d = down > 126 ? 0.0f : pow2_bits(127u - down);
+                    if (v_exp != 0)               // (before, o is 0)
+#pragma unroll
+                        for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
+                    v_exp = ve;
+                }
+                fk = pow2_bits(254u - scale_up(ke));
+                const float up[2] = {pow2_bits(scale_up(ke)), pow2_bits(scale_up(ve))};
+#pragma unroll
+                for (int w = 0; w < 2; w++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int at = tid + 128 * i, r = at / C::CH, c = at % C::CH;      // values 4 c .. + 3 of row r
+                        uint32_t h[2], l[2];
+                        split_h2(x[w][i].x * up[w], x[w][i].y * up[w], h[0], l[0]);
+                        split_h2(x[w][i].z * up[w], x[w][i].w * up[w], h[1], l[1]);
+                        unsigned char *to = sm + C::CONV + w * 2 * C::HTILE + r * C::HROW + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+                        *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
+                        *reinterpret_cast<uint2 *>(to + C::HTILE) = make_uint2(l[0], l[1]);
+                    }
+                __syncthreads();
+                kb = sm0 + C::CONV;
+                vb = kb + 2 * C::HTILE;
+            }
 
             // ---- scores
-            float s[C::NT][4];
-            if constexpr (C::F16) {
-                float s2[C::NT][4];
+            float s[C::NT][4], s2[C::NT][4];
 #pragma unroll
-                for (int i = 0; i < C::NT; i++)
+            for (int i = 0; i < C::NT; i++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s[i][j] = s2[i][j] = 0.0f;
+                for (int j = 0; j < 4; j++) s[i][j] = s2[i][j] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ks++)
+            for (int ks = 0; ks < D / 16; ks++)
 #pragma unroll
-                    for (int i = 0; i < C::NT / 2; i++) {
-                        const int r = wk * C::KW + i * 16 + ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
-                        uint32_t kf[4];
-                        ldsm4(kf, kb + r * C::KROW + ((c ^ (r & 7)) << 4));
-                        mma_f16(s[2 * i], qh[ks], kf[0], kf[1]);
-                        mma_f16(s[2 * i + 1], qh[ks], kf[2], kf[3]);
-                        mma_f16(s2[2 * i], ql[ks], kf[0], kf[1]);
-                        mma_f16(s2[2 * i + 1], ql[ks], kf[2], kf[3]);
-                    }
-#pragma unroll
-                for (int i = 0; i < C::NT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[i][j] += s2[i][j];
-            } else {
-                float s2[C::NT][4];
-#pragma unroll
-                for (int i = 0; i < C::NT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[i][j] = s2[i][j] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ks++) {
-                    float ah[2][4], al[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            ah[h][j] = tf32_hi(qf[2 * ks + h][j]);
-                            al[h][j] = qf[2 * ks + h][j] - ah[h][j];
-                        }
-#pragma unroll
-                    for (int i = 0; i < C::NT; i++) {
-                        const float4 k = lds4(kb + (wk * C::KW + i * 8 + g) * C::KROW + ks * 64 + tq * 16);
-                        const float h0 = tf32_hi(k.x), h1 = tf32_hi(k.y), h2 = tf32_hi(k.z), h3 = tf32_hi(k.w);
-                        mma_tf32(s2[i], ah[0], k.x - h0, k.y - h1);
-                        mma_tf32(s2[i], al[0], h0, h1);
-                        mma_tf32(s[i], ah[0], h0, h1);
-                        mma_tf32(s2[i], ah[1], k.z - h2, k.w - h3);
-                        mma_tf32(s2[i], al[1], h2, h3);
-                        mma_tf32(s[i], ah[1], h2, h3);
+                for (int i = 0; i < C::NT / 2; i++) {
+                    const int r = wk * C::KW + i * 16 + ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
+                    const uint32_t at = kb + r * C::HROW + ((c ^ (r & 7)) << 4);
+                    uint32_t kf[4];
+                    ldsm4(kf, at);
+                    mma_f16(s[2 * i], qh[ks], kf[0], kf[1]);
+                    mma_f16(s[2 * i + 1], qh[ks], kf[2], kf[3]);
+                    mma_f16(s2[2 * i], ql[ks], kf[0], kf[1]);
+                    mma_f16(s2[2 * i + 1], ql[ks], kf[2], kf[3]);
+                    if constexpr (!C::F16) {
+                        ldsm4(kf, at + C::HTILE);
+                        mma_f16(s2[2 * i], qh[ks], kf[0], kf[1]);
+                        mma_f16(s2[2 * i + 1], qh[ks], kf[2], kf[3]);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < C::NT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[i][j] += s2[i][j];
-            }
             // ---- softmax of the stage: s becomes the weights
+            const float g0 = f0 * fk, g1 = f1 * fk;
             float n0 = m0, n1 = m1;
 #pragma unroll
             for (int i = 0; i < C::NT; i++) {
                 const int r = wk * C::KW + i * 8 + tq * 2, p = base + r;
-                s[i][0] *= f0, s[i][1] *= f0, s[i][2] *= f1, s[i][3] *= f1;
+                s[i][0] = (s[i][0] + s2[i][0]) * g0, s[i][1] = (s[i][1] + s2[i][1]) * g0;
+                s[i][2] = (s[i][2] + s2[i][2]) * g1, s[i][3] = (s[i][3] + s2[i][3]) * g1;
                 if (masked) {
                     const int bm = (r < 32 ? bad0 : bad1) >> (r & 31);
                     const bool ok0 = p < k1 && !(bm & 1), ok1 = p + 1 < k1 && !(bm & 2);
@@ -331,13 +353,12 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             n0 = fmaxf(n0, __shfl_xor_sync(kFull, n0, 2));
             n1 = fmaxf(n1, __shfl_xor_sync(kFull, n1, 2));
             const float b0 = n0 == -INFINITY ? 0.0f : n0 - kPaShift, b1 = n1 == -INFINITY ? 0.0f : n1 - kPaShift;
-            const float c0 = ex2(m0 - n0), c1 = ex2(m1 - n1);      // NaN only while nothing was seen: o and l are 0
             if (n0 != m0 || n1 != m1) {
-                const float d0 = m0 == -INFINITY ? 0.0f : c0, d1 = m1 == -INFINITY ? 0.0f : c1;
+                const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
                 l0 *= d0;
                 l1 *= d1;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
+                for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
             }
             m0 = n0;
             m1 = n1;
@@ -349,55 +370,41 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
                 l1 += s[i][2] + s[i][3];
             }
             // ---- o += weights * V
-            if constexpr (C::F16) {
 #pragma unroll
-                for (int kk = 0; kk < C::NT / 2; kk++) {
-                    uint32_t ph[4], pl[4];
-                    split_h2(s[2 * kk][0], s[2 * kk][1], ph[0], pl[0]);
-                    split_h2(s[2 * kk][2], s[2 * kk][3], ph[1], pl[1]);
-                    split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[2], pl[2]);
-                    split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[3], pl[3]);
+            for (int kk = 0; kk < C::NT / 2; kk++) {
+                uint32_t ph[4], pl[4];
+                split_h2(s[2 * kk][0], s[2 * kk][1], ph[0], pl[0]);
+                split_h2(s[2 * kk][2], s[2 * kk][3], ph[1], pl[1]);
+                split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[2], pl[2]);
+                split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[3], pl[3]);
 #pragma unroll
-                    for (int j = 0; j < D / 16; j++) {
-                        const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = 2 * j + (lane >> 4);
-                        uint32_t vf[4];
-                        ldsm4t(vf, vb + r * C::VROW + ((c ^ (r & 7)) << 4));
+                for (int j = 0; j < C::DW / 16; j++) {
+                    const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = wd * (C::DW / 8) + 2 * j + (lane >> 4);
+                    const uint32_t at = vb + r * C::HROW + ((c ^ (r & 7)) << 4);
+                    uint32_t vf[4];
+                    ldsm4t(vf, at);
+                    mma_f16(o[2 * j], ph, vf[0], vf[1]);
+                    mma_f16(o[2 * j + 1], ph, vf[2], vf[3]);
+                    mma_f16(o[2 * j], pl, vf[0], vf[1]);
+                    mma_f16(o[2 * j + 1], pl, vf[2], vf[3]);
+                    if constexpr (!C::F16) {
+                        ldsm4t(vf, at + C::HTILE);
                         mma_f16(o[2 * j], ph, vf[0], vf[1]);
                         mma_f16(o[2 * j + 1], ph, vf[2], vf[3]);
-                        mma_f16(o[2 * j], pl, vf[0], vf[1]);
-                        mma_f16(o[2 * j + 1], pl, vf[2], vf[3]);
-                    }
-                }
-            } else {
-                // positions 2 tq, 2 tq + 1 of an 8-position tile are the fragment's k = tq, tq + 4; column g of
-                // output tile 4 j + c is dim 32 j + 4 g + c, so V too is read 16 bytes at a time
-#pragma unroll
-                for (int i = 0; i < C::NT; i++) {
-                    const float ah[4] = {tf32_hi(s[i][0]), tf32_hi(s[i][2]), tf32_hi(s[i][1]), tf32_hi(s[i][3])};
-                    const float al[4] = {s[i][0] - ah[0], s[i][2] - ah[1], s[i][1] - ah[2], s[i][3] - ah[3]};
-                    const uint32_t vr = vb + (wk * C::KW + i * 8 + tq * 2) * C::VROW + g * 16;
-#pragma unroll
-                    for (int j = 0; j < D / 32; j++) {
-                        const float4 x = lds4(vr + j * 128), y = lds4(vr + C::VROW + j * 128);
-                        const float xv[4] = {x.x, x.y, x.z, x.w}, yv[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const float xh = tf32_hi(xv[c]), yh = tf32_hi(yv[c]);
-                            mma_tf32(o[4 * j + c], ah, xv[c] - xh, yv[c] - yh);
-                            mma_tf32(o[4 * j + c], al, xh, yh);
-                            mma_tf32(o[4 * j + c], ah, xh, yh);
-                        }
                     }
                 }
             }
+            if (next < nst && tid < C::PS) put_page(next, tid, page_next);       // whole warps
         }
         cp_wait<0>();
         __syncthreads();                          // every warp is done with the stages
+        if constexpr (!C::F16) {
+            const float d = pow2_bits(254u - scale_up(v_exp));
+#pragma unroll
+            for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
+        }
         // dims of this thread's o[i][0..1] (row g) and o[i][2..3] (row g + 8)
-        auto dim = [&](int i, int j) {
-            if constexpr (C::F16) return i * 8 + tq * 2 + (j & 1);
-            else return (i >> 2) * 32 + (i & 3) + 4 * (tq * 2 + (j & 1));
-        };
+        auto dim = [&](int i, int j) { return wd * C::DW + i * 8 + tq * 2 + (j & 1); };
         if (s_flag && wk == 0) {
             // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
             for (int p = max(k0, lo_pos + 1); p < k1; p++) {
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
                 if (at < 0) continue;
                 const KT *vr = reinterpret_cast<const KT *>(a.v + at + kh * a.head_stride);
 #pragma unroll
-                for (int i = 0; i < D / 8; i++)
+                for (int i = 0; i < C::DW / 8; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const float v = kv_ld(vr + dim(i, j));
@@ -428,9 +435,9 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
                 if (tok < 0) continue;
                 float *dst = A.part_o + (po + tok) * D;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) dst[dim(i, j)] = m == -INFINITY ? 0.0f : o[i][2 * r + j];
+                for (int i = 0; i < C::DW / 8; i++)
+                    *reinterpret_cast<float2 *>(dst + dim(i, 0)) =
+                        m == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(o[i][2 * r], o[i][2 * r + 1]);
                 if (tq == 0) A.part_ml[po + tok] = make_float2(m == -INFINITY ? m : m - kPaShift, l);
             }
         } else {
@@ -441,10 +448,8 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             for (int r = 0; r < 2; r++) {
                 float *dst = red + ((wk * WR + wr) * 16 + g + 8 * r) * LD;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) dst[dim(i, j)] = o[i][2 * r + j];
-                if (tq == 0) {
+                for (int i = 0; i < C::DW / 8; i++) *reinterpret_cast<float2 *>(dst + dim(i, 0)) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+                if (tq == 0 && wd == 0) {
                     dst[D] = r ? m1 : m0;
                     dst[D + 1] = r ? l1 : l0;
                 }
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
             for (int r = warp; r < 16 * WR; r += 4) {
                 const int tok = s_tok[r];
                 if (tok < 0) continue;
-                float m = -INFINITY, l = 0.0f, x[D / 32], w[C::WK];
+                float m = -INFINITY, l = 0.0f, x[D / 32];
 #pragma unroll
                 for (int k = 0; k < C::WK; k++) m = fmaxf(m, red[(k * 16 * WR + r) * LD + D]);
 #pragma unroll
@@ -462,11 +467,11 @@ __global__ void __launch_bounds__(128) k_paged_attn(const PagedAttn A, const boo
 #pragma unroll
                     for (int k = 0; k < C::WK; k++) {
                         const float *src = red + (k * 16 * WR + r) * LD;
-                        w[k] = ex2(src[D] - m);
-                        if (w[k] == 0.0f && src[D + 1] == 0.0f) continue;      // saw nothing: its o may be 0 * inf
-                        l = fmaf(w[k], src[D + 1], l);
+                        const float w = ex2(src[D] - m);
+                        if (w == 0.0f && src[D + 1] == 0.0f) continue;         // saw nothing: its o may be 0 * inf
+                        l = fmaf(w, src[D + 1], l);
 #pragma unroll
-                        for (int d = 0; d < D / 32; d++) x[d] = fmaf(w[k], src[lane + 32 * d], x[d]);
+                        for (int d = 0; d < D / 32; d++) x[d] = fmaf(w, src[lane + 32 * d], x[d]);
                     }
                 }
 #pragma unroll
@@ -573,8 +578,8 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
 static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, 128, 148, 3.0, 6.0);
     if (wr == kPaWideSplit) return chunk_of(len, tiles, 2 * rows, 256, 148, 3.0, 6.0);
-    const double slow = type == QMS_T_F16 ? 1.0 : 2.0;
-    return chunk_of(len, tiles, rows, kPaStage, 148 * (type == QMS_T_F16 ? 2 : 1), slow * 0.7, 4.0);
+    const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
+    return chunk_of(len, tiles, rows, pa_stage(type), 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0);
 }
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
