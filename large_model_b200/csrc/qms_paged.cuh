@@ -1,6 +1,8 @@
 // qms_paged.cuh - the paged KV cache as the kernels see it (qms_paged*.cu). Not part of the C ABI.
 #pragma once
 
+#include <cuda.h>
+
 #include "qms_kv.cuh"
 
 namespace qms {
@@ -54,14 +56,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// 16 bytes global -> shared, or 16 zero bytes.
-__device__ __forceinline__ void cp_async16_or0(uint32_t dst, const void *src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
@@ -76,6 +74,13 @@ __device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_
 }
 // x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
+// A box of a paged pool: values from x of one head, the positions of the map's box from y of a page.
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int head, int y, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(head), "r"(y), "r"(page), "r"(smem_u32(bar))
+                 : "memory");
+}
 
 // Zero what is not finite in a 16-byte piece of V; true if something was.
 __device__ __forceinline__ bool drop_nonfinite(const __half *, uint4 &v) {
@@ -148,6 +153,9 @@ struct PagedAttn {
     float2 *part_ml;
 };
 
+// The pool as a tensor [page][position][head][value], in boxes of up to `rows` positions of a page: 64 fp16 values, 128-byte
+// swizzled, or a whole fp32 row.
+int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map);
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p);
 int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p);
 int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s);     // qms_paged_wide.cu

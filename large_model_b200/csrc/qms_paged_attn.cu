@@ -17,6 +17,7 @@
 
 namespace qms {
 
+constexpr uint32_t kPaSpin = 1u << 22;
 constexpr float kPaShift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
 constexpr int pa_stage(int type) { return type == QMS_T_F16 ? 64 : 32; }       // positions per stage: 32 KB of K and V
 
@@ -49,10 +50,11 @@ __device__ __forceinline__ float pow2_bits(uint32_t biased) { return __uint_as_f
 
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
 // A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows x WK groups of
-// positions x WD parts of head_dim (in the second product; the first is done by each). K and V arrive in stages
-// by cp.async (zeros where a position is past the chunk or on a bad page; page ids are fetched a stage ahead of
-// the copies), each warp scores its rows against its share of the stage, keeps its own running (m, l, o), and the
-// position groups are joined in shared memory at the end of the unit.
+// positions x WD parts of head_dim (in the second product; the first is done by each). K and V come in
+// by TMA, a stage of positions at a time, one box per page (cp.async cost some 2000 of 4300 cycles per stage in
+// issuing alone); stages start on page boundaries, so the first may begin before the unit's first position, and boxes
+// past the unit or on bad pages are not loaded: all that is masked. Each warp scores its rows against its share
+// of the stage, keeps its own running (m, l, o), and the position groups are joined in shared memory at the end.
 template <int D, typename KT, int WR>
 struct PaCfg {
     static constexpr bool F16 = sizeof(KT) == 2;
@@ -61,31 +63,45 @@ struct PaCfg {
     static constexpr int KW = PS / WK, NT = KW / 8, DW = D / WD;             // positions, 8-position tiles, output dims per warp
     static constexpr int CH = D * (int)sizeof(KT) / 16, ROW = D * (int)sizeof(KT);      // a row as it comes: 16-byte pieces, bytes
     static constexpr int STAGE = 2 * ROW * PS;                               // K, then V
-    // The tiles that the MMAs read: fp16 rows with their 16-byte pieces XOR-swizzled by the row (ldmatrix reads 8
-    // rows at one piece): the stages themselves, or (fp32) hi and lo of K, hi and lo of V after the ring.
-    static constexpr int HROW = 2 * D, HTILE = HROW * PS;
+    // The tiles that the MMAs read: fp16 rows in halves of 64 values (128 bytes), their 16-byte pieces XOR-swizzled by the
+    // row (ldmatrix reads 8 rows at one piece): the stages themselves, or (fp32) hi and lo of K, hi and lo of V
+    // after the ring.
+    static constexpr int HTILE = 2 * D * PS, HALF = 128 * PS;
+    static __device__ __forceinline__ uint32_t piece(int r, int c) { return (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
     static constexpr int NS = WR == 1 || !F16 ? 2 : 3, MINB = WR == 1 && F16 ? 3 : 2;    // stages; CTAs per SM
     static constexpr int CONV = NS * STAGE;
-    static constexpr int RED = WK > 1 ? WK * WR * 16 * (D + 2) * 4 : 0;      // the position groups' o, m, l
-    static constexpr int USED = CONV + (F16 ? 0 : 4 * HTILE), SMEM = USED > RED ? USED : RED;
+    static constexpr int RED = WK > 1 ? WK * WR * 16 * (D + 4) * 4 : 0;      // the position groups' o, m, l
+    static constexpr int USED = CONV + (F16 ? 0 : 4 * HTILE), SMEM = (USED > RED ? USED : RED) + 1024;    // (1024: alignment)
+    static constexpr int QROWS = 16 * WR, QHALF = 128 * QROWS;               // the tile's q, as HTILE: hi, lo
 };
 
 // OWN: the sequences' own positions; else the shared ones. LAST: launched beside the kernel of the other kind,
 // whose end it waits for at its own end, so that what follows this kernel follows both.
 template <int D, typename KT, int WR>
-__global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(const PagedAttn A, const bool own, const bool last) {
+__global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(const PagedAttn A, const __grid_constant__ CUtensorMap mk,
+                                                                               const __grid_constant__ CUtensorMap mv, const bool own, const bool last) {
     using C = PaCfg<D, KT, WR>;
-    extern __shared__ __align__(1024) unsigned char sm[];
+    extern __shared__ unsigned char sm_[];
+    __shared__ uint64_t s_full[C::NS];
     __shared__ int s_pos[64];                     // position of each row of the tile (-1: none)
     __shared__ int s_tok[64];                     // token row * H + q head (-1: none)
-    __shared__ int s_page[4][C::PS];              // stage st's page ids at st % 4 (-1: past the unit, or bad)
-    __shared__ int s_bad[4][2];                   // its positions on bad pages, as a bit mask
-    __shared__ uint32_t s_max[4][2];              // largest |K| and |V| of a stage (fp32), by warp
+    __shared__ float s_f[64];                     // score factor of each row
+    __shared__ int s_bad[4][2];                   // stage c's positions on bad pages, as a bit mask, at c % 4
+    __shared__ __align__(8) float s_fk[C::F16 ? 1 : C::PS];    // what undoes the scale of each K row of a stage (fp32)
+    __shared__ uint32_t s_max[4];                 // largest |V| of a stage (fp32), by warp
     __shared__ int s_flag;                        // V had values that are not finite behind the mask
+    __shared__ volatile int s_abort;
     const Paged &a = A.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     const int wr = warp % WR, wk = warp / WR % C::WK, wd = warp / WR / C::WK;
+    unsigned char *sm = sm_ + (-smem_u32(sm_) & 1023);
     const uint32_t sm0 = smem_u32(sm);
+    if (tid == 0) {
+        for (int i = 0; i < C::NS; i++) mbar_init(&s_full[i], 1);
+        s_abort = 0;
+        fence_mbar_init();
+    }
+    uint32_t c0 = 0;                              // stages of the CTA's earlier units
     // the trigger comes after the wait: a kernel that starts on it may read what this one waited for
     if (!last) pdl_wait();
     pdl_trigger();
@@ -102,9 +118,9 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             b = u % a.n_seq;
             slot = u / a.n_seq;
             if (!paged_seq(a, b, t0, n, kv) && tid == 0 && slot == 0 && tile == 0 && kh == 0) paged_err(a, QMS_PAGED_ELEN);
-            k0 = a.prefix + slot * A.p.chunk_s;
+            k0 = A.p.base_s + slot * A.p.chunk_s;
             k1 = min(kv, k0 + A.p.chunk_s);
-            if (k0 >= k1 || tile * 16 * WR >= n * a.G) continue;
+            if (max(k0, a.prefix) >= k1 || tile * 16 * WR >= n * a.G) continue;
             slot += A.p.slots_p;
         } else {
             slot = u;
@@ -112,21 +128,10 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             k1 = min(a.prefix, k0 + A.p.chunk_p);
         }
         const int *table = a.table + (own ? (int64_t)b * a.table_stride : 0);
-        // page id and bad-page bit of position `i` of stage st, by one thread per position
-        auto page_of = [&](int st, int i) {
-            const int p = k0 + st * C::PS + i;
-            return p < k1 ? table[p >> a.page_log] : -2;
-        };
-        auto put_page = [&](int st, int i, int page) {
-            const bool bad = page != -2 && (unsigned)page >= (unsigned)a.n_pages;
-            s_page[st & 3][i] = bad || page == -2 ? -1 : page;
-            const unsigned bits = __ballot_sync(kFull, bad);
-            if (lane == 0) s_bad[st & 3][i >> 5] = (int)bits;
-            if (bad) paged_err(a, QMS_PAGED_EPAGE);
-        };
+        const int kmin = own ? max(k0, a.prefix) : k0;
         const int r0 = tile * 16 * WR;
+        fence_async_smem();
         __syncthreads();                          // the previous unit is done with shared memory
-        for (int i = tid; i < C::NS * C::PS; i += 128) put_page(i / C::PS, i % C::PS, page_of(i / C::PS, i % C::PS));
         if (tid == 0) s_flag = 0;
         // rows of the tile: the sequence's own, or all tokens' (each token's sequence found by a warp)
         if (own) {
@@ -152,19 +157,57 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             }
             if (tid < 16 * WR && r0 + tid >= a.n_tok * a.G) s_pos[tid] = s_tok[tid] = -1;
         }
-        __syncthreads();
-        auto load = [&](int st) {                 // stage st of the unit into its slot
-            const int base = k0 + st * C::PS;
-            const uint32_t dk = sm0 + st % C::NS * C::STAGE, dv = dk + C::STAGE / 2;
+        // A stage's boxes (of K and V, by halves of a row where those are boxes of their own) in turn over the four warps, one
+        // lane each: a lane issues a box in some 90 cycles. Page ids are fetched a stage ahead; warp 0 also looks at
+        // all of them (box i in lane i, and i + 32) for what to expect and what is bad.
+        const int R = min(1 << a.page_log, C::PS), boxes = C::PS / R;
+        constexpr int KINDS = C::F16 ? D / 32 : 2;                 // tensors x halves
+        int pages[2], every[2];
+        auto page_of = [&](int st, int i) {
+            const int p = k0 + st * C::PS + i * R;
+            return i < boxes && p < k1 ? table[p >> a.page_log] : -2;                          // -2: past the unit
+        };
+        auto look_up = [&](int st) {
 #pragma unroll
-            for (int i = tid; i < C::PS * C::CH; i += 128) {
-                const int r = i / C::CH, c = i % C::CH, page = s_page[st & 3][r];
-                const int64_t off = page < 0 ? 0 : page * a.page_stride + ((base + r) & ((1 << a.page_log) - 1)) * a.pos_stride + kh * a.head_stride + c * 16;
-                const int cs = C::F16 ? c ^ (r & 7) : c;
-                cp_async16_or0(dk + r * C::ROW + cs * 16, a.k + off, page >= 0);
-                cp_async16_or0(dv + r * C::ROW + cs * 16, a.v + off, page >= 0);
+            for (int h = 0; h < 2; h++) {
+                pages[h] = page_of(st, ((lane + 32 * h) * 4 + warp) / KINDS);
+                every[h] = warp == 0 ? page_of(st, lane + 32 * h) : -2;
             }
         };
+        auto load = [&](int st) {                 // (its pages have been looked up)
+            const uint32_t c = c0 + st, dst = sm0 + c % C::NS * C::STAGE;
+            uint64_t *bar = &s_full[c % C::NS];
+            if (warp == 0) {
+                uint32_t have = 0, bad[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const bool b = every[h] != -2 && (unsigned)every[h] >= (unsigned)a.n_pages;
+                    have += __popc(__ballot_sync(kFull, every[h] != -2 && !b));
+                    bad[h] = __ballot_sync(kFull, b);
+                    if (b) paged_err(a, QMS_PAGED_EPAGE);
+                }
+                if (lane < 2) {                   // bits of the stage's positions
+                    uint32_t bits = 0;
+                    if (bad[0] | bad[1])
+                        for (int e = 0; e < 32; e++) {
+                            const int i = (lane * 32 + e) / R;
+                            bits |= (lane * 32 + e < C::PS ? bad[i >> 5 & 1] >> (i & 31) & 1u : 0u) << e;
+                        }
+                    s_bad[c & 3][lane] = (int)bits;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(bar, have * (uint32_t)(2 * R * C::ROW));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if ((unsigned)pages[h] < (unsigned)a.n_pages) {
+                    const int item = (lane + 32 * h) * 4 + warp, i = item / KINDS, kind = item % KINDS;
+                    const int y = (k0 + st * C::PS + i * R) & ((1 << a.page_log) - 1);
+                    const uint32_t to = dst + (kind & 1) * (C::STAGE / 2) + (C::F16 ? (kind >> 1) * C::HALF + i * R * 128 : i * R * C::ROW);
+                    tma_load4(to, kind & 1 ? &mv : &mk, (kind >> 1) * 64, kh, y, pages[h], bar);
+                }
+        };
+        look_up(0);
+        __syncthreads();
         int lo_pos = 0x7fffffff, hi_pos = -1;     // least and largest position among the tile's rows
         for (int r = lane; r < 16 * WR; r += 32) {
             const int p = s_pos[r];
@@ -173,50 +216,56 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         }
         lo_pos = __reduce_min_sync(kFull, lo_pos);
         hi_pos = __reduce_max_sync(kFull, hi_pos);
-        if (k0 > hi_pos) continue;                // nobody sees any of it
+        if (kmin > hi_pos) continue;              // nobody sees any of it
         const int k_end = min(k1, hi_pos + 1), nst = (k_end - k0 + C::PS - 1) / C::PS;
 #pragma unroll
         for (int st = 0; st < C::NS - 1; st++) {
             if (st < nst) load(st);
-            cp_commit();
+            look_up(st + 1);
         }
 
-        // ---- q: this thread's elements of rows g and g + 8 of its row group, as mma A fragments, each row scaled by a
-        // power of two into fp16's range (exact), undone in the score's factor
-        const int tok0 = s_tok[wr * 16 + g], tok1 = s_tok[wr * 16 + g + 8];
-        const int pos0 = s_pos[wr * 16 + g], pos1 = s_pos[wr * 16 + g + 8];
-        float f0, f1;
-        uint32_t qh[D / 16][4], ql[D / 16][4];
-        {
-            float x[2][D / 4];
+        // ---- q: 8 lanes per row; each row scaled by a power of two into fp16's range (exact; undone in the score's factor)
+        // and split, into the stage slot that is filled last; from there as mma A fragments
+        unsigned char *qs = sm + (c0 + C::NS - 1) % C::NS * C::STAGE;
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int tok = r ? tok1 : tok0;
-                const float *src = A.q + (tok < 0 ? 0 : (tok / a.H) * A.ldq + (int64_t)(tok % a.H) * D) + tq * 2;
-                uint32_t mx = 0;
+        for (int i = 0; i < WR; i++) {
+            const int r = (warp * WR + i) * 4 + (lane >> 3), tok = s_tok[r], t = tok < 0 ? 0 : tok / a.H;
+            const float4 *src = reinterpret_cast<const float4 *>(A.q + t * A.ldq + (int64_t)(tok < 0 ? 0 : tok - t * a.H) * D) + (lane & 7);
+            float4 x[D / 32];
+            uint32_t mx = 0;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    const float2 v = tok < 0 ? make_float2(0.0f, 0.0f) : __ldcg(reinterpret_cast<const float2 *>(src + i * 8));
-                    x[r][2 * i] = v.x;
-                    x[r][2 * i + 1] = v.y;
-                    mx = max(mx, max(finite_bits(v.x), finite_bits(v.y)));
-                }
-                mx = max(mx, __shfl_xor_sync(kFull, mx, 1));
-                mx = max(mx, __shfl_xor_sync(kFull, mx, 2));
-                const uint32_t up = scale_up(mx >> 23);
-                (r ? f1 : f0) = A.scale2 * pow2_bits(254u - up);
-                const float m = pow2_bits(up);
+            for (int k = 0; k < D / 32; k++) x[k] = tok < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(src + 8 * k);
 #pragma unroll
-                for (int i = 0; i < D / 4; i++) x[r][i] *= m;
-            }
+            for (int k = 0; k < D / 32; k++) mx = max(mx, max(max(finite_bits(x[k].x), finite_bits(x[k].y)), max(finite_bits(x[k].z), finite_bits(x[k].w))));
+            mx = max(mx, __shfl_xor_sync(kFull, mx, 1));
+            mx = max(mx, __shfl_xor_sync(kFull, mx, 2));
+            mx = max(mx, __shfl_xor_sync(kFull, mx, 4));
+            const uint32_t up = scale_up(mx >> 23);
+            if ((lane & 7) == 0) s_f[r] = A.scale2 * pow2_bits(254u - up);
+            const float m = pow2_bits(up);
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ks++) {
-                split_h2(x[0][4 * ks], x[0][4 * ks + 1], qh[ks][0], ql[ks][0]);
-                split_h2(x[1][4 * ks], x[1][4 * ks + 1], qh[ks][1], ql[ks][1]);
-                split_h2(x[0][4 * ks + 2], x[0][4 * ks + 3], qh[ks][2], ql[ks][2]);
-                split_h2(x[1][4 * ks + 2], x[1][4 * ks + 3], qh[ks][3], ql[ks][3]);
+            for (int k = 0; k < D / 32; k++) {    // values 4 (lane & 7) + 32 k .. + 3
+                const int c = 4 * k + ((lane & 7) >> 1);
+                unsigned char *to = qs + (c >> 3) * C::QHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                uint32_t h[2], l[2];
+                split_h2(x[k].x * m, x[k].y * m, h[0], l[0]);
+                split_h2(x[k].z * m, x[k].w * m, h[1], l[1]);
+                *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
+                *reinterpret_cast<uint2 *>(to + C::QROWS * D * 2) = make_uint2(l[0], l[1]);
             }
         }
+        __syncthreads();
+        const int pos0 = s_pos[wr * 16 + g], pos1 = s_pos[wr * 16 + g + 8];
+        const float f0 = s_f[wr * 16 + g], f1 = s_f[wr * 16 + g + 8];
+        uint32_t qh[D / 16][4], ql[D / 16][4];
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks++) {
+            const int r = wr * 16 + (lane & 15), c = 2 * ks + (lane >> 4);
+            const uint32_t at = smem_u32(qs) + (c >> 3) * C::QHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            ldsm4(qh[ks], at);
+            ldsm4(ql[ks], at + C::QROWS * D * 2);
+        }
+        fence_async_smem();
 
         float o[C::DW / 8][4];
 #pragma unroll
@@ -225,59 +274,106 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         uint32_t v_exp = 0;                       // fp32: largest exponent of V so far; o is in units of its scale
 
         for (int st = 0; st < nst; st++) {
-            cp_wait<C::NS - 2>();
+            const uint32_t c = c0 + st;
+            for (uint32_t n = 0; !mbar_try_wait(&s_full[c % C::NS], c / C::NS & 1) && !s_abort; n++) {
+                if (n == kPaSpin) {               // reported; the unit's result is not valid
+                    s_abort = 1;
+                    paged_err(a, QMS_PAGED_ETIMEOUT);
+                }
+                if (n > 64) __nanosleep(32);
+            }
             __syncthreads();                      // the stage has landed; the slot before it is free
-            const int base = k0 + st * C::PS, next = st + C::NS;
-            if (st + C::NS - 1 < nst) load(st + C::NS - 1);
-            cp_commit();
-            const int page_next = next < nst && tid < C::PS ? page_of(next, tid) : -2;
-            const int bad0 = s_bad[st & 3][0], bad1 = C::PS > 32 ? s_bad[st & 3][1] : 0;
-            const bool behind = base + C::PS - 1 > lo_pos;         // some row does not see all of it
-            const bool masked = behind || base + C::PS > k1 || bad0 || bad1;
-            unsigned char *raw = sm + st % C::NS * C::STAGE;
-            uint32_t kb = sm0 + st % C::NS * C::STAGE, vb = kb + C::STAGE / 2;
-            float fk = 1.0f;                      // undoes the scale of this stage's K
+            const int base = k0 + st * C::PS;
+            if (st + C::NS - 1 < nst) {
+                load(st + C::NS - 1);
+                look_up(st + C::NS);
+            }
+            const int bad0 = s_bad[c & 3][0], bad1 = C::PS > 32 ? s_bad[c & 3][1] : 0;
+            // some row does not see all of it: rows [first, seen] of the stage are seen by every row of the tile
+            const int first = kmin, seen = bad0 | bad1 ? -1 : min(lo_pos, k1 - 1);
+            const bool masked = base + C::PS - 1 > seen || base < first;
+            unsigned char *raw = sm + c % C::NS * C::STAGE;
+            uint32_t kb = sm0 + c % C::NS * C::STAGE, vb = kb + C::STAGE / 2;
             if constexpr (C::F16) {
-                if (behind) {                     // behind the causal mask a weight is 0, but 0 * inf is not
-                    bool any = false;
+                if (masked) {                     // behind the mask a weight is 0, but 0 * inf is not
                     for (int i = tid; i < C::PS * C::CH; i += 128) {
-                        if (base + i / C::CH <= lo_pos) continue;
-                        uint4 *pv = reinterpret_cast<uint4 *>(raw + C::STAGE / 2) + i;
+                        const int r = i / C::CH, p = base + r;
+                        if (p >= first && p <= seen) continue;
+                        uint4 *pv = reinterpret_cast<uint4 *>(raw + C::STAGE / 2 + C::piece(r, i % C::CH));
                         uint4 v = *pv;
                         if (drop_nonfinite((const KT *)nullptr, v)) {
                             *pv = v;
-                            any = true;
+                            if (p >= first && p < k1) s_flag = 1;      // (else left over from before: nobody's)
                         }
                     }
-                    if (any) s_flag = 1;
+                    fence_async_smem();
                     __syncthreads();
                 }
             } else {
-                // hi and lo of K and V: the stage's largest values, then scaled and split
+                // hi and lo: K by rows, each with a scale of its own (undone in its scores), V with the largest scale so
+                // far of what somebody sees (o is in its units)
                 constexpr int N = C::PS * C::CH / 128;             // 16-byte pieces of K (and of V) per thread
-                float4 x[2][N];
-                uint32_t mx[2] = {0, 0};
+                const float4 *rk = reinterpret_cast<const float4 *>(raw), *rv = reinterpret_cast<const float4 *>(raw + C::STAGE / 2);
+                // largest finite |value|: by float maxima, looked at again where one is inf (NaN is no maximum)
+                auto largest = [](const float4 &y) { return fmaxf(max3(0.0f, fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))); };
+                auto finite4 = [](const float4 &y) { return max(max(finite_bits(y.x), finite_bits(y.y)), max(finite_bits(y.z), finite_bits(y.w))); };
+                float4 x[N];
+                float mx = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 2; w++)
+                for (int i = 0; i < N; i++) x[i] = rv[tid + 128 * i];
+                if (masked)
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        const int at = tid + 128 * i;
-                        x[w][i] = *reinterpret_cast<const float4 *>(raw + w * (C::STAGE / 2) + at * 16);
-                        if (w == 1 && behind && base + at / C::CH > lo_pos) {
-                            uint4 v = *reinterpret_cast<const uint4 *>(&x[w][i]);
-                            if (drop_nonfinite((const KT *)nullptr, v)) {
-                                x[w][i] = *reinterpret_cast<const float4 *>(&v);
-                                s_flag = 1;
-                            }
+                        const int r = (tid + 128 * i) / C::CH, p = base + r;
+                        if (p >= first && p <= seen) continue;
+                        uint4 v = *reinterpret_cast<const uint4 *>(&x[i]);
+                        if (drop_nonfinite((const KT *)nullptr, v)) {
+                            x[i] = *reinterpret_cast<const float4 *>(&v);
+                            if (p >= first && p < k1) s_flag = 1;
                         }
-                        mx[w] = max(mx[w], max(max(finite_bits(x[w][i].x), finite_bits(x[w][i].y)), max(finite_bits(x[w][i].z), finite_bits(x[w][i].w))));
+                        if (p < first || p >= k1 || (bad0 >> r & 1)) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);    // no part of the unit
                     }
-                mx[0] = __reduce_max_sync(kFull, mx[0]);
-                mx[1] = __reduce_max_sync(kFull, mx[1]);
-                if (lane == 0) s_max[warp][0] = mx[0], s_max[warp][1] = mx[1];
-                __syncthreads();                  // (and the tiles of the last stage are no longer read)
-                const uint32_t ke = max(max(s_max[0][0], s_max[1][0]), max(s_max[2][0], s_max[3][0])) >> 23;
-                const uint32_t ve = max(max(max(s_max[0][1], s_max[1][1]), max(s_max[2][1], s_max[3][1])) >> 23, v_exp);
+#pragma unroll
+                for (int i = 0; i < N; i++) mx = fmaxf(mx, largest(x[i]));
+                uint32_t mb = __float_as_uint(mx);
+                if (mx == INFINITY) {
+                    mb = 0;
+                    for (int i = 0; i < N; i++) mb = max(mb, finite4(rv[tid + 128 * i]));
+                }
+                mb = __reduce_max_sync(kFull, mb);
+                if (lane == 0) s_max[warp] = mb;
+                auto put = [&](int w, int at, float4 y, float up) {
+                    const int r = at / C::CH, c = at % C::CH;      // values 4 c .. + 3 of row r
+                    const float2 y0 = f2_mul(make_float2(y.x, y.y), make_float2(up, up)), y1 = f2_mul(make_float2(y.z, y.w), make_float2(up, up));
+                    uint32_t h[2], l[2];
+                    split_h2(y0.x, y0.y, h[0], l[0]);
+                    split_h2(y1.x, y1.y, h[1], l[1]);
+                    unsigned char *to = sm + C::CONV + w * 2 * C::HTILE + C::piece(r, c >> 1) + (c & 1) * 8;
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
+                    *reinterpret_cast<uint2 *>(to + C::HTILE) = make_uint2(l[0], l[1]);
+                };
+                const unsigned peers = C::CH == 32 ? kFull : 0xffffu << (lane & 16);             // the lanes of a row
+#pragma unroll
+                for (int h = 0; h < N; h += 4) {
+                    float4 y[4];
+                    uint32_t ky[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] = rk[tid + 128 * (h + i)];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float t = largest(y[i]);
+                        ky[i] = __reduce_max_sync(peers, t == INFINITY ? finite4(y[i]) : __float_as_uint(t));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at = tid + 128 * (h + i);
+                        const uint32_t up = scale_up(ky[i] >> 23);
+                        if (at % C::CH == 0) s_fk[at / C::CH] = pow2_bits(254u - up);
+                        put(0, at, y[i], pow2_bits(up));
+                    }
+                }
+                __syncthreads();
+                const uint32_t ve = max(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])) >> 23, v_exp);
                 if (ve != v_exp) {
                     const uint32_t down = scale_up(v_exp) - scale_up(ve);
                     const float d = down > 126 ? 0.0f : pow2_bits(127u - down);
@@ -286,20 +382,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                         for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
                     v_exp = ve;
                 }
-                fk = pow2_bits(254u - scale_up(ke));
-                const float up[2] = {pow2_bits(scale_up(ke)), pow2_bits(scale_up(ve))};
 #pragma unroll
-                for (int w = 0; w < 2; w++)
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int at = tid + 128 * i, r = at / C::CH, c = at % C::CH;      // values 4 c .. + 3 of row r
-                        uint32_t h[2], l[2];
-                        split_h2(x[w][i].x * up[w], x[w][i].y * up[w], h[0], l[0]);
-                        split_h2(x[w][i].z * up[w], x[w][i].w * up[w], h[1], l[1]);
-                        unsigned char *to = sm + C::CONV + w * 2 * C::HTILE + r * C::HROW + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
-                        *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
-                        *reinterpret_cast<uint2 *>(to + C::HTILE) = make_uint2(l[0], l[1]);
-                    }
+                for (int i = 0; i < N; i++) put(1, tid + 128 * i, x[i], pow2_bits(scale_up(ve)));
                 __syncthreads();
                 kb = sm0 + C::CONV;
                 vb = kb + 2 * C::HTILE;
@@ -316,7 +400,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
 #pragma unroll
                 for (int i = 0; i < C::NT / 2; i++) {
                     const int r = wk * C::KW + i * 16 + ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
-                    const uint32_t at = kb + r * C::HROW + ((c ^ (r & 7)) << 4);
+                    const uint32_t at = kb + C::piece(r, c);
                     uint32_t kf[4];
                     ldsm4(kf, at);
                     mma_f16(s[2 * i], qh[ks], kf[0], kf[1]);
@@ -330,16 +414,16 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     }
                 }
             // ---- softmax of the stage: s becomes the weights
-            const float g0 = f0 * fk, g1 = f1 * fk;
             float n0 = m0, n1 = m1;
 #pragma unroll
             for (int i = 0; i < C::NT; i++) {
                 const int r = wk * C::KW + i * 8 + tq * 2, p = base + r;
-                s[i][0] = (s[i][0] + s2[i][0]) * g0, s[i][1] = (s[i][1] + s2[i][1]) * g0;
-                s[i][2] = (s[i][2] + s2[i][2]) * g1, s[i][3] = (s[i][3] + s2[i][3]) * g1;
+                const float2 fk = C::F16 ? make_float2(1.0f, 1.0f) : *reinterpret_cast<const float2 *>(s_fk + (C::F16 ? 0 : r));
+                s[i][0] = (s[i][0] + s2[i][0]) * (f0 * fk.x), s[i][1] = (s[i][1] + s2[i][1]) * (f0 * fk.y);
+                s[i][2] = (s[i][2] + s2[i][2]) * (f1 * fk.x), s[i][3] = (s[i][3] + s2[i][3]) * (f1 * fk.y);
                 if (masked) {
                     const int bm = (r < 32 ? bad0 : bad1) >> (r & 31);
-                    const bool ok0 = p < k1 && !(bm & 1), ok1 = p + 1 < k1 && !(bm & 2);
+                    const bool ok0 = p >= first && p < k1 && !(bm & 1), ok1 = p + 1 >= first && p + 1 < k1 && !(bm & 2);
                     if (!ok0 || p > pos0) s[i][0] = -INFINITY;
                     if (!ok1 || p + 1 > pos0) s[i][1] = -INFINITY;
                     if (!ok0 || p > pos1) s[i][2] = -INFINITY;
@@ -380,7 +464,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
 #pragma unroll
                 for (int j = 0; j < C::DW / 16; j++) {
                     const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = wd * (C::DW / 8) + 2 * j + (lane >> 4);
-                    const uint32_t at = vb + r * C::HROW + ((c ^ (r & 7)) << 4);
+                    const uint32_t at = vb + C::piece(r, c);
                     uint32_t vf[4];
                     ldsm4t(vf, at);
                     mma_f16(o[2 * j], ph, vf[0], vf[1]);
@@ -394,9 +478,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     }
                 }
             }
-            if (next < nst && tid < C::PS) put_page(next, tid, page_next);       // whole warps
         }
-        cp_wait<0>();
+        c0 += nst;
         __syncthreads();                          // every warp is done with the stages
         if constexpr (!C::F16) {
             const float d = pow2_bits(254u - scale_up(v_exp));
@@ -407,7 +490,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         auto dim = [&](int i, int j) { return wd * C::DW + i * 8 + tq * 2 + (j & 1); };
         if (s_flag && wk == 0) {
             // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
-            for (int p = max(k0, lo_pos + 1); p < k1; p++) {
+            for (int p = kmin; p < k1; p++) {
                 const int64_t at = paged_at(a, table, p);
                 if (at < 0) continue;
                 const KT *vr = reinterpret_cast<const KT *>(a.v + at + kh * a.head_stride);
@@ -427,6 +510,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         if (isnan(l0)) m0 = 0.0f;                 // scores that are all NaN leave no maximum, but are not nothing
         if (isnan(l1)) m1 = 0.0f;
         const int64_t po = (int64_t)slot * a.n_tok * a.H;
+        const int tok0 = s_tok[wr * 16 + g], tok1 = s_tok[wr * 16 + g + 8];
         if constexpr (C::WK == 1) {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
@@ -441,9 +525,9 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 if (tq == 0) A.part_ml[po + tok] = make_float2(m == -INFINITY ? m : m - kPaShift, l);
             }
         } else {
-            // join the position groups: group w's row r at red[(w * 16 WR + r)][D + 2]
+            // join the position groups: group w's row r at red[(w * 16 WR + r)][D + 4]
             float *red = reinterpret_cast<float *>(sm);
-            constexpr int LD = D + 2;
+            constexpr int LD = D + 4;            // rows on different banks; 8-byte pieces
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 float *dst = red + ((wk * WR + wr) * 16 + g + 8 * r) * LD;
@@ -455,25 +539,28 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 }
             }
             __syncthreads();
-            for (int r = warp; r < 16 * WR; r += 4) {
-                const int tok = s_tok[r];
-                if (tok < 0) continue;
-                float m = -INFINITY, l = 0.0f, x[D / 32];
 #pragma unroll
-                for (int k = 0; k < C::WK; k++) m = fmaxf(m, red[(k * 16 * WR + r) * LD + D]);
+            for (int q = 0; q < 4 * WR; q++) {
+                const int r = warp + 4 * q, tok = s_tok[r];
+                float m = -INFINITY, l = 0.0f, x[D / 32], mk_[C::WK], w[C::WK];
 #pragma unroll
-                for (int d = 0; d < D / 32; d++) x[d] = 0.0f;
-                if (m != -INFINITY) {
-#pragma unroll
-                    for (int k = 0; k < C::WK; k++) {
-                        const float *src = red + (k * 16 * WR + r) * LD;
-                        const float w = ex2(src[D] - m);
-                        if (w == 0.0f && src[D + 1] == 0.0f) continue;         // saw nothing: its o may be 0 * inf
-                        l = fmaf(w, src[D + 1], l);
-#pragma unroll
-                        for (int d = 0; d < D / 32; d++) x[d] = fmaf(w, src[lane + 32 * d], x[d]);
-                    }
+                for (int k = 0; k < C::WK; k++) {
+                    mk_[k] = red[(k * 16 * WR + r) * LD + D];
+                    m = fmaxf(m, mk_[k]);
                 }
+#pragma unroll
+                for (int k = 0; k < C::WK; k++) {
+                    w[k] = mk_[k] == -INFINITY ? 0.0f : ex2(mk_[k] - m);
+                    l = fmaf(w[k], red[(k * 16 * WR + r) * LD + D + 1], l);
+                }
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) {
+                    x[d] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < C::WK; k++)            // (a group that saw nothing: its o may be 0 * inf)
+                        x[d] = fmaf(w[k], mk_[k] == -INFINITY ? 0.0f : red[(k * 16 * WR + r) * LD + lane + 32 * d], x[d]);
+                }
+                if (tok < 0) continue;
 #pragma unroll
                 for (int d = 0; d < D / 32; d++) A.part_o[(po + tok) * D + lane + 32 * d] = x[d];
                 if (lane == 0) A.part_ml[po + tok] = make_float2(m == -INFINITY ? m : m - kPaShift, l);
@@ -484,71 +571,114 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
 }
 
 // ---- joining the slots of a row --------------------------------------------------------------------
-// One warp per (token, q head): out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the row's slots in their
-// order; 0 where nothing was seen.
-template <int D>
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the slots of a (token, q head) row in their order; 0 where
+// nothing was seen. WPR warps per row, each with every WPR-th slot; the loads of (m, l) and of the first slots go out
+// before the row's length is known (what was not written is not used), so that the chain is one round trip.
+// Bound by that latency for few rows, by the partial results' traffic (L2) for many.
+template <int D, int WPR>
 __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
-    constexpr int J = D / 32;
+    constexpr int J = D / 32, AHEAD = 4;
+    __shared__ float s_x[WPR > 1 ? 8 : 1][D], s_l[8];
     const Paged &a = A.a;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)a.n_tok * a.H;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
+    const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + warp / WPR, rows = (int64_t)a.n_tok * a.H;
+    const int t = (int)(row / a.H), slots = A.p.slots_p + A.p.slots_s;
     pdl_trigger();
     pdl_wait();
-    if (row >= rows) return;
-    const int t = (int)(row / a.H);
-    int t0 = 0, n = 0, kv = 0;
-    const int b = paged_seq_of(a, t);
-    if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
-    float x[J];
+    const bool there = row < rows;
+    // slot s of the row in the order of its use is at `at`; np: how many are of the shared positions
+    int np = 0;
+    auto at = [&](int s) { return (s < np ? s : s - np + A.p.slots_p) * rows + row; };
+    auto fetch = [&](int64_t i, float (&v)[J]) {
+        const float *src = A.part_o + i * D + lane * J;
+        if constexpr (J == 4) *reinterpret_cast<float4 *>(v) = __ldcg(reinterpret_cast<const float4 *>(src));
+        else *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(src));
+    };
+    float x[J], l = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; j++) x[j] = 0.0f;
-    float l = 0.0f;
-    const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
-    if (pos >= 0) {                               // the slots of chunks that begin past the row's position are not written
-        // slots of a kind up to place d of it: one per chunk, or two where k_paged_wide has two streams
-        auto upto = [](int d, int chunk, int wr) {
-            const int c = d / chunk;
-            return wr == kPaWideSplit ? 2 * c + (d - c * chunk >= 128 ? 2 : 1) : c + 1;
-        };
-        int np = 0;
-        if (a.prefix > 0) {
-            const int d = min(pos, a.prefix - 1);
-            if (A.p.line > 0) {
-                const unsigned h = (unsigned)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
-                const unsigned x = ((t * a.G + h - kh * a.G) / 256 * a.Hk + kh) * nt;
-                np = line_run(x + d / 128, A.p.line, A.p.line_ctas) - line_run(x, A.p.line, A.p.line_ctas) + 1;
-            } else {
-                np = upto(d, A.p.chunk_p, A.p.wr_p);
-            }
-        }
-        const int ns = np + (pos < a.prefix ? 0 : upto(pos - A.p.base_s, A.p.chunk_s, A.p.wr_s));
-        auto at = [&](int s) { return (s < np ? s : s - np + A.p.slots_p) * rows + row; };
-        float M = -INFINITY;
-        for (int s = lane; s < ns; s += 32) M = fmaxf(M, __ldcg(&A.part_ml[at(s)]).x);
-        M = warp_max(M);
-        if (M != -INFINITY) {
-            for (int s0 = 0; s0 < ns; s0 += 32) {
-                const float2 ml = s0 + lane < ns ? __ldcg(&A.part_ml[at(s0 + lane)]) : make_float2(-INFINITY, 0.0f);
-                const float w = ex2(ml.x - M);
-                l += warp_sum(w * ml.y);
-                const int ne = min(32, ns - s0);
-#pragma unroll 8
-                for (int i = 0; i < ne; i++) {
-                    const float wi = __shfl_sync(kFull, w, i);
-                    const float *src = A.part_o + at(s0 + i) * D + lane * J;
-                    float v[J];
-                    if constexpr (J == 4) *reinterpret_cast<float4 *>(v) = __ldcg(reinterpret_cast<const float4 *>(src));
-                    else *reinterpret_cast<float2 *>(v) = __ldcg(reinterpret_cast<const float2 *>(src));
+    if (there) {
+        // whatever the row's length: slot `lane`'s (m, l), and the first values of this warp's slots
+        const float2 first = lane < slots ? __ldcg(&A.part_ml[lane * rows + row]) : make_float2(-INFINITY, 0.0f);
+        float v[AHEAD][J];
 #pragma unroll
-                    for (int j = 0; j < J; j++) x[j] = fmaf(wi, v[j], x[j]);
+        for (int i = 0; i < AHEAD; i++)
+            if (sub + WPR * i < slots) fetch((sub + WPR * i) * rows + row, v[i]);
+        int t0 = 0, n = 0, kv = 0;
+        const int b = paged_seq_of(a, t);
+        if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
+        const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
+        if (pos >= 0) {                           // the slots of chunks that begin past the row's position are not written
+            // slots of a kind up to place d of it: one per chunk, or two where k_paged_wide has two streams
+            auto upto = [](int d, int chunk, int wr) {
+                const int c = d / chunk;
+                return wr == kPaWideSplit ? 2 * c + (d - c * chunk >= 128 ? 2 : 1) : c + 1;
+            };
+            if (a.prefix > 0) {
+                const int d = min(pos, a.prefix - 1);
+                if (A.p.line > 0) {
+                    const unsigned h = (unsigned)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
+                    const unsigned y = ((t * a.G + h - kh * a.G) / 256 * a.Hk + kh) * nt;
+                    np = line_run(y + d / 128, A.p.line, A.p.line_ctas) - line_run(y, A.p.line, A.p.line_ctas) + 1;
+                } else {
+                    np = upto(d, A.p.chunk_p, A.p.wr_p);
+                }
+            }
+            const int ns = np + (pos < a.prefix ? 0 : upto(pos - A.p.base_s, A.p.chunk_s, A.p.wr_s));
+            const bool dense = np == A.p.slots_p || ns == np;              // slot s is where the fetch above took it
+            float M = -INFINITY;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            for (int s0 = 0; s0 < ns; s0 += 32) {
+                const float2 y = s0 + lane >= ns ? make_float2(-INFINITY, 0.0f) : s0 == 0 && dense ? first : __ldcg(&A.part_ml[at(s0 + lane)]);
+                if (s0 == 0) ml = y;
+                M = fmaxf(M, y.x);
+            }
+            M = warp_max(M);
+            if (M != -INFINITY) {
+                for (int s0 = 0; s0 < ns; s0 += 32) {
+                    if (s0 > 0) ml = s0 + lane < ns ? __ldcg(&A.part_ml[at(s0 + lane)]) : make_float2(-INFINITY, 0.0f);
+                    const float w = ex2(ml.x - M);
+                    if (sub == 0) l += w * (ml.x == -INFINITY ? 0.0f : ml.y);
+                    const int ne = min(32, ns - s0);
+                    int i = sub;
+                    if (s0 == 0 && dense) {
+#pragma unroll
+                        for (int k = 0; k < AHEAD; k++, i += WPR) {
+                            const float wi = __shfl_sync(kFull, w, i & 31);
+                            if (i < ne)
+#pragma unroll
+                                for (int j = 0; j < J; j++) x[j] = fmaf(wi, v[k][j], x[j]);
+                        }
+                    }
+#pragma unroll 8
+                    for (; i < ne; i += WPR) {
+                        const float wi = __shfl_sync(kFull, w, i);
+                        float y[J];
+                        fetch(at(s0 + i), y);
+#pragma unroll
+                        for (int j = 0; j < J; j++) x[j] = fmaf(wi, y[j], x[j]);
+                    }
                 }
             }
         }
     }
-    float *dst = A.out + t * A.ldo + (row - (int64_t)t * a.H) * D + lane * J;
-    const float inv = 1.0f / l;
+    if (sub == 0) l = warp_sum(l);
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int j = 0; j < J; j++) dst[j] = l == 0.0f ? 0.0f : x[j] * inv;
+        for (int j = 0; j < J; j++) s_x[warp][lane * J + j] = x[j];
+        if (sub == 0 && lane == 0) s_l[warp] = l;
+        __syncthreads();
+        if (sub != 0) return;
+#pragma unroll
+        for (int k = 1; k < WPR; k++)
+#pragma unroll
+            for (int j = 0; j < J; j++) x[j] += s_x[warp + k][lane * J + j];
+    }
+    if (!there) return;
+    float *dst = A.out + t * A.ldo + (row - (int64_t)t * a.H) * D + lane * J;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if constexpr (J == 4) *reinterpret_cast<float4 *>(dst) = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    else *reinterpret_cast<float2 *>(dst) = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x[0] * inv, x[1] * inv);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -586,7 +716,7 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
     p.wr_p = row_groups(type, a.page_log, rows_p);
     p.wr_s = row_groups(type, a.page_log, rows_s);
-    p.base_s = p.wr_s <= 0 ? a.prefix & ~(std::min(1 << a.page_log, 128) - 1) : a.prefix;
+    p.base_s = a.prefix & ~(std::min(1 << a.page_log, p.wr_s <= 0 ? 128 : pa_stage(type)) - 1);
     const int own = std::max(0, a.max_kv - p.base_s);
     auto height = [](int wr) { return wr == kPaWidePair ? 256 : wr == kPaWideSplit ? 128 : 16 * wr; };
     p.tiles_p = (int)((rows_p + height(p.wr_p) - 1) / height(p.wr_p));
@@ -615,6 +745,30 @@ int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
     return al256(n * D * 4) + al256(n * 8);
 }
 
+int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    if (!encode) {
+        cudaDriverEntryPointQueryResult found;
+        void *f = nullptr;
+        QMS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
+        QMS_REQUIRE(f, QMS_CUDA_ECUDA, "paged_attention: the driver has no cuTensorMapEncodeTiled");
+        encode = (Encode)f;
+    }
+    const cuuint64_t ps = 1ull << a.page_log, row = (cuuint64_t)D * (f16 ? 2 : 4);
+    const cuuint64_t dim[4] = {(cuuint64_t)D, (cuuint64_t)a.Hk, ps, (cuuint64_t)a.n_pages};
+    // (the stride of a dimension of one has no meaning, and 0 none that the encoder takes)
+    const cuuint64_t stride[3] = {a.Hk > 1 ? (cuuint64_t)a.head_stride : row, ps > 1 ? (cuuint64_t)a.pos_stride : row,
+                                  a.n_pages > 1 ? (cuuint64_t)a.page_stride : row};
+    const cuuint32_t box[4] = {f16 ? 64u : (cuuint32_t)D, 1, (cuuint32_t)std::min<cuuint64_t>(ps, rows), 1}, one[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (void *)pool, dim, stride, box, one,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, f16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    QMS_REQUIRE(rc == CUDA_SUCCESS, QMS_CUDA_EINVAL, "paged_attention: the pool's strides do not make a tensor map (%d)", (int)rc);
+    return QMS_CUDA_OK;
+}
+
 template <int D, typename KT, int WR>
 static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
     using C = PaCfg<D, KT, WR>;
@@ -627,8 +781,11 @@ static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t 
         QMS_CK(cudaFuncSetAttribute(k_paged_attn<D, KT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         set |= 1ull << (dev & 63);
     }
+    CUtensorMap mk, mv;
+    int rc = paged_map(A.a, D, C::F16, C::PS, A.a.k, &mk);
+    if (rc || (rc = paged_map(A.a, D, C::F16, C::PS, A.a.v, &mv))) return rc;
     const int grid = (int)std::min<int64_t>(units, 148 * 8);
-    QMS_CK(launch_pdl(k_paged_attn<D, KT, WR>, dim3(grid), dim3(128), C::SMEM, s, A, own, last));
+    QMS_CK(launch_pdl(k_paged_attn<D, KT, WR>, dim3(grid), dim3(128), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
 }
 
@@ -666,10 +823,17 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, s) : launch_attn<64, __half>(A, s);
     else rc = D == 128 ? launch_attn<128, float>(A, s) : launch_attn<64, float>(A, s);
     if (rc) return rc;
+    // four warps per row while that leaves the SMs below 8 warps each, or where a row has many slots
     const int64_t rows = (int64_t)a.n_tok * a.H;
-    const dim3 grid((unsigned)((rows + 7) / 8));
-    if (D == 128) QMS_CK(launch_pdl(k_paged_merge<128>, grid, dim3(256), 0, s, A));
-    else QMS_CK(launch_pdl(k_paged_merge<64>, grid, dim3(256), 0, s, A));
+    const int wpr = rows <= 2 * 148 || p.slots_p + p.slots_s > 32 ? 4 : 1;
+    const dim3 grid((unsigned)((rows * wpr + 7) / 8));
+    if (D == 128) {
+        if (wpr == 4) QMS_CK(launch_pdl(k_paged_merge<128, 4>, grid, dim3(256), 0, s, A));
+        else QMS_CK(launch_pdl(k_paged_merge<128, 1>, grid, dim3(256), 0, s, A));
+    } else {
+        if (wpr == 4) QMS_CK(launch_pdl(k_paged_merge<64, 4>, grid, dim3(256), 0, s, A));
+        else QMS_CK(launch_pdl(k_paged_merge<64, 1>, grid, dim3(256), 0, s, A));
+    }
     return QMS_CUDA_OK;
 }
 

@@ -23,7 +23,6 @@
 // unit; such rows are masked. Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB, or (SPLIT) Q 64 KB and a
 // ring of 2 for each stream; TMEM: S 2 x 128, O 2 x 128 columns.
 // Bound by the tensor cores: 4 * 128 * 128 * head_dim flop per tile and product pair, twice for the split.
-#include <cuda.h>
 #include <math.h>
 #include <string.h>
 
@@ -93,22 +92,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A box of a paged pool: 64 values from x of one head, the positions of the map's box from y of a page.
-__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int head, int y, int page, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-                 "l"(map), "r"(x), "r"(head), "r"(y), "r"(page), "r"(smem_u32(bar))
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_tie(uint32_t (&r)[32]) {      // the same for a second array of that wait
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
                    "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
                    "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
                    "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
 }
 
 // Bounded wait for a phase of a barrier; a wait that gives up ends the CTA's work (flag) and is reported.
@@ -559,7 +547,7 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                             uint4 v = *pv;
                             if (drop_nonfinite((const __half *)nullptr, v)) {
                                 *pv = v;
-                                *s_flag = 1;
+                                if (base + r >= w.kmin && base + r < w.k1) *s_flag = 1;      // (else left over: nobody's)
                             }
                         }
                         fence_async_smem();
@@ -661,30 +649,6 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     if (last) pdl_wait();
 }
 
-// The pool as a tensor [page][position][head][value] for boxes of 64 values x min(page size, 128) positions.
-static int pool_map(const Paged &a, int D, const char *pool, CUtensorMap *map) {
-    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static Encode encode = nullptr;
-    if (!encode) {
-        cudaDriverEntryPointQueryResult found;
-        void *f = nullptr;
-        QMS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
-        QMS_REQUIRE(f, QMS_CUDA_ECUDA, "paged_attention: the driver has no cuTensorMapEncodeTiled");
-        encode = (Encode)f;
-    }
-    const cuuint64_t ps = 1ull << a.page_log;
-    const cuuint64_t dim[4] = {(cuuint64_t)D, (cuuint64_t)a.Hk, ps, (cuuint64_t)a.n_pages};
-    // (the stride of a dimension of one has no meaning, and 0 none that the encoder takes)
-    const cuuint64_t stride[3] = {(cuuint64_t)(a.Hk > 1 ? a.head_stride : 2 * D), (cuuint64_t)(ps > 1 ? a.pos_stride : 2 * D),
-                                  (cuuint64_t)(a.n_pages > 1 ? a.page_stride : 2 * D)};
-    const cuuint32_t box[4] = {64, 1, (cuuint32_t)(ps < kWTile ? ps : kWTile), 1}, one[4] = {1, 1, 1, 1};
-    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void *)pool, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    QMS_REQUIRE(rc == CUDA_SUCCESS, QMS_CUDA_EINVAL, "paged_attention: the pool's strides do not make a tensor map (%d)", (int)rc);
-    return QMS_CUDA_OK;
-}
-
 template <int D, bool SPLIT>
 static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
     using C = WideCfg<D, SPLIT>;
@@ -701,8 +665,8 @@ static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) 
         set |= 1ull << (dev & 63);
     }
     CUtensorMap mk, mv;
-    int rc = pool_map(A.a, D, A.a.k, &mk);
-    if (rc || (rc = pool_map(A.a, D, A.a.v, &mv))) return rc;
+    int rc = paged_map(A.a, D, true, kWTile, A.a.k, &mk);
+    if (rc || (rc = paged_map(A.a, D, true, kWTile, A.a.v, &mv))) return rc;
     const int grid = (int)(units < 148 ? units : 148);
     QMS_CK(launch_pdl(k_paged_wide<D, SPLIT>, dim3(grid), dim3(kWThreads), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
