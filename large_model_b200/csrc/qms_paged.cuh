@@ -75,6 +75,16 @@ __device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_
 // x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
+// Bits of the largest finite |value|, as an ordered integer: of one value (0 if it is not finite).
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+// Values whose largest has the biased exponent e go to 2^9 .. 2^10 when multiplied by 2^(up - 127), which
+// 2^(127 - up) undoes; both are normal numbers.
+__device__ __forceinline__ uint32_t scale_up(uint32_t e) { return e == 0 ? 127u : min(263u - e, 253u); }
+__device__ __forceinline__ float pow2_bits(uint32_t biased) { return __uint_as_float(biased << 23); }
+
 // A box of a paged pool: values from x of one head, the positions of the map's box from y of a page.
 __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int head, int y, int page, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
@@ -127,9 +137,10 @@ struct PagedPlan {
     int chunks_p, chunks_s;          // chunks of each kind
     int slots_p, slots_s;            // slots of each kind
     int tiles_p, tiles_s;            // row tiles of each kind
-    unsigned line, line_ctas;        // k_paged_wide's runs over the shared positions: total length (0: none), and CTAs
+    unsigned line, line_ctas;        // k_paged_wide's runs over the shared positions: total length (0: none), CTAs,
+    int line_tp, line_rows;          // positions per place of the line, rows per row tile
 };
-constexpr int kPaWidePair = 0, kPaWideSplit = -1;    // k_paged_wide: two tiles of 128 rows; one, in two streams
+constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2;   // k_paged_wide: 256 rows; 128; 128 over an fp32 cache
 
 // A line of `line` places in n runs, the first line % n of them one place longer: where run i starts, and which run
 // holds place x. (32 bits: a 64-bit division costs the kernels some 500 cycles.)

@@ -8,6 +8,7 @@
 // once per stage in shared memory, and three products kept (lo * lo is below 2^-22); the tf32 form of the same
 // (m16n8k8, three products, split in every warp) took about twice as long.
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -38,16 +39,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Biased exponent of the largest finite |value|, as an ordered integer: of one value (0 if it is not finite).
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
-}
-// Values whose largest has the biased exponent e go to 2^9 .. 2^10 when multiplied by 2^(up - 127), which
-// 2^(127 - up) undoes; both are normal numbers.
-__device__ __forceinline__ uint32_t scale_up(uint32_t e) { return e == 0 ? 127u : min(263u - e, 253u); }
-__device__ __forceinline__ float pow2_bits(uint32_t biased) { return __uint_as_float(biased << 23); }
-
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
 // A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows x WK groups of
 // positions x WD parts of head_dim (in the second product; the first is done by each). K and V come in
@@ -581,8 +572,9 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
     __shared__ float s_x[WPR > 1 ? 8 : 1][D], s_l[8];
     const Paged &a = A.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
-    const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + warp / WPR, rows = (int64_t)a.n_tok * a.H;
-    const int t = (int)(row / a.H), slots = A.p.slots_p + A.p.slots_s;
+    const unsigned row = blockIdx.x * (8 / WPR) + warp / WPR, t = row / (unsigned)a.H;
+    const int64_t rows = (int64_t)a.n_tok * a.H;
+    const int slots = A.p.slots_p + A.p.slots_s;
     pdl_trigger();
     pdl_wait();
     const bool there = row < rows;
@@ -607,24 +599,19 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
         int t0 = 0, n = 0, kv = 0;
         const int b = paged_seq_of(a, t);
         if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
-        const int pos = t >= t0 && t < t0 + n ? kv - n + (t - t0) : -1;
+        const int pos = (int)t >= t0 && (int)t < t0 + n ? kv - n + ((int)t - t0) : -1;
         if (pos >= 0) {                           // the slots of chunks that begin past the row's position are not written
-            // slots of a kind up to place d of it: one per chunk, or two where k_paged_wide has two streams
-            auto upto = [](int d, int chunk, int wr) {
-                const int c = d / chunk;
-                return wr == kPaWideSplit ? 2 * c + (d - c * chunk >= 128 ? 2 : 1) : c + 1;
-            };
             if (a.prefix > 0) {
                 const int d = min(pos, a.prefix - 1);
                 if (A.p.line > 0) {
-                    const unsigned h = (unsigned)(row - (int64_t)t * a.H), kh = h / a.G, nt = (a.prefix + 127) / 128;
-                    const unsigned y = ((t * a.G + h - kh * a.G) / 256 * a.Hk + kh) * nt;
-                    np = line_run(y + d / 128, A.p.line, A.p.line_ctas) - line_run(y, A.p.line, A.p.line_ctas) + 1;
+                    const unsigned h = row - t * a.H, kh = h / a.G, tp = A.p.line_tp, nt = (a.prefix + tp - 1) / tp;
+                    const unsigned y = ((t * a.G + h - kh * a.G) / (unsigned)A.p.line_rows * a.Hk + kh) * nt;
+                    np = line_run(y + d / tp, A.p.line, A.p.line_ctas) - line_run(y, A.p.line, A.p.line_ctas) + 1;
                 } else {
-                    np = upto(d, A.p.chunk_p, A.p.wr_p);
+                    np = d / A.p.chunk_p + 1;
                 }
             }
-            const int ns = np + (pos < a.prefix ? 0 : upto(pos - A.p.base_s, A.p.chunk_s, A.p.wr_s));
+            const int ns = np + (pos < a.prefix ? 0 : (pos - A.p.base_s) / A.p.chunk_s + 1);
             const bool dense = np == A.p.slots_p || ns == np;              // slot s is where the fetch above took it
             float M = -INFINITY;
             float2 ml = make_float2(-INFINITY, 0.0f);
@@ -675,19 +662,23 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
             for (int j = 0; j < J; j++) x[j] += s_x[warp + k][lane * J + j];
     }
     if (!there) return;
-    float *dst = A.out + t * A.ldo + (row - (int64_t)t * a.H) * D + lane * J;
+    float *dst = A.out + t * A.ldo + (int64_t)(row - t * a.H) * D + lane * J;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if constexpr (J == 4) *reinterpret_cast<float4 *>(dst) = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     else *reinterpret_cast<float2 *>(dst) = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x[0] * inv, x[1] * inv);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); an fp16 cache
-// in pages of 8 positions or more (a swizzle unit of k_paged_wide's tiles) and more rows than that: k_paged_wide.
+// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); k_paged_wide for
+// more rows over an fp16 cache in pages of 8 positions or more (a swizzle unit of its tiles), and over fp32 caches.
 static int row_groups(int type, int page_log, int64_t rows) {
+    static const int f32min = getenv("QMS_F32MIN") ? atoi(getenv("QMS_F32MIN")) : 17;
+    if (type != QMS_T_F16 && rows >= f32min) return kPaWideF32;
     if (type == QMS_T_F16 && rows > 64 && page_log >= 3) return rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
 }
+static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
+static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : wr == kPaWideF32 ? 64 : 128; }
 
 // Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
 // of resident CTAs, stages of `stage` positions (us each, us_unit once per unit) and 1 KB of partial results
@@ -706,35 +697,34 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
 }
 
 static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
-    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, 128, 148, 3.0, 6.0);
-    if (wr == kPaWideSplit) return chunk_of(len, tiles, 2 * rows, 256, 148, 3.0, 6.0);
+    const int tp = tile_positions(type, wr);
+    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0);
+    if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0);
     const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
-    return chunk_of(len, tiles, rows, pa_stage(type), 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0);
+    return chunk_of(len, tiles, rows, tp, 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0);
 }
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
+    memset(&p, 0, sizeof p);
     p.wr_p = row_groups(type, a.page_log, rows_p);
     p.wr_s = row_groups(type, a.page_log, rows_s);
-    p.base_s = a.prefix & ~(std::min(1 << a.page_log, p.wr_s <= 0 ? 128 : pa_stage(type)) - 1);
+    p.base_s = a.prefix & ~(std::min(1 << a.page_log, tile_positions(type, p.wr_s)) - 1);
     const int own = std::max(0, a.max_kv - p.base_s);
-    auto height = [](int wr) { return wr == kPaWidePair ? 256 : wr == kPaWideSplit ? 128 : 16 * wr; };
-    p.tiles_p = (int)((rows_p + height(p.wr_p) - 1) / height(p.wr_p));
-    p.tiles_s = (int)((rows_s + height(p.wr_s) - 1) / height(p.wr_s));
+    p.tiles_p = (int)((rows_p + tile_rows(p.wr_p) - 1) / tile_rows(p.wr_p));
+    p.tiles_s = (int)((rows_s + tile_rows(p.wr_s) - 1) / tile_rows(p.wr_s));
     p.chunk_p = chunk_for(type, p.wr_p, a.prefix, (int64_t)p.tiles_p * a.Hk, all);
     p.chunk_s = chunk_for(type, p.wr_s, own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all);
-    p.chunks_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
-    p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
-    p.slots_p = p.chunks_p * (p.wr_p == kPaWideSplit ? 2 : 1);
-    p.slots_s = p.chunks_s * (p.wr_s == kPaWideSplit ? 2 : 1);
-    p.line = 0;
-    p.line_ctas = 0;
-    const int64_t nt = (a.prefix + 127) / 128, line = nt * p.tiles_p * a.Hk;
-    if (p.wr_p == kPaWidePair && line > 0 && line < (1ll << 31)) {
+    p.slots_p = p.chunks_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
+    p.slots_s = p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
+    if (p.wr_p <= 0 && p.chunks_p > 0 && p.tiles_p > 0) {
+        p.line_tp = tile_positions(type, p.wr_p);
+        p.line_rows = tile_rows(p.wr_p);
+        const int64_t nt = (a.prefix + p.line_tp - 1) / p.line_tp, line = nt * p.tiles_p * a.Hk;
         p.line = (unsigned)line;
         p.line_ctas = (unsigned)std::min<int64_t>(148, line);
         // a row tile's positions meet at most this many runs
-        p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / (p.line / p.line_ctas) + 2);
+        p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / (line / p.line_ctas) + 2);
     }
 }
 
@@ -818,6 +808,8 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     A.ldo = ldo;
     A.scale2 = scale * 1.4426950408889634f;
     A.part_o = (float *)ws;
+    // (32-bit run arithmetic)
+    QMS_REQUIRE((int64_t)p.tiles_p * a.Hk * ((a.prefix + 63) / 64) < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     A.part_ml = (float2 *)((char *)ws + al256((int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H * D * 4));
     int rc;
     if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, s) : launch_attn<64, __half>(A, s);

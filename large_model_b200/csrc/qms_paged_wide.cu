@@ -1,30 +1,37 @@
-// qms_paged_wide.cu - paged attention where one K / V tile meets many rows (a shared prompt against a batch, drafted
-// tokens, a chunk of a prompt): tcgen05 tensor cores, fp16 cache, on B200 (sm_100a).
+// qms_paged_wide.cu - paged attention on tcgen05 tensor cores (B200, sm_100a): for many rows per K / V tile (a shared
+// prompt against a batch, drafted tokens, a chunk of a prompt), and for fp32 caches.
 //
-// A unit is a run of positions, 128 at a time, of one kv head against 256 rows (two tiles of 128: PAIR) or, where there
-// are no more than 128 rows, against one tile whose even and odd position tiles are two streams with an O and
-// a softmax of their own (SPLIT): either way the tensor cores have one stream to work on while the other's
-// softmax runs.
-//   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128 x N 128, K = head_dim, twice: Q = hi + lo
-//               in fp16 (22 bits, each row scaled by a power of two into fp16's range), K exact
+// A unit is a run of positions, a tile at a time, of one kv head against rows; two streams of tiles take turns, so
+// that the tensor cores work on one while the other's softmax runs:
+//   PAIR   fp16 cache, 256 rows: a stream per 128 rows, both over every tile of 128 positions
+//   SPLIT  fp16 cache, 128 rows: the even and the odd tiles, joined at the end of the unit
+//   F32    fp32 cache, 128 rows: the same with tiles of 64 positions, split into fp16 terms on the way
+// For each tile of a stream
+//   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128, N the positions, K = head_dim, with 22-bit operands: Q =
+//               hi + lo in fp16 (each row scaled by a power of two into fp16's range), K exact in fp16 (two
+//               products) or K = hi + lo, each row scaled (three: lo * lo is below 2^-22)
 //   softmax     one thread per row reads its S from TMEM, keeps the running base B and sum l, writes the
 //               weights 2^(s f - B) back over S as two fp16 terms
-//   O += P V    tcgen05.mma with P from TMEM (hi, then lo) and V as it lies in shared memory (MN-major)
+//   O += P V    tcgen05.mma with P from TMEM (hi, lo) and V as it lies in shared memory (MN-major), fp32 V = hi + lo
+//               under the largest scale so far (O is in its units)
 // O stays in TMEM over the whole unit. A base is set 2^8 below a maximum and stays until a score lies 2^15 above it
 // (fp16 holds weights to 2^16), so that the maximum needs no pass of its own; the result does not depend on
 // it beyond rounding.
 //
-// Warps 0-3 and 4-7 are the softmax of the two streams, warp 8 brings K and V in by TMA (a box of 64 values x up to 128
-// positions per page, swizzled), warp 9 clears values that are not finite out of V rows that some row does
-// not see (a weight of 0 does not cancel them), one thread each of warps 10 and 11 issues the MMAs of a stream, 16 or
-// 32 at a time under a lock: one thread for both leaves the tensor cores idle while it waits and commits (some
-// 1200 of 6150 cycles per pair of tiles: hardly one MMA is queued), two that interleave slow every MMA down. Tiles start on a
-// page boundary (or, in larger pages, a multiple of 128), so a tile may begin before the first position of its
-// unit; such rows are masked. Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB, or (SPLIT) Q 64 KB and a
-// ring of 2 for each stream; TMEM: S 2 x 128, O 2 x 128 columns.
-// Bound by the tensor cores: 4 * 128 * 128 * head_dim flop per tile and product pair, twice for the split.
+// Warps 0-3 and 4-7 are the softmax of the two streams. One warp brings K and V in by TMA, a box per page: 64 swizzled
+// values x the page's positions (fp32: whole rows, into a staging ring, from which four warps write the terms). Tiles
+// start on page boundaries, so a tile may begin before the first position of its unit: such rows are masked. V
+// values that are not finite in rows that some row does not see are set aside (a weight of 0 does not cancel
+// them), by one warp or by the four. One thread each of two warps issues the MMAs of a stream, a product at a time
+// under a lock: one thread for both leaves the tensor cores idle while it waits and commits (some 1200 of 6150 cycles
+// per pair of tiles: hardly one MMA is queued), two that interleave slow every MMA down.
+// Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB (PAIR), Q 64 KB and a ring of 2 for each stream
+// (SPLIT), Q 64 KB, 2 stages and a ring of 3 (F32); TMEM: S 2 x 128, O 2 x 128 columns.
+// Bound by the tensor cores: 4 * 128 * 128 * head_dim flop per 128 rows and positions, times 2 (fp16) or 3.
 #include <math.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "qms_moe.cuh"
 #include "qms_paged.cuh"
@@ -32,24 +39,29 @@
 
 namespace qms {
 
-constexpr int kWTile = 128, kWThreads = 384;         // 12 warps: 168 registers each
+enum { PAIR, SPLIT, F32 };
 constexpr uint32_t kWSpin = 1u << 22;
 constexpr float kWLow = 8.0f, kWHigh = 15.0f;       // a new base is 2^8 below the maximum; weights stay below 2^15
 
-template <int D, bool SPLIT>
+template <int D, int MODE>
 struct WideCfg {
+    static constexpr int TP = MODE == F32 ? 64 : 128, ROWS = MODE == PAIR ? 256 : 128;     // positions per tile, rows per unit
+    static constexpr int THREADS = MODE == F32 ? 480 : 384, REGS = MODE == F32 ? 128 : 168;    // (4, 3 warps per scheduler)
+    static constexpr int TMA_WARP = MODE == F32 ? 12 : 8, MMA_WARP = MODE == F32 ? 13 : 10;
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
-    static constexpr uint32_t HALF = kWTile * 128;              // bytes of 128 rows x 64 values
-    static constexpr uint32_t TILE = HALVES * HALF;             // a K or V tile; one term of a Q tile
-    static constexpr int SLOTS = SPLIT ? 4 : 3, CH = D / 8;     // CH: 16-byte pieces per row
-    static constexpr uint32_t RING = (SPLIT ? 2 : 4) * TILE, META = RING + SLOTS * TILE;
-    // meta: bad-page masks [8][4], barriers, flags
-    static constexpr uint32_t BAD = META, BARS = BAD + 128, SMEM = BARS + (3 * SLOTS + 9) * 8 + 32;
+    static constexpr uint32_t QHALF = 128 * 128, QTILE = HALVES * QHALF;     // one term of 128 rows of Q
+    static constexpr uint32_t HALF = TP * 128, TILE = HALVES * HALF;         // one term of a K or V tile
+    static constexpr uint32_t SLOT = (MODE == F32 ? 2 : 1) * TILE;
+    static constexpr int SLOTS = MODE == SPLIT ? 4 : 3;
+    static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT, STAGED = MODE == F32 ? TP * D * 4 : 0;
+    // then: bad-page masks [8][4]; scales of K rows [4][64], of V [4], maxima [2][4]; a stream's (B, l, V scale) by
+    // row; barriers; flags
+    static constexpr uint32_t BAD = STAGE + 2 * STAGED, FK = BAD + 128, VUP = FK + (MODE == F32 ? 1024 : 0), JOIN = VUP + 48,
+                              BARS = JOIN + (MODE == PAIR ? 0 : 128 * 12), SMEM = BARS + 24 * 8 + 32;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
-    // load n of a ring: its slot and the parity of that slot's phase. (A ring per stream in SPLIT: whoever waits
-    // for a slot waits for each of its phases.)
-    static constexpr uint32_t RINGLEN = SPLIT ? 2 : 3;
-    static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return SPLIT ? 2 * stream + (n & 1) : n % 3; }
+    // Load n of a ring (K, V, K, ...): its slot. One ring for both streams; in SPLIT a ring per stream.
+    static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return MODE == SPLIT ? 2 * stream + (n & 1) : n % 3; }
+    static constexpr uint32_t RINGLEN = MODE == SPLIT ? 2 : 3;
     static __device__ __forceinline__ uint32_t phase(uint32_t n) { return n / RINGLEN & 1; }
 };
 
@@ -119,103 +131,100 @@ struct WideSync {
 
 // One unit of work, as every role derives it.
 struct WideUnit {
-    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, tiles, lo;
+    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, lo;
     // kv head; sequence, its first row, rows and length (own); slot of the partial result; positions [k0, k1) in
     // nt tiles, of which those below kmin belong to another unit; first row and number of rows of the
-    // segment; row tiles (1 or 2); every row of the unit sees the positions up to lo
+    // segment; every row of the unit sees the positions up to lo
 };
 
 // The units of this CTA in order. Own positions: units blockIdx.x, + gridDim.x, ... of (chunk, sequence, row tile, kv
-// head). Shared positions against pairs of row tiles: all (row tile, kv head, position tile) triples in one line, cut
-// into equal runs, one per CTA; a run is one unit per row tile and kv head that it crosses.
+// head). Shared positions: all (row tile, kv head, position tile) triples in one line, cut into equal runs, one per
+// CTA; a run is one unit per row tile and kv head that it crosses.
+template <class C>
 struct WideWork {
     const PagedAttn &A;
-    const bool own, line;
+    const bool own;
     const int lo_p;
     unsigned x, end;
-    __device__ WideWork(const PagedAttn &A_, bool own_, int lo_p_) : A(A_), own(own_), line(!own_ && A_.p.line > 0), lo_p(lo_p_) {
-        if (line) {
+    __device__ WideWork(const PagedAttn &A_, bool own_, int lo_p_) : A(A_), own(own_), lo_p(lo_p_) {
+        if (own) {
+            x = blockIdx.x;
+            end = (unsigned)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk;
+        } else {
             x = line_start(blockIdx.x, A.p.line, gridDim.x);
             end = line_start(blockIdx.x + 1, A.p.line, gridDim.x);
-        } else {
-            x = blockIdx.x;
-            end = (unsigned)(own ? A.p.chunks_s * A.a.n_seq * A.p.tiles_s : A.p.chunks_p * A.p.tiles_p) * A.a.Hk;
         }
     }
     __device__ bool next(WideUnit &w) {
         const Paged &a = A.a;
-        const unsigned rows_tile = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit ? kWTile : 2 * kWTile;
-        for (; x < end;) {
+        while (x < end) {
             w.b = w.t0 = w.n = w.kv = 0;
-            if (line) {
-                const unsigned nt = (a.prefix + kWTile - 1) / kWTile, u = x / nt, j = x - u * nt, c = min(nt - j, end - x);
-                const unsigned tile = u / a.Hk;
-                w.kh = u - tile * a.Hk;
-                w.r0 = tile * rows_tile;
-                w.slot = blockIdx.x - line_run(u * nt, A.p.line, gridDim.x);
-                w.k0 = w.kmin = j * kWTile;
-                w.k1 = min(a.prefix, (int)(j + c) * kWTile);
-                x += c;
-            } else {
-                unsigned u = x;
+            if (own) {
+                unsigned u = x, d = u / a.Hk;
                 x += gridDim.x;
-                unsigned d = u / a.Hk;
                 w.kh = u - d * a.Hk;
                 u = d;
-                const unsigned nr = own ? A.p.tiles_s : A.p.tiles_p;
-                d = u / nr;
-                w.r0 = (u - d * nr) * rows_tile;
+                d = u / (unsigned)A.p.tiles_s;
+                w.r0 = (u - d * A.p.tiles_s) * C::ROWS;
                 u = d;
-                if (own) {
-                    d = u / a.n_seq;
-                    w.b = u - d * a.n_seq;
-                    u = d;
-                    paged_seq(a, w.b, w.t0, w.n, w.kv);
-                    w.k0 = A.p.base_s + u * A.p.chunk_s;
-                    w.kmin = max(w.k0, a.prefix);
-                    w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
-                    w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (int)(w.r0 + rows_tile - 1) / a.G) + 1);     // nobody sees the rest
-                } else {
-                    w.k0 = w.kmin = u * A.p.chunk_p;
-                    w.k1 = min(a.prefix, w.k0 + A.p.chunk_p);
-                }
-                w.slot = (own ? A.p.slots_p : 0) + u * (rows_tile == kWTile ? 2 : 1);
+                d = u / a.n_seq;
+                w.b = u - d * a.n_seq;
+                paged_seq(a, w.b, w.t0, w.n, w.kv);
+                w.k0 = A.p.base_s + d * A.p.chunk_s;
+                w.kmin = max(w.k0, a.prefix);
+                w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
+                w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (w.r0 + C::ROWS - 1) / a.G) + 1);     // nobody sees the rest
+                w.slot = A.p.slots_p + d;
+                w.rows = w.n * a.G;
+                w.lo = w.kv - w.n + w.r0 / a.G;
+            } else {
+                const unsigned nt = (a.prefix + C::TP - 1) / C::TP, u = x / nt, j = x - u * nt, c = min(nt - j, end - x), tile = u / a.Hk;
+                x += c;
+                w.kh = u - tile * a.Hk;
+                w.r0 = tile * C::ROWS;
+                w.slot = blockIdx.x - line_run(u * nt, A.p.line, gridDim.x);
+                w.k0 = w.kmin = j * C::TP;
+                w.k1 = min(a.prefix, (int)(j + c) * C::TP);
+                w.rows = a.n_tok * a.G;
+                w.lo = lo_p;
             }
-            w.rows = own ? w.n * a.G : a.n_tok * a.G;
-            w.lo = own ? w.kv - w.n + w.r0 / a.G : lo_p;
-            w.nt = (w.k1 - w.k0 + kWTile - 1) / kWTile;
-            w.tiles = w.rows - w.r0 > kWTile ? 2 : 1;
+            w.nt = (w.k1 - w.k0 + C::TP - 1) / C::TP;
             if (w.r0 < w.rows && w.kmin < w.k1) return true;
         }
         return false;
     }
 };
 
-template <int D, bool SPLIT>
-__global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                                             const bool own, const bool last) {
-    using C = WideCfg<D, SPLIT>;
+template <int D, int MODE>
+__global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAttn A, const __grid_constant__ CUtensorMap mk,
+                                                                 const __grid_constant__ CUtensorMap mv, const bool own, const bool last) {
+    using C = WideCfg<D, MODE>;
     extern __shared__ __align__(1024) unsigned char sm[];
     const Paged &a = A.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sm0 = smem_u32(sm);
     uint32_t *s_bad = reinterpret_cast<uint32_t *>(sm + C::BAD);
-    uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + C::SLOTS, *landed = empty + C::SLOTS;
-    uint64_t *staged = landed + C::SLOTS, *q_free = staged + 1, *q_full = q_free + 1, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
-    int *s_int = reinterpret_cast<int *>(drain + 1);              // abort, V set aside, TMEM base, least position
+    float *s_fk = reinterpret_cast<float *>(sm + C::FK);          // what undoes the scale of each K row, at tile & 3 (F32)
+    uint32_t *s_vup = reinterpret_cast<uint32_t *>(sm + C::VUP), *s_max = s_vup + 4;
+    float *s_join = reinterpret_cast<float *>(sm + C::JOIN);
+    // full, empty: of the ring's slots (F32: `full` is of stream i's K, i, and V, 2 + i); landed: V tiles that go on
+    // after a look, or (F32) the stages, at 2 + i when they are free again
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + 4, *landed = empty + 4;
+    uint64_t *joined = landed + 4, *q_full = joined + 1, *s_full = q_full + 2, *p_full = s_full + 2, *drain = p_full + 2;
+    int *s_int = reinterpret_cast<int *>(drain + 1);              // abort, V set aside, TMEM base, least position, lock
     volatile int *s_abort = s_int, *s_flag = s_int + 1;
-    int *s_lo = s_int + 3, *s_lock = s_int + 4;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(s_int + 2);
+    int *s_lo = s_int + 3, *s_lock = s_int + 4;
     if (sm0 & 1023) {                             // the swizzled tiles need it; never seen
         if (tid == 0) paged_err(a, QMS_PAGED_ETIMEOUT);
         pdl_wait();
         return;
     }
     if (tid == 0) {
-        for (int i = 0; i < C::SLOTS; i++) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], SPLIT ? 1 : 2);
-            mbar_init(&landed[i], 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(&full[i], MODE == F32 ? 128 : 1);
+            mbar_init(&empty[i], MODE == PAIR ? 2 : 1);
+            mbar_init(&landed[i], MODE == F32 && i >= 2 ? 4 : 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 128);
@@ -223,13 +232,12 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
             mbar_init(&p_full[i], 4);
         }
         mbar_init(drain, 2);
-        mbar_init(staged, 4);
-        mbar_init(q_free, 2);
+        mbar_init(joined, 4);
         s_int[0] = s_int[1] = *s_lock = 0;
         *s_lo = 0x7fffffff;
         fence_mbar_init();
     }
-    if (warp == 11) {
+    if (warp == C::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -241,7 +249,7 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     const uint32_t tmem = *s_tmem;
     if (!own) {                                   // the least position among all rows: what lies below needs no mask
         int lo = 0x7fffffff;
-        for (int b = tid; b < a.n_seq; b += kWThreads) {
+        for (int b = tid; b < a.n_seq; b += C::THREADS) {
             int t0, n, kv;
             if (paged_seq(a, b, t0, n, kv) && n > 0) lo = min(lo, kv - n);
         }
@@ -251,19 +259,22 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     }
     const int lo_p = *s_lo;
     const WideSync sy{s_abort, &a};
-    WideWork work(A, own, lo_p);
-    WideUnit w;
+    WideWork<C> work(A, own, lo_p);
+    WideUnit w = {};
+    // the tiles of stream i in a unit of nt: all (PAIR, where it has rows), or every second
+    auto tiles_of = [&](int i) { return MODE == PAIR ? (w.rows - w.r0 > 128 * i ? w.nt : 0) : (w.nt + 1 - i) / 2; };
 
     if (warp < 8) {
         // ---- softmax of stream i: thread = row = TMEM lane
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t s_col = lanes + i * kWTile, o_col = lanes + C::O_COL + i * D;
-        uint32_t ns = 0, before = 0, unit_no = 0; // phases of s_full; position tiles of the CTA's earlier units (for s_bad)
+        const uint32_t s_col = lanes + i * 128, o_col = lanes + C::O_COL + i * D;
+        uint32_t ns = 0, nv = 0, before = 0, unit_no = 0;      // phases of s_full, of V; position tiles, units before
         bool ok = true;
         for (; ok && work.next(w); before += w.nt, unit_no++) {
-            if (!SPLIT && i >= w.tiles) continue;
-            const int r = w.r0 + (SPLIT ? 0 : i * kWTile) + row, t = r / a.G;    // this row: its token, position below
+            const int nt = tiles_of(i);
+            if (MODE == PAIR && nt == 0) continue;
+            const int r = w.r0 + (MODE == PAIR ? i * 128 : 0) + row, t = r / a.G;    // this row: its token, position below
             int tok = -1;                                                        // token row * H + head (-1: none)
             int64_t qo = -1;                                                     // where its q is
             if (r < w.rows) {
@@ -272,10 +283,9 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 qo = (w.t0 + t) * A.ldq + (int64_t)h * D;
             }
             // q: 8 lanes per row, 4 rows at a time: row maximum, power-of-two scale, two fp16 terms, swizzled
-            // rows (SPLIT: one stream writes them for both, the other one only wants the scales)
+            // rows (one tile: stream 0 writes them, stream 1 only wants the scales)
             float f = 0.0f;
             const uint32_t sign = A.scale2 < 0.0f ? 0x80000000u : 0u;  // f >= 0: the largest s f has the largest s
-            float4 x[2][4][D / 32];
             auto fetch = [&](float4 (&z)[4][D / 32], int g0) {         // 16 rows of the warp
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
@@ -294,33 +304,42 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-                    // the maximum goes to 2^9 .. 2^10: times 2^(up - 127), undone by 2^(127 - up) in the score
-                    const uint32_t up = mx == 0.0f ? 127u : min(263u - (__float_as_uint(mx) >> 23), 253u);
-                    const float got = __shfl_sync(kFull, fabsf(A.scale2) * __uint_as_float((254u - up) << 23), (lane & 3) * 8);
+                    const uint32_t up = scale_up(__float_as_uint(mx) >> 23);
+                    const float got = __shfl_sync(kFull, fabsf(A.scale2) * pow2_bits(254u - up), (lane & 3) * 8);
                     if (lane >> 2 == g0 + g) f = got;
-                    if (SPLIT && i == 1) continue;
+                    if (MODE != PAIR && i == 1) continue;
                     const float m = __uint_as_float(up << 23 | sign);
                     const int rr = (warp & 3) * 32 + 4 * (g0 + g) + (lane >> 3);
-                    const uint32_t at = sm0 + (SPLIT ? 0 : i * 2 * C::TILE) + rr * 128 + (lane & 1) * 8;
+                    const uint32_t at = sm0 + (MODE == PAIR ? i * 2 * C::QTILE : 0) + rr * 128 + (lane & 1) * 8;
 #pragma unroll
                     for (int k = 0; k < D / 32; k++) {
                         const float2 y0 = f2_mul(make_float2(z[g][k].x, z[g][k].y), make_float2(m, m)), y1 = f2_mul(make_float2(z[g][k].z, z[g][k].w), make_float2(m, m));
                         const float2 h0 = make_float2(tf32_hi(y0.x), tf32_hi(y0.y)), h1 = make_float2(tf32_hi(y1.x), tf32_hi(y1.y));
                         const float2 l0 = f2_fma(h0, make_float2(-1.0f, -1.0f), y0), l1 = f2_fma(h1, make_float2(-1.0f, -1.0f), y1);
                         // values 4 (lane & 7) + 32 k .. + 3: 16-byte piece (lane & 7) / 2 + 4 (k & 1) of half k / 2
-                        const uint32_t to = at + (k >> 1) * C::HALF + (((((lane & 7) >> 1) + 4 * (k & 1)) ^ (rr & 7)) << 4);
+                        const uint32_t to = at + (k >> 1) * C::QHALF + (((((lane & 7) >> 1) + 4 * (k & 1)) ^ (rr & 7)) << 4);
                         asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(pack_h2(h0.x, h0.y)), "r"(pack_h2(h1.x, h1.y)) : "memory");
-                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + C::TILE), "r"(pack_h2(l0.x, l0.y)), "r"(pack_h2(l1.x, l1.y)) : "memory");
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + C::QTILE), "r"(pack_h2(l0.x, l0.y)), "r"(pack_h2(l1.x, l1.y)) : "memory");
                     }
                 }
             };
-            fetch(x[0], 0);
-            fetch(x[1], 4);
-            if (SPLIT && i == 0 && unit_no > 0 && !(ok = __all_sync(kFull, sy.wait(staged, (unit_no - 1) & 1)))) break;
-            place(x[0], 0);
-            place(x[1], 4);
+            if constexpr (MODE != F32) {
+                float4 x[2][4][D / 32];
+                fetch(x[0], 0);
+                fetch(x[1], 4);
+                place(x[0], 0);
+                place(x[1], 4);
+            } else {
+#pragma unroll 1
+                for (int g = 0; g < 8; g += 4) {
+                    float4 x[4][D / 32];
+                    fetch(x, g);
+                    place(x, g);
+                }
+            }
+            f = fmaxf(f, 1.17549435e-38f);        // (0 would make NaN of a masked score, -inf)
             fence_async_smem();
-            if (!SPLIT || i == 0) mbar_arrive(&q_full[i]);
+            if (MODE == PAIR || i == 0) mbar_arrive(&q_full[i]);
             int pos = -1;
             if (own) {
                 if (r < w.rows) pos = w.kv - w.n + t;
@@ -337,18 +356,32 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
             const int lim = min(pos, w.k1 - 1);   // last position that this row sees
             float B = -INFINITY;
             float2 l2 = make_float2(0.0f, 0.0f);
-            for (int j = SPLIT ? i : 0; j < w.nt; j += SPLIT ? 2 : 1) {
+            uint32_t vup = 0;                     // F32: the scale of V that O is in
+            // O times a power of 2 (the MMAs on it ended before the S at hand was announced)
+            auto scale_o = [&](float fac) {
+#pragma unroll 1
+                for (int k = 0; k < D / 32; k++) {
+                    uint32_t o[32];
+                    tmem_ld<32>(o_col + 32 * k, o);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+                    tmem_st32(o_col + 32 * k, o);
+                }
+            };
+            for (int n = 0; n < nt; n++) {
+                const int j = MODE == PAIR ? n : 2 * n + i, base = w.k0 + j * C::TP;
                 if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;    // the whole warp or none of it
                 ns++;
                 tc_fence_after();
-                const int base = w.k0 + j * kWTile;
                 const uint32_t *bad = s_bad + ((before + j) & 7) * 4;
+                uint32_t any_bad = bad[0] | bad[1];
+                if constexpr (C::TP == 128) any_bad |= bad[2] | bad[3];
                 // rows that see nothing of this unit are not read from its slot: no mask for them
-                if (__any_sync(kFull, lim >= w.kmin && lim < base + kWTile - 1) || base < w.kmin || (bad[0] | bad[1] | bad[2] | bad[3])) {
+                if (__any_sync(kFull, lim >= w.kmin && lim < base + C::TP - 1) || base < w.kmin || any_bad) {
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        const int d = lim - base - 32 * c;
-                        const int below = w.kmin - base - 32 * c;
+                    for (int c = 0; c < C::TP / 32; c++) {
+                        const int d = lim - base - 32 * c, below = w.kmin - base - 32 * c;
                         const uint32_t vis = (d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u) & ~bad[c] &
                                              (below <= 0 ? 0xffffffffu : below >= 32 ? 0u : 0xffffffffu << below);
                         uint32_t x[32];
@@ -365,6 +398,17 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 // what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
                 const float2 f2 = make_float2(f, f);
                 auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {
+                    if constexpr (MODE == F32) {
+                        const float4 *fk = reinterpret_cast<const float4 *>(s_fk + ((before + j) & 3) * 64 + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float4 k = fk[e];
+                            z[4 * e] = __float_as_uint(__uint_as_float(z[4 * e]) * k.x);
+                            z[4 * e + 1] = __float_as_uint(__uint_as_float(z[4 * e + 1]) * k.y);
+                            z[4 * e + 2] = __float_as_uint(__uint_as_float(z[4 * e + 2]) * k.z);
+                            z[4 * e + 3] = __float_as_uint(__uint_as_float(z[4 * e + 3]) * k.w);
+                        }
+                    }
                     float mx = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
                     for (int e = 3; e < 31; e += 2) mx = max3(mx, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
@@ -375,17 +419,7 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                         B = nb;
                         l2.x *= fac;
                         l2.y *= fac;
-                        if (j > 1 || (!SPLIT && j > 0)) {      // (the MMAs on O ended before this tile's S was announced)
-#pragma unroll 1
-                            for (int k = 0; k < D / 32; k++) {
-                                uint32_t o[32];
-                                tmem_ld<32>(o_col + 32 * k, o);
-                                tmem_wait_ld(o);
-#pragma unroll
-                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
-                                tmem_st32(o_col + 32 * k, o);
-                            }
-                        }
+                        if (n > 0) scale_o(fac);
                         const __half2 fh = __float2half2_rn(fac);
 #pragma unroll 1
                         for (int k = 0; k < 4; k++) {
@@ -422,48 +456,83 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 tmem_ld<32>(s_col + 32, y);       // the next 32 come while these are worked on
                 weights(x, 0, 0);
                 tmem_wait_ld(y);
-                tmem_ld<32>(s_col + 64, x);
-                weights(y, 1, 1);
-                tmem_wait_ld(x);
-                tmem_ld<32>(s_col + 96, y);
-                weights(x, 2, 3);
-                tmem_wait_ld(y);
-                weights(y, 3, 7);
+                if constexpr (C::TP == 128) {
+                    tmem_ld<32>(s_col + 64, x);
+                    weights(y, 1, 1);
+                    tmem_wait_ld(x);
+                    tmem_ld<32>(s_col + 96, y);
+                    weights(x, 2, 3);
+                    tmem_wait_ld(y);
+                    weights(y, 3, 7);
+                } else {
+                    weights(y, 1, 1);
+                    if (!(ok = __all_sync(kFull, sy.wait(&full[2 + i], nv++ & 1)))) break;     // V's scale is known
+                    const uint32_t up = s_vup[(before + j) & 3];
+                    if (up != vup && n > 0) scale_o(vup - up > 126 ? 0.0f : pow2_bits(127u - (vup - up)));
+                    vup = up;
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[i]);
             }
-            if (SPLIT && i >= w.nt) {             // no position tile for this stream
-                if (lane == 0) mbar_arrive(staged);
-                continue;
+            if (!ok) break;
+            if (nt > 0) {                         // O is complete
+                if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;
+                ns++;
+                tc_fence_after();
+            } else if (!(ok = __all_sync(kFull, sy.wait(&q_full[0], unit_no & 1)))) {          // not before the last unit is read
+                break;
             }
-            if (!ok || !(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;     // O is complete
-            ns++;
-            tc_fence_after();
-            // SPLIT: Q, where the rows are staged, is both streams'
-            if (SPLIT && !(ok = __all_sync(kFull, sy.wait(q_free, unit_no & 1)))) break;
-            const float l = l2.x + l2.y;
+            float l = l2.x + l2.y;
             if (isnan(l) && B == -INFINITY) B = 0.0f;
-            const bool put = tok >= 0 && lim >= (SPLIT && i ? w.k0 + kWTile : w.kmin), none = l == 0.0f, fix = *s_flag != 0;
-            const int64_t first = (int64_t)(w.slot + (SPLIT ? i : 0)) * a.n_tok * a.H;
+            float w0 = MODE == F32 && nt > 0 ? pow2_bits(254u - vup) : 1.0f, w1 = 0.0f;
+            if constexpr (MODE != PAIR) {
+                // stream 1 leaves its (B, l, scale); stream 0 reads both O (the same TMEM lanes) and writes the rows
+                if (i == 1) {
+                    s_join[row] = B;
+                    s_join[128 + row] = l;
+                    s_join[256 + row] = w0;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(joined);
+                    continue;                     // (its O stays until the next unit's q is written, by stream 0 after this)
+                }
+                if (!(ok = __all_sync(kFull, sy.wait(joined, unit_no & 1)))) break;
+                tc_fence_after();
+                const float B1 = s_join[row], l1 = s_join[128 + row], M = fmaxf(B, B1);
+                const float c0 = B == -INFINITY ? 0.0f : ex2(B - M), c1 = B1 == -INFINITY ? 0.0f : ex2(B1 - M);
+                w1 = c1 * s_join[256 + row];
+                w0 *= c0;
+                l = c0 * l + c1 * l1;
+                B = M;
+            }
+            const bool put = tok >= 0 && lim >= w.kmin, none = l == 0.0f, fix = *s_flag != 0;
+            const int64_t first = (int64_t)w.slot * a.n_tok * a.H;
             const int row_out = put ? tok : -1;
             float *part = A.part_o + first * D + (lane & 7) * 4;
-            // the rows leave by way of shared memory (where this warp's rows of Q are; SPLIT's second stream: of
-            // their low terms), 128 bytes of a row per 8 lanes
-            unsigned char *stage = sm + i * (SPLIT ? 1 : 2) * C::TILE + (warp & 3) * 4096;
+            // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes
+            unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
                 tmem_ld<32>(o_col + 32 * c, o);
                 tmem_wait_ld(o);
+                if constexpr (MODE != PAIR) {
+                    uint32_t o1[32];
+                    tmem_ld<32>(o_col + D + 32 * c, o1);
+                    tmem_wait_ld(o1);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)  // (a stream that saw nothing: its O may be anything)
+                        o[e] = __float_as_uint((w0 == 0.0f ? 0.0f : __uint_as_float(o[e]) * w0) + (w1 == 0.0f ? 0.0f : __uint_as_float(o1[e]) * w1));
+                }
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
+                    typedef typename std::conditional<MODE == F32, float, __half>::type KT;
                     for (int p = w.kmin; p <= lim; p++) {
-                        if (SPLIT && ((p - w.k0) / kWTile & 1) != i) continue;
                         const int64_t at = paged_at(a, a.table + (own ? (int64_t)w.b * a.table_stride : 0), p);
                         if (at < 0) continue;
-                        const __half *vr = reinterpret_cast<const __half *>(a.v + at + w.kh * a.head_stride) + 32 * c;
+                        const KT *vr = reinterpret_cast<const KT *>(a.v + at + w.kh * a.head_stride) + 32 * c;
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
                             const float v = kv_ld(vr + e);
@@ -484,70 +553,88 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                     if (to >= 0) *reinterpret_cast<uint4 *>(part + (int64_t)to * D + 32 * c) = v;
                 }
             }
-            if (SPLIT && i == 1) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(staged);
-            }
             if (put) A.part_ml[first + tok] = make_float2(none ? -INFINITY : B, l);
             tc_fence_before();
         }
-    } else if (warp < 10) {
-        // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. Warp 8 issues them; V tiles with rows that not every row sees (or that were
-        // not loaded) land on a barrier of their own and are passed on by warp 9.
+    } else if (warp == C::TMA_WARP || (MODE != F32 && warp == 9)) {
+        // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. One warp
+        // issues them; V tiles with rows that not every row sees (or that were not loaded) land on a barrier of their
+        // own and are passed on by the other (F32: all go to the stages, and the converting warps look at them).
         uint32_t c[2] = {0, 0}, t = 0, phases = 0;       // loads so far (SPLIT: of each stream); tiles; of `landed`
         bool ok = true;
-        const int R = min(1 << a.page_log, kWTile), boxes = kWTile / R;        // positions per box, boxes per 64 values
+        const int R = min(1 << a.page_log, C::TP), boxes = C::TP / R;          // positions per box, boxes per half of a row
+        constexpr int STEP = MODE == SPLIT ? 2 : 1, PER = MODE == F32 ? 2 : 1;  // boxes per lane (F32: pages of any size)
         while (ok && work.next(w)) {
             const int *table = a.table + (own ? (int64_t)w.b * a.table_stride : 0);
-            constexpr int STEP = SPLIT ? 2 : 1;
             for (int j0 = 0; ok && j0 < w.nt; j0 += STEP) {
                 const int m = min(STEP, w.nt - j0);
                 for (int k = 0; ok && k < 2 * m; k++) {
                     const bool is_v = k >= m;
-                    const int jj = is_v ? k - m : k, base = w.k0 + (j0 + jj) * kWTile;
-                    const uint32_t n = SPLIT && jj ? c[1]++ : c[0]++, slot = C::slot(jj, n);
-                    // lane x: page of box x (positions base + x R ..); boxes past the unit are not loaded
-                    const int p = base + lane * R;
-                    int page = -1;
-                    if (lane < boxes && p < w.k1) {
-                        page = table[p >> a.page_log];
-                        if ((unsigned)page >= (unsigned)a.n_pages) {
-                            page = -1;
-                            if (warp == 8) paged_err(a, QMS_PAGED_EPAGE);
-                        }
+                    const int jj = is_v ? k - m : k, base = w.k0 + (j0 + jj) * C::TP;
+                    const uint32_t n = MODE == SPLIT && jj ? c[1]++ : c[0]++, slot = C::slot(jj, n);
+                    // lane x: page of box x (positions base + x R ..), and x + 32; boxes past the unit are not loaded
+                    int page[PER];
+                    uint32_t have = 0, missing[PER];
+#pragma unroll
+                    for (int h = 0; h < PER; h++) {
+                        const int i = lane + 32 * h, p = base + i * R;
+                        const bool want = i < boxes && p < w.k1;
+                        page[h] = want ? table[p >> a.page_log] : -1;
+                        const bool good = want && (unsigned)page[h] < (unsigned)a.n_pages;
+                        if (!good) page[h] = -1;
+                        if (want && !good && warp == C::TMA_WARP) paged_err(a, QMS_PAGED_EPAGE);
+                        have += __popc(__ballot_sync(kFull, good));
+                        missing[h] = __ballot_sync(kFull, want && !good);
                     }
-                    const uint32_t have = __ballot_sync(kFull, page >= 0), want = __ballot_sync(kFull, lane < boxes && p < w.k1);
+                    uint32_t any_missing = missing[0];
+                    if constexpr (PER > 1) any_missing |= missing[PER - 1];
                     const int seen = min(w.lo, w.k1 - 1);
-                    const bool scan = is_v && (base + kWTile - 1 > seen || base < w.kmin || want != have);
-                    if (warp == 8) {
-                        if (!is_v && lane < 4) {  // bits of the tile's positions on bad pages
+                    const bool scan = MODE != F32 && is_v && (base + C::TP - 1 > seen || base < w.kmin || any_missing);
+                    if (warp == C::TMA_WARP) {
+                        if (!is_v && lane < C::TP / 32) {     // bits of the tile's positions on bad pages
                             uint32_t bits = 0;
-                            if (want != have)
-                                for (int e = 0; e < 32; e++) bits |= ((want & ~have) >> ((lane * 32 + e) / R) & 1u) << e;
+                            if (any_missing)
+                                for (int e = 0; e < 32; e++) {
+                                    const int i = (lane * 32 + e) / R;
+                                    bits |= ((PER > 1 && i >= 32 ? missing[PER - 1] : missing[0]) >> (i & 31) & 1u) << e;
+                                }
                             s_bad[((t + jj) & 7) * 4 + lane] = bits;
                         }
                         __syncwarp();
-                        if (n >= C::RINGLEN) ok = __all_sync(kFull, sy.wait(&empty[slot], C::phase(n) ^ 1));
+                        uint64_t *bar;
+                        if constexpr (MODE == F32) {
+                            if (n >= 2) ok = __all_sync(kFull, sy.wait(&landed[2 + (n & 1)], (n / 2 - 1) & 1));
+                            bar = &landed[n & 1];
+                        } else {
+                            if (n >= C::RINGLEN) ok = __all_sync(kFull, sy.wait(&empty[slot], C::phase(n) ^ 1));
+                            bar = scan ? &landed[slot] : &full[slot];
+                        }
                         if (!ok) break;
-                        uint64_t *bar = scan ? &landed[slot] : &full[slot];
-                        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * (uint32_t)(R * 128 * C::HALVES));
+                        if (lane == 0) mbar_arrive_expect_tx(bar, have * (uint32_t)(R * D * (MODE == F32 ? 4 : 2)));
                         __syncwarp();
-                        const uint32_t dst = sm0 + C::RING + slot * C::TILE + lane * R * 128;
-                        if (page >= 0)
 #pragma unroll
-                            for (int h = 0; h < C::HALVES; h++) tma_load4(dst + h * C::HALF, is_v ? &mv : &mk, h * 64, w.kh, p & ((1 << a.page_log) - 1), page, bar);
+                        for (int h = 0; h < PER; h++) {
+                            const int i = lane + 32 * h, y = (base + i * R) & ((1 << a.page_log) - 1);
+                            if (page[h] < 0) continue;
+                            if constexpr (MODE == F32)
+                                tma_load4(sm0 + C::STAGE + (n & 1) * C::STAGED + i * R * (D * 4), is_v ? &mv : &mk, 0, w.kh, y, page[h], bar);
+                            else
+#pragma unroll
+                                for (int x = 0; x < C::HALVES; x++)
+                                    tma_load4(sm0 + C::RING + slot * C::SLOT + x * C::HALF + i * R * 128, is_v ? &mv : &mk, x * 64, w.kh, y, page[h], bar);
+                        }
                     } else if (scan) {
-                        ok = __all_sync(kFull, ok && sy.wait(&landed[slot], phases >> slot & 1));
+                        ok = __all_sync(kFull, sy.wait(&landed[slot], phases >> slot & 1));
                         phases ^= 1u << slot;
-                        for (int x = lane; ok && x < kWTile * C::CH; x += 32) {
-                            const int r = x / C::CH, piece = x % C::CH;
-                            if (base + r >= w.kmin && base + r <= seen && want == have) continue;
-                            uint4 *pv = reinterpret_cast<uint4 *>(sm + C::RING + slot * C::TILE + (piece >> 3) * C::HALF + r * 128 +
+                        for (int x = lane; ok && x < C::TP * (D / 8); x += 32) {
+                            const int r = x / (D / 8), piece = x % (D / 8), p = base + r;
+                            if (p >= w.kmin && p <= seen && !any_missing) continue;
+                            uint4 *pv = reinterpret_cast<uint4 *>(sm + C::RING + slot * C::SLOT + (piece >> 3) * C::HALF + r * 128 +
                                                                   (((piece & 7) ^ (r & 7)) << 4));
                             uint4 v = *pv;
                             if (drop_nonfinite((const __half *)nullptr, v)) {
                                 *pv = v;
-                                if (base + r >= w.kmin && base + r < w.k1) *s_flag = 1;      // (else left over: nobody's)
+                                if (p >= w.kmin && p < w.k1) *s_flag = 1;      // (else left over: nobody's)
                             }
                         }
                         fence_async_smem();
@@ -558,31 +645,127 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 t += m;
             }
         }
+    } else if (MODE == F32 && warp < 12) {
+        // ---- fp32 rows from the stages into hi and lo tiles: K by rows, each with a scale of its own (undone in its scores),
+        // V with the largest scale so far of what somebody sees. A 16-byte piece of a row per lane.
+        constexpr int CH = D / 4, N = C::TP * CH / 128;
+        const int ct = tid - 256, cw = warp - 8;
+        const unsigned peers = CH == 32 ? kFull : 0xffffu << (lane & 16);             // the lanes of a row
+        uint32_t c = 0, t = 0;                    // loads, tiles so far
+        bool ok = true;
+        // largest finite |value|: by float maxima, looked at again where one is inf (NaN is no maximum)
+        auto largest = [](const float4 &y) { return fmaxf(max3(0.0f, fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))); };
+        auto finite4 = [](const float4 &y) { return max(max(finite_bits(y.x), finite_bits(y.y)), max(finite_bits(y.z), finite_bits(y.w))); };
+        while (work.next(w)) {                    // (after a failed wait: the barriers, no work)
+            uint32_t v_exp = 0;
+            const int seen0 = min(w.lo, w.k1 - 1);
+            for (int j = 0; j < w.nt; j++, t++)
+                for (int is_v = 0; is_v < 2; is_v++, c++) {
+                    const int base = w.k0 + j * C::TP;
+                    const float4 *src = reinterpret_cast<const float4 *>(sm + C::STAGE + (c & 1) * C::STAGED);
+                    unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
+                    ok = __all_sync(kFull, ok && sy.wait(&landed[c & 1], c / 2 & 1) && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
+                    auto put = [&](int at, float4 y, float up) {
+                        const int r = at / CH, q = at % CH;           // values 4 q .. + 3 of row r
+                        const float2 y0 = f2_mul(make_float2(y.x, y.y), make_float2(up, up)), y1 = f2_mul(make_float2(y.z, y.w), make_float2(up, up));
+                        uint32_t h[2], l[2];
+                        split_h2(y0.x, y0.y, h[0], l[0]);
+                        split_h2(y1.x, y1.y, h[1], l[1]);
+                        unsigned char *to = dst + (q >> 4) * C::HALF + r * 128 + ((((q & 15) >> 1) ^ (r & 7)) << 4) + (q & 1) * 8;
+                        *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
+                        *reinterpret_cast<uint2 *>(to + C::TILE) = make_uint2(l[0], l[1]);
+                    };
+                    if (!is_v) {
+                        if (ok)
+#pragma unroll 1
+                            for (int h = 0; h < N; h += 4) {
+                                float4 y[4];
+                                uint32_t ky[4];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) y[i] = src[ct + 128 * (h + i)];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const float m = largest(y[i]);
+                                    ky[i] = __reduce_max_sync(peers, m == INFINITY ? finite4(y[i]) : __float_as_uint(m));
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const int at = ct + 128 * (h + i);
+                                    const uint32_t up = scale_up(ky[i] >> 23);
+                                    if (at % CH == 0) s_fk[(t & 3) * 64 + at / CH] = pow2_bits(254u - up);
+                                    put(at, y[i], pow2_bits(up));
+                                }
+                            }
+                    } else {
+                        const uint32_t bad[2] = {s_bad[(t & 7) * 4], s_bad[(t & 7) * 4 + 1]};
+                        const int seen = bad[0] | bad[1] ? -1 : seen0;
+                        float4 x[N];
+                        float mx = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < N; i++) x[i] = src[ct + 128 * i];
+                        if (base + C::TP - 1 > seen || base < w.kmin)
+#pragma unroll
+                            for (int i = 0; i < N; i++) {
+                                const int r = (ct + 128 * i) / CH, p = base + r;
+                                if (p >= w.kmin && p <= seen) continue;
+                                uint4 v = *reinterpret_cast<const uint4 *>(&x[i]);
+                                const bool in = p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1);
+                                if (drop_nonfinite((const float *)nullptr, v)) {
+                                    x[i] = *reinterpret_cast<const float4 *>(&v);
+                                    if (in) *s_flag = 1;
+                                }
+                                if (!in) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);           // no part of the unit
+                            }
+#pragma unroll
+                        for (int i = 0; i < N; i++) mx = fmaxf(mx, largest(x[i]));
+                        uint32_t mb = __float_as_uint(mx);
+                        if (mx == INFINITY) {
+                            mb = 0;
+#pragma unroll
+                            for (int i = 0; i < N; i++) mb = max(mb, finite4(x[i]));
+                        }
+                        mb = __reduce_max_sync(kFull, mb);
+                        uint32_t *s_m = s_max + (t & 1) * 4;
+                        if (lane == 0) s_m[cw] = mb;
+                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                        v_exp = max(v_exp, max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3])) >> 23);
+                        const uint32_t up = scale_up(v_exp);
+                        if (ct == 0) s_vup[t & 3] = up;
+                        if (ok)
+#pragma unroll
+                            for (int i = 0; i < N; i++) put(ct + 128 * i, x[i], pow2_bits(up));
+                    }
+                    fence_async_smem();
+                    mbar_arrive(&full[2 * is_v + (j & 1)]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&landed[2 + (c & 1)]);
+                }
+        }
     } else {
         // ---- the MMAs of stream i, by one thread
-        const int i = warp - 10;
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_f16(kWTile, false), id_o = idesc_f16(D, true);
-            uint32_t c = 0, nq = 0, np = 0;                     // loads of the ring so far; phases of q_full, p_full
+        const int i = warp - C::MMA_WARP;
+        if (lane == 0 && i < 2) {
+            constexpr uint32_t id_s = idesc_f16(C::TP, false), id_o = idesc_f16(D, true);
+            constexpr int TERMS = MODE == F32 ? 3 : 2;          // hi hi, lo hi, (fp32) hi lo
+            uint32_t c = 0, nf = 0, nq = 0, np = 0;             // loads of the ring so far; phases of (F32) full, of q_full, p_full
             bool ok = true;
-            auto score = [&](uint32_t n) {                     // S_i = (hi + lo of Q_i) K^T
-                const uint32_t k = sm0 + C::RING + C::slot(i, n) * C::TILE, q = sm0 + (SPLIT ? 0 : i * 2 * C::TILE);
+            auto score = [&](uint32_t n) {                     // S_i = Q_i K^T
+                const uint32_t k = sm0 + C::RING + C::slot(i, n) * C::SLOT, q = sm0 + (MODE == PAIR ? i * 2 * C::QTILE : 0);
 #pragma unroll
-                for (int term = 0; term < 2; term++)
+                for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++) {
-                        const uint32_t o = (ks >> 2) * C::HALF + (ks & 3) * 32;
-                        umma_f16_ss(tmem + i * kWTile, desc_sw128(q + term * C::TILE + o, 16, 1024), desc_sw128(k + o, 16, 1024), id_s, term || ks);
-                    }
+                    for (int ks = 0; ks < D / 16; ks++)
+                        umma_f16_ss(tmem + i * 128, desc_sw128(q + (term == 1) * C::QTILE + (ks >> 2) * C::QHALF + (ks & 3) * 32, 16, 1024),
+                                    desc_sw128(k + (term == 2) * C::TILE + (ks >> 2) * C::HALF + (ks & 3) * 32, 16, 1024), id_s, term || ks);
             };
-            auto weigh = [&](uint32_t n, bool first) {         // O_i (+)= (hi + lo of P_i) V
-                const uint32_t v = sm0 + C::RING + C::slot(i, n) * C::TILE;
+            auto weigh = [&](uint32_t n, bool first) {         // O_i (+)= P_i V
+                const uint32_t v = sm0 + C::RING + C::slot(i, n) * C::SLOT;
 #pragma unroll
-                for (int term = 0; term < 2; term++)
+                for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                    for (int ks = 0; ks < kWTile / 16; ks++)
-                        umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * kWTile + (ks >> 1) * 32 + term * 16 + (ks & 1) * 8,
-                                    desc_sw128(v + ks * 2048, C::HALF, 1024), id_o, !first || term || ks);
+                    for (int ks = 0; ks < C::TP / 16; ks++)
+                        umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * 128 + (ks >> 1) * 32 + (term == 1) * 16 + (ks & 1) * 8,
+                                    desc_sw128(v + (term == 2) * C::TILE + ks * 2048, C::HALF, 1024), id_o, !first || term || ks);
             };
             auto lock = [&]() {
                 uint32_t x = 0;
@@ -591,13 +774,17 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                 } while (atomicCAS(s_lock, 0, 1) != 0 && x < kWSpin);
             };
             auto unlock = [&]() { *(volatile int *)s_lock = 0; };
-            auto full_at = [&](uint32_t n) { return sy.wait(&full[C::slot(i, n)], C::phase(n)); };
+            // K, V of this stream's tile at load n (K) or n + 1 of the ring; nf: tiles of the stream so far
+            auto k_bar = [&](uint32_t n) { return MODE == F32 ? &full[i] : &full[C::slot(i, n)]; };
+            auto v_bar = [&](uint32_t n) { return MODE == F32 ? &full[2 + i] : &full[C::slot(i, n)]; };
+            constexpr uint32_t NEXT = MODE == F32 ? 4 : 2;      // loads to the stream's next tile
             while (ok && work.next(w)) {
-                // this stream's position tiles; loads c + 2 j (K) and c + 2 j + 1 (V) of its ring are tile j of them
-                const int nt = SPLIT ? (w.nt + 1 - i) / 2 : w.nt;
-                if (SPLIT || i < w.tiles) {
-                    ok = sy.wait(&q_full[SPLIT ? 0 : i], nq++ & 1);
-                    if (ok && nt > 0 && (ok = full_at(c))) {
+                const int nt = tiles_of(i);
+                const uint32_t c1 = c + (MODE == SPLIT ? 2 * nt : 2 * w.nt);
+                if (MODE == F32) c += 2 * i;
+                if (MODE != PAIR || nt > 0) {
+                    ok = sy.wait(&q_full[MODE == PAIR ? i : 0], nq++ & 1);
+                    if (ok && nt > 0 && (ok = sy.wait(k_bar(c), MODE == F32 ? nf & 1 : C::phase(c)))) {
                         tc_fence_after();
                         lock();
                         score(c);
@@ -605,32 +792,37 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
                         umma_commit(&s_full[i]);
                         umma_commit(&empty[C::slot(i, c)]);
                     }
-                    if (SPLIT && ok && nt == 0) mbar_arrive(q_free);
-                    if (SPLIT && ok && nt == 1) umma_commit(q_free);
-                    for (int j = 0; ok && j < nt; j++, c += 2) {
+                    for (int j = 0; ok && j < nt; j++, c += NEXT, nf++) {
                         const bool more = j + 1 < nt;
-                        if (!(ok = full_at(c + 1) && sy.wait(&p_full[i], np++ & 1))) break;
+                        if (!(ok = sy.wait(v_bar(c + 1), MODE == F32 ? nf & 1 : C::phase(c + 1)) && sy.wait(&p_full[i], np++ & 1))) break;
                         tc_fence_after();
                         lock();
                         weigh(c + 1, j == 0);
                         if (more) {
-                            if (!mbar_test_wait(&full[C::slot(i, c + 2)], C::phase(c + 2))) {      // K is late: not at the other's cost
+                            const uint32_t ph = MODE == F32 ? (nf + 1) & 1 : C::phase(c + NEXT);
+                            if (!mbar_test_wait(k_bar(c + NEXT), ph)) {      // K is late: not at the other's cost
                                 unlock();
-                                if (!(ok = full_at(c + 2))) break;
+                                umma_commit(&empty[C::slot(i, c + 1)]);
+                                if (!(ok = sy.wait(k_bar(c + NEXT), ph))) break;
                                 lock();
+                                score(c + NEXT);
+                                unlock();
+                                umma_commit(&s_full[i]);
+                                umma_commit(&empty[C::slot(i, c + NEXT)]);
+                                continue;
                             }
-                            score(c + 2);
+                            score(c + NEXT);
                         }
                         unlock();
                         umma_commit(&s_full[i]);
                         umma_commit(&empty[C::slot(i, c + 1)]);
-                        if (more) umma_commit(&empty[C::slot(i, c + 2)]);
-                        if (SPLIT && j + 2 == nt) umma_commit(q_free);          // the last of the unit's reads of Q
+                        if (more) umma_commit(&empty[C::slot(i, c + NEXT)]);
                     }
                 } else {                                        // one row tile: the other stream's loads are read once
-                    for (int x = 0; ok && x < 2 * nt; x++, c++)
-                        if ((ok = full_at(c))) mbar_arrive(&empty[C::slot(i, c)]);
+                    for (uint32_t x = c; ok && x < c1; x++)
+                        if ((ok = sy.wait(&full[C::slot(i, x)], C::phase(x)))) mbar_arrive(&empty[C::slot(i, x)]);
                 }
+                c = c1;
             }
             if (!ok) {                                          // nothing of this CTA's is in flight when TMEM goes
                 umma_commit(drain);
@@ -642,40 +834,41 @@ __global__ void __maxnreg__(168) k_paged_wide(const PagedAttn A, const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 11) {
+    if (warp == C::MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
     if (last) pdl_wait();
 }
 
-template <int D, bool SPLIT>
+template <int D, int MODE>
 static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
-    using C = WideCfg<D, SPLIT>;
+    using C = WideCfg<D, MODE>;
     static_assert(C::SMEM <= 232448, "shared memory per CTA");
-    const int64_t units = !own && A.p.line > 0 ? A.p.line
-                          : own                ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk
-                                               : (int64_t)A.p.chunks_p * A.p.tiles_p * A.a.Hk;
+    const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.line_ctas;
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     static unsigned long long set = 0;                          // per device
     int dev = 0;
     QMS_CK(cudaGetDevice(&dev));
     if (!(set >> (dev & 63) & 1)) {
-        QMS_CK(cudaFuncSetAttribute(k_paged_wide<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        QMS_CK(cudaFuncSetAttribute(k_paged_wide<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         set |= 1ull << (dev & 63);
     }
     CUtensorMap mk, mv;
-    int rc = paged_map(A.a, D, true, kWTile, A.a.k, &mk);
-    if (rc || (rc = paged_map(A.a, D, true, kWTile, A.a.v, &mv))) return rc;
+    int rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.k, &mk);
+    if (rc || (rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.v, &mv))) return rc;
     const int grid = (int)(units < 148 ? units : 148);
-    QMS_CK(launch_pdl(k_paged_wide<D, SPLIT>, dim3(grid), dim3(kWThreads), C::SMEM, s, A, mk, mv, own, last));
+    QMS_CK(launch_pdl(k_paged_wide<D, MODE>, dim3(grid), dim3(C::THREADS), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
 }
 
 int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s) {
-    const bool split = (own ? A.p.wr_s : A.p.wr_p) == kPaWideSplit;
-    if (D == 128) return split ? launch_wide<128, true>(A, own, last, s) : launch_wide<128, false>(A, own, last, s);
-    return split ? launch_wide<64, true>(A, own, last, s) : launch_wide<64, false>(A, own, last, s);
+    const int kind = own ? A.p.wr_s : A.p.wr_p;
+    if (D == 128)
+        return kind == kPaWidePair ? launch_wide<128, PAIR>(A, own, last, s) : kind == kPaWideSplit ? launch_wide<128, SPLIT>(A, own, last, s)
+                                                                                                  : launch_wide<128, F32>(A, own, last, s);
+    return kind == kPaWidePair ? launch_wide<64, PAIR>(A, own, last, s) : kind == kPaWideSplit ? launch_wide<64, SPLIT>(A, own, last, s)
+                                                                                             : launch_wide<64, F32>(A, own, last, s);
 }
 
 }  // namespace qms

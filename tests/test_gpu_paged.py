@@ -154,6 +154,7 @@ def test_attention_scores(cuda, typ):
     """One position takes all the weight; equal scores; q beyond the range of 16-bit types."""
     check([1, 3], [300, 64], typ=typ, G=16, qscale=200.0)
     check([1, 3], [300, 64], typ=typ, G=16, scale=0.0)
+    check([70, 3], [300, 64], typ=typ, G=2, scale=0.0)
     check([1, 70], [300, 90], typ=typ, G=2, qscale=1e30, scale=1e-31)
     check([1, 70], [300, 90], typ=typ, G=2, qscale=1e-30, scale=1e29)
     check([1, 3], [300, 64], typ=typ, G=4, scale=-0.1)
