@@ -245,8 +245,8 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
 /* Causal grouped-query attention of the batch's rows over the paged cache: out[t][h] = sum over
  * positions j <= position of t of softmax_j(scale * q[t][h] . K[j]) V[j], fp32 in and out (rows of
  * ldq / ldo), q head h reading kv head h / (n_head / n_head_kv). What lies at positions that a row
- * does not see has no effect on it, whatever its bits (fp32 cache: a finite V that another row of the call sees
- * may be no more than about 2^20 times the row's own without costing it precision); a V value that it sees and
+ * does not see has no effect on it, whatever its bits (fp32 cache: K and V that other rows of the call see
+ * and that are over some 2^10 times larger than what the row sees cost it precision); a V value that it sees and
  * that is not finite makes that element of the row not finite. A row that sees nothing (padding, a negative
  * position, an idle sequence) is zero; positions on a bad page set *err and count as not seen.
  * ws: device workspace, 256-byte aligned, of at least qms_cuda_paged_attention_ws() bytes (a function

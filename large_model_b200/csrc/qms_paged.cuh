@@ -133,24 +133,23 @@ __device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
 struct PagedPlan {
     int wr_p, wr_s;                  // shared, own: row groups of 16 per tile (k_paged_attn), or kPaWide...
     int chunk_p, chunk_s;            // positions per chunk
+    int piece_s, pieces_s;           // positions per slot of chunk_s, slots per chunk_s
     int base_s;                      // where the own positions' chunks start: prefix, or the tile boundary before it
     int chunks_p, chunks_s;          // chunks of each kind
     int slots_p, slots_s;            // slots of each kind
     int tiles_p, tiles_s;            // row tiles of each kind
-    unsigned line, line_ctas;        // k_paged_wide's runs over the shared positions: total length (0: none), CTAs,
-    int line_tp, line_rows;          // positions per place of the line, rows per row tile
+    // k_paged_wide's runs over the shared positions: total length (0: none), runs, runs per CTA, places of the line per
+    // run (the first line_r runs have one more), position tiles; positions per place, rows per row tile
+    unsigned line, line_runs, line_per, line_q, line_r, line_nt;
+    int line_tp, line_rows;
 };
 constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2;   // k_paged_wide: 256 rows; 128; 128 over an fp32 cache
 
-// A line of `line` places in n runs, the first line % n of them one place longer: where run i starts, and which run
-// holds place x. (32 bits: a 64-bit division costs the kernels some 500 cycles.)
-__host__ __device__ inline unsigned line_start(unsigned i, unsigned line, unsigned n) {
-    const unsigned q = line / n, r = line - q * n;
-    return i * q + (i < r ? i : r);
-}
-__host__ __device__ inline unsigned line_run(unsigned x, unsigned line, unsigned n) {
-    const unsigned q = line / n, r = line - q * n;
-    return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
+// Where run i starts, and which run holds place x. (Divisions are what a short kernel's start waits for: few, of 32 bits.)
+__device__ __forceinline__ unsigned line_start(const PagedPlan &p, unsigned i) { return i * p.line_q + min(i, p.line_r); }
+__device__ __forceinline__ unsigned line_run(const PagedPlan &p, unsigned x) {
+    const unsigned longer = p.line_r * (p.line_q + 1);
+    return x < longer ? x / (p.line_q + 1) : p.line_r + (x - longer) / p.line_q;
 }
 
 struct PagedAttn {

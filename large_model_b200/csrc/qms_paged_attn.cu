@@ -8,7 +8,6 @@
 // once per stage in shared memory, and three products kept (lo * lo is below 2^-22); the tf32 form of the same
 // (m16n8k8, three products, split in every warp) took about twice as long.
 #include <math.h>
-#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -604,14 +603,14 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
             if (a.prefix > 0) {
                 const int d = min(pos, a.prefix - 1);
                 if (A.p.line > 0) {
-                    const unsigned h = row - t * a.H, kh = h / a.G, tp = A.p.line_tp, nt = (a.prefix + tp - 1) / tp;
-                    const unsigned y = ((t * a.G + h - kh * a.G) / (unsigned)A.p.line_rows * a.Hk + kh) * nt;
-                    np = line_run(y + d / tp, A.p.line, A.p.line_ctas) - line_run(y, A.p.line, A.p.line_ctas) + 1;
+                    const unsigned h = row - t * a.H, kh = h / a.G;
+                    const unsigned y = ((t * a.G + h - kh * a.G) / (unsigned)A.p.line_rows * a.Hk + kh) * A.p.line_nt;
+                    np = line_run(A.p, y + d / (unsigned)A.p.line_tp) - line_run(A.p, y) + 1;
                 } else {
                     np = d / A.p.chunk_p + 1;
                 }
             }
-            const int ns = np + (pos < a.prefix ? 0 : (pos - A.p.base_s) / A.p.chunk_s + 1);
+            const int ns = np + (pos < a.prefix ? 0 : (pos - A.p.base_s) / A.p.piece_s + 1);
             const bool dense = np == A.p.slots_p || ns == np;              // slot s is where the fetch above took it
             float M = -INFINITY;
             float2 ml = make_float2(-INFINITY, 0.0f);
@@ -669,25 +668,36 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); k_paged_wide for
-// more rows over an fp16 cache in pages of 8 positions or more (a swizzle unit of its tiles), and over fp32 caches.
+// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read), k_paged_wide
+// from 65 on (fp16: in pages of 8 positions or more, a swizzle unit of its tiles). Both sides in us, 16 sequences of 5000
+// positions, 16 q heads per kv head: 64 rows 24.7 narrow, 27 wide (fp32: 43.7, 47.7); 128 rows 40 narrow, 27 wide; 32
+// rows over an fp32 cache, 12 sequences on one prompt 23, 25.
 static int row_groups(int type, int page_log, int64_t rows) {
-    static const int f32min = getenv("QMS_F32MIN") ? atoi(getenv("QMS_F32MIN")) : 17;
-    if (type != QMS_T_F16 && rows >= f32min) return kPaWideF32;
-    if (type == QMS_T_F16 && rows > 64 && page_log >= 3) return rows > 128 ? kPaWidePair : kPaWideSplit;
+    if (rows > 64 && type != QMS_T_F16) return kPaWideF32;
+    if (rows > 64 && page_log >= 3) return rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
 }
 static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
 static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : wr == kPaWideF32 ? 64 : 128; }
 
+// Positions that one partial result may cover. The tensor cores add to fp32 by cutting bits off: each addition takes
+// up to 2^-23, on average 4e-8, of the sum away. With these bounds an output is within 7e-6 of the exact one at any
+// length (unbounded, 1.9e-5 at 9000 positions); half of them would make that 4e-6 and a long shared prompt 5% slower.
+// fp16: 288 additions, 2 per 16 positions; fp32: 252, 3 per 16. `share` accumulators have a unit's positions.
+static int most_positions(int type, int wr) {
+    const bool f16 = type == QMS_T_F16;
+    const int share = wr == kPaWidePair ? 1 : wr < 0 ? 2 : f16 ? 4 / wr : wr == 4 ? 1 : 2;
+    return (f16 ? 2304 : 1344) * share;
+}
+
 // Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
 // of resident CTAs, stages of `stage` positions (us each, us_unit once per unit) and 1 KB of partial results
 // written and read back per row and chunk.
-static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int resident, double us_stage, double us_unit) {
-    const int st = (len + stage - 1) / stage;
-    int best = st;
+static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int resident, double us_stage, double us_unit, int cap) {
+    const int st = (len + stage - 1) / stage, most = std::min(st, cap / stage);
+    int best = most;
     double least = 1e30;
-    for (int per = st; per >= 1; per = per > 64 ? per - per / 16 : per - 1) {
+    for (int per = most; per >= 1; per = per > 64 ? per - per / 16 : per - 1) {
         const int n = (st + per - 1) / per;
         const int64_t waves = (tiles * n + resident - 1) / resident;
         const double us = (double)waves * (per * us_stage + us_unit) + (double)rows * n * 2.0e-4;
@@ -697,11 +707,11 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
 }
 
 static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
-    const int tp = tile_positions(type, wr);
-    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0);
-    if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0);
+    const int tp = tile_positions(type, wr), most = most_positions(type, wr);
+    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, 1 << 30);      // (in pieces, below)
+    if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
     const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
-    return chunk_of(len, tiles, rows, tp, 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0);
+    return chunk_of(len, tiles, rows, tp, 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0, most);
 }
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
@@ -716,15 +726,30 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     p.chunk_p = chunk_for(type, p.wr_p, a.prefix, (int64_t)p.tiles_p * a.Hk, all);
     p.chunk_s = chunk_for(type, p.wr_s, own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all);
     p.slots_p = p.chunks_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
-    p.slots_s = p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
+    p.piece_s = p.chunk_s;
+    p.pieces_s = 1;
+    const int most_s = most_positions(type, p.wr_s);
+    if (p.wr_s == kPaWidePair && p.chunk_s > most_s) {                      // units of several slots
+        const int tp = tile_positions(type, p.wr_s), n = (p.chunk_s + most_s - 1) / most_s;
+        p.piece_s = ((p.chunk_s + n - 1) / n + tp - 1) / tp * tp;
+        p.pieces_s = n;
+        p.chunk_s = n * p.piece_s;
+    }
+    p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
+    p.slots_s = (own + p.piece_s - 1) / p.piece_s;
     if (p.wr_p <= 0 && p.chunks_p > 0 && p.tiles_p > 0) {
         p.line_tp = tile_positions(type, p.wr_p);
         p.line_rows = tile_rows(p.wr_p);
         const int64_t nt = (a.prefix + p.line_tp - 1) / p.line_tp, line = nt * p.tiles_p * a.Hk;
+        const int64_t ctas = std::min<int64_t>(148, line), most = most_positions(type, p.wr_p) / p.line_tp;
         p.line = (unsigned)line;
-        p.line_ctas = (unsigned)std::min<int64_t>(148, line);
+        p.line_nt = (unsigned)nt;
+        p.line_per = (unsigned)((line + ctas * most - 1) / (ctas * most));
+        p.line_runs = (unsigned)(p.line_per * ctas);
+        p.line_q = p.line / p.line_runs;
+        p.line_r = p.line % p.line_runs;
         // a row tile's positions meet at most this many runs
-        p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / (line / p.line_ctas) + 2);
+        p.slots_p = (int)std::min<int64_t>(nt, (nt - 1) / p.line_q + 2);
     }
 }
 

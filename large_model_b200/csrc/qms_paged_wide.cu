@@ -9,14 +9,15 @@
 // For each tile of a stream
 //   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128, N the positions, K = head_dim, with 22-bit operands: Q =
 //               hi + lo in fp16 (each row scaled by a power of two into fp16's range), K exact in fp16 (two
-//               products) or K = hi + lo, each row scaled (three: lo * lo is below 2^-22)
+//               products) or K = hi + lo under a scale of its tile (three: lo * lo is below 2^-22)
 //   softmax     one thread per row reads its S from TMEM, keeps the running base B and sum l, writes the
 //               weights 2^(s f - B) back over S as two fp16 terms
 //   O += P V    tcgen05.mma with P from TMEM (hi, lo) and V as it lies in shared memory (MN-major), fp32 V = hi + lo
 //               under the largest scale so far (O is in its units)
 // O stays in TMEM over the whole unit. A base is set 2^8 below a maximum and stays until a score lies 2^15 above it
 // (fp16 holds weights to 2^16), so that the maximum needs no pass of its own; the result does not depend on
-// it beyond rounding.
+// it beyond rounding. In PAIR a long unit leaves O as a partial result after every 18 tiles and starts anew (tensor cores
+// add by cutting bits off, the longer the more), with the Q that is there; the other units are that short.
 //
 // Warps 0-3 and 4-7 are the softmax of the two streams. One warp brings K and V in by TMA, a box per page: 64 swizzled
 // values x the page's positions (fp32: whole rows, into a staging ring, from which four warps write the terms). Tiles
@@ -48,15 +49,16 @@ struct WideCfg {
     static constexpr int TP = MODE == F32 ? 64 : 128, ROWS = MODE == PAIR ? 256 : 128;     // positions per tile, rows per unit
     static constexpr int THREADS = MODE == F32 ? 480 : 384, REGS = MODE == F32 ? 128 : 168;    // (4, 3 warps per scheduler)
     static constexpr int TMA_WARP = MODE == F32 ? 12 : 8, MMA_WARP = MODE == F32 ? 13 : 10;
+    static constexpr bool PIECES = MODE == PAIR;                // units of more than one partial result
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t QHALF = 128 * 128, QTILE = HALVES * QHALF;     // one term of 128 rows of Q
     static constexpr uint32_t HALF = TP * 128, TILE = HALVES * HALF;         // one term of a K or V tile
     static constexpr uint32_t SLOT = (MODE == F32 ? 2 : 1) * TILE;
     static constexpr int SLOTS = MODE == SPLIT ? 4 : 3;
     static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT, STAGED = MODE == F32 ? TP * D * 4 : 0;
-    // then: bad-page masks [8][4]; scales of K rows [4][64], of V [4], maxima [2][4]; a stream's (B, l, V scale) by
-    // row; barriers; flags
-    static constexpr uint32_t BAD = STAGE + 2 * STAGED, FK = BAD + 128, VUP = FK + (MODE == F32 ? 1024 : 0), JOIN = VUP + 48,
+    // then: bad-page masks [8][4]; scales of K and V tiles [2][4], maxima [2][4]; a stream's (B, l, V scale) by row;
+    // barriers; flags
+    static constexpr uint32_t BAD = STAGE + 2 * STAGED, UP = BAD + 128, JOIN = UP + 64,
                               BARS = JOIN + (MODE == PAIR ? 0 : 128 * 12), SMEM = BARS + 24 * 8 + 32;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
     // Load n of a ring (K, V, K, ...): its slot. One ring for both streams; in SPLIT a ring per stream.
@@ -102,6 +104,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// 32 bytes to global memory (32-byte aligned), or zeros
+__device__ __forceinline__ void st_v8(float *to, const uint32_t *v, bool zero) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(zero ? 0 : v[0]), "r"(zero ? 0 : v[1]),
+                 "r"(zero ? 0 : v[2]), "r"(zero ? 0 : v[3]), "r"(zero ? 0 : v[4]), "r"(zero ? 0 : v[5]), "r"(zero ? 0 : v[6]), "r"(zero ? 0 : v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_tie(uint32_t (&r)[32]) {      // the same for a second array of that wait
@@ -131,15 +139,15 @@ struct WideSync {
 
 // One unit of work, as every role derives it.
 struct WideUnit {
-    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, lo;
-    // kv head; sequence, its first row, rows and length (own); slot of the partial result; positions [k0, k1) in
-    // nt tiles, of which those below kmin belong to another unit; first row and number of rows of the
-    // segment; every row of the unit sees the positions up to lo
+    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, lo, run, cut;
+    // kv head; sequence, its first row, rows and length (own); slot of the (first) partial result; positions
+    // [k0, k1) in nt tiles, of which those below kmin belong to another unit; first row and number of rows of the
+    // segment; every row of the unit sees the positions up to lo; (PAIR) first run of the line, tiles in the first part
 };
 
 // The units of this CTA in order. Own positions: units blockIdx.x, + gridDim.x, ... of (chunk, sequence, row tile, kv
-// head). Shared positions: all (row tile, kv head, position tile) triples in one line, cut into equal runs, one per
-// CTA; a run is one unit per row tile and kv head that it crosses.
+// head). Shared positions: all (row tile, kv head, position tile) triples in one line, cut into equal runs, the
+// same number for each CTA; a unit is what a run (PAIR: all runs of the CTA) has of one row tile and kv head.
 template <class C>
 struct WideWork {
     const PagedAttn &A;
@@ -151,10 +159,12 @@ struct WideWork {
             x = blockIdx.x;
             end = (unsigned)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk;
         } else {
-            x = line_start(blockIdx.x, A.p.line, gridDim.x);
-            end = line_start(blockIdx.x + 1, A.p.line, gridDim.x);
+            x = line_start(A.p, blockIdx.x * A.p.line_per);
+            end = line_start(A.p, (blockIdx.x + 1) * A.p.line_per);
         }
     }
+    // tiles in part i >= 1 of the unit (a partial result of its own), or more where the unit ends in it
+    __device__ int piece(const WideUnit &w, int i) const { return own ? A.p.piece_s / C::TP : A.p.line_q + (w.run + i < A.p.line_r); }
     __device__ bool next(WideUnit &w) {
         const Paged &a = A.a;
         while (x < end) {
@@ -170,19 +180,22 @@ struct WideWork {
                 d = u / a.n_seq;
                 w.b = u - d * a.n_seq;
                 paged_seq(a, w.b, w.t0, w.n, w.kv);
+                if (C::PIECES) w.cut = A.p.piece_s / C::TP;
                 w.k0 = A.p.base_s + d * A.p.chunk_s;
                 w.kmin = max(w.k0, a.prefix);
                 w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
                 w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (w.r0 + C::ROWS - 1) / a.G) + 1);     // nobody sees the rest
-                w.slot = A.p.slots_p + d;
+                w.slot = A.p.slots_p + (C::PIECES ? d * A.p.pieces_s : d);
                 w.rows = w.n * a.G;
                 w.lo = w.kv - w.n + w.r0 / a.G;
             } else {
-                const unsigned nt = (a.prefix + C::TP - 1) / C::TP, u = x / nt, j = x - u * nt, c = min(nt - j, end - x), tile = u / a.Hk;
+                const unsigned nt = A.p.line_nt, u = x / nt, j = x - u * nt, tile = u / a.Hk;
+                const unsigned run = line_run(A.p, x), c = min(nt - j, C::PIECES ? end - x : line_start(A.p, run + 1) - x);
+                if (C::PIECES) w.run = run, w.cut = line_start(A.p, run + 1) - x;
                 x += c;
                 w.kh = u - tile * a.Hk;
                 w.r0 = tile * C::ROWS;
-                w.slot = blockIdx.x - line_run(u * nt, A.p.line, gridDim.x);
+                w.slot = run - line_run(A.p, u * nt);
                 w.k0 = w.kmin = j * C::TP;
                 w.k1 = min(a.prefix, (int)(j + c) * C::TP);
                 w.rows = a.n_tok * a.G;
@@ -204,8 +217,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sm0 = smem_u32(sm);
     uint32_t *s_bad = reinterpret_cast<uint32_t *>(sm + C::BAD);
-    float *s_fk = reinterpret_cast<float *>(sm + C::FK);          // what undoes the scale of each K row, at tile & 3 (F32)
-    uint32_t *s_vup = reinterpret_cast<uint32_t *>(sm + C::VUP), *s_max = s_vup + 4;
+    uint32_t *s_up = reinterpret_cast<uint32_t *>(sm + C::UP), *s_max = s_up + 8;     // F32: scales of K, of V (4 +), at tile & 3
     float *s_join = reinterpret_cast<float *>(sm + C::JOIN);
     // full, empty: of the ring's slots (F32: `full` is of stream i's K, i, and V, 2 + i); landed: V tiles that go on
     // after a look, or (F32) the stages, at 2 + i when they are free again
@@ -261,8 +273,14 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
     const WideSync sy{s_abort, &a};
     WideWork<C> work(A, own, lo_p);
     WideUnit w = {};
-    // the tiles of stream i in a unit of nt: all (PAIR, where it has rows), or every second
-    auto tiles_of = [&](int i) { return MODE == PAIR ? (w.rows - w.r0 > 128 * i ? w.nt : 0) : (w.nt + 1 - i) / 2; };
+    // The tiles of stream i in a unit of nt: all (PAIR, where it has rows), or every second one, from first_of(i). In F32
+    // the streams alternate over all tiles of the CTA (`before` those of earlier units), not from the start of each
+    // unit: the one ring keeps a stream's barriers at most a phase ahead of who waits for them only if its tiles
+    // never follow one another.
+    auto first_of = [&](int i, uint32_t before) { return MODE == F32 ? (int)((i ^ before) & 1) : MODE == SPLIT ? i : 0; };
+    auto tiles_of = [&](int i, uint32_t before) {
+        return MODE == PAIR ? (w.rows - w.r0 > 128 * i ? w.nt : 0) : (w.nt + 1 - first_of(i, before)) / 2;
+    };
 
     if (warp < 8) {
         // ---- softmax of stream i: thread = row = TMEM lane
@@ -272,7 +290,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
         uint32_t ns = 0, nv = 0, before = 0, unit_no = 0;      // phases of s_full, of V; position tiles, units before
         bool ok = true;
         for (; ok && work.next(w); before += w.nt, unit_no++) {
-            const int nt = tiles_of(i);
+            const int nt = tiles_of(i, before);
             if (MODE == PAIR && nt == 0) continue;
             const int r = w.r0 + (MODE == PAIR ? i * 128 : 0) + row, t = r / a.G;    // this row: its token, position below
             int tok = -1;                                                        // token row * H + head (-1: none)
@@ -354,8 +372,6 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
 
             const int lim = min(pos, w.k1 - 1);   // last position that this row sees
-            float B = -INFINITY;
-            float2 l2 = make_float2(0.0f, 0.0f);
             uint32_t vup = 0;                     // F32: the scale of V that O is in
             // O times a power of 2 (the MMAs on it ended before the S at hand was announced)
             auto scale_o = [&](float fac) {
@@ -369,16 +385,23 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     tmem_st32(o_col + 32 * k, o);
                 }
             };
-            for (int n = 0; n < nt; n++) {
-                const int j = MODE == PAIR ? n : 2 * n + i, base = w.k0 + j * C::TP;
-                if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;    // the whole warp or none of it
-                ns++;
-                tc_fence_after();
+            // a part of the unit, of one partial result: the tiles from position kp on, up to tile n1
+            int n = 0, n1 = C::PIECES ? min(nt, w.cut) : nt, kp = w.kmin, piece = 0;
+            float B = -INFINITY;
+            float2 l2 = make_float2(0.0f, 0.0f);
+        next_part:                                // (as a loop around all this, 1 us more per call)
+            for (; n < n1; n++) {
+                const int j = MODE == PAIR ? n : 2 * n + first_of(i, before), base = w.k0 + j * C::TP;
+                if (!C::PIECES || n == 0 || base > kp) {           // (else waited for already)
+                    if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;       // the whole warp or none of it
+                    ns++;
+                    tc_fence_after();
+                }
                 const uint32_t *bad = s_bad + ((before + j) & 7) * 4;
                 uint32_t any_bad = bad[0] | bad[1];
                 if constexpr (C::TP == 128) any_bad |= bad[2] | bad[3];
-                // rows that see nothing of this unit are not read from its slot: no mask for them
-                if (__any_sync(kFull, lim >= w.kmin && lim < base + C::TP - 1) || base < w.kmin || any_bad) {
+                // rows that see nothing of this part are not read from its slot: no mask for them
+                if (__any_sync(kFull, lim >= kp && lim < base + C::TP - 1) || base < w.kmin || any_bad) {
 #pragma unroll 1
                     for (int c = 0; c < C::TP / 32; c++) {
                         const int d = lim - base - 32 * c, below = w.kmin - base - 32 * c;
@@ -396,30 +419,20 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 // scores of 32 positions in z become weights, hi terms in the first 16 columns, lo in the next 16. The
                 // base of the weights is a whole number and stays, unless a score lies 2^kWHigh above it: then
                 // what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
-                const float2 f2 = make_float2(f, f);
+                const float fk = MODE == F32 ? fmaxf(f * pow2_bits(254u - s_up[(before + j) & 3]), 1.17549435e-38f) : f;
+                const float2 f2 = make_float2(fk, fk);
                 auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {
-                    if constexpr (MODE == F32) {
-                        const float4 *fk = reinterpret_cast<const float4 *>(s_fk + ((before + j) & 3) * 64 + 32 * c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float4 k = fk[e];
-                            z[4 * e] = __float_as_uint(__uint_as_float(z[4 * e]) * k.x);
-                            z[4 * e + 1] = __float_as_uint(__uint_as_float(z[4 * e + 1]) * k.y);
-                            z[4 * e + 2] = __float_as_uint(__uint_as_float(z[4 * e + 2]) * k.z);
-                            z[4 * e + 3] = __float_as_uint(__uint_as_float(z[4 * e + 3]) * k.w);
-                        }
-                    }
                     float mx = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
                     for (int e = 3; e < 31; e += 2) mx = max3(mx, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
                     mx = fmaxf(mx, __uint_as_float(z[31]));
-                    mx = mx == -INFINITY ? mx : mx * f;
+                    mx = mx == -INFINITY ? mx : mx * fk;
                     if (__any_sync(kFull, mx > B + kWHigh)) {
                         const float nb = mx > B + kWHigh ? ceilf(mx) - kWLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
                         B = nb;
                         l2.x *= fac;
                         l2.y *= fac;
-                        if (n > 0) scale_o(fac);
+                        if (n > 0 && (!C::PIECES || base > kp)) scale_o(fac);
                         const __half2 fh = __float2half2_rn(fac);
 #pragma unroll 1
                         for (int k = 0; k < 4; k++) {
@@ -467,7 +480,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 } else {
                     weights(y, 1, 1);
                     if (!(ok = __all_sync(kFull, sy.wait(&full[2 + i], nv++ & 1)))) break;     // V's scale is known
-                    const uint32_t up = s_vup[(before + j) & 3];
+                    const uint32_t up = s_up[4 + ((before + j) & 3)];
                     if (up != vup && n > 0) scale_o(vup - up > 126 ? 0.0f : pow2_bits(127u - (vup - up)));
                     vup = up;
                 }
@@ -477,11 +490,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 if (lane == 0) mbar_arrive(&p_full[i]);
             }
             if (!ok) break;
-            if (nt > 0) {                         // O is complete
+            // O is complete (no tiles at all: not before the last unit is read)
+            if (nt > 0) {
                 if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;
                 ns++;
                 tc_fence_after();
-            } else if (!(ok = __all_sync(kFull, sy.wait(&q_full[0], unit_no & 1)))) {          // not before the last unit is read
+            } else if (!(ok = __all_sync(kFull, sy.wait(&q_full[0], unit_no & 1)))) {
                 break;
             }
             float l = l2.x + l2.y;
@@ -507,11 +521,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 l = c0 * l + c1 * l1;
                 B = M;
             }
-            const bool put = tok >= 0 && lim >= w.kmin, none = l == 0.0f, fix = *s_flag != 0;
-            const int64_t first = (int64_t)w.slot * a.n_tok * a.H;
+            const bool put = tok >= 0 && lim >= kp, none = l == 0.0f, fix = *s_flag != 0;
+            const int64_t first = (int64_t)(w.slot + piece) * a.n_tok * a.H;
             const int row_out = put ? tok : -1;
             float *part = A.part_o + first * D + (lane & 7) * 4;
-            // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes
+            // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8
+            // lanes; while Q is still wanted, each lane writes its row (3 us more for 256 rows)
             unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
@@ -529,7 +544,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
                     typedef typename std::conditional<MODE == F32, float, __half>::type KT;
-                    for (int p = w.kmin; p <= lim; p++) {
+                    const int past = C::PIECES ? min(lim + 1, w.k0 + n1 * C::TP) : lim + 1;
+                    for (int p = kp; p < past; p++) {
                         const int64_t at = paged_at(a, a.table + (own ? (int64_t)w.b * a.table_stride : 0), p);
                         if (at < 0) continue;
                         const KT *vr = reinterpret_cast<const KT *>(a.v + at + w.kh * a.head_stride) + 32 * c;
@@ -539,6 +555,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                             if (!isfinite(v)) o[e] = __float_as_uint(__uint_as_float(o[e]) + v);
                         }
                     }
+                }
+                if (C::PIECES && n < nt) {
+                    if (put)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) st_v8(A.part_o + (first + tok) * D + 32 * c + e, o + e, none);
+                    continue;
                 }
                 __syncwarp();
 #pragma unroll
@@ -555,6 +577,13 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
             if (put) A.part_ml[first + tok] = make_float2(none ? -INFINITY : B, l);
             tc_fence_before();
+            if (C::PIECES && n < nt) {
+                kp = w.k0 + n * C::TP;
+                n1 = min(nt, n + work.piece(w, ++piece));
+                B = -INFINITY;
+                l2 = make_float2(0.0f, 0.0f);
+                goto next_part;
+            }
         }
     } else if (warp == C::TMA_WARP || (MODE != F32 && warp == 9)) {
         // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. One warp
@@ -646,97 +675,76 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
         }
     } else if (MODE == F32 && warp < 12) {
-        // ---- fp32 rows from the stages into hi and lo tiles: K by rows, each with a scale of its own (undone in its scores),
-        // V with the largest scale so far of what somebody sees. A 16-byte piece of a row per lane.
+        // ---- fp32 rows from the stages into hi and lo tiles, under one scale: K under the tile's, V under the largest so
+        // far, of what somebody sees. A 16-byte piece of a row per lane at a time.
         constexpr int CH = D / 4, N = C::TP * CH / 128;
         const int ct = tid - 256, cw = warp - 8;
-        const unsigned peers = CH == 32 ? kFull : 0xffffu << (lane & 16);             // the lanes of a row
         uint32_t c = 0, t = 0;                    // loads, tiles so far
         bool ok = true;
-        // largest finite |value|: by float maxima, looked at again where one is inf (NaN is no maximum)
-        auto largest = [](const float4 &y) { return fmaxf(max3(0.0f, fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))); };
-        auto finite4 = [](const float4 &y) { return max(max(finite_bits(y.x), finite_bits(y.y)), max(finite_bits(y.z), finite_bits(y.w))); };
         while (work.next(w)) {                    // (after a failed wait: the barriers, no work)
             uint32_t v_exp = 0;
             const int seen0 = min(w.lo, w.k1 - 1);
             for (int j = 0; j < w.nt; j++, t++)
+#pragma unroll 1
                 for (int is_v = 0; is_v < 2; is_v++, c++) {
                     const int base = w.k0 + j * C::TP;
-                    const float4 *src = reinterpret_cast<const float4 *>(sm + C::STAGE + (c & 1) * C::STAGED);
-                    unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
-                    ok = __all_sync(kFull, ok && sy.wait(&landed[c & 1], c / 2 & 1) && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
-                    auto put = [&](int at, float4 y, float up) {
-                        const int r = at / CH, q = at % CH;           // values 4 q .. + 3 of row r
-                        const float2 y0 = f2_mul(make_float2(y.x, y.y), make_float2(up, up)), y1 = f2_mul(make_float2(y.z, y.w), make_float2(up, up));
-                        uint32_t h[2], l[2];
-                        split_h2(y0.x, y0.y, h[0], l[0]);
-                        split_h2(y1.x, y1.y, h[1], l[1]);
-                        unsigned char *to = dst + (q >> 4) * C::HALF + r * 128 + ((((q & 15) >> 1) ^ (r & 7)) << 4) + (q & 1) * 8;
-                        *reinterpret_cast<uint2 *>(to) = make_uint2(h[0], h[1]);
-                        *reinterpret_cast<uint2 *>(to + C::TILE) = make_uint2(l[0], l[1]);
-                    };
-                    if (!is_v) {
-                        if (ok)
-#pragma unroll 1
-                            for (int h = 0; h < N; h += 4) {
-                                float4 y[4];
-                                uint32_t ky[4];
+                    const float4 *src = reinterpret_cast<const float4 *>(sm + C::STAGE + (c & 1) * C::STAGED) + ct;
+                    ok = __all_sync(kFull, ok && sy.wait(&landed[c & 1], c / 2 & 1));
+                    const uint32_t bad[2] = {s_bad[(t & 7) * 4], s_bad[(t & 7) * 4 + 1]};
+                    const int seen = bad[0] | bad[1] ? -1 : seen0;
+                    float4 x[N];
 #pragma unroll
-                                for (int i = 0; i < 4; i++) y[i] = src[ct + 128 * (h + i)];
+                    for (int i = 0; i < N; i++) x[i] = src[128 * i];
+                    if (base + C::TP - 1 > seen || base < w.kmin)
 #pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const float m = largest(y[i]);
-                                    ky[i] = __reduce_max_sync(peers, m == INFINITY ? finite4(y[i]) : __float_as_uint(m));
-                                }
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const int at = ct + 128 * (h + i);
-                                    const uint32_t up = scale_up(ky[i] >> 23);
-                                    if (at % CH == 0) s_fk[(t & 3) * 64 + at / CH] = pow2_bits(254u - up);
-                                    put(at, y[i], pow2_bits(up));
-                                }
-                            }
-                    } else {
-                        const uint32_t bad[2] = {s_bad[(t & 7) * 4], s_bad[(t & 7) * 4 + 1]};
-                        const int seen = bad[0] | bad[1] ? -1 : seen0;
-                        float4 x[N];
-                        float mx = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < N; i++) x[i] = src[ct + 128 * i];
-                        if (base + C::TP - 1 > seen || base < w.kmin)
-#pragma unroll
-                            for (int i = 0; i < N; i++) {
-                                const int r = (ct + 128 * i) / CH, p = base + r;
-                                if (p >= w.kmin && p <= seen) continue;
+                        for (int i = 0; i < N; i++) {
+                            const int r = (ct + 128 * i) / CH, p = base + r;
+                            if (p >= w.kmin && p <= seen) continue;
+                            const bool in = p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1);
+                            if (is_v) {
                                 uint4 v = *reinterpret_cast<const uint4 *>(&x[i]);
-                                const bool in = p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1);
                                 if (drop_nonfinite((const float *)nullptr, v)) {
                                     x[i] = *reinterpret_cast<const float4 *>(&v);
                                     if (in) *s_flag = 1;
                                 }
-                                if (!in) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);           // no part of the unit
                             }
-#pragma unroll
-                        for (int i = 0; i < N; i++) mx = fmaxf(mx, largest(x[i]));
-                        uint32_t mb = __float_as_uint(mx);
-                        if (mx == INFINITY) {
-                            mb = 0;
-#pragma unroll
-                            for (int i = 0; i < N; i++) mb = max(mb, finite4(x[i]));
+                            if (!in) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // no part of the unit
                         }
-                        mb = __reduce_max_sync(kFull, mb);
-                        uint32_t *s_m = s_max + (t & 1) * 4;
-                        if (lane == 0) s_m[cw] = mb;
-                        asm volatile("bar.sync 1, 128;" ::: "memory");
-                        v_exp = max(v_exp, max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3])) >> 23);
-                        const uint32_t up = scale_up(v_exp);
-                        if (ct == 0) s_vup[t & 3] = up;
-                        if (ok)
+                    // largest finite |value|: by float maxima, looked at again where it is inf (NaN is no maximum)
+                    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int i = 0; i < N; i++) put(ct + 128 * i, x[i], pow2_bits(up));
+                    for (int i = 0; i < N; i++) m[i & 3] = max3(m[i & 3], max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
+                    uint32_t mb = __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                    if (mb == 0x7f800000u) {
+                        mb = 0;
+#pragma unroll
+                        for (int i = 0; i < N; i++) mb = max(mb, max(max(finite_bits(x[i].x), finite_bits(x[i].y)), max(finite_bits(x[i].z), finite_bits(x[i].w))));
+                    }
+                    mb = __reduce_max_sync(kFull, mb);
+                    uint32_t *s_m = s_max + (c & 1) * 4;
+                    if (lane == 0) s_m[cw] = mb;
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    uint32_t exp = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3])) >> 23;
+                    if (is_v) exp = v_exp = max(v_exp, exp);
+                    const uint32_t up = scale_up(exp);
+                    if (ct == 0) s_up[4 * is_v + (t & 3)] = up;
+                    ok = __all_sync(kFull, ok && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
+                    if (ok) {
+                        const float2 u2 = make_float2(pow2_bits(up), pow2_bits(up)), minus = make_float2(-1.0f, -1.0f);
+                        unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
+#pragma unroll
+                        for (int i = 0; i < N; i++) {
+                            const int r = (ct + 128 * i) / CH, q = ct % CH;   // values 4 q .. + 3 of row r
+                            const float2 y0 = f2_mul(make_float2(x[i].x, x[i].y), u2), y1 = f2_mul(make_float2(x[i].z, x[i].w), u2);
+                            const float2 h0 = make_float2(tf32_hi(y0.x), tf32_hi(y0.y)), h1 = make_float2(tf32_hi(y1.x), tf32_hi(y1.y));
+                            const float2 l0 = f2_fma(h0, minus, y0), l1 = f2_fma(h1, minus, y1);
+                            unsigned char *to = dst + (q >> 4) * C::HALF + r * 128 + ((((q & 15) >> 1) ^ (r & 7)) << 4) + (q & 1) * 8;
+                            *reinterpret_cast<uint2 *>(to) = make_uint2(pack_h2(h0.x, h0.y), pack_h2(h1.x, h1.y));
+                            *reinterpret_cast<uint2 *>(to + C::TILE) = make_uint2(pack_h2(l0.x, l0.y), pack_h2(l1.x, l1.y));
+                        }
                     }
                     fence_async_smem();
-                    mbar_arrive(&full[2 * is_v + (j & 1)]);
+                    mbar_arrive(&full[2 * is_v + (t & 1)]);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&landed[2 + (c & 1)]);
                 }
@@ -779,9 +787,9 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             auto v_bar = [&](uint32_t n) { return MODE == F32 ? &full[2 + i] : &full[C::slot(i, n)]; };
             constexpr uint32_t NEXT = MODE == F32 ? 4 : 2;      // loads to the stream's next tile
             while (ok && work.next(w)) {
-                const int nt = tiles_of(i);
+                const int nt = tiles_of(i, c / 2);
                 const uint32_t c1 = c + (MODE == SPLIT ? 2 * nt : 2 * w.nt);
-                if (MODE == F32) c += 2 * i;
+                if (MODE == F32) c += 2 * first_of(i, c / 2);
                 if (MODE != PAIR || nt > 0) {
                     ok = sy.wait(&q_full[MODE == PAIR ? i : 0], nq++ & 1);
                     if (ok && nt > 0 && (ok = sy.wait(k_bar(c), MODE == F32 ? nf & 1 : C::phase(c)))) {
@@ -792,12 +800,14 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         umma_commit(&s_full[i]);
                         umma_commit(&empty[C::slot(i, c)]);
                     }
+                    int piece = 0, next = C::PIECES ? w.cut : nt;
                     for (int j = 0; ok && j < nt; j++, c += NEXT, nf++) {
                         const bool more = j + 1 < nt;
                         if (!(ok = sy.wait(v_bar(c + 1), MODE == F32 ? nf & 1 : C::phase(c + 1)) && sy.wait(&p_full[i], np++ & 1))) break;
                         tc_fence_after();
                         lock();
-                        weigh(c + 1, j == 0);
+                        weigh(c + 1, j == 0 || (C::PIECES && j == next));
+                        if (C::PIECES && j == next) next += work.piece(w, ++piece);
                         if (more) {
                             const uint32_t ph = MODE == F32 ? (nf + 1) & 1 : C::phase(c + NEXT);
                             if (!mbar_test_wait(k_bar(c + NEXT), ph)) {      // K is late: not at the other's cost
@@ -845,7 +855,7 @@ template <int D, int MODE>
 static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
     using C = WideCfg<D, MODE>;
     static_assert(C::SMEM <= 232448, "shared memory per CTA");
-    const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.line_ctas;
+    const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)(A.p.line_runs / A.p.line_per);
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     static unsigned long long set = 0;                          // per device
     int dev = 0;

@@ -205,6 +205,50 @@ def test_attention_masked_values_have_no_effect(cuda, typ, n, prefix, bad):
 
 
 @pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("prefix", [0, 4900])
+def test_attention_long_units(cuda, typ, prefix):
+    """So many rows that the positions are hardly cut: a result of thousands of additions. With a the additions into an
+    fp32 sum (at most 288) that each cut at most 2^-23, on average 0.72 * 2^-24, of it off, the outputs' 2-norm is off by
+    288 * 0.72 * 2^-24 / 2 = 6.2e-6 of itself where the sum grows steadily; 1e-5 with the scores' share."""
+    import torch
+    import large_model_b200 as m
+    B, n, G, Hk, D = 20, 17, 8, 8, 64
+    qs, kv = [n] * B, [5300 - 13 * b for b in range(B)]
+    pages, batch, q, K, V = make(qs, kv, typ=typ, G=G, Hk=Hk, D=D, prefix=prefix, seed=2)
+    out = m.paged_attention(pages, batch, q, G * Hk)
+    batch.status()
+    want, tol = reference(qs, kv, q, K, V, G, D ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
+    assert (out.double() - want).norm() <= 1e-5 * want.norm()
+    for _ in range(30):                              # many units, waits in every order
+        assert torch.equal(m.paged_attention(pages, batch, q, G * Hk), out)
+    batch.status()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("n,G,kv", [(5, 16, 700), (17, 8, 5000), (40, 1, 2100), (2, 4, 900)])
+def test_attention_values_that_are_not_finite(cuda, typ, n, G, kv):
+    """V of two positions of every sequence, one that only the last row sees and one that every row sees."""
+    import torch
+    import large_model_b200 as m
+    B, Hk, D = 40, 4, 64
+    qs, kvs = [n] * B, [kv - 3 * b for b in range(B)]
+    pages, batch, q, K, V = make(qs, kvs, typ=typ, G=G, Hk=Hk, D=D)
+    for b, x in enumerate(kvs):
+        for p, d, value in ((x - 1, 7, float("nan")), (x * 2 // 3, 9, float("inf"))):
+            pages.v[batch.table[b, p // 16].long(), p % 16, b % Hk, d] = value
+            V[b][p, b % Hk, d] = 0
+    out = m.paged_attention(pages, batch, q, G * Hk).view(B, n, Hk, G, D)
+    batch.status()
+    want, tol = (x.reshape(B, n, Hk, G, D) for x in reference(qs, kvs, q, K, V, G, D ** -0.5))
+    for b in range(B):
+        assert not torch.isfinite(out[b, -1, b % Hk, :, 7]).any() and not torch.isfinite(out[b, :, b % Hk, :, 9]).any()
+        out[b, -1, b % Hk, :, 7] = want[b, -1, b % Hk, :, 7].float()
+        out[b, :, b % Hk, :, 9] = want[b, :, b % Hk, :, 9].float()
+    assert ((out.double() - want).abs() <= tol + want.abs() * E24).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
 def test_attention_bad_arrays_are_reported(cuda, typ):
     import torch
     import large_model_b200 as m
