@@ -64,17 +64,11 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-// RMSNorm + NEOX rotation of one head row from preloaded values: x (the row), w (norm weights) and
-// c / s (cos / sin of the position) as lane + 32 j (src/model.c:403-422, 441-447).
+// x w inv, rotated: the second half of norm_rope_pre.
 template <int D>
-__device__ __forceinline__ void norm_rope_pre(float (&x)[D / 32], const float (&w)[D / 32], const float (&c)[D / 64],
-                                              const float (&sn)[D / 64], float eps) {
+__device__ __forceinline__ void rope_scaled(float (&x)[D / 32], const float (&w)[D / 32], const float (&c)[D / 64], const float (&sn)[D / 64],
+                                            double inv) {
     constexpr int J = D / 32, JH = J / 2;
-    double ss = 0.0;
-#pragma unroll
-    for (int j = 0; j < J; j++) ss = fma((double)x[j], (double)x[j], ss);
-    ss = warp_sum_d(ss);
-    const double inv = 1.0 / sqrt(ss / D + (double)eps);
 #pragma unroll
     for (int j = 0; j < J; j++) x[j] = __fmul_rn((float)((double)x[j] * inv), w[j]);
 #pragma unroll
@@ -83,6 +77,19 @@ __device__ __forceinline__ void norm_rope_pre(float (&x)[D / 32], const float (&
         x[j] = __fsub_rn(__fmul_rn(x1, c[j]), __fmul_rn(x2, sn[j]));
         x[j + JH] = __fadd_rn(__fmul_rn(x2, c[j]), __fmul_rn(x1, sn[j]));
     }
+}
+
+// RMSNorm + NEOX rotation of one head row from preloaded values: x (the row), w (norm weights) and
+// c / s (cos / sin of the position) as lane + 32 j (src/model.c:403-422, 441-447).
+template <int D>
+__device__ __forceinline__ void norm_rope_pre(float (&x)[D / 32], const float (&w)[D / 32], const float (&c)[D / 64],
+                                              const float (&sn)[D / 64], float eps) {
+    constexpr int J = D / 32;
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < J; j++) ss = fma((double)x[j], (double)x[j], ss);
+    ss = warp_sum_d(ss);
+    rope_scaled<D>(x, w, c, sn, 1.0 / sqrt(ss / D + (double)eps));
 }
 
 }  // namespace qms

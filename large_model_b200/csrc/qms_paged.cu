@@ -9,18 +9,45 @@
 namespace qms {
 
 // ---- append --------------------------------------------------------------------------------------
-// One warp per (token, head row of q | k | v): y = R(pos) (w * x / sqrt(mean x^2 + eps)) for q and k, v
-// unchanged. The mean's sum is held in double and the steps are k_qk_rope's, so a paged cache
-// holds the same values as the model's contiguous one.
-template <int D, typename KT>
+// A warp takes R head rows of q | k | v of one token: y = R(pos) (w * x / sqrt(mean x^2 + eps)) for q and k, v unchanged.
+// The mean's sum is held in double and the steps are k_qk_rope's, each in its order, so a paged cache holds the same
+// values as the model's contiguous one.
+// Bound by latency for few rows (R = 1: 2.6 us for one token) and by instructions for many, most of them for the 64-bit
+// mean: R = 4 rows share the exchanges of their sums and one square root and division (a lane each).
+template <int R>
+__device__ __forceinline__ void sum_rows(double (&v)[R], int lane) {      // the sum of v[r] over the lanes; R = 4: v[0] of row lane / 8
+    if constexpr (R == 1) {
+        v[0] = warp_sum_d(v[0]);
+    } else {
+        const bool hi = lane & 16, mid = lane & 8;
+        const double a = __shfl_xor_sync(kFull, hi ? v[0] : v[2], 16), b = __shfl_xor_sync(kFull, hi ? v[1] : v[3], 16);
+        const double x = (hi ? v[2] : v[0]) + a, y = (hi ? v[3] : v[1]) + b;
+        v[0] = (mid ? y : x) + __shfl_xor_sync(kFull, mid ? x : y, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) v[0] += __shfl_xor_sync(kFull, v[0], o);
+    }
+}
+
+template <int D, typename KT, int R>
 __global__ void __launch_bounds__(256) k_paged_append(const Paged a, const float *qkv, int64_t ldqkv, const float *q_norm,
                                                       const float *k_norm, float eps, const float *rope_cos,
                                                       const float *rope_sin, int n_rope, float *q, int64_t ldq) {
+    static_assert(R == 1 || R == 4, "rows per warp");
     constexpr int J = D / 32, JH = J / 2;
-    const int lane = threadIdx.x & 31, hh = blockIdx.y * 8 + (threadIdx.x >> 5), t = blockIdx.x;
+    const int lane = threadIdx.x & 31, groups = (a.H + 2 * a.Hk + R - 1) / R, nq = a.H + a.Hk;
+    const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int t = unit / groups, h0 = (unit - t * groups) * R;
     pdl_trigger();
     pdl_wait();
-    if (hh >= a.H + 2 * a.Hk) return;
+    if (t >= a.n_tok) return;
+    const float *row = qkv + t * ldqkv + h0 * D;
+    float x[R][J], w[J];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < J; j++) x[r][j] = h0 + r < nq + a.Hk ? row[r * D + lane + 32 * j] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; j++) w[j] = (h0 < a.H ? q_norm : k_norm)[lane + 32 * j];
     const int b = paged_seq_of(a, t);
     if (b >= a.n_seq) return;                                   // padding
     int t0, n, kv;
@@ -28,39 +55,66 @@ __global__ void __launch_bounds__(256) k_paged_append(const Paged a, const float
     if (ok && (t < t0 || t >= t0 + n)) return;                  // before the first sequence's rows
     const int p = kv - n + (t - t0);
     if (!ok || p < 0 || p >= n_rope) {
-        if (lane == 0 && hh == 0) paged_err(a, QMS_PAGED_ELEN);
+        if (lane == 0 && h0 == 0) paged_err(a, QMS_PAGED_ELEN);
         return;
     }
     const int64_t at = paged_at(a, a.table + (int64_t)b * a.table_stride, p);
     if (at < 0) {
-        if (lane == 0 && hh == 0) paged_err(a, QMS_PAGED_EPAGE);
+        if (lane == 0 && h0 == 0) paged_err(a, QMS_PAGED_EPAGE);
         return;
     }
-    const float *row = qkv + t * ldqkv + hh * D;
-    float x[J];
-#pragma unroll
-    for (int j = 0; j < J; j++) x[j] = row[lane + 32 * j];
-    if (hh < a.H + a.Hk) {
-        const float *nw = hh < a.H ? q_norm : k_norm;
-        float w[J], c[JH], s[JH];
-#pragma unroll
-        for (int j = 0; j < J; j++) w[j] = nw[lane + 32 * j];
+    float c[JH], s[JH];
+    double inv = 0.0;
+    if (h0 < nq) {
 #pragma unroll
         for (int j = 0; j < JH; j++) {
             c[j] = rope_cos[(int64_t)p * (D / 2) + lane + 32 * j];
             s[j] = rope_sin[(int64_t)p * (D / 2) + lane + 32 * j];
         }
-        norm_rope_pre<D>(x, w, c, s, eps);
-    }
-    if (hh < a.H) {
+        double ss[R];
 #pragma unroll
-        for (int j = 0; j < J; j++) q[t * ldq + hh * D + lane + 32 * j] = x[j];
-        return;
-    }
-    const int kh = hh < a.H + a.Hk ? hh - a.H : hh - a.H - a.Hk;
-    KT *dst = reinterpret_cast<KT *>((hh < a.H + a.Hk ? a.k : a.v) + at + kh * a.head_stride);
+        for (int r = 0; r < R; r++) {
+            ss[r] = 0.0;
 #pragma unroll
-    for (int j = 0; j < J; j++) kv_st(dst + lane + 32 * j, x[j]);
+            for (int j = 0; j < J; j++) ss[r] = fma((double)x[r][j], (double)x[r][j], ss[r]);
+        }
+        sum_rows<R>(ss, lane);
+        inv = 1.0 / sqrt(ss[0] / D + (double)eps);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int hh = h0 + r;
+        if (hh >= nq + a.Hk) return;
+        if (hh < nq) {
+            if (r > 0 && hh == a.H)                             // from q to k
+#pragma unroll
+                for (int j = 0; j < J; j++) w[j] = k_norm[lane + 32 * j];
+            rope_scaled<D>(x[r], w, c, s, R == 1 ? inv : __shfl_sync(kFull, inv, 8 * r));
+        }
+        if (hh < a.H) {
+#pragma unroll
+            for (int j = 0; j < J; j++) q[t * ldq + hh * D + lane + 32 * j] = x[r][j];
+        } else {
+            KT *dst = reinterpret_cast<KT *>((hh < nq ? a.k : a.v) + at + (hh < nq ? hh - a.H : hh - nq) * a.head_stride);
+#pragma unroll
+            for (int j = 0; j < J; j++) kv_st(dst + lane + 32 * j, x[r][j]);
+        }
+    }
+}
+
+template <int D, typename KT>
+static int launch_append(const Paged &a, const float *qkv, int64_t ldqkv, const float *q_norm, const float *k_norm, float eps,
+                         const float *rope_cos, const float *rope_sin, int n_rope, float *q, int64_t ldq, cudaStream_t s) {
+    const int heads = a.H + 2 * a.Hk;
+    // Four rows per warp once there are 48 for each SM. Both in us at 40 or 72 head rows per token: 4608 rows 3.56 one,
+    // 3.59 four; 5120 3.4, 3.8; 9216 5.2, 4.2; 10240 5.6, 4.8; 144000 50, 29 (4.9 TB/s).
+    const bool four = (int64_t)a.n_tok * heads >= 148 * 48;
+    const int64_t units = (int64_t)a.n_tok * (four ? (heads + 3) / 4 : heads);
+    QMS_REQUIRE(units < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "paged_append: too many rows");
+    const dim3 grid((unsigned)((units + 7) / 8));
+    if (four) QMS_CK(launch_pdl(k_paged_append<D, KT, 4>, grid, dim3(256), 0, s, a, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, q, ldq));
+    else QMS_CK(launch_pdl(k_paged_append<D, KT, 1>, grid, dim3(256), 0, s, a, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, q, ldq));
+    return QMS_CUDA_OK;
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -142,17 +196,14 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
     if ((rc = paged_rows("paged_append", "q", q, ldq, (int64_t)n_head * D))) return rc;
     QMS_REQUIRE(q_norm && k_norm && rope_cos && rope_sin && n_rope > 0, QMS_CUDA_EINVAL,
                 "paged_append: NULL norm weights or rotation tables");
-    const dim3 grid(a.n_tok, (n_head + 2 * a.Hk + 7) / 8);
-#define QMS_APPEND(D_, KT)                                                                                        \
-    QMS_CK(launch_pdl(k_paged_append<D_, KT>, grid, dim3(256), 0, (cudaStream_t)stream, a, qkv, ldqkv, q_norm, k_norm, \
-                      eps, rope_cos, rope_sin, n_rope, q, ldq))
+#define QMS_APPEND(D_, KT) \
+    return launch_append<D_, KT>(a, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, q, ldq, (cudaStream_t)stream)
     if (pages->type == QMS_T_F16) {
         if (D == 128) QMS_APPEND(128, __half); else QMS_APPEND(64, __half);
     } else {
         if (D == 128) QMS_APPEND(128, float); else QMS_APPEND(64, float);
     }
 #undef QMS_APPEND
-    return QMS_CUDA_OK;
 }
 
 int64_t qms_cuda_paged_attention_ws(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, int n_head) {

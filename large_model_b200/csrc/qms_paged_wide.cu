@@ -526,7 +526,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             const int row_out = put ? tok : -1;
             float *part = A.part_o + first * D + (lane & 7) * 4;
             // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8
-            // lanes; while Q is still wanted, each lane writes its row (3 us more for 256 rows)
+            // lanes; while Q is still wanted, each lane writes its row (as fast as by shuffles)
             unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {

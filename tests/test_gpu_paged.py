@@ -410,6 +410,39 @@ def test_append(cuda, typ, D, order):
     assert torch.equal(own[:T, :H * D], q[:T]) and torch.equal(own[:, H * D:], qkv[:, H * D:])
 
 
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("D,H,Hk", [(64, 6, 3), (128, 8, 4), (128, 5, 1)])
+def test_append_many_rows(cuda, typ, D, H, Hk):
+    """As many rows as several per warp are used for: the same bits as a few tokens at a time; groups of rows that cross
+    from q to k to v, and a last one that is not full."""
+    import torch
+    import large_model_b200 as m
+    n, B = 90, 12
+    qs, kv = [n - b for b in range(B)], [n + 3 * b for b in range(B)]
+    pages, batch, _, _, _ = make(qs, kv, typ=typ, D=D, Hk=Hk, G=2, garbage=0.0, pad=5)
+    T = sum(qs)
+    assert (T + 5) * (H + 2 * Hk) >= 148 * 48
+    g = torch.Generator(device="cuda").manual_seed(7)
+    qkv = 3 * torch.randn((T + 5, (H + 2 * Hk) * D), generator=g, device="cuda")
+    qkv[100] = 0
+    qn, kn = (torch.randn((D,), generator=g, device="cuda") for _ in range(2))
+    rope = m.rope_tables(max(kv), D)
+    q = m.paged_append(pages, batch, qkv, H, qn, kn, 1e-6, rope, q=torch.full((T + 5, H * D), 7.0, device="cuda"))
+    batch.status()
+    assert (q[T:] == 7).all() and (q[100] == 0).all()
+    other = m.KvPages(torch.zeros_like(pages.k), torch.zeros_like(pages.v))
+    t = 0
+    for b in range(B):
+        one = m.PagedBatch(torch.tensor([0, qs[b]], dtype=torch.int32, device="cuda"), batch.kv_len[b:b + 1].clone(), batch.table[b:b + 1].clone(),
+                           qs[b], qs[b], kv[b])
+        assert torch.equal(m.paged_append(other, one, qkv[t:t + qs[b]], H, qn, kn, 1e-6, rope), q[t:t + qs[b]])
+        one.status()
+        for j in range(kv[b] - qs[b], kv[b]):
+            pg = batch.table[b, j // 16].long()
+            assert torch.equal(other.k[pg, j % 16], pages.k[pg, j % 16]) and torch.equal(other.v[pg, j % 16], pages.v[pg, j % 16])
+        t += qs[b]
+
+
 def test_append_refuses_on_the_device(cuda):
     import torch
     import large_model_b200 as m
