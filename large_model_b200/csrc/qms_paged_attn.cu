@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         float o[C::DW / 8][4];
 #pragma unroll
         for (int i = 0; i < C::DW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, grown0 = 0.0f, grown1 = 0.0f;
         uint32_t v_exp = 0;                       // fp32: largest exponent of V so far; o is in units of its scale
 
         for (int st = 0; st < nst; st++) {
@@ -431,6 +431,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
                 l0 *= d0;
                 l1 *= d1;
+                grown0 *= d0;
+                grown1 *= d1;
 #pragma unroll
                 for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
             }
@@ -443,6 +445,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 l0 += s[i][0] + s[i][1];
                 l1 += s[i][2] + s[i][3];
             }
+            grown0 += l0;
+            grown1 += l1;
             // ---- o += weights * V
 #pragma unroll
             for (int kk = 0; kk < C::NT / 2; kk++) {
@@ -471,11 +475,19 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         }
         c0 += nst;
         __syncthreads();                          // every warp is done with the stages
-        if constexpr (!C::F16) {
-            const float d = pow2_bits(254u - scale_up(v_exp));
+        l0 += __shfl_xor_sync(kFull, l0, 1);
+        l1 += __shfl_xor_sync(kFull, l1, 1);
+        l0 += __shfl_xor_sync(kFull, l0, 2);
+        l1 += __shfl_xor_sync(kFull, l1, 2);
+        grown0 += __shfl_xor_sync(kFull, grown0, 1);
+        grown1 += __shfl_xor_sync(kFull, grown1, 1);
+        grown0 += __shfl_xor_sync(kFull, grown0, 2);
+        grown1 += __shfl_xor_sync(kFull, grown1, 2);
+        constexpr float ADDS = C::NT / 2 * (C::F16 ? 2 : 3);       // into o per stage
+        const float d = C::F16 ? 1.0f : pow2_bits(254u - scale_up(v_exp)), back0 = d * cut_back(C::F16, grown0, l0, ADDS, ADDS / 2),
+                    back1 = d * cut_back(C::F16, grown1, l1, ADDS, ADDS / 2);
 #pragma unroll
-            for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
-        }
+        for (int i = 0; i < C::DW / 8; i++) o[i][0] *= back0, o[i][1] *= back0, o[i][2] *= back1, o[i][3] *= back1;
         // dims of this thread's o[i][0..1] (row g) and o[i][2..3] (row g + 8)
         auto dim = [&](int i, int j) { return wd * C::DW + i * 8 + tq * 2 + (j & 1); };
         if (s_flag && wk == 0) {
@@ -493,10 +505,6 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     }
             }
         }
-        l0 += __shfl_xor_sync(kFull, l0, 1);
-        l1 += __shfl_xor_sync(kFull, l1, 1);
-        l0 += __shfl_xor_sync(kFull, l0, 2);
-        l1 += __shfl_xor_sync(kFull, l1, 2);
         if (isnan(l0)) m0 = 0.0f;                 // scores that are all NaN leave no maximum, but are not nothing
         if (isnan(l1)) m1 = 0.0f;
         const int64_t po = (int64_t)slot * a.n_tok * a.H;
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
                     np = d / A.p.chunk_p + 1;
                 }
             }
-            const int ns = np + (pos < a.prefix ? 0 : (pos - A.p.base_s) / A.p.piece_s + 1);
+            const int ns = np + (pos < a.prefix ? 0 : (pos - A.p.base_s) / A.p.chunk_s + 1);
             const bool dense = np == A.p.slots_p || ns == np;              // slot s is where the fetch above took it
             float M = -INFINITY;
             float2 ml = make_float2(-INFINITY, 0.0f);
@@ -680,14 +688,13 @@ static int row_groups(int type, int page_log, int64_t rows) {
 static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
 static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : wr == kPaWideF32 ? 64 : 128; }
 
-// Positions that one partial result may cover. The tensor cores add to fp32 by cutting bits off: each addition takes
-// up to 2^-23, on average 4e-8, of the sum away. With these bounds an output is within 7e-6 of the exact one at any
-// length (unbounded, 1.9e-5 at 9000 positions); half of them would make that 4e-6 and a long shared prompt 5% slower.
-// fp16: 288 additions, 2 per 16 positions; fp32: 252, 3 per 16. `share` accumulators have a unit's positions.
+// Positions that one unit may cover, by the additions into an accumulator (cut_back): fp16 144 of them, 2 per 16 positions; fp32
+// 192, 3 per 16. `share` accumulators have a unit's positions (kPaWidePair takes its own out in time). An output is then
+// within 2.5e-6 of the exact one at any length; unbounded, 1.9e-5 at 9000 positions.
 static int most_positions(int type, int wr) {
     const bool f16 = type == QMS_T_F16;
-    const int share = wr == kPaWidePair ? 1 : wr < 0 ? 2 : f16 ? 4 / wr : wr == 4 ? 1 : 2;
-    return (f16 ? 2304 : 1344) * share;
+    const int share = wr < 0 ? 2 : f16 ? 4 / wr : wr == 4 ? 1 : 2;
+    return wr == kPaWidePair ? 1 << 30 : (f16 ? 1152 : 1024) * share;
 }
 
 // Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
@@ -708,7 +715,7 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
 
 static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
     const int tp = tile_positions(type, wr), most = most_positions(type, wr);
-    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, 1 << 30);      // (in pieces, below)
+    if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
     const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, 148 * per_sm, wr == 4 ? 2.0 : 1.2, 4.0, most);
@@ -726,17 +733,7 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     p.chunk_p = chunk_for(type, p.wr_p, a.prefix, (int64_t)p.tiles_p * a.Hk, all);
     p.chunk_s = chunk_for(type, p.wr_s, own, (int64_t)p.tiles_s * a.Hk * a.n_seq, all);
     p.slots_p = p.chunks_p = (a.prefix + p.chunk_p - 1) / p.chunk_p;
-    p.piece_s = p.chunk_s;
-    p.pieces_s = 1;
-    const int most_s = most_positions(type, p.wr_s);
-    if (p.wr_s == kPaWidePair && p.chunk_s > most_s) {                      // units of several slots
-        const int tp = tile_positions(type, p.wr_s), n = (p.chunk_s + most_s - 1) / most_s;
-        p.piece_s = ((p.chunk_s + n - 1) / n + tp - 1) / tp * tp;
-        p.pieces_s = n;
-        p.chunk_s = n * p.piece_s;
-    }
-    p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
-    p.slots_s = (own + p.piece_s - 1) / p.piece_s;
+    p.slots_s = p.chunks_s = (own + p.chunk_s - 1) / p.chunk_s;
     if (p.wr_p <= 0 && p.chunks_p > 0 && p.tiles_p > 0) {
         p.line_tp = tile_positions(type, p.wr_p);
         p.line_rows = tile_rows(p.wr_p);

@@ -16,8 +16,8 @@
 //               under the largest scale so far (O is in its units)
 // O stays in TMEM over the whole unit. A base is set 2^8 below a maximum and stays until a score lies 2^15 above it
 // (fp16 holds weights to 2^16), so that the maximum needs no pass of its own; the result does not depend on
-// it beyond rounding. In PAIR a long unit leaves O as a partial result after every 18 tiles and starts anew (tensor cores
-// add by cutting bits off, the longer the more), with the Q that is there; the other units are that short.
+// it beyond rounding. In PAIR O is taken out after every 8 tiles and added to the unit's partial result in global memory
+// (tensor cores add by cutting bits off, the longer the more); the other units are that short.
 //
 // Warps 0-3 and 4-7 are the softmax of the two streams. One warp brings K and V in by TMA, a box per page: 64 swizzled
 // values x the page's positions (fp32: whole rows, into a staging ring, from which four warps write the terms). Tiles
@@ -49,7 +49,7 @@ struct WideCfg {
     static constexpr int TP = MODE == F32 ? 64 : 128, ROWS = MODE == PAIR ? 256 : 128;     // positions per tile, rows per unit
     static constexpr int THREADS = MODE == F32 ? 480 : 384, REGS = MODE == F32 ? 128 : 168;    // (4, 3 warps per scheduler)
     static constexpr int TMA_WARP = MODE == F32 ? 12 : 8, MMA_WARP = MODE == F32 ? 13 : 10;
-    static constexpr bool PIECES = MODE == PAIR;                // units of more than one partial result
+    static constexpr int PIECE = MODE == PAIR ? 8 : 1 << 30;    // tiles that O adds up before it is taken out
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t QHALF = 128 * 128, QTILE = HALVES * QHALF;     // one term of 128 rows of Q
     static constexpr uint32_t HALF = TP * 128, TILE = HALVES * HALF;         // one term of a K or V tile
@@ -59,7 +59,7 @@ struct WideCfg {
     // then: bad-page masks [8][4]; scales of K and V tiles [2][4], maxima [2][4]; a stream's (B, l, V scale) by row;
     // barriers; flags
     static constexpr uint32_t BAD = STAGE + 2 * STAGED, UP = BAD + 128, JOIN = UP + 64,
-                              BARS = JOIN + (MODE == PAIR ? 0 : 128 * 12), SMEM = BARS + 24 * 8 + 32;
+                              BARS = JOIN + (MODE == PAIR ? 256 * 8 : 128 * 12), SMEM = BARS + 24 * 8 + 32;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
     // Load n of a ring (K, V, K, ...): its slot. One ring for both streams; in SPLIT a ring per stream.
     static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return MODE == SPLIT ? 2 * stream + (n & 1) : n % 3; }
@@ -104,10 +104,26 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// 32 bytes to global memory (32-byte aligned), or zeros
-__device__ __forceinline__ void st_v8(float *to, const uint32_t *v, bool zero) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(zero ? 0 : v[0]), "r"(zero ? 0 : v[1]),
-                 "r"(zero ? 0 : v[2]), "r"(zero ? 0 : v[3]), "r"(zero ? 0 : v[4]), "r"(zero ? 0 : v[5]), "r"(zero ? 0 : v[6]), "r"(zero ? 0 : v[7])
+// Lane r of 8 holds the 16-byte pieces 0 .. 7 of row r; then lane p holds piece p of the rows 0 .. 7.
+__device__ __forceinline__ void transpose8(uint32_t (&v)[32], int lane) {
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) {
+        const bool up = lane & s;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (!(k & s))
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t &x = v[4 * k + e], &y = v[4 * (k + s) + e];
+                    const uint32_t got = __shfl_xor_sync(kFull, up ? x : y, s);
+                    x = up ? got : x;
+                    y = up ? y : got;
+                }
+    }
+}
+__device__ __forceinline__ void red4(float *to, const uint32_t *v) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(__uint_as_float(v[0])), "f"(__uint_as_float(v[1])),
+                 "f"(__uint_as_float(v[2])), "f"(__uint_as_float(v[3]))
                  : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -139,15 +155,15 @@ struct WideSync {
 
 // One unit of work, as every role derives it.
 struct WideUnit {
-    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, lo, run, cut;
-    // kv head; sequence, its first row, rows and length (own); slot of the (first) partial result; positions
+    int kh, b, t0, n, kv, slot, k0, k1, kmin, r0, rows, nt, lo;
+    // kv head; sequence, its first row, rows and length (own); slot of the partial result; positions
     // [k0, k1) in nt tiles, of which those below kmin belong to another unit; first row and number of rows of the
-    // segment; every row of the unit sees the positions up to lo; (PAIR) first run of the line, tiles in the first part
+    // segment; every row of the unit sees the positions up to lo
 };
 
 // The units of this CTA in order. Own positions: units blockIdx.x, + gridDim.x, ... of (chunk, sequence, row tile, kv
 // head). Shared positions: all (row tile, kv head, position tile) triples in one line, cut into equal runs, the
-// same number for each CTA; a unit is what a run (PAIR: all runs of the CTA) has of one row tile and kv head.
+// same number for each CTA; a run is one unit per row tile and kv head that it crosses.
 template <class C>
 struct WideWork {
     const PagedAttn &A;
@@ -163,8 +179,6 @@ struct WideWork {
             end = line_start(A.p, (blockIdx.x + 1) * A.p.line_per);
         }
     }
-    // tiles in part i >= 1 of the unit (a partial result of its own), or more where the unit ends in it
-    __device__ int piece(const WideUnit &w, int i) const { return own ? A.p.piece_s / C::TP : A.p.line_q + (w.run + i < A.p.line_r); }
     __device__ bool next(WideUnit &w) {
         const Paged &a = A.a;
         while (x < end) {
@@ -180,18 +194,16 @@ struct WideWork {
                 d = u / a.n_seq;
                 w.b = u - d * a.n_seq;
                 paged_seq(a, w.b, w.t0, w.n, w.kv);
-                if (C::PIECES) w.cut = A.p.piece_s / C::TP;
                 w.k0 = A.p.base_s + d * A.p.chunk_s;
                 w.kmin = max(w.k0, a.prefix);
                 w.k1 = min(w.kv, w.k0 + A.p.chunk_s);
                 w.k1 = min(w.k1, w.kv - w.n + min(w.n - 1, (w.r0 + C::ROWS - 1) / a.G) + 1);     // nobody sees the rest
-                w.slot = A.p.slots_p + (C::PIECES ? d * A.p.pieces_s : d);
+                w.slot = A.p.slots_p + d;
                 w.rows = w.n * a.G;
                 w.lo = w.kv - w.n + w.r0 / a.G;
             } else {
                 const unsigned nt = A.p.line_nt, u = x / nt, j = x - u * nt, tile = u / a.Hk;
-                const unsigned run = line_run(A.p, x), c = min(nt - j, C::PIECES ? end - x : line_start(A.p, run + 1) - x);
-                if (C::PIECES) w.run = run, w.cut = line_start(A.p, run + 1) - x;
+                const unsigned run = line_run(A.p, x), c = min(nt - j, line_start(A.p, run + 1) - x);
                 x += c;
                 w.kh = u - tile * a.Hk;
                 w.r0 = tile * C::ROWS;
@@ -286,6 +298,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
         // ---- softmax of stream i: thread = row = TMEM lane
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        float2 *s_sum = reinterpret_cast<float2 *>(s_join) + (MODE == PAIR ? i * 128 + row : 0);
         const uint32_t s_col = lanes + i * 128, o_col = lanes + C::O_COL + i * D;
         uint32_t ns = 0, nv = 0, before = 0, unit_no = 0;      // phases of s_full, of V; position tiles, units before
         bool ok = true;
@@ -372,6 +385,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
 
             const int lim = min(pos, w.k1 - 1);   // last position that this row sees
+            float grown = 0.0f;                   // sum over the tiles of l after each
             uint32_t vup = 0;                     // F32: the scale of V that O is in
             // O times a power of 2 (the MMAs on it ended before the S at hand was announced)
             auto scale_o = [&](float fac) {
@@ -385,14 +399,15 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     tmem_st32(o_col + 32 * k, o);
                 }
             };
-            // a part of the unit, of one partial result: the tiles from position kp on, up to tile n1
-            int n = 0, n1 = C::PIECES ? min(nt, w.cut) : nt, kp = w.kmin, piece = 0;
+            // O adds up the tiles from position kp on, up to tile n1
+            int n = 0, n1 = min(nt, C::PIECE), kp = w.kmin;
+            if (MODE == PAIR) *s_sum = make_float2(-INFINITY, 0.0f);
             float B = -INFINITY;
             float2 l2 = make_float2(0.0f, 0.0f);
         next_part:                                // (as a loop around all this, 1 us more per call)
             for (; n < n1; n++) {
                 const int j = MODE == PAIR ? n : 2 * n + first_of(i, before), base = w.k0 + j * C::TP;
-                if (!C::PIECES || n == 0 || base > kp) {           // (else waited for already)
+                if (MODE != PAIR || n == 0 || base > kp) {           // (else waited for already)
                     if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;       // the whole warp or none of it
                     ns++;
                     tc_fence_after();
@@ -400,8 +415,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 const uint32_t *bad = s_bad + ((before + j) & 7) * 4;
                 uint32_t any_bad = bad[0] | bad[1];
                 if constexpr (C::TP == 128) any_bad |= bad[2] | bad[3];
-                // rows that see nothing of this part are not read from its slot: no mask for them
-                if (__any_sync(kFull, lim >= kp && lim < base + C::TP - 1) || base < w.kmin || any_bad) {
+                // rows that see nothing of this unit are not read from its slot: no mask for them
+                if (__any_sync(kFull, lim >= w.kmin && lim < base + C::TP - 1) || base < w.kmin || any_bad) {
 #pragma unroll 1
                     for (int c = 0; c < C::TP / 32; c++) {
                         const int d = lim - base - 32 * c, below = w.kmin - base - 32 * c;
@@ -432,7 +447,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         B = nb;
                         l2.x *= fac;
                         l2.y *= fac;
-                        if (n > 0 && (!C::PIECES || base > kp)) scale_o(fac);
+                        grown *= fac;
+                        if (n > 0 && (MODE != PAIR || base > kp)) scale_o(fac);
                         const __half2 fh = __float2half2_rn(fac);
 #pragma unroll 1
                         for (int k = 0; k < 4; k++) {
@@ -484,6 +500,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     if (up != vup && n > 0) scale_o(vup - up > 126 ? 0.0f : pow2_bits(127u - (vup - up)));
                     vup = up;
                 }
+                grown += l2.x + l2.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -500,7 +517,10 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
             float l = l2.x + l2.y;
             if (isnan(l) && B == -INFINITY) B = 0.0f;
-            float w0 = MODE == F32 && nt > 0 ? pow2_bits(254u - vup) : 1.0f, w1 = 0.0f;
+            // additions per tile: of the hi terms while l grows, then of the others
+            constexpr float ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
+            float w0 = cut_back(MODE != F32, grown, l, ADDS, RISE), w1 = 0.0f;
+            if (MODE == F32 && nt > 0) w0 *= pow2_bits(254u - vup);
             if constexpr (MODE != PAIR) {
                 // stream 1 leaves its (B, l, scale); stream 0 reads both O (the same TMEM lanes) and writes the rows
                 if (i == 1) {
@@ -521,19 +541,33 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 l = c0 * l + c1 * l1;
                 B = M;
             }
-            const bool put = tok >= 0 && lim >= kp, none = l == 0.0f, fix = *s_flag != 0;
-            const int64_t first = (int64_t)(w.slot + piece) * a.n_tok * a.H;
+            const bool put = tok >= 0 && lim >= w.kmin, none = l == 0.0f, fix = *s_flag != 0;
+            const int64_t first = (int64_t)w.slot * a.n_tok * a.H;
             const int row_out = put ? tok : -1;
             float *part = A.part_o + first * D + (lane & 7) * 4;
-            // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8
-            // lanes; while Q is still wanted, each lane writes its row (as fast as by shuffles)
+            // PAIR: the unit's earlier sums are in the slot, with their base and l in *s_sum: this one joins them in that base, or,
+            // where it is far above (and for the first), takes their place
+            bool over = true;
+            if (MODE == PAIR && put) {
+                const float2 sum = *s_sum;
+                over = !(B - sum.x <= 40.0f);
+                const float f = over || none ? 1.0f : ex2(B - sum.x);
+                *s_sum = over ? make_float2(B, l + (sum.y == 0.0f ? 0.0f : sum.y * ex2(sum.x - B))) : make_float2(sum.x, fmaf(l, f, sum.y));
+                w0 *= f;
+            }
+            const uint32_t fresh = __ballot_sync(kFull, over);
+            // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes; while Q is
+            // still wanted, by shuffles
             unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
                 tmem_ld<32>(o_col + 32 * c, o);
                 tmem_wait_ld(o);
-                if constexpr (MODE != PAIR) {
+                if constexpr (MODE == PAIR) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
+                } else {
                     uint32_t o1[32];
                     tmem_ld<32>(o_col + D + 32 * c, o1);
                     tmem_wait_ld(o1);
@@ -544,7 +578,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
                     typedef typename std::conditional<MODE == F32, float, __half>::type KT;
-                    const int past = C::PIECES ? min(lim + 1, w.k0 + n1 * C::TP) : lim + 1;
+                    const int past = MODE == PAIR ? min(lim + 1, w.k0 + n1 * C::TP) : lim + 1;
                     for (int p = kp; p < past; p++) {
                         const int64_t at = paged_at(a, a.table + (own ? (int64_t)w.b * a.table_stride : 0), p);
                         if (at < 0) continue;
@@ -556,32 +590,48 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         }
                     }
                 }
-                if (C::PIECES && n < nt) {
-                    if (put)
+                if (none)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) st_v8(A.part_o + (first + tok) * D + 32 * c + e, o + e, none);
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                if (MODE == PAIR && n < nt) {
+                    transpose8(o, lane);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int rr = (lane & 24) + k, to = __shfl_sync(kFull, row_out, rr);
+                        float *dst = part + (int64_t)to * D + 32 * c;
+                        if (to >= 0 && (fresh >> rr & 1)) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        else if (to >= 0) red4(dst, o + 4 * k);
+                    }
                     continue;
                 }
                 __syncwarp();
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)   // 16-byte piece e / 4 of row `lane`, XOR-placed against bank conflicts
                     *reinterpret_cast<uint4 *>(stage + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)) =
-                        none ? make_uint4(0, 0, 0, 0) : make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 __syncwarp();
 #pragma unroll
                 for (int k = 0; k < 8; k++) {     // 4 rows of 128 bytes at a time
                     const int rr = 4 * k + (lane >> 3), to = __shfl_sync(kFull, row_out, rr);
                     const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                    if (to >= 0) *reinterpret_cast<uint4 *>(part + (int64_t)to * D + 32 * c) = v;
+                    float *dst = part + (int64_t)to * D + 32 * c;
+                    if (to >= 0 && (MODE != PAIR || (fresh >> rr & 1))) *reinterpret_cast<uint4 *>(dst) = v;
+                    else if (MODE == PAIR && to >= 0) red4(dst, reinterpret_cast<const uint32_t *>(&v));
                 }
             }
-            if (put) A.part_ml[first + tok] = make_float2(none ? -INFINITY : B, l);
+            if constexpr (MODE == PAIR) {
+                __syncwarp();                     // (other lanes may add to a row later)
+                if (put && n == nt) A.part_ml[first + tok] = make_float2(s_sum->y == 0.0f ? -INFINITY : s_sum->x, s_sum->y);
+            } else if (put) {
+                A.part_ml[first + tok] = make_float2(none ? -INFINITY : B, l);
+            }
             tc_fence_before();
-            if (C::PIECES && n < nt) {
+            if (MODE == PAIR && n < nt) {
                 kp = w.k0 + n * C::TP;
-                n1 = min(nt, n + work.piece(w, ++piece));
+                n1 = min(nt, n + C::PIECE);
                 B = -INFINITY;
                 l2 = make_float2(0.0f, 0.0f);
+                grown = 0.0f;
                 goto next_part;
             }
         }
@@ -760,11 +810,11 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             auto score = [&](uint32_t n) {                     // S_i = Q_i K^T
                 const uint32_t k = sm0 + C::RING + C::slot(i, n) * C::SLOT, q = sm0 + (MODE == PAIR ? i * 2 * C::QTILE : 0);
 #pragma unroll
-                for (int term = 0; term < TERMS; term++)
+                for (int x = 0; x < TERMS; x++)                 // (the large one last)
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++)
+                    for (int ks = 0, term = TERMS - 1 - x; ks < D / 16; ks++)
                         umma_f16_ss(tmem + i * 128, desc_sw128(q + (term == 1) * C::QTILE + (ks >> 2) * C::QHALF + (ks & 3) * 32, 16, 1024),
-                                    desc_sw128(k + (term == 2) * C::TILE + (ks >> 2) * C::HALF + (ks & 3) * 32, 16, 1024), id_s, term || ks);
+                                    desc_sw128(k + (term == 2) * C::TILE + (ks >> 2) * C::HALF + (ks & 3) * 32, 16, 1024), id_s, x || ks);
             };
             auto weigh = [&](uint32_t n, bool first) {         // O_i (+)= P_i V
                 const uint32_t v = sm0 + C::RING + C::slot(i, n) * C::SLOT;
@@ -800,14 +850,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         umma_commit(&s_full[i]);
                         umma_commit(&empty[C::slot(i, c)]);
                     }
-                    int piece = 0, next = C::PIECES ? w.cut : nt;
                     for (int j = 0; ok && j < nt; j++, c += NEXT, nf++) {
                         const bool more = j + 1 < nt;
                         if (!(ok = sy.wait(v_bar(c + 1), MODE == F32 ? nf & 1 : C::phase(c + 1)) && sy.wait(&p_full[i], np++ & 1))) break;
                         tc_fence_after();
                         lock();
-                        weigh(c + 1, j == 0 || (C::PIECES && j == next));
-                        if (C::PIECES && j == next) next += work.piece(w, ++piece);
+                        weigh(c + 1, MODE == PAIR ? j % C::PIECE == 0 : j == 0);
                         if (more) {
                             const uint32_t ph = MODE == F32 ? (nf + 1) & 1 : C::phase(c + NEXT);
                             if (!mbar_test_wait(k_bar(c + NEXT), ph)) {      // K is late: not at the other's cost

@@ -207,9 +207,9 @@ def test_attention_masked_values_have_no_effect(cuda, typ, n, prefix, bad):
 @pytest.mark.parametrize("typ", ["f16", "f32"])
 @pytest.mark.parametrize("prefix", [0, 4900])
 def test_attention_long_units(cuda, typ, prefix):
-    """So many rows that the positions are hardly cut: a result of thousands of additions. With a the additions into an
-    fp32 sum (at most 288) that each cut at most 2^-23, on average 0.72 * 2^-24, of it off, the outputs' 2-norm is off by
-    288 * 0.72 * 2^-24 / 2 = 6.2e-6 of itself where the sum grows steadily; 1e-5 with the scores' share."""
+    """So many rows that the positions are hardly cut: results of thousands of additions into one fp32 sum. Where each cuts at
+    most 2^-23, on average 0.72 * 2^-24, of the sum off, 288 of them leave the outputs' 2-norm off by 288 * 0.72 * 2^-24 / 2 =
+    6.2e-6 of itself; 1e-5 with the scores' share."""
     import torch
     import large_model_b200 as m
     B, n, G, Hk, D = 20, 17, 8, 8, 64
