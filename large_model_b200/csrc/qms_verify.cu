@@ -38,7 +38,8 @@ constexpr int kProbsKeep = 19456, kProbsThreads = 512, kProbsWarps = kProbsThrea
 // cluster. A slice comes into shared memory by cp.async (16 bytes at a time where the row is aligned); its
 // weights replace it there, relative to the slice's own maximum, and one exchange over the cluster gives every
 // CTA the common factor. The order of the additions does not depend on the row's address.
-// Bound by memory: 320 rows of 151,936 move 389 MB.
+// Bound by memory: 320 rows of 151,936 move 389 MB in 84 us, 4.6 TB/s, 0.72 of a plain copy (reading all of a row comes before
+// writing any of it; three CTAs per SM overlap). One row: 6.3 us, launch, one round trip, the exchange.
 template <bool GREEDY>
 __global__ void __launch_bounds__(kProbsThreads, 3) k_probs(const float *l, int64_t ldl, int V, float c, float *p, int64_t ldp) {
     extern __shared__ __align__(16) float x[];
@@ -231,14 +232,16 @@ struct Remains {
     }
 };
 
+constexpr int kVerifyThreads = 256;
+
 // One cluster per sequence: the drafts first (every CTA finds the same count), then the next token by
 // inversion of the cumulative weights of the row. Every warp adds up its segment, 256 values at a time, and keeps
 // those sums; the one warp whose segment holds the wanted weight finds the 256, then the 32, then the value.
-// Bound by the latencies of that chain (drafts, their probabilities, the row, the exchange, the search) for
-// one sequence, by memory for many.
-template <int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) k_verify(const VerifyArgs a) {
-    constexpr int kWarps = NT / 32;
+// Bound by the latencies of that chain (drafts, their probabilities, the row, the exchange, the search) for one sequence
+// (8.8 us), by memory for many: 64 sequences with the draft's probabilities, 78 MB in 16.8 us, 4.6 TB/s. 256 threads, so that
+// many clusters are resident: with 1024, 16 sequences took 16.1 us against 10.0, 128 sequences 76 against 32.
+__global__ void __launch_bounds__(kVerifyThreads, 4) k_verify(const VerifyArgs a) {
+    constexpr int NT = kVerifyThreads, kWarps = NT / 32;
     extern __shared__ u64 s_sum[];                         // [kWarps][batches] sums of 256 values
     __shared__ u64 s_w[kWarps], s_c[2][kRowCtas];
     __shared__ int s_n;
@@ -390,11 +393,12 @@ static int launch_rows(void (*kern)(P...), int threads, int rows, int nc, size_t
     return QMS_CUDA_OK;
 }
 
-// CTAs per row: as many as hold it in shared memory (k_probs), then, while the rows leave SMs without a CTA, twice
-// as many (of 4096 values or more).
-static int row_ctas(int rows, int V) {
+// CTAs per row: as many as hold it in shared memory (k_probs), then, while all of them are at most `sms`, twice as many (of
+// 4096 values or more). A row of 32,000 in us, by two CTAs and by four: k_probs (up to 74) 1 row 5.6, 4.5; 16 rows 5.7, 4.8; 37
+// rows 5.8, 6.7; k_verify (up to 148) 1 sequence 7.6, 6.7; 32 sequences 8.3, 6.5.
+static int row_ctas(int rows, int V, int sms) {
     int nc = 1;
-    while (nc < kRowCtas && (V > nc * kProbsKeep || ((int64_t)rows * nc * 2 <= 148 && V > nc * 8192))) nc *= 2;
+    while (nc < kRowCtas && (V > nc * kProbsKeep || ((int64_t)rows * nc * 2 <= sms && V > nc * 8192))) nc *= 2;
     return nc;
 }
 
@@ -407,7 +411,7 @@ static int launch_probs(const float *l, int64_t ldl, int rows, int V, float temp
         QMS_CK(cudaFuncSetAttribute(k_probs<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsKeep * 4));
         set |= 1ull << (dev & 63);
     }
-    const int nc = row_ctas(rows, V), slice = ((V + 3) / 4 / nc + 1) * 4;
+    const int nc = row_ctas(rows, V, 74), slice = ((V + 3) / 4 / nc + 1) * 4;
     const size_t smem = (size_t)(slice < kProbsKeep ? slice : kProbsKeep) * 4;
     if (!(temp > 0.0f)) return launch_rows(k_probs<true>, kProbsThreads, rows, nc, smem, s, l, ldl, V, 0.0f, p, ldp);
     // a scale of 0 or infinity would make NaN of the logits -inf and of the maximum
@@ -416,12 +420,9 @@ static int launch_probs(const float *l, int64_t ldl, int rows, int V, float temp
 }
 
 static int launch_verify(const VerifyArgs &a, cudaStream_t s) {
-    // few sequences: CTAs of 1024 threads, the shortest chain; more than the SMs hold of those: 256 threads, so
-    // that 64 sequences and more are resident at once
-    const int nc = row_ctas(a.n_seq, a.V), nt = a.n_seq * nc <= 148 ? 1024 : 256, segs = nc * (nt / 32);
-    const size_t smem = (size_t)(nt / 32) * ((a.V / segs + 256) / 256) * 8;
-    if (nt == 1024) return launch_rows(k_verify<1024>, nt, a.n_seq, nc, smem, s, a);
-    return launch_rows(k_verify<256>, nt, a.n_seq, nc, smem, s, a);
+    const int nc = row_ctas(a.n_seq, a.V, 148), warps = kVerifyThreads / 32;
+    const size_t smem = (size_t)warps * ((a.V / (nc * warps) + 256) / 256) * 8;
+    return launch_rows(k_verify, kVerifyThreads, a.n_seq, nc, smem, s, a);
 }
 
 }  // namespace qms
