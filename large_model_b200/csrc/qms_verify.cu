@@ -395,7 +395,8 @@ static int launch_rows(void (*kern)(P...), int threads, int rows, int nc, size_t
 
 // CTAs per row: as many as hold it in shared memory (k_probs), then, while all of them are at most `sms`, twice as many (of
 // 4096 values or more). A row of 32,000 in us, by two CTAs and by four: k_probs (up to 74) 1 row 5.6, 4.5; 16 rows 5.7, 4.8; 37
-// rows 5.8, 6.7; k_verify (up to 148) 1 sequence 7.6, 6.7; 32 sequences 8.3, 6.5.
+// rows 5.8, 6.7; k_verify (up to 148) 32 sequences
+// 8.3, 6.4.
 static int row_ctas(int rows, int V, int sms) {
     int nc = 1;
     while (nc < kRowCtas && (V > nc * kProbsKeep || ((int64_t)rows * nc * 2 <= sms && V > nc * 8192))) nc *= 2;
