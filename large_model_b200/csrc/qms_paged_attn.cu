@@ -680,13 +680,17 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read), k_paged_wide
-// from 65 on (fp16: in pages of 8 positions or more, a swizzle unit of its tiles). Narrow against wide in us, for 16 sequences
-// of 1000 positions and 16 q heads per kv head: 64 rows 25.3, 24.7 (fp32 40.4, 43.4); 80 rows 38.9, 25.9 (68.9, 43.5); 128 rows
-// 40.0, 27.3 (70.8, 46.2). On one prompt of 4096 positions narrow keeps ahead a little longer: 96 rows 23.2, 25.0 (31.4, 36.7).
-static int row_groups(int type, int page_log, int64_t rows) {
-    if (rows > 64 && type != QMS_T_F16) return kPaWideF32;
-    if (rows > 64 && page_log >= 3) return rows > 128 ? kPaWidePair : kPaWideSplit;
+// Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); k_paged_wide
+// from 65 on (fp16: in pages of 8 positions or more, a swizzle unit of its tiles) and from so many rows x positions (`rows`
+// by the 64, over all units) that its longer start pays. Narrow against wide in us, 16 q heads per kv head, 4 of these:
+// 80 rows x 16 sequences x 1000 positions 38.8, 25.8 (fp32 68.3, 43.3); 64 rows of the same 25.3, 24.7 (40.4, 43.4). By millions
+// of rows x positions: own ones 1.2 narrow 17.1, wide 21.9 (22.1, 20.9); 2.5 22.5, 26.6 (31.1, 29.3); 3.1 24.2, 23.6 (35.4, 28.1); 4.1
+// 25.2, 22.8 (39.9, 30.4); shared ones 1.6 22.8, 24.6 (34.1, 34.6); 3.1 29.2, 26.8 (41.9, 40.2); 6.3 37.4, 38.2 (62.4, 50.7); 16.8 71, 44
+// (130, 85).
+static int row_groups(int type, int page_log, int64_t rows, int64_t positions, bool shared) {
+    const bool f16 = type == QMS_T_F16;
+    if (rows > 64 && (!f16 || page_log >= 3) && (rows + 63) / 64 * 64 * positions > (f16 || shared ? 2600000 : 1200000))
+        return !f16 ? kPaWideF32 : rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
 }
 static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
@@ -728,8 +732,8 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows) {
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
     memset(&p, 0, sizeof p);
-    p.wr_p = row_groups(type, a.page_log, rows_p);
-    p.wr_s = row_groups(type, a.page_log, rows_s);
+    p.wr_p = row_groups(type, a.page_log, rows_p, (int64_t)a.prefix * a.Hk, true);
+    p.wr_s = row_groups(type, a.page_log, rows_s, (int64_t)std::max(0, a.max_kv - a.prefix) * a.Hk * a.n_seq, false);
     p.base_s = a.prefix & ~(std::min(1 << a.page_log, tile_positions(type, p.wr_s)) - 1);
     const int own = std::max(0, a.max_kv - p.base_s);
     p.tiles_p = (int)((rows_p + tile_rows(p.wr_p) - 1) / tile_rows(p.wr_p));

@@ -278,6 +278,148 @@ def test_attention_bad_arrays_are_reported(cuda, typ):
     batch.status()
 
 
+# ---- the same where many rows meet many positions: the bounds of a call say so, so idle sequences (own positions) and padding
+# rows (a shared prompt) make a small batch count as a large one
+
+def crowd(qs, kv, G, Hk, prefix=0):
+    """(qs, kv) with so many idle sequences that the own positions count as 3 million rows x positions."""
+    rows = -(-max(qs) * G // 64) * 64
+    assert max(qs) * G > 64
+    n = max(0, -(-3000000 // (rows * max(1, max(kv) - prefix) * Hk)) - len(qs))
+    return list(qs) + [0] * n, list(kv) + [prefix] * n
+
+
+def padding(qs, G, Hk, prefix):
+    """Padding rows with which the shared positions count as 3 million rows x positions."""
+    return max(0, -(-3000000 // (prefix * Hk * G)) - sum(qs))
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,kv,G,page", [(70, 70, 1, 16), (33, 300, 2, 8), (129, 129, 1, 64), (200, 1111, 4, 16), (9, 1030, 8, 128), (17, 640, 16, 512)])
+def test_attention_crowded_chunks(cuda, typ, D, n, kv, G, page):
+    qs, kvs = crowd([n, 1, 31], [kv, 40, 31], G, 2)
+    check(qs, kvs, typ=typ, D=D, G=G, Hk=2, page=page, seed=n)
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("page", [1, 2, 4, 32, 1024])
+def test_attention_crowded_page_sizes(cuda, typ, page):
+    qs, kvs = crowd([9, 3, 0, 2], [400, 129, 0, 17], 8, 1)
+    check(qs, kvs, typ=typ, page=page, G=8, Hk=1, D=64, seed=page)
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("prefix", [1, 16, 100, 127, 128, 129, 300, 2100])
+def test_attention_crowded_shared_prompt(cuda, typ, prefix):
+    qs, new = [1, 4, 0, 2, 1], [5, 4, 0, 130, 1]
+    check(qs, [prefix + n for n in new], typ=typ, prefix=prefix, G=8, D=64, seed=prefix, pad=min(12000, padding(qs, 8, 2, prefix)))
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attention_crowded_prompt_inside_the_shared_part(cuda, typ):
+    check([90, 1], [90, 91], typ=typ, prefix=90, G=4, pad=padding([91], 4, 2, 90))
+    check([150], [200], typ=typ, prefix=130, G=2, pad=padding([150], 2, 2, 130))
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attention_crowded_layouts(cuda, typ):
+    qs, kv = crowd([1, 5, 40], [77, 130, 90], 16, 2, 33)
+    check(qs, kv, typ=typ, order="hnd", prefix=33, G=16, Hk=2, pad=padding(qs, 16, 2, 33))
+    qs, kv = crowd([1, 5, 40], [77, 130, 90], 6, 3)
+    check(qs, kv, typ=typ, order="hnd", garbage=float("inf"), D=64, G=6, Hk=3)
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attention_crowded_scores(cuda, typ):
+    """One position takes all the weight; equal scores; q beyond the range of 16-bit types; scores that rise by far over the tiles."""
+    import torch
+    import large_model_b200 as m
+    qs, kv = crowd([70, 3], [1300, 64], 2, 2)
+    for kw in (dict(qscale=200.0), dict(scale=0.0), dict(qscale=1e30, scale=1e-31), dict(qscale=1e-30, scale=1e29), dict(scale=-0.1)):
+        check(qs, kv, typ=typ, G=2, **kw)
+    qs, kv = crowd([70, 130], [1300, 1290], 2, 2)
+    pages, batch, q, K, V = make(qs, kv, typ=typ, G=2)
+    for b in range(2):                               # K grows with the position, so that the maximum moves in every tile
+        K[b] *= (torch.arange(kv[b], device="cuda").to(K[b].dtype) / 100)[:, None, None]
+        j = torch.arange(kv[b], device="cuda")
+        pages.k[batch.table[b].long()[j // 16], j % 16] = K[b]
+    for scale in (0.05, 1.0):
+        out = m.paged_attention(pages, batch, q, 4, scale=scale)
+        batch.status()
+        want, tol = reference(qs, kv, q, K, V, 2, scale)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("n", [40, 130])
+def test_attention_crowded_rows_that_see_nothing(cuda, typ, n):
+    import torch
+    import large_model_b200 as m
+    qs, kv = crowd([0, n, 2, 0], [0, n - 2, 50, 7], 4, 2)
+    pages, batch, q, K, V = make(qs, kv, typ=typ, G=4, pad=3)
+    out = torch.full((sum(qs) + 3, 8 * 128), float("nan"), device="cuda")
+    m.paged_attention(pages, batch, q, 8, out=out)
+    batch.status()
+    want, tol = reference(qs, kv, q, K, V, 4, 128 ** -0.5)
+    assert (out[:2] == 0).all() and (out[-3:] == 0).all()
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+@pytest.mark.parametrize("n,prefix", [(5, 40), (64, 0), (140, 0), (9, 50)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_crowded_masked_values_have_no_effect(cuda, typ, n, prefix, bad):
+    """K and V of the newest token are not finite: only its own row may show it."""
+    import large_model_b200 as m
+    kv = 45 + n
+    qs, kvs = crowd([n, 1], [kv, prefix + 3], 16, 1, prefix)
+    pages, batch, q, K, V = make(qs, kvs, typ=typ, G=16, Hk=1, prefix=prefix, pad=padding(qs, 16, 1, prefix) if prefix else 0)
+    last = batch.table[0, (kv - 1) // 16].long()
+    pages.k[last, (kv - 1) % 16, 0, 5] = bad
+    pages.v[last, (kv - 1) % 16, 0, 7] = bad
+    K[0][-1, 0, 5] = 0
+    V[0][-1, 0, 7] = 0
+    out = m.paged_attention(pages, batch, q, 16)
+    batch.status()
+    want, tol = reference(qs, kvs, q, K, V, 16, 128 ** -0.5)
+    keep = [i for i in range(n + 1) if i != n - 1]
+    assert ((out.double() - want).abs() <= tol)[keep].all()
+    import torch
+    assert not torch.isfinite(out[n - 1].view(16, 128)[:, 7]).any()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attention_crowded_bad_arrays_are_reported(cuda, typ):
+    import torch
+    import large_model_b200 as m
+    qs, kv = crowd([1, 40, 1], [50, 60, 33], 16, 1)
+    pages, batch, q, K, V = make(qs, kv, typ=typ, G=16, Hk=1)
+    good = m.paged_attention(pages, batch, q, 16)
+    batch.status()
+    keep = batch.table.clone()
+    for bad in (-1, 10 ** 6, pages.k.shape[0]):      # a page that does not exist: not seen, and reported
+        batch.table[2, 1] = bad
+        out = m.paged_attention(pages, batch, q, 16)
+        with pytest.raises(m.QmsCudaError, match="0x2"):
+            batch.status()
+        batch.table.copy_(keep)
+        assert torch.equal(out[:41], good[:41])
+        k, v = (x[2][torch.arange(33, device="cuda") // 16 != 1] for x in (K, V))
+        want, tol = reference([1], [17], q[41:], [k], [v], 16, 128 ** -0.5)
+        assert ((out[41:].double() - want).abs() <= tol).all()
+    for what, value in (("kv_len", 61), ("kv_len", -5), ("q_start", -1), ("q_start", 100)):
+        t = getattr(batch, what)
+        was = t.clone()
+        t[1 if what == "kv_len" else 2] = value
+        m.paged_attention(pages, batch, q, 16)
+        with pytest.raises(m.QmsCudaError, match="0x1"):
+            batch.status()
+        t.copy_(was)
+    assert torch.equal(m.paged_attention(pages, batch, q, 16), good)
+    batch.status()
+
+
 @pytest.mark.parametrize("typ", ["f16", "f32"])
 def test_attention_offsets_past_32_bits(cuda, typ):
     """Two pages more than 2^32 bytes apart."""
@@ -300,6 +442,31 @@ def test_attention_offsets_past_32_bits(cuda, typ):
         batch.status()
         K, V = (x[[1, 0]].reshape(128, 1, 128)[:120] for x in (k, v))
         want, tol = reference(qs, kv, q, [K], [V], 16, 128 ** -0.5)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attention_crowded_offsets_past_32_bits(cuda, typ):
+    import torch
+    import large_model_b200 as m
+    dt, es = (torch.float16, 2) if typ == "f16" else (torch.float32, 4)
+    stride = (2 ** 32 + 2 ** 20) // es
+    pool = torch.empty((stride + 2 * 64 * 128,), dtype=dt, device="cuda")
+    k = pool.as_strided((2, 64, 1, 128), (stride, 128, 128, 1))
+    v = pool.as_strided((2, 64, 1, 128), (stride, 128, 128, 1), 64 * 128)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for x in (k, v):
+        x.copy_(torch.randn((2, 64, 1, 128), generator=g, device="cuda"))
+    for n, prefix in ((40, 0), (7, 100)):
+        qs, kv = crowd([n], [120], 16, 1, prefix)
+        q = torch.randn((n + 2000, 16 * 128), generator=g, device="cuda")
+        start = torch.tensor([0] + [n] * len(qs), dtype=torch.int32, device="cuda")
+        table = torch.tensor([[1, 0]] * len(qs), dtype=torch.int32, device="cuda")
+        batch = m.PagedBatch(start, torch.tensor(kv, dtype=torch.int32, device="cuda"), table, n + 2000, n, 120, prefix)
+        out = m.paged_attention(m.KvPages(k, v), batch, q, 16)
+        batch.status()
+        K, V = (x[[1, 0]].reshape(128, 1, 128)[:120] for x in (k, v))
+        want, tol = reference([n], [120], q, [K], [V], 16, 128 ** -0.5)
         assert ((out.double() - want).abs() <= tol).all()
 
 
