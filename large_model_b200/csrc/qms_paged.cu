@@ -12,7 +12,7 @@ namespace qms {
 // A warp takes R head rows of q | k | v of one token: y = R(pos) (w * x / sqrt(mean x^2 + eps)) for q and k, v unchanged.
 // The mean's sum is held in double and the steps are k_qk_rope's, each in its order, so a paged cache holds the same
 // values as the model's contiguous one.
-// Bound by latency for few rows (R = 1: 2.6 us for one token) and by instructions for many, most of them for the 64-bit
+// Bound by latency for few rows (R = 1: 2.5 us for one token) and by instructions for many, most of them for the 64-bit
 // mean: R = 4 rows share the exchanges of their sums and one square root and division (a lane each).
 template <int R>
 __device__ __forceinline__ void sum_rows(double (&v)[R], int lane) {      // the sum of v[r] over the lanes; R = 4: v[0] of row lane / 8
