@@ -494,9 +494,11 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         for (int i = 0; i < C::DW / 8; i++) o[i][0] *= back0, o[i][1] *= back0, o[i][2] *= back1, o[i][3] *= back1;
         // dims of this thread's o[i][0..1] (row g) and o[i][2..3] (row g + 8)
         auto dim = [&](int i, int j) { return wd * C::DW + i * 8 + tq * 2 + (j & 1); };
-        if (s_flag && wk == 0) {
-            // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
+        if (s_flag) {
+            // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight), by the group that
+            // scored the position: the join leaves out groups that saw nothing
             for (int p = kmin; p < k1; p++) {
+                if ((p - k0) % C::PS / C::KW != wk) continue;
                 const int64_t at = paged_at(a, table, p);
                 if (at < 0) continue;
                 const KT *vr = reinterpret_cast<const KT *>(a.v + at + kh * a.head_stride);
