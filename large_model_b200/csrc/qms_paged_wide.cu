@@ -129,6 +129,17 @@ __device__ __forceinline__ void red4(float *to, const uint32_t *v) {
                  "f"(__uint_as_float(v[2])), "f"(__uint_as_float(v[3]))
                  : "memory");
 }
+// v takes the place of the sums at `to`, and stays not finite where they were
+__device__ __forceinline__ void take_place(float *to, uint4 v, bool earlier) {
+    if (earlier) {
+        const float4 o = __ldcg(reinterpret_cast<const float4 *>(to));
+        v.x = __float_as_uint(fmaf(o.x, 0.0f, __uint_as_float(v.x)));
+        v.y = __float_as_uint(fmaf(o.y, 0.0f, __uint_as_float(v.y)));
+        v.z = __float_as_uint(fmaf(o.z, 0.0f, __uint_as_float(v.z)));
+        v.w = __float_as_uint(fmaf(o.w, 0.0f, __uint_as_float(v.w)));
+    }
+    *reinterpret_cast<uint4 *>(to) = v;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_tie(uint32_t (&r)[32]) {      // the same for a second array of that wait
@@ -549,7 +560,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             const int row_out = put ? tok : -1;
             float *part = A.part_o + first * D + (lane & 7) * 4;
             // PAIR: the unit's earlier sums are in the slot, with their base and l in *s_sum: this one joins them in that base, or,
-            // where it is far above (and for the first), takes their place
+            // where it is far above (and for the first), takes their place, but for what is not finite: no weight makes that nothing
             bool over = true;
             if (MODE == PAIR && put) {
                 const float2 sum = *s_sum;
@@ -558,7 +569,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 *s_sum = over ? make_float2(B, l + (sum.y == 0.0f ? 0.0f : sum.y * ex2(sum.x - B))) : make_float2(sum.x, fmaf(l, f, sum.y));
                 w0 *= f;
             }
-            const uint32_t fresh = __ballot_sync(kFull, over);
+            const uint32_t fresh = __ballot_sync(kFull, over), earlier = kp > w.kmin ? fresh : 0u;
             // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes; while Q is
             // still wanted, by shuffles
             unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
@@ -602,7 +613,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     for (int k = 0; k < 8; k++) {
                         const int rr = (lane & 24) + k, to = __shfl_sync(kFull, row_out, rr);
                         float *dst = part + (int64_t)to * D + 32 * c;
-                        if (to >= 0 && (fresh >> rr & 1)) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        if (to >= 0 && (fresh >> rr & 1)) take_place(dst, make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]), earlier >> rr & 1);
                         else if (to >= 0) red4(dst, o + 4 * k);
                     }
                     continue;
@@ -618,7 +629,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     const int rr = 4 * k + (lane >> 3), to = __shfl_sync(kFull, row_out, rr);
                     const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
                     float *dst = part + (int64_t)to * D + 32 * c;
-                    if (to >= 0 && (MODE != PAIR || (fresh >> rr & 1))) *reinterpret_cast<uint4 *>(dst) = v;
+                    if (to >= 0 && (MODE != PAIR || (fresh >> rr & 1))) take_place(dst, v, MODE == PAIR && (earlier >> rr & 1));
                     else if (MODE == PAIR && to >= 0) red4(dst, reinterpret_cast<const uint32_t *>(&v));
                 }
             }

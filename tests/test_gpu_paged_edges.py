@@ -57,3 +57,47 @@ def test_value_behind_a_bad_page(cuda, typ, G, n, kv):
     assert not torch.isfinite(out[..., 7]).any()
     out[..., 7] = want[..., 7].float()
     assert ((out.double() - want).abs() <= tol + want.abs() * 2.0 ** -24).all()
+
+
+# ---- the same in every kernel ---------------------------------------------------------------------------
+# (own positions: rows of a tile x positions x sequences; idle sequences count, and make one unit of a sequence's positions)
+
+KERNELS = [("f16", 1), ("f32", 1), ("f16", 2), ("f32", 2), ("f16", 4), ("f32", 4), ("f16", 8), ("f32", 8), ("f16", 16)]
+# tokens of 16 q heads each: 16, 32 or 64 rows over mma.sync; 128 rows over tcgen05, two streams of tiles; 256 rows, one stream per 128
+
+
+def one_unit(n, kv, **kw):
+    """One sequence of n tokens, and so many idle ones that all its positions are one unit of work."""
+    return make([n] + [0] * 69, [kv] + [0] * 69, G=16, Hk=2, page=64, **kw)
+
+
+def scores(pages, batch, q, K, s):
+    """q and K such that the scores of every row, in powers of two at scale ln 2, are s[position] (fp16 values)."""
+    import torch
+    q.zero_()
+    q[:, ::pages.head_dim] = 1.0
+    kv = len(s)
+    K[0].zero_()
+    K[0][:, :, 0] = s[:, None].to(K[0].dtype)
+    j = torch.arange(kv, device="cuda")
+    pages.k[batch.table[0].long()[j // 64], j % 64] = K[0]
+
+
+@pytest.mark.parametrize("typ,n,jump", [("f16", 16, 45), ("f16", 16, 90), ("f16", 2, 140), ("f32", 2, 140)])
+def test_value_before_scores_rise_by_far(cuda, typ, n, jump):
+    """V of an early position is inf and seen by all rows, and a later score takes all the weight: inf times any weight is not
+    finite, whatever became of the early sums meanwhile."""
+    import math
+    import torch
+    import large_model_b200 as m
+    kv, D = 2300, 128
+    pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+    for late in (70, 130, 1100, 2000):
+        s = torch.zeros(kv, device="cuda")
+        s[late] = jump
+        scores(pages, batch, q, K, s)
+        put(pages, batch, 0, 10, 1, 7, float("inf"))
+        out = m.paged_attention(pages, batch, q, 32, scale=math.log(2)).view(n, 2, 16, D)
+        batch.status()
+        assert not torch.isfinite(out[:, 1, :, 7]).any(), late
+        assert torch.isfinite(out[:, 0]).all() and torch.isfinite(out[:, 1, :, 8:]).all(), late
