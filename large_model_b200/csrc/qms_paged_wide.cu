@@ -534,6 +534,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             // additions per tile: of the hi terms while l grows, then of the others
             constexpr float ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
             float w0 = cut_back(MODE != F32, grown, l, ADDS, RISE), w1 = 0.0f;
+            bool none0 = false, none1 = false;    // a stream that saw nothing: its O may be anything
             if (MODE == F32 && nt > 0) w0 *= pow2_bits(254u - vup);
             if constexpr (MODE != PAIR) {
                 // stream 1 leaves its (B, l, scale); stream 0 reads both O (the same TMEM lanes) and writes the rows
@@ -550,6 +551,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 tc_fence_after();
                 const float B1 = s_join[row], l1 = s_join[128 + row], M = fmaxf(B, B1);
                 const float c0 = B == -INFINITY ? 0.0f : ex2(B - M), c1 = B1 == -INFINITY ? 0.0f : ex2(B1 - M);
+                none0 = B == -INFINITY, none1 = B1 == -INFINITY;
                 w1 = c1 * s_join[256 + row];
                 w0 *= c0;
                 l = c0 * l + c1 * l1;
@@ -586,8 +588,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     tmem_ld<32>(o_col + D + 32 * c, o1);
                     tmem_wait_ld(o1);
 #pragma unroll
-                    for (int e = 0; e < 32; e++)  // (a stream that saw nothing: its O may be anything)
-                        o[e] = __float_as_uint((w0 == 0.0f ? 0.0f : __uint_as_float(o[e]) * w0) + (w1 == 0.0f ? 0.0f : __uint_as_float(o1[e]) * w1));
+                    for (int e = 0; e < 32; e++)  // (a factor of 0 does not make inf nothing)
+                        o[e] = __float_as_uint((none0 ? 0.0f : __uint_as_float(o[e]) * w0) + (none1 ? 0.0f : __uint_as_float(o1[e]) * w1));
                 }
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)

@@ -83,7 +83,7 @@ def scores(pages, batch, q, K, s):
     pages.k[batch.table[0].long()[j // 64], j % 64] = K[0]
 
 
-@pytest.mark.parametrize("typ,n,jump", [("f16", 16, 45), ("f16", 16, 90), ("f16", 2, 140), ("f32", 2, 140)])
+@pytest.mark.parametrize("typ,n,jump", [("f16", 16, 45), ("f16", 16, 90), ("f16", 8, 140), ("f32", 8, 140), ("f16", 2, 140), ("f32", 2, 140)])
 def test_value_before_scores_rise_by_far(cuda, typ, n, jump):
     """V of an early position is inf and seen by all rows, and a later score takes all the weight: inf times any weight is not
     finite, whatever became of the early sums meanwhile."""
