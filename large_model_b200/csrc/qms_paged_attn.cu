@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 uint32_t mb = __float_as_uint(mx);
                 if (mx == INFINITY) {
                     mb = 0;
-                    for (int i = 0; i < N; i++) mb = max(mb, finite4(rv[tid + 128 * i]));
+#pragma unroll
+                    for (int i = 0; i < N; i++) mb = max(mb, finite4(x[i]));       // (of what is part of the unit, as above)
                 }
                 mb = __reduce_max_sync(kFull, mb);
                 if (lane == 0) s_max[warp] = mb;

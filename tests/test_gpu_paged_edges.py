@@ -59,6 +59,22 @@ def test_value_behind_a_bad_page(cuda, typ, G, n, kv):
     assert ((out.double() - want).abs() <= tol + want.abs() * 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("G,n,kv,p", [(16, 1, 40, 35), (16, 2, 40, 34), (16, 4, 50, 33), (8, 1, 5, 2), (16, 8, 40, 30)])
+def test_value_beside_what_nobody_sees(cuda, G, n, kv, p):
+    """fp32 cache: V of a seen position is inf in a tile whose other rows, past the sequence, hold large numbers."""
+    import torch
+    import large_model_b200 as m
+    pages, batch, q, K, V = make([n], [kv], typ="f32", G=G, Hk=1, page=64, garbage=1e30)
+    put(pages, batch, 0, p, 0, 7, float("inf"))
+    V[0][p, 0, 7] = 0
+    out = m.paged_attention(pages, batch, q, G).view(n, G, 128)
+    batch.status()
+    want, tol = (x.view(n, G, 128) for x in reference([n], [kv], q, K, V, G, 128 ** -0.5))
+    assert not torch.isfinite(out[..., 7]).any()
+    out[..., 7] = want[..., 7].float()
+    assert ((out.double() - want).abs() <= tol + want.abs() * 2.0 ** -24).all()
+
+
 # ---- the same in every kernel ---------------------------------------------------------------------------
 # (own positions: rows of a tile x positions x sequences; idle sequences count, and make one unit of a sequence's positions)
 
