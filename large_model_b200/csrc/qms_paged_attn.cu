@@ -34,9 +34,15 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from 0.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // ---- the kernel over mma.sync ----------------------------------------------------------------------
 // A CTA of 4 warps takes units of (16 WR rows, one chunk of positions): WR row groups of 16 rows x WK groups of
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         float o[C::DW / 8][4];
 #pragma unroll
         for (int i = 0; i < C::DW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, grown0 = 0.0f, grown1 = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         uint32_t v_exp = 0;                       // fp32: largest exponent of V so far; o is in units of its scale
 
         for (int st = 0; st < nst; st++) {
@@ -436,8 +442,6 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
                 l0 *= d0;
                 l1 *= d1;
-                grown0 *= d0;
-                grown1 *= d1;
 #pragma unroll
                 for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
             }
@@ -450,31 +454,47 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 l0 += s[i][0] + s[i][1];
                 l1 += s[i][2] + s[i][3];
             }
-            grown0 += l0;
-            grown1 += l1;
-            // ---- o += weights * V
+            // ---- o += weights * V. The tensor cores add by cutting bits off, towards 0; so they add up one stage, from 0, and its
+            // sums join o by additions that round to nearest. In us, against sums over a whole unit (off by up to 8e-6): 64 tokens
+            // over 4096 positions fp16 104, 105; 64 on a prompt of 1024 38.7, 37.5; 16 x 4 on 1000 29.8, 28.1; 8 x 4 on 2000 fp32
+            // 42.3, 40.0.
+            uint32_t ph[C::NT / 2][4], pl[C::NT / 2][4];
 #pragma unroll
             for (int kk = 0; kk < C::NT / 2; kk++) {
-                uint32_t ph[4], pl[4];
-                split_h2(s[2 * kk][0], s[2 * kk][1], ph[0], pl[0]);
-                split_h2(s[2 * kk][2], s[2 * kk][3], ph[1], pl[1]);
-                split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[2], pl[2]);
-                split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[3], pl[3]);
+                split_h2(s[2 * kk][0], s[2 * kk][1], ph[kk][0], pl[kk][0]);
+                split_h2(s[2 * kk][2], s[2 * kk][3], ph[kk][1], pl[kk][1]);
+                split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[kk][2], pl[kk][2]);
+                split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[kk][3], pl[kk][3]);
+            }
+            constexpr int JS = C::F16 ? 2 : 1;    // 16-value columns at a time
 #pragma unroll
-                for (int j = 0; j < C::DW / 16; j++) {
-                    const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = wd * (C::DW / 8) + 2 * j + (lane >> 4);
-                    const uint32_t at = vb + C::piece(r, c);
-                    uint32_t vf[4];
-                    ldsm4t(vf, at);
-                    mma_f16(o[2 * j], ph, vf[0], vf[1]);
-                    mma_f16(o[2 * j + 1], ph, vf[2], vf[3]);
-                    mma_f16(o[2 * j], pl, vf[0], vf[1]);
-                    mma_f16(o[2 * j + 1], pl, vf[2], vf[3]);
-                    if constexpr (!C::F16) {
-                        ldsm4t(vf, at + C::HTILE);
-                        mma_f16(o[2 * j], ph, vf[0], vf[1]);
-                        mma_f16(o[2 * j + 1], ph, vf[2], vf[3]);
+            for (int j0 = 0; j0 < C::DW / 16; j0 += JS) {
+                float t[2 * JS][4];
+#pragma unroll
+                for (int kk = 0; kk < C::NT / 2; kk++) {
+                    const int r = wk * C::KW + kk * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), c = wd * (C::DW / 8) + 2 * j0 + (lane >> 4);
+                    uint32_t vf[JS][4];
+#pragma unroll
+                    for (int j = 0; j < JS; j++) ldsm4t(vf[j], vb + C::piece(r, c + 2 * j));
+#pragma unroll
+                    for (int j = 0; j < 2 * JS; j++) {
+                        if (kk == 0) mma_f16_first(t[j], pl[kk], vf[j / 2][j % 2 * 2], vf[j / 2][j % 2 * 2 + 1]);
+                        else mma_f16(t[j], pl[kk], vf[j / 2][j % 2 * 2], vf[j / 2][j % 2 * 2 + 1]);
                     }
+#pragma unroll
+                    for (int j = 0; j < 2 * JS; j++) mma_f16(t[j], ph[kk], vf[j / 2][j % 2 * 2], vf[j / 2][j % 2 * 2 + 1]);
+                    if constexpr (!C::F16) {
+#pragma unroll
+                        for (int j = 0; j < JS; j++) ldsm4t(vf[j], vb + C::piece(r, c + 2 * j) + C::HTILE);
+#pragma unroll
+                        for (int j = 0; j < 2 * JS; j++) mma_f16(t[j], ph[kk], vf[j / 2][j % 2 * 2], vf[j / 2][j % 2 * 2 + 1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2 * JS; j++) {
+                    float(&x)[4] = o[2 * j0 + j];
+                    const float2 lo = f2_add(make_float2(x[0], x[1]), make_float2(t[j][0], t[j][1])), hi = f2_add(make_float2(x[2], x[3]), make_float2(t[j][2], t[j][3]));
+                    x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
                 }
             }
         }
@@ -484,15 +504,11 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         l1 += __shfl_xor_sync(kFull, l1, 1);
         l0 += __shfl_xor_sync(kFull, l0, 2);
         l1 += __shfl_xor_sync(kFull, l1, 2);
-        grown0 += __shfl_xor_sync(kFull, grown0, 1);
-        grown1 += __shfl_xor_sync(kFull, grown1, 1);
-        grown0 += __shfl_xor_sync(kFull, grown0, 2);
-        grown1 += __shfl_xor_sync(kFull, grown1, 2);
-        constexpr float ADDS = C::NT / 2 * (C::F16 ? 2 : 3);       // into o per stage
-        const float d = C::F16 ? 1.0f : pow2_bits(254u - scale_up(v_exp)), back0 = d * cut_back(C::F16, grown0, l0, ADDS, ADDS / 2),
-                    back1 = d * cut_back(C::F16, grown1, l1, ADDS, ADDS / 2);
+        if constexpr (!C::F16) {                  // out of V's scale
+            const float d = pow2_bits(254u - scale_up(v_exp));
 #pragma unroll
-        for (int i = 0; i < C::DW / 8; i++) o[i][0] *= back0, o[i][1] *= back0, o[i][2] *= back1, o[i][3] *= back1;
+            for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
+        }
         // dims of this thread's o[i][0..1] (row g) and o[i][2..3] (row g + 8)
         auto dim = [&](int i, int j) { return wd * C::DW + i * 8 + tq * 2 + (j & 1); };
         if (s_flag) {
@@ -699,14 +715,9 @@ static int row_groups(int type, int page_log, int64_t rows, int64_t positions, b
 static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
 static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : wr == kPaWideF32 ? 64 : 128; }
 
-// Positions that one unit may cover, by the additions into an accumulator (cut_back): fp16 144 of them, 2 per 16 positions; fp32
-// 192, 3 per 16. `share` accumulators have a unit's positions (kPaWidePair takes its own out in time). An output is then
-// within 2.5e-6 of the exact one at any length; unbounded, 1.9e-5 at 9000 positions.
-static int most_positions(int type, int wr) {
-    const bool f16 = type == QMS_T_F16;
-    const int share = wr < 0 ? 2 : f16 ? 4 / wr : wr == 4 ? 1 : 2;
-    return wr == kPaWidePair ? 1 << 30 : (f16 ? 1152 : 1024) * share;
-}
+// Positions that one unit of k_paged_wide may cover, by the additions into an accumulator (cut_back): fp16 144 of them, 2 per 16
+// positions; fp32 192, 3 per 16, by two streams. (kPaWidePair takes its own out in time; k_paged_attn adds up single stages.)
+static int most_positions(int wr) { return wr == kPaWideSplit ? 2304 : wr == kPaWideF32 ? 2048 : 1 << 30; }
 
 // Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
 // of resident CTAs, stages of `stage` positions (us each, us_unit once per unit) and 1 KB of partial results
@@ -726,7 +737,7 @@ static int chunk_of(int len, int64_t tiles, int64_t rows, int stage, int residen
 
 // share: what these units have of the SMs' room beside those of the other kind
 static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, double share) {
-    const int tp = tile_positions(type, wr), most = most_positions(type, wr);
+    const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
     const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
@@ -756,7 +767,7 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
         p.line_tp = tile_positions(type, p.wr_p);
         p.line_rows = tile_rows(p.wr_p);
         const int64_t nt = (a.prefix + p.line_tp - 1) / p.line_tp, line = nt * p.tiles_p * a.Hk;
-        const int64_t ctas = std::min<int64_t>(148, line), most = most_positions(type, p.wr_p) / p.line_tp;
+        const int64_t ctas = std::min<int64_t>(148, line), most = most_positions(p.wr_p) / p.line_tp;
         p.line = (unsigned)line;
         p.line_nt = (unsigned)nt;
         p.line_per = (unsigned)((line + ctas * most - 1) / (ctas * most));

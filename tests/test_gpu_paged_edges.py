@@ -117,3 +117,39 @@ def test_value_before_scores_rise_by_far(cuda, typ, n, jump):
         batch.status()
         assert not torch.isfinite(out[:, 1, :, 7]).any(), late
         assert torch.isfinite(out[:, 0]).all() and torch.isfinite(out[:, 1, :, 8:]).all(), late
+
+
+# ---- sums that are exact -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ,n", [k for k in KERNELS if k[1] < 8])
+@pytest.mark.parametrize("kv", [1000, 2300, 5000, 9000])
+def test_equal_scores_over_equal_values(cuda, typ, n, kv):
+    """The mean of the same number: the sums are exact, and some four roundings of 2^-24 are left."""
+    import torch
+    import large_model_b200 as m
+    for prefix in (0, kv - kv // 4):
+        pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+        batch.desc.prefix_len = prefix
+        j = torch.arange(kv, device="cuda")
+        pages.v[batch.table[0].long()[j // 64], j % 64] = 1.0
+        out = m.paged_attention(pages, batch, q, 32, scale=0.0)
+        batch.status()
+        assert (out - 1).abs().max() <= 1e-6, prefix
+
+
+@pytest.mark.parametrize("typ,n", [k for k in KERNELS if k[1] < 8])
+@pytest.mark.parametrize("top", [30, 40, 60])
+def test_one_position_far_above_the_others(cuda, typ, n, top):
+    """The first position's weight is 2^top of another's, over 1000 to 9000 positions."""
+    import math
+    import torch
+    import large_model_b200 as m
+    for kv in (1000, 9000):
+        pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+        s = torch.zeros(kv, device="cuda")
+        s[0] = top
+        scores(pages, batch, q, K, s)
+        out = m.paged_attention(pages, batch, q, 32, scale=math.log(2))
+        batch.status()
+        want, _ = reference([n], [kv], q, K, V, 16, math.log(2))
+        assert (out.double() - want).abs().max() <= 1e-6 * V[0].abs().max(), kv
