@@ -129,17 +129,6 @@ __device__ __forceinline__ void red4(float *to, const uint32_t *v) {
                  "f"(__uint_as_float(v[2])), "f"(__uint_as_float(v[3]))
                  : "memory");
 }
-// v takes the place of the sums at `to`, and stays not finite where they were
-__device__ __forceinline__ void take_place(float *to, uint4 v, bool earlier) {
-    if (earlier) {
-        const float4 o = __ldcg(reinterpret_cast<const float4 *>(to));
-        v.x = __float_as_uint(fmaf(o.x, 0.0f, __uint_as_float(v.x)));
-        v.y = __float_as_uint(fmaf(o.y, 0.0f, __uint_as_float(v.y)));
-        v.z = __float_as_uint(fmaf(o.z, 0.0f, __uint_as_float(v.z)));
-        v.w = __float_as_uint(fmaf(o.w, 0.0f, __uint_as_float(v.w)));
-    }
-    *reinterpret_cast<uint4 *>(to) = v;
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_tie(uint32_t (&r)[32]) {      // the same for a second array of that wait
@@ -534,7 +523,6 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             // additions per tile: of the hi terms while l grows, then of the others
             constexpr float ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
             float w0 = cut_back(MODE != F32, grown, l, ADDS, RISE), w1 = 0.0f;
-            bool none0 = false, none1 = false;    // a stream that saw nothing: its O may be anything
             if (MODE == F32 && nt > 0) w0 *= pow2_bits(254u - vup);
             if constexpr (MODE != PAIR) {
                 // stream 1 leaves its (B, l, scale); stream 0 reads both O (the same TMEM lanes) and writes the rows
@@ -551,7 +539,6 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 tc_fence_after();
                 const float B1 = s_join[row], l1 = s_join[128 + row], M = fmaxf(B, B1);
                 const float c0 = B == -INFINITY ? 0.0f : ex2(B - M), c1 = B1 == -INFINITY ? 0.0f : ex2(B1 - M);
-                none0 = B == -INFINITY, none1 = B1 == -INFINITY;
                 w1 = c1 * s_join[256 + row];
                 w0 *= c0;
                 l = c0 * l + c1 * l1;
@@ -571,25 +558,34 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 *s_sum = over ? make_float2(B, l + (sum.y == 0.0f ? 0.0f : sum.y * ex2(sum.x - B))) : make_float2(sum.x, fmaf(l, f, sum.y));
                 w0 *= f;
             }
-            const uint32_t fresh = __ballot_sync(kFull, over), earlier = kp > w.kmin ? fresh : 0u;
+            uint32_t fresh = __ballot_sync(kFull, over);
+            if (MODE == PAIR && kp > w.kmin) {    // of earlier sums that lose their place 0 is left, or NaN; the new ones are added to that
+                uint32_t later = __ballot_sync(kFull, over && put);
+                for (fresh &= ~later; later; later &= later - 1) {
+                    float *to = A.part_o + (first + __shfl_sync(kFull, tok, __ffs(later) - 1)) * D + lane;
+#pragma unroll
+                    for (int d = 0; d < D; d += 32) to[d] = __ldcg(to + d) * 0.0f;
+                }
+                __syncwarp();
+            }
+            // (the O of a stream without tiles may be anything: the other's, 0 times)
+            const uint32_t o0_col = nt > 0 ? o_col : o_col + D, o1_col = tiles_of(1, before) > 0 ? o_col + D : o_col;
             // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes; while Q is
             // still wanted, by shuffles
             unsigned char *stage = sm + (MODE == PAIR ? i * 2 * C::QTILE : 0) + (warp & 3) * 4096;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
-                tmem_ld<32>(o_col + 32 * c, o);
+                tmem_ld<32>(o0_col + 32 * c, o);
                 tmem_wait_ld(o);
-                if constexpr (MODE == PAIR) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
-                } else {
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
+                if constexpr (MODE != PAIR) {
                     uint32_t o1[32];
-                    tmem_ld<32>(o_col + D + 32 * c, o1);
+                    tmem_ld<32>(o1_col + 32 * c, o1);
                     tmem_wait_ld(o1);
 #pragma unroll
-                    for (int e = 0; e < 32; e++)  // (a factor of 0 does not make inf nothing)
-                        o[e] = __float_as_uint((none0 ? 0.0f : __uint_as_float(o[e]) * w0) + (none1 ? 0.0f : __uint_as_float(o1[e]) * w1));
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), w1, __uint_as_float(o[e])));
                 }
                 if (fix && put) {
                     // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight)
@@ -615,7 +611,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     for (int k = 0; k < 8; k++) {
                         const int rr = (lane & 24) + k, to = __shfl_sync(kFull, row_out, rr);
                         float *dst = part + (int64_t)to * D + 32 * c;
-                        if (to >= 0 && (fresh >> rr & 1)) take_place(dst, make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]), earlier >> rr & 1);
+                        if (to >= 0 && (fresh >> rr & 1)) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                         else if (to >= 0) red4(dst, o + 4 * k);
                     }
                     continue;
@@ -631,7 +627,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     const int rr = 4 * k + (lane >> 3), to = __shfl_sync(kFull, row_out, rr);
                     const uint4 v = *reinterpret_cast<const uint4 *>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
                     float *dst = part + (int64_t)to * D + 32 * c;
-                    if (to >= 0 && (MODE != PAIR || (fresh >> rr & 1))) take_place(dst, v, MODE == PAIR && (earlier >> rr & 1));
+                    if (to >= 0 && (MODE != PAIR || (fresh >> rr & 1))) *reinterpret_cast<uint4 *>(dst) = v;
                     else if (MODE == PAIR && to >= 0) red4(dst, reinterpret_cast<const uint32_t *>(&v));
                 }
             }
