@@ -123,19 +123,6 @@ __device__ __forceinline__ bool drop_nonfinite(const float *, uint4 &v) {
     return any;
 }
 
-// The tensor cores add into fp32 by cutting bits off, towards 0: an addition into an accumulator takes some
-// kCut of it away on average: 2^-24 E[1 / mantissa] = 0.72 * 2^-24 where the terms have bits behind the sum's last (fp32 caches);
-// products of fp16 values have few (0.6 * 2^-24 measured). A sum o = sum p v grows with
-// l = sum p, so that what N additions took is, for given o, expected at kCut * o * sum over the additions of l then / l at
-// the end: that is given back. What is left, the chance of a cut and o's own way there, goes as 0.3 kCut N; N is bounded
-// where the work is cut up (a sum outside the tensor cores is rounded to nearest).
-constexpr float kCutF32 = 4.3e-8f, kCutF16 = 3.6e-8f;
-// 1 + what is to be given back: `grown` the sum of l after each tile or stage of `adds` additions, `rise` how many of those
-// the last one's l falls short of
-__device__ __forceinline__ float cut_back(bool f16, float grown, float l, float adds, float rise) {
-    return l > 0.0f && l < INFINITY ? fmaf(f16 ? kCutF16 : kCutF32, fmaf(adds, __fdividef(grown, l), -rise), 1.0f) : 1.0f;
-}
-
 // ---- attention: the work and its split ----------------------------------------------------------
 // Two kinds of units, per kv head: the shared positions [0, prefix) against tiles of all token rows, and
 // a sequence's own positions [prefix, kv_len) against tiles of its rows. A row is a (token, q head of the

@@ -715,7 +715,7 @@ static int row_groups(int type, int page_log, int64_t rows, int64_t positions, b
 static int tile_rows(int wr) { return wr == kPaWidePair ? 256 : wr < 0 ? 128 : 16 * wr; }
 static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : wr == kPaWideF32 ? 64 : 128; }
 
-// Positions that one unit of k_paged_wide may cover, by the additions into an accumulator (cut_back): fp16 144 of them, 2 per 16
+// Positions that one unit of k_paged_wide may cover, by the additions into an accumulator (its CUT): fp16 144 of them, 2 per 16
 // positions; fp32 192, 3 per 16, by two streams. (kPaWidePair takes its own out in time; k_paged_attn adds up single stages.)
 static int most_positions(int wr) { return wr == kPaWideSplit ? 2304 : wr == kPaWideF32 ? 2048 : 1 << 30; }
 

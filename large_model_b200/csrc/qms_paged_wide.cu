@@ -64,6 +64,17 @@ struct WideCfg {
     static constexpr uint32_t BAD = STAGE + 2 * STAGED, UP = BAD + 128, JOIN = UP + 64,
                               BARS = JOIN + (MODE == PAIR ? 256 * 8 : 128 * 12), SMEM = BARS + 24 * 8 + 32;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
+    // The tensor cores add into fp32 by cutting bits off, towards 0: an addition takes CUT of the sum away on average, 2^-24
+    // E[1 / mantissa] = 0.72 * 2^-24 where the terms have bits behind the sum's last (fp32 caches); products of fp16 values
+    // have few (0.6 * 2^-24 measured). A sum o = sum p v grows with l = sum p, so that what a tile's ADDS additions take of o is,
+    // for given o, expected at ADDS * CUT * o * (l then) / (l at the end), and at half the tile's own weights at most: that is given
+    // back at the end. (RISE: while l grows within a tile, of the hi terms.) Nothing is given back where nothing was cut: where l
+    // has so few bits that all weights are alike (fp16 values add up exactly then; of fp32 values those whose o has few bits too).
+    // What is left, of an output: 1 to 2e-6 for values of either sign, as a plain fp32 softmax. Values of one sign lose up to 1.1e-5
+    // (PAIR, SPLIT) or 1.4e-5 (F32) more than is given back, since every product is cut at the sum's last bits by itself; a row
+    // whose first weight is 2^14 to 2^26 times each other one is up to 5e-6 too large. Half the additions per sum would leave half
+    // of that, for 1.12 times the time (F32: 1.19).
+    static constexpr float CUT = MODE == F32 ? 4.3e-8f : 3.6e-8f, ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
     // Load n of a ring (K, V, K, ...): its slot. One ring for both streams; in SPLIT a ring per stream.
     static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return MODE == SPLIT ? 2 * stream + (n & 1) : n % 3; }
     static constexpr uint32_t RINGLEN = MODE == SPLIT ? 2 : 3;
@@ -388,7 +399,6 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
 
             const int lim = min(pos, w.k1 - 1);   // last position that this row sees
-            float grown = 0.0f;                   // sum over the tiles of l after each
             uint32_t vup = 0;                     // F32: the scale of V that O is in
             // O times a power of 2 (the MMAs on it ended before the S at hand was announced)
             auto scale_o = [&](float fac) {
@@ -405,8 +415,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             // O adds up the tiles from position kp on, up to tile n1
             int n = 0, n1 = min(nt, C::PIECE), kp = w.kmin;
             if (MODE == PAIR) *s_sum = make_float2(-INFINITY, 0.0f);
-            float B = -INFINITY;
-            float2 l2 = make_float2(0.0f, 0.0f);
+            float B = -INFINITY, l = 0.0f, cut = 0.0f;
         next_part:                                // (as a loop around all this, 1 us more per call)
             for (; n < n1; n++) {
                 const int j = MODE == PAIR ? n : 2 * n + first_of(i, before), base = w.k0 + j * C::TP;
@@ -439,6 +448,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 // what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
                 const float fk = MODE == F32 ? fmaxf(f * pow2_bits(254u - s_up[(before + j) & 3]), 1.17549435e-38f) : f;
                 const float2 f2 = make_float2(fk, fk);
+                float S = 0.0f;                   // the tile's weights
                 auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {
                     float mx = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
 #pragma unroll
@@ -448,9 +458,9 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     if (__any_sync(kFull, mx > B + kWHigh)) {
                         const float nb = mx > B + kWHigh ? ceilf(mx) - kWLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
                         B = nb;
-                        l2.x *= fac;
-                        l2.y *= fac;
-                        grown *= fac;
+                        S *= fac;
+                        l *= fac;
+                        cut *= fac;
                         if (n > 0 && (MODE != PAIR || base > kp)) scale_o(fac);
                         const __half2 fh = __float2half2_rn(fac);
 #pragma unroll 1
@@ -470,6 +480,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     }
                     const float2 nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
                     uint32_t o[32];
+                    float2 l2 = make_float2(0.0f, 0.0f);             // (sums of 16: a weight far above the others hides few)
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         const float2 q = f2_fma(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), f2, nB);
@@ -481,6 +492,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         o[16 + e / 2] = pack_h2(lo.x, lo.y);
                     }
                     tmem_st32(s_col + 32 * c, o);
+                    S += l2.x + l2.y;
                 };
                 uint32_t x[32], y[32];
                 tmem_ld<32>(s_col, x);
@@ -503,11 +515,13 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     if (up != vup && n > 0) scale_o(vup - up > 126 ? 0.0f : pow2_bits(127u - (vup - up)));
                     vup = up;
                 }
-                grown += l2.x + l2.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[i]);
+                const float sum = l + S;          // (and what rounding takes of l itself)
+                cut += fminf(C::ADDS * C::CUT * sum, 0.5f * S) - (S - (sum - l));
+                l = sum;
             }
             if (!ok) break;
             // O is complete (no tiles at all: not before the last unit is read)
@@ -518,11 +532,10 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             } else if (!(ok = __all_sync(kFull, sy.wait(&q_full[0], unit_no & 1)))) {
                 break;
             }
-            float l = l2.x + l2.y;
             if (isnan(l) && B == -INFINITY) B = 0.0f;
-            // additions per tile: of the hi terms while l grows, then of the others
-            constexpr float ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
-            float w0 = cut_back(MODE != F32, grown, l, ADDS, RISE), w1 = 0.0f;
+            auto alike = [](float x) { return (__float_as_uint(x) & 0xfffu) == 0; };
+            float w0 = l > 0.0f && l < INFINITY && (MODE == F32 || !alike(l)) ? 1.0f + fmaxf(__fdividef(cut, l) - C::RISE * C::CUT, 0.0f) : 1.0f, w1 = 0.0f;
+            float even0 = 1.0f, even1 = 1.0f;     // F32: what undoes the giving back, for streams whose weights are all alike
             if (MODE == F32 && nt > 0) w0 *= pow2_bits(254u - vup);
             if constexpr (MODE != PAIR) {
                 // stream 1 leaves its (B, l, scale); stream 0 reads both O (the same TMEM lanes) and writes the rows
@@ -539,7 +552,10 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 tc_fence_after();
                 const float B1 = s_join[row], l1 = s_join[128 + row], M = fmaxf(B, B1);
                 const float c0 = B == -INFINITY ? 0.0f : ex2(B - M), c1 = B1 == -INFINITY ? 0.0f : ex2(B1 - M);
-                w1 = c1 * s_join[256 + row];
+                auto undo = [&](float x, float w) { return alike(x) && x > 0.0f ? __fdividef(__uint_as_float(__float_as_uint(w) & 0x7f800000u), w) : 1.0f; };
+                w1 = s_join[256 + row];
+                if (MODE == F32) even0 = undo(l, w0), even1 = undo(l1, w1);
+                w1 *= c1;
                 w0 *= c0;
                 l = c0 * l + c1 * l1;
                 B = M;
@@ -568,6 +584,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 }
                 __syncwarp();
             }
+            const bool any_even = MODE == F32 && __any_sync(kFull, even0 != 1.0f || even1 != 1.0f);
+            auto uncut = [](uint32_t (&o)[32], float f) {     // o's sums of few bits
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                    if ((o[e] & 0xffu) == 0) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            };
             // (the O of a stream without tiles may be anything: the other's, 0 times)
             const uint32_t o0_col = nt > 0 ? o_col : o_col + D, o1_col = tiles_of(1, before) > 0 ? o_col + D : o_col;
             // the rows leave by way of shared memory (where this warp's rows of Q are), 128 bytes of a row per 8 lanes; while Q is
@@ -578,12 +600,14 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 uint32_t o[32];
                 tmem_ld<32>(o0_col + 32 * c, o);
                 tmem_wait_ld(o);
+                if (any_even) uncut(o, even0);
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
                 if constexpr (MODE != PAIR) {
                     uint32_t o1[32];
                     tmem_ld<32>(o1_col + 32 * c, o1);
                     tmem_wait_ld(o1);
+                    if (any_even) uncut(o1, even1);
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), w1, __uint_as_float(o[e])));
                 }
@@ -642,8 +666,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 kp = w.k0 + n * C::TP;
                 n1 = min(nt, n + C::PIECE);
                 B = -INFINITY;
-                l2 = make_float2(0.0f, 0.0f);
-                grown = 0.0f;
+                l = cut = 0.0f;
                 goto next_part;
             }
         }

@@ -121,7 +121,7 @@ def test_value_before_scores_rise_by_far(cuda, typ, n, jump):
 
 # ---- sums that are exact -------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("typ,n", [k for k in KERNELS if k[1] < 8])
+@pytest.mark.parametrize("typ,n", KERNELS)
 @pytest.mark.parametrize("kv", [1000, 2300, 5000, 9000])
 def test_equal_scores_over_equal_values(cuda, typ, n, kv):
     """The mean of the same number: the sums are exact, and some four roundings of 2^-24 are left."""
@@ -137,7 +137,7 @@ def test_equal_scores_over_equal_values(cuda, typ, n, kv):
         assert (out - 1).abs().max() <= 1e-6, prefix
 
 
-@pytest.mark.parametrize("typ,n", [k for k in KERNELS if k[1] < 8])
+@pytest.mark.parametrize("typ,n", KERNELS)
 @pytest.mark.parametrize("top", [30, 40, 60])
 def test_one_position_far_above_the_others(cuda, typ, n, top):
     """The first position's weight is 2^top of another's, over 1000 to 9000 positions."""
