@@ -462,7 +462,6 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         l *= fac;
                         cut *= fac;
                         if (n > 0 && (MODE != PAIR || base > kp)) scale_o(fac);
-                        const __half2 fh = __float2half2_rn(fac);
 #pragma unroll 1
                         for (int k = 0; k < 4; k++) {
                             if (!(done >> k & 1)) continue;
@@ -471,9 +470,11 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                             tmem_ld<32>(s_col + 32 * k, o);
                             tmem_wait_ld(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                const __half2 p2 = __hmul2(*reinterpret_cast<const __half2 *>(&o[e]), fh);
-                                o[e] = *reinterpret_cast<const uint32_t *>(&p2);
+                            for (int e = 0; e < 16; e++) {           // (in fp32: in fp16 a factor below 2^-24 is 0, and 2^15 times it is not)
+                                const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&o[e]));
+                                const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&o[16 + e]));
+                                const float2 y = f2_mul(f2_add(h, lo), make_float2(fac, fac));
+                                split_h2(y.x, y.y, o[e], o[16 + e]);
                             }
                             tmem_st32(s_col + 32 * k, o);
                         }

@@ -119,6 +119,27 @@ def test_value_before_scores_rise_by_far(cuda, typ, n, jump):
         assert torch.isfinite(out[:, 0]).all() and torch.isfinite(out[:, 1, :, 8:]).all(), late
 
 
+@pytest.mark.parametrize("typ,n", [k for k in KERNELS if k[1] >= 8])
+@pytest.mark.parametrize("up", [20, 25, 30])
+def test_scores_that_jump_inside_a_tile(cuda, typ, n, up):
+    """A tile of scores 6 above those before it, and at its end one far above: the 6s keep their share, 2^(6 - up) each of the
+    row. Scores are exact, so a weight is off by its own roundings, some 25 * 2^-24 for the exponent: 4e-6 of max |V|."""
+    import math
+    import torch
+    import large_model_b200 as m
+    kv, TP = 1152, 128 if typ == "f16" else 64
+    pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+    for tile in (2, 3, 8):
+        s = torch.zeros(kv, device="cuda")
+        s[tile * TP:(tile + 1) * TP - 32] = 6
+        s[(tile + 1) * TP - 5] = up
+        scores(pages, batch, q, K, s)
+        out = m.paged_attention(pages, batch, q, 32, scale=math.log(2))
+        batch.status()
+        want, _ = reference([n], [kv], q, K, V, 16, math.log(2))
+        assert (out.double() - want).abs().max() <= 4e-6 * V[0].abs().max(), tile
+
+
 # ---- sums that are exact -------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("typ,n", KERNELS)
