@@ -235,9 +235,9 @@ typedef struct {
  * arithmetic of the whole model's own cache, value for value). qkv: fp32 [n_tok] rows of ldqkv: n_head
  * q heads, n_head_kv k heads, n_head_kv v heads of head_dim, as the projections leave them; q_norm,
  * k_norm: fp32 [head_dim]; rope_cos / rope_sin: fp32 [n_rope][head_dim / 2]. q receives the normalised and
- * rotated q heads (rows of ldq; may be qkv itself), K and V go to the pages. Padding rows are left
- * alone; a row whose position is negative, at or past n_rope, or on a bad page sets *err and
- * writes nothing. */
+ * rotated q heads (rows of ldq; may be qkv itself with ldq = ldqkv, but overlaps it in no other way),
+ * K and V go to the pages. Padding rows are left alone; a row whose position is negative, at or past
+ * n_rope, or on a bad page sets *err and writes nothing. */
 int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *qkv, int64_t ldqkv,
                           int n_head, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
                           const float *rope_sin, int n_rope, float *q, int64_t ldq, int *err, void *stream);

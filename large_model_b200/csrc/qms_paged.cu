@@ -194,6 +194,8 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
     const int D = pages->head_dim;
     if ((rc = paged_rows("paged_append", "qkv", qkv, ldqkv, (int64_t)(n_head + 2 * a.Hk) * D))) return rc;
     if ((rc = paged_rows("paged_append", "q", q, ldq, (int64_t)n_head * D))) return rc;
+    QMS_REQUIRE(q != qkv || ldq == ldqkv || a.n_tok == 1, QMS_CUDA_EINVAL,
+                "paged_append: in place, q and qkv need rows at one distance (%lld, %lld)", (long long)ldq, (long long)ldqkv);
     QMS_REQUIRE(q_norm && k_norm && rope_cos && rope_sin && n_rope > 0, QMS_CUDA_EINVAL,
                 "paged_append: NULL norm weights or rotation tables");
 #define QMS_APPEND(D_, KT) \
