@@ -443,6 +443,20 @@ def _raw_stream(stream, t) -> int:
     return get(t.get_device()) if get else torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _on_stream(raw: int, device):
+    """That stream as torch's current one: what is allocated under it is reused in its order."""
+    torch = _torch()
+    return torch.cuda.stream(torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device))
+
+
+def _empty(shape: tuple, dtype, device, stream):
+    """A result of a call on that stream (None: the current one)."""
+    if stream is None:
+        return _torch().empty(shape, dtype=dtype, device=device)
+    with _on_stream(stream.cuda_stream, device):
+        return _torch().empty(shape, dtype=dtype, device=device)
+
+
 class KvPages:
     """A pool of KV cache pages (QmsCudaPages): k, v CUDA tensors [n_pages][page_size][n_head_kv][head_dim] of
     one shape, type (float32 or float16) and strides, the last dimension contiguous. Another order in
@@ -478,7 +492,8 @@ class PagedBatch:
     """New tokens of a batch of sequences over a paged cache (QmsCudaPagedBatch): q_start CUDA int32 [n_seq + 1],
     kv_len int32 [n_seq], table int32 [n_seq][pages]; n_tok token rows; max_q / max_kv bound a sequence's
     rows and positions. The tensors may be rewritten in place between calls (and between replays of a
-    captured graph); the bounds may not be exceeded. Device-side errors collect in `err`."""
+    captured graph); the bounds may not be exceeded. Device-side errors collect in `err`. Calls may be on any stream; `err`
+    and the workspaces are the object's own business, the order of the other tensors the caller's."""
 
     def __init__(self, q_start, kv_len, table, n_tok: int, max_q: int, max_kv: int, prefix_len: int = 0):
         torch = _torch()
@@ -487,30 +502,53 @@ class PagedBatch:
         self.n_tok = int(n_tok)
         self.err = torch.zeros((1,), dtype=torch.int32, device=kv_len.device)
         self._err = self.err.data_ptr()
+        self._cleared()
         self.desc = PagedBatchDesc(n, self.n_tok, _ints(q_start, (n + 1,), "q_start"), _ints(kv_len, (n,), "kv_len"),
                                    _ints(table, (n, table.shape[1]), "table"), table.shape[1], int(max_q), int(max_kv),
                                    int(prefix_len))
         self._ref = C.byref(self.desc)
         self._ws = {}
 
+    def _cleared(self):
+        """`err` is set to zero in the order of the current stream; other streams wait for that once (_use)."""
+        self._made = _torch().cuda.current_stream(self.err.device)
+        self._ready = {self._made.cuda_stream}
+
+    def _use(self, stream, t) -> int:
+        """The raw stream of a call, on which `err` may be used."""
+        raw = _raw_stream(stream, t)
+        if raw not in self._ready:
+            torch = _torch()
+            with _on_stream(raw, self.err.device):
+                if not torch.cuda.is_current_stream_capturing():     # (torch waits for the device before a capture)
+                    s = torch.cuda.current_stream(self.err.device)
+                    s.wait_stream(self._made)
+                    self.err.record_stream(s)
+                    self._ready.add(raw)
+        return raw
+
     def status(self):
-        """Raise if a device-side check refused work since the last call (waits for the device)."""
+        """Raise if a device-side check refused work since the last call (waits for the device, all streams)."""
+        _torch().cuda.synchronize(self.err.device)
         e = int(self.err.item())
         if e:
             self.err.zero_()
+            self._cleared()
             raise QmsCudaError(ETIMEOUT if e & 16 else EINVAL, f"paged batch: device-side errors 0x{e:x} (1 = lengths or "
                                "positions, 2 = page id, 4 = drafted id, 8 = no probability, 16 = a wait gave up)")
 
-    def workspace(self, pages: KvPages, n_head: int):
-        """The attention's workspace for these sizes, allocated on first use and kept: (address, bytes).
-        Calls that overlap on the GPU (on several streams) need a batch object each."""
-        key = (pages._key, n_head)
+    def workspace(self, pages: KvPages, n_head: int, stream: int | None = None):
+        """The attention's workspace for these sizes on a (raw) stream, allocated on first use and kept: (address, bytes).
+        Captured graphs that overlap on the GPU need a batch object each."""
+        raw = _raw_stream(None, pages.k) if stream is None else stream
+        key = (pages._key, n_head, raw)
         if key not in self._ws:
             torch = _torch()
             n = lib().qms_cuda_paged_attention_ws(pages._ref, self._ref, n_head)
             if n < 0:
                 check(n)
-            w = torch.empty((n + 256,), dtype=torch.uint8, device=pages.k.device)
+            with _on_stream(raw, pages.k.device):
+                w = torch.empty((n + 256,), dtype=torch.uint8, device=pages.k.device)
             self._ws[key] = (w, (w.data_ptr() + 255) // 256 * 256, n)
         return self._ws[key][1:]
 
@@ -529,7 +567,7 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     [n_tok][n_head * head_dim]."""
     D = pages.head_dim
     if q is None:
-        q = _torch().empty((batch.n_tok, n_head * D), dtype=_torch().float32, device=qkv.device)
+        q = _empty((batch.n_tok, n_head * D), _torch().float32, qkv.device, stream)
     x, n, ldx = _rows(qkv, (n_head + 2 * pages.n_head_kv) * D, "qkv")
     y, ny, ldy = _rows(q, n_head * D, "q")
     cos, sin = rope
@@ -538,7 +576,7 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
         raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens")
     rc = lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
                                      eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy,
-                                     batch._err, _raw_stream(stream, qkv))
+                                     batch._err, batch._use(stream, qkv))
     if rc:
         check(rc)
     return q
@@ -549,14 +587,15 @@ def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: fl
     [n_tok][n_head * head_dim]; scale defaults to 1 / sqrt(head_dim). Returns [n_tok][n_head * head_dim]."""
     D = pages.head_dim
     if out is None:
-        out = _torch().empty((batch.n_tok, n_head * D), dtype=_torch().float32, device=q.device)
+        out = _empty((batch.n_tok, n_head * D), _torch().float32, q.device, stream)
     x, n, ldx = _rows(q, n_head * D, "q")
     y, ny, ldy = _rows(out, n_head * D, "out")
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_attention: {n} q and {ny} out rows for {batch.n_tok} tokens")
-    ws, nb = batch.workspace(pages, n_head)
+    raw = batch._use(stream, q)
+    ws, nb = batch.workspace(pages, n_head, raw)
     rc = lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
-                                        ws, nb, batch._err, _raw_stream(stream, q))
+                                        ws, nb, batch._err, raw)
     if rc:
         check(rc)
     return out
@@ -566,7 +605,7 @@ def probs(logits, temp: float, out=None, stream=None):
     """Probabilities of rows of logits (CUDA float32 [rows][vocab]) at a temperature (qms_cuda_probs); temp <= 0:
     1 at the first maximum. out may be logits."""
     if out is None:
-        out = _torch().empty(logits.shape, dtype=_torch().float32, device=logits.device)
+        out = _empty(logits.shape, _torch().float32, logits.device, stream)
     V = logits.shape[-1]
     x, n, ldx = _rows(logits, V, "logits")
     y, ny, ldy = _rows(out, V, "out")
@@ -586,9 +625,9 @@ def verify(p, draft, u, q=None, n_draft=None, row_start=None, n_accept=None, tok
     B, N = draft.shape
     V = p.shape[-1]
     if n_accept is None:
-        n_accept = torch.empty((B,), dtype=torch.int32, device=p.device)
+        n_accept = _empty((B,), torch.int32, p.device, stream)
     if tokens is None:
-        tokens = torch.empty((B, N + 1), dtype=torch.int32, device=p.device)
+        tokens = _empty((B, N + 1), torch.int32, p.device, stream)
     x, n, ldx = _rows(p, V, "p")
     y, ny, ldy = (None, B * N, V) if q is None else _rows(q, V, "q")
     if ny != B * N:
