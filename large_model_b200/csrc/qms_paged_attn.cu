@@ -273,16 +273,20 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         uint32_t v_exp = 0;                       // fp32: largest exponent of V so far; o is in units of its scale
 
+        bool gave_up = false;
         for (int st = 0; st < nst; st++) {
             const uint32_t c = c0 + st;
             for (uint32_t n = 0; !mbar_try_wait(&s_full[c % C::NS], c / C::NS & 1) && !s_abort; n++) {
-                if (n == kPaSpin) {               // reported; the unit's result is not valid
-                    s_abort = 1;
-                    paged_err(a, QMS_PAGED_ETIMEOUT);
-                }
+                if (n == kPaSpin) s_abort = 1;
                 if (n > 64) __nanosleep(32);
             }
             __syncthreads();                      // the stage has landed; the slot before it is free
+            if (s_abort) {                        // reported; the CTA's results are not valid. Its copies have 0.1 s to land before its memory goes.
+                if (tid == 0) paged_err(a, QMS_PAGED_ETIMEOUT);
+                for (int n = 0; n < 1 << 20; n++) __nanosleep(100);
+                gave_up = true;
+                break;
+            }
             const int base = k0 + st * C::PS;
             if (st + C::NS - 1 < nst) {
                 load(st + C::NS - 1);
@@ -498,6 +502,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 }
             }
         }
+        if (gave_up) break;
         c0 += nst;
         __syncthreads();                          // every warp is done with the stages
         l0 += __shfl_xor_sync(kFull, l0, 1);

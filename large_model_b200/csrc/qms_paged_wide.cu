@@ -671,6 +671,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 goto next_part;
             }
         }
+        tmem_wait_st();
     } else if (warp == C::TMA_WARP || (MODE != F32 && warp == 9)) {
         // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. One warp
         // issues them; V tiles with rows that not every row sees (or that were not loaded) land on a barrier of their
@@ -918,16 +919,16 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 }
                 c = c1;
             }
-            if (!ok) {                                          // nothing of this CTA's is in flight when TMEM goes
-                umma_commit(drain);
-                *s_abort = 1;
-                for (uint32_t n = 0; n < kWSpin && !mbar_try_wait(drain, 0); n++) __nanosleep(32);
-            }
+            if (!ok) *s_abort = 1;
+            umma_commit(drain);                                 // nothing of this CTA's is in flight when TMEM goes
+            for (uint32_t n = 0; n < kWSpin && !mbar_try_wait(drain, 0); n++) __nanosleep(32);
         }
         __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
+    if (*s_abort)                                 // copies in flight have 0.1 s to land before the CTA's memory goes
+        for (int n = 0; n < 1 << 20; n++) __nanosleep(100);
     if (warp == C::MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
