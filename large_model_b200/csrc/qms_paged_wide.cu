@@ -350,7 +350,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
                     mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
                     const uint32_t up = scale_up(__float_as_uint(mx) >> 23);
-                    const float got = __shfl_sync(kFull, fabsf(A.scale2) * pow2_bits(254u - up), (lane & 3) * 8);
+                    const float got = __shfl_sync(kFull, (MODE == F32 ? 1.0f : fabsf(A.scale2)) * pow2_bits(254u - up), (lane & 3) * 8);
                     if (lane >> 2 == g0 + g) f = got;
                     if (MODE != PAIR && i == 1) continue;
                     const float m = __uint_as_float(up << 23 | sign);
@@ -446,7 +446,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 // scores of 32 positions in z become weights, hi terms in the first 16 columns, lo in the next 16. The
                 // base of the weights is a whole number and stays, unless a score lies 2^kWHigh above it: then
                 // what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
-                const float fk = MODE == F32 ? fmaxf(f * pow2_bits(254u - s_up[(before + j) & 3]), 1.17549435e-38f) : f;
+                // (F32: the powers of 2 of q and K first: small q may meet large K)
+                const float fk = MODE == F32 ? fmaxf(fabsf(A.scale2) * (f * pow2_bits(254u - s_up[(before + j) & 3])), 1.17549435e-38f) : f;
                 const float2 f2 = make_float2(fk, fk);
                 float S = 0.0f;                   // the tile's weights
                 auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {

@@ -174,3 +174,22 @@ def test_one_position_far_above_the_others(cuda, typ, n, top):
         batch.status()
         want, _ = reference([n], [kv], q, K, V, 16, math.log(2))
         assert (out.double() - want).abs().max() <= 1e-6 * V[0].abs().max(), kv
+
+
+# ---- orders of magnitude -------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [1, 2, 4, 8])
+def test_small_q_and_large_k(cuda, n):
+    """fp32: q near the smallest normal numbers, K so large that the scores are ordinary."""
+    import torch
+    import large_model_b200 as m
+    kv = 700
+    pages, batch, q, K, V = one_unit(n, kv, typ="f32")
+    q *= 2.0 ** -120
+    K[0] *= 2.0 ** 120
+    j = torch.arange(kv, device="cuda")
+    pages.k[batch.table[0].long()[j // 64], j % 64] = K[0]
+    out = m.paged_attention(pages, batch, q, 32)
+    batch.status()
+    want, tol = reference([n], [kv], q, K, V, 16, 128 ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
