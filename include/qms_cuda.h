@@ -221,8 +221,9 @@ typedef struct {
  * Rows past q_start[n_seq] are padding. The first prefix_len positions are the same in every
  * sequence and are read through table row 0 (0: nothing is shared); they may end inside a page, of
  * which each sequence then has its own copy. max_q and max_kv bound the rows and positions of a
- * sequence (they size grids and workspaces; a sequence beyond them sets QMS_PAGED_ELEN and is
- * treated as idle); max_kv <= table_stride * page_size. Pointers: device int. */
+ * sequence (they size grids and workspaces; a sequence beyond them sets QMS_PAGED_ELEN and is treated as
+ * idle; the append looks at those with rows, the attention at all); max_kv <= table_stride * page_size.
+ * Pointers: device int. */
 typedef struct {
     int n_seq, n_tok;              /* n_tok: token rows of the call, padding included */
     const int *q_start;            /* [n_seq + 1], ascending */

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         if (own) {
             b = u % a.n_seq;
             slot = u / a.n_seq;
-            if (!paged_seq(a, b, t0, n, kv) && tid == 0 && slot == 0 && tile == 0 && kh == 0) paged_err(a, QMS_PAGED_ELEN);
+            paged_seq(a, b, t0, n, kv);
             k0 = A.p.base_s + slot * A.p.chunk_s;
             k1 = min(kv, k0 + A.p.chunk_s);
             if (max(k0, a.prefix) >= k1 || tile * 16 * WR >= n * a.G) continue;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             for (int t = first + warp; t < end; t += 4) {
                 int s0 = 0, sn = 0, skv = 0;
                 const int sb = paged_seq_of(a, t);
-                if (sb < a.n_seq && !paged_seq(a, sb, s0, sn, skv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
+                if (sb < a.n_seq) paged_seq(a, sb, s0, sn, skv);
                 const int pos = t >= s0 && t < s0 + sn ? skv - sn + (t - s0) : -1;
                 for (int j = lane; j < a.G; j += 32) {
                     const int r = t * a.G + j - r0;
@@ -613,6 +613,12 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
     pdl_trigger();
     pdl_wait();
     const bool there = row < rows;
+    // the batch arrays, checked once for all kernels (rows or not: a sequence without any counts too)
+    if (blockIdx.x == gridDim.x - 1)
+        for (int b = threadIdx.x; b < a.n_seq; b += 256) {
+            int t0, n, kv;
+            if (!paged_seq(a, b, t0, n, kv)) paged_err(a, QMS_PAGED_ELEN);
+        }
     // slot s of the row in the order of its use is at `at`; np: how many are of the shared positions
     int np = 0;
     auto at = [&](int s) { return (s < np ? s : s - np + A.p.slots_p) * rows + row; };
@@ -633,7 +639,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
             if (sub + WPR * i < slots) fetch((sub + WPR * i) * rows + row, v[i]);
         int t0 = 0, n = 0, kv = 0;
         const int b = paged_seq_of(a, t);
-        if (b < a.n_seq && !paged_seq(a, b, t0, n, kv) && lane == 0) paged_err(a, QMS_PAGED_ELEN);
+        if (b < a.n_seq) paged_seq(a, b, t0, n, kv);
         const int pos = (int)t >= t0 && (int)t < t0 + n ? kv - n + ((int)t - t0) : -1;
         if (pos >= 0) {                           // the slots of chunks that begin past the row's position are not written
             if (a.prefix > 0) {

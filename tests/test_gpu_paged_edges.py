@@ -193,3 +193,21 @@ def test_small_q_and_large_k(cuda, n):
     batch.status()
     want, tol = reference([n], [kv], q, K, V, 16, 128 ** -0.5)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+# ---- lengths -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ,n", KERNELS)
+def test_lengths_of_idle_sequences_are_checked(cuda, typ, n):
+    """A sequence without rows whose length is past max_kv, or negative: reported, whichever kernel runs."""
+    import torch
+    import large_model_b200 as m
+    pages, batch, q, K, V = one_unit(n, 700, typ=typ)
+    good = m.paged_attention(pages, batch, q, 32)
+    batch.status()
+    for value in (701, -1):
+        batch.kv_len[69] = value
+        out = m.paged_attention(pages, batch, q, 32)
+        with pytest.raises(m.QmsCudaError, match="0x1"):
+            batch.status()
+        assert torch.equal(out, good)
