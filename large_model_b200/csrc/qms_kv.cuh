@@ -2,6 +2,8 @@
 // and the paged ones (qms_paged*.cu): cache elements, asynchronous copies, QK-norm + rotation of a row.
 #pragma once
 
+#include <atomic>
+
 #include "qms_async.cuh"
 #include "qms_common.cuh"
 
@@ -18,6 +20,18 @@ __device__ __forceinline__ double warp_max_d(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kFull, v, o));
     return v;
+}
+
+// That much dynamic shared memory for a kernel, once per device (a bit of `done` each). Any number of threads may call.
+template <typename K>
+inline int allow_smem(std::atomic<unsigned long long> &done, K *kern, int bytes) {
+    int dev = 0;
+    QMS_CK(cudaGetDevice(&dev));
+    if (!(done.load() >> (dev & 63) & 1)) {
+        QMS_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(1ull << (dev & 63));
+    }
+    return QMS_CUDA_OK;
 }
 
 // KV cache elements: fp32 (the reference's cache, src/model.c:459-460) or fp16 (compacted: each K / V

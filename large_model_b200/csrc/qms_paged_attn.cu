@@ -800,13 +800,14 @@ int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
 int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map) {
     typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static Encode encode = nullptr;
+    static std::atomic<Encode> known{nullptr};
+    Encode encode = known.load();
     if (!encode) {
         cudaDriverEntryPointQueryResult found;
         void *f = nullptr;
         QMS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
         QMS_REQUIRE(f, QMS_CUDA_ECUDA, "paged_attention: the driver has no cuTensorMapEncodeTiled");
-        encode = (Encode)f;
+        known = encode = (Encode)f;
     }
     const cuuint64_t ps = 1ull << a.page_log, row = (cuuint64_t)D * (f16 ? 2 : 4);
     const cuuint64_t dim[4] = {(cuuint64_t)D, (cuuint64_t)a.Hk, ps, (cuuint64_t)a.n_pages};
@@ -826,15 +827,11 @@ static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t 
     using C = PaCfg<D, KT, WR>;
     const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.chunks_p * A.p.tiles_p * A.a.Hk;
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
-    static unsigned long long set = 0;                          // per device
-    int dev = 0;
-    QMS_CK(cudaGetDevice(&dev));
-    if (!(set >> (dev & 63) & 1)) {
-        QMS_CK(cudaFuncSetAttribute(k_paged_attn<D, KT, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-        set |= 1ull << (dev & 63);
-    }
+    static std::atomic<unsigned long long> done{0};
+    int rc = allow_smem(done, k_paged_attn<D, KT, WR>, C::SMEM);
+    if (rc) return rc;
     CUtensorMap mk, mv;
-    int rc = paged_map(A.a, D, C::F16, C::PS, A.a.k, &mk);
+    rc = paged_map(A.a, D, C::F16, C::PS, A.a.k, &mk);
     if (rc || (rc = paged_map(A.a, D, C::F16, C::PS, A.a.v, &mv))) return rc;
     const int grid = (int)std::min<int64_t>(units, 148 * 8);
     QMS_CK(launch_pdl(k_paged_attn<D, KT, WR>, dim3(grid), dim3(128), C::SMEM, s, A, mk, mv, own, last));

@@ -943,15 +943,11 @@ static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) 
     static_assert(C::SMEM <= 232448, "shared memory per CTA");
     const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)(A.p.line_runs / A.p.line_per);
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
-    static unsigned long long set = 0;                          // per device
-    int dev = 0;
-    QMS_CK(cudaGetDevice(&dev));
-    if (!(set >> (dev & 63) & 1)) {
-        QMS_CK(cudaFuncSetAttribute(k_paged_wide<D, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-        set |= 1ull << (dev & 63);
-    }
+    static std::atomic<unsigned long long> done{0};
+    int rc = allow_smem(done, k_paged_wide<D, MODE>, C::SMEM);
+    if (rc) return rc;
     CUtensorMap mk, mv;
-    int rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.k, &mk);
+    rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.k, &mk);
     if (rc || (rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.v, &mv))) return rc;
     const int grid = (int)(units < 148 ? units : 148);
     QMS_CK(launch_pdl(k_paged_wide<D, MODE>, dim3(grid), dim3(C::THREADS), C::SMEM, s, A, mk, mv, own, last));

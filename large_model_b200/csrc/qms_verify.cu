@@ -404,14 +404,9 @@ static int row_ctas(int rows, int V, int sms) {
 }
 
 static int launch_probs(const float *l, int64_t ldl, int rows, int V, float temp, float *p, int64_t ldp, cudaStream_t s) {
-    static unsigned long long set = 0;                     // per device
-    int dev = 0;
-    QMS_CK(cudaGetDevice(&dev));
-    if (!(set >> (dev & 63) & 1)) {
-        QMS_CK(cudaFuncSetAttribute(k_probs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsKeep * 4));
-        QMS_CK(cudaFuncSetAttribute(k_probs<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsKeep * 4));
-        set |= 1ull << (dev & 63);
-    }
+    static std::atomic<unsigned long long> done[2];
+    int rc = allow_smem(done[0], k_probs<true>, kProbsKeep * 4);
+    if (rc || (rc = allow_smem(done[1], k_probs<false>, kProbsKeep * 4))) return rc;
     const int nc = row_ctas(rows, V, 74), slice = ((V + 3) / 4 / nc + 1) * 4;
     const size_t smem = (size_t)(slice < kProbsKeep ? slice : kProbsKeep) * 4;
     if (!(temp > 0.0f)) return launch_rows(k_probs<true>, kProbsThreads, rows, nc, smem, s, l, ldl, V, 0.0f, p, ldp);

@@ -103,3 +103,45 @@ def test_results_of_probs_and_verify_on_another_stream(cuda):
     n2, t2 = m.verify(p2, draft, u, stream=side)
     torch.cuda.synchronize()
     assert torch.equal(p, p2) and torch.equal(n, n2) and torch.equal(t, t2)
+
+
+FIRST_CALLS = """
+import threading, torch
+import large_model_b200 as m
+m.init(0)
+g = torch.Generator(device="cuda").manual_seed(1)
+P, Hk, D, H, n = 16, 2, 128, 32, 5
+k, v = (torch.randn((12, P, Hk, D), generator=g, device="cuda") for _ in range(2))
+q = torch.randn((2 * n, H * D), generator=g, device="cuda")
+logits = torch.randn((4, 32003), generator=g, device="cuda")
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+start, kv, table = ints([0, n, 2 * n]), ints([90, 50]), ints([list(range(6)), list(range(6, 12))])
+torch.cuda.synchronize()
+res, go = [None] * 8, threading.Barrier(8)
+
+def work(i):
+    torch.cuda.set_device(0)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        batch = m.PagedBatch(start, kv, table, 2 * n, n, 96)
+        pages = m.KvPages(k, v) if i % 2 else m.KvPages(k.half(), v.half())
+        torch.cuda.current_stream().synchronize()
+        go.wait()
+        out = [m.paged_attention(pages, batch, q, H), m.probs(logits, 0.8 * (i % 4 > 1))]
+        batch.status()
+        res[i] = out
+
+t = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+[x.start() for x in t]
+[x.join() for x in t]
+for i in range(4, 8):
+    assert torch.equal(res[i][0], res[i - 4][0]) and torch.equal(res[i][1], res[i - 4][1])
+print("same")
+"""
+
+
+def test_first_calls_from_several_threads(cuda):
+    import subprocess
+    import sys
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
