@@ -248,7 +248,8 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
  * ldq / ldo), q head h reading kv head h / (n_head / n_head_kv). What lies at positions that a row
  * does not see has no effect on it, whatever its bits (fp32 cache: K and V that other rows of the call see
  * and that are over some 2^10 times larger than what the row sees cost it precision); a V value that it sees and
- * that is not finite makes that element of the row not finite. A row that sees nothing (padding, a negative
+ * that is not finite makes that element of the row not finite. Scores of -inf have weight 0 (a row with no
+ * other is 0 or NaN); rows with K that is not finite take a slow path. A row that sees nothing (padding, a negative
  * position, an idle sequence) is zero; positions on a bad page set *err and count as not seen.
  * ws: device workspace, 256-byte aligned, of at least qms_cuda_paged_attention_ws() bytes (a function
  * of the sizes in the two descriptors; negative: a status), contents irrelevant before and after. */

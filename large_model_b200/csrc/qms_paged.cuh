@@ -158,6 +158,7 @@ struct PagedAttn {
     float *out;
     int64_t ldq, ldo;
     float scale2;                    // scale * log2(e)
+    bool f16;                        // the cache's type
     float *part_o;
     float2 *part_ml;
 };

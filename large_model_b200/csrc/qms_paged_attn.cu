@@ -596,13 +596,65 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
     if (last) pdl_wait();
 }
 
+// ---- a row as it is defined --------------------------------------------------------------------------
+// Row `row` (token * H + q head) of the output in plain fp32, by one warp: for rows whose weights' sum came out NaN. The two fp16
+// terms of an operand make NaN of an infinite value (inf - inf, 0 * inf) also where the score is -inf and the weight 0. Reached by
+// values that are not finite alone; a q that is not makes the row NaN in any case, and is left. False then.
+template <typename T>
+__device__ __forceinline__ void fetch_part(const T *src, float (&v)[4]) { *reinterpret_cast<float4 *>(v) = kv_ldg4(src); }
+template <typename T>
+__device__ __forceinline__ void fetch_part(const T *src, float (&v)[2]) { *reinterpret_cast<float2 *>(v) = kv_ldg2(src); }
+
+template <int D>
+__device__ __noinline__ bool plain_row(const PagedAttn &A, unsigned row) {
+    constexpr int J = D / 32;
+    float x[J];
+    const Paged &a = A.a;
+    const int lane = threadIdx.x & 31, t = row / (unsigned)a.H, h = row - t * a.H;
+    float q[J], m = -INFINITY, l = 0.0f;
+    int b = 0, t0, n, kv;
+    while (b < a.n_seq && a.q_start[b + 1] <= t) b++;           // (one by one: paged_seq_of twice in a kernel costs each row)
+    if (b == a.n_seq || !paged_seq(a, b, t0, n, kv) || t < t0) return false;
+    fetch_part(A.q + t * A.ldq + (int64_t)h * D + lane * J, q);
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < J; j++) finite = finite && isfinite(q[j]), x[j] = 0.0f;
+    if (!__all_sync(kFull, finite)) return false;
+#pragma unroll 1
+    for (int p = 0; p < kv - n + (t - t0) + 1; p++) {
+        const int64_t at = paged_at(a, a.table + (p < a.prefix ? 0 : (int64_t)b * a.table_stride), p);
+        if (at < 0) continue;
+        const int64_t head = at + h / a.G * a.head_stride;
+        float k[J], v[J], s = 0.0f;
+        if (A.f16) {
+            fetch_part(reinterpret_cast<const __half *>(a.k + head) + lane * J, k);
+            fetch_part(reinterpret_cast<const __half *>(a.v + head) + lane * J, v);
+        } else {
+            fetch_part(reinterpret_cast<const float *>(a.k + head) + lane * J, k);
+            fetch_part(reinterpret_cast<const float *>(a.v + head) + lane * J, v);
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++) s = fmaf(q[j], k[j], s);
+        s = warp_sum(s) * A.scale2;
+        const float f = s > m ? ex2(m - s) : 1.0f;              // (from -inf: 0)
+        m = fmaxf(m, s);
+        const float w = m == -INFINITY && !isnan(s) ? 0.0f : ex2(s - m);
+        l = fmaf(l, f, w);
+#pragma unroll
+        for (int j = 0; j < J; j++) x[j] = fmaf(w, v[j], x[j] * f);
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) A.out[t * A.ldo + (int64_t)h * D + lane * J + j] = x[j] / l;
+    return true;
+}
+
 // ---- joining the slots of a row --------------------------------------------------------------------
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the slots of a (token, q head) row in their order; 0 where
 // nothing was seen. WPR warps per row, each with every WPR-th slot; the loads of (m, l) and of the first slots go out
 // before the row's length is known (what was not written is not used), so that the chain is one round trip.
 // Bound by that latency for few rows, by the partial results' traffic (L2) for many.
 template <int D, int WPR>
-__global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
+__global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ PagedAttn A) {
     constexpr int J = D / 32, AHEAD = 4;
     __shared__ float s_x[WPR > 1 ? 8 : 1][D], s_l[8];
     const Paged &a = A.a;
@@ -704,6 +756,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const PagedAttn A) {
     }
     if (!there) return;
     float *dst = A.out + t * A.ldo + (int64_t)(row - t * a.H) * D + lane * J;
+    if (__any_sync(kFull, isnan(l)) && plain_row<D>(A, row)) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if constexpr (J == 4) *reinterpret_cast<float4 *>(dst) = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     else *reinterpret_cast<float2 *>(dst) = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x[0] * inv, x[1] * inv);
@@ -866,6 +919,7 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     A.ldq = ldq;
     A.ldo = ldo;
     A.scale2 = scale * 1.4426950408889634f;
+    A.f16 = type == QMS_T_F16;
     A.part_o = (float *)ws;
     // (32-bit run arithmetic)
     QMS_REQUIRE((int64_t)p.tiles_p * a.Hk * ((a.prefix + 63) / 64) < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");

@@ -195,6 +195,41 @@ def test_small_q_and_large_k(cuda, n):
     assert ((out.double() - want).abs() <= tol).all()
 
 
+# ---- K that is not finite ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("typ,n", KERNELS)
+def test_infinite_scores(cuda, typ, n):
+    """K of one seen position is infinite in one value. A row whose q there makes the score -inf gives the position no weight; where it
+    makes +inf, or q is 0 there, nothing finite is left (inf - inf, 0 * inf)."""
+    import torch
+    import large_model_b200 as m
+    kv, p = 700, 321
+    for bad in (float("inf"), -float("inf")):
+        pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+        x = q.view(n, 2, 16, 128)
+        x[0, 0, 3, 5] = 0.0
+        x[0, 0, 4, 5] = 1e-30
+        x[0, 0, 5, 5] = -1e-30
+        put(pages, batch, 0, p, 0, 5, bad, "k")
+        out = m.paged_attention(pages, batch, q, 32).view(n, 2, 16, 128)
+        batch.status()
+        keep = torch.arange(kv, device="cuda") != p
+        # (the reference: head 1 as it is; head 0 without the position, whose weight is 0)
+        full, tol1 = reference([n], [kv], q, K, V, 16, 128 ** -0.5)
+        less = torch.zeros_like(full).view(n, 2, 16, 128)
+        tol = torch.zeros_like(less)
+        for i in range(n):
+            last = kv - n + i + 1
+            a, b = reference([1], [last - 1], q[i:i + 1], [K[0][:last][keep[:last]]], [V[0][:last][keep[:last]]], 16, 128 ** -0.5)
+            less[i], tol[i] = a.view(2, 16, 128), b.view(2, 16, 128)
+        less[:, 1], tol[:, 1] = full.view(n, 2, 16, 128)[:, 1], tol1.view(n, 2, 16, 128)[:, 1]
+        none = x[:, 0, :, 5] * bad < 0               # [n, 16]: score -inf
+        ok = torch.ones((n, 2, 16), dtype=torch.bool, device="cuda")
+        ok[:, 0] = none
+        assert not torch.isfinite(out[~ok]).any()
+        assert ((out.double() - less).abs() <= tol)[ok].all()
+
+
 # ---- lengths -------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("typ,n", KERNELS)
