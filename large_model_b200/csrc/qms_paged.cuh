@@ -66,11 +66,14 @@ __device__ __forceinline__ uint32_t pack_h2(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// (x, y) = hi + lo in fp16 pairs
+// (x, y) = hi + lo in fp16 pairs, hi to nearest (so that lo has either sign: the tensor cores cut every product at the last bits
+// of the sum, towards 0, and cuts of either sign cancel)
 __device__ __forceinline__ void split_h2(float x, float y, uint32_t &hi, uint32_t &lo) {
     hi = pack_h2(x, y);
-    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    lo = pack_h2(x - h.x, y - h.y);
+    asm("{\n\t.reg .b16 a, b, m;\n\t.reg .f32 x, y;\n\tmov.b32 {a, b}, %1;\n\tmov.b16 m, 0xBC00;\n\t"
+        "fma.rn.f32.f16 x, a, m, %2;\n\tfma.rn.f32.f16 y, b, m, %3;\n\tcvt.rn.f16x2.f32 %0, y, x;\n\t}"
+        : "=r"(lo)
+        : "r"(hi), "f"(x), "f"(y));
 }
 // x = hi + lo, hi the 11 leading bits (what a tf32 operand keeps)
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }

@@ -70,10 +70,10 @@ struct WideCfg {
     // for given o, expected at ADDS * CUT * o * (l then) / (l at the end), and at half the tile's own weights at most: that is given
     // back at the end. (RISE: while l grows within a tile, of the hi terms.) Nothing is given back where nothing was cut: where l
     // has so few bits that all weights are alike (fp16 values add up exactly then; of fp32 values those whose o has few bits too).
-    // What is left, of an output: 1 to 2e-6 for values of either sign, as a plain fp32 softmax. Values of one sign lose up to 1.1e-5
-    // (PAIR, SPLIT) or 1.4e-5 (F32) more than is given back, since every product is cut at the sum's last bits by itself; a row
-    // whose first weight is 2^14 to 2^26 times each other one is up to 5e-6 too large. Half the additions per sum would leave half
-    // of that, for 1.12 times the time (F32: 1.19).
+    // What is left, of an output: 1 to 2e-6 for values of either sign, as a plain fp32 softmax; up to 6e-6 for values of one sign (every
+    // product is cut at the sum's last bits by itself; the low terms have either sign and lose nothing by that). A row whose
+    // first weight is 2^14 to 2^26 times each other one is up to 5e-6 too large, or with values of one sign 9e-6 too small. Half
+    // the additions per sum would leave half of that, for 1.12 times the time (F32: 1.19).
     static constexpr float CUT = MODE == F32 ? 4.3e-8f : 3.6e-8f, ADDS = MODE == F32 ? 12.0f : 16.0f, RISE = MODE == F32 ? 2.0f : 4.0f;
     // Load n of a ring (K, V, K, ...): its slot. One ring for both streams; in SPLIT a ring per stream.
     static __device__ __forceinline__ uint32_t slot(int stream, uint32_t n) { return MODE == SPLIT ? 2 * stream + (n & 1) : n % 3; }
@@ -480,11 +480,8 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     for (int e = 0; e < 32; e += 2) {
                         const float2 q = f2_fma(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), f2, nB);
                         const float2 w2 = make_float2(ex2(q.x), ex2(q.y));
-                        const float2 h = make_float2(tf32_hi(w2.x), tf32_hi(w2.y));        // 11 bits: an fp16 value
-                        const float2 lo = f2_fma(h, make_float2(-1.0f, -1.0f), w2);
                         l2 = f2_add(l2, w2);
-                        o[e / 2] = pack_h2(h.x, h.y);
-                        o[16 + e / 2] = pack_h2(lo.x, lo.y);
+                        split_h2(w2.x, w2.y, o[e / 2], o[16 + e / 2]);
                     }
                     tmem_st32(s_col + 32 * c, o);
                     S += l2.x + l2.y;
@@ -811,17 +808,18 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     if (ct == 0) s_up[4 * is_v + (t & 3)] = up;
                     ok = __all_sync(kFull, ok && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
                     if (ok) {
-                        const float2 u2 = make_float2(pow2_bits(up), pow2_bits(up)), minus = make_float2(-1.0f, -1.0f);
+                        const float2 u2 = make_float2(pow2_bits(up), pow2_bits(up));
                         unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
 #pragma unroll
                         for (int i = 0; i < N; i++) {
                             const int r = (ct + 128 * i) / CH, q = ct % CH;   // values 4 q .. + 3 of row r
                             const float2 y0 = f2_mul(make_float2(x[i].x, x[i].y), u2), y1 = f2_mul(make_float2(x[i].z, x[i].w), u2);
-                            const float2 h0 = make_float2(tf32_hi(y0.x), tf32_hi(y0.y)), h1 = make_float2(tf32_hi(y1.x), tf32_hi(y1.y));
-                            const float2 l0 = f2_fma(h0, minus, y0), l1 = f2_fma(h1, minus, y1);
+                            uint32_t h0, h1, l0, l1;
+                            split_h2(y0.x, y0.y, h0, l0);
+                            split_h2(y1.x, y1.y, h1, l1);
                             unsigned char *to = dst + (q >> 4) * C::HALF + r * 128 + ((((q & 15) >> 1) ^ (r & 7)) << 4) + (q & 1) * 8;
-                            *reinterpret_cast<uint2 *>(to) = make_uint2(pack_h2(h0.x, h0.y), pack_h2(h1.x, h1.y));
-                            *reinterpret_cast<uint2 *>(to + C::TILE) = make_uint2(pack_h2(l0.x, l0.y), pack_h2(l1.x, l1.y));
+                            *reinterpret_cast<uint2 *>(to) = make_uint2(h0, h1);
+                            *reinterpret_cast<uint2 *>(to + C::TILE) = make_uint2(l0, l1);
                         }
                     }
                     fence_async_smem();

@@ -176,6 +176,28 @@ def test_one_position_far_above_the_others(cuda, typ, n, top):
         assert (out.double() - want).abs().max() <= 1e-6 * V[0].abs().max(), kv
 
 
+@pytest.mark.parametrize("typ,n", KERNELS)
+@pytest.mark.parametrize("kv", [2300, 9000])
+def test_values_of_one_sign(cuda, typ, n, kv):
+    """All products of a sum have its sign, so that what the tensor cores cut off each adds up: 16 products of an addition at some 2^-27
+    of the sum each, 64 additions of hi terms while it grows from 0, is 64 * 16 * 2^-27 / 2 = 4e-6 of an output; 8e-6 with the
+    additions themselves and the scores' share."""
+    import torch
+    import large_model_b200 as m
+    for kind in range(2):
+        pages, batch, q, K, V = one_unit(n, kv, typ=typ)
+        if kind:
+            V[0].abs_()
+        else:
+            V[0].mul_(0.1).add_(1)
+        j = torch.arange(kv, device="cuda")
+        pages.v[batch.table[0].long()[j // 64], j % 64] = V[0]
+        out = m.paged_attention(pages, batch, q, 32)
+        batch.status()
+        want, _ = reference([n], [kv], q, K, V, 16, 128 ** -0.5)
+        assert (out.double() - want).norm() <= 8e-6 * want.norm(), kind
+
+
 # ---- orders of magnitude -------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("n", [1, 2, 4, 8])
