@@ -985,6 +985,13 @@ def main():
                     help="batched modes: Zipf(s) expert popularity (config 5: --mode prefill --zipf 1.1)")
     a = ap.parse_args()
     a.warmup = max(a.warmup, 3)
+    from oracle import reference_available
+    if not reference_available():
+        if a.impl == "reference":
+            if int(os.environ.get("RANK", "0")) == 0:
+                print(json.dumps({"impl": "reference", "unavailable": "no build of the reference's sources here (make -C oracle ref needs them)"}), flush=True)
+            return 0
+        a.no_cpu = True                                  # no CPU sample either: the line's cpu_baseline is null
     if a.impl == "reference":
         return run_model_reference_arm(a) if a.mode in ("model", "model-bs64") else run_reference_arm(a)
     if a.mode == "model":
