@@ -246,11 +246,16 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
 /* Causal grouped-query attention of the batch's rows over the paged cache: out[t][h] = sum over
  * positions j <= position of t of softmax_j(scale * q[t][h] . K[j]) V[j], fp32 in and out (rows of
  * ldq / ldo), q head h reading kv head h / (n_head / n_head_kv). What lies at positions that a row
- * does not see has no effect on it, whatever its bits (fp32 cache: K and V that other rows of the call see
- * and that are over some 2^10 times larger than what the row sees cost it precision); a V value that it sees and
- * that is not finite makes that element of the row not finite. Scores of -inf have weight 0 (a row with no
- * other is 0 or NaN); rows with K that is not finite take a slow path. A row that sees nothing (padding, a negative
- * position, an idle sequence) is zero; positions on a bad page set *err and count as not seen.
+ * does not see has no effect on it, whatever its bits (fp32 cache: but for the scales below). A V
+ * value that it sees and that is not finite makes that element of the row not finite. Scores of -inf
+ * have weight 0 (a row with no other is 0 or NaN); rows with K that is not finite take a slow path. A
+ * row that sees nothing (padding, a negative position, an idle sequence) is zero; positions on a bad
+ * page set *err and count as not seen.
+ * Precision: q, the weights and an fp32 cache's K and V enter the products as two fp16 terms, 22 bits,
+ * under power-of-two scales: of q by row, of K by position or by 64 of them, of V by the largest so
+ * far that any row sees that shares the K and V tiles. What is 2^-10 of the largest or less is kept to
+ * 2^-33 of the largest. Sums are fp32: an output is off by some 1e-6 of itself, or up to 6e-6 where
+ * many rows meet many positions and the values have one sign.
  * ws: device workspace, 256-byte aligned, of at least qms_cuda_paged_attention_ws() bytes (a function
  * of the sizes in the two descriptors; negative: a status), contents irrelevant before and after. */
 int64_t qms_cuda_paged_attention_ws(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, int n_head);
@@ -261,7 +266,8 @@ int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch 
 /* Probabilities of rows of logits at a temperature: p = exp((l - max) / temp) / sum, fp32 rows of ldl /
  * ldp (p may be the logits themselves); temp <= 0: 1 at the first maximum, 0 elsewhere, the greedy
  * choice of qms_cuda_sample. -inf logits have probability 0; a row of nothing else is all 0; a row with
- * NaN or +inf is NaN (greedy: NaN is never chosen). */
+ * NaN or +inf is NaN (greedy: NaN is never chosen). No top-k or top-p: qms_cuda_sample, which always cuts,
+ * draws from another distribution at temp > 0. */
 int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float temp, float *p, int64_t ldp, void *stream);
 
 /* Speculative verification: which drafted tokens stand, and the token after them, such that the
@@ -272,9 +278,9 @@ int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float 
  * Draft i stands when those before it do and u[b][i] * q(x_i) < p(x_i). n_accept[b] of them stand; the
  * next token comes from max(0, p - q) at the first that does not (from p where that is 0
  * everywhere), or from the row after the last: the lowest index whose cumulative weight exceeds
- * u[b][max_draft] * total, weights rounded to multiples of 2^-40 (and limited to 1) and added as
- * integers, so the token does not depend on the order of the additions. tokens [n_seq][max_draft +
- * 1]: the standing drafts, the next token, then -1. A draft id outside the vocabulary never stands;
+ * u[b][max_draft] (taken down to a multiple of 2^-24) * total, weights rounded to multiples of 2^-40
+ * (and limited to 1) and added as integers, so the token does not depend on the order of the
+ * additions. tokens [n_seq][max_draft + 1]: the standing drafts, the next token, then -1. A draft id outside the vocabulary never stands;
  * no positive weight gives token -1; bad row or draft counts give n_accept 0 and token -1. */
 int qms_cuda_verify(const float *p, int64_t ldp, int p_rows, const int *row_start, const float *q, int64_t ldq,
                     const int *draft, const int *n_draft, int n_seq, int max_draft, int vocab, const float *u,

@@ -51,9 +51,9 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
 // issuing alone); stages start on page boundaries, so the first may begin before the unit's first position, and boxes
 // past the unit or on bad pages are not loaded: all that is masked. Each warp scores its rows against its share
 // of the stage, keeps its own running (m, l, o), and the position groups are joined in shared memory at the end.
-// One token each of 64 sequences of 4096 positions (64 q heads, 4 kv heads): fp16 105 us, 5.1 TB/s, 0.80 of a plain copy;
-// fp32 313 us, 3.4 TB/s. What is left goes to the chain of each stage: the barrier, the scores, the softmax and (fp32) the
-// split before them; issue slots are 37% used, tensor cores 30% (22%). One sequence of 1100 positions: 12 us, of which some 4
+// One token each of 64 sequences of 4096 positions (64 q heads, 4 kv heads): fp16 104 us, 5.2 TB/s, 0.80 of a plain copy;
+// fp32 308 us, 3.5 TB/s. What is left goes to the chain of each stage: the barrier, the scores, the softmax and (fp32) the
+// split before them; issue slots are 36% (31%) used, tensor cores 31% (22%). One sequence of 1100 positions: 12 us, of which some 4
 // are the launch and 4 the join of the slots.
 template <int D, typename KT, int WR>
 struct PaCfg {
@@ -460,8 +460,8 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             }
             // ---- o += weights * V. The tensor cores add by cutting bits off, towards 0; so they add up one stage, from 0, and its
             // sums join o by additions that round to nearest. In us, against sums over a whole unit (off by up to 8e-6): 64 tokens
-            // over 4096 positions fp16 104, 105; 64 on a prompt of 1024 38.7, 37.5; 16 x 4 on 1000 29.8, 28.1; 8 x 4 on 2000 fp32
-            // 42.3, 40.0.
+            // over 4096 positions fp16 104, 105; 64 on a prompt of 1024 37.7, 37.5; 16 x 4 on 1000 29.4, 28.1; 8 x 4 on 2000 fp32
+            // 42.4, 40.0.
             uint32_t ph[C::NT / 2][4], pl[C::NT / 2][4];
 #pragma unroll
             for (int kk = 0; kk < C::NT / 2; kk++) {
@@ -766,10 +766,10 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
 // Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); k_paged_wide
 // from 65 on (fp16: in pages of 8 positions or more, a swizzle unit of its tiles) and from so many rows x positions (`rows`
 // by the 64, over all units) that its longer start pays. Narrow against wide in us, 16 q heads per kv head, 4 of these:
-// 80 rows x 16 sequences x 1000 positions 38.8, 25.8 (fp32 68.3, 43.3); 64 rows of the same 25.3, 24.7 (40.4, 43.4). By millions
-// of rows x positions: own ones 1.2 narrow 17.1, wide 21.9 (22.1, 20.9); 2.5 22.5, 26.6 (31.1, 29.3); 3.1 24.2, 23.6 (35.4, 28.1); 4.1
-// 25.2, 22.8 (39.9, 30.4); shared ones 1.6 22.8, 24.6 (34.1, 34.6); 3.1 29.2, 26.8 (41.9, 40.2); 6.3 37.4, 38.2 (62.4, 50.7); 16.8 71, 44
-// (130, 85).
+// 80 rows x 16 sequences x 1000 positions 40.9, 26.5 (fp32 74.2, 47.1); 64 rows of the same 27.8, 26.1 (44.6, 45.6). By millions
+// of rows x positions: 8 sequences of 5 tokens, own positions 1.2 narrow 17.6, wide 19.5 (22.2, 21.4); 1.8 19.5, 19.2 (26.1, 28.1); 2.5
+// 21.8, 18.4 (29.8, 27.2); 4.1 25.9, 19.6 (42.3, 31.0); 20 tokens on a prompt, shared ones 1.6 23.4, 25.1 (35.4, 36.9); 2.0 27.8, 27.2 (38.0,
+// 37.7); 3.1 31.3, 35.1 (45.7, 46.5); 6.3 39.8, 43.5 (65.8, 58.2); 16.8 69, 63 (139, 96).
 static int row_groups(int type, int page_log, int64_t rows, int64_t positions, bool shared) {
     const bool f16 = type == QMS_T_F16;
     if (rows > 64 && (!f16 || page_log >= 3) && (rows + 63) / 64 * 64 * positions > (f16 || shared ? 2600000 : 1200000))

@@ -30,8 +30,8 @@
 // (SPLIT), Q 64 KB, 2 stages and a ring of 3 (F32); TMEM: S 2 x 128, O 2 x 128 columns.
 // Bound by the tensor cores, 4 * 128 * 128 * head_dim flop per 128 rows and positions, times 2 (fp16) or 3, and by the softmax
 // between a tile's two products where the other stream does not cover it: 64 sequences of 5 tokens (64 q heads, 4 kv heads)
-// over 8192 shared and 640 own fp16 positions take 237 us, 391 TFLOP/s by the definition and 780 with the split; tensor
-// cores 43% active. A prompt chunk of 256 tokens over 4096 positions: 82 us, 407 TFLOP/s.
+// over 8192 shared and 640 own fp16 positions take 235 us, 394 TFLOP/s by the definition and 788 with the split; tensor
+// cores 45% active. A prompt chunk of 256 tokens over 4096 positions: 85 us, 394 TFLOP/s.
 #include <math.h>
 #include <string.h>
 
