@@ -270,6 +270,17 @@ int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch 
  * draws from another distribution at temp > 0. */
 int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float temp, float *p, int64_t ldp, void *stream);
 
+/* Log probabilities of given tokens, and of the likeliest ones, and the entropy of rows of logits (fp32 rows of
+ * ldl) at a temperature > 0: with x = (l - max) / temp, log p = x - log sum exp(x), entropy = -sum p log p, natural logarithms. logp
+ * [rows][n_ids] of tokens ids [rows][n_ids]; entropy [rows] (NULL: not wanted); top_id, top_logp [rows][n_top], the
+ * n_top <= 32 largest logits in their order, the lowest id first among equals (n_top 0: not wanted). Values near 0 are as
+ * exact as others: the sum is kept without its largest term. A token of logit -inf has -inf, and is never among the
+ * likeliest: where the others do not fill n_top the rest are -1 and -inf. A row of nothing else has -inf everywhere and entropy 0;
+ * a row with NaN or +inf is NaN everywhere but in top_id (NaN is never chosen). An id outside [0, vocab) has NaN and sets
+ * QMS_PAGED_ETOKEN in *err. */
+int qms_cuda_logprobs(const float *logits, int64_t ldl, int rows, int vocab, float temp, const int *ids, int n_ids, float *logp,
+                      float *entropy, int n_top, int *top_id, float *top_logp, int *err, void *stream);
+
 /* Speculative verification: which drafted tokens stand, and the token after them, such that the
  * result is distributed as draws from the target's p. Sequence b has rows row_start[b] + i (NULL:
  * b * (max_draft + 1) + i), i = 0 .. n_draft[b], of p (p_rows rows of ldp), drafted tokens draft[b][i] with i <

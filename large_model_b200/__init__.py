@@ -15,6 +15,7 @@ and adds the operators of batched serving behind a shared prompt, with drafted t
     paged_append(...)            QK-norm, rotation and the cache append in one pass
     paged_attention(...)         causal attention over the pages, a shared prompt read once
     probs(logits, temp)          probabilities of logits rows
+    logprobs(logits, ids, top)   log probabilities of given tokens, the entropy, the likeliest tokens
     verify(p, draft, u)          which drafted tokens stand, and the token after them
 
 Device buffers are torch CUDA tensors (plumbing only); every computation runs in
@@ -137,6 +138,7 @@ def lib() -> C.CDLL:
     L.qms_cuda_paged_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, vp, i64, vp, vp]
     L.qms_cuda_paged_attention_ws.argtypes = [pg, pb, i32]
     L.qms_cuda_paged_attention_ws.restype = i64
+    L.qms_cuda_logprobs.argtypes = [vp, i64, i32, i32, f32, vp, i32, vp, vp, i32, vp, vp, vp, vp]
     L.qms_cuda_paged_attention.argtypes = [pg, pb, vp, i64, i32, f32, vp, i64, vp, i64, vp, vp]
     L.qms_cuda_probs.argtypes = [vp, i64, i32, i32, f32, vp, i64, vp]
     L.qms_cuda_verify.argtypes = [vp, i64, i32, vp, vp, i64, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp]
@@ -449,6 +451,31 @@ def _on_stream(raw: int, device):
     return torch.cuda.stream(torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device))
 
 
+class _Same:
+    """Nothing to enter: the call's device is the current one."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_same = _Same()
+
+
+def _device_of(t):
+    """t's device as the current one, for the call."""
+    torch = _torch()
+    return _same if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _one_device(who: str, t, *others):
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{who}: tensors on {t.device} and {o.device}")
+
+
 def _empty(shape: tuple, dtype, device, stream):
     """A result of a call on that stream (None: the current one)."""
     if stream is None:
@@ -615,6 +642,34 @@ def probs(logits, temp: float, out=None, stream=None):
     if rc:
         check(rc)
     return out
+
+
+def logprobs(logits, ids=None, top: int = 0, temp: float = 1.0, out=None, err=None, stream=None):
+    """Log probabilities of rows of logits (CUDA float32 [rows][vocab]) at a temperature (qms_cuda_logprobs): returns
+    (logp float32 [rows][n] of the tokens ids int32 [rows][n] or [rows], entropy float32 [rows], the `top` likeliest tokens int32
+    [rows][top], their logp float32 [rows][top]). out: those four tensors; err: CUDA int32 [1] or None."""
+    torch = _torch()
+    V = logits.shape[-1]
+    x, n, ldx = _rows(logits, V, "logits")
+    k = 0 if ids is None else 1 if ids.dim() == 1 else ids.shape[-1]
+    if ids is not None and tuple(ids.shape) not in ((n, k), (n,)):
+        raise ValueError(f"logprobs: ids {tuple(ids.shape)} for {n} rows")
+    dev = logits.device
+    if out is None:
+        out = (_empty((n, k), torch.float32, dev, stream), _empty((n,), torch.float32, dev, stream),
+               _empty((n, top), torch.int32, dev, stream), _empty((n, top), torch.float32, dev, stream))
+    logp, entropy, top_id, top_logp = out
+    _one_device("logprobs", logits, ids, err, *out)
+    if n == 0:
+        return logp, entropy, top_id, top_logp
+    with _device_of(logits):
+        rc = lib().qms_cuda_logprobs(x, ldx, n, V, temp, _ints(ids, tuple(ids.shape), "ids") if k else None, k,
+                                     _vec(logp, n * k, "logp") if k else None, _vec(entropy, n, "entropy"), top,
+                                     _ints(top_id, (n, top), "top_id") if top else None, _vec(top_logp, n * top, "top_logp") if top else None,
+                                     None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, logits))
+    if rc:
+        check(rc)
+    return logp, entropy, top_id, top_logp
 
 
 def verify(p, draft, u, q=None, n_draft=None, row_start=None, n_accept=None, tokens=None, err=None, stream=None):
