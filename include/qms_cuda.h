@@ -28,6 +28,9 @@ extern "C" {
 enum { QMS_T_F32 = 0, QMS_T_F16 = 1, QMS_T_Q4_0 = 2, QMS_T_Q4_1 = 3, QMS_T_Q8_0 = 8, QMS_T_Q6_K = 14 };
 #endif
 
+/* bfloat16, GGUF numbering, for the entries that take 16-bit rows. */
+enum { QMS_CUDA_T_BF16 = 30 };
+
 /* Status codes. */
 enum {
     QMS_CUDA_OK = 0,
@@ -208,7 +211,13 @@ enum {
 /* A pool of n_pages pages of page_size positions (a power of two). K of (page, position in it, kv
  * head) starts at k + page * page_stride + position * pos_stride + head * head_stride elements of
  * `type` (QMS_T_F32 or QMS_T_F16), its head_dim values contiguous; V alike. Any order of the three
- * strides; the pointers and strides are multiples of 16 bytes. head_dim 64 or 128. */
+ * strides; the pointers and strides are multiples of 16 bytes. head_dim 64 or 128.
+ * QMS_T_Q4_0, 4.5 bits a value: the strides are bytes, pos_stride is 0, page_size at least 16. At page * page_stride + head *
+ * head_stride lie first the positions' nibbles n, head_dim / 2 bytes each, value i of every 8 in bits 4 (i / 2) + 16 (i % 2) of
+ * a 32-bit word, then the positions' scales d, an fp16 number for every 32 values. A value is d (n - 8). The append takes for d the
+ * value of largest magnitude (the first of equals) over -8, rounded to 8 significant bits and to at most 2720, n = floor(x / d + 8.5)
+ * within 0 .. 15; 32 values of which one is not finite are NaN. Scales from elsewhere keep to those 8 bits and 2720, or lose what is
+ * beyond fp16's 11 bits in the product. */
 typedef struct {
     int type, n_pages, page_size, n_head_kv, head_dim;
     int64_t page_stride, pos_stride, head_stride;
@@ -233,7 +242,7 @@ typedef struct {
 } QmsCudaPagedBatch;
 
 /* QK-norm, NEOX rotation and the cache append of new tokens in one pass (src/model.c:436-462, the
- * arithmetic of the whole model's own cache, value for value). qkv: fp32 [n_tok] rows of ldqkv: n_head
+ * arithmetic of the whole model's own cache, value for value; into 4 bits, K goes in double to the end). qkv: fp32 [n_tok] rows of ldqkv: n_head
  * q heads, n_head_kv k heads, n_head_kv v heads of head_dim, as the projections leave them; q_norm,
  * k_norm: fp32 [head_dim]; rope_cos / rope_sin: fp32 [n_rope][head_dim / 2]. q receives the normalised and
  * rotated q heads (rows of ldq; may be qkv itself with ldq = ldqkv, but overlaps it in no other way),
@@ -243,6 +252,17 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
                           int n_head, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
                           const float *rope_sin, int n_rope, float *q, int64_t ldq, int *err, void *stream);
 
+/* The same for whole prompts, with all heads' rows as qms_cuda_prompt_attention reads them: q | k | v heads of each token,
+ * normalised and rotated, in 16 bits (type QMS_T_F16 or QMS_CUDA_T_BF16; rows of ldrows values, a multiple of 8; 16-byte
+ * aligned), each value rounded once from fp32. The pages receive what qms_cuda_paged_append gives them. Without a cache (n_pages 0, k and
+ * v NULL) nothing is stored, and kv_len and table are not looked at: a row's position is its index in its sequence. */
+int qms_cuda_prompt_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *qkv, int64_t ldqkv, int n_head,
+                           const float *q_norm, const float *k_norm, float eps, const float *rope_cos, const float *rope_sin,
+                           int n_rope, int type, void *rows, int64_t ldrows, int *err, void *stream);
+
+/* What a pool holds: fp32 [n_pages][page_size][n_head_kv][head_dim] of K and of V (16-byte aligned), pages in use or not. */
+int qms_cuda_paged_values(const QmsCudaPages *pages, float *k, float *v, void *stream);
+
 /* Causal grouped-query attention of the batch's rows over the paged cache: out[t][h] = sum over
  * positions j <= position of t of softmax_j(scale * q[t][h] . K[j]) V[j], fp32 in and out (rows of
  * ldq / ldo), q head h reading kv head h / (n_head / n_head_kv). What lies at positions that a row
@@ -251,7 +271,7 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
  * have weight 0 (a row with no other is 0 or NaN); rows with K that is not finite take a slow path. A
  * row that sees nothing (padding, a negative position, an idle sequence) is zero; positions on a bad
  * page set *err and count as not seen.
- * Precision: q, the weights and an fp32 cache's K and V enter the products as two fp16 terms, 22 bits,
+ * Precision: q, the weights and an fp32 cache's K and V (those of an fp16 one and of one in 4 bits are exact in fp16) enter the products as two fp16 terms, 22 bits,
  * under power-of-two scales: of q by row, of K by position or by 64 of them, of V by the largest so
  * far that any row sees that shares the K and V tiles. What is 2^-10 of the largest or less is kept to
  * 2^-33 of the largest. Sums are fp32: an output is off by some 1e-6 of itself, or up to 6e-6 where

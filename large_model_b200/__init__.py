@@ -12,7 +12,8 @@ with ctypes and mirrors the reference's operator interface for tests and benchma
 and adds the operators of batched serving behind a shared prompt, with drafted tokens:
 
     KvPages, PagedBatch          a paged KV cache, and a batch of new tokens over it
-    paged_append(...)            QK-norm, rotation and the cache append in one pass
+    paged_append(...)            QK-norm, rotation and the cache append in one pass (pages of fp32, fp16 or 4 bits)
+    prompt_append(...)           the same for whole prompts, with the heads' rows in 16 bits
     paged_attention(...)         causal attention over the pages, a shared prompt read once
     probs(logits, temp)          probabilities of logits rows
     logprobs(logits, ids, top)   log probabilities of given tokens, the entropy, the likeliest tokens
@@ -33,7 +34,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libqms_cuda.so"
 HEADER = PKG.parent / "include" / "qms_cuda.h"
 
-T_F32, T_F16, T_Q4_0, T_Q4_1, T_Q8_0, T_Q6_K = 0, 1, 2, 3, 8, 14
+T_F32, T_F16, T_Q4_0, T_Q4_1, T_Q8_0, T_Q6_K, T_BF16 = 0, 1, 2, 3, 8, 14, 30
 OK, EINVAL, ECUDA, ENOMEM, EUNSUPPORTED, ENODEV, ETIMEOUT = 0, -1, -2, -3, -4, -5, -6
 
 Q8_DTYPE = np.dtype([("d", "<f4"), ("ds", "<f4"), ("s16", "<i2", (2,)), ("q", "i1", (32,))])
@@ -136,6 +137,8 @@ def lib() -> C.CDLL:
     L.qms_cuda_moe_route_noalloc.argtypes = [vp, i32, i32, i32, vp, i32, vp, vp, vp, vp]
     pg, pb, f32 = C.POINTER(PagesDesc), C.POINTER(PagedBatchDesc), C.c_float
     L.qms_cuda_paged_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, vp, i64, vp, vp]
+    L.qms_cuda_prompt_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, i32, vp, i64, vp, vp]
+    L.qms_cuda_paged_values.argtypes = [pg, vp, vp, vp]
     L.qms_cuda_paged_attention_ws.argtypes = [pg, pb, i32]
     L.qms_cuda_paged_attention_ws.restype = i64
     L.qms_cuda_logprobs.argtypes = [vp, i64, i32, i32, f32, vp, i32, vp, vp, i32, vp, vp, vp, vp]
@@ -487,7 +490,7 @@ def _empty(shape: tuple, dtype, device, stream):
 class KvPages:
     """A pool of KV cache pages (QmsCudaPages): k, v CUDA tensors [n_pages][page_size][n_head_kv][head_dim] of
     one shape, type (float32 or float16) and strides, the last dimension contiguous. Another order in
-    memory, such as heads before positions, is a transposed view."""
+    memory, such as heads before positions, is a transposed view. A pool in 4 bits: KvPages.packed, or empty(..., T_Q4_0)."""
 
     def __init__(self, k, v):
         torch = _torch()
@@ -510,9 +513,46 @@ class KvPages:
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, kv_type: int = T_F32) -> "KvPages":
         torch = _torch()
+        if kv_type == T_Q4_0:
+            shape = (n_pages, n_head_kv, page_size * head_dim * 9 // 16)
+            return cls.packed(*(torch.zeros(shape, dtype=torch.uint8, device="cuda") for _ in range(2)), head_dim)
         dt = {T_F32: torch.float32, T_F16: torch.float16}[kv_type]
         k, v = (torch.zeros((n_pages, page_size, n_head_kv, head_dim), dtype=dt, device="cuda") for _ in range(2))
         return cls(k, v)
+
+    @classmethod
+    def packed(cls, k, v, head_dim: int) -> "KvPages":
+        """A pool in 4 bits (T_Q4_0): k, v CUDA uint8 [n_pages][n_head_kv][page_size * head_dim * 9 / 16], the last dimension
+        contiguous; nibbles and scales as QmsCudaPages has them."""
+        torch = _torch()
+        if k.dim() != 3 or k.shape != v.shape or k.stride() != v.stride() or k.stride(2) != 1 or k.dtype is not torch.uint8 or v.dtype is not torch.uint8:
+            raise ValueError("KvPages.packed: k and v need one shape [n_pages][n_head_kv][bytes], uint8, and one set of strides, the "
+                             "last of them 1")
+        if not (k.is_cuda and k.device == v.device):
+            raise ValueError("KvPages.packed: k and v must be on one CUDA device")
+        if head_dim <= 0 or k.shape[2] * 16 % (9 * head_dim):
+            raise ValueError(f"KvPages.packed: {k.shape[2]} bytes are no number of positions of {head_dim} values")
+        self = cls.__new__(cls)
+        self.k, self.v = k, v
+        self.n_head_kv, self.head_dim = k.shape[1], int(head_dim)
+        page = k.shape[2] * 16 // (9 * head_dim)
+        self.desc = PagesDesc(T_Q4_0, k.shape[0], page, k.shape[1], head_dim, k.stride(0), 0, k.stride(1), k.data_ptr(), v.data_ptr())
+        self._ref = C.byref(self.desc)
+        self._key = (T_Q4_0, page, k.shape[1], int(head_dim))
+        return self
+
+    def values(self, k=None, v=None, stream=None):
+        """What the pool holds, as CUDA float32 [n_pages][page_size][n_head_kv][head_dim] (qms_cuda_paged_values): (k, v)."""
+        d = self.desc
+        shape = (d.n_pages, d.page_size, d.n_head_kv, d.head_dim)
+        n = shape[0] * shape[1] * shape[2] * shape[3]
+        k, v = (_empty(shape, _torch().float32, self.k.device, stream) if x is None else x for x in (k, v))
+        _one_device("KvPages.values", self.k, k, v)
+        with _device_of(self.k):
+            rc = lib().qms_cuda_paged_values(self._ref, _vec(k, n, "k"), _vec(v, n, "v"), _raw_stream(stream, self.k))
+        if rc:
+            check(rc)
+        return k, v
 
 
 class PagedBatch:
@@ -535,6 +575,22 @@ class PagedBatch:
                                    int(prefix_len))
         self._ref = C.byref(self.desc)
         self._ws = {}
+
+    @classmethod
+    def prompts(cls, q_start, n_tok: int, max_q: int) -> "PagedBatch":
+        """Whole prompts without a cache, for prompt_append and prompt_attention: prompt b's token rows are q_start[b] ..
+        q_start[b + 1] - 1."""
+        torch = _torch()
+        self = cls.__new__(cls)
+        n = q_start.shape[0] - 1
+        self.q_start, self.kv_len, self.table, self.n_tok = q_start, None, None, int(n_tok)
+        self.err = torch.zeros((1,), dtype=torch.int32, device=q_start.device)
+        self._err = self.err.data_ptr()
+        self._cleared()
+        self.desc = PagedBatchDesc(n, self.n_tok, _ints(q_start, (n + 1,), "q_start"), None, None, 0, int(max_q), 0, 0)
+        self._ref = C.byref(self.desc)
+        self._ws = {}
+        return self
 
     def _cleared(self):
         """`err` is set to zero in the order of the current stream; other streams wait for that once (_use)."""
@@ -607,6 +663,50 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     if rc:
         check(rc)
     return q
+
+
+def _rows16(t, cols: int, what: str):
+    """A CUDA float16 or bfloat16 tensor of rows whose values are contiguous: (type, address, rows, stride)."""
+    torch = _torch()
+    if t.dim() != 2:
+        t = t.view(-1, cols)                # raises where the rows are not contiguous
+    typ = {torch.float16: T_F16, torch.bfloat16: T_BF16}.get(t.dtype)
+    n, c = t.shape
+    ld, one = t.stride()
+    if c != cols or (one != 1 and cols > 1) or typ is None or not t.is_cuda:
+        raise ValueError(f"{what}: CUDA float16 or bfloat16 rows of {cols} contiguous values are needed, got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}, strides {tuple(t.stride())}")
+    return typ, t.data_ptr(), n, ld if n > 1 else max(ld, cols)
+
+
+def prompt_append(pages: KvPages | None, batch: PagedBatch, qkv, n_head: int, q_norm, k_norm, eps: float, rope, rows=None, dtype=None,
+                  n_head_kv: int | None = None, stream=None):
+    """QK-norm and rotation of whole prompts, their cache append (pages None: no cache, n_head_kv is needed then), and all heads' rows
+    q | k | v in 16 bits for prompt_attention (qms_cuda_prompt_append): qkv CUDA float32 [n_tok][(n_head + 2 n_head_kv) * head_dim].
+    Returns rows [n_tok][n_head + 2 n_head_kv][head_dim] of dtype (bfloat16 if not said), or the given rows."""
+    torch = _torch()
+    D = q_norm.numel()
+    Hk = pages.n_head_kv if pages is not None else n_head_kv
+    if Hk is None:
+        raise ValueError("prompt_append: without pages n_head_kv is needed")
+    W = (n_head + 2 * Hk) * D
+    if rows is None:
+        rows = _empty((batch.n_tok, n_head + 2 * Hk, D), dtype or torch.bfloat16, qkv.device, stream)
+    x, n, ldx = _rows(qkv, W, "qkv")
+    typ, y, ny, ldy = _rows16(rows.flatten(1) if rows.dim() == 3 and rows.is_contiguous() else rows, W, "rows")
+    cos, sin = rope
+    nc = cos.shape[0]
+    if n < batch.n_tok or ny < batch.n_tok:
+        raise ValueError(f"prompt_append: {n} qkv and {ny} result rows for {batch.n_tok} tokens")
+    _one_device("prompt_append", qkv, rows, batch.err, q_norm, k_norm, cos, sin, None if pages is None else pages.k)
+    ref = C.byref(PagesDesc(T_F32, 0, 0, Hk, D, 0, 0, 0, None, None)) if pages is None else pages._ref
+    with _device_of(qkv):
+        rc = lib().qms_cuda_prompt_append(ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"), eps,
+                                          _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, typ, y, ldy, batch._err,
+                                          batch._use(stream, qkv))
+    if rc:
+        check(rc)
+    return rows
 
 
 def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: float | None = None, out=None, stream=None):

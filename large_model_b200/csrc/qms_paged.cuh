@@ -41,12 +41,55 @@ __device__ __forceinline__ bool paged_seq(const Paged &a, int b, int &t0, int &n
     return false;
 }
 
+// The same for whole prompts, whose rows are all there is of them: kv_len is not looked at.
+__device__ __forceinline__ bool prompt_seq(const Paged &a, int b, int &t0, int &n, int &kv) {
+    t0 = a.q_start[b];
+    n = kv = a.q_start[b + 1] - t0;
+    if (t0 >= 0 && n >= 0 && n <= a.max_q && n <= a.n_tok - t0) return true;
+    n = kv = 0;
+    return false;
+}
+
 // Byte offset of position p of table row `row` in the K / V pool, or -1 on a bad page id.
 // 0 <= p < table_stride * page_size.
 __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int p) {
     const int page = row[p >> a.page_log];
     if ((unsigned)page >= (unsigned)a.n_pages) return -1;
     return page * a.page_stride + (p & ((1 << a.page_log) - 1)) * a.pos_stride;
+}
+
+// ---- a cache in 4 bits ----
+// Of a (page, kv head) lie first the positions' nibbles, D / 2 bytes each, then their scales, an fp16 number for 32 values. A value
+// is d (n - 8): d has 8 significant bits and |d| <= 2720, so that the value is exact in fp16, and so are its 24 d below.
+// (Paged: pos_stride is D / 2, and paged_at leads to the position's nibbles.)
+struct Q4 {};
+constexpr float kQ4Most = 2720.0f;
+
+__host__ __device__ constexpr int q4_row(int D) { return D / 2 + D / 16; }
+// Byte distance from the nibbles of position `off` of a page to its scales.
+template <int D>
+__device__ __forceinline__ int64_t q4_scales(const Paged &a, int off) {
+    return (int64_t)((1 << a.page_log) - off) * (D / 2) + off * (D / 16);
+}
+// 8 values of a word: value i in bits 4 (i / 2) + 16 (i % 2). A nibble in the upper bits of a mantissa is 16 + n, from there one
+// fused step, d (16 + n) - 24 d, exact. m24: -24 d.
+__device__ __forceinline__ uint4 q4_dequant(uint32_t w, __half2 d, __half2 m24) {
+    uint32_t x[4] = {w << 6, w << 2, w >> 2, w >> 6};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[i] = (x[i] & 0x03C003C0u) | 0x4C004C00u;
+        const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&x[i]), d, m24);
+        x[i] = *reinterpret_cast<const uint32_t *>(&y);
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// One value of a row.
+template <int D>
+__device__ __forceinline__ float q4_ld(const char *nibbles, int64_t scales, int i) {
+    const __half d = __ldcg(reinterpret_cast<const __half *>(nibbles + scales) + (i >> 5));
+    const uint32_t w = __ldcg(reinterpret_cast<const unsigned int *>(nibbles) + (i >> 3));
+    const int n = w >> (4 * ((i & 7) >> 1) + 16 * (i & 1)) & 15;
+    return __half2float(__hfma(__int2half_rn(16 + n), d, __hmul(d, __float2half(-24.0f))));
 }
 
 // ---- pieces of the attention kernels ----
@@ -145,7 +188,8 @@ struct PagedPlan {
     unsigned line, line_runs, line_per, line_q, line_r, line_nt;
     int line_tp, line_rows;
 };
-constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2;   // k_paged_wide: 256 rows; 128; 128 over an fp32 cache
+// k_paged_wide: 256 rows; 128; 128 over an fp32 cache; 128 over one in 4 bits
+constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2, kPaWideQ4 = -3;
 
 // Where run i starts, and which run holds place x. (Divisions are what a short kernel's start waits for: few, of 32 bits.)
 __device__ __forceinline__ unsigned line_start(const PagedPlan &p, unsigned i) { return i * p.line_q + min(i, p.line_r); }
@@ -161,7 +205,7 @@ struct PagedAttn {
     float *out;
     int64_t ldq, ldo;
     float scale2;                    // scale * log2(e)
-    bool f16;                        // the cache's type
+    int type;                        // the cache's
     float *part_o;
     float2 *part_ml;
 };

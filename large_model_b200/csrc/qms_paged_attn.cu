@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "qms_moe.cuh"
 #include "qms_paged.cuh"
@@ -19,7 +20,7 @@ namespace qms {
 
 constexpr uint32_t kPaSpin = 1u << 22;
 constexpr float kPaShift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
-constexpr int pa_stage(int type) { return type == QMS_T_F16 ? 64 : 32; }       // positions per stage: 32 KB of K and V
+constexpr int pa_stage(int type) { return type == QMS_T_F32 ? 32 : 64; }       // positions per stage: 32 KB of K and V (in 4 bits 9)
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -57,21 +58,21 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
 // are the launch and 4 the join of the slots.
 template <int D, typename KT, int WR>
 struct PaCfg {
-    static constexpr bool F16 = sizeof(KT) == 2;
-    static constexpr int PS = F16 ? 64 : 32;
-    static constexpr int WD = !F16 && WR == 1 ? 2 : 1, WK = 4 / WR / WD;
+    static constexpr bool F16 = std::is_same<KT, __half>::value, F32 = std::is_same<KT, float>::value, P4 = std::is_same<KT, Q4>::value;
+    static constexpr int PS = F32 ? 32 : 64;
+    static constexpr int WD = F32 && WR == 1 ? 2 : 1, WK = 4 / WR / WD;
     static constexpr int KW = PS / WK, NT = KW / 8, DW = D / WD;             // positions, 8-position tiles, output dims per warp
-    static constexpr int CH = D * (int)sizeof(KT) / 16, ROW = D * (int)sizeof(KT);      // a row as it comes: 16-byte pieces, bytes
+    static constexpr int ROW = P4 ? q4_row(D) : D * (int)sizeof(KT), CH = ROW / 16;     // a row as it comes: bytes, 16-byte pieces
     static constexpr int STAGE = 2 * ROW * PS;                               // K, then V
     // The tiles that the MMAs read: fp16 rows in halves of 64 values (128 bytes), their 16-byte pieces XOR-swizzled by the
-    // row (ldmatrix reads 8 rows at one piece): the stages themselves, or (fp32) hi and lo of K, hi and lo of V
-    // after the ring.
+    // row (ldmatrix reads 8 rows at one piece): the stages themselves, or after the ring (fp32) hi and lo of K, hi and lo of V,
+    // (4 bits) K and V in fp16.
     static constexpr int HTILE = 2 * D * PS, HALF = 128 * PS;
     static __device__ __forceinline__ uint32_t piece(int r, int c) { return (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
-    static constexpr int NS = WR == 1 || !F16 ? 2 : 3, MINB = WR == 1 && F16 ? 3 : 2;    // stages; CTAs per SM
+    static constexpr int NS = P4 ? 4 : WR == 1 || F32 ? 2 : 3, MINB = WR == 1 && !F32 ? 3 : 2;    // stages; CTAs per SM
     static constexpr int CONV = NS * STAGE;
     static constexpr int RED = WK > 1 ? WK * WR * 16 * (D + 4) * 4 : 0;      // the position groups' o, m, l
-    static constexpr int USED = CONV + (F16 ? 0 : 4 * HTILE), SMEM = (USED > RED ? USED : RED) + 1024;    // (1024: alignment)
+    static constexpr int USED = CONV + (F16 ? 0 : P4 ? 2 * HTILE : 4 * HTILE), SMEM = (USED > RED ? USED : RED) + 1024;    // (1024: alignment)
     static constexpr int QROWS = 16 * WR, QHALF = 128 * QROWS;               // the tile's q, as HTILE: hi, lo
 };
 
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
     __shared__ int s_tok[64];                     // token row * H + q head (-1: none)
     __shared__ float s_f[64];                     // score factor of each row
     __shared__ int s_bad[4][2];                   // stage c's positions on bad pages, as a bit mask, at c % 4
-    __shared__ __align__(8) float s_fk[C::F16 ? 1 : C::PS];    // what undoes the scale of each K row of a stage (fp32)
+    __shared__ __align__(8) float s_fk[C::F32 ? C::PS : 1];    // what undoes the scale of each K row of a stage (fp32)
     __shared__ uint32_t s_max[4];                 // largest |V| of a stage (fp32), by warp
     __shared__ int s_flag;                        // V had values that are not finite behind the mask
     __shared__ volatile int s_abort;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         // lane each: a lane issues a box in some 90 cycles. Page ids are fetched a stage ahead; warp 0 also looks at
         // all of them (box i in lane i, and i + 32) for what to expect and what is bad.
         const int R = min(1 << a.page_log, C::PS), boxes = C::PS / R;
-        constexpr int KINDS = C::F16 ? D / 32 : 2;                 // tensors x halves
+        constexpr int KINDS = C::F16 ? D / 32 : C::P4 ? 4 : 2;     // tensors x halves, or x nibbles and scales
         int pages[2], every[2];
         auto page_of = [&](int st, int i) {
             const int p = k0 + st * C::PS + i * R;
@@ -202,6 +203,13 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 if ((unsigned)pages[h] < (unsigned)a.n_pages) {
                     const int item = (lane + 32 * h) * 4 + warp, i = item / KINDS, kind = item % KINDS;
                     const int y = (k0 + st * C::PS + i * R) & ((1 << a.page_log) - 1);
+                    if constexpr (C::P4) {
+                        const char *src = (kind & 1 ? a.v : a.k) + pages[h] * a.page_stride + kh * a.head_stride;
+                        const uint32_t to = dst + (kind & 1) * (C::STAGE / 2);
+                        if (kind < 2) bulk_load(to + i * R * (D / 2), src + y * (D / 2), R * (D / 2), bar);
+                        else bulk_load(to + C::PS * (D / 2) + i * R * (D / 16), src + (D / 2 << a.page_log) + y * (D / 16), R * (D / 16), bar);
+                        continue;
+                    }
                     const uint32_t to = dst + (kind & 1) * (C::STAGE / 2) + (C::F16 ? (kind >> 1) * C::HALF + i * R * 128 : i * R * C::ROW);
                     tma_load4(to, kind & 1 ? &mv : &mk, (kind >> 1) * 64, kh, y, pages[h], bar);
                 }
@@ -225,8 +233,9 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         }
 
         // ---- q: 8 lanes per row; each row scaled by a power of two into fp16's range (exact; undone in the score's factor)
-        // and split, into the stage slot that is filled last; from there as mma A fragments
-        unsigned char *qs = sm + (c0 + C::NS - 1) % C::NS * C::STAGE;
+        // and split, into the stage slot that is filled last (4 bits: where the first stage's K and V will be); from there as mma A
+        // fragments
+        unsigned char *qs = sm + (C::P4 ? C::CONV : (c0 + C::NS - 1) % C::NS * C::STAGE);
 #pragma unroll
         for (int i = 0; i < WR; i++) {
             const int r = (warp * WR + i) * 4 + (lane >> 3), tok = s_tok[r], t = tok < 0 ? 0 : tok / a.H;
@@ -313,6 +322,31 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     fence_async_smem();
                     __syncthreads();
                 }
+            } else if constexpr (C::P4) {
+                // 32 values with one scale at a time, 16 bytes, to fp16. A group's four pieces go out in an order that lets 8 lanes
+                // write to all banks (the halves of a row lie on the same ones).
+                constexpr int GR = D / 32, N = C::PS * GR / 128;   // groups per row, of K and of V per thread
+#pragma unroll
+                for (int i = 0; i < 2 * N; i++) {
+                    const int at = tid + 128 * (i % N), r = at / GR, g = at % GR, is_v = i / N;
+                    const unsigned char *src = raw + is_v * (C::STAGE / 2);
+                    uint4 w = *reinterpret_cast<const uint4 *>(src + at * 16);
+                    const __half2 d = __half2half2(reinterpret_cast<const __half *>(src + C::PS * (D / 2))[at]), m24 = __hmul2(d, __float2half2_rn(-24.0f));
+                    const int turn = g & 2;
+                    if (turn) w = make_uint4(w.z, w.w, w.x, w.y);
+                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                    const int p = base + r;
+                    const bool look = masked && is_v && (p < first || p > seen);    // behind the mask a weight is 0, but 0 * inf is not
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint4 y = q4_dequant(ww[k], d, m24);
+                        if (look && drop_nonfinite((const __half *)nullptr, y) && p >= first && p < k1) s_flag = 1;
+                        *reinterpret_cast<uint4 *>(sm + C::CONV + is_v * C::HTILE + C::piece(r, 4 * g + (k ^ turn))) = y;
+                    }
+                }
+                __syncthreads();
+                kb = sm0 + C::CONV;
+                vb = kb + C::HTILE;
             } else {
                 // hi and lo: K by rows, each with a scale of its own (undone in its scores), V with the largest scale so
                 // far of what somebody sees (o is in its units)
@@ -412,7 +446,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     mma_f16(s[2 * i + 1], qh[ks], kf[2], kf[3]);
                     mma_f16(s2[2 * i], ql[ks], kf[0], kf[1]);
                     mma_f16(s2[2 * i + 1], ql[ks], kf[2], kf[3]);
-                    if constexpr (!C::F16) {
+                    if constexpr (C::F32) {
                         ldsm4(kf, at + C::HTILE);
                         mma_f16(s2[2 * i], qh[ks], kf[0], kf[1]);
                         mma_f16(s2[2 * i + 1], qh[ks], kf[2], kf[3]);
@@ -423,7 +457,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
 #pragma unroll
             for (int i = 0; i < C::NT; i++) {
                 const int r = wk * C::KW + i * 8 + tq * 2, p = base + r;
-                const float2 fk = C::F16 ? make_float2(1.0f, 1.0f) : *reinterpret_cast<const float2 *>(s_fk + (C::F16 ? 0 : r));
+                const float2 fk = C::F32 ? *reinterpret_cast<const float2 *>(s_fk + (C::F32 ? r : 0)) : make_float2(1.0f, 1.0f);
                 s[i][0] = (s[i][0] + s2[i][0]) * (f0 * fk.x), s[i][1] = (s[i][1] + s2[i][1]) * (f0 * fk.y);
                 s[i][2] = (s[i][2] + s2[i][2]) * (f1 * fk.x), s[i][3] = (s[i][3] + s2[i][3]) * (f1 * fk.y);
                 if (masked) {
@@ -470,7 +504,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 split_h2(s[2 * kk + 1][0], s[2 * kk + 1][1], ph[kk][2], pl[kk][2]);
                 split_h2(s[2 * kk + 1][2], s[2 * kk + 1][3], ph[kk][3], pl[kk][3]);
             }
-            constexpr int JS = C::F16 ? 2 : 1;    // 16-value columns at a time
+            constexpr int JS = C::F32 ? 1 : 2;    // 16-value columns at a time
 #pragma unroll
             for (int j0 = 0; j0 < C::DW / 16; j0 += JS) {
                 float t[2 * JS][4];
@@ -487,7 +521,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     }
 #pragma unroll
                     for (int j = 0; j < 2 * JS; j++) mma_f16(t[j], ph[kk], vf[j / 2][j % 2 * 2], vf[j / 2][j % 2 * 2 + 1]);
-                    if constexpr (!C::F16) {
+                    if constexpr (C::F32) {
 #pragma unroll
                         for (int j = 0; j < JS; j++) ldsm4t(vf[j], vb + C::piece(r, c + 2 * j) + C::HTILE);
 #pragma unroll
@@ -509,7 +543,7 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
         l1 += __shfl_xor_sync(kFull, l1, 1);
         l0 += __shfl_xor_sync(kFull, l0, 2);
         l1 += __shfl_xor_sync(kFull, l1, 2);
-        if constexpr (!C::F16) {                  // out of V's scale
+        if constexpr (C::F32) {                   // out of V's scale
             const float d = pow2_bits(254u - scale_up(v_exp));
 #pragma unroll
             for (int i = 0; i < C::DW / 8; i++) o[i][0] *= d, o[i][1] *= d, o[i][2] *= d, o[i][3] *= d;
@@ -523,12 +557,16 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                 if ((p - k0) % C::PS / C::KW != wk) continue;
                 const int64_t at = paged_at(a, table, p);
                 if (at < 0) continue;
-                const KT *vr = reinterpret_cast<const KT *>(a.v + at + kh * a.head_stride);
+                const char *vr = a.v + at + kh * a.head_stride;
+                auto value = [&](int x) {
+                    if constexpr (C::P4) return q4_ld<D>(vr, q4_scales<D>(a, p & ((1 << a.page_log) - 1)), x);
+                    else return kv_ld(reinterpret_cast<const KT *>(vr) + x);
+                };
 #pragma unroll
                 for (int i = 0; i < C::DW / 8; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const float v = kv_ld(vr + dim(i, j));
+                        const float v = value(dim(i, j));
                         if (!isfinite(v) && p <= (j < 2 ? pos0 : pos1)) o[i][j] += v;
                     }
             }
@@ -626,7 +664,11 @@ __device__ __noinline__ bool plain_row(const PagedAttn &A, unsigned row) {
         if (at < 0) continue;
         const int64_t head = at + h / a.G * a.head_stride;
         float k[J], v[J], s = 0.0f;
-        if (A.f16) {
+        if (A.type == QMS_T_Q4_0) {
+            const int64_t sc = q4_scales<D>(a, p & ((1 << a.page_log) - 1));
+#pragma unroll
+            for (int j = 0; j < J; j++) k[j] = q4_ld<D>(a.k + head, sc, lane * J + j), v[j] = q4_ld<D>(a.v + head, sc, lane * J + j);
+        } else if (A.type == QMS_T_F16) {
             fetch_part(reinterpret_cast<const __half *>(a.k + head) + lane * J, k);
             fetch_part(reinterpret_cast<const __half *>(a.v + head) + lane * J, v);
         } else {
@@ -772,6 +814,7 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
 // 37.7); 3.1 31.3, 35.1 (45.7, 46.5); 6.3 39.8, 43.5 (65.8, 58.2); 16.8 69, 63 (139, 96).
 static int row_groups(int type, int page_log, int64_t rows, int64_t positions, bool shared) {
     const bool f16 = type == QMS_T_F16;
+    if (type == QMS_T_Q4_0) return rows > 64 && (rows + 63) / 64 * 64 * positions > 2600000 ? kPaWideQ4 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
     if (rows > 64 && (!f16 || page_log >= 3) && (rows + 63) / 64 * 64 * positions > (f16 || shared ? 2600000 : 1200000))
         return !f16 ? kPaWideF32 : rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
@@ -781,7 +824,7 @@ static int tile_positions(int type, int wr) { return wr > 0 ? pa_stage(type) : w
 
 // Positions that one unit of k_paged_wide may cover, by the additions into an accumulator (its CUT): fp16 144 of them, 2 per 16
 // positions; fp32 192, 3 per 16, by two streams. (kPaWidePair takes its own out in time; k_paged_attn adds up single stages.)
-static int most_positions(int wr) { return wr == kPaWideSplit ? 2304 : wr == kPaWideF32 ? 2048 : 1 << 30; }
+static int most_positions(int wr) { return wr == kPaWideSplit || wr == kPaWideQ4 ? 2304 : wr == kPaWideF32 ? 2048 : 1 << 30; }
 
 // Chunks of `len` positions for `tiles` units of rows: the number of chunks with the least estimated time, from waves
 // of resident CTAs, stages of `stage` positions (us each, us_unit once per unit) and 1 KB of partial results
@@ -804,7 +847,7 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, dou
     const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
-    const int per_sm = type == QMS_T_F16 && wr == 1 ? 3 : 2;
+    const int per_sm = type != QMS_T_F32 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * per_sm * share)), wr == 4 ? 2.0 : 1.2, 4.0, most);
 }
 
@@ -884,8 +927,13 @@ static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t 
     int rc = allow_smem(done, k_paged_attn<D, KT, WR>, C::SMEM);
     if (rc) return rc;
     CUtensorMap mk, mv;
-    rc = paged_map(A.a, D, C::F16, C::PS, A.a.k, &mk);
-    if (rc || (rc = paged_map(A.a, D, C::F16, C::PS, A.a.v, &mv))) return rc;
+    if constexpr (C::P4) {
+        memset(&mk, 0, sizeof mk);                // (its copies need none)
+        mv = mk;
+    } else {
+        rc = paged_map(A.a, D, C::F16, C::PS, A.a.k, &mk);
+        if (rc || (rc = paged_map(A.a, D, C::F16, C::PS, A.a.v, &mv))) return rc;
+    }
     const int grid = (int)std::min<int64_t>(units, 148 * 8);
     QMS_CK(launch_pdl(k_paged_attn<D, KT, WR>, dim3(grid), dim3(128), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
@@ -919,13 +967,14 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     A.ldq = ldq;
     A.ldo = ldo;
     A.scale2 = scale * 1.4426950408889634f;
-    A.f16 = type == QMS_T_F16;
+    A.type = type;
     A.part_o = (float *)ws;
     // (32-bit run arithmetic)
     QMS_REQUIRE((int64_t)p.tiles_p * a.Hk * ((a.prefix + 63) / 64) < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     A.part_ml = (float2 *)((char *)ws + al256((int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H * D * 4));
     int rc;
     if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, s) : launch_attn<64, __half>(A, s);
+    else if (type == QMS_T_Q4_0) rc = D == 128 ? launch_attn<128, Q4>(A, s) : launch_attn<64, Q4>(A, s);
     else rc = D == 128 ? launch_attn<128, float>(A, s) : launch_attn<64, float>(A, s);
     if (rc) return rc;
     // Four warps per row while there are few rows, or many slots for each. Four against one in us: 320 rows (5 tokens, 2000

@@ -43,22 +43,23 @@
 
 namespace qms {
 
-enum { PAIR, SPLIT, F32 };
+enum { PAIR, SPLIT, F32, NIB };
 constexpr uint32_t kWSpin = 1u << 22;
 constexpr float kWLow = 8.0f, kWHigh = 15.0f;       // a new base is 2^8 below the maximum; weights stay below 2^15
 
 template <int D, int MODE>
 struct WideCfg {
+    static constexpr bool CONV = MODE == F32 || MODE == NIB;    // K and V are written by four warps, from stages
     static constexpr int TP = MODE == F32 ? 64 : 128, ROWS = MODE == PAIR ? 256 : 128;     // positions per tile, rows per unit
-    static constexpr int THREADS = MODE == F32 ? 480 : 384, REGS = MODE == F32 ? 128 : 168;    // (4, 3 warps per scheduler)
-    static constexpr int TMA_WARP = MODE == F32 ? 12 : 8, MMA_WARP = MODE == F32 ? 13 : 10;
+    static constexpr int THREADS = CONV ? 480 : 384, REGS = CONV ? 128 : 168;    // (4, 3 warps per scheduler)
+    static constexpr int TMA_WARP = CONV ? 12 : 8, MMA_WARP = CONV ? 13 : 10;
     static constexpr int PIECE = MODE == PAIR ? 8 : 1 << 30;    // tiles that O adds up before it is taken out
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t QHALF = 128 * 128, QTILE = HALVES * QHALF;     // one term of 128 rows of Q
     static constexpr uint32_t HALF = TP * 128, TILE = HALVES * HALF;         // one term of a K or V tile
     static constexpr uint32_t SLOT = (MODE == F32 ? 2 : 1) * TILE;
     static constexpr int SLOTS = MODE == SPLIT ? 4 : 3;
-    static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT, STAGED = MODE == F32 ? TP * D * 4 : 0;
+    static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT, STAGED = MODE == F32 ? TP * D * 4 : MODE == NIB ? TP * q4_row(D) : 0;
     // then: bad-page masks [8][4]; scales of K and V tiles [2][4], maxima [2][4]; a stream's (B, l, V scale) by row;
     // barriers; flags
     static constexpr uint32_t BAD = STAGE + 2 * STAGED, UP = BAD + 128, JOIN = UP + 64,
@@ -253,9 +254,9 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
     }
     if (tid == 0) {
         for (int i = 0; i < 4; i++) {
-            mbar_init(&full[i], MODE == F32 ? 128 : 1);
+            mbar_init(&full[i], C::CONV ? 128 : 1);
             mbar_init(&empty[i], MODE == PAIR ? 2 : 1);
-            mbar_init(&landed[i], MODE == F32 && i >= 2 ? 4 : 1);
+            mbar_init(&landed[i], C::CONV && i >= 2 ? 4 : 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 128);
@@ -296,7 +297,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
     // the streams alternate over all tiles of the CTA (`before` those of earlier units), not from the start of each
     // unit: the one ring keeps a stream's barriers at most a phase ahead of who waits for them only if its tiles
     // never follow one another.
-    auto first_of = [&](int i, uint32_t before) { return MODE == F32 ? (int)((i ^ before) & 1) : MODE == SPLIT ? i : 0; };
+    auto first_of = [&](int i, uint32_t before) { return C::CONV ? (int)((i ^ before) & 1) : MODE == SPLIT ? i : 0; };
     auto tiles_of = [&](int i, uint32_t before) {
         return MODE == PAIR ? (w.rows - w.r0 > 128 * i ? w.nt : 0) : (w.nt + 1 - first_of(i, before)) / 2;
     };
@@ -610,10 +611,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     for (int p = kp; p < past; p++) {
                         const int64_t at = paged_at(a, a.table + (own ? (int64_t)w.b * a.table_stride : 0), p);
                         if (at < 0) continue;
-                        const KT *vr = reinterpret_cast<const KT *>(a.v + at + w.kh * a.head_stride) + 32 * c;
+                        const char *vr = a.v + at + w.kh * a.head_stride;
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
-                            const float v = kv_ld(vr + e);
+                            float v;
+                            if constexpr (MODE == NIB) v = q4_ld<D>(vr, q4_scales<D>(a, p & ((1 << a.page_log) - 1)), 32 * c + e);
+                            else v = kv_ld(reinterpret_cast<const KT *>(vr) + 32 * c + e);
                             if (!isfinite(v)) o[e] = __float_as_uint(__uint_as_float(o[e]) + v);
                         }
                     }
@@ -663,7 +666,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             }
         }
         tmem_wait_st();
-    } else if (warp == C::TMA_WARP || (MODE != F32 && warp == 9)) {
+    } else if (warp == C::TMA_WARP || (!C::CONV && warp == 9)) {
         // ---- K and V, in the order of their use: K, V of each position tile, or (SPLIT) K, K, V, V of two. One warp
         // issues them; V tiles with rows that not every row sees (or that were not loaded) land on a barrier of their
         // own and are passed on by the other (F32: all go to the stages, and the converting warps look at them).
@@ -696,7 +699,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     uint32_t any_missing = missing[0];
                     if constexpr (PER > 1) any_missing |= missing[PER - 1];
                     const int seen = min(w.lo, w.k1 - 1);
-                    const bool scan = MODE != F32 && is_v && (base + C::TP - 1 > seen || base < w.kmin || any_missing);
+                    const bool scan = !C::CONV && is_v && (base + C::TP - 1 > seen || base < w.kmin || any_missing);
                     if (warp == C::TMA_WARP) {
                         if (!is_v && lane < C::TP / 32) {     // bits of the tile's positions on bad pages
                             uint32_t bits = 0;
@@ -709,7 +712,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                         }
                         __syncwarp();
                         uint64_t *bar;
-                        if constexpr (MODE == F32) {
+                        if constexpr (C::CONV) {
                             if (n >= 2) ok = __all_sync(kFull, sy.wait(&landed[2 + (n & 1)], (n / 2 - 1) & 1));
                             bar = &landed[n & 1];
                         } else {
@@ -717,13 +720,18 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                             bar = scan ? &landed[slot] : &full[slot];
                         }
                         if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(bar, have * (uint32_t)(R * D * (MODE == F32 ? 4 : 2)));
+                        if (lane == 0) mbar_arrive_expect_tx(bar, have * (uint32_t)(R * (MODE == NIB ? q4_row(D) : D * (MODE == F32 ? 4 : 2))));
                         __syncwarp();
 #pragma unroll
                         for (int h = 0; h < PER; h++) {
                             const int i = lane + 32 * h, y = (base + i * R) & ((1 << a.page_log) - 1);
                             if (page[h] < 0) continue;
-                            if constexpr (MODE == F32)
+                            if constexpr (MODE == NIB) {
+                                const char *src = (is_v ? a.v : a.k) + page[h] * a.page_stride + w.kh * a.head_stride;
+                                const uint32_t to = sm0 + C::STAGE + (n & 1) * C::STAGED;
+                                bulk_load(to + i * R * (D / 2), src + y * (D / 2), R * (D / 2), bar);
+                                bulk_load(to + C::TP * (D / 2) + i * R * (D / 16), src + (D / 2 << a.page_log) + y * (D / 16), R * (D / 16), bar);
+                            } else if constexpr (MODE == F32)
                                 tma_load4(sm0 + C::STAGE + (n & 1) * C::STAGED + i * R * (D * 4), is_v ? &mv : &mk, 0, w.kh, y, page[h], bar);
                             else
 #pragma unroll
@@ -751,6 +759,51 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                 }
                 t += m;
             }
+        }
+    } else if (MODE == NIB && warp < 12) {
+        // ---- nibbles from the stages to fp16 tiles, 32 values with one scale at a time: what the unit holds, V that is not finite
+        // where some row does not see it set aside. A group's pieces go out in an order that lets 8 lanes write to all banks.
+        constexpr int GR = D / 32, N = C::TP * GR / 128;
+        const int ct = tid - 256;
+        uint32_t c = 0, t = 0;                    // loads, tiles so far
+        bool ok = true;
+        while (work.next(w)) {                    // (after a failed wait: the barriers, no work)
+            const int seen0 = min(w.lo, w.k1 - 1);
+            for (int j = 0; j < w.nt; j++, t++)
+#pragma unroll 1
+                for (int is_v = 0; is_v < 2; is_v++, c++) {
+                    const int base = w.k0 + j * C::TP;
+                    const unsigned char *src = sm + C::STAGE + (c & 1) * C::STAGED;
+                    ok = __all_sync(kFull, ok && sy.wait(&landed[c & 1], c / 2 & 1));
+                    const uint32_t *bad = s_bad + (t & 7) * 4;
+                    const int seen = bad[0] | bad[1] | bad[2] | bad[3] ? -1 : seen0;
+                    const bool look = base + C::TP - 1 > seen || base < w.kmin;
+                    ok = __all_sync(kFull, ok && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
+                    if (ok) {
+                        unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
+#pragma unroll
+                        for (int i = 0; i < N; i++) {
+                            const int at = ct + 128 * i, r = at / GR, g = at % GR, turn = g & 2, p = base + r;
+                            uint4 x = *reinterpret_cast<const uint4 *>(src + at * 16);
+                            const __half2 d = __half2half2(reinterpret_cast<const __half *>(src + C::TP * (D / 2))[at]), m24 = __hmul2(d, __float2half2_rn(-24.0f));
+                            if (turn) x = make_uint4(x.z, x.w, x.x, x.y);
+                            const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
+                            const bool in = !look || (p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1)), part = look && is_v && p > seen;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                uint4 y = q4_dequant(xx[k], d, m24);
+                                if (!in) y = make_uint4(0, 0, 0, 0);
+                                if (part && drop_nonfinite((const __half *)nullptr, y)) *s_flag = 1;
+                                const int q = 4 * g + (k ^ turn);
+                                *reinterpret_cast<uint4 *>(dst + (q >> 3) * C::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4)) = y;
+                            }
+                        }
+                    }
+                    fence_async_smem();
+                    mbar_arrive(&full[2 * is_v + (t & 1)]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&landed[2 + (c & 1)]);
+                }
         }
     } else if (MODE == F32 && warp < 12) {
         // ---- fp32 rows from the stages into hi and lo tiles, under one scale: K under the tile's, V under the largest so
@@ -834,7 +887,7 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
         if (lane == 0 && i < 2) {
             constexpr uint32_t id_s = idesc_f16(C::TP, false), id_o = idesc_f16(D, true);
             constexpr int TERMS = MODE == F32 ? 3 : 2;          // hi hi, lo hi, (fp32) hi lo
-            uint32_t c = 0, nf = 0, nq = 0, np = 0;             // loads of the ring so far; phases of (F32) full, of q_full, p_full
+            uint32_t c = 0, nf = 0, nq = 0, np = 0;             // loads of the ring so far; phases of (CONV) full, of q_full, p_full
             bool ok = true;
             auto score = [&](uint32_t n) {                     // S_i = Q_i K^T
                 const uint32_t k = sm0 + C::RING + C::slot(i, n) * C::SLOT, q = sm0 + (MODE == PAIR ? i * 2 * C::QTILE : 0);
@@ -862,16 +915,16 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
             };
             auto unlock = [&]() { *(volatile int *)s_lock = 0; };
             // K, V of this stream's tile at load n (K) or n + 1 of the ring; nf: tiles of the stream so far
-            auto k_bar = [&](uint32_t n) { return MODE == F32 ? &full[i] : &full[C::slot(i, n)]; };
-            auto v_bar = [&](uint32_t n) { return MODE == F32 ? &full[2 + i] : &full[C::slot(i, n)]; };
-            constexpr uint32_t NEXT = MODE == F32 ? 4 : 2;      // loads to the stream's next tile
+            auto k_bar = [&](uint32_t n) { return C::CONV ? &full[i] : &full[C::slot(i, n)]; };
+            auto v_bar = [&](uint32_t n) { return C::CONV ? &full[2 + i] : &full[C::slot(i, n)]; };
+            constexpr uint32_t NEXT = C::CONV ? 4 : 2;      // loads to the stream's next tile
             while (ok && work.next(w)) {
                 const int nt = tiles_of(i, c / 2);
                 const uint32_t c1 = c + (MODE == SPLIT ? 2 * nt : 2 * w.nt);
-                if (MODE == F32) c += 2 * first_of(i, c / 2);
+                if (C::CONV) c += 2 * first_of(i, c / 2);
                 if (MODE != PAIR || nt > 0) {
                     ok = sy.wait(&q_full[MODE == PAIR ? i : 0], nq++ & 1);
-                    if (ok && nt > 0 && (ok = sy.wait(k_bar(c), MODE == F32 ? nf & 1 : C::phase(c)))) {
+                    if (ok && nt > 0 && (ok = sy.wait(k_bar(c), C::CONV ? nf & 1 : C::phase(c)))) {
                         tc_fence_after();
                         lock();
                         score(c);
@@ -881,12 +934,12 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     }
                     for (int j = 0; ok && j < nt; j++, c += NEXT, nf++) {
                         const bool more = j + 1 < nt;
-                        if (!(ok = sy.wait(v_bar(c + 1), MODE == F32 ? nf & 1 : C::phase(c + 1)) && sy.wait(&p_full[i], np++ & 1))) break;
+                        if (!(ok = sy.wait(v_bar(c + 1), C::CONV ? nf & 1 : C::phase(c + 1)) && sy.wait(&p_full[i], np++ & 1))) break;
                         tc_fence_after();
                         lock();
                         weigh(c + 1, MODE == PAIR ? j % C::PIECE == 0 : j == 0);
                         if (more) {
-                            const uint32_t ph = MODE == F32 ? (nf + 1) & 1 : C::phase(c + NEXT);
+                            const uint32_t ph = C::CONV ? (nf + 1) & 1 : C::phase(c + NEXT);
                             if (!mbar_test_wait(k_bar(c + NEXT), ph)) {      // K is late: not at the other's cost
                                 unlock();
                                 umma_commit(&empty[C::slot(i, c + 1)]);
@@ -938,8 +991,13 @@ static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) 
     int rc = allow_smem(done, k_paged_wide<D, MODE>, C::SMEM);
     if (rc) return rc;
     CUtensorMap mk, mv;
-    rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.k, &mk);
-    if (rc || (rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.v, &mv))) return rc;
+    if constexpr (MODE == NIB) {
+        memset(&mk, 0, sizeof mk);                // (its copies need none)
+        mv = mk;
+    } else {
+        rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.k, &mk);
+        if (rc || (rc = paged_map(A.a, D, MODE != F32, C::TP, A.a.v, &mv))) return rc;
+    }
     const int grid = (int)(units < 148 ? units : 148);
     QMS_CK(launch_pdl(k_paged_wide<D, MODE>, dim3(grid), dim3(C::THREADS), C::SMEM, s, A, mk, mv, own, last));
     return QMS_CUDA_OK;
@@ -947,6 +1005,7 @@ static int launch_wide(const PagedAttn &A, bool own, bool last, cudaStream_t s) 
 
 int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s) {
     const int kind = own ? A.p.wr_s : A.p.wr_p;
+    if (kind == kPaWideQ4) return D == 128 ? launch_wide<128, NIB>(A, own, last, s) : launch_wide<64, NIB>(A, own, last, s);
     if (D == 128)
         return kind == kPaWidePair ? launch_wide<128, PAIR>(A, own, last, s) : kind == kPaWideSplit ? launch_wide<128, SPLIT>(A, own, last, s)
                                                                                                   : launch_wide<128, F32>(A, own, last, s);
