@@ -260,6 +260,25 @@ int qms_cuda_prompt_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *b
                            const float *q_norm, const float *k_norm, float eps, const float *rope_cos, const float *rope_sin,
                            int n_rope, int type, void *rows, int64_t ldrows, int *err, void *stream);
 
+/* Rows of heads: the values of (token, head) start at data + token * tok_stride + head * head_stride elements, head_dim
+ * contiguous ones. data and strides are multiples of 16 bytes. */
+typedef struct {
+    void *data;
+    int64_t tok_stride, head_stride;
+} QmsCudaHeads;
+
+/* Causal grouped-query attention within whole prompts, packed one after another: prompt b's tokens are rows q_start[b] ..
+ * q_start[b + 1] - 1, at most max_q of them (of the batch, n_seq, n_tok, q_start and max_q are looked at), out[t][h] = sum over the
+ * prompt's tokens j <= t of softmax_j(scale * q[t][h] . k[j][h / (n_head / n_head_kv)]) v[j]. q, k, v of type QMS_T_F16 or
+ * QMS_CUDA_T_BF16, out of that type or QMS_T_F32; out may be q itself, of its type and strides, and overlaps nothing else. head_dim 64
+ * or 128, up to 128 q heads per kv head, scale > 0. Rows of no prompt are left as they were; a prompt whose rows make no sense sets
+ * QMS_PAGED_ELEN and is left out. What a row does not see has no effect on it, whatever its bits; a V value that it sees and that is
+ * not finite makes that element of the row not finite. Precision: q, k, v are exact, a weight is rounded to the type once (as
+ * the output is), scores and sums are fp32. */
+int qms_cuda_prompt_attention(const QmsCudaPagedBatch *batch, int type, const QmsCudaHeads *q, const QmsCudaHeads *k, const QmsCudaHeads *v,
+                              int n_head, int n_head_kv, int head_dim, float scale, int out_type, const QmsCudaHeads *out, int *err,
+                              void *stream);
+
 /* What a pool holds: fp32 [n_pages][page_size][n_head_kv][head_dim] of K and of V (16-byte aligned), pages in use or not. */
 int qms_cuda_paged_values(const QmsCudaPages *pages, float *k, float *v, void *stream);
 

@@ -14,6 +14,7 @@ and adds the operators of batched serving behind a shared prompt, with drafted t
     KvPages, PagedBatch          a paged KV cache, and a batch of new tokens over it
     paged_append(...)            QK-norm, rotation and the cache append in one pass (pages of fp32, fp16 or 4 bits)
     prompt_append(...)           the same for whole prompts, with the heads' rows in 16 bits
+    prompt_attention(...)        causal attention within whole prompts, packed, in 16 bits
     paged_attention(...)         causal attention over the pages, a shared prompt read once
     probs(logits, temp)          probabilities of logits rows
     logprobs(logits, ids, top)   log probabilities of given tokens, the entropy, the likeliest tokens
@@ -71,6 +72,10 @@ class PagedBatchDesc(C.Structure):
     _fields_ = [("n_seq", C.c_int), ("n_tok", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
                 ("table", C.c_void_p), ("table_stride", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int),
                 ("prefix_len", C.c_int)]
+
+
+class HeadsDesc(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("tok_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 class LayerDesc(C.Structure):
@@ -138,6 +143,8 @@ def lib() -> C.CDLL:
     pg, pb, f32 = C.POINTER(PagesDesc), C.POINTER(PagedBatchDesc), C.c_float
     L.qms_cuda_paged_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, vp, i64, vp, vp]
     L.qms_cuda_prompt_append.argtypes = [pg, pb, vp, i64, i32, vp, vp, f32, vp, vp, i32, i32, vp, i64, vp, vp]
+    hd = C.POINTER(HeadsDesc)
+    L.qms_cuda_prompt_attention.argtypes = [pb, i32, hd, hd, hd, i32, i32, i32, f32, i32, hd, vp, vp]
     L.qms_cuda_paged_values.argtypes = [pg, vp, vp, vp]
     L.qms_cuda_paged_attention_ws.argtypes = [pg, pb, i32]
     L.qms_cuda_paged_attention_ws.restype = i64
@@ -707,6 +714,45 @@ def prompt_append(pages: KvPages | None, batch: PagedBatch, qkv, n_head: int, q_
     if rc:
         check(rc)
     return rows
+
+
+def _heads(t, n_tok: int, what: str):
+    """A CUDA tensor [tokens][heads][head_dim] as QmsCudaHeads, the last dimension contiguous."""
+    if t.dim() != 3 or t.shape[0] < n_tok or (t.stride(2) != 1 and t.shape[2] > 1) or not t.is_cuda:
+        raise ValueError(f"{what}: a CUDA tensor [{n_tok} tokens][heads][head_dim] with contiguous values is needed, got {tuple(t.shape)} on "
+                         f"{t.device}, strides {tuple(t.stride())}")
+    n, h, d = t.shape
+    st, sh = t.stride(0), t.stride(1)
+    # (the stride of a dimension of one has no meaning)
+    return HeadsDesc(t.data_ptr(), st if n > 1 else max(h * d, d), sh if h > 1 else d)
+
+
+def prompt_attention(batch: PagedBatch, q, k, v, scale: float | None = None, out=None, out_dtype=None, stream=None):
+    """Causal attention within whole prompts, packed one after another (qms_cuda_prompt_attention): batch = PagedBatch.prompts(...), or
+    the one that prompt_append took; q [n_tok][n_head][head_dim], k, v [n_tok][n_head_kv][head_dim] of float16 or bfloat16, such as slices
+    of prompt_append's rows; scale defaults to 1 / sqrt(head_dim). Returns [n_tok][n_head][head_dim] of q's type, or out_dtype =
+    torch.float32; out may be q. Rows behind the last prompt are left as they were."""
+    torch = _torch()
+    n, H, D = q.shape
+    typ = {torch.float16: T_F16, torch.bfloat16: T_BF16}.get(q.dtype)
+    if typ is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"prompt_attention: float16 or bfloat16, one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape != v.shape or k.dim() != 3 or k.shape[2] != D:
+        raise ValueError(f"prompt_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if out is None:
+        out = _empty((batch.n_tok, H, D), out_dtype or q.dtype, q.device, stream)
+    otyp = typ if out.dtype == q.dtype else T_F32 if out.dtype == torch.float32 else None
+    if otyp is None or out.shape[1:] != q.shape[1:]:
+        raise ValueError(f"prompt_attention: out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
+    _one_device("prompt_attention", q, k, v, out, batch.err)
+    T = batch.n_tok
+    with _device_of(q):
+        rc = lib().qms_cuda_prompt_attention(batch._ref, typ, _heads(q, T, "q"), _heads(k, T, "k"), _heads(v, T, "v"), H, k.shape[1], D,
+                                             D ** -0.5 if scale is None else scale, otyp, _heads(out, T, "out"), batch._err,
+                                             batch._use(stream, q))
+    if rc:
+        check(rc)
+    return out
 
 
 def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: float | None = None, out=None, stream=None):

@@ -210,6 +210,31 @@ struct PagedAttn {
     float2 *part_ml;
 };
 
+constexpr uint32_t kWSpin = 1u << 22;
+
+// Bounded wait for a phase of a barrier; a wait that gives up ends the CTA's work (flag) and is reported.
+struct WideSync {
+    volatile int *abort;
+    const Paged *a;
+    __device__ bool wait(uint64_t *bar, uint32_t parity) const {
+        for (uint32_t n = 0; !mbar_try_wait(bar, parity); n++) {
+            if (*abort) return false;
+            if (n == kWSpin) {
+                *abort = 1;
+                paged_err(*a, QMS_PAGED_ETIMEOUT);
+                return false;
+            }
+            if (n > 64) __nanosleep(32);
+        }
+        return true;
+    }
+};
+
+// The driver's cuTensorMapEncodeTiled, looked up once.
+typedef CUresult (*TensorEncode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int tensor_encode(TensorEncode *encode);                                                   // qms_paged_attn.cu
+
 // The pool as a tensor [page][position][head][value], in boxes of up to `rows` positions of a page: 64 fp16 values, 128-byte
 // swizzled, or a whole fp32 row.
 int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map);

@@ -893,18 +893,23 @@ int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
     return al256(n * D * 4) + al256(n * 8);
 }
 
-int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map) {
-    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static std::atomic<Encode> known{nullptr};
-    Encode encode = known.load();
-    if (!encode) {
+int tensor_encode(TensorEncode *encode) {
+    static std::atomic<TensorEncode> known{nullptr};
+    *encode = known.load();
+    if (!*encode) {
         cudaDriverEntryPointQueryResult found;
         void *f = nullptr;
         QMS_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found));
-        QMS_REQUIRE(f, QMS_CUDA_ECUDA, "paged_attention: the driver has no cuTensorMapEncodeTiled");
-        known = encode = (Encode)f;
+        QMS_REQUIRE(f, QMS_CUDA_ECUDA, "attention: the driver has no cuTensorMapEncodeTiled");
+        known = *encode = (TensorEncode)f;
     }
+    return QMS_CUDA_OK;
+}
+
+int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUtensorMap *map) {
+    TensorEncode encode;
+    const int got = tensor_encode(&encode);
+    if (got) return got;
     const cuuint64_t ps = 1ull << a.page_log, row = (cuuint64_t)D * (f16 ? 2 : 4);
     const cuuint64_t dim[4] = {(cuuint64_t)D, (cuuint64_t)a.Hk, ps, (cuuint64_t)a.n_pages};
     // (the stride of a dimension of one has no meaning, and 0 none that the encoder takes)

@@ -1,4 +1,4 @@
-// qms_tcgen05.cuh - tcgen05 helpers shared by the tensor-core kernels (qms_moe_mma.cu, qms_paged_wide.cu).
+// qms_tcgen05.cuh - tcgen05 helpers shared by the tensor-core kernels (qms_moe_mma.cu, qms_paged_wide.cu, qms_prompt.cu).
 #pragma once
 
 #include "qms_async.cuh"
@@ -49,5 +49,62 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[C]) {
                      : "r"(taddr));
     }
 }
+
+// ---- pieces of the attention kernels ----
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) { return umma_desc(saddr, lbo, sbo) | (2ull << 61); }
+
+// D[tmem] (+)= A B^T, fp16 in, fp32 out: A from shared memory / from TMEM
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+// M 128 x N, f16 x f16 -> f32, A K-major, B K-major or MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(int N, bool b_mn) {
+    return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// The loads into r are complete, and no use of r may move before this.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Lane r of 8 holds the 16-byte pieces 0 .. 7 of row r; then lane p holds piece p of the rows 0 .. 7.
+__device__ __forceinline__ void transpose8(uint32_t (&v)[32], int lane) {
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) {
+        const bool up = lane & s;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (!(k & s))
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t &x = v[4 * k + e], &y = v[4 * (k + s) + e];
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? x : y, s);
+                    x = up ? got : x;
+                    y = up ? y : got;
+                }
+    }
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 }  // namespace qms
