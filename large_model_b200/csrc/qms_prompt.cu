@@ -8,9 +8,10 @@
 //   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128, K = head_dim, N the tile's positions (rounded up to 16)
 //   softmax     one thread per row: base-2 exponents, the running base B and sum l in fp32; the weights 2^(s f - B), rounded to the
 //               type once, go back over S. (The rounding of a weight is the type's half step of itself, as the output's own rounding
-//               is; l adds up what was not rounded.)
+//               is; l adds up what was rounded, so that rows of few positions hardly have it.)
 //   O += P V    P from TMEM, V as it lies in shared memory (MN-major), in fp32 over the whole unit
-// B is a whole number and stays until a score lies 2^15 above it, so that the maximum needs no pass of its own.
+// B is a whole number and stays until a score lies 2^15 above it. A thread holds its row's 128 scores in registers: one look at their
+// maximum, one vote, and then nothing that the exponentials wait for.
 #include <cuda_bf16.h>
 #include <math.h>
 #include <string.h>
@@ -24,6 +25,7 @@
 namespace qms {
 
 constexpr float kPrLow = 8.0f, kPrHigh = 15.0f;     // a new base is 2^8 below the maximum; weights stay below 2^15
+constexpr int kPrRegs = 216, kPrRegsOther = 64;     // of 168 each at launch: 256 x 216 + 128 x 64 <= 384 x 168
 
 struct PromptAttn {
     Paged a;                         // q_start, n_seq, n_tok, max_q, H, Hk, G, err
@@ -37,11 +39,13 @@ struct PromptAttn {
 
 template <int D>
 struct PrCfg {
-    static constexpr int THREADS = 384, TMA_WARP = 8, SCAN_WARP = 9, MMA_WARP = 10;
+    static constexpr int THREADS = 384, TMA_WARP = 8, SCAN_WARP = 9, MMA_WARP = 10, UNIT_WARP = 11;
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t HALF = 128 * 128, TILE = HALVES * HALF;
     static constexpr uint32_t SLOTS = D == 128 ? 5 : 8;
-    static constexpr uint32_t RING = 2 * TILE, BARS = RING + SLOTS * TILE, SMEM = BARS + (3 * SLOTS + 11) * 8 + 32;
+    // then: the unit at hand and the answer of who asked for the next; barriers; a number for each row and half
+    static constexpr uint32_t RING = 2 * TILE, UNIT = RING + SLOTS * TILE, BARS = UNIT + 32, SUMS = BARS + (3 * SLOTS + 14) * 8 + 16,
+                              SMEM = SUMS + 2 * 2 * 128 * 4;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
 };
 
@@ -49,10 +53,10 @@ struct PrCfg {
 template <uint32_t SLOTS>
 struct RingAt {
     uint32_t slot = 0, phase = 0;
-    __device__ __forceinline__ void next(uint32_t n = 1) {
-        slot += n;
-        if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+    __device__ __forceinline__ void next() {
+        if (++slot == SLOTS) slot = 0, phase ^= 1;
     }
+    __device__ __forceinline__ void skip(uint32_t n) { slot = (slot + n) % SLOTS; }        // (the slot alone)
 };
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -70,6 +74,23 @@ __device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap *map, 
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(head), "r"(tok), "r"(smem_u32(bar))
                  : "memory");
+}
+
+// The MMAs by the low words of the operands' descriptors; the high word is the same for all: 1024 bytes between groups of 8 rows,
+// 128-byte swizzle.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (uint32_t)desc_sw128(saddr, lbo, 1024); }
+constexpr uint32_t kDescHi = 1024u >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_ss_lo(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(da), "r"(db), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts_lo(uint32_t d, uint32_t a, uint32_t db, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(db), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHi)
+        : "memory");
 }
 
 // Two fp32 as a pair of the 16-bit type, and back.
@@ -107,7 +128,19 @@ __device__ __forceinline__ bool drop_nonfinite16(uint4 &v) {        // zero what
     return any;
 }
 
-// One unit of work, as every role derives it: kv head; the sequence's first token row and length; the unit's first token.
+// x += the first, y += the second of a pair of the 16-bit type, in fp32.
+template <bool BF>
+__device__ __forceinline__ void add16(uint32_t v, float &x, float &y) {
+    if constexpr (BF)
+        asm("{\n\t.reg .b16 a, b, o;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 o, 0x3F80;\n\tfma.rn.f32.bf16 %0, a, o, %0;\n\tfma.rn.f32.bf16 %1, b, o, %1;\n\t}"
+            : "+f"(x), "+f"(y)
+            : "r"(v));
+    else
+        asm("{\n\t.reg .b16 a, b, o;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 o, 0x3C00;\n\tfma.rn.f32.f16 %0, a, o, %0;\n\tfma.rn.f32.f16 %1, b, o, %1;\n\t}"
+            : "+f"(x), "+f"(y)
+            : "r"(v));
+}
+// One unit of work: kv head; the sequence's first token row and length (-1: there are no more units); the unit's first token.
 struct PromptUnit {
     int kh, t0, n, tok0;
     __device__ __forceinline__ int last(int i, int tq) const { return min(n, tok0 + (i + 1) * tq) - 1; }      // of stream i
@@ -156,10 +189,10 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
     // full, empty: of the ring's slots; landed: V tiles that go on after a look
     uint64_t *full = reinterpret_cast<uint64_t *>(sm + C::BARS), *empty = full + C::SLOTS, *landed = empty + C::SLOTS, *q_full = landed + C::SLOTS;
     uint64_t *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2, *drain = o_full + 2;
-    int *s_int = reinterpret_cast<int *>(drain + 1);            // abort, V set aside, TMEM base, lock
+    uint64_t *u_full = drain + 1, *u_empty = u_full + 1, *u_got = u_empty + 1;
+    int *s_int = reinterpret_cast<int *>(u_got + 1);            // abort, V set aside, TMEM base
     volatile int *s_abort = s_int, *s_flag = s_int + 1;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(s_int + 2);
-    int *s_lock = s_int + 3;
     if (sm0 & 1023) {                             // the swizzled tiles need it; never seen
         if (tid == 0) paged_err(a, QMS_PAGED_ETIMEOUT);
         return;
@@ -167,7 +200,7 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
     if (tid == 0) {
         for (uint32_t i = 0; i < C::SLOTS; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 2);
+            mbar_init(&empty[i], 1);
             mbar_init(&landed[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -177,8 +210,11 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
             mbar_init(&p_full[i], 4);
             mbar_init(&o_full[i], 1);
         }
-        mbar_init(drain, 2);
-        s_int[0] = s_int[1] = *s_lock = 0;
+        mbar_init(drain, 1);
+        mbar_init(u_full, 1);
+        mbar_init(u_empty, 11);
+        mbar_init(u_got, 1);
+        s_int[0] = s_int[1] = 0;
         fence_mbar_init();
     }
     if (warp == C::MMA_WARP) {
@@ -199,23 +235,41 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
     const uint32_t tmem = *s_tmem;
     const WideSync sy{s_abort, &a};
     PromptUnit w;
+    // the next unit, by each warp but the one that finds them; false: a wait gave up
+    uint32_t units = 0;
+    auto next_unit = [&]() {
+        if (!__all_sync(kFull, sy.wait(u_full, units++ & 1))) return false;
+        const volatile int *x = reinterpret_cast<const int *>(sm + C::UNIT);
+        w = PromptUnit{x[0], x[1], x[2], x[3]};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(u_empty);
+        return true;
+    };
     if (blockIdx.x == 0)                          // the batch's arrays, checked once
         for (int b = tid; b < a.n_seq; b += C::THREADS) {
             int t0, n, kv;
             if (!prompt_seq(a, b, t0, n, kv)) paged_err(a, QMS_PAGED_ELEN);
         }
 
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsOther));
     if (warp < 8) {
         // ---- softmax of stream i: thread = row = TMEM lane
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrRegs));
         const int i = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_col = lanes + i * 128, o_col = lanes + C::O_COL + i * D;
         const int my_tok = row / G, my_head = row - my_tok * G;
         const float f = A.f;
         uint32_t ns = 0, no = 0;
+        RingAt<C::SLOTS> at;
+        const bool gives = (warp & 3) == 0 && lane == 0;
         bool ok = true;
-        for (unsigned u = blockIdx.x; ok && prompt_unit(A, u, w); u += gridDim.x) {
+        while (ok && (ok = next_unit()) && w.n >= 0) {
             const int nt = w.tiles(i, tq);
-            if (nt == 0) continue;
+            const bool gives_kv = gives && w.there(1, tq) == (i == 1);             // the stream that uses a tile last (it has as many, or more)
+            if (nt == 0) {
+                at.skip(2 * w.tiles(0, tq));
+                continue;
+            }
             const int lo = w.tok0 + i * tq, last = w.last(i, tq), tok = lo + my_tok;       // every row sees the positions up to lo
             const bool there = my_tok < tq && tok <= last;
             const int pos = there ? tok : -1;
@@ -235,87 +289,71 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                 if (!(ok = __all_sync(kFull, sy.wait(&s_full[i], ns & 1)))) break;
                 ns++;
                 tc_fence_after();
-                const float2 f2 = make_float2(f, f);
-                float S = 0.0f;                   // the tile's weights
-                // scores of 32 positions in z become weights, pairs in 16 columns. The base stays unless a score lies 2^kPrHigh above
-                // it: then what was computed with the old one (o; this tile's weights so far) is scaled by a power of 2.
-                auto weights = [&](uint32_t (&z)[32], int c, uint32_t done) {
-                    float mx = max3(__uint_as_float(z[0]), __uint_as_float(z[1]), __uint_as_float(z[2]));
+                // what the MMAs that ended before this S read can be written again: K of this tile, V of the last, Q
+                if (gives_kv) {
+                    mbar_arrive(&empty[at.slot]);
+                    if (j > 0) mbar_arrive(&empty[at.slot == 0 ? C::SLOTS - 1 : at.slot - 1]);
+                }
+                if (gives && j + 1 == nt) mbar_arrive(&q_empty[i]);
+                at.skip(2);
+                // the tile's scores of this row, all of them: the maximum first, then the weights without a wait
+                uint32_t z[4][32];
+                const int chunks = min(4, (last - j * 128) / 32 + 1);
 #pragma unroll
-                    for (int e = 3; e < 31; e += 2) mx = max3(mx, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
-                    mx = fmaxf(mx, __uint_as_float(z[31]));
-                    mx *= f;
-                    if (__any_sync(kFull, mx > B + kPrHigh)) {
-                        const float nb = mx > B + kPrHigh ? ceilf(mx) - kPrLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
-                        B = nb;
-                        S *= fac;
-                        l *= fac;
-                        if (j > 0) scale_o(fac);
-#pragma unroll 1
-                        for (int k = 0; k < 4; k++) {
-                            if (!(done >> k & 1)) continue;
-                            uint32_t o[16];
-                            tmem_wait_st();
-                            tmem_ld<16>(s_col + 16 * k, o);
-                            tmem_wait_ld16(o);
+                for (int c = 0; c < 4; c++) tmem_ld<32>(s_col + 32 * c, z[c]);
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const float2 y = unpack16<BF>(o[e]);
-                                o[e] = pack16<BF>(y.x * fac, y.y * fac);
-                            }
-                            tmem_st16(s_col + 16 * k, o);
-                        }
-                    }
-                    const float2 nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
-                    uint32_t o[16];
-                    float2 l2 = make_float2(0.0f, 0.0f);
+                for (int c = 0; c < 4; c++) tmem_wait_ld(z[c]);
+                if (j * 128 + 127 > lo)           // some row does not see the whole tile
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 q = f2_fma(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), f2, nB);
-                        const float2 w2 = make_float2(ex2(q.x), ex2(q.y));
-                        l2 = f2_add(l2, w2);
-                        o[e / 2] = pack16<BF>(w2.x, w2.y);
-                    }
-                    tmem_st16(s_col + 16 * c, o);
-                    S += l2.x + l2.y;
-                };
-                uint32_t x[32], y[32];
-                if (j * 128 + 127 <= lo) {        // every row sees the whole tile
-                    tmem_ld<32>(s_col, x);
-                    tmem_wait_ld(x);
-                    tmem_ld<32>(s_col + 32, y);   // the next 32 come while these are worked on
-                    weights(x, 0, 0);
-                    tmem_wait_ld(y);
-                    tmem_ld<32>(s_col + 64, x);
-                    weights(y, 1, 1);
-                    tmem_wait_ld(x);
-                    tmem_ld<32>(s_col + 96, y);
-                    weights(x, 2, 3);
-                    tmem_wait_ld(y);
-                    weights(y, 3, 7);
-                } else {
-                    const int chunks = min(4, (last - j * 128) / 32 + 1);
-#pragma unroll 1
-                    for (int c = 0; c < chunks; c++) {
+                    for (int c = 0; c < 4; c++) {
                         const int d = pos - j * 128 - 32 * c;
                         const uint32_t vis = d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u;
-                        tmem_ld<32>(s_col + 32 * c, x);
-                        tmem_wait_ld(x);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) x[e] = vis >> e & 1 ? x[e] : 0xff800000u;
-                        weights(x, c, (1u << c) - 1u);
+                        for (int e = 0; e < 32; e++) z[c][e] = vis >> e & 1 ? z[c][e] : 0xff800000u;
                     }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    mx[c] = max3(__uint_as_float(z[c][0]), __uint_as_float(z[c][1]), __uint_as_float(z[c][2]));
+#pragma unroll
+                    for (int e = 3; e < 31; e += 2) mx[c] = max3(mx[c], __uint_as_float(z[c][e]), __uint_as_float(z[c][e + 1]));
+                    mx[c] = fmaxf(mx[c], __uint_as_float(z[c][31]));
                 }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                // the base stays unless a score lies 2^kPrHigh above it: then what was computed with the old one is scaled
+                if (__any_sync(kFull, top > B + kPrHigh)) {
+                    const float nb = top > B + kPrHigh ? ceilf(top) - kPrLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
+                    B = nb;
+                    l *= fac;
+                    if (j > 0) scale_o(fac);
+                }
+                const float2 f2 = make_float2(f, f), nB = B == -INFINITY ? make_float2(0.0f, 0.0f) : make_float2(-B, -B);
+                float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c >= chunks) break;
+                    uint32_t o[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 q = f2_fma(make_float2(__uint_as_float(z[c][e]), __uint_as_float(z[c][e + 1])), f2, nB);
+                        o[e / 2] = pack16<BF>(ex2(q.x), ex2(q.y));
+                        if (e & 2) add16<BF>(o[e / 2], l0, l1);
+                        else add16<BF>(o[e / 2], l2, l3);
+                    }
+                    tmem_st16(s_col + 16 * c, o);
+                }
+                l += (l0 + l1) + (l2 + l3);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[i]);
-                l += S;
             }
             if (!ok) break;
             if (!(ok = __all_sync(kFull, sy.wait(&o_full[i], no & 1)))) break;
             no++;
             tc_fence_after();
+            if (gives_kv) mbar_arrive(&empty[at.slot == 0 ? C::SLOTS - 1 : at.slot - 1]);      // V of the last tile
+            at.skip(2 * (max(w.tiles(0, tq), w.tiles(1, tq)) - nt));
             // ---- the rows: O / l, 128 bytes of a row at a time by 8 lanes
             const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
             const bool none = l == 0.0f, fix = *s_flag != 0;
@@ -375,7 +413,7 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
         RingAt<C::SLOTS> at;
         uint32_t n = 0, nq[2] = {0, 0};
         bool ok = true;
-        for (unsigned u = blockIdx.x; ok && prompt_unit(A, u, w); u += gridDim.x) {
+        while (ok && (ok = next_unit()) && w.n >= 0) {
             const int nt = max(w.tiles(0, tq), w.tiles(1, tq));
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -405,7 +443,7 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
         RingAt<C::SLOTS> at;
         uint32_t phases = 0;                      // of `landed`
         bool ok = true;
-        for (unsigned u = blockIdx.x; ok && prompt_unit(A, u, w); u += gridDim.x) {
+        while (ok && (ok = next_unit()) && w.n >= 0) {
             const int nt = max(w.tiles(0, tq), w.tiles(1, tq)), end = max(w.last(0, tq), w.last(1, tq)) + 1;
             for (int j = 0; ok && j < nt; j++) {
                 at.next();
@@ -431,83 +469,75 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                 at.next();
             }
         }
-    } else {
-        // ---- the MMAs of stream i, by one thread
-        const int i = warp - C::MMA_WARP;
+    } else if (warp == C::MMA_WARP) {
+        // ---- the MMAs of both streams in turn, by one thread. An instruction runs 64 cycles, so what leads to the next one has to be
+        // little: descriptors of which only the low word changes, by a constant. (Made anew for each they took 100 cycles, in loops
+        // that are not unrolled 130; two threads, one per stream and under a lock, were no better.)
         constexpr uint32_t kind = BF ? 1u << 7 | 1u << 10 : 0u, id_o = idesc_f16(D, true) | kind;
         RingAt<C::SLOTS> at;
-        uint32_t nq = 0, np = 0;
+        uint32_t np = 0, nq = 0;                               // phases of p_full, q_full
         bool ok = true;
-        auto score = [&](uint32_t slot, int cnt) {             // S_i = Q_i K^T
-            const uint32_t k = sm0 + C::RING + slot * C::TILE, q = sm0 + i * C::TILE, id_s = idesc_f16((cnt + 15) & ~15, false) | kind;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ks++)
-                umma_f16_ss(tmem + i * 128, desc_sw128(q + (ks >> 2) * C::HALF + (ks & 3) * 32, 16, 1024),
-                            desc_sw128(k + (ks >> 2) * C::HALF + (ks & 3) * 32, 16, 1024), id_s, ks > 0);
+        auto wait = [&](uint64_t *bar, uint32_t parity) {      // (no sleep: what follows is late by as much)
+            for (uint32_t n = 0; !mbar_test_wait(bar, parity); n++) {
+                if (*s_abort) return false;
+                if (n == kWSpin) {
+                    *s_abort = 1;
+                    paged_err(a, QMS_PAGED_ETIMEOUT);
+                    return false;
+                }
+            }
+            return true;
         };
-        auto weigh = [&](uint32_t slot, int cnt, bool first) { // O_i (+)= P_i V
-            const uint32_t v = sm0 + C::RING + slot * C::TILE;
+        auto score = [&](int i, uint32_t slot, int cnt) {      // S_i = Q_i K^T
+            const uint32_t id_s = idesc_f16((cnt + 15) & ~15, false) | kind;
+            const uint32_t dq = desc_lo(sm0 + i * C::TILE, 16), dk = desc_lo(sm0 + C::RING + slot * C::TILE, 16);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++) {
+                const uint32_t off = ((ks >> 2) * C::HALF + (ks & 3) * 32) >> 4;
+                umma_ss_lo(tmem + i * 128, dq + off, dk + off, id_s, ks > 0);
+            }
+        };
+        auto weigh = [&](int i, uint32_t slot, int cnt, bool first) {      // O_i (+)= P_i V
+            const uint32_t dv = desc_lo(sm0 + C::RING + slot * C::TILE, C::HALF);
 #pragma unroll
             for (int ks = 0; ks < 8; ks++)
-                if (ks * 16 < cnt)
-                    umma_f16_ts(tmem + C::O_COL + i * D, tmem + i * 128 + ks * 8, desc_sw128(v + ks * 2048, C::HALF, 1024), id_o, !first || ks > 0);
+                if (ks * 16 < cnt) umma_ts_lo(tmem + C::O_COL + i * D, tmem + i * 128 + ks * 8, dv + ks * 128, id_o, ks > 0 || !first);
         };
-        auto lock = [&]() {
-            uint32_t x = 0;
-            do {                                               // (reading costs less than trying)
-                while (*(volatile int *)s_lock != 0 && ++x < kWSpin) {}
-            } while (atomicCAS(s_lock, 0, 1) != 0 && x < kWSpin);
-        };
-        auto unlock = [&]() { *(volatile int *)s_lock = 0; };
-        for (unsigned u = blockIdx.x; ok && prompt_unit(A, u, w); u += gridDim.x) {
-            const int nt = w.tiles(i, tq), all = max(nt, w.tiles(i ^ 1, tq)), last = w.last(i, tq);
+        while (ok && (ok = next_unit()) && w.n >= 0) {
             if (lane == 0) {
-                auto cnt = [&](int j) { return min(128, last + 1 - 128 * j); };
-                if (nt > 0) {
-                    ok = sy.wait(&q_full[i], nq++ & 1) && sy.wait(&full[at.slot], at.phase);
-                    if (ok) {
-                        tc_fence_after();
-                        lock();
-                        score(at.slot, cnt(0));
-                        unlock();
-                        umma_commit(&s_full[i]);
-                        umma_commit(&empty[at.slot]);
-                        if (nt == 1) umma_commit(&q_empty[i]);
-                    }
-                }
-                for (int j = 0; ok && j < nt; j++) {
-                    at.next();                                 // V of tile j
-                    if (!(ok = sy.wait(&full[at.slot], at.phase) && sy.wait(&p_full[i], np++ & 1))) break;
+                const int nt0 = w.tiles(0, tq), nt1 = w.tiles(1, tq), all = max(nt0, nt1);
+                ok = wait(&full[at.slot], at.phase);
+#pragma unroll 1
+                for (int i = 0; i < 2; i++) {
+                    if (!ok || (i && nt1 == 0)) break;
+                    if (!(ok = wait(&q_full[i], nq >> i & 1))) break;
+                    nq ^= 1u << i;
                     tc_fence_after();
-                    const RingAt<C::SLOTS> v = at;
-                    at.next();                                 // K of the next, or of the next unit
-                    lock();
-                    weigh(v.slot, cnt(j), j == 0);
-                    if (j + 1 == nt) {
-                        unlock();
-                        umma_commit(&o_full[i]);
-                        umma_commit(&empty[v.slot]);
-                        break;
-                    }
-                    if (!mbar_test_wait(&full[at.slot], at.phase)) {         // K is late: not at the other's cost
-                        unlock();
-                        umma_commit(&empty[v.slot]);
-                        if (!(ok = sy.wait(&full[at.slot], at.phase))) break;
-                        tc_fence_after();
-                        lock();
-                        score(at.slot, cnt(j + 1));
-                        unlock();
-                    } else {
-                        score(at.slot, cnt(j + 1));
-                        unlock();
-                        umma_commit(&empty[v.slot]);
-                    }
+                    score(i, at.slot, min(128, w.last(i, tq) + 1));
                     umma_commit(&s_full[i]);
-                    umma_commit(&empty[at.slot]);
-                    if (j + 2 == nt) umma_commit(&q_empty[i]);
                 }
-                for (int x = 2 * nt; ok && x < 2 * all; x++, at.next())      // the other stream's alone
-                    if ((ok = sy.wait(&full[at.slot], at.phase))) mbar_arrive(&empty[at.slot]);
+                for (int j = 0; ok && j < all; j++) {
+                    at.next();                                 // V of tile j
+                    const RingAt<C::SLOTS> va = at;
+                    at.next();                                 // K of the next (or of the next unit)
+                    if (!(ok = wait(&full[va.slot], va.phase))) break;
+                    if (j + 1 < all && !(ok = wait(&full[at.slot], at.phase))) break;
+#pragma unroll 1
+                    for (int i = 0; i < 2; i++) {
+                        if (j >= (i ? nt1 : nt0)) continue;
+                        if (!(ok = wait(&p_full[i], np >> i & 1))) break;
+                        np ^= 1u << i;
+                        tc_fence_after();
+                        const int cnt = w.last(i, tq) + 1 - 128 * j;
+                        weigh(i, va.slot, cnt, j == 0);
+                        if (cnt > 128) {
+                            score(i, at.slot, min(128, cnt - 128));
+                            umma_commit(&s_full[i]);
+                        } else {
+                            umma_commit(&o_full[i]);
+                        }
+                    }
+                }
             }
             ok = __shfl_sync(kFull, (int)ok, 0);
         }
@@ -517,6 +547,53 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
             for (uint32_t n = 0; n < kWSpin && !mbar_try_wait(drain, 0); n++) __nanosleep(32);
         }
         __syncwarp();
+    } else {
+        // ---- which unit is next: the CTA's own, then those of CTAs of the grid that have not started, one ahead of the softmax
+        uint32_t k = 0;
+        bool ok = true;
+        auto publish = [&](const PromptUnit &x) {
+            if (k > 0 && !__all_sync(kFull, sy.wait(u_empty, (k - 1) & 1))) return false;
+            k++;
+            if (lane == 0) {
+                volatile int *to = reinterpret_cast<int *>(sm + C::UNIT);
+                to[0] = x.kh, to[1] = x.t0, to[2] = x.n, to[3] = x.tok0;
+                mbar_arrive(u_full);
+            }
+            __syncwarp();
+            return true;
+        };
+        unsigned u = blockIdx.x;
+        for (uint32_t asked = 0;; asked++) {
+            if (prompt_unit(A, u, w) && !(ok = publish(w))) break;
+            if (lane == 0) {
+                fence_async_smem();
+                mbar_arrive_expect_tx(u_got, 16);
+                asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(sm0 + C::UNIT + 16),
+                             "r"(smem_u32(u_got))
+                             : "memory");
+            }
+            __syncwarp();
+            uint32_t n = 0;                       // (not given up before the answer is there, abort or not: it is written to this CTA's memory)
+            while (!mbar_try_wait(u_got, asked & 1) && ++n < kWSpin) {}
+            if (!__all_sync(kFull, n < kWSpin)) {
+                *s_abort = 1;
+                if (lane == 0) paged_err(a, QMS_PAGED_ETIMEOUT);
+                ok = false;
+                break;
+            }
+            uint32_t got, x;
+            asm volatile(
+                "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
+                "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+                : "=r"(got), "=r"(x)
+                : "r"(sm0 + C::UNIT + 16)
+                : "memory");
+            __syncwarp();
+            if (!got) break;
+            u = x;
+        }
+        if (ok) publish(PromptUnit{0, 0, -1, 0});
     }
     tc_fence_before();
     __syncthreads();
@@ -557,7 +634,8 @@ static int launch_prompt(const PromptAttn &A, const QmsCudaHeads &q, const QmsCu
         (rc = heads_map(v, BF, D, A.a.Hk, A.a.n_tok, 1, 128, &mv)))
         return rc;
     const int64_t most = ((int64_t)A.a.n_tok / (2 * A.tq) + std::min(A.a.n_seq, A.a.n_tok)) * A.a.Hk;      // units there can be
-    const int grid = (int)std::min<int64_t>(most, 148);
+    QMS_REQUIRE(most < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "prompt_attention: too many units of work");
+    const unsigned grid = (unsigned)most;          // (those that have not started are taken over by CTAs that have)
     QMS_CK(launch_pdl(k_prompt_attn<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM, s, A, mq, mk, mv));
     return QMS_CUDA_OK;
 }

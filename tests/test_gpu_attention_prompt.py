@@ -1,10 +1,12 @@
 """Attention within whole prompts on a B200 through the C ABI (qms_cuda_prompt_attention), against its formula in 64 bits.
 
 Bounds, with e = 2^-24 and h the type's half step (bf16 2^-8, fp16 2^-11). q, k, v are exact. A score is off by at most head_dim additions
-that cut at e, times A = scale * sum |q k|; a weight by that relatively, by the exponential's 4 e and by its rounding, h; an fp16 weight
-also by half of fp16's smallest step, 2^-25, where the row's largest weight is 2^7 at least. The output is a weighted mean of V: with L
-the positions that the row sees and M = sum p |v| it is off by ((D + 8) e A + 8 e + h) M, by 2^-32 L max |v| (fp16) and by the sums' own
-cuts, (L / 16 + 8) 2 e M; then by its own rounding, h of itself (fp32 out: none)."""
+that cut at e, times A = scale * sum |q k|; a weight by that relatively, by the exponential's 2.6e-6 < 44 e (a polynomial of that error, or 4 e)
+and by its rounding, h; an fp16 weight also by half of fp16's smallest step, 2^-25, where the row's largest weight is 2^7 at least.
+The sum that divides is that of the rounded weights: with relative errors d_i of the weights p_i the output is off by sum p_i d_i (v_i - o)
+/ (1 + sum p_i d_i), at most max |d| (1 + 2 h) (M + |o|) with M = sum p |v|. So by ((D + 8) e A + 48 e + h) (1 + 2 h) (M + |o|), by 2^-31 L
+max |v| (fp16; L the positions that the row sees) and by the sums' own cuts, (L / 16 + 8) 2 e M; then by its own rounding, h of
+itself (fp32 out: none)."""
 from __future__ import annotations
 
 import numpy as np
@@ -56,9 +58,9 @@ def reference(lens, q, k, v, scale, out32=False, start0=0):
                 p = torch.softmax(s.masked_fill(late, -float("inf")), -1)
                 want[t + i:t + e, hk * G:(hk + 1) * G] = (p @ vv).transpose(0, 1)
                 M, L = p @ vv.abs(), torch.arange(i + 1, e + 1, device="cuda").double()[:, None]
-                b = ((D + 8) * E * A + 8 * E + h)[..., None] * M + (L / 16 + 8) * 2 * E * M
+                b = ((D + 8) * E * A + 48 * E + h)[..., None] * (1 + 2 * h) * (M + (p @ vv).abs()) + (L / 16 + 8) * 2 * E * M
                 if q.dtype == torch.float16:
-                    b = b + 2.0 ** -32 * L * vv.abs().amax()
+                    b = b + 2.0 ** -31 * L * vv.abs().amax()
                 tol[t + i:t + e, hk * G:(hk + 1) * G] = b.transpose(0, 1)
         t += n
     if not out32:
