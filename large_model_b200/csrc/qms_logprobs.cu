@@ -12,7 +12,9 @@ namespace qms {
 
 typedef unsigned long long u64;
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpList = 2048;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32;
+constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2;       // a warp's: groups of 4 values per lane, values per chunk, chunks in flight
+constexpr uint32_t kLpSpin = 1u << 22;
 
 struct LogprobArgs {
     const float *l;
@@ -26,221 +28,291 @@ struct LogprobArgs {
 
 // A value and its index as one number that grows with the value and, among equals, falls with the index. Never 0 for a value that
 // is not NaN.
-__device__ __forceinline__ u64 lp_key(float x, int i) {
+__device__ __forceinline__ uint32_t lp_order(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);                   // (-0 counts as 0)
-    return (u64)(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u)) << 32 | (uint32_t)~i;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float lp_value(u64 key) {
-    const uint32_t b = (uint32_t)(key >> 32);
-    return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+__device__ __forceinline__ u64 lp_key(float x, int i) { return (u64)lp_order(x) << 32 | (uint32_t)~i; }
+__device__ __forceinline__ float lp_unorder(uint32_t b) { return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b); }
+__device__ __forceinline__ float lp_value(u64 key) { return lp_unorder((uint32_t)(key >> 32)); }
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
-// What one CTA knows of its slice: the maximum m; z, t: sums of w and w log2(w), w = 2^((l - m) c), without one value that is m.
+// How many entries of `lists` lists, each of kLpTop in falling order, are above the key.
+__device__ __forceinline__ int lp_above(const u64 *list, int lists, u64 key) {
+    static_assert(kLpTop == 32, "5 steps to one of 32, a sixth for none or all");
+    int at[kRowCtas] = {};
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1)
+#pragma unroll
+        for (int w = 0; w < kRowCtas; w++)
+            if (w < lists && list[w * kLpTop + at[w] + step - 1] > key) at[w] += step;
+    int above = 0;
+#pragma unroll
+    for (int w = 0; w < kRowCtas; w++)
+        if (w < lists) above += at[w] + (at[w] == 31 && list[w * kLpTop + 31] > key);
+    return above;
+}
+
+// What is known of some values: the maximum m; z, t: sums of w and w log2(w), w = 2^((l - m) c), without one value that is m.
 struct LpPart {
     float m, z, t;
 };
+// p under the maximum M of several parts; `first`: it is the one whose m is left out. Nothing seen: z is 0, or NaN.
+__device__ __forceinline__ LpPart lp_under(const LpPart &p, float M, bool first, float c) {
+    if (first) return p;
+    const float d = p.m == -INFINITY ? -INFINITY : (p.m - M) * c, f = ex2f(d), one = p.z + 1.0f;
+    return LpPart{M, one * f, f * fmaf(one, fmaxf(d, -256.0f), p.t)};
+}
 
 // With x = (l - max) / temp: log p = x - log Z and the entropy log Z - sum p x, where Z = 1 + z and z leaves out one value that is the
-// maximum: of a sure row z is what matters, and 1 + z would round it away. Grid: rows x cluster, a slice per CTA, kept in shared memory
-// as in k_probs. First pass over a slice: every lane's maximum. From these a bound that at least n_top values of the slice
-// reach: the least over the warps of each warp's r-th largest lane maximum, r n_top over the number of warps. Second
-// pass: z and t, and the values at or above the bound go to a list, some 50 of 19,000; a value's rank is the number of list entries
-// above it. A list that overflows (thousands of equal values) is not used: n_top rounds of the largest below the last one.
-// The cluster's first CTA joins the parts and the lists.
-__global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a) {
-    extern __shared__ __align__(16) float x[];
-    __shared__ u64 s_list[kLpList], s_all[kRowCtas * kLpTop], s_key[kLpWarps];
-    __shared__ float s_m[kLpWarps], s_r[kLpWarps], s_z[kLpWarps], s_t[kLpWarps];
-    __shared__ LpPart s_part[kRowCtas];
-    __shared__ int s_n, s_most;
+// maximum: of a sure row z is what matters, and 1 + z would round it away. One pass, and no warp waits for another before its end: a row
+// is cut over a cluster, the warps of a CTA take its chunks in turn, each into its part of shared memory by bulk copies. A lane keeps two running maxima apart from its sums (what is no longer the largest is added), under a
+// base that follows them at a distance of 2^4 at most.
+// The likeliest: lane i holds the i-th largest of its warp's so far. Values that reach a bound are put in their place: first one that n_top
+// lanes' largest of the first chunk reach, then the n_top-th itself, of this warp or of another that is further. Some 35
+// of 2400 values reach it; those of a chunk are put in together. The first CTA of the cluster joins all.
+__global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a) {
+    extern __shared__ __align__(128) float rings[];        // [kLpWarps][kLpRing][kLpChunk]
+    __shared__ u64 s_all[kRowCtas * kLpTop], s_list[kLpWarps * kLpTop], s_some[kLpWarps][48];
+    __shared__ uint64_t s_full[kLpWarps][kLpRing];
+    __shared__ LpPart s_warp[kLpWarps], s_part[kRowCtas];
+    __shared__ uint32_t s_bound;                           // the highest bound of a warp, by lp_order
+    __shared__ int s_abort;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
-    if (tid < nc * kLpTop) s_all[tid] = 0;
-    if (tid == 0) s_n = s_most = 0;
+    float *ring = rings + warp * kLpRing * kLpChunk;
+    for (int i = tid; i < nc * kLpTop; i += kLpThreads) s_all[i] = 0;
+    if (tid == 0) s_abort = 0, s_bound = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kLpRing; i++) mbar_init(&s_full[warp][i], 1);
+        fence_mbar_init();
+    }
     auto started = cl.barrier_arrive();                    // waited for before the first write to another CTA
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
+    // the row: up to 3 values before a 16-byte boundary, groups of 4 that are cut over all warps, up to 3 behind them
     const int64_t r = blockIdx.x / nc;
-    const int groups = (a.V + 3) >> 2;                     // slices start at multiples of 4 values
-    const int lo = (int)((int64_t)groups * rank / nc) * 4, n = min(a.V, (int)((int64_t)groups * (rank + 1) / nc) * 4) - lo;
-    const float *row = a.l + r * a.ldl, *l = row + lo;
-    const int kept = min(n, kProbsKeep), n4 = (kept + 3) >> 2;
-    const float4 *x4 = reinterpret_cast<const float4 *>(x);
-    if (((uintptr_t)l & 15) == 0) {
-        for (int i = tid; i < kept >> 2; i += kLpThreads) cp_async16(x + 4 * i, l + 4 * i);
-        if (tid < (kept & 3)) cp_async4(x + (kept & ~3) + tid, l + (kept & ~3) + tid);
-    } else {
-#pragma unroll 4
-        for (int i = tid; i < kept; i += kLpThreads) cp_async4(x + i, l + i);
-    }
-    if (tid >= kept && tid < 4 * n4) x[tid] = -INFINITY;   // (a slice below one group)
-    for (int i = max(kept, kLpThreads) + tid; i < 4 * n4; i += kLpThreads) x[i] = -INFINITY;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-
-    // ---- first pass: maxima
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = tid; i < n4; i += kLpThreads) {
-        const float4 y = x4[i];
-        m = fmaxf(m, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
-    }
-    for (int i = kept + tid; i < n; i += kLpThreads) m = fmaxf(m, l[i]);
-    const int busy = min(kLpWarps, (n4 + 31) >> 5);        // warps with values
-    const int rounds = (a.n_top + max(busy, 1) - 1) / max(busy, 1);
-    {
-        uint32_t k = __float_as_uint(m + 0.0f);
-        k ^= (uint32_t)((int)k >> 31) | 0x80000000u;
-        uint32_t best = __reduce_max_sync(kFull, k), top = best;
-        for (int i = 1; i < rounds; i++) {                 // the next largest lane
-            const unsigned hit = __ballot_sync(kFull, k == best);
-            if (lane == __ffs(hit) - 1) k = 0;
-            best = __reduce_max_sync(kFull, k);
-        }
-        if (lane == 0) {
-            s_m[warp] = lp_value((u64)top << 32);
-            s_r[warp] = best == 0 ? -INFINITY : lp_value((u64)best << 32);
-        }
-    }
-    __syncthreads();
-    m = s_m[lane & (kLpWarps - 1)];
-    float bound = (lane & (kLpWarps - 1)) < busy ? s_r[lane & (kLpWarps - 1)] : INFINITY;
-#pragma unroll
-    for (int o = kLpWarps / 2; o > 0; o >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-        bound = fminf(bound, __shfl_xor_sync(kFull, bound, o));
-    }
-    bound = a.n_top == 0 ? m : fmaxf(fminf(bound, m), -FLT_MAX);
-    const float M = m == -INFINITY ? 0.0f : m;
-
-    // ---- second pass: sums, and the list
-    float z = 0.0f, t = 0.0f;
-    auto add = [&](float v, float &gz, float &gt) {
-        const float y = (v - M) * a.c, w = ex2f(y);
-        gz += w;
-        gt = fmaf(w, fmaxf(y, -256.0f), gt);               // (weights below 2^-126 are 0; 0 * inf is not)
+    const float *row = a.l + r * a.ldl;
+    const int head = min(a.V, (int)(-((uintptr_t)row >> 2) & 3)), groups = (a.V - head) >> 2, tail = head + 4 * groups;
+    const int lo = head + (int)((int64_t)groups * rank / nc) * 4, hi = head + (int)((int64_t)groups * (rank + 1) / nc) * 4;
+    const int chunks = ((hi - lo + kLpChunk - 1) / kLpChunk - warp + kLpWarps - 1) / kLpWarps;     // in turn over the warps
+    auto load = [&](int k) {                               // by one lane
+        const int base = lo + (k * kLpWarps + warp) * kLpChunk, n = min(kLpChunk, hi - base);
+        mbar_arrive_expect_tx(&s_full[warp][k % kLpRing], n * 4);
+        bulk_load(smem_u32(ring + k % kLpRing * kLpChunk), row + base, n * 4, &s_full[warp][k % kLpRing]);
     };
-    // a value at the bound or above: listed; the maxima are counted and left out of the sums
-    auto look = [&](float v, int i) {
-        if (v >= bound && v > -INFINITY) {
-            if (a.n_top > 0) {
-                const int k = atomicAdd(&s_n, 1);
-                if (k < kLpList) s_list[k] = lp_key(v, lo + i);
-            }
-            if (v == m) {
-                atomicAdd(&s_most, 1);
-                return -INFINITY;
-            }
+    if (lane == 0)
+        for (int k = 0; k < min(chunks, kLpRing); k++) load(k);
+    const float mine = tid < a.n_ids && rank == 0 && (unsigned)a.ids[r * a.n_ids + tid] < (unsigned)a.V ? row[a.ids[r * a.n_ids + tid]] : 0.0f;
+    __syncthreads();                                       // s_bound, s_abort
+
+    float B = -FLT_MAX, m[2] = {-INFINITY, -INFINITY}, z[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+    float bound = -FLT_MAX;                                // a value has to reach it
+    u64 best = 0;                                          // the lane-th largest of the warp's
+    // new values, up to 32 in s_new, take their places among the n_top largest: a key's place is the number of keys above it
+    u64 *s_new = s_some[warp], *s_mine = s_list + warp * kLpTop;
+    auto merge = [&](int n) {
+        __syncwarp();
+        const u64 key = lane < n ? s_new[lane] : 0;
+        int at = 0, down = lane;
+        for (int i = 0; i < n; i++) {
+            const u64 k = s_new[i];
+            at += k > key;
+            down += k > best;
         }
-        return v;
+        for (int i = 0; i < a.n_top; i++) at += __shfl_sync(kFull, best, i) > key;
+        s_mine[lane] = 0;
+        __syncwarp();
+        if (best != 0 && down < a.n_top) s_mine[down] = best;
+        if (key != 0 && at < a.n_top) s_mine[at] = key;
+        __syncwarp();
+        best = s_mine[lane];
     };
-    for (int i0 = tid; i0 < n4; i0 += 8 * kLpThreads) {    // sums of 32: no long chain of roundings
-        float gz = 0.0f, gt = 0.0f;
+    int news = 0;
+    auto look = [&](float v, int i) {                      // v: a value of each lane
+        const unsigned hit = __ballot_sync(kFull, v >= bound);
+        if (hit == 0) return;
+        if (v >= bound) s_new[news + __popc(hit & ((1u << lane) - 1u))] = lp_key(v, i);
+        news += __popc(hit);
+        if (news > 16) {
+            merge(min(news, 32));
+            news = max(news - 32, 0);
+            const u64 rest = lane < news ? s_new[32 + lane] : 0;
+            __syncwarp();
+            if (lane < news) s_new[lane] = rest;
+        }
+    };
+    // between chunks: what comes later has a higher index, and has to be more than the n_top-th
+    auto raise = [&]() {
+        if (news > 4) {
+            merge(news);
+        } else {                                           // (one costs a third of a merge)
+            __syncwarp();
+            for (int i = 0; i < news; i++) {
+                const u64 key = s_new[i], up = __shfl_up_sync(kFull, best, 1);
+                const int at = __popc(__ballot_sync(kFull, best > key));
+                if (lane > at) best = up;
+                if (lane == at) best = key;
+                if (lane >= a.n_top) best = 0;
+            }
+            __syncwarp();
+        }
+        news = 0;
+        const uint32_t own = __shfl_sync(kFull, (uint32_t)(best >> 32), a.n_top - 1);     // (0: there are not so many yet)
+        if (own == 0) return;
+        if (lane == 0) atomicMax(&s_bound, own);
+        bound = fmaxf(bound, lp_unorder(own + 1));           // (the next number above; of the largest finite one inf)
+    };
+    auto rebase = [&](float top) {
+        if ((top - B) * a.c > 4.0f) {
+            const float d = fmaxf((B - top) * a.c, -256.0f), f = ex2f(d);
+            B = top;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int i = i0 + k * kLpThreads;
-            if (i < n4) {
-                float4 y = x4[i];
-                if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound)
-                    y = make_float4(look(y.x, 4 * i), look(y.y, 4 * i + 1), look(y.z, 4 * i + 2), look(y.w, 4 * i + 3));
-                add(y.x, gz, gt), add(y.y, gz, gt), add(y.z, gz, gt), add(y.w, gz, gt);
+            for (int e = 0; e < 2; e++) {
+                t[e] = f * fmaf(z[e], d, t[e]);
+                z[e] *= f;
             }
         }
-        z += gz;
-        t += gt;
-    }
-    for (int i0 = kept + tid; i0 < n; i0 += 32 * kLpThreads) {
-        float gz = 0.0f, gt = 0.0f;
-        for (int i = i0; i < n && i < i0 + 32 * kLpThreads; i += kLpThreads) add(look(l[i], i), gz, gt);
-        z += gz;
-        t += gt;
-    }
-    z = warp_sum(z);
-    t = warp_sum(t);
-    if (lane == 0) s_z[warp] = z, s_t[warp] = t;
-    __syncthreads();
-    const int listed = s_n;
-    u64 *all = cl.map_shared_rank(s_all, 0) + rank * kLpTop;
-    if (tid < 32) {
-        z = lane < kLpWarps ? s_z[lane] : 0.0f;
-        t = lane < kLpWarps ? s_t[lane] : 0.0f;
-        z = warp_sum(z) + (float)max(s_most - 1, 0);
-        t = warp_sum(t);
-    }
-    cl.barrier_wait(std::move(started));
-    if (tid == 0) {
-        if (m == INFINITY) z = NAN;
-        *cl.map_shared_rank(&s_part[rank], 0) = LpPart{m, z, t};
-    }
-    if (listed <= kLpList) {
-        for (int i = tid; i < listed; i += kLpThreads) {
-            const u64 k = s_list[i];
-            int above = 0;
-            for (int j = 0; j < listed; j++) above += s_list[j] > k;
-            if (above < a.n_top) all[above] = k;
+    };
+    auto add = [&](float v, int e) {                       // to the sums: v, or the largest so far that it replaces
+        const float y = (min_nan(m[e], v) - B) * a.c, w = ex2f(y);
+        m[e] = fmaxf(m[e], v);
+        z[e] += w;
+        t[e] = fmaf(w, fmaxf(y, -256.0f), t[e]);           // (weights below 2^-126 are 0; 0 * inf is not)
+    };
+    if (rank == 0 && warp == 0) {                                      // the values before the first boundary
+        const float v = lane < head ? row[lane] : -INFINITY;
+        rebase(v);
+        if (a.n_top > 0) {
+            look(v, lane);
+            raise();
         }
-    } else {
-        u64 last = ~0ull;
-        for (int q = 0; q < a.n_top; q++) {
-            u64 best = 0;
-            auto offer = [&](float v, int i) {
-                if (v >= bound) {                          // (NaN is not)
-                    const u64 k = lp_key(v, lo + i);
-                    if (k < last && k > best) best = k;
+        add(v, 0);
+    }
+    bool gave_up = false;
+    for (int k = 0, slot = 0, phase = 0; k < chunks; k++) {
+        for (uint32_t n = 0; !gave_up && !mbar_try_wait(&s_full[warp][slot], phase); n++) {
+            gave_up = n == kLpSpin;
+            if (n > 64) __nanosleep(32);
+        }
+        if ((gave_up = __any_sync(kFull, gave_up))) {      // the copies have 0.1 s to land before this CTA's memory goes
+            for (int n = 0; n < 1 << 20; n++) __nanosleep(100);
+            if (lane == 0) s_abort = 1;
+            break;
+        }
+        const int base = lo + (k * kLpWarps + warp) * kLpChunk, n4 = min(kLpChunk, hi - base) >> 2;
+        const float4 *x4 = reinterpret_cast<const float4 *>(ring + slot * kLpChunk);
+        float4 y[kLpQuads];
+        float top[kLpQuads];
+#pragma unroll
+        for (int e = 0; e < kLpQuads; e++) {
+            const int i = lane + e * 32;
+            y[e] = i < n4 ? x4[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            top[e] = fmaxf(fmaxf(y[e].x, y[e].y), fmaxf(y[e].z, y[e].w));
+        }
+        static_assert(kLpQuads == 4, "the largest of 4 groups");
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        rebase(most);
+#pragma unroll
+        for (int e = 0; e < kLpQuads; e++) add(y[e].x, e & 1), add(y[e].y, e & 1), add(y[e].z, e & 1), add(y[e].w, e & 1);
+        if (a.n_top > 0) {
+            if (k == 0) {                                  // the n_top-th of the lanes' largest (NaN is none)
+                uint32_t o = lp_order(fmaxf(most, -INFINITY)), at = __reduce_max_sync(kFull, o);
+                for (int i = 1; i < a.n_top; i++) {
+                    if (lane == __ffs(__ballot_sync(kFull, o == at)) - 1) o = 0;
+                    at = __reduce_max_sync(kFull, o);
                 }
-            };
-            for (int i = tid; i < kept; i += kLpThreads) offer(x[i], i);
-            for (int i = kept + tid; i < n; i += kLpThreads) offer(l[i], i);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const u64 other = __shfl_xor_sync(kFull, best, o);
-                best = other > best ? other : best;
+                bound = fmaxf(bound, at == 0 ? -FLT_MAX : lp_unorder(at));
             }
-            if (lane == 0) s_key[warp] = best;
-            __syncthreads();
-            for (int w = 0; w < kLpWarps; w++) best = s_key[w] > best ? s_key[w] : best;
-            __syncthreads();
-            if (tid == 0) all[q] = best;
-            last = best;
+            const uint32_t others = *(volatile uint32_t *)&s_bound;      // what another warp has found
+            if (others != 0) bound = fmaxf(bound, lp_unorder(others));
+            if (__any_sync(kFull, most >= bound)) {
+#pragma unroll
+                for (int e = 0; e < kLpQuads; e++) {
+                    if (!__any_sync(kFull, top[e] >= bound)) continue;
+                    const int i = base + 4 * (lane + e * 32);
+                    look(y[e].x, i), look(y[e].y, i + 1), look(y[e].z, i + 2), look(y[e].w, i + 3);
+                }
+                raise();
+            }
         }
+        __syncwarp();
+        if (lane == 0 && k + kLpRing < chunks) {
+            fence_async_smem();
+            load(k + kLpRing);
+        }
+        if (++slot == kLpRing) slot = 0, phase ^= 1;
+    }
+    if (rank == nc - 1 && warp == kLpWarps - 1) {                             // the values behind the last group
+        const float v = tail + lane < a.V ? row[tail + lane] : -INFINITY;
+        rebase(v);
+        if (a.n_top > 0) {
+            look(v, tail + lane);
+            raise();
+        }
+        add(v, 0);
+    }
+
+    // ---- lanes to warps, warps to the CTA
+    LpPart p;
+    {
+        const bool second = m[1] > m[0];                   // of the two maxima one joins the sums
+        const float y = ((second ? m[0] : m[1]) - B) * a.c, w = ex2f(y);
+        p.m = second ? m[1] : m[0];
+        p.z = z[0] + z[1] + w;
+        p.t = fmaf(w, fmaxf(y, -256.0f), t[0] + t[1]);
+        const float d = p.m == -INFINITY ? 0.0f : (B - p.m) * a.c, f = ex2f(d);            // from the base to the maximum
+        p.t = f * fmaf(p.z, d, p.t);
+        p.z *= f;
+    }
+    auto join = [&](LpPart p) {                            // of a warp's lanes
+        const uint32_t k = lp_order(p.m), most = __reduce_max_sync(kFull, k);
+        const int first = __ffs(__ballot_sync(kFull, k == most)) - 1;
+        p = lp_under(p, lp_unorder(most), lane == first, a.c);
+        p.z = warp_sum(p.z);
+        p.t = warp_sum(p.t);
+        p.m = lp_unorder(most);
+        return p;
+    };
+    p = join(p);
+    if (lane == 0) s_warp[warp] = p;
+    s_list[tid] = best;
+    cl.barrier_wait(std::move(started));
+    __syncthreads();
+    if (warp == 0) {
+        p = join(lane < kLpWarps ? s_warp[lane] : LpPart{-INFINITY, 0.0f, 0.0f});
+        if (s_abort || p.m == INFINITY) p.z = NAN;
+        if (lane == 0) *cl.map_shared_rank(&s_part[rank], 0) = p;
+    }
+    if (best != 0) {
+        const int above = lp_above(s_list, kLpWarps, best);
+        if (above < a.n_top) cl.map_shared_rank(s_all, 0)[rank * kLpTop + above] = best;
     }
     cl.sync();
+    if (s_abort && tid == 0 && a.err) atomicOr(a.err, QMS_PAGED_ETIMEOUT);
     if (rank != 0) return;
 
     // ---- the row: parts and lists joined
-    m = -INFINITY;
-    int first = 0;
-    for (int k = nc - 1; k >= 0; k--)
-        if (s_part[k].m >= m) m = s_part[k].m, first = k;
-    z = t = 0.0f;
-    for (int k = 0; k < nc; k++) {
-        const LpPart p = s_part[k];
-        if (k == first || p.m == -INFINITY) {              // (of a slice of -inf alone z is 0, or NaN)
-            z += p.z;
-            t += p.t;
-        } else {
-            const float d = (p.m - m) * a.c, f = ex2f(d), one = p.z + 1.0f;
-            z = fmaf(one, f, z);
-            t = fmaf(f, fmaf(one, fmaxf(d, -256.0f), p.t), t);
-        }
-    }
-    const bool none = m == -INFINITY && !isnan(z);         // a row of -inf
-    const float lz = log1pf(z);
-    auto logp = [&](float v) { return none || v == -INFINITY ? (isnan(z) ? NAN : -INFINITY) : __fdiv_rn(v - m, a.temp) - lz; };
+    p = join(lane < nc ? s_part[lane] : LpPart{-INFINITY, 0.0f, 0.0f});
+    const bool none = p.m == -INFINITY && !isnan(p.z);     // a row of -inf
+    const float lz = log1pf(p.z);
+    auto logp = [&](float v) { return none || v == -INFINITY ? (isnan(p.z) ? NAN : -INFINITY) : __fdiv_rn(v - p.m, a.temp) - lz; };
     for (int i = tid; i < a.n_ids; i += kLpThreads) {
         const int id = a.ids[r * a.n_ids + i];
         const bool good = (unsigned)id < (unsigned)a.V;
         if (!good && a.err) atomicOr(a.err, QMS_PAGED_ETOKEN);
-        a.lp[r * a.n_ids + i] = good ? logp(__ldcg(row + id)) : NAN;
+        a.lp[r * a.n_ids + i] = good ? logp(i < kLpThreads ? mine : row[id]) : NAN;
     }
-    if (tid == 0 && a.entropy) a.entropy[r] = none ? 0.0f : lz - 0.69314718056f * t / (1.0f + z);
+    if (tid == 0 && a.entropy) a.entropy[r] = none ? 0.0f : lz - 0.69314718056f * p.t / (1.0f + p.z);
     if (a.n_top == 0) return;
     const u64 k = tid < nc * kLpTop ? s_all[tid] : 0;
     const int found = __syncthreads_count(k != 0);
     if (k != 0) {
-        int above = 0;
-        for (int i = 0; i < nc; i++)
-            for (int j = 0; j < a.n_top; j++) above += s_all[i * kLpTop + j] > k;
+        const int above = lp_above(s_all, nc, k);
         if (above < a.n_top) {
             a.top_id[r * a.n_top + above] = (int)~(uint32_t)k;
             a.top_lp[r * a.n_top + above] = logp(lp_value(k));
@@ -248,16 +320,18 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_logprobs(const LogprobArgs a)
     }
     if (tid >= found && tid < a.n_top) {
         a.top_id[r * a.n_top + tid] = -1;
-        a.top_lp[r * a.n_top + tid] = isnan(z) ? NAN : -INFINITY;
+        a.top_lp[r * a.n_top + tid] = isnan(p.z) ? NAN : -INFINITY;
     }
 }
 
 static int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t s) {
+    constexpr int smem = kLpWarps * kLpRing * kLpChunk * 4;
     static std::atomic<unsigned long long> done{0};
-    const int rc = allow_smem(done, k_logprobs, kProbsKeep * 4);
+    const int rc = allow_smem(done, k_logprobs, smem);
     if (rc) return rc;
-    const int nc = row_ctas(rows, a.V, 74), slice = ((a.V + 3) / 4 / nc + 1) * 4;
-    const size_t smem = (size_t)(slice < kProbsKeep ? slice : kProbsKeep) * 4;
+    // CTAs per row: at most 8, a warp's piece a chunk at least, and as many as fill the device
+    int nc = 1;
+    while (nc < kRowCtas && a.V > nc * kLpWarps * kLpChunk && (int64_t)rows * nc < 500) nc *= 2;
     return launch_rows(k_logprobs, kLpThreads, rows, nc, smem, s, a);
 }
 

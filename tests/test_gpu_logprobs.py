@@ -3,7 +3,8 @@
 Bounds, with e = 2^-24, x = (l - max) / temp <= 0, p the probabilities, A = sum p |x|, Q = sum p x^2. A weight 2^(x log2 e) is off by the
 exponent's two roundings, 2 e |x| relatively, and by the exponential's own 4 e; a sum has at most 48 roundings on its way. So Z is off by
 (52 + 2 A) e relatively, log Z by as much, log p by that, three roundings of x, the logarithm's two and the difference's: e (52 + 2 A + 3 |x|
-+ 2 log Z + |log p|). sum p x: every term's weight as above and two roundings more, and Z: e (54 A + 2 Q + (52 + 2 A) A)."""
++ 2 log Z + |log p|). sum p x: every term's weight as above and two roundings more, and Z: e (54 A + 2 Q + (52 + 2 A) A); the logarithms are taken under a base up to 2^4 below
+the largest value so far, which adds up to 4 ln 2 < 3 to each of them: 54 * 3 e more."""
 from __future__ import annotations
 
 import numpy as np
@@ -23,7 +24,7 @@ def _want(l, ids, temp):
     A, Q = -px.sum(-1, keepdim=True), torch.where(p > 0, px * x, 0.0).sum(-1, keepdim=True)
     lp = x - lz
     tol = E * (52 + 2 * A + 3 * x.abs() + 2 * lz + lp.abs())
-    ent, tol_ent = (lz + A)[:, 0], (E * (52 + 2 * A + 2 * lz + 54 * A + 2 * Q + (52 + 2 * A) * A + 2 * (lz + A)))[:, 0]
+    ent, tol_ent = (lz + A)[:, 0], (E * (52 + 2 * A + 2 * lz + 54 * (A + 3) + 2 * Q + (52 + 2 * A) * A + 2 * (lz + A)))[:, 0]
     return lp, tol, ent, tol_ent
 
 
