@@ -307,26 +307,12 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
             const bool masked = base + C::PS - 1 > seen || base < first;
             unsigned char *raw = sm + c % C::NS * C::STAGE;
             uint32_t kb = sm0 + c % C::NS * C::STAGE, vb = kb + C::STAGE / 2;
-            if constexpr (C::F16) {
-                if (masked) {                     // behind the mask a weight is 0, but 0 * inf is not
-                    for (int i = tid; i < C::PS * C::CH; i += 128) {
-                        const int r = i / C::CH, p = base + r;
-                        if (p >= first && p <= seen) continue;
-                        uint4 *pv = reinterpret_cast<uint4 *>(raw + C::STAGE / 2 + C::piece(r, i % C::CH));
-                        uint4 v = *pv;
-                        if (drop_nonfinite((const KT *)nullptr, v)) {
-                            *pv = v;
-                            if (p >= first && p < k1) s_flag = 1;      // (else left over from before: nobody's)
-                        }
-                    }
-                    fence_async_smem();
-                    __syncthreads();
-                }
-            } else if constexpr (C::P4) {
+            if constexpr (C::P4) {
                 // 32 values with one scale at a time, 16 bytes, to fp16. A group's four pieces go out in an order that lets 8 lanes
-                // write to all banks (the halves of a row lie on the same ones).
+                // write to all banks (the halves of a row lie on the same ones). Not unrolled: with the loops' 4 groups and the look
+                // behind the mask in line, half of all warps' time went into waiting for instructions.
                 constexpr int GR = D / 32, N = C::PS * GR / 128;   // groups per row, of K and of V per thread
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < 2 * N; i++) {
                     const int at = tid + 128 * (i % N), r = at / GR, g = at % GR, is_v = i / N;
                     const unsigned char *src = raw + is_v * (C::STAGE / 2);
@@ -335,18 +321,30 @@ __global__ void __launch_bounds__(128, PaCfg<D, KT, WR>::MINB) k_paged_attn(cons
                     const int turn = g & 2;
                     if (turn) w = make_uint4(w.z, w.w, w.x, w.y);
                     const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                    const int p = base + r;
-                    const bool look = masked && is_v && (p < first || p > seen);    // behind the mask a weight is 0, but 0 * inf is not
+                    unsigned char *dst = sm + C::CONV + is_v * C::HTILE;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint4 y = q4_dequant(ww[k], d, m24);
-                        if (look && drop_nonfinite((const __half *)nullptr, y) && p >= first && p < k1) s_flag = 1;
-                        *reinterpret_cast<uint4 *>(sm + C::CONV + is_v * C::HTILE + C::piece(r, 4 * g + (k ^ turn))) = y;
-                    }
+                    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4 *>(dst + C::piece(r, 4 * g + (k ^ turn))) = q4_dequant(ww[k], d, m24);
                 }
                 __syncthreads();
                 kb = sm0 + C::CONV;
                 vb = kb + C::HTILE;
+            }
+            if constexpr (!C::F32) {
+                if (masked) {                     // behind the mask a weight is 0, but 0 * inf is not
+                    unsigned char *vt = C::P4 ? sm + C::CONV + C::HTILE : raw + C::STAGE / 2;
+                    for (int i = tid; i < C::PS * (D / 8); i += 128) {
+                        const int r = i / (D / 8), p = base + r;
+                        if (p >= first && p <= seen) continue;
+                        uint4 *pv = reinterpret_cast<uint4 *>(vt + C::piece(r, i % (D / 8)));
+                        uint4 v = *pv;
+                        if (drop_nonfinite((const __half *)nullptr, v)) {
+                            *pv = v;
+                            if (p >= first && p < k1) s_flag = 1;      // (else left over from before: nobody's)
+                        }
+                    }
+                    if constexpr (C::F16) fence_async_smem();
+                    __syncthreads();
+                }
             } else {
                 // hi and lo: K by rows, each with a scale of its own (undone in its scores), V with the largest scale so
                 // far of what somebody sees (o is in its units)

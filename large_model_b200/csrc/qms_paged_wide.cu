@@ -707,23 +707,29 @@ __global__ void __maxnreg__((WideCfg<D, MODE>::REGS)) k_paged_wide(const PagedAt
                     ok = __all_sync(kFull, ok && (c < 3 || sy.wait(&empty[c % 3], (c / 3 - 1) & 1)));
                     if (ok) {
                         unsigned char *dst = sm + C::RING + c % 3 * C::SLOT;
-#pragma unroll
-                        for (int i = 0; i < N; i++) {
-                            const int at = ct + 128 * i, r = at / GR, g = at % GR, turn = g & 2, p = base + r;
+#pragma unroll 1
+                        for (int i = 0; i < N; i++) {          // (in line four times, the warps waited for instructions)
+                            const int at = ct + 128 * i, r = at / GR, g = at % GR, turn = g & 2;
                             uint4 x = *reinterpret_cast<const uint4 *>(src + at * 16);
                             const __half2 d = __half2half2(reinterpret_cast<const __half *>(src + C::TP * (D / 2))[at]), m24 = __hmul2(d, __float2half2_rn(-24.0f));
                             if (turn) x = make_uint4(x.z, x.w, x.x, x.y);
                             const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
-                            const bool in = !look || (p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1)), part = look && is_v && p > seen;
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                uint4 y = q4_dequant(xx[k], d, m24);
-                                if (!in) y = make_uint4(0, 0, 0, 0);
-                                if (part && drop_nonfinite((const __half *)nullptr, y)) *s_flag = 1;
                                 const int q = 4 * g + (k ^ turn);
-                                *reinterpret_cast<uint4 *>(dst + (q >> 3) * C::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4)) = y;
+                                *reinterpret_cast<uint4 *>(dst + (q >> 3) * C::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4)) = q4_dequant(xx[k], d, m24);
                             }
                         }
+                        if (look)                              // what this thread wrote, again
+#pragma unroll 1
+                            for (int i = 0; i < 4 * N; i++) {
+                                const int at = ct + 128 * (i >> 2), r = at / GR, q = at % GR * 4 + (i & 3), p = base + r;
+                                const bool in = p >= w.kmin && p < w.k1 && !(bad[r >> 5] >> (r & 31) & 1);
+                                uint4 *py = reinterpret_cast<uint4 *>(dst + (q >> 3) * C::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+                                uint4 y = in ? *py : make_uint4(0, 0, 0, 0);
+                                if (in && is_v && p > seen && drop_nonfinite((const __half *)nullptr, y)) *s_flag = 1;
+                                *py = y;
+                            }
                     }
                     fence_async_smem();
                     mbar_arrive(&full[2 * is_v + (t & 1)]);
