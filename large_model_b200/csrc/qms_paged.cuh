@@ -241,6 +241,7 @@ int paged_map(const Paged &a, int D, bool f16, int rows, const char *pool, CUten
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p);
 int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p);
 int launch_paged_wide(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s);     // qms_paged_wide.cu
+int launch_paged_q4(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s);       // qms_paged_q4.cu
 int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, const float *q, int64_t ldq, float scale,
                            float *out, int64_t ldo, void *ws, cudaStream_t s);
 

@@ -949,10 +949,17 @@ static int launch_attn(const PagedAttn &A, cudaStream_t s) {
         const bool own = kind == 1;
         if (own ? !(A.p.chunks_s && A.p.tiles_s && A.a.n_seq) : !(A.p.chunks_p && A.p.tiles_p)) continue;
         const int wr = own ? A.p.wr_s : A.p.wr_p;
-        const int rc = wr <= 0   ? launch_paged_wide(A, D, own, before, s)
-                       : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
-                       : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
-                                 : launch_attn_wr<D, KT, 1>(A, own, before, s);
+        int rc;
+        if constexpr (std::is_same<KT, Q4>::value)
+            rc = wr <= 0   ? launch_paged_wide(A, D, own, before, s)
+                 : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
+                 : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
+                           : launch_paged_q4(A, D, own, before, s);
+        else
+            rc = wr <= 0   ? launch_paged_wide(A, D, own, before, s)
+                 : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
+                 : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
+                           : launch_attn_wr<D, KT, 1>(A, own, before, s);
         if (rc) return rc;
         before = true;
     }
