@@ -19,8 +19,7 @@
 
 namespace qms {
 
-constexpr uint32_t kQ4Spin = 1u << 22;
-constexpr float kQ4Shift = 8.0f;      // weights reach 2^8: their fp16 low terms stay clear of the subnormals
+constexpr float kQ4Shift = 8.0f, kQ4High = 7.0f;      // weights reach 2^8, from there up to 2^15: their fp16 low terms stay clear of the subnormals
 
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -32,9 +31,10 @@ __device__ __forceinline__ void mma_16_first(float (&c)[4], const uint32_t (&a)[
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// The pair of nibbles at bits 4 e and 16 + 4 e as d (n - 8).
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w, int e, __half2 d, __half2 m24) {
-    const uint32_t x = ((e == 0 ? w << 6 : e == 1 ? w << 2 : e == 2 ? w >> 2 : w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+// The pair of nibbles at bits 4 e and 16 + 4 e as d (n - 8). six: 0x4C004C00, in a register (two constants in one step need one).
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w, int e, __half2 d, __half2 m24, uint32_t six) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, 0x03C003C0, %2, 0xEA;" : "=r"(x) : "r"(e == 0 ? w << 6 : e == 1 ? w << 2 : e == 2 ? w >> 2 : w >> 6), "r"(six));
     const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&x), d, m24);
     return *reinterpret_cast<const uint32_t *>(&y);
 }
@@ -42,10 +42,11 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t w, int e, __half2 d, __half
 template <int D>
 struct Q4Cfg {
     static constexpr int NIB = 16 * (D / 2), SC = 16 * (D / 16), TILE = NIB + SC;      // bytes of a tile of 16 positions, of K or of V
-    static constexpr int STAGE = 4 * TILE, NS = 3;                                      // two tiles of K and V, in flight per warp
+    static constexpr int STAGE = 4 * TILE, NS = 2;                                      // two tiles of K and V; stages per warp
     static constexpr int RING = 4 * NS * STAGE;
     static constexpr int LD = D / 8 * 9 + 2;                                            // the warps' o, m, l: 9 per 8 values (banks)
-    static constexpr int RED = 4 * 16 * LD * 4, SMEM = (RING > RED ? RING : RED) + 128;
+    static constexpr int RED = 4 * 16 * LD * 4, Q = (RING > RED ? RING : RED) + 127 & ~127;
+    static constexpr int SMEM = Q + D / 16 * 2 * 512 + 128;                             // q as A operands: [step][hi, lo][lane]
 };
 
 template <int D>
@@ -53,19 +54,12 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
     using C = Q4Cfg<D>;
     constexpr int KS = D / 16, W = D / 32, VW = D / 64;      // steps of 16 values; words of K per thread and position, of V
     extern __shared__ unsigned char sm_[];
-    __shared__ uint64_t s_full[4][C::NS];
     __shared__ int s_pos[16], s_tok[16];          // position of each row of the tile; token row * H + q head (-1: none)
-    __shared__ int s_flag, s_abort;               // V had values that are not finite behind the mask
+    __shared__ int s_flag;                        // V had values that are not finite behind the mask
     const Paged &a = A.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
     unsigned char *sm = sm_ + (-smem_u32(sm_) & 127);
     unsigned char *ring = sm + warp * C::NS * C::STAGE;
-    if (lane == 0) {
-        for (int i = 0; i < C::NS; i++) mbar_init(&s_full[warp][i], 1);
-        fence_mbar_init();
-    }
-    if (tid == 0) s_abort = 0;
-    uint32_t slot = 0, phase = 0;                 // where the next stage is read
     // the trigger comes after the wait: a kernel that starts on it may read what this one waited for
     if (!last) pdl_wait();
     pdl_trigger();
@@ -93,7 +87,6 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
         }
         const int *table = a.table + (own ? (int64_t)b * a.table_stride : 0);
         const int kmin = own ? max(k0, a.prefix) : k0, r0 = tile * 16;
-        fence_async_smem();
         __syncthreads();                          // the previous unit is done with shared memory
         if (tid == 0) s_flag = 0;
         if (own) {
@@ -124,45 +117,49 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
         const int hi_pos = __reduce_max_sync(kFull, pos_l), lo_pos = __reduce_min_sync(kFull, pos_l < 0 ? 0x7fffffff : pos_l);
         if (kmin > hi_pos) continue;              // nobody sees any of it (the same for all warps)
         const int k_end = min(k1, hi_pos + 1), nst = (k_end - k0 - warp * 16 + 127) / 128;       // stages in which this warp has positions
-        // A stage: positions k0 + 128 st + 16 warp .. + 15, and 64 further; lane = tile * 4 + what: nibbles of K, of V, scales of K, of V.
-        // A tile lies in one page. Which tiles there are, and on good pages, is kept in bits 2 (st % 16) on.
+        // A stage: tile 0, positions k0 + 128 st + 16 warp .. + 15, and tile 1, 64 further; each lies in one page. Which tiles there are,
+        // and on good pages, is kept in bits 2 (st % 16) on. Plain asynchronous copies: eight bulk copies of 128 bytes to 1 KB per stage
+        // were what the kernel waited for.
         uint32_t tiles = 0;
-        int page = -1;
+        int page = -1;                            // lane x: of tile x
         auto look_up = [&](int st) {
-            const int p = k0 + st * 128 + (lane >> 2 & 1) * 64 + warp * 16;
-            page = lane < 8 && st < nst && p < k_end ? table[p >> a.page_log] : -2;            // -2: nothing there
+            const int p = k0 + st * 128 + (lane & 1) * 64 + warp * 16;
+            page = lane < 2 && st < nst && p < k_end ? table[p >> a.page_log] : -2;            // -2: nothing there
         };
         auto load = [&](int st, uint32_t at) {    // (its pages have been looked up)
             const bool there = (unsigned)page < (unsigned)a.n_pages;
-            if (lane < 8 && page != -2 && !there) paged_err(a, QMS_PAGED_EPAGE);
-            const uint32_t good = __ballot_sync(kFull, there);
-            const uint32_t two = (good & 1) | (good >> 3 & 2);
+            if (page != -2 && !there) paged_err(a, QMS_PAGED_EPAGE);
+            const uint32_t two = __ballot_sync(kFull, there) & 3;
             tiles = (tiles & ~(3u << 2 * (st & 15))) | two << 2 * (st & 15);
-            uint64_t *bar = &s_full[warp][at];
-            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(two) * 2 * C::TILE);
-            __syncwarp();
-            if (there) {
-                const int x = lane >> 2, is_v = lane & 1, p = k0 + st * 128 + x * 64 + warp * 16, y = p & ((1 << a.page_log) - 1);
-                const char *src = (is_v ? a.v : a.k) + page * a.page_stride + kh * a.head_stride;
-                const uint32_t to = smem_u32(ring + at * C::STAGE + (2 * x + is_v) * C::TILE);
-                if (lane & 2) bulk_load(to + C::NIB, src + (D / 2 << a.page_log) + y * (D / 16), C::SC, bar);
-                else bulk_load(to, src + y * (D / 2), C::NIB, bar);
+            unsigned char *to = ring + at * C::STAGE;
+            int64_t from[2];                      // where a tile's page and head start
+            int y[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                from[x] = __shfl_sync(kFull, page, x) * a.page_stride + kh * a.head_stride;
+                y[x] = (k0 + st * 128 + x * 64 + warp * 16) & ((1 << a.page_log) - 1);
+                if (!(two >> x & 1)) continue;
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+#pragma unroll
+                    for (int c = 0; c < C::NIB / 512; c++)
+                        cp_async16(to + (2 * x + v) * C::TILE + c * 512 + lane * 16, (v ? a.v : a.k) + from[x] + y[x] * (D / 2) + c * 512 + lane * 16);
             }
+            constexpr int N = C::SC / 16;         // 16-byte pieces of a tile's scales
+            const int x = lane / (2 * N), v = lane / N & 1, c = lane % N;
+            if (lane < 4 * N && (two >> x & 1))
+                cp_async16(to + (2 * x + v) * C::TILE + C::NIB + c * 16, (v ? a.v : a.k) + from[x] + (D / 2 << a.page_log) + y[x] * (D / 16) + c * 16);
         };
         look_up(0);
-        uint32_t ahead = slot;
-        for (int st = 0; st < C::NS - 1; st++) {
-            if (st < nst) {
-                load(st, ahead);
-                if (++ahead == C::NS) ahead = 0;
-            }
-            look_up(st + 1);
-        }
+        if (nst > 0) load(0, 0);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        look_up(1);
         // ---- q: rows g and g + 8, this thread's D / 4 values of each; a row scaled by a power of two into fp16's range (undone in the
         // score's factor) and split
-        uint32_t qh[KS][4], ql[KS][4];
+        // (warp w: steps w, w + 4)
         float f[2];
         int pos[2];
+        uint32_t qs[KS / 4][2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int tok = s_tok[g + 8 * h], t = tok < 0 ? 0 : tok / a.H;
@@ -171,7 +168,7 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
             float4 x[KS];
             uint32_t mx = 0;
 #pragma unroll
-            for (int k = 0; k < KS; k++) x[k] = tok < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(src + k);
+            for (int k = 0; k < KS; k++) x[k] = tok < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(src + (k + warp) % KS);
 #pragma unroll
             for (int k = 0; k < KS; k++) mx = max(mx, max(max(finite_bits(x[k].x), finite_bits(x[k].y)), max(finite_bits(x[k].z), finite_bits(x[k].w))));
             mx = max(mx, __shfl_xor_sync(kFull, mx, 1));
@@ -180,145 +177,168 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
             f[h] = A.scale2 * pow2_bits(254u - up);
             const float m = pow2_bits(up);
 #pragma unroll
-            for (int k = 0; k < KS; k++) {        // values 4 k .. 4 k + 3: the two pairs of step k
-                split_h2(x[k].x * m, x[k].y * m, qh[k][h], ql[k][h]);
-                split_h2(x[k].z * m, x[k].w * m, qh[k][2 + h], ql[k][2 + h]);
+            for (int k = 0; k < KS / 4; k++) {    // values 4 k .. 4 k + 3 of step k: its two pairs
+                split_h2(x[4 * k].x * m, x[4 * k].y * m, qs[k][0][h], qs[k][1][h]);
+                split_h2(x[4 * k].z * m, x[4 * k].w * m, qs[k][0][2 + h], qs[k][1][2 + h]);
             }
         }
+        uint4 *s_q = reinterpret_cast<uint4 *>(sm + C::Q);
+#pragma unroll
+        for (int k = 0; k < KS / 4; k++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) s_q[((4 * k + warp) * 2 + e) * 32 + lane] = make_uint4(qs[k][e][0], qs[k][e][1], qs[k][e][2], qs[k][e][3]);
+        __syncthreads();
+        s_q += lane;
         float o[D / 8][4];                        // value 16 n + i (D 64: 8 n + i) of rows g, g + 8 in o[i], n = 2 tq, 2 tq + 1
 #pragma unroll
         for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        bool gave_up = false;
+        uint32_t six;
+        asm volatile("mov.b32 %0, 0x4C004C00;" : "=r"(six));
 #pragma unroll 1
         for (int st = 0; st < nst; st++) {
-            for (uint32_t c = 0; !gave_up && !mbar_try_wait(&s_full[warp][slot], phase); c++) {
-                gave_up = c == kQ4Spin;
-                if (c > 64) __nanosleep(32);
+            __syncwarp();                         // (the other slot was read in the last round)
+            if (st + 1 < nst) {
+                load(st + 1, st + 1 & 1);
+                look_up(st + 2);
             }
-            if ((gave_up = __any_sync(kFull, gave_up))) {      // reported; the copies have 0.1 s to land before this CTA's memory goes
-                if (lane == 0) {
-                    s_abort = 1;
-                    paged_err(a, QMS_PAGED_ETIMEOUT);
-                }
-                for (int c = 0; c < 1 << 20; c++) __nanosleep(100);
-                break;
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
             const uint32_t there = tiles >> 2 * (st & 15);
-            if (st + C::NS - 1 < nst) {           // (the slot before this one was read in the last round)
-                fence_async_smem();
-                __syncwarp();
-                load(st + C::NS - 1, slot == 0 ? C::NS - 1 : slot - 1);
-                look_up(st + C::NS);
-            }
-#pragma unroll 1
-            for (int x = 0; x < 2; x++) {
-                if (!(there >> x & 1)) continue;
-                const int p0 = k0 + st * 128 + x * 64 + warp * 16;
-                const unsigned char *kn = ring + slot * C::STAGE + 2 * x * C::TILE, *vn = kn + C::TILE;
-                // ---- scores: column c of 8-position tile i is position 8 i + (c >> 1) + 4 (c & 1)
-                float s[2][4], s2[2][4];
+            const int base = k0 + st * 128 + warp * 16;        // tile x: positions base + 64 x ..
+            const unsigned char *stage = ring + (st & 1) * C::STAGE;
+            // ---- scores: column c of 8-position tile i is position 64 (i / 2) + 8 (i % 2) + (c >> 1) + 4 (c & 1) from base on
+            float s[4][4], s2[4][4];
+            {
+                uint32_t w[4][W];
+                __half2 d[4], m24[4];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int r = 8 * i + (g >> 1) + 4 * (g & 1);
-                    uint32_t w[W];
-                    if constexpr (D == 128) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(kn + r * 64 + tq * 16);
-                    else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(kn + r * 32 + tq * 8);
-                    const __half2 d = __half2half2(reinterpret_cast<const __half *>(kn + C::NIB)[r * (D / 32) + (D == 128 ? tq : tq >> 1)]);
-                    const __half2 m24 = __hmul2(d, __float2half2_rn(-24.0f));
+                for (int i = 0; i < 4; i++) {
+                    const unsigned char *kn = stage + (i >> 1) * 2 * C::TILE;
+                    const int r = 8 * (i & 1) + (g >> 1) + 4 * (g & 1);
+                    if constexpr (D == 128) *reinterpret_cast<uint4 *>(w[i]) = *reinterpret_cast<const uint4 *>(kn + r * 64 + tq * 16);
+                    else *reinterpret_cast<uint2 *>(w[i]) = *reinterpret_cast<const uint2 *>(kn + r * 32 + tq * 8);
+                    d[i] = __half2half2(reinterpret_cast<const __half *>(kn + C::NIB)[r * (D / 32) + (D == 128 ? tq : tq >> 1)]);
+                    m24[i] = __hmul2(d[i], __float2half2_rn(-24.0f));
+                }
 #pragma unroll
-                    for (int k = 0; k < KS; k++) {
-                        const uint32_t b0 = q4_pair(w[k / 2], 2 * (k & 1), d, m24), b1 = q4_pair(w[k / 2], 2 * (k & 1) + 1, d, m24);
+                for (int k = 0; k < KS; k++) {
+                    const uint4 h4 = s_q[(2 * k) * 32], l4 = s_q[(2 * k + 1) * 32];
+                    const uint32_t qh[4] = {h4.x, h4.y, h4.z, h4.w}, ql[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t b0 = q4_pair(w[i][k / 2], 2 * (k & 1), d[i], m24[i], six), b1 = q4_pair(w[i][k / 2], 2 * (k & 1) + 1, d[i], m24[i], six);
                         if (k == 0) {
-                            mma_16_first(s[i], qh[k], b0, b1);
-                            mma_16_first(s2[i], ql[k], b0, b1);
+                            mma_16_first(s[i], qh, b0, b1);
+                            mma_16_first(s2[i], ql, b0, b1);
                         } else {
-                            mma_16(s[i], qh[k], b0, b1);
-                            mma_16(s2[i], ql[k], b0, b1);
+                            mma_16(s[i], qh, b0, b1);
+                            mma_16(s2[i], ql, b0, b1);
                         }
                     }
                 }
-                // some row does not see all of it
-                const int seen = min(lo_pos, k1 - 1);
-                const bool masked = p0 + 15 > seen || p0 < kmin;
-                float n0 = m0, n1 = m1;
+            }
+            // some row does not see all of it
+            const int seen = (there & 3) == 3 ? min(lo_pos, k1 - 1) : -1;
+            const bool masked = base + 79 > seen || base < kmin;
+            auto gone = [&](int x, int p) { return !(there >> x & 1) || p < kmin || p >= k1; };      // a position of tile x that is no part of it
+            float n0 = -INFINITY, n1 = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s[i][j] = (s[i][j] + s2[i][j]) * f[j >> 1];
-                    if (masked) {
+                for (int j = 0; j < 4; j++) s[i][j] = (s[i][j] + s2[i][j]) * f[j >> 1];
+                if (masked) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int p = p0 + 8 * i + tq + 4 * (j & 1);
-                            if (p < kmin || p >= k1 || p > pos[j >> 1]) s[i][j] = -INFINITY;
-                        }
+                    for (int j = 0; j < 4; j++) {
+                        const int p = base + 64 * (i >> 1) + 8 * (i & 1) + tq + 4 * (j & 1);
+                        if (gone(i >> 1, p) || p > pos[j >> 1]) s[i][j] = -INFINITY;
                     }
-                    n0 = fmaxf(n0, fmaxf(s[i][0], s[i][1]));
-                    n1 = fmaxf(n1, fmaxf(s[i][2], s[i][3]));
                 }
+                n0 = fmaxf(n0, fmaxf(s[i][0], s[i][1]));
+                n1 = fmaxf(n1, fmaxf(s[i][2], s[i][3]));
+            }
+            // the base of the weights stays until a score lies 2^kQ4High above it (in short units nearly every stage holds some row's
+            // new maximum)
+            if (__any_sync(kFull, n0 > m0 + kQ4High || n1 > m1 + kQ4High)) {
                 n0 = fmaxf(n0, __shfl_xor_sync(kFull, n0, 1));
                 n1 = fmaxf(n1, __shfl_xor_sync(kFull, n1, 1));
-                n0 = fmaxf(n0, __shfl_xor_sync(kFull, n0, 2));
-                n1 = fmaxf(n1, __shfl_xor_sync(kFull, n1, 2));
-                if (__any_sync(kFull, n0 != m0 || n1 != m1)) {
-                    const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
-                    l0 *= d0;
-                    l1 *= d1;
+                n0 = fmaxf(m0, fmaxf(n0, __shfl_xor_sync(kFull, n0, 2)));
+                n1 = fmaxf(m1, fmaxf(n1, __shfl_xor_sync(kFull, n1, 2)));
+                const float d0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), d1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
+                l0 *= d0;
+                l1 *= d1;
 #pragma unroll
-                    for (int i = 0; i < D / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
-                    m0 = n0;
-                    m1 = n1;
-                }
-                const float b0 = n0 == -INFINITY ? 0.0f : n0 - kQ4Shift, b1 = n1 == -INFINITY ? 0.0f : n1 - kQ4Shift;
-                uint32_t ph[4], pl[4];
+                for (int i = 0; i < D / 8; i++) o[i][0] *= d0, o[i][1] *= d0, o[i][2] *= d1, o[i][3] *= d1;
+                m0 = n0;
+                m1 = n1;
+            }
+            const float b0 = m0 == -INFINITY ? 0.0f : m0 - kQ4Shift, b1 = m1 == -INFINITY ? 0.0f : m1 - kQ4Shift;
+            uint32_t ph[2][4], pl[2][4];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    s[i][0] = ex2(s[i][0] - b0), s[i][1] = ex2(s[i][1] - b0);
-                    s[i][2] = ex2(s[i][2] - b1), s[i][3] = ex2(s[i][3] - b1);
-                    l0 += s[i][0] + s[i][1];
-                    l1 += s[i][2] + s[i][3];
-                    split_h2(s[i][0], s[i][1], ph[2 * i], pl[2 * i]);
-                    split_h2(s[i][2], s[i][3], ph[2 * i + 1], pl[2 * i + 1]);
-                }
-                // ---- o += weights * V: of positions tq, 4 + tq (a pair), 8 + tq, 12 + tq
-                uint32_t w[4][VW];
-                __half d[4];
+            for (int i = 0; i < 4; i++) {
+                s[i][0] = ex2(s[i][0] - b0), s[i][1] = ex2(s[i][1] - b0);
+                s[i][2] = ex2(s[i][2] - b1), s[i][3] = ex2(s[i][3] - b1);
+                l0 += s[i][0] + s[i][1];
+                l1 += s[i][2] + s[i][3];
+                split_h2(s[i][0], s[i][1], ph[i >> 1][2 * (i & 1)], pl[i >> 1][2 * (i & 1)]);
+                split_h2(s[i][2], s[i][3], ph[i >> 1][2 * (i & 1) + 1], pl[i >> 1][2 * (i & 1) + 1]);
+            }
+            // ---- o += weights * V: of each tile positions tq, 4 + tq (a pair), 8 + tq, 12 + tq; the tensor cores add up a stage, from 0
+            // (they cut bits off), and its sums join o by additions that round
+            uint32_t w[2][4][VW];
+            __half2 d[2][2], m24[2][2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const unsigned char *vn = stage + (2 * x + 1) * C::TILE;
+                __half e[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int r = 4 * i + tq;
-                    if constexpr (D == 128) *reinterpret_cast<uint2 *>(w[i]) = *reinterpret_cast<const uint2 *>(vn + r * 64 + g * 8);
-                    else w[i][0] = *reinterpret_cast<const uint32_t *>(vn + r * 32 + g * 4);
-                    d[i] = reinterpret_cast<const __half *>(vn + C::NIB)[r * (D / 32) + (D == 128 ? g >> 1 : g >> 2)];
+                    if constexpr (D == 128) *reinterpret_cast<uint2 *>(w[x][i]) = *reinterpret_cast<const uint2 *>(vn + r * 64 + g * 8);
+                    else w[x][i][0] = *reinterpret_cast<const uint32_t *>(vn + r * 32 + g * 4);
+                    e[i] = reinterpret_cast<const __half *>(vn + C::NIB)[r * (D / 32) + (D == 128 ? g >> 1 : g >> 2)];
                 }
                 if (masked)                       // behind the mask a weight is 0, but 0 * inf is not
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int p = p0 + 4 * i + tq;
-                        if ((p < kmin || p > seen) && (__half_as_ushort(d[i]) & 0x7C00u) == 0x7C00u) {
-                            if (p >= kmin && p < k1) s_flag = 1;   // (else nobody's)
-                            d[i] = __float2half(0.0f);
+                        const int p = base + 64 * x + 4 * i + tq;
+                        const bool none = gone(x, p);
+                        if (none || (p > seen && !(fabsf(__half2float(e[i])) <= kQ4Most))) {
+                            if (!none) s_flag = 1;         // (else nobody's)
+                            e[i] = __float2half(0.0f);
                         }
                     }
-                const __half2 d0 = __halves2half2(d[0], d[1]), d1 = __halves2half2(d[2], d[3]);
-                const __half2 e0 = __hmul2(d0, __float2half2_rn(-24.0f)), e1 = __hmul2(d1, __float2half2_rn(-24.0f));
-#pragma unroll
-                for (int i = 0; i < VW; i++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) { // values 0, 2, 4, 6 and 1, 3, 5, 7 of a word
-                        const uint32_t w0 = __byte_perm(w[0][i], w[1][i], h ? 0x7632 : 0x5410), w1 = __byte_perm(w[2][i], w[3][i], h ? 0x7632 : 0x5410);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float(&y)[4] = o[8 * i + 2 * e + h];
-                            const uint32_t v0 = q4_pair(w0, e, d0, e0), v1 = q4_pair(w1, e, d1, e1);
-                            float t[4];
-                            mma_16_first(t, pl, v0, v1);
-                            mma_16(t, ph, v0, v1);
-                            const float2 lo = f2_add(make_float2(y[0], y[1]), make_float2(t[0], t[1])), hi = f2_add(make_float2(y[2], y[3]), make_float2(t[2], t[3]));
-                            y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
-                        }
-                    }
+                d[x][0] = __halves2half2(e[0], e[1]);
+                d[x][1] = __halves2half2(e[2], e[3]);
+                m24[x][0] = __hmul2(d[x][0], __float2half2_rn(-24.0f));
+                m24[x][1] = __hmul2(d[x][1], __float2half2_rn(-24.0f));
             }
-            if (++slot == C::NS) slot = 0, phase ^= 1;
+#pragma unroll
+            for (int i = 0; i < VW; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {     // values 0, 2, 4, 6 and 1, 3, 5, 7 of a word
+                    uint32_t v[2][2];
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        v[x][0] = __byte_perm(w[x][0][i], w[x][1][i], h ? 0x7632 : 0x5410);
+                        v[x][1] = __byte_perm(w[x][2][i], w[x][3][i], h ? 0x7632 : 0x5410);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float t[4];
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t v0 = q4_pair(v[x][0], e, d[x][0], m24[x][0], six), v1 = q4_pair(v[x][1], e, d[x][1], m24[x][1], six);
+                            if (x == 0) mma_16_first(t, pl[x], v0, v1);
+                            else mma_16(t, pl[x], v0, v1);
+                            mma_16(t, ph[x], v0, v1);
+                        }
+                        float(&y)[4] = o[8 * i + 2 * e + h];
+                        const float2 lo = f2_add(make_float2(y[0], y[1]), make_float2(t[0], t[1])), hi = f2_add(make_float2(y[2], y[3]), make_float2(t[2], t[3]));
+                        y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
+                    }
+                }
         }
         l0 += __shfl_xor_sync(kFull, l0, 1);
         l1 += __shfl_xor_sync(kFull, l1, 1);
@@ -327,7 +347,6 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
         if (isnan(l0)) m0 = 0.0f;                 // scores that are all NaN leave no maximum, but are not nothing
         if (isnan(l1)) m1 = 0.0f;
         __syncthreads();                          // every warp is done with its stages
-        if (s_abort) break;
         if (s_flag) {
             // V that were set aside: added where the row sees them (inf and NaN are not changed by a weight), by the warp that scored the
             // position: the join leaves out warps that saw nothing
