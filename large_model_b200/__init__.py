@@ -481,8 +481,9 @@ def _device_of(t):
 
 
 def _one_device(who: str, t, *others):
+    d = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != d:
             raise ValueError(f"{who}: tensors on {t.device} and {o.device}")
 
 
@@ -718,13 +719,12 @@ def prompt_append(pages: KvPages | None, batch: PagedBatch, qkv, n_head: int, q_
 
 def _heads(t, n_tok: int, what: str):
     """A CUDA tensor [tokens][heads][head_dim] as QmsCudaHeads, the last dimension contiguous."""
-    if t.dim() != 3 or t.shape[0] < n_tok or (t.stride(2) != 1 and t.shape[2] > 1) or not t.is_cuda:
-        raise ValueError(f"{what}: a CUDA tensor [{n_tok} tokens][heads][head_dim] with contiguous values is needed, got {tuple(t.shape)} on "
-                         f"{t.device}, strides {tuple(t.stride())}")
-    n, h, d = t.shape
-    st, sh = t.stride(0), t.stride(1)
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or sh[0] < n_tok or (st[2] != 1 and sh[2] > 1) or not t.is_cuda:
+        raise ValueError(f"{what}: a CUDA tensor [{n_tok} tokens][heads][head_dim] with contiguous values is needed, got {tuple(sh)} on "
+                         f"{t.device}, strides {tuple(st)}")
     # (the stride of a dimension of one has no meaning)
-    return HeadsDesc(t.data_ptr(), st if n > 1 else max(h * d, d), sh if h > 1 else d)
+    return HeadsDesc(t.data_ptr(), st[0] if sh[0] > 1 else sh[1] * sh[2], st[1] if sh[1] > 1 else sh[2])
 
 
 def prompt_attention(batch: PagedBatch, q, k, v, scale: float | None = None, out=None, out_dtype=None, stream=None):
@@ -733,21 +733,23 @@ def prompt_attention(batch: PagedBatch, q, k, v, scale: float | None = None, out
     of prompt_append's rows; scale defaults to 1 / sqrt(head_dim). Returns [n_tok][n_head][head_dim] of q's type, or out_dtype =
     torch.float32; out may be q. Rows behind the last prompt are left as they were."""
     torch = _torch()
-    n, H, D = q.shape
-    typ = {torch.float16: T_F16, torch.bfloat16: T_BF16}.get(q.dtype)
-    if typ is None or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt, ks = q.dtype, k.shape
+    typ = T_BF16 if dt is torch.bfloat16 else T_F16 if dt is torch.float16 else None
+    if typ is None or k.dtype is not dt or v.dtype is not dt:
         raise ValueError(f"prompt_attention: float16 or bfloat16, one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.shape != v.shape or k.dim() != 3 or k.shape[2] != D:
+    if q.dim() != 3 or len(ks) != 3 or v.shape != ks or ks[2] != q.shape[2]:
         raise ValueError(f"prompt_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    n, H, D = q.shape
     if out is None:
-        out = _empty((batch.n_tok, H, D), out_dtype or q.dtype, q.device, stream)
-    otyp = typ if out.dtype == q.dtype else T_F32 if out.dtype == torch.float32 else None
-    if otyp is None or out.shape[1:] != q.shape[1:]:
+        out = _empty((batch.n_tok, H, D), out_dtype or dt, q.device, stream)
+    odt = out.dtype
+    otyp = typ if odt is dt else T_F32 if odt is torch.float32 else None
+    if otyp is None or out.shape[1:] != (H, D):
         raise ValueError(f"prompt_attention: out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
     _one_device("prompt_attention", q, k, v, out, batch.err)
     T = batch.n_tok
     with _device_of(q):
-        rc = lib().qms_cuda_prompt_attention(batch._ref, typ, _heads(q, T, "q"), _heads(k, T, "k"), _heads(v, T, "v"), H, k.shape[1], D,
+        rc = lib().qms_cuda_prompt_attention(batch._ref, typ, _heads(q, T, "q"), _heads(k, T, "k"), _heads(v, T, "v"), H, ks[1], D,
                                              D ** -0.5 if scale is None else scale, otyp, _heads(out, T, "out"), batch._err,
                                              batch._use(stream, q))
     if rc:

@@ -130,7 +130,7 @@ struct Q4Group {
     uint32_t n;
     __half d;
 };
-__device__ __forceinline__ Q4Group q4_quantize(double y) {
+__device__ __noinline__ Q4Group q4_quantize_exact(double y) {
     const unsigned long long bits = __double_as_longlong(y) & 0x7fffffffffffffffull;
     const uint32_t hi = (uint32_t)(bits >> 32), lo = (uint32_t)bits, mh = __reduce_max_sync(kFull, hi);
     const uint32_t ml = __reduce_max_sync(kFull, hi == mh ? lo : 0u);
@@ -149,6 +149,24 @@ __device__ __forceinline__ Q4Group q4_quantize(double y) {
     const double held = (double)__half2float(q.d);
     if (held == 0.0) q.n = 8;
     else q.n = (uint32_t)min(max(__double2int_rd(fma(y, 1.0 / held, 8.5 + 0x1p-40)), 0), 15);
+    return q;
+}
+
+// The same in fp32 where that is certain to give the same: one value of largest magnitude, by more than 2 in its last place; a scale
+// that is not within 8 of the border between two of 8 bits; quotients (off by some 2e-6) that are 2e-5 from a border. One group in 1000
+// of random values is not, and takes 5 times as long.
+__device__ __forceinline__ Q4Group q4_quantize(double y) {
+    const float yf = (float)y;
+    const uint32_t b = __float_as_uint(yf) & 0x7fffffffu, most = __reduce_max_sync(kFull, b);
+    const unsigned near = __ballot_sync(kFull, b + 2 >= most);
+    const float m = __shfl_sync(kFull, yf, __ffs(near) - 1);
+    const uint32_t db = __float_as_uint(m * -0.125f);
+    Q4Group q;
+    q.d = __float2half_rn(fminf(fmaxf(__uint_as_float((db + 0x7fffu + (db >> 16 & 1)) & 0xffff0000u), -kQ4Most), kQ4Most));
+    const float held = __half2float(q.d), t = fmaf(yf, __frcp_rn(held), 8.5f);
+    q.n = (uint32_t)min(max(__float2int_rd(t), 0), 15);
+    const bool sure = most < 0x7f800000u && most >= 0x01000000u && (near & (near - 1)) == 0 && (uint32_t)((int)(db & 0xffffu) - 0x7ff8) > 16u && held != 0.0f;
+    if (!sure || __any_sync(kFull, fabsf(t - rintf(t)) < 2e-5f)) return q4_quantize_exact(y);
     return q;
 }
 
@@ -179,7 +197,8 @@ __device__ __forceinline__ void row_st(__nv_bfloat16 *p, float v) { *p = __float
 // k_paged_append's steps where the cache or the rows that go out are of another kind: a cache in 4 bits (K normalised and rotated in
 // double, see above), or none; rows out of fp32, the q heads, or of 16 bits, all heads q | k | v as the prompt attention reads
 // them, each value rounded once from fp32.
-// (rows out of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.)
+// (rows out of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.) A warp takes R q heads, or one K or V
+// head: what is stored in 4 bits takes as long as four q heads.
 template <int D, typename OT, int R>
 __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int type, const float *qkv, int64_t ldqkv, const float *q_norm,
                                                      const float *k_norm, float eps, const float *rope_cos, const float *rope_sin, int n_rope,
@@ -187,9 +206,9 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
     static_assert(R == 1 || R == 4, "rows per warp");
     constexpr bool ALL = sizeof(OT) == 2;
     constexpr int J = D / 32, JH = J / 2;
-    const int lane = threadIdx.x & 31, groups = (a.H + 2 * a.Hk + R - 1) / R, nq = a.H + a.Hk;
+    const int lane = threadIdx.x & 31, gq = (a.H + R - 1) / R, groups = gq + 2 * a.Hk, nq = a.H + a.Hk;
     const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = unit / groups, h0 = (unit - t * groups) * R;
+    const int t = unit / groups, j0 = unit - t * groups, h0 = j0 < gq ? j0 * R : a.H + j0 - gq, cnt = j0 < gq ? min(R, a.H - h0) : 1;
     pdl_trigger();
     pdl_wait();
     if (t >= a.n_tok) return;
@@ -198,7 +217,7 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int j = 0; j < J; j++) x[r][j] = h0 + r < nq + a.Hk ? row[r * D + lane + 32 * j] : 0.0f;
+        for (int j = 0; j < J; j++) x[r][j] = r < cnt ? row[r * D + lane + 32 * j] : 0.0f;
 #pragma unroll
     for (int j = 0; j < J; j++) w[j] = (h0 < a.H ? q_norm : k_norm)[lane + 32 * j];
     const int b = paged_seq_of(a, t);
@@ -234,20 +253,15 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
         sum_rows<R>(ss, lane);
         inv = 1.0 / sqrt(ss[0] / D + (double)eps);
     }
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int hh = h0 + r;
-        if (hh >= nq + a.Hk) return;
-        const double iv = R == 1 ? inv : __shfl_sync(kFull, inv, 8 * r);
-        if (r > 0 && hh == a.H)                                 // from q to k
-#pragma unroll
-            for (int j = 0; j < J; j++) w[j] = k_norm[lane + 32 * j];
-        char *dst = hh < a.H || a.n_pages == 0 ? nullptr : (hh < nq ? a.k : a.v) + at + (hh < nq ? hh - a.H : hh - nq) * a.head_stride;
+    if (h0 >= a.H) {                                            // a K or V head
+        const double iv = R == 1 ? inv : __shfl_sync(kFull, inv, 0);
+        const bool is_k = h0 < nq;
+        char *dst = a.n_pages == 0 ? nullptr : (is_k ? a.k : a.v) + at + (is_k ? h0 - a.H : h0 - nq) * a.head_stride;
         if (dst && type == QMS_T_Q4_0) {
             double y[J];
 #pragma unroll
-            for (int j = 0; j < J; j++) y[j] = hh < nq ? (double)x[r][j] * iv * (double)w[j] : (double)x[r][j];
-            if (hh < nq) {
+            for (int j = 0; j < J; j++) y[j] = is_k ? (double)x[0][j] * iv * (double)w[j] : (double)x[0][j];
+            if (is_k) {
 #pragma unroll
                 for (int j = 0; j < JH; j++) {
                     const double y1 = y[j], y2 = y[j + JH];
@@ -257,17 +271,25 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
             }
             q4_store<D>(a, dst, p & ((1 << a.page_log) - 1), y, lane);
         }
-        if (hh < nq && (ALL || hh < a.H)) rope_scaled<D>(x[r], w, c, s, iv);
+        if (is_k && (ALL || type != QMS_T_Q4_0)) rope_scaled<D>(x[0], w, c, s, iv);
         if (dst && type != QMS_T_Q4_0) {
 #pragma unroll
             for (int j = 0; j < J; j++) {
-                if (type == QMS_T_F16) kv_st(reinterpret_cast<__half *>(dst) + lane + 32 * j, x[r][j]);
-                else kv_st(reinterpret_cast<float *>(dst) + lane + 32 * j, x[r][j]);
+                if (type == QMS_T_F16) kv_st(reinterpret_cast<__half *>(dst) + lane + 32 * j, x[0][j]);
+                else kv_st(reinterpret_cast<float *>(dst) + lane + 32 * j, x[0][j]);
             }
         }
-        if (ALL || hh < a.H)
+        if (ALL)
 #pragma unroll
-            for (int j = 0; j < J; j++) row_st(out + t * ldo + hh * D + lane + 32 * j, x[r][j]);
+            for (int j = 0; j < J; j++) row_st(out + t * ldo + h0 * D + lane + 32 * j, x[0][j]);
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (r >= cnt) return;
+        rope_scaled<D>(x[r], w, c, s, R == 1 ? inv : __shfl_sync(kFull, inv, 8 * r));
+#pragma unroll
+        for (int j = 0; j < J; j++) row_st(out + t * ldo + (h0 + r) * D + lane + 32 * j, x[r][j]);
     }
 }
 
@@ -276,7 +298,7 @@ static int launch_rows_append(const Paged &a, int type, const float *qkv, int64_
                               const float *rope_cos, const float *rope_sin, int n_rope, OT *out, int64_t ldo, cudaStream_t s) {
     const int heads = a.H + 2 * a.Hk;
     const bool four = (int64_t)a.n_tok * heads >= 148 * 48;     // (as k_paged_append)
-    const int64_t units = (int64_t)a.n_tok * (four ? (heads + 3) / 4 : heads);
+    const int64_t units = (int64_t)a.n_tok * (four ? (a.H + 3) / 4 + 2 * a.Hk : heads);
     QMS_REQUIRE(units < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "append: too many rows");
     const dim3 grid((unsigned)((units + 7) / 8));
     if (four) QMS_CK(launch_pdl(k_rows_append<D, OT, 4>, grid, dim3(256), 0, s, a, type, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, out, ldo));

@@ -325,18 +325,25 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
                         v[x][1] = __byte_perm(w[x][2][i], w[x][3][i], h ? 0x7632 : 0x5410);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float t[4];
+                    for (int e = 0; e < 4; e += 2) {
+                        float t2[2][4];
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            const uint32_t v0 = q4_pair(v[x][0], e, d[x][0], m24[x][0], six), v1 = q4_pair(v[x][1], e, d[x][1], m24[x][1], six);
-                            if (x == 0) mma_16_first(t, pl[x], v0, v1);
-                            else mma_16(t, pl[x], v0, v1);
-                            mma_16(t, ph[x], v0, v1);
+                            uint32_t v0[2], v1[2];
+#pragma unroll
+                            for (int ee = 0; ee < 2; ee++) v0[ee] = q4_pair(v[x][0], e + ee, d[x][0], m24[x][0], six), v1[ee] = q4_pair(v[x][1], e + ee, d[x][1], m24[x][1], six);
+#pragma unroll
+                            for (int ee = 0; ee < 2; ee++) { if (x == 0) mma_16_first(t2[ee], pl[x], v0[ee], v1[ee]); else mma_16(t2[ee], pl[x], v0[ee], v1[ee]); }
+#pragma unroll
+                            for (int ee = 0; ee < 2; ee++) mma_16(t2[ee], ph[x], v0[ee], v1[ee]);
                         }
-                        float(&y)[4] = o[8 * i + 2 * e + h];
+#pragma unroll
+                        for (int ee = 0; ee < 2; ee++) {
+                        float(&t)[4] = t2[ee];
+                        float(&y)[4] = o[8 * i + 2 * (e + ee) + h];
                         const float2 lo = f2_add(make_float2(y[0], y[1]), make_float2(t[0], t[1])), hi = f2_add(make_float2(y[2], y[3]), make_float2(t[2], t[3]));
                         y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
+                        }
                     }
                 }
         }
