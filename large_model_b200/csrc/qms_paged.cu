@@ -193,6 +193,33 @@ __device__ __forceinline__ void q4_store(const Paged &a, char *nibbles, int off,
 __device__ __forceinline__ void row_st(float *p, float v) { *p = v; }
 __device__ __forceinline__ void row_st(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void row_st(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void row_st2(float *p, float x, float y) { *reinterpret_cast<float2 *>(p) = make_float2(x, y); }
+__device__ __forceinline__ void row_st2(__half *p, float x, float y) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(x, y); }
+__device__ __forceinline__ void row_st2(__nv_bfloat16 *p, float x, float y) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x, y); }
+
+// R q heads of one token to 16 bits, in fp32: y = R(pos) (w x / sqrt(mean x^2 + eps)). Of 128 values a lane has 2 l, 2 l + 1 and the two 64
+// further, which they are rotated with.
+template <typename OT, int R>
+__device__ __forceinline__ void q_rows16(const float2 (&x)[R][2], int cnt, const float *norm, float eps, const float *cos, const float *sin, OT *out, int lane) {
+    auto two = [&](const float *v) { return make_float2(v[2 * lane], v[2 * lane + 1]); };       // (of any alignment)
+    const float2 w0 = two(norm), w1 = two(norm + 64), c = two(cos), s = two(sin);
+    float ss[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) ss[r] = fmaf(x[r][0].x, x[r][0].x, x[r][0].y * x[r][0].y) + fmaf(x[r][1].x, x[r][1].x, x[r][1].y * x[r][1].y);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int r = 0; r < R; r++) ss[r] += __shfl_xor_sync(kFull, ss[r], o);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (r >= cnt) return;
+        const float inv = 1.0f / sqrtf(fmaf(ss[r], 1.0f / 128.0f, eps));
+        const float a0 = x[r][0].x * inv * w0.x, a1 = x[r][0].y * inv * w0.y, b0 = x[r][1].x * inv * w1.x, b1 = x[r][1].y * inv * w1.y;
+        OT *to = out + r * 128 + 2 * lane;
+        row_st2(to, a0 * c.x - b0 * s.x, a1 * c.y - b1 * s.y);
+        row_st2(to + 64, b0 * c.x + a0 * s.x, b1 * c.y + a1 * s.y);
+    }
+}
 
 // k_paged_append's steps where the cache or the rows that go out are of another kind: a cache in 4 bits (K normalised and rotated in
 // double, see above), or none; rows out of fp32, the q heads, or of 16 bits, all heads q | k | v as the prompt attention reads
@@ -213,11 +240,20 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
     pdl_wait();
     if (t >= a.n_tok) return;
     const float *row = qkv + t * ldqkv + h0 * D;
+    constexpr bool Q16 = ALL && D == 128;
     float x[R][J], w[J];
+    float2 x2[R][2];
+    if (Q16 && h0 < a.H) {
 #pragma unroll
-    for (int r = 0; r < R; r++)
+        for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int j = 0; j < J; j++) x[r][j] = r < cnt ? row[r * D + lane + 32 * j] : 0.0f;
+            for (int j = 0; j < 2; j++) x2[r][j] = r < cnt ? reinterpret_cast<const float2 *>(row + r * D)[lane + 32 * j] : make_float2(0.0f, 0.0f);
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < J; j++) x[r][j] = r < cnt ? row[r * D + lane + 32 * j] : 0.0f;
+    }
 #pragma unroll
     for (int j = 0; j < J; j++) w[j] = (h0 < a.H ? q_norm : k_norm)[lane + 32 * j];
     const int b = paged_seq_of(a, t);
@@ -234,6 +270,12 @@ __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int ty
     if (at < 0) {
         if (lane == 0 && h0 == 0) paged_err(a, QMS_PAGED_EPAGE);
         return;
+    }
+    if constexpr (Q16) {
+        if (h0 < a.H) {
+            q_rows16<OT, R>(x2, cnt, q_norm, eps, rope_cos + (int64_t)p * (D / 2), rope_sin + (int64_t)p * (D / 2), out + t * ldo + h0 * D, lane);
+            return;
+        }
     }
     float c[JH], s[JH];
     double inv = 0.0;

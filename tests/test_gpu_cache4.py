@@ -499,3 +499,18 @@ def test_refusals(cuda):
             m.paged_attention(pages, batch, torch.zeros((1, 2 * pages.head_dim), device="cuda"), 2)
         with pytest.raises(m.QmsCudaError):
             pages.values()
+
+
+def test_prompt_append_takes_weights_and_tables_of_any_alignment(cuda):
+    import torch
+    import large_model_b200 as m
+    g = torch.Generator(device="cuda").manual_seed(1)
+    T, H, Hk, D = 40, 8, 2, 128
+    qkv = torch.randn((T, (H + 2 * Hk) * D), generator=g, device="cuda")
+    w = torch.randn((D,), generator=g, device="cuda")
+    cos, sin = m.rope_tables(64, D)
+    off = lambda x: torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)
+    batch = m.PagedBatch.prompts(torch.tensor([0, T], dtype=torch.int32, device="cuda"), T, T)
+    want = m.prompt_append(None, batch, qkv, H, w, w, 1e-6, (cos, sin), n_head_kv=Hk)
+    got = m.prompt_append(None, batch, qkv, H, off(w), off(w), 1e-6, (off(cos), off(sin)), n_head_kv=Hk)
+    assert off(w).data_ptr() % 8 == 4 and torch.equal(got, want)
