@@ -13,8 +13,9 @@ namespace qms {
 typedef unsigned long long u64;
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32;
-constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2;       // a warp's: groups of 4 values per lane, values per chunk, chunks in flight
+constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2, kLpKeep = 6, kLpList = 2048;       // a warp's: groups of 4 values per lane, values per chunk, chunks in flight, or kept
 constexpr uint32_t kLpSpin = 1u << 22;
+constexpr int kLpFew = 74;            // CTAs up to which a row's slices are kept in shared memory (launch_logprobs)
 
 struct LogprobArgs {
     const float *l;
@@ -75,20 +76,25 @@ __device__ __forceinline__ LpPart lp_under(const LpPart &p, float M, bool first,
 // The likeliest: lane i holds the i-th largest of its warp's so far. Values that reach a bound are put in their place: first one that n_top
 // lanes' largest of the first chunk reach, then the n_top-th itself, of this warp or of another that is further. Some 35
 // of 2400 values reach it; those of a chunk are put in together. The first CTA of the cluster joins all.
-__global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a) {
-    extern __shared__ __align__(128) float rings[];        // [kLpWarps][kLpRing][kLpChunk]
+// KEEP: for few rows, where that chain of steps is what the row takes: all of a slice stays in shared memory, the bound comes from all lanes'
+// largest (the least over the warps of each one's r-th, r = n_top over the number of warps), and a second look lists what reaches it, some
+// 60 of 19,000, whose places are the numbers of entries above them.
+template <bool KEEP>
+__global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const LogprobArgs a) {
+    constexpr int RING = KEEP ? kLpKeep : kLpRing;
+    extern __shared__ __align__(128) float rings[];        // [kLpWarps][RING][kLpChunk], then (KEEP) the list
     __shared__ u64 s_all[kRowCtas * kLpTop], s_list[kLpWarps * kLpTop], s_some[kLpWarps][48];
-    __shared__ uint64_t s_full[kLpWarps][kLpRing];
+    __shared__ uint64_t s_full[kLpWarps][RING];
     __shared__ LpPart s_warp[kLpWarps], s_part[kRowCtas];
-    __shared__ uint32_t s_bound;                           // the highest bound of a warp, by lp_order
-    __shared__ int s_abort;
+    __shared__ uint32_t s_bound, s_r[kLpWarps];            // the highest bound of a warp, by lp_order
+    __shared__ int s_abort, s_n;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
-    float *ring = rings + warp * kLpRing * kLpChunk;
+    float *ring = rings + warp * RING * kLpChunk;
     for (int i = tid; i < nc * kLpTop; i += kLpThreads) s_all[i] = 0;
     if (tid == 0) s_abort = 0, s_bound = 0;
     if (lane == 0) {
-        for (int i = 0; i < kLpRing; i++) mbar_init(&s_full[warp][i], 1);
+        for (int i = 0; i < RING; i++) mbar_init(&s_full[warp][i], 1);
         fence_mbar_init();
     }
     auto started = cl.barrier_arrive();                    // waited for before the first write to another CTA
@@ -102,11 +108,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
     const int chunks = ((hi - lo + kLpChunk - 1) / kLpChunk - warp + kLpWarps - 1) / kLpWarps;     // in turn over the warps
     auto load = [&](int k) {                               // by one lane
         const int base = lo + (k * kLpWarps + warp) * kLpChunk, n = min(kLpChunk, hi - base);
-        mbar_arrive_expect_tx(&s_full[warp][k % kLpRing], n * 4);
-        bulk_load(smem_u32(ring + k % kLpRing * kLpChunk), row + base, n * 4, &s_full[warp][k % kLpRing]);
+        mbar_arrive_expect_tx(&s_full[warp][k % RING], n * 4);
+        bulk_load(smem_u32(ring + k % RING * kLpChunk), row + base, n * 4, &s_full[warp][k % RING]);
     };
     if (lane == 0)
-        for (int k = 0; k < min(chunks, kLpRing); k++) load(k);
+        for (int k = 0; k < min(chunks, RING); k++) load(k);
     const float mine = tid < a.n_ids && rank == 0 && (unsigned)a.ids[r * a.n_ids + tid] < (unsigned)a.V ? row[a.ids[r * a.n_ids + tid]] : 0.0f;
     __syncthreads();                                       // s_bound, s_abort
 
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
     if (rank == 0 && warp == 0) {                                      // the values before the first boundary
         const float v = lane < head ? row[lane] : -INFINITY;
         rebase(v);
-        if (a.n_top > 0) {
+        if (!KEEP && a.n_top > 0) {
             look(v, lane);
             raise();
         }
@@ -219,7 +225,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
         rebase(most);
 #pragma unroll
         for (int e = 0; e < kLpQuads; e++) add(y[e].x, e & 1), add(y[e].y, e & 1), add(y[e].z, e & 1), add(y[e].w, e & 1);
-        if (a.n_top > 0) {
+        if (!KEEP && a.n_top > 0) {
             if (k == 0) {                                  // the n_top-th of the lanes' largest (NaN is none)
                 uint32_t o = lp_order(fmaxf(most, -INFINITY)), at = __reduce_max_sync(kFull, o);
                 for (int i = 1; i < a.n_top; i++) {
@@ -241,16 +247,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
             }
         }
         __syncwarp();
-        if (lane == 0 && k + kLpRing < chunks) {
+        if (!KEEP && lane == 0 && k + RING < chunks) {
             fence_async_smem();
-            load(k + kLpRing);
+            load(k + RING);
         }
-        if (++slot == kLpRing) slot = 0, phase ^= 1;
+        if (++slot == RING) slot = 0, phase ^= 1;
     }
     if (rank == nc - 1 && warp == kLpWarps - 1) {                             // the values behind the last group
         const float v = tail + lane < a.V ? row[tail + lane] : -INFINITY;
         rebase(v);
-        if (a.n_top > 0) {
+        if (!KEEP && a.n_top > 0) {
             look(v, tail + lane);
             raise();
         }
@@ -281,6 +287,73 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
     p = join(p);
     if (lane == 0) s_warp[warp] = p;
     s_list[tid] = best;
+    u64 *list = reinterpret_cast<u64 *>(rings + kLpWarps * RING * kLpChunk);
+    int listed = 0;
+    if constexpr (KEEP) {
+        if (a.n_top > 0) {
+            // warps without a value do not count
+            const int busy = max(1, min(kLpWarps, (hi - lo + kLpChunk - 1) / kLpChunk)), rounds = (a.n_top + busy - 1) / busy;
+            uint32_t o = lp_order(fmaxf(m[0], m[1])), at = __reduce_max_sync(kFull, o);
+            for (int i = 1; i < rounds; i++) {
+                if (lane == __ffs(__ballot_sync(kFull, o == at)) - 1) o = 0;
+                at = __reduce_max_sync(kFull, o);
+            }
+            if (lane == 0) s_r[warp] = at;
+            if (tid == 0) s_n = 0;
+            __syncthreads();
+            uint32_t least = s_r[0];
+            for (int w = 1; w < busy; w++) least = min(least, s_r[w]);
+            bound = fmaxf(least == 0 ? -FLT_MAX : lp_unorder(least), -FLT_MAX);
+            auto take = [&](float v, int i) {
+                if (v >= bound) {
+                    const int n = atomicAdd(&s_n, 1);
+                    if (n < kLpList) list[n] = lp_key(v, i);
+                }
+            };
+            auto all_values = [&](auto &&f) {              // of this thread
+                for (int k = 0; k < chunks; k++) {
+                    const int base = lo + (k * kLpWarps + warp) * kLpChunk, n4 = min(kLpChunk, hi - base) >> 2;
+                    const float4 *x4 = reinterpret_cast<const float4 *>(ring + k * kLpChunk);
+#pragma unroll
+                    for (int e = 0; e < kLpQuads; e++) {
+                        const int i = lane + e * 32;
+                        if (i >= n4) break;
+                        const float4 y = x4[i];
+                        if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound) f(y.x, base + 4 * i), f(y.y, base + 4 * i + 1), f(y.z, base + 4 * i + 2), f(y.w, base + 4 * i + 3);
+                    }
+                }
+                if (rank == 0 && tid < head) f(row[tid], tid);
+                if (rank == nc - 1 && tail + tid < a.V && tid < 4) f(row[tail + tid], tail + tid);
+            };
+            all_values(take);
+            __syncthreads();
+            listed = s_n;
+            if (listed > kLpList) {                        // many equal values: one after the other
+                u64 last = ~0ull;
+                for (int q = 0; q < a.n_top; q++) {
+                    u64 most = 0;
+                    all_values([&](float v, int i) {
+                        if (v >= bound) {
+                            const u64 k = lp_key(v, i);
+                            if (k < last && k > most) most = k;
+                        }
+                    });
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const u64 other = __shfl_xor_sync(kFull, most, o);
+                        most = other > most ? other : most;
+                    }
+                    if (lane == 0) s_list[warp] = most;
+                    __syncthreads();
+                    for (int w = 0; w < kLpWarps; w++) most = s_list[w] > most ? s_list[w] : most;
+                    __syncthreads();
+                    if (tid == 0) list[q] = most;
+                    last = most;
+                }
+                listed = a.n_top;
+            }
+        }
+    }
     cl.barrier_wait(std::move(started));
     __syncthreads();
     if (warp == 0) {
@@ -288,7 +361,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
         if (s_abort || p.m == INFINITY) p.z = NAN;
         if (lane == 0) *cl.map_shared_rank(&s_part[rank], 0) = p;
     }
-    if (best != 0) {
+    if constexpr (KEEP) {
+        for (int i = tid; i < listed; i += kLpThreads) {
+            const u64 k = list[i];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < listed; j++) above += list[j] > k;
+            if (k != 0 && above < a.n_top) cl.map_shared_rank(s_all, 0)[rank * kLpTop + above] = k;
+        }
+    } else if (best != 0) {
         const int above = lp_above(s_list, kLpWarps, best);
         if (above < a.n_top) cl.map_shared_rank(s_all, 0)[rank * kLpTop + above] = best;
     }
@@ -325,14 +406,17 @@ __global__ void __launch_bounds__(kLpThreads, 4) k_logprobs(const LogprobArgs a)
 }
 
 static int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t s) {
-    constexpr int smem = kLpWarps * kLpRing * kLpChunk * 4;
-    static std::atomic<unsigned long long> done{0};
-    const int rc = allow_smem(done, k_logprobs, smem);
-    if (rc) return rc;
+    constexpr int ring = kLpWarps * kLpRing * kLpChunk * 4, keep = kLpWarps * kLpKeep * kLpChunk * 4 + kLpList * 8;
+    static std::atomic<unsigned long long> done[2];
+    int rc = allow_smem(done[0], k_logprobs<false>, ring);
+    if (rc || (rc = allow_smem(done[1], k_logprobs<true>, keep))) return rc;
     // CTAs per row: at most 8, a warp's piece a chunk at least, and as many as fill the device
     int nc = 1;
     while (nc < kRowCtas && a.V > nc * kLpWarps * kLpChunk && (int64_t)rows * nc < 500) nc *= 2;
-    return launch_rows(k_logprobs, kLpThreads, rows, nc, smem, s, a);
+    // Kept in shared memory for few CTAs. Both in us, not kept and kept: 1 row of 151,936 14.3, 10.2; 8 rows 14.8, 11.3; 19 rows 16.9, 18.5; 64
+    // rows of 4096 8.4, 7.2; 16 rows of 32,003 9.1, 11.7.
+    if ((int64_t)rows * nc <= kLpFew && a.V / nc + 8 <= kLpWarps * kLpKeep * kLpChunk) return launch_rows(k_logprobs<true>, kLpThreads, rows, nc, keep, s, a);
+    return launch_rows(k_logprobs<false>, kLpThreads, rows, nc, ring, s, a);
 }
 
 }  // namespace qms
