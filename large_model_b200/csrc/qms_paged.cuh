@@ -187,6 +187,7 @@ struct PagedPlan {
     // run (the first line_r runs have one more), position tiles; positions per place, rows per row tile
     unsigned line, line_runs, line_per, line_q, line_r, line_nt;
     int line_tp, line_rows;
+    int flat;                        // 4 bits: positions that go to the workspace in fp16 (0: none), for every kind that is kPaWidePair
 };
 // k_paged_wide: 256 rows; 128; 128 over an fp32 cache; 128 over one in 4 bits
 constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2, kPaWideQ4 = -3;

@@ -802,6 +802,39 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
     else *reinterpret_cast<float2 *>(dst) = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x[0] * inv, x[1] * inv);
 }
 
+// ---- 4 bits to fp16 in the workspace -----------------------------------------------------------------
+// The positions that many rows read, [0, prefix) or all of one sequence's, as fp16 (exact) in pages of their own, with the table that
+// leads there (-1 where the cache's page does not exist: reported by who reads it). A thread per 8 values of K and of V. Bound by L2: 144
+// bytes in, 512 out per position and kv head of 128.
+template <int D>
+__global__ void __launch_bounds__(256) k_paged_flat(const Paged a, const Paged to, const bool own, int *table) {
+    constexpr int W = D / 8;
+    pdl_wait();
+    pdl_trigger();
+    int limit = a.prefix;
+    if (own) {
+        int t0, n, kv;
+        paged_seq(a, 0, t0, n, kv);
+        limit = max(limit, kv);
+    }
+    // whole copies of the kernels that read them: 128 positions, or a page
+    const int unit = min(1 << a.page_log, 128), end = (limit + unit - 1) & ~(unit - 1);
+    const int64_t total = (int64_t)end * a.Hk * W;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int w = (int)(i % W), p16 = (int)(i / W) & 15, y = (int)(i / (16 * W)), h = y % a.Hk, p = y / a.Hk * 16 + p16;
+        const int off = p & ((1 << a.page_log) - 1), page = a.table[p >> a.page_log];
+        const bool good = (unsigned)page < (unsigned)a.n_pages;
+        if (off == 0 && h == 0 && w == 0) table[p >> a.page_log] = good ? p >> a.page_log : -1;
+        if (!good) continue;
+        const int64_t from = page * a.page_stride + off * a.pos_stride + h * a.head_stride, sc = from + q4_scales<D>(a, off) + w / 4 * 2;
+        const int64_t at = (p >> a.page_log) * to.page_stride + h * to.head_stride + off * to.pos_stride + w * 16;
+        const uint32_t kw = __ldcg(reinterpret_cast<const unsigned int *>(a.k + from) + w), vw = __ldcg(reinterpret_cast<const unsigned int *>(a.v + from) + w);
+        const __half2 dk = __half2half2(__ldcg(reinterpret_cast<const __half *>(a.k + sc))), dv = __half2half2(__ldcg(reinterpret_cast<const __half *>(a.v + sc)));
+        *reinterpret_cast<uint4 *>(to.k + at) = q4_dequant(kw, dk, __hmul2(dk, __float2half2_rn(-24.0f)));
+        *reinterpret_cast<uint4 *>(to.v + at) = q4_dequant(vw, dv, __hmul2(dv, __float2half2_rn(-24.0f)));
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------
 // Rows per tile: 16, 32 or 64 for k_paged_attn, as tall as the rows there are (more rows per K / V read); k_paged_wide
 // from 65 on (fp16: in pages of 8 positions or more, a swizzle unit of its tiles) and from so many rows x positions (`rows`
@@ -810,9 +843,11 @@ __global__ void __launch_bounds__(256) k_paged_merge(const __grid_constant__ Pag
 // of rows x positions: 8 sequences of 5 tokens, own positions 1.2 narrow 17.6, wide 19.5 (22.2, 21.4); 1.8 19.5, 19.2 (26.1, 28.1); 2.5
 // 21.8, 18.4 (29.8, 27.2); 4.1 25.9, 19.6 (42.3, 31.0); 20 tokens on a prompt, shared ones 1.6 23.4, 25.1 (35.4, 36.9); 2.0 27.8, 27.2 (38.0,
 // 37.7); 3.1 31.3, 35.1 (45.7, 46.5); 6.3 39.8, 43.5 (65.8, 58.2); 16.8 69, 63 (139, 96).
+// 4 bits narrow against wide in us: own positions 2.0 19.1, 22.0; 4.1 27.4, 23.1 (20 tokens of one sequence 29.8, 24.8; 128 29.3, 28.1); 8.2 44.6, 30.3;
+// shared ones 1.3 23.5, 26.7; 2.6 30.7, 37.7; 4.2 41.8, 38.0; 10.5 57.2, 51.8.
 static int row_groups(int type, int page_log, int64_t rows, int64_t positions, bool shared) {
     const bool f16 = type == QMS_T_F16;
-    if (type == QMS_T_Q4_0) return rows > 64 && (rows + 63) / 64 * 64 * positions > 2600000 ? kPaWideQ4 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    if (type == QMS_T_Q4_0) return rows > 64 && (rows + 63) / 64 * 64 * positions > 3000000 ? kPaWideQ4 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
     if (rows > 64 && (!f16 || page_log >= 3) && (rows + 63) / 64 * 64 * positions > (f16 || shared ? 2600000 : 1200000))
         return !f16 ? kPaWideF32 : rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
@@ -845,15 +880,30 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, dou
     const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
+    // (4 bits, up to 16 rows, with 1.2 and 4.0 us as the others: 64 x 4096 positions 95.2, 89.6; 131072 58.5, 54.7)
+    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * 3 * share)), 0.6, 3.0, most);
     const int per_sm = type != QMS_T_F32 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * per_sm * share)), wr == 4 ? 2.0 : 1.2, 4.0, most);
 }
+
+// What `positions` of the cache take in fp16, K or V, in pages of the cache's size.
+static int64_t flat_pages(const Paged &a, int positions) { return ((int64_t)positions + (1 << a.page_log) - 1) >> a.page_log; }
+static int64_t flat_bytes(const Paged &a, int D, int positions) { return (flat_pages(a, positions) << a.page_log) * a.Hk * D * 2; }
+constexpr int64_t kFlatMost = 128ll << 20;         // a bound on the workspace, not on what pays
+
+static int64_t al256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
     memset(&p, 0, sizeof p);
     p.wr_p = row_groups(type, a.page_log, rows_p, (int64_t)a.prefix * a.Hk, true);
     p.wr_s = row_groups(type, a.page_log, rows_s, (int64_t)std::max(0, a.max_kv - a.prefix) * a.Hk * a.n_seq, false);
+    // 4 bits for many rows, on positions of one sequence's table: to fp16 once, not once per 128 rows, and 256 rows at a time. That
+    // against kPaWideQ4 in us, 16 q heads per kv head, 4 of these: 320 tokens on a prompt of 8192 positions 251, 348; 64 62.8, 74.8; 20 50.9, 51.5; 10 (160 rows)
+    // 46.2, 43.0; a sequence's 256 tokens on 4096 positions 86.4, 118.5; 32 30.2, 31.4; 16 (256 rows) 28.4, 25.3.
+    auto flat = [&](int wr, int64_t rows, int positions) { return wr == kPaWideQ4 && rows > 256 && flat_bytes(a, D, positions) <= kFlatMost; };
+    if (flat(p.wr_p, rows_p, a.prefix)) p.flat = a.prefix, p.wr_p = kPaWidePair;
+    if (a.n_seq == 1 && flat(p.wr_s, rows_s, a.max_kv)) p.flat = a.max_kv, p.wr_s = kPaWidePair;
     p.base_s = a.prefix & ~(std::min(1 << a.page_log, tile_positions(type, p.wr_s)) - 1);
     const int own = std::max(0, a.max_kv - p.base_s);
     p.tiles_p = (int)((rows_p + tile_rows(p.wr_p) - 1) / tile_rows(p.wr_p));
@@ -884,11 +934,9 @@ void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     }
 }
 
-static int64_t al256(int64_t x) { return (x + 255) & ~(int64_t)255; }
-
 int64_t paged_ws_bytes(const Paged &a, int D, const PagedPlan &p) {
     const int64_t n = (int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H;
-    return al256(n * D * 4) + al256(n * 8);
+    return al256(n * D * 4) + al256(n * 8) + (p.flat ? al256(flat_pages(a, p.flat) * 4) + 2 * al256(flat_bytes(a, D, p.flat)) : 0);
 }
 
 int tensor_encode(TensorEncode *encode) {
@@ -943,7 +991,7 @@ static int launch_attn_wr(const PagedAttn &A, bool own, bool last, cudaStream_t 
 }
 
 template <int D, typename KT>
-static int launch_attn(const PagedAttn &A, cudaStream_t s) {
+static int launch_attn(const PagedAttn &A, const PagedAttn &F, cudaStream_t s) {
     bool before = false;
     for (int kind = 0; kind < 2; kind++) {
         const bool own = kind == 1;
@@ -951,7 +999,7 @@ static int launch_attn(const PagedAttn &A, cudaStream_t s) {
         const int wr = own ? A.p.wr_s : A.p.wr_p;
         int rc;
         if constexpr (std::is_same<KT, Q4>::value)
-            rc = wr <= 0   ? launch_paged_wide(A, D, own, before, s)
+            rc = wr <= 0   ? launch_paged_wide(wr == kPaWidePair ? F : A, D, own, before, s)
                  : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
                  : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
                            : launch_paged_q4(A, D, own, before, s);
@@ -982,10 +1030,27 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     // (32-bit run arithmetic)
     QMS_REQUIRE((int64_t)p.tiles_p * a.Hk * ((a.prefix + 63) / 64) < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     A.part_ml = (float2 *)((char *)ws + al256((int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H * D * 4));
+    PagedAttn F = A;
+    if (p.flat) {
+        const int64_t pages = flat_pages(a, p.flat), bytes = al256(flat_bytes(a, D, p.flat));
+        int *table = (int *)((char *)A.part_ml + al256((int64_t)(p.slots_p + p.slots_s) * a.n_tok * a.H * 8));
+        F.type = QMS_T_F16;
+        F.a.table = table;
+        F.a.n_pages = (int)pages;
+        F.a.k = (char *)table + al256(pages * 4);
+        F.a.v = F.a.k + bytes;
+        F.a.pos_stride = D * 2;
+        F.a.head_stride = (int64_t)(D * 2) << a.page_log;
+        F.a.page_stride = F.a.head_stride * a.Hk;
+        const int64_t words = (((int64_t)p.flat + 127) & ~127ll) * a.Hk * (D / 8);
+        const dim3 ctas((unsigned)std::min<int64_t>((words + 255) / 256, 148 * 8));
+        if (D == 128) QMS_CK(launch_pdl(k_paged_flat<128>, ctas, dim3(256), 0, s, a, F.a, p.wr_s == kPaWidePair, table));
+        else QMS_CK(launch_pdl(k_paged_flat<64>, ctas, dim3(256), 0, s, a, F.a, p.wr_s == kPaWidePair, table));
+    }
     int rc;
-    if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, s) : launch_attn<64, __half>(A, s);
-    else if (type == QMS_T_Q4_0) rc = D == 128 ? launch_attn<128, Q4>(A, s) : launch_attn<64, Q4>(A, s);
-    else rc = D == 128 ? launch_attn<128, float>(A, s) : launch_attn<64, float>(A, s);
+    if (type == QMS_T_F16) rc = D == 128 ? launch_attn<128, __half>(A, A, s) : launch_attn<64, __half>(A, A, s);
+    else if (type == QMS_T_Q4_0) rc = D == 128 ? launch_attn<128, Q4>(A, F, s) : launch_attn<64, Q4>(A, F, s);
+    else rc = D == 128 ? launch_attn<128, float>(A, A, s) : launch_attn<64, float>(A, A, s);
     if (rc) return rc;
     // Four warps per row while there are few rows, or many slots for each. Four against one in us: 320 rows (5 tokens, 2000
     // positions) 14.9, 16.1; 512 rows on a prompt of 4096 positions 24.7, 28.9; 1024 rows of 100 positions 11.5, 9.1; 3072 rows

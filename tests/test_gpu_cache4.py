@@ -514,3 +514,61 @@ def test_prompt_append_takes_weights_and_tables_of_any_alignment(cuda):
     want = m.prompt_append(None, batch, qkv, H, w, w, 1e-6, (cos, sin), n_head_kv=Hk)
     got = m.prompt_append(None, batch, qkv, H, off(w), off(w), 1e-6, (off(cos), off(sin)), n_head_kv=Hk)
     assert off(w).data_ptr() % 8 == 4 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("qs,kv,G,Hk,D,page,prefix", [
+    ([70], [1400], 16, 2, 128, 32, 0),                            # one sequence's own positions
+    ([130], [6001], 4, 1, 128, 512, 0),                           # a page larger than a tile
+    ([40], [6500], 8, 2, 64, 16, 0),
+    ([20, 0, 41, 1, 20], [1400, 1310, 1361, 20, 1302], 16, 2, 128, 16, 1301),     # a shared prompt, and a sequence shorter than it
+    ([70], [3000], 16, 2, 128, 64, 1500),                         # a prompt and own positions, both
+    ([16], [6100], 16, 2, 128, 64, 0),                            # 256 rows: 4 bits to the kernel
+    ([3, 2, 3], [6500, 6500, 6410], 16, 2, 64, 64, 6400),
+])
+def test_attention_many_rows_by_fp16(cuda, qs, kv, G, Hk, D, page, prefix):
+    check(qs, kv, G=G, Hk=Hk, D=D, page=page, prefix=prefix, pad=2, seed=sum(kv))
+
+
+def test_many_rows_of_a_sequence_shorter_than_the_batch_allows(cuda):
+    """Table entries past the sequence's length lead nowhere, and count for nothing; the same batch object grows afterwards."""
+    import torch
+    import large_model_b200 as m
+    n, kv, G = 70, 1400, 16
+    pages, small, q, K, V = make([n], [kv], G=G, page=32, seed=9)
+    table = torch.full((1, 64), 1 << 20, dtype=torch.int32, device="cuda")
+    table[:, :small.table.shape[1]] = small.table
+    batch = m.PagedBatch(small.q_start, torch.tensor([kv], dtype=torch.int32, device="cuda"), table, n, n, 2048)
+    for now in (kv, 801, n, kv):
+        batch.kv_len.fill_(now)
+        out = m.paged_attention(pages, batch, q, 2 * G)
+        batch.status()
+        want, tol = reference([n], [now], q, [K[0][:now]], [V[0][:now]], G, 128 ** -0.5)
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_masked_values_and_bad_pages_of_many_rows_in_two_sequences(cuda):
+    """What holds for one sequence's many rows, for the kernel that reads 4 bits."""
+    import torch
+    import large_model_b200 as m
+    n, kv, G, D = 80, 1300, 16, 128
+    clean = make([n, 1], [kv, 5], G=G, seed=1)
+    want = m.paged_attention(clean[0], clean[1], clean[2], 2 * G)
+
+    def edit(z, b, x):
+        if b == 0:
+            x[kv - 1, :, 40] = np.nan if z else np.inf
+    pages, batch, q, _, _ = make([n, 1], [kv, 5], G=G, seed=1, edit=edit)
+    out = m.paged_attention(pages, batch, q, 2 * G)
+    batch.status()
+    assert torch.isfinite(out[:n - 1]).all() and torch.isfinite(out[n]).all()
+    assert (out[:n - 1] - want[:n - 1]).abs().max().item() <= 32 * E24 * 16
+    assert out[n - 1].isnan().any()
+
+    pages, batch, q, K, V = make([n, 1], [kv, 5], G=G, seed=7, page=32)
+    batch.table[0, 3] = -5
+    out = m.paged_attention(pages, batch, q, 2 * G)
+    with pytest.raises(m.QmsCudaError, match="0x2"):
+        batch.status()
+    keep = [j for j in range(kv) if j // 32 != 3]
+    want, tol = reference([n, 1], [kv - 32, 5], q, [K[0][keep], K[1]], [V[0][keep], V[1]], G, 128 ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
