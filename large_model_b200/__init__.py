@@ -665,9 +665,11 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     nc = cos.shape[0]
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens")
-    rc = lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
-                                     eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy,
-                                     batch._err, batch._use(stream, qkv))
+    _one_device("paged_append", qkv, q, pages.k, batch.err, q_norm, k_norm, cos, sin)
+    with _device_of(qkv):
+        rc = lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
+                                         eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy,
+                                         batch._err, batch._use(stream, qkv))
     if rc:
         check(rc)
     return q
@@ -767,10 +769,12 @@ def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: fl
     y, ny, ldy = _rows(out, n_head * D, "out")
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_attention: {n} q and {ny} out rows for {batch.n_tok} tokens")
-    raw = batch._use(stream, q)
-    ws, nb = batch.workspace(pages, n_head, raw)
-    rc = lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
-                                        ws, nb, batch._err, raw)
+    _one_device("paged_attention", q, out, pages.k, batch.err)
+    with _device_of(q):
+        raw = batch._use(stream, q)
+        ws, nb = batch.workspace(pages, n_head, raw)
+        rc = lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
+                                            ws, nb, batch._err, raw)
     if rc:
         check(rc)
     return out
