@@ -42,6 +42,33 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     return d;
 }
 
+// Two fp32 at once.
+__device__ __forceinline__ u64 two(float a, float b) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 of_two(u64 x) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+    return d;
+}
+__device__ __forceinline__ u64 add_two(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 mul_two(u64 a, u64 b) {
+    u64 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 fma_two(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // How many entries of `lists` lists, each of kLpTop in falling order, are above the key.
 __device__ __forceinline__ int lp_above(const u64 *list, int lists, u64 key) {
     static_assert(kLpTop == 32, "5 steps to one of 32, a sixth for none or all");
@@ -116,7 +143,9 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
     const float mine = tid < a.n_ids && rank == 0 && (unsigned)a.ids[r * a.n_ids + tid] < (unsigned)a.V ? row[a.ids[r * a.n_ids + tid]] : 0.0f;
     __syncthreads();                                       // s_bound, s_abort
 
-    float B = -FLT_MAX, m[2] = {-INFINITY, -INFINITY}, z[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+    float B = -FLT_MAX, m[2] = {-INFINITY, -INFINITY};
+    u64 z2 = 0, t2 = 0;                                     // (two sums each)
+    const u64 c2 = two(a.c, a.c);
     float bound = -FLT_MAX;                                // a value has to reach it
     u64 best = 0;                                          // the lane-th largest of the warp's
     // new values, up to 32 in s_new, take their places among the n_top largest: a key's place is the number of keys above it
@@ -177,18 +206,16 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
         if ((top - B) * a.c > 4.0f) {
             const float d = fmaxf((B - top) * a.c, -256.0f), f = ex2f(d);
             B = top;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                t[e] = f * fmaf(z[e], d, t[e]);
-                z[e] *= f;
-            }
+            t2 = mul_two(two(f, f), fma_two(z2, two(d, d), t2));
+            z2 = mul_two(z2, two(f, f));
         }
     };
-    auto add = [&](float v, int e) {                       // to the sums: v, or the largest so far that it replaces
-        const float y = (min_nan(m[e], v) - B) * a.c, w = ex2f(y);
-        m[e] = fmaxf(m[e], v);
-        z[e] += w;
-        t[e] = fmaf(w, fmaxf(y, -256.0f), t[e]);           // (weights below 2^-126 are 0; 0 * inf is not)
+    auto add = [&](float v0, float v1) {                   // to the sums: each value, or the largest so far that it replaces
+        const float2 y = of_two(mul_two(add_two(two(min_nan(m[0], v0), min_nan(m[1], v1)), two(-B, -B)), c2));
+        const u64 w = two(ex2f(y.x), ex2f(y.y));
+        m[0] = fmaxf(m[0], v0), m[1] = fmaxf(m[1], v1);
+        z2 = add_two(z2, w);
+        t2 = fma_two(w, two(fmaxf(y.x, -256.0f), fmaxf(y.y, -256.0f)), t2);          // (weights below 2^-126 are 0; 0 * inf is not)
     };
     if (rank == 0 && warp == 0) {                                      // the values before the first boundary
         const float v = lane < head ? row[lane] : -INFINITY;
@@ -197,7 +224,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
             look(v, lane);
             raise();
         }
-        add(v, 0);
+        add(v, -INFINITY);
     }
     bool gave_up = false;
     for (int k = 0, slot = 0, phase = 0; k < chunks; k++) {
@@ -224,7 +251,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         rebase(most);
 #pragma unroll
-        for (int e = 0; e < kLpQuads; e++) add(y[e].x, e & 1), add(y[e].y, e & 1), add(y[e].z, e & 1), add(y[e].w, e & 1);
+        for (int e = 0; e < kLpQuads; e++) add(y[e].x, y[e].y), add(y[e].z, y[e].w);
         if (!KEEP && a.n_top > 0) {
             if (k == 0) {                                  // the n_top-th of the lanes' largest (NaN is none)
                 uint32_t o = lp_order(fmaxf(most, -INFINITY)), at = __reduce_max_sync(kFull, o);
@@ -260,17 +287,18 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
             look(v, tail + lane);
             raise();
         }
-        add(v, 0);
+        add(v, -INFINITY);
     }
 
     // ---- lanes to warps, warps to the CTA
     LpPart p;
     {
+        const float2 z = of_two(z2), t = of_two(t2);
         const bool second = m[1] > m[0];                   // of the two maxima one joins the sums
         const float y = ((second ? m[0] : m[1]) - B) * a.c, w = ex2f(y);
         p.m = second ? m[1] : m[0];
-        p.z = z[0] + z[1] + w;
-        p.t = fmaf(w, fmaxf(y, -256.0f), t[0] + t[1]);
+        p.z = z.x + z.y + w;
+        p.t = fmaf(w, fmaxf(y, -256.0f), t.x + t.y);
         const float d = p.m == -INFINITY ? 0.0f : (B - p.m) * a.c, f = ex2f(d);            // from the base to the maximum
         p.t = f * fmaf(p.z, d, p.t);
         p.z *= f;
