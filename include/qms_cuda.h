@@ -242,8 +242,8 @@ typedef struct {
 } QmsCudaPagedBatch;
 
 /* QK-norm, NEOX rotation and the cache append of new tokens in one pass (src/model.c:436-462, the
- * arithmetic of the whole model's own cache, value for value; into 4 bits, K goes in double to the end). qkv: fp32 [n_tok] rows of ldqkv: n_head
- * q heads, n_head_kv k heads, n_head_kv v heads of head_dim, as the projections leave them; q_norm,
+ * arithmetic of the whole model's own cache, value for value; into 4 bits, K goes in double to the
+ * end). qkv: fp32 [n_tok] rows of ldqkv: n_head q heads, n_head_kv k heads, n_head_kv v heads of head_dim, as the projections leave them; q_norm,
  * k_norm: fp32 [head_dim]; rope_cos / rope_sin: fp32 [n_rope][head_dim / 2]. q receives the normalised and
  * rotated q heads (rows of ldq; may be qkv itself with ldq = ldqkv, but overlaps it in no other way),
  * K and V go to the pages. Padding rows are left alone; a row whose position is negative, at or past
@@ -274,7 +274,7 @@ typedef struct {
  * or 128, up to 128 q heads per kv head, scale > 0. Rows of no prompt are left as they were; a prompt whose rows make no sense sets
  * QMS_PAGED_ELEN and is left out. What a row does not see has no effect on it, whatever its bits; a V value that it sees and that is
  * not finite makes that element of the row not finite. Precision: q, k, v are exact, a weight is rounded to the type once (as
- * the output is), scores and sums are fp32. */
+ * the output is), scores and sums are fp32. Scores are below 10^7 in magnitude: a row with larger ones may be NaN. */
 int qms_cuda_prompt_attention(const QmsCudaPagedBatch *batch, int type, const QmsCudaHeads *q, const QmsCudaHeads *k, const QmsCudaHeads *v,
                               int n_head, int n_head_kv, int head_dim, float scale, int out_type, const QmsCudaHeads *out, int *err,
                               void *stream);
@@ -290,13 +290,15 @@ int qms_cuda_paged_values(const QmsCudaPages *pages, float *k, float *v, void *s
  * have weight 0 (a row with no other is 0 or NaN); rows with K that is not finite take a slow path. A
  * row that sees nothing (padding, a negative position, an idle sequence) is zero; positions on a bad
  * page set *err and count as not seen.
- * Precision: q, the weights and an fp32 cache's K and V (those of an fp16 one and of one in 4 bits are exact in fp16) enter the products as two fp16 terms, 22 bits,
+ * Precision: q, the weights and an fp32 cache's K and V (those of an fp16 one and of one in 4 bits are
+ * exact in fp16) enter the products as two fp16 terms, 22 bits,
  * under power-of-two scales: of q by row, of K by position or by 64 of them, of V by the largest so
  * far that any row sees that shares the K and V tiles. What is 2^-10 of the largest or less is kept to
  * 2^-33 of the largest. Sums are fp32: an output is off by some 1e-6 of itself, or up to 6e-6 where
- * many rows meet many positions and the values have one sign.
+ * many rows meet many positions and the values have one sign. Scores are below 2^26 in magnitude.
  * ws: device workspace, 256-byte aligned, of at least qms_cuda_paged_attention_ws() bytes (a function
- * of the sizes in the two descriptors; negative: a status), contents irrelevant before and after. */
+ * of the sizes in the two descriptors; negative: a status), contents irrelevant before and after. Over pages in 4 bits, where more than
+ * 256 rows meet a shared prompt, or a single sequence, it has room for those positions in fp16, up to 128 MiB each of K and V. */
 int64_t qms_cuda_paged_attention_ws(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, int n_head);
 int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *q, int64_t ldq,
                              int n_head, float scale, float *out, int64_t ldo, void *ws, int64_t ws_bytes, int *err,

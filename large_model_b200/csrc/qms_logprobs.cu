@@ -13,7 +13,8 @@ namespace qms {
 typedef unsigned long long u64;
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32;
-constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2, kLpKeep = 6, kLpList = 2048;       // a warp's: groups of 4 values per lane, values per chunk, chunks in flight, or kept
+// a warp's groups of 4 values per lane, values per chunk, chunks in flight, or kept; entries of the list
+constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2, kLpKeep = 6, kLpList = 2048;
 constexpr uint32_t kLpSpin = 1u << 22;
 constexpr int kLpFew = 74;            // CTAs up to which a row's slices are kept in shared memory (launch_logprobs)
 
@@ -98,14 +99,17 @@ __device__ __forceinline__ LpPart lp_under(const LpPart &p, float M, bool first,
 
 // With x = (l - max) / temp: log p = x - log Z and the entropy log Z - sum p x, where Z = 1 + z and z leaves out one value that is the
 // maximum: of a sure row z is what matters, and 1 + z would round it away. One pass, and no warp waits for another before its end: a row
-// is cut over a cluster, the warps of a CTA take its chunks in turn, each into its part of shared memory by bulk copies. A lane keeps two running maxima apart from its sums (what is no longer the largest is added), under a
-// base that follows them at a distance of 2^4 at most.
+// is cut over a cluster, the warps of a CTA take its chunks in turn, each into its part of shared memory by bulk copies. A lane keeps two
+// running maxima apart from its sums (what is no longer the largest is added), under a base that follows them at a distance of 2^4 at
+// most, and adds two values by one instruction (512 rows 84 us, one by one 88).
 // The likeliest: lane i holds the i-th largest of its warp's so far. Values that reach a bound are put in their place: first one that n_top
-// lanes' largest of the first chunk reach, then the n_top-th itself, of this warp or of another that is further. Some 35
-// of 2400 values reach it; those of a chunk are put in together. The first CTA of the cluster joins all.
+// lanes' largest of the first chunk reach, then the n_top-th itself, of this warp or of another that is further. Some 40 of 19,000 values
+// reach it, in 14 chunks of 37; those of a chunk are put in together. The first CTA of the cluster joins all.
 // KEEP: for few rows, where that chain of steps is what the row takes: all of a slice stays in shared memory, the bound comes from all lanes'
 // largest (the least over the warps of each one's r-th, r = n_top over the number of warps), and a second look lists what reaches it, some
 // 60 of 19,000, whose places are the numbers of entries above them.
+// Bound by instructions for many rows, some 17 per value and lane (0.7 per cycle and scheduler), a third more with ten alternatives: 512 rows of 151,936 84 us,
+// 3.7 TB/s, without alternatives 57, 5.5 TB/s, 0.83 of a plain copy. One row by the chain of its steps: 10.2 us, without alternatives 5.2.
 template <bool KEEP>
 __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const LogprobArgs a) {
     constexpr int RING = KEEP ? kLpKeep : kLpRing;
@@ -347,7 +351,9 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
                         const int i = lane + e * 32;
                         if (i >= n4) break;
                         const float4 y = x4[i];
-                        if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound) f(y.x, base + 4 * i), f(y.y, base + 4 * i + 1), f(y.z, base + 4 * i + 2), f(y.w, base + 4 * i + 3);
+                        if (fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= bound) {
+                            f(y.x, base + 4 * i), f(y.y, base + 4 * i + 1), f(y.z, base + 4 * i + 2), f(y.w, base + 4 * i + 3);
+                        }
                     }
                 }
                 if (rank == 0 && tid < head) f(row[tid], tid);
@@ -443,7 +449,8 @@ static int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t s) {
     while (nc < kRowCtas && a.V > nc * kLpWarps * kLpChunk && (int64_t)rows * nc < 500) nc *= 2;
     // Kept in shared memory for few CTAs. Both in us, not kept and kept: 1 row of 151,936 14.3, 10.2; 8 rows 14.8, 11.3; 19 rows 16.9, 18.5; 64
     // rows of 4096 8.4, 7.2; 16 rows of 32,003 9.1, 11.7.
-    if ((int64_t)rows * nc <= kLpFew && a.V / nc + 8 <= kLpWarps * kLpKeep * kLpChunk) return launch_rows(k_logprobs<true>, kLpThreads, rows, nc, keep, s, a);
+    const bool few = (int64_t)rows * nc <= kLpFew && a.V / nc + 8 <= kLpWarps * kLpKeep * kLpChunk;
+    if (few) return launch_rows(k_logprobs<true>, kLpThreads, rows, nc, keep, s, a);
     return launch_rows(k_logprobs<false>, kLpThreads, rows, nc, ring, s, a);
 }
 

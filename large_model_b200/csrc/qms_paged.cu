@@ -223,9 +223,10 @@ __device__ __forceinline__ void q_rows16(const float2 (&x)[R][2], int cnt, const
 
 // k_paged_append's steps where the cache or the rows that go out are of another kind: a cache in 4 bits (K normalised and rotated in
 // double, see above), or none; rows out of fp32, the q heads, or of 16 bits, all heads q | k | v as the prompt attention reads
-// them, each value rounded once from fp32.
-// (rows out of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.) A warp takes R q heads, or one K or V
-// head: what is stored in 4 bits takes as long as four q heads.
+// them, each value rounded once from fp32. (Rows of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.)
+// A warp takes R q heads, or one K or V head: what is stored in 4 bits takes as long as four q heads.
+// Bound by latency for few rows (64 tokens of 72 heads 4.1 us, one token 3.1), by instructions for many, those of the exchanges within 32
+// values and, for K, of double where fp32 does not settle a border: 700 tokens of 40 heads 9.9 us with rows in 16 bits, 2.5 TB/s.
 template <int D, typename OT, int R>
 __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int type, const float *qkv, int64_t ldqkv, const float *q_norm,
                                                      const float *k_norm, float eps, const float *rope_cos, const float *rope_sin, int n_rope,
@@ -339,18 +340,20 @@ template <int D, typename OT>
 static int launch_rows_append(const Paged &a, int type, const float *qkv, int64_t ldqkv, const float *q_norm, const float *k_norm, float eps,
                               const float *rope_cos, const float *rope_sin, int n_rope, OT *out, int64_t ldo, cudaStream_t s) {
     const int heads = a.H + 2 * a.Hk;
-    const bool four = (int64_t)a.n_tok * heads >= 148 * 48;     // (as k_paged_append)
+    // Four q heads per warp from 32 head rows for each SM on. Both in us, one and four: 2304 rows 3.6, 3.6; 4608 4.1, 4.1; 5120 5.3, 4.1; 7200 5.6, 4.3;
+    // 28,000 14.6, 11.3; 160,000 78, 55 (rows in 16 bits 69, 45).
+    const bool four = (int64_t)a.n_tok * heads >= 148 * 32;
     const int64_t units = (int64_t)a.n_tok * (four ? (a.H + 3) / 4 + 2 * a.Hk : heads);
     QMS_REQUIRE(units < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "append: too many rows");
     const dim3 grid((unsigned)((units + 7) / 8));
-    if (four) QMS_CK(launch_pdl(k_rows_append<D, OT, 4>, grid, dim3(256), 0, s, a, type, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, out, ldo));
-    else QMS_CK(launch_pdl(k_rows_append<D, OT, 1>, grid, dim3(256), 0, s, a, type, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, out, ldo));
+    const auto k = four ? k_rows_append<D, OT, 4> : k_rows_append<D, OT, 1>;
+    QMS_CK(launch_pdl(k, grid, dim3(256), 0, s, a, type, qkv, ldqkv, q_norm, k_norm, eps, rope_cos, rope_sin, n_rope, out, ldo));
     return QMS_CUDA_OK;
 }
 
 // ---- what a pool's pages hold, as fp32 ---------------------------------------------------------------
 // 8 values per thread, in the order of the result [page][position][head][value]: whole lines are written. Grid y: K, V. Bound by
-// those writes.
+// those writes: 64 pages of 16 positions and 4 heads 3.6 us.
 template <int D>
 __global__ void __launch_bounds__(256) k_paged_values(const Paged a, const int type, float *ko, float *vo) {
     pdl_trigger();
@@ -376,7 +379,8 @@ __global__ void __launch_bounds__(256) k_paged_values(const Paged a, const int t
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                const float4 f = type == QMS_T_F16 ? kv_ldg4(reinterpret_cast<const __half *>(src) + 8 * w + e) : kv_ldg4(reinterpret_cast<const float *>(src) + 8 * w + e);
+                const float4 f = type == QMS_T_F16 ? kv_ldg4(reinterpret_cast<const __half *>(src) + 8 * w + e)
+                                                   : kv_ldg4(reinterpret_cast<const float *>(src) + 8 * w + e);
                 x[e] = f.x, x[e + 1] = f.y, x[e + 2] = f.z, x[e + 3] = f.w;
             }
         }

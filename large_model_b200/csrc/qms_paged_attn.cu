@@ -6,7 +6,8 @@
 // into two fp16 terms (one alone would leave an error of 2^-12), and their products are added in fp32.
 // Over an fp16 cache K and V are exact: two mma.sync m16n8k16 per product. Over an fp32 cache K and V are split too,
 // once per stage in shared memory, and three products kept (lo * lo is below 2^-22); the tf32 form of the same
-// (m16n8k8, three products, split in every warp) took about twice as long.
+// (m16n8k8, three products, split in every warp) took about twice as long. Over a cache in 4 bits K and V go to fp16, exact, once per
+// stage in shared memory, for 17 to 64 rows; up to 16 rows are k_paged_q4's.
 #include <math.h>
 #include <string.h>
 
@@ -880,8 +881,9 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, dou
     const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
-    // (4 bits, up to 16 rows, with 1.2 and 4.0 us as the others: 64 x 4096 positions 95.2, 89.6; 131072 58.5, 54.7)
-    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * 3 * share)), 0.6, 3.0, most);
+    // 4 bits, up to 16 rows (k_paged_q4): stages of 128 positions, three CTAs per SM. Cut by the 64 in us, and so: 1100 positions 11.5, 10.1; 131,072
+    // 58.4, 51.8; 64 sequences of 2048 56.5, 53.7; of 4096 89.5, 89.5. Two or six per SM 61.5, 62.5 on 131,072.
+    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, 128, std::max(1, (int)(148 * 3 * share)), 1.2, 3.0, most);
     const int per_sm = type != QMS_T_F32 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * per_sm * share)), wr == 4 ? 2.0 : 1.2, 4.0, most);
 }
@@ -999,7 +1001,7 @@ static int launch_attn(const PagedAttn &A, const PagedAttn &F, cudaStream_t s) {
         const int wr = own ? A.p.wr_s : A.p.wr_p;
         int rc;
         if constexpr (std::is_same<KT, Q4>::value)
-            rc = wr <= 0   ? launch_paged_wide(wr == kPaWidePair ? F : A, D, own, before, s)
+            rc = wr <= 0   ? launch_paged_wide(wr == kPaWidePair ? F : A, D, own, before, s)      // (PAIR: over the workspace's fp16)
                  : wr == 4 ? launch_attn_wr<D, KT, 4>(A, own, before, s)
                  : wr == 2 ? launch_attn_wr<D, KT, 2>(A, own, before, s)
                            : launch_paged_q4(A, D, own, before, s);

@@ -10,7 +10,11 @@
 // A nibble becomes d (n - 8) by a shift, a mask and one fused step, exact in fp16 (q4_dequant). q and the weights have two terms,
 // sums join by rounded additions, as in k_paged_attn. Each warp has positions of its own, in tiles of 16 in turn, its own copies in
 // flight and its own (m, l, o); they meet at the end of a unit.
-// Bound by instructions: some 400 per warp for 16 positions of 2.3 KB.
+// Bound by instructions: some 1320 per warp for 32 positions (4.6 KB), 128 of them MMAs, 350 for what comes out of the nibbles; 0.44 per cycle and
+// scheduler, where each next step waits for the one before it. 64 sequences of 4096 positions (64 q heads, 4 kv heads) 89.5 us, 1.69 TB/s; one of
+// 131,072 (32 q heads) 51.8, 1.46 TB/s; one of 1100 10.1, of which some 4 are the launch and 4 the join of the slots.
+// The same with K and V's transpose as tcgen05's M operand, 128 positions or values, and the rows as its N: 110 us and 55, by the way of K and
+// V through shared memory in fp16 (164 KB in and out for 18 that are read).
 #include <math.h>
 #include <string.h>
 
@@ -228,7 +232,8 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
                     const uint32_t qh[4] = {h4.x, h4.y, h4.z, h4.w}, ql[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint32_t b0 = q4_pair(w[i][k / 2], 2 * (k & 1), d[i], m24[i], six), b1 = q4_pair(w[i][k / 2], 2 * (k & 1) + 1, d[i], m24[i], six);
+                        const uint32_t b0 = q4_pair(w[i][k / 2], 2 * (k & 1), d[i], m24[i], six);
+                        const uint32_t b1 = q4_pair(w[i][k / 2], 2 * (k & 1) + 1, d[i], m24[i], six);
                         if (k == 0) {
                             mma_16_first(s[i], qh, b0, b1);
                             mma_16_first(s2[i], ql, b0, b1);
@@ -325,24 +330,29 @@ __global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bo
                         v[x][1] = __byte_perm(w[x][2][i], w[x][3][i], h ? 0x7632 : 0x5410);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        float t2[2][4];
+                    for (int e = 0; e < 4; e += 2) {             // two products at a time
+                        float sum[2][4];
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            uint32_t v0[2], v1[2];
+                            uint32_t b[2][2];
 #pragma unroll
-                            for (int ee = 0; ee < 2; ee++) v0[ee] = q4_pair(v[x][0], e + ee, d[x][0], m24[x][0], six), v1[ee] = q4_pair(v[x][1], e + ee, d[x][1], m24[x][1], six);
+                            for (int k = 0; k < 2; k++)
 #pragma unroll
-                            for (int ee = 0; ee < 2; ee++) { if (x == 0) mma_16_first(t2[ee], pl[x], v0[ee], v1[ee]); else mma_16(t2[ee], pl[x], v0[ee], v1[ee]); }
+                                for (int z = 0; z < 2; z++) b[k][z] = q4_pair(v[x][z], e + k, d[x][z], m24[x][z], six);
 #pragma unroll
-                            for (int ee = 0; ee < 2; ee++) mma_16(t2[ee], ph[x], v0[ee], v1[ee]);
+                            for (int k = 0; k < 2; k++) {
+                                if (x == 0) mma_16_first(sum[k], pl[x], b[k][0], b[k][1]);
+                                else mma_16(sum[k], pl[x], b[k][0], b[k][1]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 2; k++) mma_16(sum[k], ph[x], b[k][0], b[k][1]);
                         }
 #pragma unroll
-                        for (int ee = 0; ee < 2; ee++) {
-                        float(&t)[4] = t2[ee];
-                        float(&y)[4] = o[8 * i + 2 * (e + ee) + h];
-                        const float2 lo = f2_add(make_float2(y[0], y[1]), make_float2(t[0], t[1])), hi = f2_add(make_float2(y[2], y[3]), make_float2(t[2], t[3]));
-                        y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
+                        for (int k = 0; k < 2; k++) {
+                            float(&y)[4] = o[8 * i + 2 * (e + k) + h];
+                            const float2 lo = f2_add(make_float2(y[0], y[1]), make_float2(sum[k][0], sum[k][1]));
+                            const float2 hi = f2_add(make_float2(y[2], y[3]), make_float2(sum[k][2], sum[k][3]));
+                            y[0] = lo.x, y[1] = lo.y, y[2] = hi.x, y[3] = hi.y;
                         }
                     }
                 }

@@ -6,6 +6,8 @@
 //   PAIR   fp16 cache, 256 rows: a stream per 128 rows, both over every tile of 128 positions
 //   SPLIT  fp16 cache, 128 rows: the even and the odd tiles, joined at the end of the unit
 //   F32    fp32 cache, 128 rows: the same with tiles of 64 positions, split into fp16 terms on the way
+//   NIB    cache in 4 bits, 128 rows: as F32, tiles of 128 positions, to fp16 on the way, exact (one term); for up to 256 rows on a
+//          position or several sequences' own ones (beyond that the positions go to fp16 in the workspace first, and PAIR reads them)
 // For each tile of a stream
 //   S = Q K^T   tcgen05.mma kind::f16 from shared memory, M 128, N the positions, K = head_dim, with 22-bit operands: Q =
 //               hi + lo in fp16 (each row scaled by a power of two into fp16's range), K exact in fp16 (two
@@ -27,11 +29,12 @@
 // under a lock: one thread for both leaves the tensor cores idle while it waits and commits (some 1200 of 6150 cycles
 // per pair of tiles: hardly one MMA is queued), two that interleave slow every MMA down.
 // Shared memory at head_dim 128: Q 128 KB and a ring of 3 tiles of 32 KB (PAIR), Q 64 KB and a ring of 2 for each stream
-// (SPLIT), Q 64 KB, 2 stages and a ring of 3 (F32); TMEM: S 2 x 128, O 2 x 128 columns.
+// (SPLIT), Q 64 KB, 2 stages and a ring of 3 (F32, NIB); TMEM: S 2 x 128, O 2 x 128 columns.
 // Bound by the tensor cores, 4 * 128 * 128 * head_dim flop per 128 rows and positions, times 2 (fp16) or 3, and by the softmax
 // between a tile's two products where the other stream does not cover it: 64 sequences of 5 tokens (64 q heads, 4 kv heads)
 // over 8192 shared and 640 own fp16 positions take 235 us, 394 TFLOP/s by the definition and 788 with the split; tensor
-// cores 45% active. A prompt chunk of 256 tokens over 4096 positions: 85 us, 394 TFLOP/s.
+// cores 45% active. A prompt chunk of 256 tokens over 4096 positions: 85 us, 394 TFLOP/s. Over 4 bits by way of the workspace 251 and 86 us
+// (the step to fp16 some 8 of the 251); NIB for the same 348 and 119: its four warps convert each tile for 128 rows, some 2000 cycles.
 #include <math.h>
 #include <string.h>
 
@@ -58,7 +61,8 @@ struct WideCfg {
     static constexpr uint32_t HALF = TP * 128, TILE = HALVES * HALF;         // one term of a K or V tile
     static constexpr uint32_t SLOT = (MODE == F32 ? 2 : 1) * TILE;
     static constexpr int SLOTS = MODE == SPLIT ? 4 : 3;
-    static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT, STAGED = MODE == F32 ? TP * D * 4 : MODE == NIB ? TP * q4_row(D) : 0;
+    static constexpr uint32_t RING = (MODE == PAIR ? 4 : 2) * QTILE, STAGE = RING + SLOTS * SLOT;
+    static constexpr uint32_t STAGED = MODE == F32 ? TP * D * 4 : MODE == NIB ? TP * q4_row(D) : 0;
     // then: bad-page masks [8][4]; scales of K and V tiles [2][4], maxima [2][4]; a stream's (B, l, V scale) by row;
     // barriers; flags
     static constexpr uint32_t BAD = STAGE + 2 * STAGED, UP = BAD + 128, JOIN = UP + 64,

@@ -13,6 +13,10 @@
 // B is a whole number and stays until a score lies 2^15 above it. S is read twice, for its maximum and for the weights: one vote per
 // tile, nothing that the exponentials wait for, and short loops (a row's 128 scores in registers, all in line: 1.03 times as fast over 8192
 // positions, 0.87 over 1500).
+// Bound by the two products and the exponentials in turn (16 of a row's 128 per cycle and SM), and by what is between them where two streams
+// do not cover it: 8192 tokens of 64 q heads and 4 kv heads 1062 to 1179 us with the clock, 0.93 to 1.03 PFLOP/s, 0.56 to 0.62 of the library's rate for one large product;
+// 17 prompts of up to 1500 tokens 160, 0.59 PFLOP/s (the tiles on the diagonal, and two or three tiles to start and to end with). Short ones by the
+// chain of one unit, 9 us: 100 tokens 9.1, 64 prompts of up to 333 tokens with 8 heads of 64 values 26.5 for 2.6 units per SM.
 #include <cuda_bf16.h>
 #include <math.h>
 #include <string.h>
@@ -43,9 +47,8 @@ struct PrCfg {
     static constexpr int HALVES = D / 64;                       // 64 values = 128 bytes: one swizzle row
     static constexpr uint32_t HALF = 128 * 128, TILE = HALVES * HALF;
     static constexpr uint32_t SLOTS = D == 128 ? 5 : 8;
-    // then: the unit at hand and the answer of who asked for the next; barriers; a number for each row and half
-    static constexpr uint32_t RING = 2 * TILE, UNIT = RING + SLOTS * TILE, BARS = UNIT + 32, SUMS = BARS + (3 * SLOTS + 14) * 8 + 16,
-                              SMEM = SUMS + 2 * 2 * 128 * 4;
+    // then: the unit at hand and the answer of who asked for the next; barriers; flags
+    static constexpr uint32_t RING = 2 * TILE, UNIT = RING + SLOTS * TILE, BARS = UNIT + 32, SMEM = BARS + (3 * SLOTS + 14) * 8 + 16;
     static constexpr uint32_t O_COL = 256;                      // TMEM columns: S0, S1, O0, O1
 };
 
@@ -64,11 +67,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
                  "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 __device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap *map, int x, int head, int tok, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
@@ -311,23 +309,29 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                 uint32_t x[32], y[32];
                 const int chunks = min(4, (last - j * 128) / 32 + 1);
                 float mx0 = -INFINITY, mx1 = -INFINITY;
+                auto most = [&](const uint32_t (&z)[32], int e) {
+                    mx0 = max3(mx0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                    mx1 = max3(mx1, __uint_as_float(z[e + 2]), __uint_as_float(z[e + 3]));
+                };
                 tmem_ld<32>(s_col, x);
 #pragma unroll 1
                 for (int c = 0; c < 4; c += 2) {
                     tmem_wait_ld(x);
                     tmem_ld<32>(s_col + 32 * c + 32, y);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) mx0 = max3(mx0, __uint_as_float(x[e]), __uint_as_float(x[e + 1])), mx1 = max3(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                    for (int e = 0; e < 32; e += 4) most(x, e);
                     tmem_wait_ld(y);
                     if (c == 0) tmem_ld<32>(s_col + 64, x);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) mx0 = max3(mx0, __uint_as_float(y[e]), __uint_as_float(y[e + 1])), mx1 = max3(mx1, __uint_as_float(y[e + 2]), __uint_as_float(y[e + 3]));
+                    for (int e = 0; e < 32; e += 4) most(y, e);
                 }
                 tmem_ld<32>(s_col, x);
                 const float top = fmaxf(mx0, mx1) * f;
                 // the base stays unless a score lies 2^kPrHigh above it: then what was computed with the old one is scaled
-                if (__any_sync(kFull, top > B + kPrHigh)) {
-                    const float nb = top > B + kPrHigh ? ceilf(top) - kPrLow : B, fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
+                if (__any_sync(kFull, top - B > kPrHigh)) {
+                    // (from 2^24 on a score's own rounding would move the weights by powers of 2: NaN says so)
+                    const float far = fabsf(top) < 16777216.0f ? ceilf(top) - kPrLow : NAN, nb = top - B > kPrHigh ? far : B;
+                    const float fac = B == nb ? 1.0f : B == -INFINITY ? 0.0f : ex2(B - nb);
                     B = nb;
                     l *= fac;
                     if (j > 0) scale_o(fac);

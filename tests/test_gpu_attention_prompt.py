@@ -254,3 +254,25 @@ def test_refusals(cuda):
                 lambda: m.prompt_attention(batch, q, k, v, scale=-1.0), lambda: m.prompt_attention(batch, q[..., :96], k[..., :96], v[..., :96])):
         with pytest.raises(m.QmsCudaError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_scores_beyond_two_to_the_27(cuda, dtype):
+    """Scores whose own rounding in fp32 is whole powers of 2 of a weight: the rows say so. (What a row does not see is no reason to.)"""
+    import torch
+    import large_model_b200 as m
+    n, D = 200, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    step = torch.randperm(n, generator=g, device="cuda") // 2 + 100          # two positions each
+    typ = getattr(torch, dtype)
+    q = torch.full((n, 2, D), 4096.0, device="cuda", dtype=typ)
+    k = (step * 256.0)[:, None, None].expand(n, 1, D).to(typ).contiguous()
+    v = torch.randn((n, 1, D), generator=g, device="cuda").to(typ)
+    batch = m.PagedBatch.prompts(torch.tensor([0, n], dtype=torch.int32, device="cuda"), n, n)
+    out = m.prompt_attention(batch, q, k, v, out_dtype=torch.float32)
+    batch.status()
+    assert out.isnan().all()
+    q[:150] = 0
+    out = m.prompt_attention(batch, q, k, v, out_dtype=torch.float32)
+    want = v[:, 0].double().cumsum(0)[:150] / torch.arange(1, 151, device="cuda")[:, None]
+    assert ((out[:150].double() - want[:, None]).abs() <= 32 * E * v.abs().max()).all() and out[150:].isnan().all()
