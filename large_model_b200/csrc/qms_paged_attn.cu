@@ -1058,15 +1058,14 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     // positions) 14.9, 16.1; 512 rows on a prompt of 4096 positions 24.7, 28.9; 1024 rows of 100 positions 11.5, 9.1; 3072 rows
     // of 1000 positions 28.3, 25.2.
     const int64_t rows = (int64_t)a.n_tok * a.H;
-    const int wpr = rows <= 4 * 148 || p.slots_p + p.slots_s > 32 ? 4 : 1;
+    // Over 4 bits eight for a row per SM or less and more than 12 slots, four against eight: 9 slots 10.0, 10.1; 32 14.2, 13.2; 55 (16,384 positions)
+    // 24.3, 22.7; 103 (131,072) 54.9, 53.3. (The others keep the order of their sums.)
+    const int slots = p.slots_p + p.slots_s;
+    const int wpr = type == QMS_T_Q4_0 && slots > 12 && rows <= 148 ? 8 : rows <= 4 * 148 || slots > 32 ? 4 : 1;
     const dim3 grid((unsigned)((rows * wpr + 7) / 8));
-    if (D == 128) {
-        if (wpr == 4) QMS_CK(launch_pdl(k_paged_merge<128, 4>, grid, dim3(256), 0, s, A));
-        else QMS_CK(launch_pdl(k_paged_merge<128, 1>, grid, dim3(256), 0, s, A));
-    } else {
-        if (wpr == 4) QMS_CK(launch_pdl(k_paged_merge<64, 4>, grid, dim3(256), 0, s, A));
-        else QMS_CK(launch_pdl(k_paged_merge<64, 1>, grid, dim3(256), 0, s, A));
-    }
+    const auto merge = D == 128 ? wpr == 8 ? k_paged_merge<128, 8> : wpr == 4 ? k_paged_merge<128, 4> : k_paged_merge<128, 1>
+                                : wpr == 8 ? k_paged_merge<64, 8> : wpr == 4 ? k_paged_merge<64, 4> : k_paged_merge<64, 1>;
+    QMS_CK(launch_pdl(merge, grid, dim3(256), 0, s, A));
     return QMS_CUDA_OK;
 }
 
