@@ -254,7 +254,7 @@ int qms_cuda_paged_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *ba
 
 /* The same for whole prompts, with all heads' rows as qms_cuda_prompt_attention reads them: q | k | v heads of each token,
  * normalised and rotated, in 16 bits (type QMS_T_F16 or QMS_CUDA_T_BF16; rows of ldrows values, a multiple of 8; 16-byte
- * aligned), each value rounded once from fp32. The pages receive what qms_cuda_paged_append gives them. Without a cache (n_pages 0, k and
+ * aligned; they overlap nothing else), each value rounded once from fp32. The pages receive what qms_cuda_paged_append gives them. Without a cache (n_pages 0, k and
  * v NULL) nothing is stored, and kv_len and table are not looked at: a row's position is its index in its sequence. */
 int qms_cuda_prompt_append(const QmsCudaPages *pages, const QmsCudaPagedBatch *batch, const float *qkv, int64_t ldqkv, int n_head,
                            const float *q_norm, const float *k_norm, float eps, const float *rope_cos, const float *rope_sin,
