@@ -461,30 +461,22 @@ def _on_stream(raw: int, device):
     return torch.cuda.stream(torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device))
 
 
-class _Same:
-    """Nothing to enter: the call's device is the current one."""
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *_):
-        pass
-
-
-_same = _Same()
-
-
-def _device_of(t):
-    """t's device as the current one, for the call."""
+def _on_device(d: int, call, *args) -> int:
+    """A call into the library with device d as the current one."""
     torch = _torch()
-    return _same if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    if torch._C._cuda_getDevice() == d:
+        return call(*args)
+    with torch.cuda.device(d):
+        return call(*args)
 
 
-def _one_device(who: str, t, *others):
+def _one_device(who: str, t, *others) -> int:
+    """The index of the device on which all of them lie."""
     d = t.get_device()
     for o in others:
         if o is not None and o.get_device() != d:
             raise ValueError(f"{who}: tensors on {t.device} and {o.device}")
+    return d
 
 
 def _empty(shape: tuple, dtype, device, stream):
@@ -515,7 +507,7 @@ class KvPages:
         st = k.stride()
         self.desc = PagesDesc(typ, k.shape[0], k.shape[1], k.shape[2], k.shape[3], st[0], st[1], st[2], k.data_ptr(),
                               v.data_ptr())
-        self._ref = C.byref(self.desc)
+        self._ref, self._dev = C.byref(self.desc), k.get_device()
         self._key = (typ,) + tuple(k.shape[1:])
 
     @classmethod
@@ -545,7 +537,7 @@ class KvPages:
         self.n_head_kv, self.head_dim = k.shape[1], int(head_dim)
         page = k.shape[2] * 16 // (9 * head_dim)
         self.desc = PagesDesc(T_Q4_0, k.shape[0], page, k.shape[1], head_dim, k.stride(0), 0, k.stride(1), k.data_ptr(), v.data_ptr())
-        self._ref = C.byref(self.desc)
+        self._ref, self._dev = C.byref(self.desc), k.get_device()
         self._key = (T_Q4_0, page, k.shape[1], int(head_dim))
         return self
 
@@ -555,9 +547,8 @@ class KvPages:
         shape = (d.n_pages, d.page_size, d.n_head_kv, d.head_dim)
         n = shape[0] * shape[1] * shape[2] * shape[3]
         k, v = (_empty(shape, _torch().float32, self.k.device, stream) if x is None else x for x in (k, v))
-        _one_device("KvPages.values", self.k, k, v)
-        with _device_of(self.k):
-            rc = lib().qms_cuda_paged_values(self._ref, _vec(k, n, "k"), _vec(v, n, "v"), _raw_stream(stream, self.k))
+        rc = _on_device(_one_device("KvPages.values", self.k, k, v), lib().qms_cuda_paged_values, self._ref, _vec(k, n, "k"), _vec(v, n, "v"),
+                        _raw_stream(stream, self.k))
         if rc:
             check(rc)
         return k, v
@@ -576,7 +567,7 @@ class PagedBatch:
         self.q_start, self.kv_len, self.table = q_start, kv_len, table
         self.n_tok = int(n_tok)
         self.err = torch.zeros((1,), dtype=torch.int32, device=kv_len.device)
-        self._err = self.err.data_ptr()
+        self._err, self._dev = self.err.data_ptr(), self.err.get_device()
         self._cleared()
         self.desc = PagedBatchDesc(n, self.n_tok, _ints(q_start, (n + 1,), "q_start"), _ints(kv_len, (n,), "kv_len"),
                                    _ints(table, (n, table.shape[1]), "table"), table.shape[1], int(max_q), int(max_kv),
@@ -593,7 +584,7 @@ class PagedBatch:
         n = q_start.shape[0] - 1
         self.q_start, self.kv_len, self.table, self.n_tok = q_start, None, None, int(n_tok)
         self.err = torch.zeros((1,), dtype=torch.int32, device=q_start.device)
-        self._err = self.err.data_ptr()
+        self._err, self._dev = self.err.data_ptr(), self.err.get_device()
         self._cleared()
         self.desc = PagedBatchDesc(n, self.n_tok, _ints(q_start, (n + 1,), "q_start"), None, None, 0, int(max_q), 0, 0)
         self._ref = C.byref(self.desc)
@@ -665,11 +656,12 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     nc = cos.shape[0]
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens")
-    _one_device("paged_append", qkv, q, pages.k, batch.err, q_norm, k_norm, cos, sin)
-    with _device_of(qkv):
-        rc = lib().qms_cuda_paged_append(pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
-                                         eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy,
-                                         batch._err, batch._use(stream, qkv))
+    d = qkv.get_device()
+    if d != pages._dev or d != batch._dev or q.get_device() != d or q_norm.get_device() != d or cos.get_device() != d:
+        _one_device("paged_append", qkv, q, pages.k, batch.err, q_norm, cos)
+    rc = _on_device(d, lib().qms_cuda_paged_append, pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
+                    eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy, batch._err,
+                    batch._use(stream, qkv))
     if rc:
         check(rc)
     return q
@@ -708,12 +700,11 @@ def prompt_append(pages: KvPages | None, batch: PagedBatch, qkv, n_head: int, q_
     nc = cos.shape[0]
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"prompt_append: {n} qkv and {ny} result rows for {batch.n_tok} tokens")
-    _one_device("prompt_append", qkv, rows, batch.err, q_norm, k_norm, cos, sin, None if pages is None else pages.k)
+    d = _one_device("prompt_append", qkv, rows, batch.err, q_norm, k_norm, cos, sin, None if pages is None else pages.k)
     ref = C.byref(PagesDesc(T_F32, 0, 0, Hk, D, 0, 0, 0, None, None)) if pages is None else pages._ref
-    with _device_of(qkv):
-        rc = lib().qms_cuda_prompt_append(ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"), eps,
-                                          _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, typ, y, ldy, batch._err,
-                                          batch._use(stream, qkv))
+    rc = _on_device(d, lib().qms_cuda_prompt_append, ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"), eps,
+                    _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, typ, y, ldy, batch._err,
+                    batch._use(stream, qkv))
     if rc:
         check(rc)
     return rows
@@ -748,12 +739,10 @@ def prompt_attention(batch: PagedBatch, q, k, v, scale: float | None = None, out
     otyp = typ if odt is dt else T_F32 if odt is torch.float32 else None
     if otyp is None or out.shape[1:] != (H, D):
         raise ValueError(f"prompt_attention: out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
-    _one_device("prompt_attention", q, k, v, out, batch.err)
+    d = _one_device("prompt_attention", q, k, v, out, batch.err)
     T = batch.n_tok
-    with _device_of(q):
-        rc = lib().qms_cuda_prompt_attention(batch._ref, typ, _heads(q, T, "q"), _heads(k, T, "k"), _heads(v, T, "v"), H, ks[1], D,
-                                             D ** -0.5 if scale is None else scale, otyp, _heads(out, T, "out"), batch._err,
-                                             batch._use(stream, q))
+    rc = _on_device(d, lib().qms_cuda_prompt_attention, batch._ref, typ, _heads(q, T, "q"), _heads(k, T, "k"), _heads(v, T, "v"), H, ks[1], D,
+                    D ** -0.5 if scale is None else scale, otyp, _heads(out, T, "out"), batch._err, batch._use(stream, q))
     if rc:
         check(rc)
     return out
@@ -769,12 +758,13 @@ def paged_attention(pages: KvPages, batch: PagedBatch, q, n_head: int, scale: fl
     y, ny, ldy = _rows(out, n_head * D, "out")
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_attention: {n} q and {ny} out rows for {batch.n_tok} tokens")
-    _one_device("paged_attention", q, out, pages.k, batch.err)
-    with _device_of(q):
-        raw = batch._use(stream, q)
-        ws, nb = batch.workspace(pages, n_head, raw)
-        rc = lib().qms_cuda_paged_attention(pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
-                                            ws, nb, batch._err, raw)
+    d = q.get_device()
+    if d != pages._dev or d != batch._dev or out.get_device() != d:
+        _one_device("paged_attention", q, out, pages.k, batch.err)
+    raw = batch._use(stream, q)
+    ws, nb = batch.workspace(pages, n_head, raw)
+    rc = _on_device(d, lib().qms_cuda_paged_attention, pages._ref, batch._ref, x, ldx, n_head, D ** -0.5 if scale is None else scale, y, ldy,
+                    ws, nb, batch._err, raw)
     if rc:
         check(rc)
     return out
@@ -811,14 +801,13 @@ def logprobs(logits, ids=None, top: int = 0, temp: float = 1.0, out=None, err=No
         out = (_empty((n, k), torch.float32, dev, stream), _empty((n,), torch.float32, dev, stream),
                _empty((n, top), torch.int32, dev, stream), _empty((n, top), torch.float32, dev, stream))
     logp, entropy, top_id, top_logp = out
-    _one_device("logprobs", logits, ids, err, *out)
+    d = _one_device("logprobs", logits, ids, err, *out)
     if n == 0:
         return logp, entropy, top_id, top_logp
-    with _device_of(logits):
-        rc = lib().qms_cuda_logprobs(x, ldx, n, V, temp, _ints(ids, tuple(ids.shape), "ids") if k else None, k,
-                                     _vec(logp, n * k, "logp") if k else None, _vec(entropy, n, "entropy"), top,
-                                     _ints(top_id, (n, top), "top_id") if top else None, _vec(top_logp, n * top, "top_logp") if top else None,
-                                     None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, logits))
+    rc = _on_device(d, lib().qms_cuda_logprobs, x, ldx, n, V, temp, _ints(ids, tuple(ids.shape), "ids") if k else None, k,
+                    _vec(logp, n * k, "logp") if k else None, _vec(entropy, n, "entropy"), top,
+                    _ints(top_id, (n, top), "top_id") if top else None, _vec(top_logp, n * top, "top_logp") if top else None,
+                    None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, logits))
     if rc:
         check(rc)
     return logp, entropy, top_id, top_logp
