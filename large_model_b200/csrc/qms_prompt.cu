@@ -304,20 +304,6 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                 }
                 if (gives && j + 1 == nt) mbar_arrive(&q_empty[i]);
                 at.skip(2);
-                if (j * 128 + 127 > lo) {         // some row does not see the whole tile
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        const int d = pos - j * 128 - 32 * c;
-                        const uint32_t vis = d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u;
-                        uint32_t x[32];
-                        tmem_ld<32>(s_col + 32 * c, x);
-                        tmem_wait_ld(x);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) x[e] = vis >> e & 1 ? x[e] : 0xff800000u;
-                        tmem_st32(s_col + 32 * c, x);
-                    }
-                    tmem_wait_st();
-                }
                 uint32_t x[32], y[32];
                 const int chunks = min(4, (last - j * 128) / 32 + 1);
                 float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -325,17 +311,33 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                     mx0 = max3(mx0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
                     mx1 = max3(mx1, __uint_as_float(z[e + 2]), __uint_as_float(z[e + 3]));
                 };
-                tmem_ld<32>(s_col, x);
+                if (j * 128 + 127 > lo) {         // some row does not see the whole tile
 #pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {
-                    tmem_wait_ld(x);
-                    tmem_ld<32>(s_col + 32 * c + 32, y);
+                    for (int c = 0; c < chunks; c++) {
+                        const int d = pos - j * 128 - 32 * c;
+                        const uint32_t vis = d < 0 ? 0u : d >= 31 ? 0xffffffffu : (2u << d) - 1u;
+                        tmem_ld<32>(s_col + 32 * c, x);
+                        tmem_wait_ld(x);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) most(x, e);
-                    tmem_wait_ld(y);
-                    if (c == 0) tmem_ld<32>(s_col + 64, x);
+                        for (int e = 0; e < 32; e++) x[e] = vis >> e & 1 ? x[e] : 0xff800000u;
+                        tmem_st32(s_col + 32 * c, x);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) most(y, e);
+                        for (int e = 0; e < 32; e += 4) most(x, e);
+                    }
+                    tmem_wait_st();
+                } else {
+                    tmem_ld<32>(s_col, x);
+#pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        tmem_wait_ld(x);
+                        tmem_ld<32>(s_col + 32 * c + 32, y);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) most(x, e);
+                        tmem_wait_ld(y);
+                        if (c == 0) tmem_ld<32>(s_col + 64, x);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) most(y, e);
+                    }
                 }
                 tmem_ld<32>(s_col, x);
                 const float top = fmaxf(mx0, mx1) * f;
