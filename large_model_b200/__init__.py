@@ -546,7 +546,10 @@ class KvPages:
         d = self.desc
         shape = (d.n_pages, d.page_size, d.n_head_kv, d.head_dim)
         n = shape[0] * shape[1] * shape[2] * shape[3]
-        k, v = (_empty(shape, _torch().float32, self.k.device, stream) if x is None else x for x in (k, v))
+        if k is None:
+            k = _empty(shape, _torch().float32, self.k.device, stream)
+        if v is None:
+            v = _empty(shape, _torch().float32, self.k.device, stream)
         rc = _on_device(_one_device("KvPages.values", self.k, k, v), lib().qms_cuda_paged_values, self._ref, _vec(k, n, "k"), _vec(v, n, "v"),
                         _raw_stream(stream, self.k))
         if rc:

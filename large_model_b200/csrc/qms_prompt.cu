@@ -14,9 +14,10 @@
 // tile, nothing that the exponentials wait for, and short loops (a row's 128 scores in registers, all in line: 1.03 times as fast over 8192
 // positions, 0.87 over 1500).
 // Bound by the two products and the exponentials in turn (16 of a row's 128 per cycle and SM), and by what is between them where two streams
-// do not cover it: 8192 tokens of 64 q heads and 4 kv heads 1062 to 1179 us with the clock, 0.93 to 1.03 PFLOP/s, 0.56 to 0.62 of the library's rate for one large product;
-// 17 prompts of up to 1500 tokens 160, 0.59 PFLOP/s (the tiles on the diagonal, and two or three tiles to start and to end with). Short ones by the
-// chain of one unit, 9 us: 100 tokens 9.1, 64 prompts of up to 333 tokens with 8 heads of 64 values 26.5 for 2.6 units per SM.
+// do not cover it: 8192 tokens of 64 q heads and 4 kv heads 1060 to 1190 us with the clock, 0.93 to 1.03 PFLOP/s, 0.55 to 0.62 of the library's rate
+// for one large product; 17 prompts of up to 1500 tokens 152, 0.63 PFLOP/s: of some 20,000 cycles per unit 5000 are its first S, its last
+// product and its rows. Short ones by the chain of one unit: 100 tokens 8.7 us, 64 prompts of up to 333 tokens with 8 heads of 64 values 24.4 for
+// three units per SM.
 #include <cuda_bf16.h>
 #include <math.h>
 #include <string.h>
@@ -386,8 +387,8 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
             if (gives_kv) mbar_arrive(&empty[at.slot == 0 ? C::SLOTS - 1 : at.slot - 1]);      // V of the last tile
             at.skip(2 * (max(w.tiles(0, tq), w.tiles(1, tq)) - nt));
             // ---- the rows: O / l, each thread its own, a sector of 32 bytes by one store. (Few instructions: they are new to the
-            // instructions' cache at the end of every unit. Rows exchanged between 8 threads, for whole lines: 27 us for 64 prompts of up to 333 tokens,
-            // so 24.6; between 4 26.5.)
+            // instructions' cache at the end of every unit. 64 prompts of up to 333 tokens: rows exchanged between 8 threads, for whole lines, 27 us;
+            // between 4 26.5; so 24.6.)
             const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
             const bool none = l == 0.0f, fix = *s_flag != 0;
             char *dst = A.out + ((int64_t)(w.t0 + tok) * A.o_tok + (int64_t)(w.kh * G + my_head) * A.o_head) * (A.out32 ? 4 : 2);
