@@ -276,3 +276,30 @@ def test_scores_beyond_two_to_the_27(cuda, dtype):
     out = m.prompt_attention(batch, q, k, v, out_dtype=torch.float32)
     want = v[:, 0].double().cumsum(0)[:150] / torch.arange(1, 151, device="cuda")[:, None]
     assert ((out[:150].double() - want[:, None]).abs() <= 32 * E * v.abs().max()).all() and out[150:].isnan().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype,out", [("float16", "float16"), ("bfloat16", "bfloat16"), ("float16", "float32")])
+def test_rows_out_on_16_byte_boundaries(cuda, D, dtype, out):
+    """Rows that begin between two sectors of 32 bytes hold the same bits, and what lies between them stays."""
+    import torch
+    import large_model_b200 as m
+    lens, H, Hk = [37, 1, 150], 6, 2
+    n = sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x = torch.randn((n, H + 2 * Hk, D), generator=g, device="cuda").to(getattr(torch, dtype))
+    q, k, v = x[:, :H], x[:, H:H + Hk], x[:, H + Hk:]
+    batch = m.PagedBatch.prompts(torch.tensor([0] + np.cumsum(lens).tolist(), dtype=torch.int32, device="cuda"), n, max(lens))
+    typ = getattr(torch, out)
+    step = 16 // typ.itemsize                        # values in 16 bytes
+    want = m.prompt_attention(batch, q, k, v, out_dtype=typ)
+    for first, gap in ((step, 0), (0, step), (step, step)):
+        flat = torch.full((first + n * (H * D + gap),), float("nan"), dtype=typ, device="cuda")
+        rows = flat[first:].view(n, H * D + gap)
+        m.prompt_attention(batch, q, k, v, out=rows[:, :H * D].unflatten(1, (H, D)))
+        assert torch.equal(rows[:, :H * D], want.flatten(1))
+        assert flat[:first].isnan().all() and rows[:, H * D:].isnan().all()
+    heads = torch.full((H, n * D + step), float("nan"), dtype=typ, device="cuda")             # heads before tokens
+    m.prompt_attention(batch, q, k, v, out=heads[:, step:].unflatten(1, (n, D)).transpose(0, 1))
+    assert torch.equal(heads[:, step:].unflatten(1, (n, D)).transpose(0, 1), want) and heads[:, :step].isnan().all()
+    batch.status()
