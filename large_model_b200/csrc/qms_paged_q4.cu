@@ -10,8 +10,8 @@
 // A nibble becomes d (n - 8) by a shift, a mask and one fused step, exact in fp16 (q4_dequant). q and the weights have two terms,
 // sums join by rounded additions, as in k_paged_attn. Each warp has positions of its own, in tiles of 16 in turn, its own copies in
 // flight and its own (m, l, o); they meet at the end of a unit.
-// Bound by instructions: some 1320 per warp for 32 positions (4.6 KB), 128 of them MMAs, 350 for what comes out of the nibbles; 0.44 per cycle and
-// scheduler, where each next step waits for the one before it. 64 sequences of 4096 positions (64 q heads, 4 kv heads) 89.5 us, 1.69 TB/s; one of
+// Bound by instructions: some 1140 per warp for 32 positions (4.6 KB), 128 of them MMAs (the tensor pipe is busy for 41 % of the time), 350 for what
+// comes out of the nibbles; 0.45 per cycle and scheduler with 3 warps each, where most steps wait for the one before them (registers leave no fourth). 64 sequences of 4096 positions (64 q heads, 4 kv heads) 89.5 us, 1.69 TB/s; one of
 // 131,072 (32 q heads) 51.8, 1.46 TB/s; one of 1100 10.1, of which some 4 are the launch and 4 the join of the slots.
 // The same with K and V's transpose as tcgen05's M operand, 128 positions or values, and the rows as its N: 110 us and 55, by the way of K and
 // V through shared memory in fp16 (164 KB in and out for 18 that are read).
