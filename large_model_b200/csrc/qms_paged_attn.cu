@@ -881,9 +881,9 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, dou
     const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
-    // 4 bits, up to 16 rows (k_paged_q4): stages of 128 positions, three CTAs per SM. Cut by the 64 in us, and so: 1100 positions 11.5, 10.1; 131,072
-    // 58.4, 51.8; 64 sequences of 2048 56.5, 53.7; of 4096 89.5, 89.5. Two or six per SM 61.5, 62.5 on 131,072.
-    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, 128, std::max(1, (int)(148 * 3 * share)), 1.2, 3.0, most);
+    // 4 bits, up to 16 rows (k_paged_q4): stages of 128 positions, two CTAs per SM. Cut by the 64 in us, and by these: 1100 positions 11.5, 10.1; 131,072
+    // 58.4, 51.8; 64 sequences of 2048 56.5, 53.7; of 4096 89.5, 89.5 (with three CTAs).
+    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, 128, std::max(1, (int)(148 * 2 * share)), 0.9, 3.0, most);
     const int per_sm = type != QMS_T_F32 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * per_sm * share)), wr == 4 ? 2.0 : 1.2, 4.0, most);
 }

@@ -11,8 +11,10 @@
 // sums join by rounded additions, as in k_paged_attn. Each warp has positions of its own, in tiles of 16 in turn, its own copies in
 // flight and its own (m, l, o); they meet at the end of a unit.
 // Bound by instructions: some 1140 per warp for 32 positions (4.6 KB), 128 of them MMAs (the tensor pipe is busy for 41 % of the time), 350 for what
-// comes out of the nibbles; 0.45 per cycle and scheduler with 3 warps each, where most steps wait for the one before them (registers leave no fourth). 64 sequences of 4096 positions (64 q heads, 4 kv heads) 89.5 us, 1.69 TB/s; one of
-// 131,072 (32 q heads) 51.8, 1.46 TB/s; one of 1100 10.1, of which some 4 are the launch and 4 the join of the slots.
+// comes out of the nibbles, where most steps wait for the one before them. Two CTAs per SM, whose warps hold more products in flight: three took 89.5,
+// 53.3, 10.1 us for the figures that follow, four 97, 64, 10.5; a third stage of copies changed nothing.
+// 64 sequences of 4096 positions (64 q heads, 4 kv heads) 81.1 us, 1.86 TB/s; one of 131,072 (32 q heads) 48.0, 1.57 TB/s; one of 1100 9.8, of which some 4 are
+// the launch and 4 the join of the slots.
 // The same with K and V's transpose as tcgen05's M operand, 128 positions or values, and the rows as its N: 110 us and 55, by the way of K and
 // V through shared memory in fp16 (164 KB in and out for 18 that are read).
 #include <math.h>
@@ -54,7 +56,7 @@ struct Q4Cfg {
 };
 
 template <int D>
-__global__ void __launch_bounds__(128, 3) k_paged_q4(const PagedAttn A, const bool own, const bool last) {
+__global__ void __launch_bounds__(128, 2) k_paged_q4(const PagedAttn A, const bool own, const bool last) {
     using C = Q4Cfg<D>;
     constexpr int KS = D / 16, W = D / 32, VW = D / 64;      // steps of 16 values; words of K per thread and position, of V
     extern __shared__ unsigned char sm_[];
