@@ -189,6 +189,11 @@ struct PagedPlan {
     int line_tp, line_rows;
     int flat;                        // 4 bits: positions that go to the workspace in fp16 (0: none), for every kind that is kPaWidePair
 };
+// CTAs of k_paged_q4 per SM for so many tiles of rows: two have more products in flight each, three even out sequences of
+// unlike lengths, and waves. Two and three in us: 4 tiles (one token on 131,072 positions) 48.0, 53.3; on 16,384 18.7, 22.7; 32 19.7, 22.6; 160 28.5, 25.9; 256 81.1,
+// 89.1, of lengths up to that 60 to 77, 57; 512 150.6, 145.7.
+inline int q4_per_sm(int64_t tiles) { return tiles < 148 ? 2 : 3; }
+
 // k_paged_wide: 256 rows; 128; 128 over an fp32 cache; 128 over one in 4 bits
 constexpr int kPaWidePair = 0, kPaWideSplit = -1, kPaWideF32 = -2, kPaWideQ4 = -3;
 

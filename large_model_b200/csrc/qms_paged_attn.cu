@@ -7,7 +7,7 @@
 // Over an fp16 cache K and V are exact: two mma.sync m16n8k16 per product. Over an fp32 cache K and V are split too,
 // once per stage in shared memory, and three products kept (lo * lo is below 2^-22); the tf32 form of the same
 // (m16n8k8, three products, split in every warp) took about twice as long. Over a cache in 4 bits K and V go to fp16, exact, once per
-// stage in shared memory, for 17 to 64 rows; up to 16 rows are k_paged_q4's.
+// stage in shared memory, for many tiles of 17 to 64 rows; the others are k_paged_q4's.
 #include <math.h>
 #include <string.h>
 
@@ -845,10 +845,16 @@ __global__ void __launch_bounds__(256) k_paged_flat(const Paged a, const Paged t
 // 21.8, 18.4 (29.8, 27.2); 4.1 25.9, 19.6 (42.3, 31.0); 20 tokens on a prompt, shared ones 1.6 23.4, 25.1 (35.4, 36.9); 2.0 27.8, 27.2 (38.0,
 // 37.7); 3.1 31.3, 35.1 (45.7, 46.5); 6.3 39.8, 43.5 (65.8, 58.2); 16.8 69, 63 (139, 96).
 // 4 bits narrow against wide in us: own positions 2.0 19.1, 22.0; 4.1 27.4, 23.1 (20 tokens of one sequence 29.8, 24.8; 128 29.3, 28.1); 8.2 44.6, 30.3;
-// shared ones 1.3 23.5, 26.7; 2.6 30.7, 37.7; 4.2 41.8, 38.0; 10.5 57.2, 51.8.
-static int row_groups(int type, int page_log, int64_t rows, int64_t positions, bool shared) {
+// shared ones 1.3 23.5, 26.7; 2.6 30.7, 37.7; 4.2 41.8, 38.0; 10.5 57.2, 51.8. Narrow is k_paged_q4 with 16 rows a tile while there are fewer of them
+// than SMs (`sets` of all the rows: kv heads, and sequences), then k_paged_attn with taller ones: 8 tiles 11.1 taller, 9.8 by the 16 (2 tokens on 1000
+// positions); 16 32.6, 28.4 (4 on 16,000); 40 29.9, 22.3; 80 16.5, 14.3; 96 22.8, 16.3; 160 19.1, 19.3 and 27.1, 26.0; 256 39.9, 37.7; 320 44.8, 44.8; 512
+// 24.6, 29.8; 1024 21.5, 42.8; 1280 41.0, 49.4 and 70, 92.
+static int row_groups(int type, int page_log, int64_t rows, int64_t positions, int64_t sets, bool shared) {
     const bool f16 = type == QMS_T_F16;
-    if (type == QMS_T_Q4_0) return rows > 64 && (rows + 63) / 64 * 64 * positions > 3000000 ? kPaWideQ4 : rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    if (type == QMS_T_Q4_0) {
+        if (rows > 64 && (rows + 63) / 64 * 64 * positions > 3000000) return kPaWideQ4;
+        return rows <= 16 || (rows + 15) / 16 * sets < 148 ? 1 : rows > 32 ? 4 : 2;
+    }
     if (rows > 64 && (!f16 || page_log >= 3) && (rows + 63) / 64 * 64 * positions > (f16 || shared ? 2600000 : 1200000))
         return !f16 ? kPaWideF32 : rows > 128 ? kPaWidePair : kPaWideSplit;
     return rows > 32 ? 4 : rows > 16 ? 2 : 1;
@@ -881,9 +887,12 @@ static int chunk_for(int type, int wr, int len, int64_t tiles, int64_t rows, dou
     const int tp = tile_positions(type, wr), most = most_positions(wr);
     if (wr == kPaWidePair) return chunk_of(len, tiles, rows, tp, 148, 3.0, 8.0, most);
     if (wr <= 0) return chunk_of(len, tiles, rows, tp, 148, 1.5, 8.0, most);
-    // 4 bits, up to 16 rows (k_paged_q4): stages of 128 positions, two CTAs per SM. Cut by the 64 in us, and by these: 1100 positions 11.5, 10.1; 131,072
+    // 4 bits, 16 rows a tile (k_paged_q4): stages of 128 positions. Cut by the 64 in us, and by these: 1100 positions 11.5, 10.1; 131,072
     // 58.4, 51.8; 64 sequences of 2048 56.5, 53.7; of 4096 89.5, 89.5 (with three CTAs).
-    if (type == QMS_T_Q4_0 && wr == 1) return chunk_of(len, tiles, rows, 128, std::max(1, (int)(148 * 2 * share)), 0.9, 3.0, most);
+    if (type == QMS_T_Q4_0 && wr == 1) {
+        const int per_sm = q4_per_sm(tiles);
+        return chunk_of(len, tiles, rows, 128, std::max(1, (int)(148 * per_sm * share)), per_sm == 2 ? 0.9 : 1.2, 3.0, most);
+    }
     const int per_sm = type != QMS_T_F32 && wr == 1 ? 3 : 2;
     return chunk_of(len, tiles, rows, tp, std::max(1, (int)(148 * per_sm * share)), wr == 4 ? 2.0 : 1.2, 4.0, most);
 }
@@ -898,8 +907,8 @@ static int64_t al256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 void paged_plan(const Paged &a, int type, int D, PagedPlan &p) {
     const int64_t rows_p = (int64_t)a.n_tok * a.G, rows_s = (int64_t)a.max_q * a.G, all = (int64_t)a.n_tok * a.H;
     memset(&p, 0, sizeof p);
-    p.wr_p = row_groups(type, a.page_log, rows_p, (int64_t)a.prefix * a.Hk, true);
-    p.wr_s = row_groups(type, a.page_log, rows_s, (int64_t)std::max(0, a.max_kv - a.prefix) * a.Hk * a.n_seq, false);
+    p.wr_p = row_groups(type, a.page_log, rows_p, (int64_t)a.prefix * a.Hk, a.Hk, true);
+    p.wr_s = row_groups(type, a.page_log, rows_s, (int64_t)std::max(0, a.max_kv - a.prefix) * a.Hk * a.n_seq, (int64_t)a.Hk * a.n_seq, false);
     // 4 bits for many rows, on positions of one sequence's table: to fp16 once, not once per 128 rows, and 256 rows at a time. That
     // against kPaWideQ4 in us, 16 q heads per kv head, 4 of these: 320 tokens on a prompt of 8192 positions 251, 348; 64 62.8, 74.8; 20 50.9, 51.5; 10 (160 rows)
     // 46.2, 43.0; a sequence's 256 tokens on 4096 positions 86.4, 118.5; 32 30.2, 31.4; 16 (256 rows) 28.4, 25.3.

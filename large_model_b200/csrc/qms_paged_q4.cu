@@ -1,5 +1,5 @@
 // qms_paged_q4.cu - attention of few rows over a paged KV cache in 4 bits on B200 (sm_100a): up to 16 rows per tile (one token of
-// 16 q heads on a kv head). More rows: qms_paged_attn.cu, from some 65 on qms_paged_wide.cu.
+// 16 q heads on a kv head), several tiles while they are few. More rows: qms_paged_attn.cu, qms_paged_wide.cu.
 //
 // K and V go from nibbles straight into the registers that mma.sync m16n8k16 wants them in, never to fp16 in shared memory. A product's
 // operands may have the head's values, and the positions, in any order that is the same on both sides, so that
@@ -11,10 +11,8 @@
 // sums join by rounded additions, as in k_paged_attn. Each warp has positions of its own, in tiles of 16 in turn, its own copies in
 // flight and its own (m, l, o); they meet at the end of a unit.
 // Bound by instructions: some 1140 per warp for 32 positions (4.6 KB), 128 of them MMAs (the tensor pipe is busy for 41 % of the time), 350 for what
-// comes out of the nibbles, where most steps wait for the one before them. Two CTAs per SM, whose warps hold more products in flight: three took 89.5,
-// 53.3, 10.1 us for the figures that follow, four 97, 64, 10.5; a third stage of copies changed nothing.
-// 64 sequences of 4096 positions (64 q heads, 4 kv heads) 81.1 us, 1.86 TB/s; one of 131,072 (32 q heads) 48.0, 1.57 TB/s; one of 1100 9.8, of which some 4 are
-// the launch and 4 the join of the slots.
+// comes out of the nibbles, where most steps wait for the one before them. 64 sequences of 4096 positions (64 q heads, 4 kv heads) 89 us, 1.69 TB/s; one
+// of 131,072 (32 q heads) 48.0, 1.57 TB/s; one of 1100 9.8, of which some 4 are the launch and 4 the join of the slots. A third stage of copies changed nothing.
 // The same with K and V's transpose as tcgen05's M operand, 128 positions or values, and the rows as its N: 110 us and 55, by the way of K and
 // V through shared memory in fp16 (164 KB in and out for 18 that are read).
 #include <math.h>
@@ -55,8 +53,8 @@ struct Q4Cfg {
     static constexpr int SMEM = Q + D / 16 * 2 * 512 + 128;                             // q as A operands: [step][hi, lo][lane]
 };
 
-template <int D>
-__global__ void __launch_bounds__(128, 2) k_paged_q4(const PagedAttn A, const bool own, const bool last) {
+template <int D, int PER_SM>
+__global__ void __launch_bounds__(128, PER_SM) k_paged_q4(const PagedAttn A, const bool own, const bool last) {
     using C = Q4Cfg<D>;
     constexpr int KS = D / 16, W = D / 32, VW = D / 64;      // steps of 16 values; words of K per thread and position, of V
     extern __shared__ unsigned char sm_[];
@@ -428,21 +426,23 @@ __global__ void __launch_bounds__(128, 2) k_paged_q4(const PagedAttn A, const bo
     if (last) pdl_wait();
 }
 
-template <int D>
+template <int D, int PER_SM>
 static int launch_q4(const PagedAttn &A, bool own, bool last, cudaStream_t s) {
     using C = Q4Cfg<D>;
     const int64_t units = own ? (int64_t)A.p.chunks_s * A.a.n_seq * A.p.tiles_s * A.a.Hk : (int64_t)A.p.chunks_p * A.p.tiles_p * A.a.Hk;
     QMS_REQUIRE(units < (1ll << 30), QMS_CUDA_EUNSUPPORTED, "paged_attention: too many units of work");
     static std::atomic<unsigned long long> done{0};
-    const int rc = allow_smem(done, k_paged_q4<D>, C::SMEM);
+    const int rc = allow_smem(done, k_paged_q4<D, PER_SM>, C::SMEM);
     if (rc) return rc;
     const int grid = (int)(units < 148 * 8 ? units : 148 * 8);
-    QMS_CK(launch_pdl(k_paged_q4<D>, dim3(grid), dim3(128), C::SMEM, s, A, own, last));
+    QMS_CK(launch_pdl(k_paged_q4<D, PER_SM>, dim3(grid), dim3(128), C::SMEM, s, A, own, last));
     return QMS_CUDA_OK;
 }
 
 int launch_paged_q4(const PagedAttn &A, int D, bool own, bool last, cudaStream_t s) {
-    return D == 128 ? launch_q4<128>(A, own, last, s) : launch_q4<64>(A, own, last, s);
+    const int64_t tiles = own ? (int64_t)A.p.tiles_s * A.a.Hk * A.a.n_seq : (int64_t)A.p.tiles_p * A.a.Hk;
+    if (q4_per_sm(tiles) == 2) return D == 128 ? launch_q4<128, 2>(A, own, last, s) : launch_q4<64, 2>(A, own, last, s);
+    return D == 128 ? launch_q4<128, 3>(A, own, last, s) : launch_q4<64, 3>(A, own, last, s);
 }
 
 }  // namespace qms
