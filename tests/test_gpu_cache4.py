@@ -572,3 +572,27 @@ def test_masked_values_and_bad_pages_of_many_rows_in_two_sequences(cuda):
     keep = [j for j in range(kv) if j // 32 != 3]
     want, tol = reference([n, 1], [kv - 32, 5], q, [K[0][keep], K[1]], [V[0][keep], V[1]], G, 128 ** -0.5)
     assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q", [2, 3, 4, 5])
+def test_attention_many_tiles_of_rows(cuda, D, q):
+    """Two to five tokens of 40 sequences, short ones and idle ones among them: tiles of 32 and 64 rows; and one of their pages missing."""
+    import torch
+    import large_model_b200 as m
+    qs = [0 if b % 13 == 5 else min(q, 1 + b % (q + 2)) for b in range(40)]
+    qs[0] = q
+    kv = [n + (17 * b) % 90 for b, n in enumerate(qs)]
+    check(qs, kv, G=16, D=D, page=32, seed=q, pad=1)
+    check(qs, [n + 70 for n in kv], G=16, D=D, page=16, prefix=70, seed=q)
+    pages, batch, rows, K, V = make(qs, kv, G=16, D=D, page=16, seed=7)
+    b = max(range(40), key=lambda b: kv[b])
+    batch.table[b, 1] = -1
+    out = m.paged_attention(pages, batch, rows, 32)
+    with pytest.raises(m.QmsCudaError, match="0x2"):
+        batch.status()
+    keep = [j for j in range(kv[b]) if j // 16 != 1]
+    K, V = ([x[keep] if i == b else x for i, x in enumerate(z)] for z in (K, V))
+    lens = [len(keep) if i == b else n for i, n in enumerate(kv)]
+    want, tol = reference(qs, lens, rows, K, V, 16, D ** -0.5)
+    assert ((out.double() - want).abs() <= tol).all()
