@@ -146,7 +146,7 @@ def _scales(x):
     a = x.abs()
     at = (a == a.amax(-1, keepdim=True)).int().argmax(-1, keepdim=True)         # the first of equals
     m, e = torch.frexp(x.gather(-1, at).double() / -8.0)
-    return torch.ldexp(torch.round(m * 256.0) / 256.0, e).clamp(-2720.0, 2720.0).half().double()
+    return torch.ldexp(torch.round(m * 256.0) / 256.0, e).clamp(-8160.0, 8160.0).half().double()
 
 
 def _pack(x):
