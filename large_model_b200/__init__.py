@@ -648,7 +648,7 @@ def rope_tables(n_pos: int, head_dim: int, base: float = 1e6, device="cuda"):
 
 def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_norm, eps: float, rope, q=None, stream=None):
     """QK-norm, rotation and cache append of the batch's rows (qms_cuda_paged_append): qkv CUDA float32
-    [n_tok][(n_head + 2 n_head_kv) * head_dim], rope = rope_tables(...). Returns the q heads
+    [n_tok][(n_head + 2 n_head_kv) * head_dim], rope = rope_tables(...). All tensors lie on one device. Returns the q heads
     [n_tok][n_head * head_dim]."""
     D = pages.head_dim
     if q is None:
@@ -660,8 +660,9 @@ def paged_append(pages: KvPages, batch: PagedBatch, qkv, n_head: int, q_norm, k_
     if n < batch.n_tok or ny < batch.n_tok:
         raise ValueError(f"paged_append: {n} qkv and {ny} q rows for {batch.n_tok} tokens")
     d = qkv.get_device()
-    if d != pages._dev or d != batch._dev or q.get_device() != d or q_norm.get_device() != d or cos.get_device() != d:
-        _one_device("paged_append", qkv, q, pages.k, batch.err, q_norm, cos)
+    if (d != pages._dev or d != batch._dev or q.get_device() != d or q_norm.get_device() != d or k_norm.get_device() != d or
+            cos.get_device() != d or sin.get_device() != d):
+        _one_device("paged_append", qkv, q, pages.k, batch.err, q_norm, k_norm, cos, sin)
     rc = _on_device(d, lib().qms_cuda_paged_append, pages._ref, batch._ref, x, ldx, n_head, _vec(q_norm, D, "q_norm"), _vec(k_norm, D, "k_norm"),
                     eps, _vec(cos, nc * (D // 2), "rope cos"), _vec(sin, nc * (D // 2), "rope sin"), nc, y, ldy, batch._err,
                     batch._use(stream, qkv))

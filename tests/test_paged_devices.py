@@ -1,0 +1,100 @@
+"""The paged operators' Python calls refuse tensors that lie on several devices, before any library call: a kernel would read the
+other device's address. Stand-ins for CUDA tensors; CPU only."""
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+import large_model_b200 as m
+
+
+class On:
+    """What the calls look at of a contiguous CUDA tensor on device `d`."""
+
+    def __init__(self, shape, d=0, dtype=torch.float32):
+        self.shape, self.dtype, self.d, self.is_cuda = torch.Size(shape), dtype, d, True
+        self.device = torch.device("cuda", d)
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def stride(self):
+        st, n = [], 1
+        for x in reversed(self.shape):
+            st.insert(0, n)
+            n *= x
+        return tuple(st)
+
+    def is_contiguous(self):
+        return True
+
+    def flatten(self, first):
+        return On((*self.shape[:first], self.shape[first:].numel()), self.d, self.dtype)
+
+    def data_ptr(self):
+        return 4096
+
+    def get_device(self):
+        return self.d
+
+
+class Library:
+    """Every entry records its name and says OK."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    L = Library()
+    monkeypatch.setattr(m, "lib", lambda: L)
+    monkeypatch.setattr(m, "_raw_stream", lambda stream, t: 0)
+    monkeypatch.setattr(m, "_on_device", lambda d, call, *a: call(*a))
+    return L
+
+
+def pool(d=0, head_dim=128):
+    p = m.KvPages.__new__(m.KvPages)
+    p.k = p.v = On((4, 16, 2, head_dim), d)
+    p.n_head_kv, p.head_dim, p._dev, p._key = 2, head_dim, d, ("pool", head_dim)
+    p.desc = m.PagesDesc(m.T_F32, 4, 16, 2, head_dim, 16 * 2 * head_dim, 2 * head_dim, head_dim, 4096, 4096)
+    p._ref = C.byref(p.desc)
+    return p
+
+
+def batch(d=0, n_tok=3):
+    b = m.PagedBatch.__new__(m.PagedBatch)
+    b.n_tok, b.err, b._err, b._dev, b._ready, b._ws = n_tok, On((1,), d, torch.int32), 4096, d, {0}, {}
+    b.desc = m.PagedBatchDesc(2, n_tok, 4096, 4096, 4096, 2, 2, 32, 0)
+    b._ref = C.byref(b.desc)
+    return b
+
+
+APPEND = dict(qkv=(3, 8 * 128), q=(3, 512), q_norm=(128,), k_norm=(128,), cos=(32, 64), sin=(32, 64))
+
+
+def append(other=None):
+    t = {k: On(s, int(k == other)) for k, s in APPEND.items()}
+    return m.paged_append(pool(int(other == "pages")), batch(int(other == "batch")), t["qkv"], 4, t["q_norm"], t["k_norm"], 1e-6,
+                          (t["cos"], t["sin"]), q=t["q"])
+
+
+@pytest.mark.parametrize("other", [*APPEND, "pages", "batch"])
+def test_append_on_two_devices(library, other):
+    with pytest.raises(ValueError, match="paged_append: tensors on"):
+        append(other)
+    assert library.calls == []
+
+
+def test_append_on_one_device(library):
+    append()
+    assert library.calls == ["qms_cuda_paged_append"]
