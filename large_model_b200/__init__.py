@@ -691,10 +691,11 @@ def prompt_append(pages: KvPages | None, batch: PagedBatch, qkv, n_head: int, q_
     q | k | v in 16 bits for prompt_attention (qms_cuda_prompt_append): qkv CUDA float32 [n_tok][(n_head + 2 n_head_kv) * head_dim].
     Returns rows [n_tok][n_head + 2 n_head_kv][head_dim] of dtype (bfloat16 if not said), or the given rows."""
     torch = _torch()
-    D = q_norm.numel()
-    Hk = pages.n_head_kv if pages is not None else n_head_kv
+    D, Hk = (q_norm.numel(), n_head_kv) if pages is None else (pages.head_dim, pages.n_head_kv)
     if Hk is None:
         raise ValueError("prompt_append: without pages n_head_kv is needed")
+    if n_head_kv is not None and n_head_kv != Hk:
+        raise ValueError(f"prompt_append: n_head_kv {n_head_kv} for pages of {Hk} kv heads")
     W = (n_head + 2 * Hk) * D
     if rows is None:
         rows = _empty((batch.n_tok, n_head + 2 * Hk, D), dtype or torch.bfloat16, qkv.device, stream)
