@@ -785,7 +785,8 @@ def probs(logits, temp: float, out=None, stream=None):
     y, ny, ldy = _rows(out, V, "out")
     if n != ny:
         raise ValueError(f"probs: {n} rows of logits, {ny} of out")
-    rc = lib().qms_cuda_probs(x, ldx, n, V, temp, y, ldy, _raw_stream(stream, logits))
+    d = _one_device("probs", logits, out)
+    rc = _on_device(d, lib().qms_cuda_probs, x, ldx, n, V, temp, y, ldy, _raw_stream(stream, logits))
     if rc:
         check(rc)
     return out
@@ -835,10 +836,11 @@ def verify(p, draft, u, q=None, n_draft=None, row_start=None, n_accept=None, tok
         raise ValueError(f"verify: {ny} draft rows for {B} sequences of {N} drafts")
     if row_start is None and n < B * (N + 1):
         raise ValueError(f"verify: {n} rows of p for {B} sequences of {N} drafts")
-    rc = lib().qms_cuda_verify(x, ldx, n, None if row_start is None else _ints(row_start, (B,), "row_start"), y, ldy,
-                               _ints(draft, (B, N), "draft"), None if n_draft is None else _ints(n_draft, (B,), "n_draft"), B, N, V,
-                               _vec(u, B * (N + 1), "u"), _ints(n_accept, (B,), "n_accept"), _ints(tokens, (B, N + 1), "tokens"),
-                               None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, p))
+    d = _one_device("verify", p, draft, u, q, n_draft, row_start, n_accept, tokens, err)
+    rc = _on_device(d, lib().qms_cuda_verify, x, ldx, n, None if row_start is None else _ints(row_start, (B,), "row_start"), y, ldy,
+                    _ints(draft, (B, N), "draft"), None if n_draft is None else _ints(n_draft, (B,), "n_draft"), B, N, V,
+                    _vec(u, B * (N + 1), "u"), _ints(n_accept, (B,), "n_accept"), _ints(tokens, (B, N + 1), "tokens"),
+                    None if err is None else _ints(err, (1,), "err"), _raw_stream(stream, p))
     if rc:
         check(rc)
     return n_accept, tokens

@@ -98,3 +98,37 @@ def test_append_on_two_devices(library, other):
 def test_append_on_one_device(library):
     append()
     assert library.calls == ["qms_cuda_paged_append"]
+
+
+I32 = torch.int32
+PROBS = dict(logits=(3, 50), out=(3, 50))
+VERIFY = dict(p=(6, 50), draft=(2, 2), u=(2, 3), q=(2, 2, 50), n_draft=(2,), row_start=(2,), n_accept=(2,), tokens=(2, 3), err=(1,))
+
+
+def verify(other=None):
+    t = {k: On(s, int(k == other), torch.float32 if k in ("p", "u", "q") else I32) for k, s in VERIFY.items()}
+    t["q"].view = lambda *shape: On((4, 50), t["q"].d)
+    return m.verify(**t)
+
+
+@pytest.mark.parametrize("other", PROBS)
+def test_probs_on_two_devices(library, other):
+    with pytest.raises(ValueError, match="probs: tensors on"):
+        m.probs(On(PROBS["logits"], int(other == "logits")), 1.0, out=On(PROBS["out"], int(other == "out")))
+    assert library.calls == []
+
+
+@pytest.mark.parametrize("other", VERIFY)
+def test_verify_on_two_devices(library, other):
+    with pytest.raises(ValueError, match="verify: tensors on"):
+        verify(other)
+    assert library.calls == []
+
+
+def test_probs_and_verify_on_one_device(library, monkeypatch):
+    """The call is made with the tensors' device as the current one."""
+    devices = []
+    monkeypatch.setattr(m, "_on_device", lambda d, call, *a: devices.append(d) or call(*a))
+    m.probs(On((3, 50), 1), 1.0, out=On((3, 50), 1))
+    verify()
+    assert library.calls == ["qms_cuda_probs", "qms_cuda_verify"] and devices == [1, 0]
