@@ -567,6 +567,7 @@ class PagedBatch:
     def __init__(self, q_start, kv_len, table, n_tok: int, max_q: int, max_kv: int, prefix_len: int = 0):
         torch = _torch()
         n = kv_len.shape[0]
+        _one_device("PagedBatch", kv_len, q_start, table)
         self.q_start, self.kv_len, self.table = q_start, kv_len, table
         self.n_tok = int(n_tok)
         self.err = torch.zeros((1,), dtype=torch.int32, device=kv_len.device)

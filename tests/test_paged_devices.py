@@ -132,3 +132,16 @@ def test_probs_and_verify_on_one_device(library, monkeypatch):
     m.probs(On((3, 50), 1), 1.0, out=On((3, 50), 1))
     verify()
     assert library.calls == ["qms_cuda_probs", "qms_cuda_verify"] and devices == [1, 0]
+
+
+def test_a_batch_on_two_devices(monkeypatch):
+    monkeypatch.setattr(torch, "zeros", lambda shape, dtype, device: On(shape, device.index, dtype))
+    monkeypatch.setattr(m.PagedBatch, "_cleared", lambda self: None)
+    for other in (None, "q_start", "kv_len", "table"):
+        t = {k: On(s, int(k == other), I32) for k, s in dict(q_start=(3,), kv_len=(2,), table=(2, 2)).items()}
+        make = lambda: m.PagedBatch(t["q_start"], t["kv_len"], t["table"], 3, 2, 32)
+        if other is None:
+            assert make()._dev == 0
+            continue
+        with pytest.raises(ValueError, match="PagedBatch: tensors on"):
+            make()
