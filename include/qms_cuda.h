@@ -216,8 +216,9 @@ enum {
  * head_stride lie first the positions' nibbles n, head_dim / 2 bytes each, value i of every 8 in bits 4 (i / 2) + 16 (i % 2) of
  * a 32-bit word, then the positions' scales d, an fp16 number for every 32 values. A value is d (n - 8). The append takes for d the
  * value of largest magnitude (the first of equals) over -8, rounded to 8 significant bits and to at most 2720, n = floor(x / d + 8.5)
- * within 0 .. 15; 32 values of which one is not finite are NaN. Scales from elsewhere keep to those 8 bits and 2720, or lose what is
- * beyond fp16's 11 bits in the product. */
+ * within 0 .. 15; 32 values of which one is not finite are NaN. (So values beyond 21760 in magnitude are held as that.) Scales from
+ * elsewhere keep to those 8 bits and 2720: others are read as d (16 + n) - 24 d with 24 d and the difference rounded to fp16, which
+ * from 2730 on is not finite. These are not GGUF's blocks of the same type, which hold a scale and its 32 nibbles together. */
 typedef struct {
     int type, n_pages, page_size, n_head_kv, head_dim;
     int64_t page_stride, pos_stride, head_stride;

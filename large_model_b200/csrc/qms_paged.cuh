@@ -60,10 +60,11 @@ __device__ __forceinline__ int64_t paged_at(const Paged &a, const int *row, int 
 
 // ---- a cache in 4 bits ----
 // Of a (page, kv head) lie first the positions' nibbles, D / 2 bytes each, then their scales, an fp16 number for 32 values. A value
-// is d (n - 8): d has 8 significant bits and |d| <= 2720, so that the value is exact in fp16, and so are its 24 d below.
+// is d (n - 8): d has 8 significant bits and |d| <= 2720, so that the value is exact in fp16, and so are its 24 d below. (Of a larger
+// scale 24 d is finite up to 2728; the values of one beyond that are not finite, all 32 of them.)
 // (Paged: pos_stride is D / 2, and paged_at leads to the position's nibbles.)
 struct Q4 {};
-constexpr float kQ4Most = 2720.0f;
+constexpr float kQ4Most = 2720.0f, kQ4Finite = 2728.0f;
 
 __host__ __device__ constexpr int q4_row(int D) { return D / 2 + D / 16; }
 // Byte distance from the nibbles of position `off` of a page to its scales.

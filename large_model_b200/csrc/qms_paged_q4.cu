@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(128, PER_SM) k_paged_q4(const PagedAttn A, con
                     for (int i = 0; i < 4; i++) {
                         const int p = base + 64 * x + 4 * i + tq;
                         const bool none = gone(x, p);
-                        if (none || (p > seen && !(fabsf(__half2float(e[i])) <= kQ4Most))) {
+                        if (none || (p > seen && !(fabsf(__half2float(e[i])) <= kQ4Finite))) {
                             if (!none) s_flag = 1;         // (else nobody's)
                             e[i] = __float2half(0.0f);
                         }
