@@ -273,9 +273,10 @@ typedef struct {
  * prompt's tokens j <= t of softmax_j(scale * q[t][h] . k[j][h / (n_head / n_head_kv)]) v[j]. q, k, v of type QMS_T_F16 or
  * QMS_CUDA_T_BF16, out of that type or QMS_T_F32; out may be q itself, of its type and strides, and overlaps nothing else. head_dim 64
  * or 128, up to 128 q heads per kv head, scale > 0. Rows of no prompt are left as they were; a prompt whose rows make no sense sets
- * QMS_PAGED_ELEN and is left out. What a row does not see has no effect on it, whatever its bits; a V value that it sees and that is
- * not finite makes that element of the row not finite. Precision: q, k, v are exact, a weight is rounded to the type once (as
- * the output is), scores and sums are fp32. Scores are below 10^7 in magnitude: a row with larger ones may be NaN. */
+ * QMS_PAGED_ELEN and is left out (where q_start falls, prompts after it may be left out too). What a row does not see has no effect
+ * on it, whatever its bits; a V value that it sees and that is not finite makes that element of the row not finite. Precision: q, k, v
+ * are exact, a weight is rounded to the type once (as the output is), scores and sums are fp32. Scores are below 10^7 in magnitude: a
+ * row with larger ones may be NaN. */
 int qms_cuda_prompt_attention(const QmsCudaPagedBatch *batch, int type, const QmsCudaHeads *q, const QmsCudaHeads *k, const QmsCudaHeads *v,
                               int n_head, int n_head_kv, int head_dim, float scale, int out_type, const QmsCudaHeads *out, int *err,
                               void *stream);

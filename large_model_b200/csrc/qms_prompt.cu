@@ -39,6 +39,7 @@ struct PromptAttn {
     int64_t v_tok, v_head, o_tok, o_head;           // elements
     float f;                         // scale * log2(e)
     int tq;                          // tokens per tile: 128 / G
+    int share;                       // sequences per unit number
     int out32, whole;                // fp32 rows out; rows out on 32-byte boundaries
 };
 
@@ -256,11 +257,6 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
         if (lane == 0) mbar_arrive(u_empty);
         return true;
     };
-    if (blockIdx.x == 0)                          // the batch's arrays, checked once
-        for (int b = tid; b < a.n_seq; b += C::THREADS) {
-            int t0, n, kv;
-            if (!prompt_seq(a, b, t0, n, kv)) paged_err(a, QMS_PAGED_ELEN);
-        }
 
     if (warp < 8) {
         // ---- softmax of stream i: thread = row = TMEM lane
@@ -590,6 +586,13 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
                              "r"(smem_u32(u_got))
                              : "memory");
             }
+            // the batch's arrays, checked once: a share of them goes with each unit number, by whoever takes it (no CTA is sure to start),
+            // while the answer is on its way
+            const int64_t b1 = min((int64_t)a.n_seq, ((int64_t)u + 1) * A.share);
+            for (int64_t b = (int64_t)u * A.share + lane; b < b1; b += 32) {
+                int t0, cnt, kv;
+                if (!prompt_seq(a, (int)b, t0, cnt, kv)) paged_err(a, QMS_PAGED_ELEN);
+            }
             __syncwarp();
             uint32_t n = 0;                       // (not given up before the answer is there, abort or not: it is written to this CTA's memory)
             while (!mbar_try_wait(u_got, asked & 1) && ++n < kWSpin) {}
@@ -641,7 +644,7 @@ static int heads_map(const QmsCudaHeads &h, bool bf, int D, int heads, int n_tok
 }
 
 template <int D, bool BF>
-static int launch_prompt(const PromptAttn &A, const QmsCudaHeads &q, const QmsCudaHeads &k, const QmsCudaHeads &v, cudaStream_t s) {
+static int launch_prompt(PromptAttn &A, const QmsCudaHeads &q, const QmsCudaHeads &k, const QmsCudaHeads &v, cudaStream_t s) {
     using C = PrCfg<D>;
     static_assert(C::SMEM <= 232448, "shared memory per CTA");
     static std::atomic<unsigned long long> done{0};
@@ -654,6 +657,7 @@ static int launch_prompt(const PromptAttn &A, const QmsCudaHeads &q, const QmsCu
     const int64_t most = ((int64_t)A.a.n_tok / (2 * A.tq) + std::min(A.a.n_seq, A.a.n_tok)) * A.a.Hk;      // units there can be
     QMS_REQUIRE(most < (1ll << 31), QMS_CUDA_EUNSUPPORTED, "prompt_attention: too many units of work");
     const unsigned grid = (unsigned)most;          // (those that have not started are taken over by CTAs that have)
+    A.share = (int)((A.a.n_seq + most - 1) / most);
     QMS_CK(launch_pdl(k_prompt_attn<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM, s, A, mq, mk, mv));
     return QMS_CUDA_OK;
 }
