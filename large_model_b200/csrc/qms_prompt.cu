@@ -160,21 +160,28 @@ struct PromptUnit {
     __device__ __forceinline__ int tiles(int i, int tq) const { return there(i, tq) ? last(i, tq) / 128 + 1 : 0; }
 };
 
+// The search for a unit's rows goes on from where the last one was found, since a CTA's unit numbers grow but for chance: otherwise n_seq
+// prompts would take n_seq^2 / 64 steps (65,536 of a token each took 160 ms so, 1.6 as it is).
+struct UnitSearch {
+    int b0 = 0, before = 0;          // 32 sequences from b0 on, and the units (of a kv head) of those before them
+};
+
 // Unit u of the call, by the whole warp: kv heads in the innermost, a sequence's tiles from its end (long ones first). False: there
 // are not so many.
-__device__ __forceinline__ bool prompt_unit(const PromptAttn &A, unsigned u, PromptUnit &w) {
+__device__ __forceinline__ bool prompt_unit(const PromptAttn &A, unsigned u, UnitSearch &s, PromptUnit &w) {
     const Paged &a = A.a;
     const int lane = threadIdx.x & 31;
-    int v = u / a.Hk;
+    const int v = u / a.Hk;
     w.kh = u - v * a.Hk;
-    for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+    if (v < s.before) s = UnitSearch();
+    for (; s.b0 < a.n_seq; s.b0 += 32) {
         int t0 = 0, n = 0, kv;
-        if (b0 + lane < a.n_seq) prompt_seq(a, b0 + lane, t0, n, kv);
+        if (s.b0 + lane < a.n_seq) prompt_seq(a, s.b0 + lane, t0, n, kv);
         const int mine = (n + 2 * A.tq - 1) / (2 * A.tq);
-        int upto = mine;
+        int upto = s.before + mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(kFull, upto, o);
+            const int x = __shfl_up_sync(kFull, upto, o) - s.before;
             if (lane >= o) upto += x;
         }
         const unsigned hit = __ballot_sync(kFull, upto > v);
@@ -185,7 +192,7 @@ __device__ __forceinline__ bool prompt_unit(const PromptAttn &A, unsigned u, Pro
             w.tok0 = (__shfl_sync(kFull, upto, at) - 1 - v) * 2 * A.tq;
             return true;
         }
-        v -= __shfl_sync(kFull, upto, 31);
+        s.before = __shfl_sync(kFull, upto, 31);
     }
     return false;
 }
@@ -577,8 +584,9 @@ __global__ void __launch_bounds__(384, 1) k_prompt_attn(const PromptAttn A, cons
             return true;
         };
         unsigned u = blockIdx.x;
+        UnitSearch search;
         for (uint32_t asked = 0;; asked++) {
-            if (prompt_unit(A, u, w) && !(ok = publish(w))) break;
+            if (prompt_unit(A, u, search, w) && !(ok = publish(w))) break;
             if (lane == 0) {
                 fence_async_smem();
                 mbar_arrive_expect_tx(u_got, 16);
