@@ -314,7 +314,7 @@ int qms_cuda_paged_attention(const QmsCudaPages *pages, const QmsCudaPagedBatch 
 int qms_cuda_probs(const float *logits, int64_t ldl, int rows, int vocab, float temp, float *p, int64_t ldp, void *stream);
 
 /* Log probabilities of given tokens, and of the likeliest ones, and the entropy of rows of logits (fp32 rows of
- * ldl) at a temperature > 0: with x = (l - max) / temp, log p = x - log sum exp(x), entropy = -sum p log p, natural logarithms. logp
+ * ldl) at a temperature of 2^-126 or more: with x = (l - max) / temp, log p = x - log sum exp(x), entropy = -sum p log p, natural logarithms. logp
  * [rows][n_ids] of tokens ids [rows][n_ids]; entropy [rows] (NULL: not wanted); top_id, top_logp [rows][n_top], the
  * n_top <= 32 largest logits in their order, the lowest id first among equals (n_top 0: not wanted). Values near 0 are as
  * exact as others: the sum is kept without its largest term. A token of logit -inf has -inf, and is never among the

@@ -23,7 +23,7 @@ struct LogprobArgs {
     int64_t ldl;
     int V, n_ids, n_top;
     const int *ids;
-    float c, temp;                   // log2(e) / temp
+    float h, c, temp;                // (l h - max h) c is (l - max) log2(e) / temp; temp: h times the temperature
     float *lp, *entropy, *top_lp;
     int *top_id, *err;
 };
@@ -91,9 +91,9 @@ struct LpPart {
     float m, z, t;
 };
 // p under the maximum M of several parts; `first`: it is the one whose m is left out. Nothing seen: z is 0, or NaN.
-__device__ __forceinline__ LpPart lp_under(const LpPart &p, float M, bool first, float c) {
+__device__ __forceinline__ LpPart lp_under(const LpPart &p, float M, bool first, float h, float c) {
     if (first) return p;
-    const float d = p.m == -INFINITY ? -INFINITY : (p.m - M) * c, f = ex2f(d), one = p.z + 1.0f;
+    const float d = p.m == -INFINITY ? -INFINITY : (p.m * h - M * h) * c, f = ex2f(d), one = p.z + 1.0f;
     return LpPart{M, one * f, f * fmaf(one, fmaxf(d, -256.0f), p.t)};
 }
 
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
 
     float B = -FLT_MAX, m[2] = {-INFINITY, -INFINITY};
     u64 z2 = 0, t2 = 0;                                     // (two sums each)
-    const u64 c2 = two(a.c, a.c);
+    const u64 h2 = two(a.h, a.h), c2 = two(a.c, a.c);
     float bound = -FLT_MAX;                                // a value has to reach it
     u64 best = 0;                                          // the lane-th largest of the warp's
     // new values, up to 32 in s_new, take their places among the n_top largest: a key's place is the number of keys above it
@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
         if (lane == 0) atomicMax(&s_bound, own);
         bound = fmaxf(bound, lp_unorder(own + 1));           // (the next number above; of the largest finite one inf)
     };
-    auto rebase = [&](float top) {
+    auto rebase = [&](float top) {                         // (B is h times a value)
+        top *= a.h;
         if ((top - B) * a.c > 4.0f) {
             const float d = fmaxf((B - top) * a.c, -256.0f), f = ex2f(d);
             B = top;
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
         }
     };
     auto add = [&](float v0, float v1) {                   // to the sums: each value, or the largest so far that it replaces
-        const float2 y = of_two(mul_two(add_two(two(min_nan(m[0], v0), min_nan(m[1], v1)), two(-B, -B)), c2));
+        const float2 y = of_two(mul_two(fma_two(two(min_nan(m[0], v0), min_nan(m[1], v1)), h2, two(-B, -B)), c2));
         const u64 w = two(ex2f(y.x), ex2f(y.y));
         m[0] = fmaxf(m[0], v0), m[1] = fmaxf(m[1], v1);
         z2 = add_two(z2, w);
@@ -299,18 +300,18 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
     {
         const float2 z = of_two(z2), t = of_two(t2);
         const bool second = m[1] > m[0];                   // of the two maxima one joins the sums
-        const float y = ((second ? m[0] : m[1]) - B) * a.c, w = ex2f(y);
+        const float y = ((second ? m[0] : m[1]) * a.h - B) * a.c, w = ex2f(y);
         p.m = second ? m[1] : m[0];
         p.z = z.x + z.y + w;
         p.t = fmaf(w, fmaxf(y, -256.0f), t.x + t.y);
-        const float d = p.m == -INFINITY ? 0.0f : (B - p.m) * a.c, f = ex2f(d);            // from the base to the maximum
+        const float d = p.m == -INFINITY ? 0.0f : (B - p.m * a.h) * a.c, f = ex2f(d);            // from the base to the maximum
         p.t = f * fmaf(p.z, d, p.t);
         p.z *= f;
     }
     auto join = [&](LpPart p) {                            // of a warp's lanes
         const uint32_t k = lp_order(p.m), most = __reduce_max_sync(kFull, k);
         const int first = __ffs(__ballot_sync(kFull, k == most)) - 1;
-        p = lp_under(p, lp_unorder(most), lane == first, a.c);
+        p = lp_under(p, lp_unorder(most), lane == first, a.h, a.c);
         p.z = warp_sum(p.z);
         p.t = warp_sum(p.t);
         p.m = lp_unorder(most);
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
     p = join(lane < nc ? s_part[lane] : LpPart{-INFINITY, 0.0f, 0.0f});
     const bool none = p.m == -INFINITY && !isnan(p.z);     // a row of -inf
     const float lz = log1pf(p.z);
-    auto logp = [&](float v) { return none || v == -INFINITY ? (isnan(p.z) ? NAN : -INFINITY) : __fdiv_rn(v - p.m, a.temp) - lz; };
+    auto logp = [&](float v) { return none || v == -INFINITY ? (isnan(p.z) ? NAN : -INFINITY) : __fdiv_rn(v * a.h - p.m * a.h, a.temp) - lz; };
     for (int i = tid; i < a.n_ids; i += kLpThreads) {
         const int id = a.ids[r * a.n_ids + i];
         const bool good = (unsigned)id < (unsigned)a.V;
@@ -466,7 +467,7 @@ int qms_cuda_logprobs(const float *logits, int64_t ldl, int rows, int vocab, flo
     QMS_REQUIRE(logits && vocab > 0 && vocab <= (1 << 22) && rows >= 0, QMS_CUDA_EINVAL,
                 "logprobs: NULL logits, rows %d or vocab %d (at most %d)", rows, vocab, 1 << 22);
     QMS_REQUIRE(ldl >= vocab, QMS_CUDA_EINVAL, "logprobs: rows of %d need ldl of at least that", vocab);
-    QMS_REQUIRE(temp > 0.0f && temp <= FLT_MAX, QMS_CUDA_EINVAL, "logprobs: temp must be positive and finite");
+    QMS_REQUIRE(temp >= FLT_MIN && temp <= FLT_MAX, QMS_CUDA_EINVAL, "logprobs: temp must be positive and finite, at least 2^-126");
     QMS_REQUIRE(n_ids >= 0 && (n_ids == 0 || (ids && logp)), QMS_CUDA_EINVAL, "logprobs: %d ids per row need ids and logp", n_ids);
     QMS_REQUIRE(n_top >= 0 && n_top <= kLpTop && (n_top == 0 || (top_id && top_logp)), n_top > kLpTop ? QMS_CUDA_EUNSUPPORTED : QMS_CUDA_EINVAL,
                 "logprobs: %d likeliest tokens (at most %d) need top_id and top_logp", n_top, kLpTop);
@@ -481,9 +482,11 @@ int qms_cuda_logprobs(const float *logits, int64_t ldl, int rows, int vocab, flo
     a.n_ids = n_ids;
     a.n_top = n_top;
     a.ids = ids;
-    // a scale of 0 or infinity would make NaN of the maximum and of -inf
-    a.c = fminf(fmaxf(1.4426950408889634f / temp, 1e-37f), 1e37f);
-    a.temp = temp;
+    // From a temperature of 1 on a difference is taken of the halves: of two values of fp32's whole range it may be past that range where x is
+    // not. (Below 1 x is then too.) c is neither 0 nor infinite, which would make NaN of the maximum and of -inf.
+    a.h = temp >= 1.0f ? 0.5f : 1.0f;
+    a.temp = temp * a.h;
+    a.c = 1.4426950408889634f / a.temp;
     a.lp = logp;
     a.entropy = entropy;
     a.top_lp = top_logp;
