@@ -13,8 +13,8 @@ namespace qms {
 typedef unsigned long long u64;
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpTop = 32;
-// a warp's groups of 4 values per lane, values per chunk, chunks in flight, or kept; entries of the list
-constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2, kLpKeep = 6, kLpList = 2048;
+// a warp's groups of 4 values per lane, values per chunk, chunks in flight, or kept; entries of the list, what is short for one
+constexpr int kLpQuads = 4, kLpChunk = 128 * kLpQuads, kLpRing = 2, kLpKeep = 6, kLpShort = 256, kLpList = 512;
 constexpr uint32_t kLpSpin = 1u << 22;
 constexpr int kLpFew = 74;            // CTAs up to which a row's slices are kept in shared memory (launch_logprobs)
 
@@ -70,6 +70,11 @@ __device__ __forceinline__ u64 fma_two(u64 a, u64 b, u64 c) {
     return d;
 }
 
+__device__ __forceinline__ u64 max_key(u64 key) {                   // of a warp's lanes
+    const uint32_t hi = __reduce_max_sync(kFull, (uint32_t)(key >> 32));
+    return (u64)hi << 32 | __reduce_max_sync(kFull, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+}
+
 // How many entries of `lists` lists, each of kLpTop in falling order, are above the key.
 __device__ __forceinline__ int lp_above(const u64 *list, int lists, u64 key) {
     static_assert(kLpTop == 32, "5 steps to one of 32, a sixth for none or all");
@@ -118,6 +123,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
     __shared__ uint64_t s_full[kLpWarps][RING];
     __shared__ LpPart s_warp[kLpWarps], s_part[kRowCtas];
     __shared__ uint32_t s_bound, s_r[kLpWarps];            // the highest bound of a warp, by lp_order
+    __shared__ u64 s_lowest;
     __shared__ int s_abort, s_n;
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
@@ -337,8 +343,9 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
             uint32_t least = s_r[0];
             for (int w = 1; w < busy; w++) least = min(least, s_r[w]);
             bound = fmaxf(least == 0 ? -FLT_MAX : lp_unorder(least), -FLT_MAX);
+            u64 lowest = 0;                                // a key has to reach it
             auto take = [&](float v, int i) {
-                if (v >= bound) {
+                if (v >= bound && lp_key(v, i) >= lowest) {
                     const int n = atomicAdd(&s_n, 1);
                     if (n < kLpList) list[n] = lp_key(v, i);
                 }
@@ -360,10 +367,31 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
                 if (rank == 0 && tid < head) f(row[tid], tid);
                 if (rank == nc - 1 && tail + tid < a.V && tid < 4) f(row[tail + tid], tail + tid);
             };
-            all_values(take);
-            __syncthreads();
-            listed = s_n;
-            if (listed > kLpList) {                        // many equal values: one after the other
+            for (bool again = false;; again = true) {
+                all_values(take);
+                __syncthreads();
+                listed = s_n;
+                if (listed <= kLpShort || again) break;
+                // A warp whose values are few, masked away or equal lets the bound be anything: then the n_top-th of all lanes' largest
+                // keys. (All of them listed and ranked: one row of 1540 values 100 us, so 9.0; one of 151,936 with 60,000 masked 152, so 13.7.)
+                u64 own = 0, key = 0;
+                all_values([&](float v, int i) {
+                    if (v >= bound) own = max(own, lp_key(v, i));
+                });
+                for (int i = 0; i < a.n_top; i++) {        // the warp's, in falling order
+                    const u64 most = max_key(own);
+                    if (lane == i) key = most;
+                    if (own == most) own = 0;
+                }
+                s_list[tid] = key;
+                __syncthreads();
+                if (tid == 0) s_n = 0, s_lowest = 0;
+                __syncthreads();
+                if (key != 0 && lp_above(s_list, kLpWarps, key) == a.n_top - 1) s_lowest = key;
+                __syncthreads();
+                lowest = s_lowest;
+            }
+            if (listed > kLpList) {                        // fewer lanes than n_top have all the values: one after the other
                 u64 last = ~0ull;
                 for (int q = 0; q < a.n_top; q++) {
                     u64 most = 0;
@@ -373,11 +401,7 @@ __global__ void __launch_bounds__(kLpThreads, KEEP ? 2 : 4) k_logprobs(const Log
                             if (k < last && k > most) most = k;
                         }
                     });
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        const u64 other = __shfl_xor_sync(kFull, most, o);
-                        most = other > most ? other : most;
-                    }
+                    most = max_key(most);
                     if (lane == 0) s_list[warp] = most;
                     __syncthreads();
                     for (int w = 0; w < kLpWarps; w++) most = s_list[w] > most ? s_list[w] : most;
