@@ -197,8 +197,9 @@ __device__ __forceinline__ void row_st2(float *p, float x, float y) { *reinterpr
 __device__ __forceinline__ void row_st2(__half *p, float x, float y) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(x, y); }
 __device__ __forceinline__ void row_st2(__nv_bfloat16 *p, float x, float y) { *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x, y); }
 
-// R q heads of one token to 16 bits, in fp32: y = R(pos) (w x / sqrt(mean x^2 + eps)). Of 128 values a lane has 2 l, 2 l + 1 and the two 64
-// further, which they are rotated with.
+// R q heads of one token to 16 bits, in fp32: y = R(pos) (w x / sqrt(mean x^2 + eps)). (The mean too: 9 roundings on the way of a square, half
+// of them after the root, are 2^-21 of y, 2^-10 of fp16's half step.) Of 128 values a lane has 2 l, 2 l + 1 and the two 64 further, which
+// they are rotated with.
 template <typename OT, int R>
 __device__ __forceinline__ void q_rows16(const float2 (&x)[R][2], int cnt, const float *norm, float eps, const float *cos, const float *sin, OT *out, int lane) {
     auto two = [&](const float *v) { return make_float2(v[2 * lane], v[2 * lane + 1]); };       // (of any alignment)
@@ -223,10 +224,10 @@ __device__ __forceinline__ void q_rows16(const float2 (&x)[R][2], int cnt, const
 
 // k_paged_append's steps where the cache or the rows that go out are of another kind: a cache in 4 bits (K normalised and rotated in
 // double, see above), or none; rows out of fp32, the q heads, or of 16 bits, all heads q | k | v as the prompt attention reads
-// them, each value rounded once from fp32. (Rows of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.)
+// them, each value rounded once from fp32. (What is stored in 4 bits: q4_quantize. Rows of 16 bits next to a cache of fp32 or fp16: that cache's values are k_paged_append's.)
 // A warp takes R q heads, or one K or V head: what is stored in 4 bits takes as long as four q heads.
 // Bound by latency for few rows (64 tokens of 72 heads 4.1 us, one token 3.1), by instructions for many, those of the exchanges within 32
-// values and, for K, of double where fp32 does not settle a border: 700 tokens of 40 heads 9.9 us with rows in 16 bits, 2.5 TB/s.
+// values and, for K, of double up to the rotated value: 700 tokens of 40 heads 9.9 us with rows in 16 bits, 2.5 TB/s.
 template <int D, typename OT, int R>
 __global__ void __launch_bounds__(256) k_rows_append(const Paged a, const int type, const float *qkv, int64_t ldqkv, const float *q_norm,
                                                      const float *k_norm, float eps, const float *rope_cos, const float *rope_sin, int n_rope,

@@ -1064,7 +1064,7 @@ int launch_paged_attention(const Paged &a, int type, int D, const PagedPlan &p, 
     else rc = D == 128 ? launch_attn<128, float>(A, A, s) : launch_attn<64, float>(A, A, s);
     if (rc) return rc;
     // Four warps per row while there are few rows, or many slots for each. Four against one in us: 320 rows (5 tokens, 2000
-    // positions) 14.9, 16.1; 512 rows on a prompt of 4096 positions 24.7, 28.9; 1024 rows of 100 positions 11.5, 9.1; 3072 rows
+    // positions) 14.9, 16.1; 512 rows on a prompt of 4096 positions 24.7, 28.9; 1024 rows of 100 positions 11.5, 9.1; some 3000 rows
     // of 1000 positions 28.3, 25.2.
     const int64_t rows = (int64_t)a.n_tok * a.H;
     // Over 4 bits eight for a row per SM or less and more than 12 slots, four against eight: 9 slots 10.0, 10.1; 32 14.2, 13.2; 55 (16,384 positions)

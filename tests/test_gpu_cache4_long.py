@@ -89,7 +89,7 @@ def test_many_rows_on_both_sides_of_the_workspace(cuda, qs, kv, G, Hk, D, page, 
 
 def test_the_workspace_is_bounded(cuda):
     """Past 128 MiB there are the slots alone: one per unit of at most 2304 positions, and of more than 512 here (320 rows in 3 tiles on 4 kv
-    heads are 12 units per slot, so 256 slots would be 3072 units for 148 CTAs), 520 bytes per row and slot."""
+    heads are 12 units per slot, so 256 slots would be some 3000 units for 148 CTAs), 520 bytes per row and slot."""
     import large_model_b200 as m
     import torch
     Hk, D, page, H = 4, 128, 64, 64
